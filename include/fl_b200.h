@@ -401,6 +401,89 @@ FL_B200_API int fl_b200_softmax_bwd_scaled(const void* dy, int64_t ld_dy, const 
                                            int in_dtype, int out_dtype,
                                            fl_b200_stream_t stream);
 
+/* ------------------------------------------------------------------------ *
+ * Rows of the vocabulary: a teacher's top logits, the distillation loss on   *
+ * them, and the verification of drafted tokens.  The reference has none of   *
+ * these (its HF path would run them op by op).                              *
+ *                                                                           *
+ * The k largest of each row, descending; equal values (and -0 and +0) by    *
+ * ascending index, NaN above everything (as argmax orders them).  x: F32/   *
+ * BF16/F16 [rows, cols], stride ld.  values (x's dtype, the elements' own    *
+ * bits) and indices are dense [rows, k], k <= min(cols,                      *
+ * FL_B200_TOPK_MAX).  Any alignment.                                        */
+#define FL_B200_TOPK_MAX 1024
+FL_B200_API int fl_b200_topk_lastdim(const void* x, int64_t ld, int64_t rows, int64_t cols,
+                                     int64_t k, void* values, int64_t* indices, int dtype,
+                                     fl_b200_stream_t stream);
+/* Its gradient: dx (dense [rows, cols]) = 0 but dvalues at the indices       *
+ * (both dense [rows, k]; an index outside the row is left out).             */
+FL_B200_API int fl_b200_topk_bwd(const void* dvalues, const int64_t* indices, void* dx, int64_t rows,
+                                 int64_t cols, int64_t k, int dtype, fl_b200_stream_t stream);
+
+/* Distillation from a teacher's top logits.  Row r holds the student's      *
+ * logits z (F32/BF16/F16, stride ld), and a list of k <= FL_B200_DISTILL_MAX *
+ * teacher logits t (F32/BF16/F16, its own dtype and stride) with token ids   *
+ * (I32/I64); entries whose id lies outside [0, cols) are absent.            *
+ *   p = softmax over the present entries of t / temperature,                *
+ *   q = softmax of z / temperature,                                         *
+ *   loss[r] = temperature^2 * sum_j p_j (log p_j - log q[id_j]).            *
+ * A row without entries has loss 0, whatever its logits hold; an id may     *
+ * repeat (its entries add).  loss and stats are F32; stats (2 a row, 8-byte *
+ * aligned) is what the backward needs: the row's maximum and the sum of     *
+ * exp((z - max) / temperature), 0 for a row without entries.                */
+#define FL_B200_DISTILL_MAX 1024
+FL_B200_API int fl_b200_distill_topk_fwd(const void* logits, int64_t ld, const void* teacher,
+                                         int64_t ld_t, int t_dtype, const void* ids, int64_t ld_ids,
+                                         int ids_dtype, int64_t rows, int64_t cols, int64_t k,
+                                         float temperature, float* loss, float* stats, int dtype,
+                                         fl_b200_stream_t stream);
+/* Gradients for dloss[r * dloss_stride] (F32; NULL: 1 for every row):       *
+ *   dlogits_v = dloss * temperature * (q_v - sum over id_j = v of p_j),      *
+ *   dteacher_j = dloss * temperature * p_j (log p_j - log q[id_j] - KL).    *
+ * dlogits (logits' dtype, stride ld_dlogits; not in place) and dteacher     *
+ * (the teacher's dtype, dense [rows, k]) may each be NULL.  Rows are stored *
+ * 16 bytes at a time when the logits' and the gradient's rows begin at the   *
+ * same offset from a 16-byte boundary, one element at a time otherwise.     */
+FL_B200_API int fl_b200_distill_topk_bwd(const float* dloss, int64_t dloss_stride,
+                                         const void* logits, int64_t ld, const float* stats,
+                                         const void* teacher, int64_t ld_t, int t_dtype,
+                                         const void* ids, int64_t ld_ids, int ids_dtype,
+                                         void* dlogits, int64_t ld_dlogits, void* dteacher,
+                                         int64_t rows, int64_t cols, int64_t k, float temperature,
+                                         int dtype, fl_b200_stream_t stream);
+/* Loss and dlogits at once, for row weights that are known beforehand       *
+ * (row_weight takes dloss's place).  stats as in the forward.               */
+FL_B200_API int fl_b200_distill_topk_grad(const void* logits, int64_t ld, const void* teacher,
+                                          int64_t ld_t, int t_dtype, const void* ids,
+                                          int64_t ld_ids, int ids_dtype, const float* row_weight,
+                                          int64_t weight_stride, int64_t rows, int64_t cols,
+                                          int64_t k, float temperature, float* loss, float* stats,
+                                          void* dlogits, int64_t ld_dlogits, int dtype,
+                                          fl_b200_stream_t stream);
+
+/* Verification of drafted tokens (speculative sampling).  Sequence b has    *
+ * n = lens[b] (clamped to [0, drafts]; lens NULL: drafts) drafted tokens     *
+ * x_i = draft_ids[b * ld_ids + i], the target's probabilities p (F32/BF16/   *
+ * F16, row i at b * p_stride_b + i * p_stride_i, drafts + 1 rows of vocab    *
+ * contiguous elements) and the draft model's q (p's dtype, drafts rows;     *
+ * NULL: 1 at x_i).  In order, x_i is kept while u_i q_i(x_i) < p_i(x_i)      *
+ * with u_i = uniform[b * ld_u + i] in [0, 1); an id outside the vocabulary  *
+ * is not.  The next token is drawn from max(p_i - q_i, 0) at the first      *
+ * token turned down (from p_i where that leaves nothing), from p_n when     *
+ * all were kept, as the first index whose cumulative sum exceeds            *
+ * floor(t W / 2^24): W the row's total, t = floor(u 2^24) for              *
+ * u = uniform[b * ld_u + drafts], probabilities as whole multiples of 2^-36 *
+ * (clamped to [0, 1], NaN as 0).  So the result does not depend on the     *
+ * order of any sum.                                                         *
+ * tokens (dense [batch, drafts + 1]): the kept tokens, the drawn one (-1     *
+ * from a row without mass), then -1; accepted[b]: how many were kept.       */
+FL_B200_API int fl_b200_verify_draft(const int64_t* draft_ids, int64_t ld_ids, const void* p,
+                                     int64_t p_stride_b, int64_t p_stride_i, const void* q,
+                                     int64_t q_stride_b, int64_t q_stride_i, const float* uniform,
+                                     int64_t ld_u, const int64_t* lens, int64_t batch,
+                                     int64_t drafts, int64_t vocab, int64_t* tokens,
+                                     int64_t* accepted, int dtype, fl_b200_stream_t stream);
+
 #ifdef __cplusplus
 } /* extern "C" */
 #endif

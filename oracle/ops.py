@@ -403,3 +403,94 @@ def rope_bwd_golden(dq_out, cos, sin, dtype: str):
     h = t.shape[-1] // 2
     rt = np.concatenate([t[..., h:], -t[..., :h]], axis=-1)
     return round_to(d64 * c64 + rt, dtype)
+
+
+# ------------------------------------------------------ rows of the vocabulary
+# A teacher's top logits, the distillation loss on them and the verification
+# of drafted tokens, from their definitions in 64 bits.
+def topk_golden(x, k: int) -> tuple[np.ndarray, np.ndarray]:
+    """(values, indices) of the k largest over the last dim: descending, equal
+    values by ascending index, NaN above everything."""
+    x = np.asarray(x, np.float64)
+    key = np.where(np.isnan(x), np.inf, x)
+    # NaN sorts before +inf: two stable passes, the later one decides
+    order = np.argsort(-key, axis=-1, kind="stable")
+    first = np.take_along_axis(~np.isnan(x), order, -1)
+    order = np.take_along_axis(order, np.argsort(first, axis=-1, kind="stable"), -1)[..., :k]
+    return np.take_along_axis(x, order, -1), order
+
+
+def distill_topk_golden(z, t, ids, temperature: float, weight=None):
+    """(loss [R], dlogits [R, V], dteacher [R, k]) of
+    temperature^2 KL(softmax over the list's present entries of t / temperature
+    || softmax(z / temperature)), for row weights (None: 1)."""
+    z, t, ids = np.asarray(z, np.float64), np.asarray(t, np.float64), np.asarray(ids)
+    R, V = z.shape
+    w = np.ones(R) if weight is None else np.broadcast_to(np.asarray(weight, np.float64), (R,))
+    tau = float(temperature)
+    loss, dz, dt = np.zeros(R), np.zeros_like(z), np.zeros_like(t)
+    for r in range(R):
+        at = np.flatnonzero((ids[r] >= 0) & (ids[r] < V))
+        tr = t[r, at] / tau
+        if at.size == 0 or np.all(tr == -np.inf):
+            continue
+        with np.errstate(all="ignore"):
+            log_p = tr - tr.max() - np.log(np.exp(tr - tr.max()).sum())
+            p = np.exp(log_p)
+            zr = z[r] / tau
+            log_q = zr - zr.max() - np.log(np.exp(zr - zr.max()).sum())
+            gap = np.where(p > 0, log_p - log_q[ids[r, at]], 0.0)
+            kl = (p * gap).sum()
+            loss[r] = tau * tau * kl
+            g = np.exp(log_q)
+            np.subtract.at(g, ids[r, at], p)
+            dz[r] = w[r] * tau * g
+            dt[r, at] = w[r] * tau * p * (gap - kl)
+    return loss, dz, dt
+
+
+def verify_draft_golden(ids, p, q, u, lens=None):
+    """(tokens, accepted): speculative sampling's verification, the draw in
+    whole multiples of 2^-36 with Python's integers."""
+    ids, u = np.asarray(ids), np.asarray(u, np.float64)
+    p = np.asarray(p, np.float64)
+    q = None if q is None else np.asarray(q, np.float64)
+    B, K = ids.shape
+    V = p.shape[-1]
+
+    def fixed(row):
+        return np.rint(np.clip(np.nan_to_num(row, nan=0.0), 0.0, 1.0) * 2.0 ** 36).astype(np.int64)
+
+    def clean(v):
+        return 0.0 if np.isnan(v) else min(max(v, 0.0), 1.0)
+
+    tokens, accepted = np.full((B, K + 1), -1, np.int64), np.zeros(B, np.int64)
+    for b in range(B):
+        n = K if lens is None else min(K, max(0, int(lens[b])))
+        i = 0
+        while i < n:
+            x = int(ids[b, i])
+            if not 0 <= x < V:
+                break
+            if not max(u[b, i], 0.0) * (1.0 if q is None else clean(q[b, i, x])) < clean(p[b, i, x]):
+                break
+            tokens[b, i] = x
+            i += 1
+        accepted[b] = i
+        base = fixed(p[b, i])
+        left = base
+        if i < n:
+            if q is None:
+                left = base.copy()
+                if 0 <= int(ids[b, i]) < V:
+                    left[int(ids[b, i])] = 0
+            else:
+                left = np.maximum(base - fixed(q[b, i]), 0)
+            if left.sum() == 0:
+                left = base
+        total = int(left.sum())
+        if total == 0:
+            continue
+        t = min(int(min(max(u[b, K], 0.0), 1.0) * 2 ** 24), 2 ** 24 - 1)
+        tokens[b, i] = int(np.searchsorted(np.cumsum(left), t * total >> 24, side="right"))
+    return tokens, accepted

@@ -5,6 +5,8 @@
 // on the input's device and launches on that device's current stream.
 #include <torch/library.h>
 
+#include <cmath>
+
 #include "tensor_utils.h"
 
 namespace flb200::aten {
@@ -335,6 +337,212 @@ at::Tensor SoftmaxBackward(const at::Tensor& dy_in, const at::Tensor& y_in,
   return dx;
 }
 
+// ------------------------------------------------- rows of the vocabulary --
+// A teacher's top logits, the distillation loss on them, and the
+// verification of drafted tokens.
+std::tuple<at::Tensor, at::Tensor> Topk(const at::Tensor& x_in, int64_t k) {
+  const char* op = "flagos::topk";
+  const int code = FloatCode(x_in, op);
+  TORCH_CHECK(x_in.dim() >= 1, op, ": x must have at least one dim");
+  TORCH_CHECK(k >= 0 && k <= x_in.size(-1) && k <= FL_B200_TOPK_MAX, op, ": k must lie in [0, ",
+              std::to_string(std::min<int64_t>(x_in.size(-1), FL_B200_TOPK_MAX)), "], got ", std::to_string(k));
+  at::Tensor x;
+  const RowsView r = Rows(x_in, x);
+  std::vector<int64_t> sizes(x.sizes().begin(), x.sizes().end());
+  sizes.back() = k;
+  at::Tensor values = at::empty(sizes, x.options());
+  at::Tensor indices = at::empty(sizes, x.options().dtype(at::kLong));
+  GpuGuard g(x);
+  CheckB200(fl_b200_topk_lastdim(x.data_ptr(), r.ld, r.rows, r.cols, k, values.data_ptr(),
+                                 indices.data_ptr<int64_t>(), code, StreamOf(x)),
+            op);
+  return {values, indices};
+}
+
+at::Tensor TopkBackward(const at::Tensor& dvalues, const at::Tensor& indices, int64_t cols) {
+  const char* op = "flagos::topk_backward";
+  const int code = FloatCode(dvalues, op);
+  SameDevice(dvalues, indices, op);
+  TORCH_CHECK(dvalues.dim() >= 1 && dvalues.sizes() == indices.sizes() &&
+                  indices.scalar_type() == at::kLong,
+              op, ": dvalues and int64 indices must match");
+  const int64_t k = dvalues.size(-1);
+  TORCH_CHECK(cols >= k && k <= FL_B200_TOPK_MAX, op, ": at most min(cols, ",
+              std::to_string(FL_B200_TOPK_MAX), ") values a row");
+  at::Tensor d = dvalues.contiguous(), i = indices.contiguous();
+  std::vector<int64_t> sizes(d.sizes().begin(), d.sizes().end());
+  int64_t rows = 1;
+  for (size_t n = 0; n + 1 < sizes.size(); ++n) rows *= sizes[n];
+  sizes.back() = cols;
+  at::Tensor dx = at::empty(sizes, d.options());
+  GpuGuard g(d);
+  CheckB200(fl_b200_topk_bwd(d.data_ptr(), i.data_ptr<int64_t>(), dx.data_ptr(), rows, cols, k, code,
+                             StreamOf(d)),
+            op);
+  return dx;
+}
+
+// The student's rows and the teacher's lists of one call, checked.
+struct Distill {
+  at::Tensor x, t, ids;
+  RowsView rx, rt, ri;
+  int code, t_code, ids_code;
+  at::IntArrayRef lead;  // logits' leading dims: the loss's shape
+};
+Distill DistillArgs(const at::Tensor& logits, const at::Tensor& teacher, const at::Tensor& ids,
+                    double temperature, const char* op) {
+  Distill d;
+  d.code = FloatCode(logits, op);
+  d.t_code = FloatCode(teacher, op);
+  SameDevice(logits, teacher, op);
+  SameDevice(logits, ids, op);
+  TORCH_CHECK(ids.scalar_type() == at::kLong || ids.scalar_type() == at::kInt, op,
+              ": teacher_ids must be int32 or int64, got ", ids.scalar_type());
+  d.ids_code = B200Dtype(ids.scalar_type());
+  TORCH_CHECK(logits.dim() >= 1 && teacher.dim() == logits.dim() && teacher.sizes() == ids.sizes(), op,
+              ": logits [..., vocab] with teacher_logits and teacher_ids [..., k] expected");
+  d.lead = logits.sizes().slice(0, logits.dim() - 1);
+  TORCH_CHECK(teacher.sizes().slice(0, teacher.dim() - 1) == d.lead, op,
+              ": teacher_logits' leading dims must be the logits'");
+  TORCH_CHECK(teacher.size(-1) <= FL_B200_DISTILL_MAX, op, ": at most ", std::to_string(FL_B200_DISTILL_MAX),
+              " teacher logits a row, got ", std::to_string(teacher.size(-1)));
+  TORCH_CHECK(logits.size(-1) > 0 || logits.numel() == 0, op, ": an empty vocabulary");
+  TORCH_CHECK(temperature > 0 && std::isfinite((float)temperature) && (float)temperature > 0, op,
+              ": temperature must be positive and finite, got ", std::to_string(temperature));
+  d.rx = Rows(logits, d.x);
+  d.rt = Rows(teacher, d.t);
+  d.ri = Rows(ids, d.ids);
+  int64_t rows = 1;
+  for (int64_t n : d.lead) rows *= n;
+  d.rx.rows = rows;
+  TORCH_CHECK(rows == 0 || d.rx.cols > 0, op, ": an empty vocabulary");
+  return d;
+}
+
+// Row weights (or dloss) of the loss's shape, or one that broadcasts to it,
+// as a pointer and one stride over the rows; undefined: every row 1.
+const float* RowWeights(const std::optional<at::Tensor>& w, const Distill& d, at::Tensor& keep,
+                        int64_t& stride, const char* name, const char* op) {
+  stride = 0;
+  if (!w.has_value() || !w->defined()) return nullptr;
+  SameDevice(d.x, *w, op);
+  TORCH_CHECK(w->scalar_type() == at::kFloat, op, ": ", name, " must be float32, got ", w->scalar_type());
+  keep = w->expand(d.lead).reshape({d.rx.rows});
+  stride = d.rx.rows > 1 ? keep.stride(0) : 0;
+  return keep.data_ptr<float>();
+}
+
+std::tuple<at::Tensor, at::Tensor> DistillTopk(const at::Tensor& logits, const at::Tensor& teacher,
+                                               const at::Tensor& ids, double temperature) {
+  const char* op = "flagos::distill_topk";
+  const Distill d = DistillArgs(logits, teacher, ids, temperature, op);
+  at::Tensor loss = at::empty(d.lead, d.x.options().dtype(at::kFloat));
+  at::Tensor stats = at::empty({d.rx.rows, 2}, loss.options());
+  GpuGuard g(d.x);
+  CheckB200(fl_b200_distill_topk_fwd(d.x.data_ptr(), d.rx.ld, d.t.data_ptr(), d.rt.ld, d.t_code,
+                                     d.ids.data_ptr(), d.ri.ld, d.ids_code, d.rx.rows, d.rx.cols,
+                                     d.t.size(-1), (float)temperature, loss.data_ptr<float>(),
+                                     stats.data_ptr<float>(), d.code, StreamOf(d.x)),
+            op);
+  return {loss, stats};
+}
+
+std::tuple<at::Tensor, at::Tensor> DistillTopkBackward(const at::Tensor& dloss, const at::Tensor& logits,
+                                                       const at::Tensor& stats, const at::Tensor& teacher,
+                                                       const at::Tensor& ids, double temperature,
+                                                       bool need_logits, bool need_teacher) {
+  const char* op = "flagos::distill_topk_backward";
+  const Distill d = DistillArgs(logits, teacher, ids, temperature, op);
+  SameDevice(logits, stats, op);
+  TORCH_CHECK(stats.scalar_type() == at::kFloat && stats.dim() == 2 && stats.size(0) == d.rx.rows &&
+                  stats.size(1) == 2 && stats.is_contiguous(),
+              op, ": stats must be the forward's [rows, 2] float32 tensor");
+  at::Tensor w;
+  int64_t ws;
+  const float* wp = RowWeights(dloss, d, w, ws, "dloss", op);
+  at::Tensor dx = need_logits ? at::empty(logits.sizes(), d.x.options()) : at::empty({0}, d.x.options());
+  at::Tensor dt = need_teacher ? at::empty(teacher.sizes(), d.t.options()) : at::empty({0}, d.t.options());
+  GpuGuard g(d.x);
+  CheckB200(fl_b200_distill_topk_bwd(wp, ws, d.x.data_ptr(), d.rx.ld, stats.data_ptr<float>(),
+                                     d.t.data_ptr(), d.rt.ld, d.t_code, d.ids.data_ptr(), d.ri.ld,
+                                     d.ids_code, need_logits ? dx.data_ptr() : nullptr, d.rx.cols,
+                                     need_teacher ? dt.data_ptr() : nullptr, d.rx.rows, d.rx.cols,
+                                     d.t.size(-1), (float)temperature, d.code, StreamOf(d.x)),
+            op);
+  return {dx, dt};
+}
+
+std::tuple<at::Tensor, at::Tensor> DistillTopkGrad(const at::Tensor& logits, const at::Tensor& teacher,
+                                                   const at::Tensor& ids, double temperature,
+                                                   const std::optional<at::Tensor>& row_weight) {
+  const char* op = "flagos::distill_topk_grad";
+  const Distill d = DistillArgs(logits, teacher, ids, temperature, op);
+  at::Tensor w;
+  int64_t ws;
+  const float* wp = RowWeights(row_weight, d, w, ws, "row_weight", op);
+  at::Tensor loss = at::empty(d.lead, d.x.options().dtype(at::kFloat));
+  at::Tensor stats = at::empty({d.rx.rows, 2}, loss.options());
+  at::Tensor dx = at::empty(logits.sizes(), d.x.options());
+  GpuGuard g(d.x);
+  CheckB200(fl_b200_distill_topk_grad(d.x.data_ptr(), d.rx.ld, d.t.data_ptr(), d.rt.ld, d.t_code,
+                                      d.ids.data_ptr(), d.ri.ld, d.ids_code, wp, ws, d.rx.rows,
+                                      d.rx.cols, d.t.size(-1), (float)temperature,
+                                      loss.data_ptr<float>(), stats.data_ptr<float>(), dx.data_ptr(),
+                                      d.rx.cols, d.code, StreamOf(d.x)),
+            op);
+  return {loss, dx};
+}
+
+std::tuple<at::Tensor, at::Tensor> VerifyDraft(const at::Tensor& draft_ids, const at::Tensor& target,
+                                               const std::optional<at::Tensor>& draft,
+                                               const at::Tensor& uniform,
+                                               const std::optional<at::Tensor>& draft_lens) {
+  const char* op = "flagos::verify_draft";
+  const int code = FloatCode(target, op);
+  SameDevice(target, draft_ids, op);
+  SameDevice(target, uniform, op);
+  TORCH_CHECK(draft_ids.dim() == 2 && draft_ids.scalar_type() == at::kLong, op,
+              ": draft_ids must be an int64 [batch, drafts] tensor");
+  const int64_t B = draft_ids.size(0), K = draft_ids.size(1);
+  TORCH_CHECK(target.dim() == 3 && target.size(0) == B && target.size(1) == K + 1, op,
+              ": target_probs must be [batch, drafts + 1, vocab]");
+  const int64_t V = target.size(2);
+  TORCH_CHECK(B == 0 || V > 0, op, ": an empty vocabulary");
+  TORCH_CHECK(uniform.dim() == 2 && uniform.size(0) == B && uniform.size(1) == K + 1 &&
+                  uniform.scalar_type() == at::kFloat,
+              op, ": uniform must be a float32 [batch, drafts + 1] tensor");
+  const auto unit = [](const at::Tensor& t) {
+    return t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous();
+  };
+  at::Tensor ids = unit(draft_ids), p = unit(target), u = unit(uniform), q, lens;
+  if (draft.has_value() && draft->defined()) {
+    SameDevice(target, *draft, op);
+    TORCH_CHECK(draft->scalar_type() == target.scalar_type() && draft->dim() == 3 &&
+                    draft->size(0) == B && draft->size(1) == K && draft->size(2) == V,
+                op, ": draft_probs must be [batch, drafts, vocab] of target_probs' dtype");
+    q = unit(*draft);
+  }
+  if (draft_lens.has_value() && draft_lens->defined()) {
+    SameDevice(target, *draft_lens, op);
+    TORCH_CHECK(draft_lens->scalar_type() == at::kLong && draft_lens->dim() == 1 &&
+                    draft_lens->size(0) == B,
+                op, ": draft_lens must be an int64 [batch] tensor");
+    lens = draft_lens->contiguous();
+  }
+  at::Tensor tokens = at::empty({B, K + 1}, ids.options()), accepted = at::empty({B}, ids.options());
+  GpuGuard g(p);
+  // (without a single drafted token q has no rows, and none is read)
+  CheckB200(fl_b200_verify_draft(ids.data_ptr<int64_t>(), ids.stride(0), p.data_ptr(), p.stride(0),
+                                 p.stride(1), q.defined() ? q.data_ptr() : nullptr,
+                                 q.defined() ? q.stride(0) : 0, q.defined() ? q.stride(1) : 0,
+                                 u.data_ptr<float>(), u.stride(0),
+                                 lens.defined() ? lens.data_ptr<int64_t>() : nullptr, B, K, V,
+                                 tokens.data_ptr<int64_t>(), accepted.data_ptr<int64_t>(), code,
+                                 StreamOf(p)),
+            op);
+  return {tokens, accepted};
+}
+
 }  // namespace
 
 TORCH_LIBRARY(flagos, m) {
@@ -354,6 +562,17 @@ TORCH_LIBRARY(flagos, m) {
   m.def("softmax_backward(Tensor dy, Tensor y, ScalarType? dtype=None, float scale=1.0) -> Tensor");
   m.def("masked_softmax(Tensor x, Tensor? mask=None, float scale=1.0, ScalarType? dtype=None, "
         "str rounding='fused') -> Tensor");
+  m.def("topk(Tensor x, int k) -> (Tensor, Tensor)");
+  m.def("topk_backward(Tensor dvalues, Tensor indices, int cols) -> Tensor");
+  m.def("distill_topk(Tensor logits, Tensor teacher_logits, Tensor teacher_ids, "
+        "float temperature=1.0) -> (Tensor, Tensor)");
+  m.def("distill_topk_backward(Tensor dloss, Tensor logits, Tensor stats, Tensor teacher_logits, "
+        "Tensor teacher_ids, float temperature=1.0, bool need_logits=True, "
+        "bool need_teacher=False) -> (Tensor, Tensor)");
+  m.def("distill_topk_grad(Tensor logits, Tensor teacher_logits, Tensor teacher_ids, "
+        "float temperature=1.0, Tensor? row_weight=None) -> (Tensor, Tensor)");
+  m.def("verify_draft(Tensor draft_ids, Tensor target_probs, Tensor? draft_probs, Tensor uniform, "
+        "Tensor? draft_lens=None) -> (Tensor, Tensor)");
 }
 
 #define FLB_FUSED_IMPLS(m)                          \
@@ -367,7 +586,13 @@ TORCH_LIBRARY(flagos, m) {
   m.impl("rms_norm_backward", RmsNormBackward);     \
   m.impl("swiglu_backward", SwigluBackward);        \
   m.impl("softmax_backward", SoftmaxBackward);      \
-  m.impl("masked_softmax", MaskedSoftmax);
+  m.impl("masked_softmax", MaskedSoftmax);          \
+  m.impl("topk", Topk);                             \
+  m.impl("topk_backward", TopkBackward);            \
+  m.impl("distill_topk", DistillTopk);              \
+  m.impl("distill_topk_backward", DistillTopkBackward); \
+  m.impl("distill_topk_grad", DistillTopkGrad);     \
+  m.impl("verify_draft", VerifyDraft);
 
 TORCH_LIBRARY_IMPL(flagos, PrivateUse1, m) { FLB_FUSED_IMPLS(m) }
 TORCH_LIBRARY_IMPL(flagos, CUDA, m) { FLB_FUSED_IMPLS(m) }

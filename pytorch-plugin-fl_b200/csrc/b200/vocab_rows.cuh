@@ -1,0 +1,138 @@
+// Helpers of the vocabulary-row kernels (distill.cu, topk.cu, verify.cu):
+// rows of any length and alignment split into 16-byte packs, thread-block
+// clusters that share one row, and small typed loads.
+#pragma once
+
+#include "common.cuh"
+
+namespace flb200 {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kLowest = -3.402823466e+38f;  // running maxima start here, not at -inf:
+                                              // x - m stays defined for x = -inf
+
+// 2^x, relative error about 2^-22; results below 2^-126 flush to 0.
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// A row as `head` single elements, `nvec` 16-byte packs on 16-byte
+// boundaries, and `tail` single elements (head, tail < elements per pack).
+struct RowSplit {
+  int head, nvec, tail;
+};
+template <typename T>
+__device__ __forceinline__ RowSplit split_row(const T* x, int cols) {
+  constexpr int VW = Elem<T>::kVec;
+  const int off = (int)((reinterpret_cast<uintptr_t>(x) & 15u) / sizeof(T));
+  RowSplit s;
+  s.head = min((VW - off) % VW, cols);
+  s.nvec = (cols - s.head) / VW;
+  s.tail = cols - s.head - s.nvec * VW;
+  return s;
+}
+// The single element of thread `t` (a CTA has at least 16 threads): threads
+// 0..7 take the head, 8..15 the tail; -1 where there is none.
+__device__ __forceinline__ int single_of(const RowSplit& s, int t, int vw) {
+  if (t < s.head) return t;
+  if (t >= 8 && t < 8 + s.tail) return s.head + s.nvec * vw + (t - 8);
+  return -1;
+}
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_id() {
+  uint32_t r;
+  asm("mov.u32 %0, %%clusterid.x;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_count() {
+  uint32_t r;
+  asm("mov.u32 %0, %%nclusterid.x;" : "=r"(r));
+  return r;
+}
+// Barrier of every thread of the cluster (release / acquire at cluster scope).
+__device__ __forceinline__ void cluster_sync_all() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Address of this CTA's shared object `p` in CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t remote_smem(const void* p, uint32_t rank) {
+  const uint32_t a = (uint32_t)__cvta_generic_to_shared(p);
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float2 ld_remote_f2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];"
+               : "=f"(v.x), "=f"(v.y)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ long long ld_remote_s64(uint32_t addr) {
+  long long v;
+  asm volatile("ld.shared::cluster.s64 %0, [%1];" : "=l"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+// Element i of an array whose type is known at run time.
+__device__ __forceinline__ float load_float(const void* p, int dtype, int64_t i) {
+  if (dtype == FL_B200_F32) return reinterpret_cast<const float*>(p)[i];
+  if (dtype == FL_B200_BF16)
+    return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
+  return __half2float(reinterpret_cast<const __half*>(p)[i]);
+}
+__device__ __forceinline__ void store_float(void* p, int dtype, int64_t i, float v) {
+  if (dtype == FL_B200_F32) {
+    reinterpret_cast<float*>(p)[i] = v;
+  } else if (dtype == FL_B200_BF16) {
+    reinterpret_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+  } else {
+    reinterpret_cast<__half*>(p)[i] = __float2half_rn(v);
+  }
+}
+__device__ __forceinline__ int64_t load_index(const void* p, int dtype, int64_t i) {
+  return dtype == FL_B200_I64 ? reinterpret_cast<const int64_t*>(p)[i]
+                              : (int64_t)reinterpret_cast<const int32_t*>(p)[i];
+}
+
+__device__ __forceinline__ float warp_sum(float v) { return group_reduce_warp<SumOp, 32>(v); }
+
+// Launches `kern` with `ctas` CTAs in clusters of `cluster`.
+template <typename... KArgs, typename... Args>
+inline int launch_cluster(void (*kern)(KArgs...), int64_t ctas, int cluster, int block, size_t smem,
+                          cudaStream_t stream, Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.blockDim = dim3((unsigned)block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)cluster;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  (void)cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
+  return launch_status();
+}
+
+}  // namespace
+}  // namespace flb200

@@ -83,6 +83,19 @@ PROTOTYPES: dict[str, tuple] = {
     "fl_b200_softmax_bwd": (_i32, [_p, _i64, _p, _i64, _p, _i64, _i64, _i64, _i32, _i32, _p]),
     "fl_b200_softmax_bwd_scaled": (
         _i32, [_p, _i64, _p, _i64, _p, _i64, _i64, _i64, _f32, _i32, _i32, _p]),
+    "fl_b200_topk_lastdim": (_i32, [_p, _i64, _i64, _i64, _i64, _p, _p, _i32, _p]),
+    "fl_b200_topk_bwd": (_i32, [_p, _p, _p, _i64, _i64, _i64, _i32, _p]),
+    "fl_b200_distill_topk_fwd": (
+        _i32, [_p, _i64, _p, _i64, _i32, _p, _i64, _i32, _i64, _i64, _i64, _f32, _p, _p, _i32, _p]),
+    "fl_b200_distill_topk_bwd": (
+        _i32, [_p, _i64, _p, _i64, _p, _p, _i64, _i32, _p, _i64, _i32, _p, _i64, _p,
+               _i64, _i64, _i64, _f32, _i32, _p]),
+    "fl_b200_distill_topk_grad": (
+        _i32, [_p, _i64, _p, _i64, _i32, _p, _i64, _i32, _p, _i64, _i64, _i64, _i64, _f32,
+               _p, _p, _p, _i64, _i32, _p]),
+    "fl_b200_verify_draft": (
+        _i32, [_p, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _p, _i64, _i64, _i64, _p, _p,
+               _i32, _p]),
 }
 
 

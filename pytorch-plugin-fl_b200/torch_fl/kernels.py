@@ -552,6 +552,144 @@ def sum_i32_i64(x: torch.Tensor, full: bool) -> torch.Tensor:
     return out
 
 
+# ------------------------------------------------------ rows of the vocabulary
+def topk_lastdim(x: torch.Tensor, k: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """(values, int64 indices) of the k largest over the last dim, descending;
+    ties by ascending index, NaN above everything."""
+    x, rows, cols, ld = _rows_or_contig(x)
+    shape = list(x.shape[:-1]) + [k]
+    values = torch.empty(shape, dtype=x.dtype, device=x.device)
+    indices = torch.empty(shape, dtype=torch.int64, device=x.device)
+    with _on_device(x):
+        _abi.call("fl_b200_topk_lastdim", x.data_ptr(), ld, rows, cols, k, values.data_ptr(),
+                  indices.data_ptr(), dtype_code(x), _stream(x))
+    return values, indices
+
+
+def topk_backward(dvalues: torch.Tensor, indices: torch.Tensor, cols: int) -> torch.Tensor:
+    """dx [..., cols] of topk_lastdim's values."""
+    if dvalues.shape != indices.shape or indices.dtype != torch.int64:
+        raise ValueError("dvalues and int64 indices must match")
+    dvalues, indices = dvalues.contiguous(), indices.contiguous()
+    k = dvalues.shape[-1]
+    rows = dvalues.shape[:-1].numel()
+    dx = torch.empty(list(dvalues.shape[:-1]) + [cols], dtype=dvalues.dtype, device=dvalues.device)
+    with _on_device(dvalues):
+        _abi.call("fl_b200_topk_bwd", dvalues.data_ptr(), indices.data_ptr(), dx.data_ptr(), rows,
+                  cols, k, dtype_code(dvalues), _stream(dvalues))
+    return dx
+
+
+def _taught(logits, teacher_logits, teacher_ids):
+    """Rows views of a student's logits and its teacher's lists, checked."""
+    if teacher_ids.dtype not in (torch.int32, torch.int64):
+        raise TypeError("teacher_ids must be int32 or int64")
+    if teacher_logits.shape != teacher_ids.shape or teacher_ids.shape[:-1] != logits.shape[:-1]:
+        raise ValueError("logits [..., vocab] with teacher_logits and teacher_ids [..., k] expected")
+    x, rows, cols, ld = _rows_or_contig(logits)
+    t, _, k, ld_t = _rows_or_contig(teacher_logits)
+    i, _, _, ld_i = _rows_or_contig(teacher_ids)
+    head = (x.data_ptr(), ld)
+    lists = (t.data_ptr(), ld_t, dtype_code(t), i.data_ptr(), ld_i, dtype_code(i))
+    return (x, t, i), head, lists, logits.shape[:-1].numel(), cols, k
+
+
+def _row_weight(w, shape):
+    """A float32 tensor that broadcasts to the loss as (tensor, pointer, row stride)."""
+    if w is None:
+        return None, None, 0
+    if w.dtype != torch.float32:
+        raise TypeError("row weights must be float32")
+    w = w.expand(shape).reshape(-1)
+    return w, w.data_ptr(), w.stride(0) if w.numel() > 1 else 0
+
+
+def distill_topk(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ids: torch.Tensor,
+                 temperature: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
+    """(loss [...], stats [rows, 2]), both float32: temperature^2 * KL of the
+    teacher's list against the student's softmax, and what the backward needs."""
+    (x, *keep), head, lists, rows, cols, k = _taught(logits, teacher_logits, teacher_ids)
+    loss = torch.empty(logits.shape[:-1], dtype=torch.float32, device=x.device)
+    stats = torch.empty((rows, 2), dtype=torch.float32, device=x.device)
+    with _on_device(x):
+        _abi.call("fl_b200_distill_topk_fwd", *head, *lists, rows, cols, k, float(temperature),
+                  loss.data_ptr(), stats.data_ptr(), dtype_code(x), _stream(x))
+    return loss, stats
+
+
+def distill_topk_backward(dloss: torch.Tensor | None, logits: torch.Tensor, stats: torch.Tensor,
+                          teacher_logits: torch.Tensor, teacher_ids: torch.Tensor,
+                          temperature: float = 1.0, need_logits: bool = True,
+                          need_teacher: bool = False):
+    """(dlogits, dteacher) from the forward's stats; None for one not needed.
+    dloss broadcasts to the loss; None is 1 for every row."""
+    (x, *keep), head, lists, rows, cols, k = _taught(logits, teacher_logits, teacher_ids)
+    if stats.dtype != torch.float32 or tuple(stats.shape) != (rows, 2) or not stats.is_contiguous():
+        raise ValueError("stats must be the forward's [rows, 2] float32 tensor")
+    w, wp, ws = _row_weight(dloss, logits.shape[:-1])
+    dx = torch.empty(logits.shape, dtype=x.dtype, device=x.device) if need_logits else None
+    dt = torch.empty(teacher_logits.shape, dtype=teacher_logits.dtype,
+                     device=x.device) if need_teacher else None
+    with _on_device(x):
+        _abi.call("fl_b200_distill_topk_bwd", wp, ws, *head, stats.data_ptr(), *lists,
+                  dx.data_ptr() if need_logits else None, cols,
+                  dt.data_ptr() if need_teacher else None, rows, cols, k, float(temperature),
+                  dtype_code(x), _stream(x))
+    return dx, dt
+
+
+def distill_topk_grad(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ids: torch.Tensor,
+                      temperature: float = 1.0, row_weight: torch.Tensor | None = None,
+                      out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """(loss, dlogits) of sum(row_weight * loss) in one call."""
+    (x, *keep), head, lists, rows, cols, k = _taught(logits, teacher_logits, teacher_ids)
+    w, wp, ws = _row_weight(row_weight, logits.shape[:-1])
+    loss = torch.empty(logits.shape[:-1], dtype=torch.float32, device=x.device)
+    stats = torch.empty((rows, 2), dtype=torch.float32, device=x.device)
+    dx = torch.empty(logits.shape, dtype=x.dtype, device=x.device) if out is None else out
+    if dx.shape != logits.shape or dx.dtype != x.dtype:
+        raise ValueError("out must have the logits' shape and dtype")
+    _, _, ldo = _rows_view(dx)
+    with _on_device(x):
+        _abi.call("fl_b200_distill_topk_grad", *head, *lists, wp, ws, rows, cols, k,
+                  float(temperature), loss.data_ptr(), stats.data_ptr(), dx.data_ptr(), ldo,
+                  dtype_code(x), _stream(x))
+    return loss, dx
+
+
+def verify_draft(draft_ids: torch.Tensor, target_probs: torch.Tensor,
+                 draft_probs: torch.Tensor | None, uniform: torch.Tensor,
+                 draft_lens: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """(tokens [batch, drafts + 1], accepted [batch]) of speculative sampling;
+    see ops.verify_draft."""
+    B, n = draft_ids.shape
+    V = target_probs.shape[-1]
+    if draft_ids.dtype != torch.int64 or uniform.dtype != torch.float32:
+        raise TypeError("draft_ids must be int64 and uniform float32")
+    if tuple(target_probs.shape) != (B, n + 1, V) or tuple(uniform.shape) != (B, n + 1):
+        raise ValueError("target_probs [batch, drafts + 1, vocab] and uniform [batch, drafts + 1] expected")
+    if draft_probs is not None and (tuple(draft_probs.shape) != (B, n, V)
+                                    or draft_probs.dtype != target_probs.dtype):
+        raise ValueError("draft_probs must be [batch, drafts, vocab] of target_probs' dtype")
+    if draft_lens is not None and (tuple(draft_lens.shape) != (B,) or draft_lens.dtype != torch.int64):
+        raise ValueError("draft_lens must be int64 [batch]")
+
+    def unit(t):
+        return t if t is None or t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
+
+    ids, p, q, u = unit(draft_ids), unit(target_probs), unit(draft_probs), unit(uniform)
+    lens = None if draft_lens is None else draft_lens.contiguous()
+    tokens = torch.empty((B, n + 1), dtype=torch.int64, device=p.device)
+    accepted = torch.empty((B,), dtype=torch.int64, device=p.device)
+    with _on_device(p):
+        _abi.call("fl_b200_verify_draft", ids.data_ptr(), ids.stride(0), p.data_ptr(), p.stride(0),
+                  p.stride(1), None if q is None else q.data_ptr(), 0 if q is None else q.stride(0),
+                  0 if q is None else q.stride(1), u.data_ptr(), u.stride(0),
+                  None if lens is None else lens.data_ptr(), B, n, V, tokens.data_ptr(),
+                  accepted.data_ptr(), dtype_code(p), _stream(p))
+    return tokens, accepted
+
+
 # -------------------------------------------------------------------- backward
 def rms_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, eps: float,
                       need_dw: bool = True) -> tuple[torch.Tensor, torch.Tensor | None]:

@@ -75,3 +75,59 @@ def masked_softmax(x, mask=None, scale: float = 1.0, dtype: torch.dtype | None =
     fused) or float32."""
     return torch.ops.flagos.masked_softmax(x, mask, float(scale), dtype,
                                            rounding or default_rounding())
+
+
+# ---------------------------------------------------- rows of the vocabulary
+def topk(x, k: int):
+    """(values, indices) of the k <= 1024 largest elements over the last dim,
+    descending; equal values (-0 and +0 among them) by ascending index, NaN
+    above everything, so there is one right answer.  Gradient: dvalues at the
+    indices."""
+    return torch.ops.flagos.topk(x, int(k))
+
+
+def distill_topk(logits, teacher_logits, teacher_ids, temperature: float = 1.0):
+    """The distillation loss of each row, float32 [...]:
+
+        temperature^2 * KL(softmax(teacher_logits / temperature) ||
+                           softmax(logits / temperature)[teacher_ids])
+
+    for a student's logits [..., vocab] and the k <= 1024 logits [..., k] that
+    were kept of a teacher (`topk`), with their token ids (int32 or int64).
+    The teacher's softmax is over its list; entries whose id lies outside
+    [0, vocab) (-1, say) are absent, and a row without any has loss 0 and zero
+    gradients whatever its logits hold.  Repeated ids add.  Differentiable in
+    logits and in teacher_logits; the gradient is computed from the saved
+    logits, so they are read three times in all: `distill_topk_grad` reads
+    them once."""
+    return torch.ops.flagos.distill_topk(logits, teacher_logits, teacher_ids, float(temperature))[0]
+
+
+def distill_topk_grad(logits, teacher_logits, teacher_ids, temperature: float = 1.0,
+                      row_weight=None):
+    """(loss, dlogits): `distill_topk`'s loss of each row, and the gradient of
+    sum(row_weight * loss) with respect to the logits, in one call, for
+    training loops whose row weights are known beforehand (1 / tokens, a loss
+    mask, a loss scale).  row_weight is float32 and broadcasts to the loss;
+    None weighs every row 1.  Not differentiable: hand dlogits on with
+    `logits.backward(dlogits)`."""
+    return torch.ops.flagos.distill_topk_grad(logits, teacher_logits, teacher_ids,
+                                              float(temperature), row_weight)
+
+
+def verify_draft(draft_ids, target_probs, draft_probs, uniform, draft_lens=None):
+    """Speculative sampling's verification: (tokens, accepted), int64
+    [batch, drafts + 1] and [batch].
+
+    draft_ids [batch, drafts] are the drafted tokens, draft_lens [batch] how
+    many of them each sequence has (None: all), target_probs
+    [batch, drafts + 1, vocab] the target's probabilities at each and after
+    the last, draft_probs [batch, drafts, vocab] the draft model's (None:
+    drafts that come without, as looked-up ones do), uniform
+    [batch, drafts + 1] float32 numbers in [0, 1).  Token i is kept while
+    uniform[i] * q(token) < p(token); the next is drawn with uniform[drafts]
+    from max(p - q, 0) at the first token turned down, else from the target's
+    row after the last.  tokens holds the kept ones, the drawn one, then -1;
+    accepted how many were kept.  The draw is exact in 36-bit fixed point, so
+    it does not depend on the order of any sum."""
+    return torch.ops.flagos.verify_draft(draft_ids, target_probs, draft_probs, uniform, draft_lens)
