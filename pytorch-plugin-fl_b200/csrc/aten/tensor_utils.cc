@@ -44,8 +44,11 @@ int B200Dtype(at::ScalarType t) {
 
 void CheckB200(int status, const char* op) {
   if (status == FL_B200_OK) return;
-  TORCH_CHECK(false, op, " (b200 route): ", fl_b200_status_string(status), " [status ", status,
-              ", cuda error ", fl_b200_last_cuda_error(), "]");
+  // (numbers are formatted first: inserting an integer into the message's
+  // stream crashes where libtorch and this module differ in libstdc++)
+  TORCH_CHECK(false, op, " (b200 route): ", fl_b200_status_string(status), " [status ",
+              std::to_string(status), ", cuda error ", std::to_string(fl_b200_last_cuda_error()),
+              "]");
 }
 
 std::optional<RowsView> AsRows(const at::Tensor& x) {

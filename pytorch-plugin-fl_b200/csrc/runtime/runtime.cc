@@ -41,8 +41,8 @@ c10::DeviceIndex current_device() {
 }
 
 void set_device(c10::DeviceIndex d) {
-  TORCH_CHECK(d >= 0 && d < device_count(), "flagos: invalid device index ", int(d),
-              " (", int(device_count()), " devices)");
+  TORCH_CHECK(d >= 0 && d < device_count(), "flagos: invalid device index ", std::to_string(d),
+              " (", std::to_string(device_count()), " devices)");
   int cur = -1;
   C10_CUDA_CHECK(cudaGetDevice(&cur));
   if (cur != d) C10_CUDA_CHECK(cudaSetDevice(d));
@@ -121,8 +121,8 @@ class PoolAllocator final : public c10::Allocator {
     }
     if (e != cudaSuccess) {
       (void)cudaGetLastError();
-      TORCH_CHECK(false, "flagos: out of device memory allocating ", nbytes,
-                  " bytes on device ", int(d), ": ", cudaGetErrorString(e));
+      TORCH_CHECK(false, "flagos: out of device memory allocating ", std::to_string(nbytes),
+                  " bytes on device ", std::to_string(d), ": ", cudaGetErrorString(e));
     }
     {
       std::lock_guard<std::mutex> lock(mu_);
@@ -365,8 +365,8 @@ struct GuardImpl final : public c10::impl::DeviceGuardImplInterface {
   void record(void** event, const c10::Stream& stream, const c10::DeviceIndex device_index,
               const c10::EventFlag flag) const override {
     TORCH_CHECK(device_index == -1 || device_index == stream.device_index(),
-                "flagos: event device ", int(device_index), " does not match stream device ",
-                int(stream.device_index()));
+                "flagos: event device ", std::to_string(device_index),
+                " does not match stream device ", std::to_string(stream.device_index()));
     DeviceScope scope(stream.device_index());
     auto ev = static_cast<cudaEvent_t>(*event);
     if (!ev) {

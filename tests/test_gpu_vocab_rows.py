@@ -453,6 +453,13 @@ def test_refusals_of_the_ops():
             bad()
 
 
+def test_a_status_of_the_library_is_an_error_with_its_text():
+    p = torch.zeros(1, 1, 1 << 26, dtype=torch.bfloat16, device=DEV)
+    ids = torch.zeros(1, 0, dtype=torch.int64, device=DEV)
+    with pytest.raises(RuntimeError, match="exceeds the fixed maximum.*status 7"):
+        torch.ops.flagos.verify_draft(ids, p, None, torch.zeros(1, 1, device=DEV))
+
+
 def test_streams_and_graph_replay():
     """Each op on a side stream, and captured into a graph that is replayed on
     new inputs."""

@@ -2,6 +2,10 @@
 finite differences and by its own distribution, and the host-side refusals of
 the C ABI (nothing here launches a kernel)."""
 
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 
@@ -138,3 +142,14 @@ def test_empty_work_is_a_no_op():
               0, 8, 4, 1.0, 1, None)
     _abi.call("fl_b200_distill_topk_grad", None, 0, None, 0, 1, None, 0, 4, None, 0, 0, 8, 4, 1.0, None,
               None, None, 0, 1, None)
+
+
+def test_a_message_with_numbers_is_an_error_not_a_crash():
+    """Native checks whose message holds integers raise (in a child process:
+    they once ended it)."""
+    pkg = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "pytorch-plugin-fl_b200")
+    code = ("import torch_fl\nfrom torch_fl import _C\n"
+            "try:\n    _C._set_device(99)\nexcept RuntimeError as e:\n    print('raised', e)\n")
+    r = subprocess.run([sys.executable, "-c", code], env=dict(os.environ, PYTHONPATH=pkg),
+                       capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "raised flagos: invalid device index 99" in r.stdout, (r.returncode, r.stdout, r.stderr[-300:])
