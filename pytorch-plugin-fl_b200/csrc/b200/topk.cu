@@ -9,10 +9,17 @@
 namespace flb200 {
 namespace {
 
-constexpr int kMaxTop = 1024;
+constexpr int kMaxTop = FL_B200_TOPK_MAX;
 constexpr int kBlock = 512;
+constexpr int kWarps = kBlock / 32;
+constexpr int kPacks = 8;      // 16-byte packs a thread holds: a chunk of the row is kBlock * kPacks
+constexpr int kCap = 3072;     // candidates kept
+constexpr int kTighten = 1536; // above this many the threshold is raised over the candidates
+constexpr int kQueue = 512;    // packs of a chunk that hold candidates
+constexpr int kSort = 2048;    // keys sorted at the end: at most 1.25 * kMaxTop
 
-// Monotone 32-bit image of a value: unsigned order is float order, NaN on top.
+// Monotone 32-bit image of a value: unsigned order is float order, NaN on
+// top; never 0.
 __device__ __forceinline__ uint32_t value_key(float f) {
   const uint32_t u = __float_as_uint(f + 0.0f);  // -0 -> +0
   if (f != f) return 0xffffffffu;
@@ -22,19 +29,114 @@ __device__ __forceinline__ uint64_t element_key(float f, uint32_t index) {
   return ((uint64_t)value_key(f) << 32) | (uint32_t)~index;
 }
 
-// Descending bitonic sort of n (a power of two) keys in shared memory by the
-// whole CTA.
-__device__ __forceinline__ void sort_desc(uint64_t* s, int n) {
+// NaN-propagating maximum of a pack.
+template <typename T>
+__device__ __forceinline__ float pack_top(const uint4& u) {
+  float r;
+  if constexpr (std::is_same<T, float>::value) {
+    float a, b;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(a) : "f"(__uint_as_float(u.x)), "f"(__uint_as_float(u.y)));
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(b) : "f"(__uint_as_float(u.z)), "f"(__uint_as_float(u.w)));
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  } else {
+    uint32_t a, b, c;
+    if constexpr (std::is_same<T, __half>::value) {
+      asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(a) : "r"(u.x), "r"(u.y));
+      asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(b) : "r"(u.z), "r"(u.w));
+      asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(c) : "r"(a), "r"(b));
+    } else {
+      asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(a) : "r"(u.x), "r"(u.y));
+      asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(b) : "r"(u.z), "r"(u.w));
+      asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(c) : "r"(a), "r"(b));
+    }
+    const uint64_t p = pair_from_bits<T>(c);
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(f2_lo(p)), "f"(f2_hi(p)));
+  }
+  return r;
+}
+
+template <typename T>
+struct Shared {
+  uint64_t cand[kCap];       // candidates, in no order
+  union {
+    struct {
+      uint4 pack[kQueue];
+      int at[kQueue];
+    } q;
+    uint64_t sort[kSort];
+  };
+  int sums[2][kWarps];
+  int hist[256];
+  int filled, queued, pick, above;
+  int found;                 // candidates this CTA offers its cluster
+};
+
+// Sum of v over the CTA, in every thread.  `parity` alternates between the
+// two halves of the scratch, so that one barrier a call is enough.
+template <typename S>
+__device__ __forceinline__ int block_sum(S& s, int v, int& parity) {
+  const int lane = threadIdx.x & 31;
+  v = __reduce_add_sync(0xffffffffu, v);
+  if (lane == 0) s.sums[parity][threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = __reduce_add_sync(0xffffffffu, lane < kWarps ? s.sums[parity][lane] : 0);
+  parity ^= 1;
+  return v;
+}
+
+// The largest key K (a prefix of `bits` bits, zeros below) that at least k of
+// the counted keys reach, found bit by bit from the top; stops early once at
+// most `enough` reach it.  count(K) is the thread's own number of keys >= K.
+template <typename K, typename S, typename F>
+__device__ __forceinline__ K bisect(S& s, int k, int enough, int& parity, F count) {
+  K at = 0;
+  for (int bit = (int)sizeof(K) * 8 - 1; bit >= 0; --bit) {
+    const K tried = at | ((K)1 << bit);
+    const int n = block_sum(s, count(tried), parity);
+    if (n >= k) {
+      at = tried;
+      if (n <= enough) break;
+    }
+  }
+  return at;
+}
+
+template <typename S>
+__device__ __forceinline__ void append(S& s, uint64_t key) {
+  const int slot = atomicAdd(&s.filled, 1);
+  if (slot < kCap) s.cand[slot] = key;
+}
+
+// Keeps the candidates at or above a 64-bit key.
+template <typename S>
+__device__ __forceinline__ void keep_above(S& s, int n, uint64_t floor) {
+  uint64_t mine[kCap / kBlock];
+#pragma unroll
+  for (int i = 0; i < kCap / kBlock; ++i) {
+    const int j = threadIdx.x + i * kBlock;
+    mine[i] = j < n ? s.cand[j] : 0;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) s.filled = 0;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kCap / kBlock; ++i)
+    if (mine[i] >= floor && mine[i] != 0) append(s, mine[i]);
+  __syncthreads();
+}
+
+// Descending bitonic sort of s.sort[0..n), n a power of two.
+template <typename S>
+__device__ __forceinline__ void sort_desc(S& s, int n) {
   for (int size = 2; size <= n; size <<= 1) {
     for (int stride = size >> 1; stride > 0; stride >>= 1) {
       __syncthreads();
       for (int i = threadIdx.x; i < n / 2; i += kBlock) {
         const int lo = 2 * i - (i & (stride - 1));
-        const uint64_t a = s[lo], b = s[lo + stride];
-        const bool desc = (lo & size) == 0;
-        if ((a < b) == desc) {
-          s[lo] = b;
-          s[lo + stride] = a;
+        const uint64_t a = s.sort[lo], b = s.sort[lo + stride];
+        if ((a < b) == ((lo & size) == 0)) {
+          s.sort[lo] = b;
+          s.sort[lo + stride] = a;
         }
       }
     }
@@ -42,57 +144,229 @@ __device__ __forceinline__ void sort_desc(uint64_t* s, int n) {
   __syncthreads();
 }
 
-// The k largest keys of a row by radix selection: eight passes at most over
-// the row, each a histogram of the next 8 bits of the keys that match the
-// prefix found so far, until the keys at or above the prefix are exactly k.
+// The k largest keys of elements [lo, hi) by radix selection: eight passes
+// at most, each a histogram of the next 8 bits of the keys that match the
+// prefix found so far, until exactly k keys reach it.  For slices whose
+// candidates overflow; right for any values.
 template <typename T>
-__global__ void __launch_bounds__(kBlock)
-topk_kernel(const T* __restrict__ x, int64_t ld, int cols, int k, int kpow2, T* __restrict__ values,
-            int64_t* __restrict__ indices) {
-  __shared__ uint64_t best[kMaxTop];
-  __shared__ int hist[256];
-  __shared__ int pick, above, filled;
-  pdl_prologue();
-  const int64_t row = blockIdx.x;
-  const T* xr = x + row * ld;
+__device__ __noinline__ void radix_select(Shared<T>& s, const T* xr, int lo, int hi, int k) {
   const int tid = threadIdx.x;
   uint64_t prefix = 0;
   int need = k, shift = 64;
   while (shift > 0) {
     shift -= 8;
-    for (int i = tid; i < 256; i += kBlock) hist[i] = 0;
+    for (int i = tid; i < 256; i += kBlock) s.hist[i] = 0;
     __syncthreads();
-    for (int i = tid; i < cols; i += kBlock) {
+    for (int i = lo + tid; i < hi; i += kBlock) {
       const uint64_t key = element_key(Elem<T>::to_f(xr[i]), (uint32_t)i);
       if (shift == 56 || (key >> (shift + 8)) == (prefix >> (shift + 8)))
-        atomicAdd(&hist[(key >> shift) & 255], 1);
+        atomicAdd(&s.hist[(key >> shift) & 255], 1);
     }
     __syncthreads();
     if (tid == 0) {
       int sum = 0, d = 255;
-      while (sum + hist[d] < need) sum += hist[d--];
-      pick = d;
-      above = sum;
+      while (d > 0 && sum + s.hist[d] < need) sum += s.hist[d--];
+      s.pick = d;
+      s.above = sum;
     }
     __syncthreads();
-    prefix |= (uint64_t)pick << shift;
-    need -= above;
-    const bool done = hist[pick] == need;
+    prefix |= (uint64_t)s.pick << shift;
+    need -= s.above;
+    const bool done = s.hist[s.pick] == need;
     __syncthreads();
     if (done) break;
   }
-  if (tid == 0) filled = 0;
-  for (int i = tid; i < kpow2; i += kBlock) best[i] = 0;
+  if (tid == 0) s.filled = 0;
   __syncthreads();
-  for (int i = tid; i < cols; i += kBlock) {
+  for (int i = lo + tid; i < hi; i += kBlock) {
     const uint64_t key = element_key(Elem<T>::to_f(xr[i]), (uint32_t)i);
-    if (key >= prefix) best[atomicAdd(&filled, 1)] = key;
+    if (key >= prefix) append(s, key);
   }
-  sort_desc(best, kpow2);
-  for (int i = tid; i < k; i += kBlock) {
-    const uint32_t at = ~(uint32_t)best[i];
-    indices[row * k + i] = at;
-    values[row * k + i] = xr[at];
+  __syncthreads();
+}
+
+// Candidates of elements [lo, hi) of a row, which hold its k largest keys
+// (k <= hi - lo); returns their number, in every thread.
+//
+// The slice is read once, a chunk at a time, against a threshold below which
+// nothing can be among the k largest.  A first threshold is the k-th largest
+// maximum of the first chunk's packs: k packs, hence k elements, reach it.
+// After that a pack matters only if its maximum exceeds the threshold, which
+// few do: they go to a queue whose elements the whole CTA then tests.  An
+// element of a later chunk that only equals the threshold loses to the k
+// before it, so the test is strict there and ties resolve by index.
+template <typename T>
+__device__ __forceinline__ int collect(Shared<T>& s, const T* xr, int lo, int hi, int k, int& parity) {
+  constexpr int VW = Elem<T>::kVec;
+  const int tid = threadIdx.x;
+  const RowSplit sp = split_row(xr + lo, hi - lo);
+  const uint4* body = reinterpret_cast<const uint4*>(xr + lo + sp.head);
+  if (tid == 0) s.filled = s.queued = 0;
+  __syncthreads();
+  if (tid < sp.head) append(s, element_key(Elem<T>::to_f(xr[lo + tid]), (uint32_t)(lo + tid)));
+  uint32_t floor = 0;  // nothing at or below it matters any more (0: none yet)
+  for (int base = 0; base < sp.nvec; base += kBlock * kPacks) {
+    uint4 u[kPacks];
+    uint32_t top[kPacks];
+#pragma unroll
+    for (int i = 0; i < kPacks; ++i) {
+      const int p = base + i * kBlock + tid;
+      u[i] = p < sp.nvec ? ld_stream(body + p) : make_uint4(0, 0, 0, 0);
+    }
+    int over = 0;
+#pragma unroll
+    for (int i = 0; i < kPacks; ++i) {
+      top[i] = base + i * kBlock + tid < sp.nvec ? value_key(pack_top<T>(u[i])) : 0;
+      over += top[i] > floor;
+    }
+    int hits = block_sum(s, over, parity);
+    int n = s.filled;  // (appends follow the next barrier)
+    if (n > kCap) return n;
+    uint32_t least = floor + 1;  // elements of this chunk need at least this key
+    if (floor == 0xffffffffu) least = floor, hits = 0;
+    if (hits >= (floor == 0 ? k : 4 * k)) {
+      const uint32_t t = bisect<uint32_t>(s, k, k + k / 8, parity, [&](uint32_t c) {
+        int m = 0;
+#pragma unroll
+        for (int i = 0; i < kPacks; ++i) m += top[i] >= c;
+        return m;
+      });
+      if (t > floor) {
+        floor = t;
+        least = t;
+        int m = 0;
+#pragma unroll
+        for (int i = 0; i < kPacks; ++i) m += top[i] >= least;
+        hits = block_sum(s, m, parity);
+      }
+    }
+    if (n > kTighten) {
+      const uint32_t t = bisect<uint32_t>(s, k, k + k / 8, parity, [&](uint32_t c) {
+        int m = 0;
+        for (int j = tid; j < n; j += kBlock) m += (uint32_t)(s.cand[j] >> 32) >= c;
+        return m;
+      });
+      keep_above(s, n, (uint64_t)t << 32);
+      if (t > floor) {
+        floor = t;
+        least = t == 0xffffffffu ? t : t + 1;
+      }
+    }
+    __syncthreads();
+    if (hits == 0) continue;
+    if (hits <= kQueue) {
+#pragma unroll
+      for (int i = 0; i < kPacks; ++i) {
+        if (top[i] < least) continue;
+        const int slot = atomicAdd(&s.queued, 1);
+        s.q.pack[slot] = u[i];
+        s.q.at[slot] = base + i * kBlock + tid;
+      }
+      __syncthreads();
+      const int queued = s.queued;
+      const T* q = reinterpret_cast<const T*>(s.q.pack);
+      for (int j = tid; j < queued * VW; j += kBlock) {
+        const int e = lo + sp.head + s.q.at[j / VW] * VW + j % VW;
+        const uint64_t key = element_key(Elem<T>::to_f(q[j]), (uint32_t)e);
+        if ((uint32_t)(key >> 32) >= least) append(s, key);
+      }
+      __syncthreads();
+      if (tid == 0) s.queued = 0;
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPacks; ++i) {
+        if (top[i] < least) continue;
+        float f[VW];
+        unpack<T>(u[i], f);
+#pragma unroll
+        for (int j = 0; j < VW; ++j) {
+          const int e = lo + sp.head + (base + i * kBlock + tid) * VW + j;
+          if (value_key(f[j]) >= least) append(s, element_key(f[j], (uint32_t)e));
+        }
+      }
+    }
+  }
+  __syncthreads();
+  if (tid < sp.tail) {
+    const int e = hi - sp.tail + tid;
+    append(s, element_key(Elem<T>::to_f(xr[e]), (uint32_t)e));
+  }
+  __syncthreads();
+  return s.filled;
+}
+
+// One CTA a row, or a cluster with a slice of the row in each CTA when there
+// are few rows: every CTA finds its slice's candidates, CTA 0 takes them all
+// and orders the k largest.
+template <typename T>
+__global__ void __launch_bounds__(kBlock, 2)
+topk_kernel(const T* __restrict__ x, int64_t ld, int cols, int k, T* __restrict__ values,
+            int64_t* __restrict__ indices) {
+  __shared__ Shared<T> s;
+  pdl_prologue();
+  const int C = (int)cluster_size(), rank = (int)cluster_rank();
+  const int64_t row = cluster_id();
+  const T* xr = x + row * ld;
+  const int tid = threadIdx.x;
+  int parity = 0;
+  // slices of whole groups of 64 elements
+  const int per = (int)(ceil_div(ceil_div(cols, C), 64) * 64);
+  const int lo = min(cols, rank * per), hi = min(cols, lo + per);
+  const int want = min(k, hi - lo);
+  int n = collect(s, xr, lo, hi, want, parity);
+  if (n > kCap) {
+    radix_select(s, xr, lo, hi, want);
+    n = want;
+  }
+  const auto shrink = [&](int most) {  // to the k largest, at most `most` of them
+    const uint64_t floor = bisect<uint64_t>(s, min(k, n), most, parity, [&](uint64_t c) {
+      int m = 0;
+      for (int j = tid; j < n; j += kBlock) m += s.cand[j] >= c;
+      return m;
+    });
+    keep_above(s, n, floor);
+    n = s.filled;
+  };
+  if (C > 1) {
+    if (n > k) shrink(k);
+    if (tid == 0) s.found = n;
+    cluster_sync_all();
+    if (rank == 0) {
+      for (int r = 1; r < C; ++r) {
+        int m;
+        asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(m) : "r"(remote_smem(&s.found, r)) : "memory");
+        const uint32_t from = remote_smem(s.cand, r);
+        for (int j = tid; j < m; j += kBlock) s.cand[n + j] = (uint64_t)ld_remote_s64(from + 8 * j);
+        n += m;
+      }
+      __syncthreads();
+    }
+    cluster_sync_all();
+    if (rank != 0) return;
+  }
+  const int most = max(k + k / 4, 128);
+  if (n > most) shrink(most);
+  const auto put = [&](int place, uint64_t key) {
+    const uint32_t at = ~(uint32_t)key;
+    indices[row * k + place] = at;
+    values[row * k + place] = xr[at];
+  };
+  if (n <= kBlock / 2) {
+    // few keys: each one's place is the number of keys above it
+    int per_key = 32;
+    while (per_key * n > kBlock) per_key >>= 1;
+    const int i = tid / per_key;
+    const uint64_t key = i < n ? s.cand[i] : 0;
+    int place = 0;
+    for (int j = tid % per_key; j < n; j += per_key) place += s.cand[j] > key;
+    for (int o = per_key >> 1; o > 0; o >>= 1) place += __shfl_xor_sync(0xffffffffu, place, o);
+    if (i < n && tid % per_key == 0 && place < k) put(place, key);
+  } else {
+    int size = 1;
+    while (size < n) size <<= 1;
+    for (int i = tid; i < size; i += kBlock) s.sort[i] = i < n ? s.cand[i] : 0;
+    sort_desc(s, size);
+    for (int i = tid; i < k; i += kBlock) put(i, s.sort[i]);
   }
 }
 
@@ -130,14 +404,20 @@ FL_B200_API int fl_b200_topk_lastdim(const void* x, int64_t ld, int64_t rows, in
   if (k > kMaxTop || rows > 0x7fffffffLL || cols > 0x7fffff00LL) return FL_B200_ERR_TOO_LARGE;
   if (rows == 0 || k == 0) return FL_B200_OK;
   FLB_CHECK_ARG(x && values && indices && (rows == 1 || ld >= cols));
-  int kpow2 = 1;
-  while (kpow2 < k) kpow2 *= 2;
+  DeviceInfo dev;
+  const int st = current_device_info(&dev);
+  if (st != FL_B200_OK) return st;
   return dispatch_float(dtype, [&](auto t) {
     using T = decltype(t);
-    launch_k(topk_kernel<T>, dim3((unsigned)rows), dim3(kBlock), 0, (cudaStream_t)stream,
-             reinterpret_cast<const T*>(x), ld, (int)cols, (int)k, kpow2,
-             reinterpret_cast<T*>(values), indices);
-    return launch_status();
+    // few rows: up to 8 CTAs a row, of at least half a chunk each, whose
+    // candidates fit CTA 0
+    int cluster = 1;
+    while (cluster < 8 && rows * cluster < dev.sm_count && cluster * 2 * k <= kCap &&
+           cols / (cluster * 2) >= kBlock * Elem<T>::kVec)
+      cluster *= 2;
+    return launch_cluster(topk_kernel<T>, rows * cluster, cluster, kBlock, 0, (cudaStream_t)stream,
+                          reinterpret_cast<const T*>(x), ld, (int)cols, (int)k,
+                          reinterpret_cast<T*>(values), indices);
   });
 }
 
