@@ -55,7 +55,6 @@ __device__ __forceinline__ float pack_top(const uint4& u) {
   return r;
 }
 
-template <typename T>
 struct Shared {
   uint64_t cand[kCap];       // candidates, in no order
   union {
@@ -67,14 +66,13 @@ struct Shared {
   };
   int sums[2][kWarps];
   int hist[256];
-  int filled, queued, pick, above;
-  int found;                 // candidates this CTA offers its cluster
+  int filled, queued[2], pick, above;
+  uint4 stage[kPacks][kBlock];  // the next chunk, each thread's own packs
 };
 
 // Sum of v over the CTA, in every thread.  `parity` alternates between the
 // two halves of the scratch, so that one barrier a call is enough.
-template <typename S>
-__device__ __forceinline__ int block_sum(S& s, int v, int& parity) {
+__device__ __forceinline__ int block_sum(Shared& s, int v, int& parity) {
   const int lane = threadIdx.x & 31;
   v = __reduce_add_sync(0xffffffffu, v);
   if (lane == 0) s.sums[parity][threadIdx.x >> 5] = v;
@@ -84,13 +82,17 @@ __device__ __forceinline__ int block_sum(S& s, int v, int& parity) {
   return v;
 }
 
-// The largest key K (a prefix of `bits` bits, zeros below) that at least k of
-// the counted keys reach, found bit by bit from the top; stops early once at
-// most `enough` reach it.  count(K) is the thread's own number of keys >= K.
-template <typename K, typename S, typename F>
-__device__ __forceinline__ K bisect(S& s, int k, int enough, int& parity, F count) {
-  K at = 0;
-  for (int bit = (int)sizeof(K) * 8 - 1; bit >= 0; --bit) {
+// A key K that at least k of the counted keys reach, and at most `enough`
+// where that is possible: found bit by bit below the bits that `lo` and `hi`
+// share, all counted keys lying between these two.  count(K) is the thread's
+// own number of keys >= K.
+template <typename K, typename F>
+__device__ __forceinline__ K bisect(Shared& s, K lo, K hi, int k, int enough, int& parity, F count) {
+  K at = lo;
+  int bit = (int)sizeof(K) * 8 - 1;
+  while (bit >= 0 && (((lo ^ hi) >> bit) & 1) == 0) --bit;
+  at = bit < 0 ? lo : (lo >> bit >> 1) << bit << 1;
+  for (; bit >= 0; --bit) {
     const K tried = at | ((K)1 << bit);
     const int n = block_sum(s, count(tried), parity);
     if (n >= k) {
@@ -101,15 +103,13 @@ __device__ __forceinline__ K bisect(S& s, int k, int enough, int& parity, F coun
   return at;
 }
 
-template <typename S>
-__device__ __forceinline__ void append(S& s, uint64_t key) {
+__device__ __forceinline__ void append(Shared& s, uint64_t key) {
   const int slot = atomicAdd(&s.filled, 1);
   if (slot < kCap) s.cand[slot] = key;
 }
 
 // Keeps the candidates at or above a 64-bit key.
-template <typename S>
-__device__ __forceinline__ void keep_above(S& s, int n, uint64_t floor) {
+__device__ __forceinline__ void keep_above(Shared& s, int n, uint64_t floor) {
   uint64_t mine[kCap / kBlock];
 #pragma unroll
   for (int i = 0; i < kCap / kBlock; ++i) {
@@ -126,8 +126,7 @@ __device__ __forceinline__ void keep_above(S& s, int n, uint64_t floor) {
 }
 
 // Descending bitonic sort of s.sort[0..n), n a power of two.
-template <typename S>
-__device__ __forceinline__ void sort_desc(S& s, int n) {
+__device__ __forceinline__ void sort_desc(Shared& s, int n) {
   for (int size = 2; size <= n; size <<= 1) {
     for (int stride = size >> 1; stride > 0; stride >>= 1) {
       __syncthreads();
@@ -149,7 +148,7 @@ __device__ __forceinline__ void sort_desc(S& s, int n) {
 // prefix found so far, until exactly k keys reach it.  For slices whose
 // candidates overflow; right for any values.
 template <typename T>
-__device__ __noinline__ void radix_select(Shared<T>& s, const T* xr, int lo, int hi, int k) {
+__device__ __noinline__ void radix_select(Shared& s, const T* xr, int lo, int hi, int k) {
   const int tid = threadIdx.x;
   uint64_t prefix = 0;
   int need = k, shift = 64;
@@ -185,94 +184,141 @@ __device__ __noinline__ void radix_select(Shared<T>& s, const T* xr, int lo, int
   __syncthreads();
 }
 
+// Descending bitonic sort across the lanes of a warp.
+__device__ __forceinline__ uint32_t warp_sort_desc(uint32_t v) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int size = 2; size <= 32; size <<= 1) {
+#pragma unroll
+    for (int stride = size >> 1; stride > 0; stride >>= 1) {
+      const uint32_t w = __shfl_xor_sync(0xffffffffu, v, stride);
+      const bool larger = ((lane & stride) == 0) == ((lane & size) == 0);
+      v = larger ? max(v, w) : min(v, w);
+    }
+  }
+  return v;
+}
+
+// The 16-byte packs of one slice.
+struct Packs {
+  const uint4* body;
+  int nvec;
+};
+// Copies chunk `base` of the slice into the thread's own stage slots.
+__device__ __forceinline__ void issue(Shared& s, const Packs& src, int base) {
+#pragma unroll
+  for (int i = 0; i < kPacks; ++i) {
+    const int p = base + i * kBlock + threadIdx.x;
+    if (p < src.nvec) cp_async16(&s.stage[i][threadIdx.x], src.body + p);
+  }
+  cp_async_commit();
+}
+
 // Candidates of elements [lo, hi) of a row, which hold its k largest keys
-// (k <= hi - lo); returns their number, in every thread.
+// (k <= hi - lo); returns their number, in every thread, more than kCap when
+// they did not fit.  The slice's first chunk has been issued; the first chunk
+// of `next` is when this returns.
 //
 // The slice is read once, a chunk at a time, against a threshold below which
-// nothing can be among the k largest.  A first threshold is the k-th largest
-// maximum of the first chunk's packs: k packs, hence k elements, reach it.
-// After that a pack matters only if its maximum exceeds the threshold, which
-// few do: they go to a queue whose elements the whole CTA then tests.  An
-// element of a later chunk that only equals the threshold loses to the k
-// before it, so the test is strict there and ties resolve by index.
+// nothing can be among the k largest.  The first threshold comes from the
+// first chunk: each of its W warps sorts its threads' maxima, and the least
+// of the warps' ceil(k / W)-th is reached by k elements (a little over twice
+// k reach it when the row is in no order).  After that a pack matters only if
+// its maximum exceeds the threshold, which few do: they go to a queue whose
+// elements the whole CTA then tests.  An element of a later chunk that only
+// equals the threshold loses to the k before it, so the test is strict there
+// and ties resolve by index.
 template <typename T>
-__device__ __forceinline__ int collect(Shared<T>& s, const T* xr, int lo, int hi, int k, int& parity) {
+__device__ __forceinline__ int collect(Shared& s, const T* xr, int lo, int hi, int k, const Packs& next,
+                                       int& parity) {
   constexpr int VW = Elem<T>::kVec;
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid & 31;
   const RowSplit sp = split_row(xr + lo, hi - lo);
-  const uint4* body = reinterpret_cast<const uint4*>(xr + lo + sp.head);
-  if (tid == 0) s.filled = s.queued = 0;
+  const Packs src = {reinterpret_cast<const uint4*>(xr + lo + sp.head), sp.nvec};
+  if (tid == 0) s.filled = s.queued[0] = s.queued[1] = 0;
   __syncthreads();
   if (tid < sp.head) append(s, element_key(Elem<T>::to_f(xr[lo + tid]), (uint32_t)(lo + tid)));
-  uint32_t floor = 0;  // nothing at or below it matters any more (0: none yet)
-  for (int base = 0; base < sp.nvec; base += kBlock * kPacks) {
+  if (sp.nvec == 0) issue(s, next, 0);
+  uint32_t reached = 0;  // a key that k elements seen so far reach (0: none known)
+  int turn = 0;
+  bool fits = true;
+  for (int base = 0; base < sp.nvec; base += kBlock * kPacks, turn ^= 1) {
     uint4 u[kPacks];
     uint32_t top[kPacks];
+    cp_async_wait_all();
 #pragma unroll
     for (int i = 0; i < kPacks; ++i) {
       const int p = base + i * kBlock + tid;
-      u[i] = p < sp.nvec ? ld_stream(body + p) : make_uint4(0, 0, 0, 0);
+      u[i] = s.stage[i][tid];
+      top[i] = p < sp.nvec ? value_key(pack_top<T>(u[i])) : 0;
     }
-    int over = 0;
-#pragma unroll
-    for (int i = 0; i < kPacks; ++i) {
-      top[i] = base + i * kBlock + tid < sp.nvec ? value_key(pack_top<T>(u[i])) : 0;
-      over += top[i] > floor;
+    if (base + kBlock * kPacks < sp.nvec) {
+      issue(s, src, base + kBlock * kPacks);
+    } else {
+      issue(s, next, 0);
     }
-    int hits = block_sum(s, over, parity);
-    int n = s.filled;  // (appends follow the next barrier)
-    if (n > kCap) return n;
-    uint32_t least = floor + 1;  // elements of this chunk need at least this key
-    if (floor == 0xffffffffu) least = floor, hits = 0;
-    if (hits >= (floor == 0 ? k : 4 * k)) {
-      const uint32_t t = bisect<uint32_t>(s, k, k + k / 8, parity, [&](uint32_t c) {
-        int m = 0;
+    if (!fits || reached == 0xffffffffu) continue;  // (k NaN are kept)
+    uint32_t least = reached + 1;  // what an element of this chunk must reach to matter
+    const int warps = min(kWarps, (sp.nvec - base) / 32);  // with a pack in every thread
+    if (reached == 0 && warps * 32 >= k) {
+      uint32_t most = top[0];
 #pragma unroll
-        for (int i = 0; i < kPacks; ++i) m += top[i] >= c;
-        return m;
-      });
-      if (t > floor) {
-        floor = t;
-        least = t;
-        int m = 0;
+      for (int i = 1; i < kPacks; ++i) most = max(most, top[i]);
+      most = __shfl_sync(0xffffffffu, warp_sort_desc(most), (k + warps - 1) / warps - 1);
+      if (lane == 0) s.sums[parity][tid >> 5] = (int)most;
+      __syncthreads();
+      least = reached =
+          __reduce_min_sync(0xffffffffu, lane < warps ? (uint32_t)s.sums[parity][lane] : 0xffffffffu);
+      parity ^= 1;
+    }
+    const auto packs_over = [&](uint32_t c) {
+      int m = 0;
 #pragma unroll
-        for (int i = 0; i < kPacks; ++i) m += top[i] >= least;
-        hits = block_sum(s, m, parity);
+      for (int i = 0; i < kPacks; ++i) m += top[i] >= c;
+      return m;
+    };
+    int hits = block_sum(s, packs_over(least), parity);
+    const int n = s.filled;  // (appends follow the next barrier)
+    if (tid == 0) s.queued[turn ^ 1] = 0;
+    fits = n <= kCap;
+    if (!fits) continue;
+    if (n > kTighten || hits > max(4 * k, kQueue)) {
+      if (hits >= k) {  // rising rows: the k-th largest maximum of this chunk's packs
+        const uint32_t t = bisect<uint32_t>(s, 0u, ~0u, k, k + k / 8, parity, packs_over);
+        if (t > least) least = reached = t;
       }
-    }
-    if (n > kTighten) {
-      const uint32_t t = bisect<uint32_t>(s, k, k + k / 8, parity, [&](uint32_t c) {
-        int m = 0;
-        for (int j = tid; j < n; j += kBlock) m += (uint32_t)(s.cand[j] >> 32) >= c;
-        return m;
-      });
-      keep_above(s, n, (uint64_t)t << 32);
-      if (t > floor) {
-        floor = t;
-        least = t == 0xffffffffu ? t : t + 1;
+      if (n > kTighten) {  // the k-th largest of the candidates
+        const uint32_t t = bisect<uint32_t>(s, 0u, ~0u, k, k + k / 8, parity, [&](uint32_t c) {
+          int m = 0;
+          for (int j = tid; j < n; j += kBlock) m += (uint32_t)(s.cand[j] >> 32) >= c;
+          return m;
+        });
+        keep_above(s, n, (uint64_t)t << 32);
+        reached = max(reached, t);
+        if (t == 0xffffffffu) continue;
+        least = max(least, t + 1);
       }
+      hits = block_sum(s, packs_over(least), parity);
     }
-    __syncthreads();
     if (hits == 0) continue;
     if (hits <= kQueue) {
 #pragma unroll
       for (int i = 0; i < kPacks; ++i) {
         if (top[i] < least) continue;
-        const int slot = atomicAdd(&s.queued, 1);
+        const int slot = atomicAdd(&s.queued[turn], 1);
         s.q.pack[slot] = u[i];
         s.q.at[slot] = base + i * kBlock + tid;
       }
       __syncthreads();
-      const int queued = s.queued;
+      const int queued = s.queued[turn];
       const T* q = reinterpret_cast<const T*>(s.q.pack);
       for (int j = tid; j < queued * VW; j += kBlock) {
         const int e = lo + sp.head + s.q.at[j / VW] * VW + j % VW;
         const uint64_t key = element_key(Elem<T>::to_f(q[j]), (uint32_t)e);
         if ((uint32_t)(key >> 32) >= least) append(s, key);
       }
-      __syncthreads();
-      if (tid == 0) s.queued = 0;
     } else {
+      __syncthreads();
 #pragma unroll
       for (int i = 0; i < kPacks; ++i) {
         if (top[i] < least) continue;
@@ -292,82 +338,103 @@ __device__ __forceinline__ int collect(Shared<T>& s, const T* xr, int lo, int hi
     append(s, element_key(Elem<T>::to_f(xr[e]), (uint32_t)e));
   }
   __syncthreads();
-  return s.filled;
+  return fits ? s.filled : kCap + 1;
 }
 
-// One CTA a row, or a cluster with a slice of the row in each CTA when there
-// are few rows: every CTA finds its slice's candidates, CTA 0 takes them all
-// and orders the k largest.
+// One CTA a row, walking rows, or a cluster with a slice of the row in each
+// CTA when there are few: every CTA finds its slice's k largest, CTA 0 takes
+// them all and orders the k largest of the row.
 template <typename T>
 __global__ void __launch_bounds__(kBlock, 2)
-topk_kernel(const T* __restrict__ x, int64_t ld, int cols, int k, T* __restrict__ values,
+topk_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int cols, int k, T* __restrict__ values,
             int64_t* __restrict__ indices) {
-  __shared__ Shared<T> s;
+  extern __shared__ __align__(16) unsigned char smem[];
+  Shared& s = *reinterpret_cast<Shared*>(smem);
   pdl_prologue();
   const int C = (int)cluster_size(), rank = (int)cluster_rank();
-  const int64_t row = cluster_id();
-  const T* xr = x + row * ld;
   const int tid = threadIdx.x;
   int parity = 0;
   // slices of whole groups of 64 elements
   const int per = (int)(ceil_div(ceil_div(cols, C), 64) * 64);
   const int lo = min(cols, rank * per), hi = min(cols, lo + per);
   const int want = min(k, hi - lo);
-  int n = collect(s, xr, lo, hi, want, parity);
-  if (n > kCap) {
-    radix_select(s, xr, lo, hi, want);
-    n = want;
-  }
-  const auto shrink = [&](int most) {  // to the k largest, at most `most` of them
-    const uint64_t floor = bisect<uint64_t>(s, min(k, n), most, parity, [&](uint64_t c) {
-      int m = 0;
-      for (int j = tid; j < n; j += kBlock) m += s.cand[j] >= c;
-      return m;
-    });
-    keep_above(s, n, floor);
-    n = s.filled;
+  const auto packs_of = [&](int64_t row) {
+    if (row >= rows) return Packs{nullptr, 0};
+    const T* at = x + row * ld + lo;
+    const RowSplit sp = split_row(at, hi - lo);
+    return Packs{reinterpret_cast<const uint4*>(at + sp.head), sp.nvec};
   };
-  if (C > 1) {
-    if (n > k) shrink(k);
-    if (tid == 0) s.found = n;
-    cluster_sync_all();
-    if (rank == 0) {
-      for (int r = 1; r < C; ++r) {
-        int m;
-        asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(m) : "r"(remote_smem(&s.found, r)) : "memory");
-        const uint32_t from = remote_smem(s.cand, r);
-        for (int j = tid; j < m; j += kBlock) s.cand[n + j] = (uint64_t)ld_remote_s64(from + 8 * j);
-        n += m;
-      }
-      __syncthreads();
+  const int64_t step = cluster_count();
+  issue(s, packs_of(cluster_id()), 0);
+  for (int64_t row = cluster_id(); row < rows; row += step) {
+    const T* xr = x + row * ld;
+    int n = collect(s, xr, lo, hi, want, packs_of(row + step), parity);
+    if (n > kCap) {
+      radix_select(s, xr, lo, hi, want);
+      n = want;
     }
-    cluster_sync_all();
-    if (rank != 0) return;
-  }
-  const int most = max(k + k / 4, 128);
-  if (n > most) shrink(most);
-  const auto put = [&](int place, uint64_t key) {
-    const uint32_t at = ~(uint32_t)key;
-    indices[row * k + place] = at;
-    values[row * k + place] = xr[at];
-  };
-  if (n <= kBlock / 2) {
+    // to a few more than k at most, without their order
+    const auto shrink = [&](int most) {
+      const uint64_t f = bisect<uint64_t>(s, 0ull, ~0ull, min(k, n), most, parity, [&](uint64_t c) {
+        int m = 0;
+        for (int j = tid; j < n; j += kBlock) m += s.cand[j] >= c;
+        return m;
+      });
+      keep_above(s, n, f);
+      n = s.filled;
+    };
     // few keys: each one's place is the number of keys above it
-    int per_key = 32;
-    while (per_key * n > kBlock) per_key >>= 1;
-    const int i = tid / per_key;
-    const uint64_t key = i < n ? s.cand[i] : 0;
-    int place = 0;
-    for (int j = tid % per_key; j < n; j += per_key) place += s.cand[j] > key;
-    for (int o = per_key >> 1; o > 0; o >>= 1) place += __shfl_xor_sync(0xffffffffu, place, o);
-    if (i < n && tid % per_key == 0 && place < k) put(place, key);
-  } else {
-    int size = 1;
-    while (size < n) size <<= 1;
-    for (int i = tid; i < size; i += kBlock) s.sort[i] = i < n ? s.cand[i] : 0;
-    sort_desc(s, size);
-    for (int i = tid; i < k; i += kBlock) put(i, s.sort[i]);
+    const auto place_all = [&](auto put) {
+      int per_key = 32;
+      while (per_key * n > kBlock) per_key >>= 1;
+      const int i = tid / per_key;
+      const uint64_t key = i < n ? s.cand[i] : 0;
+      int place = 0;
+      for (int j = tid % per_key; j < n; j += per_key) place += s.cand[j] > key;
+      for (int o = per_key >> 1; o > 0; o >>= 1) place += __shfl_xor_sync(0xffffffffu, place, o);
+      if (i < n && tid % per_key == 0 && place < k) put(place, key);
+    };
+    const int most = max(k + k / 4, 128);
+    if (n > most) shrink(most);
+    if (C > 1) {
+      // this slice's k largest, 0 past the last
+      if (n <= kBlock / 2) {
+        for (int i = tid; i < k; i += kBlock) s.sort[i] = 0;
+        __syncthreads();
+        place_all([&](int place, uint64_t key) { s.sort[place] = key; });
+      } else {
+        if (n > k) shrink(k);
+        for (int i = tid; i < k; i += kBlock) s.sort[i] = i < n ? s.cand[i] : 0;
+      }
+      cluster_sync_all();
+      if (rank == 0) {
+        for (int i = tid; i < C * k; i += kBlock)
+          s.cand[i] = (uint64_t)ld_remote_s64(remote_smem(&s.sort[i % k], i / k));
+        n = C * k;
+        __syncthreads();
+      }
+      cluster_sync_all();  // the others' lists are read
+      if (rank == 0 && n > most) shrink(most);
+    }
+    if (rank == 0) {
+      const auto put = [&](int place, uint64_t key) {
+        const uint32_t at = ~(uint32_t)key;
+        indices[row * k + place] = at;
+        values[row * k + place] = xr[at];
+      };
+      if (n <= kBlock / 2) {
+        place_all(put);
+      } else {
+        int size = 1;
+        while (size < n) size <<= 1;
+        for (int i = tid; i < size; i += kBlock) s.sort[i] = i < n ? s.cand[i] : 0;
+        sort_desc(s, size);
+        for (int i = tid; i < k; i += kBlock) put(i, s.sort[i]);
+      }
+    }
+    __syncthreads();  // the next row's candidates take these ones' place
   }
+  cp_async_wait_all();
 }
 
 // Gradient: zeros, and dvalues at the indices (distinct in a row).
@@ -409,15 +476,20 @@ FL_B200_API int fl_b200_topk_lastdim(const void* x, int64_t ld, int64_t rows, in
   if (st != FL_B200_OK) return st;
   return dispatch_float(dtype, [&](auto t) {
     using T = decltype(t);
-    // few rows: up to 8 CTAs a row, of at least half a chunk each, whose
-    // candidates fit CTA 0
+    // few rows: up to 8 CTAs a row, with a pack a thread at least, whose
+    // lists fit CTA 0
     int cluster = 1;
     while (cluster < 8 && rows * cluster < dev.sm_count && cluster * 2 * k <= kCap &&
            cols / (cluster * 2) >= kBlock * Elem<T>::kVec)
       cluster *= 2;
-    return launch_cluster(topk_kernel<T>, rows * cluster, cluster, kBlock, 0, (cudaStream_t)stream,
-                          reinterpret_cast<const T*>(x), ld, (int)cols, (int)k,
-                          reinterpret_cast<T*>(values), indices);
+    // (per launch: the attribute is held per device)
+    if (cudaFuncSetAttribute(topk_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             (int)sizeof(Shared)) != cudaSuccess)
+      return launch_status();
+    const int64_t ctas = std::min<int64_t>(rows, 2 * dev.sm_count) * cluster;
+    return launch_cluster(topk_kernel<T>, cluster > 1 ? rows * cluster : ctas, cluster, kBlock,
+                          sizeof(Shared), (cudaStream_t)stream, reinterpret_cast<const T*>(x), ld,
+                          rows, (int)cols, (int)k, reinterpret_cast<T*>(values), indices);
   });
 }
 
