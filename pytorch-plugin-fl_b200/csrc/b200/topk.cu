@@ -12,11 +12,10 @@ namespace {
 constexpr int kMaxTop = FL_B200_TOPK_MAX;
 constexpr int kBlock = 512;
 constexpr int kWarps = kBlock / 32;
-constexpr int kPacks = 8;      // 16-byte packs a thread holds: a chunk of the row is kBlock * kPacks
-constexpr int kCap = 3072;     // candidates kept
-constexpr int kTighten = 1536; // above this many the threshold is raised over the candidates
-constexpr int kQueue = 512;    // packs of a chunk that hold candidates
-constexpr int kSort = 2048;    // keys sorted at the end: at most 1.25 * kMaxTop
+constexpr int kPacks = 8;    // 16-byte packs a thread has in flight
+constexpr int kChunk = kBlock * kPacks;  // packs after which the groups repeat
+constexpr int kCap = 3072;   // candidates kept
+constexpr int kSort = 2048;  // keys sorted at the end: at most 1.25 * kMaxTop
 
 // Monotone 32-bit image of a value: unsigned order is float order, NaN on
 // top; never 0.
@@ -25,50 +24,78 @@ __device__ __forceinline__ uint32_t value_key(float f) {
   if (f != f) return 0xffffffffu;
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
+// The value with that key (NaN for 0, which no value has).
+__device__ __forceinline__ float key_value(uint32_t key) {
+  return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+}
 __device__ __forceinline__ uint64_t element_key(float f, uint32_t index) {
   return ((uint64_t)value_key(f) << 32) | (uint32_t)~index;
 }
 
-// NaN-propagating maximum of a pack.
+// NaN-propagating maximum of the elements in two words, element by element
+// (two 16-bit elements a word), and of the elements of one word.
 template <typename T>
-__device__ __forceinline__ float pack_top(const uint4& u) {
-  float r;
+__device__ __forceinline__ uint32_t word_max(uint32_t a, uint32_t b) {
+  uint32_t r;
   if constexpr (std::is_same<T, float>::value) {
-    float a, b;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(a) : "f"(__uint_as_float(u.x)), "f"(__uint_as_float(u.y)));
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(b) : "f"(__uint_as_float(u.z)), "f"(__uint_as_float(u.w)));
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    asm("{ .reg .f32 x, y, z; mov.b32 x, %1; mov.b32 y, %2; max.NaN.f32 z, x, y; mov.b32 %0, z; }"
+        : "=r"(r)
+        : "r"(a), "r"(b));
+  } else if constexpr (std::is_same<T, __half>::value) {
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   } else {
-    uint32_t a, b, c;
-    if constexpr (std::is_same<T, __half>::value) {
-      asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(a) : "r"(u.x), "r"(u.y));
-      asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(b) : "r"(u.z), "r"(u.w));
-      asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(c) : "r"(a), "r"(b));
-    } else {
-      asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(a) : "r"(u.x), "r"(u.y));
-      asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(b) : "r"(u.z), "r"(u.w));
-      asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(c) : "r"(a), "r"(b));
-    }
-    const uint64_t p = pair_from_bits<T>(c);
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(f2_lo(p)), "f"(f2_hi(p)));
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   }
   return r;
 }
+template <typename T>
+__device__ __forceinline__ float word_top(uint32_t w) {
+  if constexpr (std::is_same<T, float>::value) {
+    return __uint_as_float(w);
+  } else {
+    const uint64_t p = pair_from_bits<T>(w);
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(f2_lo(p)), "f"(f2_hi(p)));
+    return r;
+  }
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack_max(const uint4& u) {
+  return word_max<T>(word_max<T>(u.x, u.y), word_max<T>(u.z, u.w));
+}
+// Word of -infinities.
+template <typename T>
+__device__ __forceinline__ uint32_t word_lowest() {
+  return std::is_same<T, float>::value ? 0xff800000u
+         : std::is_same<T, __half>::value ? 0xfc00fc00u
+                                          : 0xff80ff80u;
+}
 
 struct Shared {
-  uint64_t cand[kCap];       // candidates, in no order
+  uint64_t cand[kCap];  // candidates, in no order
   union {
-    struct {
-      uint4 pack[kQueue];
-      int at[kQueue];
-    } q;
     uint64_t sort[kSort];
+    int list[kChunk];   // groups of packs that hold candidates
   };
   int sums[2][kWarps];
+  uint32_t run[kBlock];  // the threads' maxima
   int hist[256];
-  int filled, queued[2], pick, above;
-  uint4 stage[kPacks][kBlock];  // the next chunk, each thread's own packs
+  uint32_t least;
+  int filled, listed, pick, above;
+  uint4 stage[kPacks][kBlock];  // packs on their way, each thread its own
 };
+
+// One more of `*counter`: the old value.  (Inline: these are rare, and what
+// the compiler does to share one atomic among a warp's lanes costs more than
+// it saves.)
+__device__ __forceinline__ int take_slot(int* counter) {
+  int slot;
+  asm volatile("atom.shared.add.s32 %0, [%1], 1;"
+               : "=r"(slot)
+               : "r"((uint32_t)__cvta_generic_to_shared(counter))
+               : "memory");
+  return slot;
+}
 
 // Sum of v over the CTA, in every thread.  `parity` alternates between the
 // two halves of the scratch, so that one barrier a call is enough.
@@ -104,7 +131,7 @@ __device__ __forceinline__ K bisect(Shared& s, K lo, K hi, int k, int enough, in
 }
 
 __device__ __forceinline__ void append(Shared& s, uint64_t key) {
-  const int slot = atomicAdd(&s.filled, 1);
+  const int slot = take_slot(&s.filled);
   if (slot < kCap) s.cand[slot] = key;
 }
 
@@ -143,23 +170,30 @@ __device__ __forceinline__ void sort_desc(Shared& s, int n) {
   __syncthreads();
 }
 
-// The k largest keys of elements [lo, hi) by radix selection: eight passes
-// at most, each a histogram of the next 8 bits of the keys that match the
-// prefix found so far, until exactly k keys reach it.  For slices whose
-// candidates overflow; right for any values.
+// The k largest keys of elements [lo, hi) in four passes (five in f16, six in
+// float32) that any values take: a histogram of the values' keys 8 bits at a time
+// down to the k-th largest value, the elements above it, and the first ones
+// equal to it in index order.  For slices whose candidates overflow: long
+// ties (a masked row, say) and rows that rise steeply.
 template <typename T>
-__device__ __noinline__ void radix_select(Shared& s, const T* xr, int lo, int hi, int k) {
-  const int tid = threadIdx.x;
-  uint64_t prefix = 0;
-  int need = k, shift = 64;
-  while (shift > 0) {
-    shift -= 8;
+__device__ __noinline__ void select_any(Shared& s, const T* xr, int lo, int hi, int k) {
+  // the upper bits that tell two values' keys apart: 16 of a bf16 value's, 19
+  // of an f16 value's (5 + 10 bits and the sign, with fp32's 8 bits of exponent)
+  constexpr int kBits = std::is_same<T, float>::value ? 32 : std::is_same<T, __half>::value ? 24 : 16;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int rounds = (hi - lo + kBlock - 1) / kBlock;
+  uint32_t value = 0;
+  int need = k;
+  for (int shift = kBits - 8; shift >= 0; shift -= 8) {
     for (int i = tid; i < 256; i += kBlock) s.hist[i] = 0;
     __syncthreads();
-    for (int i = lo + tid; i < hi; i += kBlock) {
-      const uint64_t key = element_key(Elem<T>::to_f(xr[i]), (uint32_t)i);
-      if (shift == 56 || (key >> (shift + 8)) == (prefix >> (shift + 8)))
-        atomicAdd(&s.hist[(key >> shift) & 255], 1);
+    for (int r = 0; r < rounds; ++r) {
+      const int i = lo + r * kBlock + tid;
+      const uint32_t key = i < hi ? value_key(Elem<T>::to_f(xr[i])) >> (32 - kBits) : 0;
+      const bool in = i < hi && (uint64_t)key >> (shift + 8) == (uint64_t)value >> (shift + 8);
+      const uint32_t digit = in ? (key >> shift) & 255 : 256;
+      const uint32_t same = __match_any_sync(0xffffffffu, digit);
+      if (in && __ffs(same) - 1 == lane) atomicAdd(&s.hist[digit], __popc(same));
     }
     __syncthreads();
     if (tid == 0) {
@@ -167,36 +201,64 @@ __device__ __noinline__ void radix_select(Shared& s, const T* xr, int lo, int hi
       while (d > 0 && sum + s.hist[d] < need) sum += s.hist[d--];
       s.pick = d;
       s.above = sum;
+      s.filled = 0;
     }
     __syncthreads();
-    prefix |= (uint64_t)s.pick << shift;
+    value |= (uint32_t)s.pick << shift;
     need -= s.above;
-    const bool done = s.hist[s.pick] == need;
-    __syncthreads();
-    if (done) break;
   }
-  if (tid == 0) s.filled = 0;
-  __syncthreads();
   for (int i = lo + tid; i < hi; i += kBlock) {
-    const uint64_t key = element_key(Elem<T>::to_f(xr[i]), (uint32_t)i);
-    if (key >= prefix) append(s, key);
+    const float f = Elem<T>::to_f(xr[i]);
+    if (value_key(f) >> (32 - kBits) > value) append(s, element_key(f, (uint32_t)i));
+  }
+  int parity = 0, taken = 0;
+  for (int r = 0; r < rounds && taken < need; ++r) {
+    const int i = lo + r * kBlock + tid;
+    const float f = i < hi ? Elem<T>::to_f(xr[i]) : 0.f;
+    const bool is = i < hi && value_key(f) >> (32 - kBits) == value;
+    const uint32_t vote = __ballot_sync(0xffffffffu, is);
+    if (lane == 0) s.sums[parity][tid >> 5] = __popc(vote);
+    __syncthreads();
+    int before = taken, total = 0;
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < tid >> 5) before += s.sums[parity][w];
+      total += s.sums[parity][w];
+    }
+    parity ^= 1;
+    if (is && before + __popc(vote & ((1u << lane) - 1)) < need) append(s, element_key(f, (uint32_t)i));
+    taken += total;
   }
   __syncthreads();
 }
 
-// Descending bitonic sort across the lanes of a warp.
-__device__ __forceinline__ uint32_t warp_sort_desc(uint32_t v) {
+// The k-th largest of the threads' maxima (or one that a few more reach), by
+// the lanes of one warp; 0 when there are fewer.
+__device__ __forceinline__ uint32_t kth_maximum(const Shared& s, int k) {
+  constexpr int kEach = kBlock / 32;
   const int lane = threadIdx.x & 31;
+  uint32_t v[kEach], lo = 0xffffffffu, hi = 0;
 #pragma unroll
-  for (int size = 2; size <= 32; size <<= 1) {
+  for (int i = 0; i < kEach; ++i) {
+    v[i] = s.run[i * 32 + lane];
+    lo = min(lo, v[i]);
+    hi = max(hi, v[i]);
+  }
+  lo = __reduce_min_sync(0xffffffffu, lo);
+  hi = __reduce_max_sync(0xffffffffu, hi);
+  const int top = 32 - __clz(lo ^ hi);  // below it the keys' bits differ
+  uint32_t at = top < 32 ? lo >> top << top : 0;
+  for (int bit = top; bit-- > 0;) {
+    const uint32_t tried = at | (1u << bit);
+    int n = 0;
 #pragma unroll
-    for (int stride = size >> 1; stride > 0; stride >>= 1) {
-      const uint32_t w = __shfl_xor_sync(0xffffffffu, v, stride);
-      const bool larger = ((lane & stride) == 0) == ((lane & size) == 0);
-      v = larger ? max(v, w) : min(v, w);
+    for (int i = 0; i < kEach; ++i) n += v[i] >= tried;
+    n = __reduce_add_sync(0xffffffffu, n);
+    if (n >= k) {
+      at = tried;
+      if (n <= k + k / 8) break;
     }
   }
-  return v;
+  return at;  // (0 among the keys: lo = 0, and `at` stays 0 unless k reach more)
 }
 
 // The 16-byte packs of one slice.
@@ -204,13 +266,13 @@ struct Packs {
   const uint4* body;
   int nvec;
 };
-// Copies chunk `base` of the slice into the thread's own stage slots.
-__device__ __forceinline__ void issue(Shared& s, const Packs& src, int base) {
+// Copies half `h` of the thread's packs of chunk `base` into its stage slots.
+__device__ __forceinline__ void issue(Shared& s, const Packs& src, int base, int h) {
+  const uint4* from = src.body + base + threadIdx.x;
+  const int left = src.nvec - base - (int)threadIdx.x;
 #pragma unroll
-  for (int i = 0; i < kPacks; ++i) {
-    const int p = base + i * kBlock + threadIdx.x;
-    if (p < src.nvec) cp_async16(&s.stage[i][threadIdx.x], src.body + p);
-  }
+  for (int i = h * kPacks / 2; i < (h + 1) * kPacks / 2; ++i)
+    if (i * kBlock < left) cp_async16(&s.stage[i][threadIdx.x], from + i * kBlock);
   cp_async_commit();
 }
 
@@ -219,126 +281,93 @@ __device__ __forceinline__ void issue(Shared& s, const Packs& src, int base) {
 // they did not fit.  The slice's first chunk has been issued; the first chunk
 // of `next` is when this returns.
 //
-// The slice is read once, a chunk at a time, against a threshold below which
-// nothing can be among the k largest.  The first threshold comes from the
-// first chunk: each of its W warps sorts its threads' maxima, and the least
-// of the warps' ceil(k / W)-th is reached by k elements (a little over twice
-// k reach it when the row is in no order).  After that a pack matters only if
-// its maximum exceeds the threshold, which few do: they go to a queue whose
-// elements the whole CTA then tests.  An element of a later chunk that only
-// equals the threshold loses to the k before it, so the test is strict there
-// and ties resolve by index.
+// The slice streams through once, each thread keeping one maximum for each of
+// its pack slots: 4096 groups of every 4096th pack.  k groups reach the k-th
+// largest of these maxima, so an element below it is not among the k largest,
+// and in a row without order little over k elements reach it.  Only the packs
+// of the groups that do, about k of 4096, are read again (from L2) for their
+// elements.  Elements equal to the threshold are kept, so ties are settled by
+// index at the end.  For k <= 256 the k-th largest of the threads' maxima
+// serves, which one warp finds: a little lower, and without a barrier a step.
 template <typename T>
 __device__ __forceinline__ int collect(Shared& s, const T* xr, int lo, int hi, int k, const Packs& next,
                                        int& parity) {
   constexpr int VW = Elem<T>::kVec;
-  const int tid = threadIdx.x, lane = tid & 31;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const RowSplit sp = split_row(xr + lo, hi - lo);
   const Packs src = {reinterpret_cast<const uint4*>(xr + lo + sp.head), sp.nvec};
-  if (tid == 0) s.filled = s.queued[0] = s.queued[1] = 0;
-  __syncthreads();
-  if (tid < sp.head) append(s, element_key(Elem<T>::to_f(xr[lo + tid]), (uint32_t)(lo + tid)));
-  if (sp.nvec == 0) issue(s, next, 0);
-  uint32_t reached = 0;  // a key that k elements seen so far reach (0: none known)
-  int turn = 0;
-  bool fits = true;
-  for (int base = 0; base < sp.nvec; base += kBlock * kPacks, turn ^= 1) {
-    uint4 u[kPacks];
-    uint32_t top[kPacks];
-    cp_async_wait_all();
+  if (tid == 0) s.filled = s.listed = 0;
+  uint32_t group[kPacks];
 #pragma unroll
-    for (int i = 0; i < kPacks; ++i) {
-      const int p = base + i * kBlock + tid;
-      u[i] = s.stage[i][tid];
-      top[i] = p < sp.nvec ? value_key(pack_top<T>(u[i])) : 0;
-    }
-    if (base + kBlock * kPacks < sp.nvec) {
-      issue(s, src, base + kBlock * kPacks);
-    } else {
-      issue(s, next, 0);
-    }
-    if (!fits || reached == 0xffffffffu) continue;  // (k NaN are kept)
-    uint32_t least = reached + 1;  // what an element of this chunk must reach to matter
-    const int warps = min(kWarps, (sp.nvec - base) / 32);  // with a pack in every thread
-    if (reached == 0 && warps * 32 >= k) {
-      uint32_t most = top[0];
+  for (int i = 0; i < kPacks; ++i) group[i] = word_lowest<T>();
+  for (int base = 0; base < max(sp.nvec, 1); base += kChunk) {
+    const int left = sp.nvec - base - tid;  // the thread's packs end here
+    const bool more = base + kChunk < sp.nvec;
 #pragma unroll
-      for (int i = 1; i < kPacks; ++i) most = max(most, top[i]);
-      most = __shfl_sync(0xffffffffu, warp_sort_desc(most), (k + warps - 1) / warps - 1);
-      if (lane == 0) s.sums[parity][tid >> 5] = (int)most;
-      __syncthreads();
-      least = reached =
-          __reduce_min_sync(0xffffffffu, lane < warps ? (uint32_t)s.sums[parity][lane] : 0xffffffffu);
-      parity ^= 1;
-    }
-    const auto packs_over = [&](uint32_t c) {
-      int m = 0;
+    for (int h = 0; h < 2; ++h) {
+      cp_async_wait_pending<1>();
 #pragma unroll
-      for (int i = 0; i < kPacks; ++i) m += top[i] >= c;
-      return m;
-    };
-    int hits = block_sum(s, packs_over(least), parity);
-    const int n = s.filled;  // (appends follow the next barrier)
-    if (tid == 0) s.queued[turn ^ 1] = 0;
-    fits = n <= kCap;
-    if (!fits) continue;
-    if (n > kTighten || hits > max(4 * k, kQueue)) {
-      if (hits >= k) {  // rising rows: the k-th largest maximum of this chunk's packs
-        const uint32_t t = bisect<uint32_t>(s, 0u, ~0u, k, k + k / 8, parity, packs_over);
-        if (t > least) least = reached = t;
+      for (int i = h * kPacks / 2; i < (h + 1) * kPacks / 2; ++i) {
+        const uint4 u = s.stage[i][tid];
+        if (i * kBlock < left) group[i] = word_max<T>(group[i], pack_max<T>(u));
       }
-      if (n > kTighten) {  // the k-th largest of the candidates
-        const uint32_t t = bisect<uint32_t>(s, 0u, ~0u, k, k + k / 8, parity, [&](uint32_t c) {
-          int m = 0;
-          for (int j = tid; j < n; j += kBlock) m += (uint32_t)(s.cand[j] >> 32) >= c;
-          return m;
-        });
-        keep_above(s, n, (uint64_t)t << 32);
-        reached = max(reached, t);
-        if (t == 0xffffffffu) continue;
-        least = max(least, t + 1);
-      }
-      hits = block_sum(s, packs_over(least), parity);
-    }
-    if (hits == 0) continue;
-    if (hits <= kQueue) {
-#pragma unroll
-      for (int i = 0; i < kPacks; ++i) {
-        if (top[i] < least) continue;
-        const int slot = atomicAdd(&s.queued[turn], 1);
-        s.q.pack[slot] = u[i];
-        s.q.at[slot] = base + i * kBlock + tid;
-      }
-      __syncthreads();
-      const int queued = s.queued[turn];
-      const T* q = reinterpret_cast<const T*>(s.q.pack);
-      for (int j = tid; j < queued * VW; j += kBlock) {
-        const int e = lo + sp.head + s.q.at[j / VW] * VW + j % VW;
-        const uint64_t key = element_key(Elem<T>::to_f(q[j]), (uint32_t)e);
-        if ((uint32_t)(key >> 32) >= least) append(s, key);
-      }
-    } else {
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < kPacks; ++i) {
-        if (top[i] < least) continue;
-        float f[VW];
-        unpack<T>(u[i], f);
-#pragma unroll
-        for (int j = 0; j < VW; ++j) {
-          const int e = lo + sp.head + (base + i * kBlock + tid) * VW + j;
-          if (value_key(f[j]) >= least) append(s, element_key(f[j], (uint32_t)e));
-        }
+      if (more) {
+        issue(s, src, base + kChunk, h);
+      } else {
+        issue(s, next, 0, h);
       }
     }
   }
-  __syncthreads();
+  uint32_t most = 0;
+#pragma unroll
+  for (int i = 0; i < kPacks; ++i) {
+    group[i] = i * kBlock + tid < sp.nvec ? value_key(word_top<T>(group[i])) : 0;
+    most = max(most, group[i]);
+  }
+  uint32_t least;
+  if (k <= kBlock / 2) {
+    s.run[tid] = most;
+    __syncthreads();
+    if (warp == 0) {
+      const uint32_t v = kth_maximum(s, k);
+      if (lane == 0) s.least = v;
+    }
+    __syncthreads();
+    least = s.least;
+  } else {
+    __syncthreads();
+    least = bisect<uint32_t>(s, 0u, ~0u, k, k + k / 8, parity, [&](uint32_t c) {
+      int m = 0;
+#pragma unroll
+      for (int i = 0; i < kPacks; ++i) m += group[i] >= c;
+      return m;
+    });
+  }
+  if (tid < sp.head) append(s, element_key(Elem<T>::to_f(xr[lo + tid]), (uint32_t)(lo + tid)));
   if (tid < sp.tail) {
     const int e = hi - sp.tail + tid;
     append(s, element_key(Elem<T>::to_f(xr[e]), (uint32_t)e));
   }
+#pragma unroll
+  for (int i = 0; i < kPacks; ++i)
+    if (group[i] >= max(least, 1u)) s.list[take_slot(&s.listed)] = i * kBlock + tid;
   __syncthreads();
-  return fits ? s.filled : kCap + 1;
+  const int depth = (sp.nvec + kChunk - 1) / kChunk;  // packs of a group
+  const int items = s.listed * depth;
+  const float bar = key_value(least);  // (NaN while everything passes, or only NaN does)
+  for (int j = tid; j < items; j += kBlock) {
+    const int p = s.list[j / depth] + j % depth * kChunk;
+    if (p >= sp.nvec) continue;
+    const uint4 u = ld_cached(src.body + p);
+    if (word_top<T>(pack_max<T>(u)) < bar) continue;
+    float f[VW];
+    unpack<T>(u, f);
+#pragma unroll
+    for (int i = 0; i < VW; ++i)
+      if (value_key(f[i]) >= least) append(s, element_key(f[i], (uint32_t)(lo + sp.head + p * VW + i)));
+  }
+  __syncthreads();
+  return s.filled;
 }
 
 // One CTA a row, walking rows, or a cluster with a slice of the row in each
@@ -364,13 +393,15 @@ topk_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int cols, int k, 
     const RowSplit sp = split_row(at, hi - lo);
     return Packs{reinterpret_cast<const uint4*>(at + sp.head), sp.nvec};
   };
+  const int most = max(k + k / 4, 128);  // keys to order at the end
   const int64_t step = cluster_count();
-  issue(s, packs_of(cluster_id()), 0);
+  issue(s, packs_of(cluster_id()), 0, 0);
+  issue(s, packs_of(cluster_id()), 0, 1);
   for (int64_t row = cluster_id(); row < rows; row += step) {
     const T* xr = x + row * ld;
     int n = collect(s, xr, lo, hi, want, packs_of(row + step), parity);
     if (n > kCap) {
-      radix_select(s, xr, lo, hi, want);
+      select_any(s, xr, lo, hi, want);
       n = want;
     }
     // to a few more than k at most, without their order
@@ -390,11 +421,12 @@ topk_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int cols, int k, 
       const int i = tid / per_key;
       const uint64_t key = i < n ? s.cand[i] : 0;
       int place = 0;
-      for (int j = tid % per_key; j < n; j += per_key) place += s.cand[j] > key;
+      if (i < n)
+        for (int j = tid % per_key; j < n; j += per_key) place += s.cand[j] > key;
+      __syncwarp();
       for (int o = per_key >> 1; o > 0; o >>= 1) place += __shfl_xor_sync(0xffffffffu, place, o);
       if (i < n && tid % per_key == 0 && place < k) put(place, key);
     };
-    const int most = max(k + k / 4, 128);
     if (n > most) shrink(most);
     if (C > 1) {
       // this slice's k largest, 0 past the last
