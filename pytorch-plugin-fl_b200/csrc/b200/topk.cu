@@ -10,12 +10,9 @@ namespace flb200 {
 namespace {
 
 constexpr int kMaxTop = FL_B200_TOPK_MAX;
-constexpr int kBlock = 512;
-constexpr int kWarps = kBlock / 32;
-constexpr int kPacks = 8;    // 16-byte packs a thread has in flight
-constexpr int kChunk = kBlock * kPacks;  // packs after which the groups repeat
-constexpr int kCap = 3072;   // candidates kept
-constexpr int kSort = 2048;  // keys sorted at the end: at most 1.25 * kMaxTop
+constexpr int kPacks = 8;     // 16-byte packs a thread has in flight
+constexpr int kCap = 2048;    // candidates kept
+constexpr int kShared = 512;  // the longest list that clusters exchange
 
 // Monotone 32-bit image of a value: unsigned order is float order, NaN on
 // top; never 0.
@@ -71,18 +68,22 @@ __device__ __forceinline__ uint32_t word_lowest() {
                                           : 0xff80ff80u;
 }
 
+// B threads a CTA.
+template <int B>
 struct Shared {
+  static constexpr int kWarps = B / 32;
+  static constexpr int kChunk = B * kPacks;  // packs after which the groups repeat
   uint64_t cand[kCap];  // candidates, in no order
   union {
-    uint64_t sort[kSort];
-    int list[kChunk];   // groups of packs that hold candidates
+    uint64_t top[kShared];  // this slice's largest, for CTA 0
+    uint16_t list[kChunk];  // groups of packs that hold candidates
   };
   int sums[2][kWarps];
-  uint32_t run[kBlock];  // the threads' maxima
+  uint32_t run[B];  // the threads' maxima
   int hist[256];
   uint32_t least;
   int filled, listed, pick, above;
-  uint4 stage[kPacks][kBlock];  // packs on their way, each thread its own
+  uint4 stage[kPacks][B];  // packs on their way, each thread its own
 };
 
 // One more of `*counter`: the old value.  (Inline: these are rare, and what
@@ -99,7 +100,9 @@ __device__ __forceinline__ int take_slot(int* counter) {
 
 // Sum of v over the CTA, in every thread.  `parity` alternates between the
 // two halves of the scratch, so that one barrier a call is enough.
-__device__ __forceinline__ int block_sum(Shared& s, int v, int& parity) {
+template <int B>
+__device__ __forceinline__ int block_sum(Shared<B>& s, int v, int& parity) {
+  constexpr int kWarps = B / 32;
   const int lane = threadIdx.x & 31;
   v = __reduce_add_sync(0xffffffffu, v);
   if (lane == 0) s.sums[parity][threadIdx.x >> 5] = v;
@@ -113,8 +116,8 @@ __device__ __forceinline__ int block_sum(Shared& s, int v, int& parity) {
 // where that is possible: found bit by bit below the bits that `lo` and `hi`
 // share, all counted keys lying between these two.  count(K) is the thread's
 // own number of keys >= K.
-template <typename K, typename F>
-__device__ __forceinline__ K bisect(Shared& s, K lo, K hi, int k, int enough, int& parity, F count) {
+template <typename K, int B, typename F>
+__device__ __forceinline__ K bisect(Shared<B>& s, K lo, K hi, int k, int enough, int& parity, F count) {
   K at = lo;
   int bit = (int)sizeof(K) * 8 - 1;
   while (bit >= 0 && (((lo ^ hi) >> bit) & 1) == 0) --bit;
@@ -130,39 +133,42 @@ __device__ __forceinline__ K bisect(Shared& s, K lo, K hi, int k, int enough, in
   return at;
 }
 
-__device__ __forceinline__ void append(Shared& s, uint64_t key) {
+template <int B>
+__device__ __forceinline__ void append(Shared<B>& s, uint64_t key) {
   const int slot = take_slot(&s.filled);
   if (slot < kCap) s.cand[slot] = key;
 }
 
 // Keeps the candidates at or above a 64-bit key.
-__device__ __forceinline__ void keep_above(Shared& s, int n, uint64_t floor) {
-  uint64_t mine[kCap / kBlock];
+template <int B>
+__device__ __forceinline__ void keep_above(Shared<B>& s, int n, uint64_t floor) {
+  uint64_t mine[kCap / B];
 #pragma unroll
-  for (int i = 0; i < kCap / kBlock; ++i) {
-    const int j = threadIdx.x + i * kBlock;
+  for (int i = 0; i < kCap / B; ++i) {
+    const int j = threadIdx.x + i * B;
     mine[i] = j < n ? s.cand[j] : 0;
   }
   __syncthreads();
   if (threadIdx.x == 0) s.filled = 0;
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kCap / kBlock; ++i)
+  for (int i = 0; i < kCap / B; ++i)
     if (mine[i] >= floor && mine[i] != 0) append(s, mine[i]);
   __syncthreads();
 }
 
-// Descending bitonic sort of s.sort[0..n), n a power of two.
-__device__ __forceinline__ void sort_desc(Shared& s, int n) {
+// Descending bitonic sort of the first n candidates, n a power of two.
+template <int B>
+__device__ __forceinline__ void sort_desc(Shared<B>& s, int n) {
   for (int size = 2; size <= n; size <<= 1) {
     for (int stride = size >> 1; stride > 0; stride >>= 1) {
       __syncthreads();
-      for (int i = threadIdx.x; i < n / 2; i += kBlock) {
+      for (int i = threadIdx.x; i < n / 2; i += B) {
         const int lo = 2 * i - (i & (stride - 1));
-        const uint64_t a = s.sort[lo], b = s.sort[lo + stride];
+        const uint64_t a = s.cand[lo], b = s.cand[lo + stride];
         if ((a < b) == ((lo & size) == 0)) {
-          s.sort[lo] = b;
-          s.sort[lo + stride] = a;
+          s.cand[lo] = b;
+          s.cand[lo + stride] = a;
         }
       }
     }
@@ -175,20 +181,20 @@ __device__ __forceinline__ void sort_desc(Shared& s, int n) {
 // down to the k-th largest value, the elements above it, and the first ones
 // equal to it in index order.  For slices whose candidates overflow: long
 // ties (a masked row, say) and rows that rise steeply.
-template <typename T>
-__device__ __noinline__ void select_any(Shared& s, const T* xr, int lo, int hi, int k) {
+template <typename T, int B>
+__device__ __noinline__ void select_any(Shared<B>& s, const T* xr, int lo, int hi, int k) {
   // the upper bits that tell two values' keys apart: 16 of a bf16 value's, 19
   // of an f16 value's (5 + 10 bits and the sign, with fp32's 8 bits of exponent)
   constexpr int kBits = std::is_same<T, float>::value ? 32 : std::is_same<T, __half>::value ? 24 : 16;
   const int tid = threadIdx.x, lane = tid & 31;
-  const int rounds = (hi - lo + kBlock - 1) / kBlock;
+  const int rounds = (hi - lo + B - 1) / B;
   uint32_t value = 0;
   int need = k;
   for (int shift = kBits - 8; shift >= 0; shift -= 8) {
-    for (int i = tid; i < 256; i += kBlock) s.hist[i] = 0;
+    for (int i = tid; i < 256; i += B) s.hist[i] = 0;
     __syncthreads();
     for (int r = 0; r < rounds; ++r) {
-      const int i = lo + r * kBlock + tid;
+      const int i = lo + r * B + tid;
       const uint32_t key = i < hi ? value_key(Elem<T>::to_f(xr[i])) >> (32 - kBits) : 0;
       const bool in = i < hi && (uint64_t)key >> (shift + 8) == (uint64_t)value >> (shift + 8);
       const uint32_t digit = in ? (key >> shift) & 255 : 256;
@@ -207,20 +213,20 @@ __device__ __noinline__ void select_any(Shared& s, const T* xr, int lo, int hi, 
     value |= (uint32_t)s.pick << shift;
     need -= s.above;
   }
-  for (int i = lo + tid; i < hi; i += kBlock) {
+  for (int i = lo + tid; i < hi; i += B) {
     const float f = Elem<T>::to_f(xr[i]);
     if (value_key(f) >> (32 - kBits) > value) append(s, element_key(f, (uint32_t)i));
   }
   int parity = 0, taken = 0;
   for (int r = 0; r < rounds && taken < need; ++r) {
-    const int i = lo + r * kBlock + tid;
+    const int i = lo + r * B + tid;
     const float f = i < hi ? Elem<T>::to_f(xr[i]) : 0.f;
     const bool is = i < hi && value_key(f) >> (32 - kBits) == value;
     const uint32_t vote = __ballot_sync(0xffffffffu, is);
     if (lane == 0) s.sums[parity][tid >> 5] = __popc(vote);
     __syncthreads();
     int before = taken, total = 0;
-    for (int w = 0; w < kWarps; ++w) {
+    for (int w = 0; w < B / 32; ++w) {
       if (w < tid >> 5) before += s.sums[parity][w];
       total += s.sums[parity][w];
     }
@@ -233,8 +239,9 @@ __device__ __noinline__ void select_any(Shared& s, const T* xr, int lo, int hi, 
 
 // The k-th largest of the threads' maxima (or one that a few more reach), by
 // the lanes of one warp; 0 when there are fewer.
-__device__ __forceinline__ uint32_t kth_maximum(const Shared& s, int k) {
-  constexpr int kEach = kBlock / 32;
+template <int B>
+__device__ __forceinline__ uint32_t kth_maximum(const Shared<B>& s, int k) {
+  constexpr int kEach = B / 32;
   const int lane = threadIdx.x & 31;
   uint32_t v[kEach], lo = 0xffffffffu, hi = 0;
 #pragma unroll
@@ -267,12 +274,13 @@ struct Packs {
   int nvec;
 };
 // Copies half `h` of the thread's packs of chunk `base` into its stage slots.
-__device__ __forceinline__ void issue(Shared& s, const Packs& src, int base, int h) {
+template <int B>
+__device__ __forceinline__ void issue(Shared<B>& s, const Packs& src, int base, int h) {
   const uint4* from = src.body + base + threadIdx.x;
   const int left = src.nvec - base - (int)threadIdx.x;
 #pragma unroll
   for (int i = h * kPacks / 2; i < (h + 1) * kPacks / 2; ++i)
-    if (i * kBlock < left) cp_async16(&s.stage[i][threadIdx.x], from + i * kBlock);
+    if (i * B < left) cp_async16(&s.stage[i][threadIdx.x], from + i * B);
   cp_async_commit();
 }
 
@@ -282,16 +290,17 @@ __device__ __forceinline__ void issue(Shared& s, const Packs& src, int base, int
 // of `next` is when this returns.
 //
 // The slice streams through once, each thread keeping one maximum for each of
-// its pack slots: 4096 groups of every 4096th pack.  k groups reach the k-th
+// its pack slots: groups of every kChunk-th pack.  k groups reach the k-th
 // largest of these maxima, so an element below it is not among the k largest,
 // and in a row without order little over k elements reach it.  Only the packs
-// of the groups that do, about k of 4096, are read again (from L2) for their
+// of the groups that do, about k of kChunk, are read again (from L2) for their
 // elements.  Elements equal to the threshold are kept, so ties are settled by
-// index at the end.  For k <= 256 the k-th largest of the threads' maxima
+// index at the end.  For k <= B / 2 the k-th largest of the threads' maxima
 // serves, which one warp finds: a little lower, and without a barrier a step.
-template <typename T>
-__device__ __forceinline__ int collect(Shared& s, const T* xr, int lo, int hi, int k, const Packs& next,
-                                       int& parity) {
+template <typename T, int B>
+__device__ __forceinline__ int collect(Shared<B>& s, const T* xr, int lo, int hi, int k,
+                                       const Packs& next, int& parity) {
+  constexpr int kChunk = Shared<B>::kChunk;
   constexpr int VW = Elem<T>::kVec;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const RowSplit sp = split_row(xr + lo, hi - lo);
@@ -309,7 +318,7 @@ __device__ __forceinline__ int collect(Shared& s, const T* xr, int lo, int hi, i
 #pragma unroll
       for (int i = h * kPacks / 2; i < (h + 1) * kPacks / 2; ++i) {
         const uint4 u = s.stage[i][tid];
-        if (i * kBlock < left) group[i] = word_max<T>(group[i], pack_max<T>(u));
+        if (i * B < left) group[i] = word_max<T>(group[i], pack_max<T>(u));
       }
       if (more) {
         issue(s, src, base + kChunk, h);
@@ -321,11 +330,11 @@ __device__ __forceinline__ int collect(Shared& s, const T* xr, int lo, int hi, i
   uint32_t most = 0;
 #pragma unroll
   for (int i = 0; i < kPacks; ++i) {
-    group[i] = i * kBlock + tid < sp.nvec ? value_key(word_top<T>(group[i])) : 0;
+    group[i] = i * B + tid < sp.nvec ? value_key(word_top<T>(group[i])) : 0;
     most = max(most, group[i]);
   }
   uint32_t least;
-  if (k <= kBlock / 2) {
+  if (k <= B / 2) {
     s.run[tid] = most;
     __syncthreads();
     if (warp == 0) {
@@ -350,12 +359,12 @@ __device__ __forceinline__ int collect(Shared& s, const T* xr, int lo, int hi, i
   }
 #pragma unroll
   for (int i = 0; i < kPacks; ++i)
-    if (group[i] >= max(least, 1u)) s.list[take_slot(&s.listed)] = i * kBlock + tid;
+    if (group[i] >= max(least, 1u)) s.list[take_slot(&s.listed)] = (uint16_t)(i * B + tid);
   __syncthreads();
   const int depth = (sp.nvec + kChunk - 1) / kChunk;  // packs of a group
   const int items = s.listed * depth;
   const float bar = key_value(least);  // (NaN while everything passes, or only NaN does)
-  for (int j = tid; j < items; j += kBlock) {
+  for (int j = tid; j < items; j += B) {
     const int p = s.list[j / depth] + j % depth * kChunk;
     if (p >= sp.nvec) continue;
     const uint4 u = ld_cached(src.body + p);
@@ -373,12 +382,12 @@ __device__ __forceinline__ int collect(Shared& s, const T* xr, int lo, int hi, i
 // One CTA a row, walking rows, or a cluster with a slice of the row in each
 // CTA when there are few: every CTA finds its slice's k largest, CTA 0 takes
 // them all and orders the k largest of the row.
-template <typename T>
-__global__ void __launch_bounds__(kBlock, 2)
+template <typename T, int B>
+__global__ void __launch_bounds__(B, 1024 / B)
 topk_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int cols, int k, T* __restrict__ values,
             int64_t* __restrict__ indices) {
   extern __shared__ __align__(16) unsigned char smem[];
-  Shared& s = *reinterpret_cast<Shared*>(smem);
+  Shared<B>& s = *reinterpret_cast<Shared<B>*>(smem);
   pdl_prologue();
   const int C = (int)cluster_size(), rank = (int)cluster_rank();
   const int tid = threadIdx.x;
@@ -408,7 +417,7 @@ topk_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int cols, int k, 
     const auto shrink = [&](int most) {
       const uint64_t f = bisect<uint64_t>(s, 0ull, ~0ull, min(k, n), most, parity, [&](uint64_t c) {
         int m = 0;
-        for (int j = tid; j < n; j += kBlock) m += s.cand[j] >= c;
+        for (int j = tid; j < n; j += B) m += s.cand[j] >= c;
         return m;
       });
       keep_above(s, n, f);
@@ -417,7 +426,7 @@ topk_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int cols, int k, 
     // few keys: each one's place is the number of keys above it
     const auto place_all = [&](auto put) {
       int per_key = 32;
-      while (per_key * n > kBlock) per_key >>= 1;
+      while (per_key * n > B) per_key >>= 1;
       const int i = tid / per_key;
       const uint64_t key = i < n ? s.cand[i] : 0;
       int place = 0;
@@ -430,18 +439,18 @@ topk_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int cols, int k, 
     if (n > most) shrink(most);
     if (C > 1) {
       // this slice's k largest, 0 past the last
-      if (n <= kBlock / 2) {
-        for (int i = tid; i < k; i += kBlock) s.sort[i] = 0;
+      if (n <= B / 2) {
+        for (int i = tid; i < k; i += B) s.top[i] = 0;
         __syncthreads();
-        place_all([&](int place, uint64_t key) { s.sort[place] = key; });
+        place_all([&](int place, uint64_t key) { s.top[place] = key; });
       } else {
         if (n > k) shrink(k);
-        for (int i = tid; i < k; i += kBlock) s.sort[i] = i < n ? s.cand[i] : 0;
+        for (int i = tid; i < k; i += B) s.top[i] = i < n ? s.cand[i] : 0;
       }
       cluster_sync_all();
       if (rank == 0) {
-        for (int i = tid; i < C * k; i += kBlock)
-          s.cand[i] = (uint64_t)ld_remote_s64(remote_smem(&s.sort[i % k], i / k));
+        for (int i = tid; i < C * k; i += B)
+          s.cand[i] = (uint64_t)ld_remote_s64(remote_smem(&s.top[i % k], i / k));
         n = C * k;
         __syncthreads();
       }
@@ -454,20 +463,22 @@ topk_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int cols, int k, 
         indices[row * k + place] = at;
         values[row * k + place] = xr[at];
       };
-      if (n <= kBlock / 2) {
+      if (n <= B / 2) {
         place_all(put);
       } else {
         int size = 1;
         while (size < n) size <<= 1;
-        for (int i = tid; i < size; i += kBlock) s.sort[i] = i < n ? s.cand[i] : 0;
+        for (int i = n + tid; i < size; i += B) s.cand[i] = 0;
         sort_desc(s, size);
-        for (int i = tid; i < k; i += kBlock) put(i, s.sort[i]);
+        for (int i = tid; i < k; i += B) put(i, s.cand[i]);
       }
     }
     __syncthreads();  // the next row's candidates take these ones' place
   }
   cp_async_wait_all();
 }
+
+constexpr int kBlock = 512;
 
 // Gradient: zeros, and dvalues at the indices (distinct in a row).
 template <typename T>
@@ -508,20 +519,29 @@ FL_B200_API int fl_b200_topk_lastdim(const void* x, int64_t ld, int64_t rows, in
   if (st != FL_B200_OK) return st;
   return dispatch_float(dtype, [&](auto t) {
     using T = decltype(t);
-    // few rows: up to 8 CTAs a row, with a pack a thread at least, whose
-    // lists fit CTA 0
-    int cluster = 1;
-    while (cluster < 8 && rows * cluster < dev.sm_count && cluster * 2 * k <= kCap &&
-           cols / (cluster * 2) >= kBlock * Elem<T>::kVec)
-      cluster *= 2;
-    // (per launch: the attribute is held per device)
-    if (cudaFuncSetAttribute(topk_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             (int)sizeof(Shared)) != cudaSuccess)
-      return launch_status();
-    const int64_t ctas = std::min<int64_t>(rows, 2 * dev.sm_count) * cluster;
-    return launch_cluster(topk_kernel<T>, cluster > 1 ? rows * cluster : ctas, cluster, kBlock,
-                          sizeof(Shared), (cudaStream_t)stream, reinterpret_cast<const T*>(x), ld,
-                          rows, (int)cols, (int)k, reinterpret_cast<T*>(values), indices);
+    const auto go = [&](auto block) {
+      constexpr int B = decltype(block)::value;
+      // few rows: up to 8 CTAs a row, with two packs a thread at least, whose
+      // lists fit CTA 0
+      int cluster = 1;
+      while (cluster < 8 && rows * cluster < dev.sm_count && cluster * 2 * k <= kCap && k <= kShared &&
+             cols / (cluster * 2) >= 2 * B * Elem<T>::kVec)
+        cluster *= 2;
+      // (per launch: the attribute is held per device)
+      const auto kern = topk_kernel<T, B>;
+      if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               (int)sizeof(Shared<B>)) != cudaSuccess)
+        return launch_status();
+      const int64_t ctas = std::min<int64_t>(rows, 1024 / B * dev.sm_count);
+      return launch_cluster(kern, cluster > 1 ? rows * cluster : ctas, cluster, B, sizeof(Shared<B>),
+                            (cudaStream_t)stream, reinterpret_cast<const T*>(x), ld, rows, (int)cols,
+                            (int)k, reinterpret_cast<T*>(values), indices);
+    };
+    // 512 threads a row stream fastest (4096 rows of 128256 bf16: 184 us, 203 us
+    // with 256); with no more rows than CTAs of 256 threads fit, those end
+    // sooner (333 rows of 40003 float32: 18.6 us, 20.4 us with 512)
+    return rows > 4 * dev.sm_count ? go(std::integral_constant<int, 512>{})
+                                   : go(std::integral_constant<int, 256>{});
   });
 }
 
