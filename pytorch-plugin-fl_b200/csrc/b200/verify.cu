@@ -48,33 +48,108 @@ struct VerifyArgs {
   int64_t* accepted;
 };
 
-// What the row's weights are made of once the drafts are judged.
-template <typename T>
-struct Row {
-  const T* p;
-  const T* q;    // null: no subtraction
-  int without;   // an index whose weight is 0, or -1
-  __device__ long long weight(int i) const {
-    const long long w = fixed(Elem<T>::to_f(p[i]));
-    if (q != nullptr) return max(w - fixed(Elem<T>::to_f(q[i])), 0LL);
-    return i == without ? 0 : w;
-  }
-};
-
 __device__ __forceinline__ long long warp_sum64(long long v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
 
-// One CTA a sequence.  Warp w sums the w-th slice of the row; the warp whose
-// slice holds the mark walks it again in index order.
+// The row that the next token is drawn from: weights p, p - q where that is
+// positive, or p without one token.
 template <typename T>
-__global__ void __launch_bounds__(kBlock) verify_kernel(VerifyArgs<T> a) {
+struct Row {
+  const T* p;
+  const T* q;   // null: nothing subtracted
+  int without;  // an index whose weight is 0, or -1
+
+  __device__ __forceinline__ static long long excess(T p, T q) {
+    const long long d = fixed(Elem<T>::to_f(p)) - fixed(Elem<T>::to_f(q));
+    return d > 0 ? d : 0;
+  }
+  __device__ __forceinline__ long long weight(int i) const {
+    if (q != nullptr) return excess(p[i], q[i]);
+    return i == without ? 0 : fixed(Elem<T>::to_f(p[i]));
+  }
+
+  // This lane's part of the weights of packs [from, to) of the row's split,
+  // of which q's are packs too when `packed`.
+  __device__ __forceinline__ long long sum(const RowSplit& sp, int from, int to, bool packed) const {
+    constexpr int VW = Elem<T>::kVec;
+    constexpr int U = 4;
+    const int lane = threadIdx.x & 31;
+    long long s = 0;
+    const uint4* pv = reinterpret_cast<const uint4*>(p + sp.head);
+    const auto add = [&](const uint4& a) {
+      float f[VW];
+      unpack<T>(a, f);
+#pragma unroll
+      for (int j = 0; j < VW; ++j) s += fixed(f[j]);
+    };
+    const auto add2 = [&](const uint4& a, const uint4& b) {
+      float f[VW], g[VW];
+      unpack<T>(a, f);
+      unpack<T>(b, g);
+#pragma unroll
+      for (int j = 0; j < VW; ++j) {
+        const long long d = fixed(f[j]) - fixed(g[j]);
+        s += d > 0 ? d : 0;
+      }
+    };
+    if (q == nullptr) {
+      for (int i = from + lane; i < to; i += 32 * U) {
+        uint4 a[U];
+#pragma unroll
+        for (int k = 0; k < U; ++k)
+          a[k] = i + 32 * k < to ? ld_cached(pv + i + 32 * k) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int k = 0; k < U; ++k) add(a[k]);
+      }
+      const int x = without - sp.head;  // (a single element's owner leaves it out itself)
+      if (lane == 0 && x >= from * VW && x < to * VW) s -= fixed(Elem<T>::to_f(p[without]));
+    } else if (packed) {
+      const uint4* qv = reinterpret_cast<const uint4*>(q + sp.head);
+      for (int i = from + lane; i < to; i += 32 * U) {
+        uint4 a[U], b[U];
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+          const bool in = i + 32 * k < to;
+          a[k] = in ? ld_cached(pv + i + 32 * k) : make_uint4(0, 0, 0, 0);
+          b[k] = in ? ld_cached(qv + i + 32 * k) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int k = 0; k < U; ++k) add2(a[k], b[k]);
+      }
+    } else {
+      const int end = sp.head + to * VW;
+      for (int e = sp.head + from * VW + lane; e < end; e += 32 * 2 * U) {
+        T a[2 * U], b[2 * U];
+#pragma unroll
+        for (int k = 0; k < 2 * U; ++k) {
+          const bool in = e + 32 * k < end;
+          a[k] = in ? p[e + 32 * k] : Elem<T>::from_f(0.f);
+          b[k] = in ? q[e + 32 * k] : Elem<T>::from_f(0.f);
+        }
+#pragma unroll
+        for (int k = 0; k < 2 * U; ++k) s += excess(a[k], b[k]);
+      }
+    }
+    return s;
+  }
+};
+
+// A cluster of CTAs a sequence.  Every CTA judges the drafts for itself; the
+// row is cut into one segment a warp, in index order, and each warp sums its
+// own; the CTAs' totals meet through distributed shared memory, and the warp
+// whose segment holds the mark walks it again, 16 elements a lane at a time.
+template <typename T>
+__global__ void __launch_bounds__(kBlock, 2) verify_kernel(VerifyArgs<T> a) {
+  constexpr int VW = Elem<T>::kVec;
   __shared__ long long part[kWarps];
+  __shared__ long long mine[2];  // this CTA's total, of either attempt
   __shared__ int kept;
   pdl_prologue();
-  const int64_t b = blockIdx.x;
+  const int C = (int)cluster_size(), rank = (int)cluster_rank();
+  const int64_t b = cluster_id();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t* ids = a.ids + b * a.ld_ids;
   const float* u = a.u + b * a.ld_u;
@@ -111,49 +186,84 @@ __global__ void __launch_bounds__(kBlock) verify_kernel(VerifyArgs<T> a) {
     const int64_t x = ids[count];
     r.without = x >= 0 && x < a.vocab ? (int)x : -1;
   }
-  const int per = (a.vocab + kWarps - 1) / kWarps;
-  const int from = min(a.vocab, warp * per), to = min(a.vocab, from + per);
-  long long total = 0;
-  for (int pass = 0; pass < 2; ++pass) {
-    long long s = 0;
-    for (int i = from + lane; i < to; i += 32) s += r.weight(i);
-    s = warp_sum64(s);
+  const RowSplit sp = split_row(r.p, a.vocab);
+  const bool packed = ((reinterpret_cast<uintptr_t>(r.p) ^ reinterpret_cast<uintptr_t>(r.q)) & 15u) == 0;
+  const int segments = C * kWarps, seg = rank * kWarps + warp;
+  const int per = (sp.nvec + segments - 1) / segments;
+  const int from = min(sp.nvec, seg * per), to = min(sp.nvec, from + per);
+  const int first = seg == 0 ? 0 : sp.head + from * VW;
+  const int last = seg == segments - 1 ? a.vocab : sp.head + to * VW;
+  long long before = 0, total = 0, own = 0;
+  for (int attempt = 0; attempt < 2; ++attempt) {
+    long long s = r.sum(sp, from, to, packed);
+    // the row's single elements belong to its first and last segment
+    if (seg == 0 && lane < sp.head) s += r.weight(lane);
+    if (seg == segments - 1 && lane < sp.tail) s += r.weight(a.vocab - sp.tail + lane);
+    own = warp_sum64(s);
+    if (lane == 0) part[warp] = own;
     __syncthreads();
-    if (lane == 0) part[warp] = s;
-    __syncthreads();
+    before = 0;
     total = 0;
-    for (int w = 0; w < kWarps; ++w) total += part[w];
+    for (int w = 0; w < kWarps; ++w) {
+      if (w == warp) before = total;
+      total += part[w];
+    }
+    if (C > 1) {
+      if (tid == 0) mine[attempt] = total;
+      cluster_sync_all();
+      const long long v = lane < C ? ld_remote_s64(remote_smem(&mine[attempt], lane)) : 0;
+      before += warp_sum64(lane < rank ? v : 0);
+      total = warp_sum64(v);
+    }
     if (total > 0 || !cut) break;
     r.q = nullptr;  // nothing left of the residual
     r.without = -1;
+    __syncthreads();
   }
-  for (int i = tid; i <= a.drafts; i += kBlock) {
-    if (i < count) a.tokens[b * (a.drafts + 1) + i] = ids[i];
-    if (i > count || (i == count && total == 0)) a.tokens[b * (a.drafts + 1) + i] = -1;
+  if (C > 1) cluster_sync_all();  // the totals are read: no CTA leaves before
+  if (rank == 0) {
+    for (int i = tid; i <= a.drafts; i += kBlock) {
+      if (i < count) a.tokens[b * (a.drafts + 1) + i] = ids[i];
+      if (i > count || (i == count && total == 0)) a.tokens[b * (a.drafts + 1) + i] = -1;
+    }
+    if (tid == 0) a.accepted[b] = count;
   }
-  if (tid == 0) a.accepted[b] = count;
   if (total == 0) return;
   const float us = __saturatef(u[a.drafts]);
   const unsigned long long t = min((unsigned long long)(us * 16777216.0f), 16777215ull);
   const unsigned long long hi = __umul64hi(t, (unsigned long long)total);
-  const long long mark = (long long)((hi << 40) | ((t * (unsigned long long)total) >> 24));
-  long long before = 0;
-  for (int w = 0; w < warp; ++w) before += part[w];
-  if (mark < before || mark >= before + part[warp]) return;
-  for (int i = from; i < to; i += 32) {
-    const long long w = i + lane < to ? r.weight(i + lane) : 0;
-    long long sum = w;
+  const long long mark = (long long)((hi << 40) | ((t * (unsigned long long)total) >> 24)) - before;
+  if (mark < 0 || mark >= own) return;
+  constexpr int E = 16;
+  long long passed = 0;
+  for (int i = first + lane * E; i - lane * E < last; i += 32 * E) {
+    long long w[E], sum = 0;
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      w[j] = i + j < last ? r.weight(i + j) : 0;
+      sum += w[j];
+    }
+    long long upto = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long v = __shfl_up_sync(0xffffffffu, sum, o);
-      if (lane >= o) sum += v;
+      const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
     }
-    const uint32_t over = __ballot_sync(0xffffffffu, before + sum > mark);
-    if (over != 0) {
-      if (lane == 0) a.tokens[b * (a.drafts + 1) + count] = i + __ffs(over) - 1;
+    const long long round = __shfl_sync(0xffffffffu, upto, 31);
+    if (passed + round > mark) {
+      long long c = passed + upto - sum;
+      if (c <= mark && mark < c + sum) {
+        int at = 0;
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+          c += w[j];
+          at += c <= mark;
+        }
+        a.tokens[b * (a.drafts + 1) + count] = i + at;
+      }
       return;
     }
-    before += __shfl_sync(0xffffffffu, sum, 31);
+    passed += round;
   }
 }
 
@@ -177,13 +287,21 @@ FL_B200_API int fl_b200_verify_draft(const int64_t* draft_ids, int64_t ld_ids, c
   FLB_CHECK_ARG(vocab > 0 && p && uniform && tokens && accepted && (drafts == 0 || draft_ids));
   FLB_CHECK_ARG(ld_ids >= 0 && p_stride_b >= 0 && p_stride_i >= 0 && q_stride_b >= 0 &&
                 q_stride_i >= 0 && ld_u >= 0);
+  DeviceInfo dev;
+  const int st = current_device_info(&dev);
+  if (st != FL_B200_OK) return st;
   return dispatch_float(dtype, [&](auto t) {
     using T = decltype(t);
     VerifyArgs<T> a = {draft_ids, ld_ids, reinterpret_cast<const T*>(p), p_stride_b, p_stride_i,
                        reinterpret_cast<const T*>(q), q_stride_b, q_stride_i, uniform, ld_u, lens,
                        (int)drafts, (int)vocab, tokens, accepted};
-    launch_k(verify_kernel<T>, dim3((unsigned)batch), dim3(kBlock), 0, (cudaStream_t)stream, a);
-    return launch_status();
+    // up to 8 CTAs a sequence, a pack a thread at least, until every SM has two
+    int cluster = 1;
+    while (cluster < 8 && batch * cluster < 2 * dev.sm_count &&
+           vocab / (cluster * 2) >= kBlock * Elem<T>::kVec)
+      cluster *= 2;
+    if (batch * cluster > 0x7fffffffLL) return (int)FL_B200_ERR_TOO_LARGE;
+    return launch_cluster(verify_kernel<T>, batch * cluster, cluster, kBlock, 0, (cudaStream_t)stream, a);
   });
 }
 
