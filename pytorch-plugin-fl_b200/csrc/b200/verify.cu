@@ -25,7 +25,7 @@
 namespace flb200 {
 namespace {
 
-constexpr int kBlock = 512;
+constexpr int kBlock = 256;
 constexpr int kWarps = kBlock / 32;
 
 __device__ __forceinline__ long long fixed(float p) {
@@ -142,7 +142,7 @@ struct Row {
 // own; the CTAs' totals meet through distributed shared memory, and the warp
 // whose segment holds the mark walks it again, 16 elements a lane at a time.
 template <typename T>
-__global__ void __launch_bounds__(kBlock, 2) verify_kernel(VerifyArgs<T> a) {
+__global__ void __launch_bounds__(kBlock, 4) verify_kernel(VerifyArgs<T> a) {
   constexpr int VW = Elem<T>::kVec;
   __shared__ long long part[kWarps];
   __shared__ long long mine[2];  // this CTA's total, of either attempt
@@ -295,9 +295,9 @@ FL_B200_API int fl_b200_verify_draft(const int64_t* draft_ids, int64_t ld_ids, c
     VerifyArgs<T> a = {draft_ids, ld_ids, reinterpret_cast<const T*>(p), p_stride_b, p_stride_i,
                        reinterpret_cast<const T*>(q), q_stride_b, q_stride_i, uniform, ld_u, lens,
                        (int)drafts, (int)vocab, tokens, accepted};
-    // up to 8 CTAs a sequence, a pack a thread at least, until every SM has two
+    // up to 8 CTAs a sequence, a pack a thread at least, until every SM has eight
     int cluster = 1;
-    while (cluster < 8 && batch * cluster < 2 * dev.sm_count &&
+    while (cluster < 8 && batch * cluster < 8 * dev.sm_count &&
            vocab / (cluster * 2) >= kBlock * Elem<T>::kVec)
       cluster *= 2;
     if (batch * cluster > 0x7fffffffLL) return (int)FL_B200_ERR_TOO_LARGE;
