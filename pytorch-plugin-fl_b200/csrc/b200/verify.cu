@@ -139,8 +139,8 @@ struct Row {
 
 // A cluster of CTAs a sequence.  Every CTA judges the drafts for itself; the
 // row is cut into one segment a warp, in index order, and each warp sums its
-// own; the CTAs' totals meet through distributed shared memory, and the warp
-// whose segment holds the mark walks it again, 16 elements a lane at a time.
+// own; the CTAs' totals meet through distributed shared memory, and the CTA
+// that has the mark walks the one segment that holds it again.
 template <typename T>
 __global__ void __launch_bounds__(kBlock, 4) verify_kernel(VerifyArgs<T> a) {
   constexpr int VW = Elem<T>::kVec;
@@ -154,20 +154,25 @@ __global__ void __launch_bounds__(kBlock, 4) verify_kernel(VerifyArgs<T> a) {
   const int64_t* ids = a.ids + b * a.ld_ids;
   const float* u = a.u + b * a.ld_u;
   int n = a.drafts;
-  if (a.lens != nullptr) n = (int)min((int64_t)a.drafts, max((int64_t)0, a.lens[b]));
+  const int64_t len = a.lens != nullptr ? a.lens[b] : n;
   if (warp == 0) {
     int at = 0;
-    for (; at < n; at += 32) {
+    // (the loads of a draft do not wait for the length: two trips to memory,
+    // not three)
+    for (; at < a.drafts; at += 32) {
       const int i = at + lane;
-      bool ok = i >= n;
-      if (!ok) {
+      bool ok = true;
+      if (i < a.drafts) {
         const int64_t x = ids[i];
+        const float ui = u[i];
+        ok = false;
         if (x >= 0 && x < a.vocab) {
           const float pt = __saturatef(Elem<T>::to_f(a.p[b * a.spb + i * a.sps + x]));
           const float qt =
               a.q != nullptr ? __saturatef(Elem<T>::to_f(a.q[b * a.sqb + i * a.sqs + x])) : 1.f;
-          ok = (double)fmaxf(u[i], 0.f) * (double)qt < (double)pt;
+          ok = (double)fmaxf(ui, 0.f) * (double)qt < (double)pt;
         }
+        ok = ok || i >= len;
       }
       const uint32_t no = __ballot_sync(0xffffffffu, !ok);
       if (no != 0) {
@@ -175,8 +180,10 @@ __global__ void __launch_bounds__(kBlock, 4) verify_kernel(VerifyArgs<T> a) {
         break;
       }
     }
+    n = (int)min((int64_t)n, max((int64_t)0, len));
     if (lane == 0) kept = min(at, n);
   }
+  n = (int)min((int64_t)a.drafts, max((int64_t)0, len));
   __syncthreads();
   const int count = kept;
   const bool cut = count < n;
@@ -191,28 +198,23 @@ __global__ void __launch_bounds__(kBlock, 4) verify_kernel(VerifyArgs<T> a) {
   const int segments = C * kWarps, seg = rank * kWarps + warp;
   const int per = (sp.nvec + segments - 1) / segments;
   const int from = min(sp.nvec, seg * per), to = min(sp.nvec, from + per);
-  const int first = seg == 0 ? 0 : sp.head + from * VW;
-  const int last = seg == segments - 1 ? a.vocab : sp.head + to * VW;
-  long long before = 0, total = 0, own = 0;
+  long long before = 0, total = 0;  // weights ahead of this CTA's, of the row
   for (int attempt = 0; attempt < 2; ++attempt) {
     long long s = r.sum(sp, from, to, packed);
     // the row's single elements belong to its first and last segment
     if (seg == 0 && lane < sp.head) s += r.weight(lane);
     if (seg == segments - 1 && lane < sp.tail) s += r.weight(a.vocab - sp.tail + lane);
-    own = warp_sum64(s);
-    if (lane == 0) part[warp] = own;
+    s = warp_sum64(s);
+    if (lane == 0) part[warp] = s;
     __syncthreads();
-    before = 0;
-    total = 0;
-    for (int w = 0; w < kWarps; ++w) {
-      if (w == warp) before = total;
-      total += part[w];
-    }
+    before = total = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) total += part[w];
     if (C > 1) {
       if (tid == 0) mine[attempt] = total;
       cluster_sync_all();
       const long long v = lane < C ? ld_remote_s64(remote_smem(&mine[attempt], lane)) : 0;
-      before += warp_sum64(lane < rank ? v : 0);
+      before = warp_sum64(lane < rank ? v : 0);
       total = warp_sum64(v);
     }
     if (total > 0 || !cut) break;
@@ -232,38 +234,52 @@ __global__ void __launch_bounds__(kBlock, 4) verify_kernel(VerifyArgs<T> a) {
   const float us = __saturatef(u[a.drafts]);
   const unsigned long long t = min((unsigned long long)(us * 16777216.0f), 16777215ull);
   const unsigned long long hi = __umul64hi(t, (unsigned long long)total);
-  const long long mark = (long long)((hi << 40) | ((t * (unsigned long long)total) >> 24)) - before;
-  if (mark < 0 || mark >= own) return;
-  constexpr int E = 16;
-  long long passed = 0;
-  for (int i = first + lane * E; i - lane * E < last; i += 32 * E) {
-    long long w[E], sum = 0;
+  long long mark = (long long)((hi << 40) | ((t * (unsigned long long)total) >> 24)) - before;
+  // the warp whose segment holds the mark, if it is one of this CTA's
+  int w = 0;
+  while (w < kWarps && mark >= part[w]) mark -= part[w++];
+  if (mark < 0 || w == kWarps) return;
+  const int at = rank * kWarps + w;
+  const int first = at == 0 ? 0 : sp.head + min(sp.nvec, at * per) * VW;
+  const int last = at == segments - 1 ? a.vocab : sp.head + min(sp.nvec, (at + 1) * per) * VW;
+  // the CTA walks that segment again, E elements a thread
+  constexpr int E = 8;
+  for (int base = first; base < last; base += kBlock * E) {
+    const int i = base + tid * E;
+    long long v[E], sum = 0;
 #pragma unroll
     for (int j = 0; j < E; ++j) {
-      w[j] = i + j < last ? r.weight(i + j) : 0;
-      sum += w[j];
+      v[j] = i + j < last ? r.weight(i + j) : 0;
+      sum += v[j];
     }
     long long upto = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long v = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += v;
+      const long long x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += x;
     }
-    const long long round = __shfl_sync(0xffffffffu, upto, 31);
-    if (passed + round > mark) {
-      long long c = passed + upto - sum;
+    __syncthreads();  // part has been read
+    if (lane == 31) part[warp] = upto;
+    __syncthreads();
+    long long c = upto - sum, round = 0;
+#pragma unroll
+    for (int x = 0; x < kWarps; ++x) {
+      if (x < warp) c += part[x];
+      round += part[x];
+    }
+    if (mark < round) {
       if (c <= mark && mark < c + sum) {
-        int at = 0;
+        int more = 0;
 #pragma unroll
         for (int j = 0; j < E; ++j) {
-          c += w[j];
-          at += c <= mark;
+          c += v[j];
+          more += c <= mark;
         }
-        a.tokens[b * (a.drafts + 1) + count] = i + at;
+        a.tokens[b * (a.drafts + 1) + count] = i + more;
       }
       return;
     }
-    passed += round;
+    mark -= round;
   }
 }
 
