@@ -89,6 +89,62 @@ __device__ __forceinline__ long long ld_remote_s64(uint32_t addr) {
   return v;
 }
 
+// ---- transaction barriers in shared memory: a CTA's exchange slots ---------
+__device__ __forceinline__ void bar_init(uint64_t* bar, int count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"((uint32_t)__cvta_generic_to_shared(bar)),
+               "r"(count)
+               : "memory");
+}
+// Makes initialised barriers visible to the cluster (followed by a cluster
+// barrier).
+__device__ __forceinline__ void bar_init_fence() {
+  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+}
+// One arrival that announces `bytes` to come in this phase.
+__device__ __forceinline__ void bar_expect(uint64_t* bar, int bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(
+                   (uint32_t)__cvta_generic_to_shared(bar)),
+               "r"(bytes)
+               : "memory");
+}
+// Stores (a, b) to `slot` of a CTA of the cluster and counts its 8 bytes on
+// that CTA's barrier (both addresses from remote_smem).
+__device__ __forceinline__ void send_f2(uint32_t slot, float a, float b, uint32_t bar) {
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];" ::"r"(
+                   slot),
+               "f"(a), "f"(b), "r"(bar)
+               : "memory");
+}
+// Waits for the phase of this parity, a bounded number of tries (seconds;
+// a wait takes microseconds).  When they run out, *lost is set, after which
+// no wait of the CTA tries again; the caller reports what it computed then
+// as NaN.
+__device__ __forceinline__ void bar_wait(uint64_t* bar, uint32_t parity, volatile int* lost) {
+  const uint32_t addr = (uint32_t)__cvta_generic_to_shared(bar);
+  for (int tries = 0;; ++tries) {
+    uint32_t done;
+    asm volatile(
+        "{ .reg .pred p; mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2; "
+        "selp.u32 %0, 1, 0, p; }"
+        : "=r"(done)
+        : "r"(addr), "r"(parity)
+        : "memory");
+    if (done) return;
+    if (tries > (1 << 20) || *lost) {
+      *lost = 1;
+      return;
+    }
+  }
+}
+// Named barriers: all `threads` threads meet (sync), or are counted without
+// waiting (arrive).
+__device__ __forceinline__ void named_sync(int id, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+__device__ __forceinline__ void named_arrive(int id, int threads) {
+  asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
 // Element i of an array whose type is known at run time.
 __device__ __forceinline__ float load_float(const void* p, int dtype, int64_t i) {
   if (dtype == FL_B200_F32) return reinterpret_cast<const float*>(p)[i];
