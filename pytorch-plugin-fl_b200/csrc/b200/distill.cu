@@ -324,20 +324,23 @@ distill_bwd_kernel(const float* __restrict__ dloss, int64_t dloss_stride, const 
 // ---------------------------------------------- loss and gradient at once ---
 //
 // One read of the logits and one write of the gradient: a cluster holds a row
-// on chip, 32 elements a thread, as exponentials 2^((z - m_w) c) against the
-// warp's own maximum.  Every warp sends its (m_w, sum) to every CTA of the
-// cluster (st.async on a transaction barrier: no fence, no second hop through
-// a CTA total); each warp then folds all pairs to (M, S) and stores
-// w tau e 2^((m_w - M) c) / S.  While a row is exchanged and stored, the next
-// ones travel to shared memory through a ring of cp.async copies, each thread
-// its own.  A further warp reads the teacher's lists one row ahead, writes the
-// tokens of its CTA's slice again once the row is stored, and in CTA 0 the
-// loss.
+// on chip, 128 bytes of logits a thread, as exponentials 2^((z - m_w) c)
+// against the warp's own maximum.  Every warp sends its (m_w, sum) to every
+// CTA of the cluster (st.async on a transaction barrier: no fence, no second
+// hop through a CTA total); each warp then folds all pairs to (M, S) and
+// writes w tau e 2^((m_w - M) c) / S over the logits in shared memory.  Three
+// stages of a row's slice take turns: one arriving, one in hand, one leaving,
+// each by one bulk copy, so that neither memory direction holds up the warps
+// (stores from registers did: a third of a row's time was theirs).
+//
+// Two further warps: one reads the teacher's lists a row ahead, puts the
+// gradients of the tokens they name in place, and in CTA 0 writes the loss;
+// the other issues the copies.
 constexpr int kGradList = 256;       // teacher entries a row that this kernel takes
-constexpr int kHold = 32;            // elements a thread holds
-constexpr int kQuads = 3;            // ring slots of four packs
+constexpr int kPacks = 8;            // 16-byte packs a thread holds
+constexpr int kStages = 3;
 constexpr int kMaxCluster = 16;
-constexpr int kMarkBits = 32768;     // marks of the tokens named so far, by id modulo this
+constexpr int kMarkBits = 16384;     // marks of the tokens named so far, by id modulo this
 
 struct GradList {
   int id[kGradList];      // -1: absent
@@ -348,97 +351,125 @@ struct GradList {
 
 template <int NT>
 struct GradShared {
-  uint4 ring[kQuads][4][NT];
+  uint4 stage[kStages][kPacks][NT];
   float2 pair[2][kMaxCluster * (NT / 32)];
   GradList list[2];
   uint32_t marks[kMarkBits / 32];
   float2 stat[2];   // (M, S) of the row, for the list's warp
   float by[2];      // w tau
   float total[2];   // of the list's 2^t2; 0: nothing taught
-  uint64_t bar[2];
+  uint64_t bar[2];          // the row's pairs have come
+  uint64_t full[kStages];   // the stage's logits have come
   int lost;
 };
 
-// Reads a row's list; one warp.
-template <typename T, int NT>
-__device__ __forceinline__ void read_list(GradShared<NT>& s, int par, const Taught& a, const T* x,
-                                          int64_t row, int cols, int lo, int hi, float by) {
-  constexpr int U = 4;  // entries a lane whose loads are in flight together
-  GradList& l = s.list[par];
-  const int lane = threadIdx.x & 31;
-  float top = -INFINITY;
-  for (int j0 = lane; j0 < a.k; j0 += 32 * U) {
-    int64_t id[U];
-    float t[U], z[U];
+constexpr int kHelpers = 64;  // threads besides the NT that hold the row
+// Named barriers, two of each for alternate rows, one of the last a stage: a
+// barrier's next use follows, through the others, every wait on this one.
+constexpr int kListed = 1;  // the list is known: the holders wait for its warp
+constexpr int kHeld = 3;    // the gradient is in place: the list's warp waits for the holders
+constexpr int kReady = 5;   // and the list's tokens: the copies' warp waits for the list's
+
+// A row's list on its way, kGradList / 32 entries a lane.
+struct ListAhead {
+  static constexpr int kEach = kGradList / 32;
+  int id[kEach];    // -1: absent
+  float t[kEach];
+  float w;
+
+  __device__ __forceinline__ void load(const Taught& a, const float* weight, int64_t weight_stride,
+                                       int64_t row, int cols) {
+    const int lane = threadIdx.x & 31;
+    w = weight != nullptr ? weight[row * weight_stride] : 1.f;
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int j = j0 + 32 * i;
-      id[i] = j < a.k ? load_index(a.ids, a.ids_dtype, row * a.ld_ids + j) : -1;
+    for (int i = 0; i < kEach; ++i) {
+      const int j = lane + 32 * i;
+      if (32 * i >= a.k) break;
+      const int64_t v = j < a.k ? load_index(a.ids, a.ids_dtype, row * a.ld_ids + j) : -1;
+      id[i] = v >= 0 && v < cols ? (int)v : -1;
       t[i] = j < a.k ? load_float(a.t, a.t_dtype, row * a.ld_t + j) : 0.f;
     }
+  }
+};
+
+// Sets up list `par` from the entries of row x that have arrived; one warp.
+// Logits are read for the entries in [lo, hi).
+template <typename T, int NT>
+__device__ __forceinline__ void set_list(GradShared<NT>& s, int par, const Taught& a, const ListAhead& in,
+                                         const T* x, int lo, int hi) {
+  GradList& l = s.list[par];
+  const int lane = threadIdx.x & 31;
+  float z[ListAhead::kEach], e[ListAhead::kEach];
+  float top = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < U; ++i) z[i] = id[i] >= lo && id[i] < hi ? Elem<T>::to_f(x[id[i]]) : 0.f;
-#pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int j = j0 + 32 * i;
-      if (j >= a.k) break;
-      const bool in = id[i] >= 0 && id[i] < cols;
-      l.id[j] = in ? (int)id[i] : -1;
-      l.t2[j] = in ? t[i] : -INFINITY;
-      l.z[j] = z[i];
-      top = MaxOp::combine(top, l.t2[j]);
-    }
+  for (int i = 0; i < ListAhead::kEach; ++i) {
+    if (32 * i >= a.k) break;
+    z[i] = in.id[i] >= lo && in.id[i] < hi ? Elem<T>::to_f(x[in.id[i]]) : 0.f;
+    e[i] = in.id[i] >= 0 ? in.t[i] : -INFINITY;
+    top = MaxOp::combine(top, e[i]);
   }
   top = group_reduce_warp<MaxOp, 32>(top);
   float total = 0.f;
   if (top != -INFINITY) {
-    for (int j = lane; j < a.k; j += 32) {
-      l.t2[j] = (l.t2[j] - top) * a.c;
-      if (l.id[j] >= 0) total += exp2f(l.t2[j]);
+#pragma unroll
+    for (int i = 0; i < ListAhead::kEach; ++i) {
+      if (32 * i >= a.k) break;
+      const float t2 = (e[i] - top) * a.c;
+      if (lane + 32 * i < a.k) l.t2[lane + 32 * i] = t2;
+      e[i] = in.id[i] >= 0 ? exp2f(t2) : 0.f;
+      total += e[i];
     }
   }
   total = warp_sum(total);
-  // masses: an id whose mark was set already may be a repeated one
+  if (lane == 0) {
+    s.total[par] = total;
+    s.by[par] = in.w * a.tau;
+  }
   __syncwarp();
-  for (int j0 = 0; j0 < a.k; j0 += 32) {
-    const int j = j0 + lane;
-    const int id = j < a.k ? l.id[j] : -1;
+  named_arrive(kListed + par, NT + 32);  // the row may be written
+  // masses: an id whose mark was set already may be a repeated one
+  const float inverse = 1.f / total;
+#pragma unroll
+  for (int i = 0; i < ListAhead::kEach; ++i) {
+    if (32 * i >= a.k) break;
+    const int j = lane + 32 * i, id = in.id[i];
     bool again = false;
+    if (j < a.k) {
+      l.id[j] = id;
+      l.z[j] = z[i];
+      l.mass[j] = id >= 0 ? e[i] * inverse : -1.f;
+    }
     if (id >= 0) {
       const uint32_t h = (uint32_t)id % kMarkBits;
       again = (atomicOr(&s.marks[h / 32], 1u << (h % 32)) >> (h % 32)) & 1;
-      l.mass[j] = exp2f(l.t2[j]) / total;
-    } else if (j < a.k) {
-      l.mass[j] = -1.f;
     }
     __syncwarp();
     uint32_t votes = __ballot_sync(0xffffffffu, again);
     while (votes != 0) {
       // the warp goes over the list so far for one such id: its first entry
       // takes the sum of all
-      const int same = l.id[j0 + __ffs(votes) - 1];
+      const int same = l.id[32 * i + __ffs(votes) - 1];
       votes &= votes - 1;
-      const int end = min(a.k, j0 + 32);
+      const int end = min(a.k, 32 * i + 32);
       int first = end;
       float mass = 0.f;
-      for (int i = lane; i < end; i += 32) {
-        if (l.id[i] != same) continue;
-        first = min(first, i);
-        if (l.mass[i] != -1.f) mass += l.mass[i];
+      for (int n = lane; n < end; n += 32) {
+        if (l.id[n] != same) continue;
+        first = min(first, n);
+        if (l.mass[n] != -1.f) mass += l.mass[n];
       }
       __syncwarp();
       first = __reduce_min_sync(0xffffffffu, first);
       mass = warp_sum(mass);
-      for (int i = lane; i < end; i += 32)
-        if (l.id[i] == same) l.mass[i] = i == first ? mass : -1.f;
+      for (int n = lane; n < end; n += 32)
+        if (l.id[n] == same) l.mass[n] = n == first ? mass : -1.f;
       __syncwarp();
     }
   }
-  for (int j = lane; j < a.k; j += 32)
-    if (l.id[j] >= 0) s.marks[(uint32_t)l.id[j] % kMarkBits / 32] = 0;
-  if (lane == 0) {
-    s.total[par] = total;
-    s.by[par] = by;
+#pragma unroll
+  for (int i = 0; i < ListAhead::kEach; ++i) {
+    if (32 * i >= a.k) break;
+    if (in.id[i] >= 0) s.marks[(uint32_t)in.id[i] % kMarkBits / 32] = 0;
   }
   __syncwarp();
 }
@@ -450,54 +481,111 @@ __device__ __forceinline__ float warp_max(float v) {
   return r;
 }
 
+// Maximum of a pack's elements (NaN ignored unless all are).
+template <typename T>
+__device__ __forceinline__ float pack_max(const uint4& u) {
+  if constexpr (std::is_same<T, float>::value) {
+    return fmaxf(fmax3(__uint_as_float(u.x), __uint_as_float(u.y), __uint_as_float(u.z)),
+                 __uint_as_float(u.w));
+  } else {
+    uint32_t a, b, c;
+    if constexpr (std::is_same<T, __half>::value) {
+      asm("max.f16x2 %0, %1, %2;" : "=r"(a) : "r"(u.x), "r"(u.y));
+      asm("max.f16x2 %0, %1, %2;" : "=r"(b) : "r"(u.z), "r"(u.w));
+      asm("max.f16x2 %0, %1, %2;" : "=r"(c) : "r"(a), "r"(b));
+    } else {
+      asm("max.bf16x2 %0, %1, %2;" : "=r"(a) : "r"(u.x), "r"(u.y));
+      asm("max.bf16x2 %0, %1, %2;" : "=r"(b) : "r"(u.z), "r"(u.w));
+      asm("max.bf16x2 %0, %1, %2;" : "=r"(c) : "r"(a), "r"(b));
+    }
+    const uint64_t p = pair_from_bits<T>(c);
+    return fmaxf(f2_lo(p), f2_hi(p));
+  }
+}
+// A word of -infinities.
+template <typename T>
+__device__ __forceinline__ uint32_t lowest_word() {
+  return std::is_same<T, float>::value ? 0xff800000u
+         : std::is_same<T, __half>::value ? 0xfc00fc00u
+                                          : 0xff80ff80u;
+}
+// A pack as fp32 pairs, and pairs times f rounded to a pack.
+template <typename T>
+__device__ __forceinline__ void to_pairs(const uint4& u, uint64_t (&e)[Elem<T>::kVec / 2]) {
+  if constexpr (std::is_same<T, float>::value) {
+    e[0] = f2_make(__uint_as_float(u.x), __uint_as_float(u.y));
+    e[1] = f2_make(__uint_as_float(u.z), __uint_as_float(u.w));
+  } else {
+    e[0] = pair_from_bits<T>(u.x);
+    e[1] = pair_from_bits<T>(u.y);
+    e[2] = pair_from_bits<T>(u.z);
+    e[3] = pair_from_bits<T>(u.w);
+  }
+}
+template <typename T>
+__device__ __forceinline__ uint4 from_pairs(const uint64_t (&e)[Elem<T>::kVec / 2], uint64_t f) {
+  if constexpr (std::is_same<T, float>::value) {
+    const uint64_t a = f2_mul(e[0], f), b = f2_mul(e[1], f);
+    return make_uint4(__float_as_uint(f2_lo(a)), __float_as_uint(f2_hi(a)), __float_as_uint(f2_lo(b)),
+                      __float_as_uint(f2_hi(b)));
+  } else {
+    return make_uint4(pair_to_bits<T>(f2_mul(e[0], f)), pair_to_bits<T>(f2_mul(e[1], f)),
+                      pair_to_bits<T>(f2_mul(e[2], f)), pair_to_bits<T>(f2_mul(e[3], f)));
+  }
+}
+
 template <typename T, int NT, int MINB>
-__global__ void __launch_bounds__(NT + 32, MINB)
+__global__ void __launch_bounds__(NT + kHelpers, MINB)
 distill_grad_kernel(const T* __restrict__ x, int64_t ld, Taught a, const float* __restrict__ weight,
                     int64_t weight_stride, int64_t rows, int cols, float* __restrict__ loss,
                     float2* __restrict__ stats, T* __restrict__ dx, int64_t ld_dx) {
   constexpr int VW = Elem<T>::kVec;
-  constexpr int P = kHold / VW;  // packs a thread: 4 of a 16-bit type, 8 of fp32
-  constexpr int Q = P / 4;       // ring slots a row
+  constexpr int P = kPacks;
   constexpr int W = NT / 32;
-  constexpr int kListed = 1, kStored = 3;  // named barriers, two of each
   extern __shared__ __align__(16) unsigned char smem[];
   GradShared<NT>& s = *reinterpret_cast<GradShared<NT>*>(smem);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int C = (int)cluster_size(), rank = (int)cluster_rank();
   const int64_t first = cluster_id(), step = cluster_count();
-  for (int i = tid; i < kMarkBits / 32; i += NT + 32) s.marks[i] = 0;
+  for (int i = tid; i < kMarkBits / 32; i += NT + kHelpers) s.marks[i] = 0;
   if (tid == 0) {
     bar_init(&s.bar[0], 1);
     bar_init(&s.bar[1], 1);
+    for (int i = 0; i < kStages; ++i) bar_init(&s.full[i], 1);
     s.lost = 0;
     bar_init_fence();
   }
   pdl_prologue();
   cluster_sync_all();
-  // this CTA's packs [from, to) of a row's split
+  // this CTA's packs [from, to) of a row's split (a row has cols / VW packs or
+  // one fewer, by its alignment: no division a row)
+  const int most = cols / VW, per_most = (most + C - 1) / C, per_less = (most + C - 2) / C;
   const auto slice = [&](const RowSplit& sp, int& from, int& to) {
-    const int per = (sp.nvec + C - 1) / C;
+    const int per = sp.nvec == most ? per_most : per_less;
     from = min(sp.nvec, rank * per);
     to = min(sp.nvec, from + per);
   };
   if (warp == W) {
     // the teacher's lists
-    const auto read = [&](int64_t row, int par) {
-      if (row >= rows) return;
+    ListAhead next;
+    const auto set = [&](int64_t row, int par) {
       const T* xr = x + row * ld;
       const RowSplit sp = split_row(xr, cols);
       int from, to;
       slice(sp, from, to);
-      const float w = weight != nullptr ? weight[row * weight_stride] : 1.f;
-      read_list<T, NT>(s, par, a, xr, row, cols, rank == 0 ? 0 : sp.head + from * VW,
-                       rank == 0 ? cols : sp.head + to * VW, w * a.tau);
-      named_arrive(kListed + par, NT + 32);
+      set_list<T, NT>(s, par, a, next, xr, rank == 0 ? 0 : sp.head + from * VW,
+                      rank == 0 ? cols : sp.head + to * VW);
     };
-    read(first, 0);
-    int par = 0;
+    if (first < rows) {
+      next.load(a, weight, weight_stride, first, cols);
+      set(first, 0);
+      if (first + step < rows) next.load(a, weight, weight_stride, first + step, cols);
+    }
+    int par = 0, stage = 0;
     for (int64_t row = first; row < rows; row += step, par ^= 1) {
-      read(row + step, par ^ 1);
-      named_sync(kStored + par, NT + 32);
+      if (row + step < rows) set(row + step, par ^ 1);
+      if (row + 2 * step < rows) next.load(a, weight, weight_stride, row + 2 * step, cols);
+      named_sync(kHeld + par, NT + 32);
       const GradList& l = s.list[par];
       const float total = s.total[par], by = s.by[par];
       const float2 st = s.stat[par];
@@ -507,15 +595,24 @@ distill_grad_kernel(const T* __restrict__ x, int64_t ld, Taught a, const float* 
         int from, to;
         slice(sp, from, to);
         const int lo = sp.head + from * VW, hi = sp.head + to * VW;
+        T* held = reinterpret_cast<T*>(s.stage[stage]);
         T* dr = dx + row * ld_dx;
         for (int j = lane; j < a.k; j += 32) {
           const int id = l.id[j];
-          const bool single = id < sp.head || id >= sp.head + sp.nvec * VW;  // CTA 0's
           if (id < 0 || l.mass[j] == -1.f) continue;
+          const bool single = id < sp.head || id >= sp.head + sp.nvec * VW;  // CTA 0's
           if (single ? rank != 0 : (id < lo || id >= hi)) continue;
-          dr[id] = Elem<T>::from_f(by * (ex2((l.z[j] - st.x) * a.c) / st.y - l.mass[j]));
+          const T g = Elem<T>::from_f(by * (ex2((l.z[j] - st.x) * a.c) / st.y - l.mass[j]));
+          if (single) {
+            dr[id] = g;
+          } else {
+            held[id - lo] = g;
+          }
         }
+        bulk_fence();
+        __syncwarp();
       }
+      named_arrive(kReady + stage, 64);
       if (rank == 0) {
         float d = 0.f;
         if (live) {
@@ -533,79 +630,96 @@ distill_grad_kernel(const T* __restrict__ x, int64_t ld, Taught a, const float* 
         }
       }
       __syncwarp();  // the list has been read
+      stage = stage + 1 == kStages ? 0 : stage + 1;
     }
-  } else {
-    const auto issue = [&](int64_t row, int quad, int slot) {
-      if (row < rows) {
-        const T* xr = x + row * ld;
-        const RowSplit sp = split_row(xr, cols);
-        int from, to;
-        slice(sp, from, to);
-        from += quad * 4 * NT + tid;
-        const uint4* at = reinterpret_cast<const uint4*>(xr + sp.head) + from;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (from + i * NT < to) cp_async16(&s.ring[slot][i][tid], at + i * NT);
-      }
-      cp_async_commit();
-    };
-    int64_t ahead = first;  // the next quad to issue
-    int ahead_quad = 0;
-    const auto issue_next = [&](int slot) {
-      issue(ahead, ahead_quad, slot);
-      if (++ahead_quad == Q) {
-        ahead_quad = 0;
-        ahead += step;
-      }
-    };
-#pragma unroll
-    for (int i = 0; i < kQuads; ++i) issue_next(i);
-    // where this warp's pairs go: lane r's copy to CTA r
-    const uint32_t to_pair = remote_smem(&s.pair[0][rank * W + warp], lane < C ? lane : 0);
-    const uint32_t to_bar = remote_smem(&s.bar[0], lane < C ? lane : 0);
-    int par = 0, slot = 0;
-    uint32_t phase = 0;
-    for (int64_t row = first; row < rows; row += step) {
+  } else if (warp == W + 1) {
+    // the copies
+    const auto load = [&](int64_t row, int stage) {
+      if (row >= rows || lane != 0) return;
       const T* xr = x + row * ld;
       const RowSplit sp = split_row(xr, cols);
       int from, to;
       slice(sp, from, to);
+      bar_expect(&s.full[stage], (to - from) * 16);
+      if (to > from)
+        bulk_load(s.stage[stage], reinterpret_cast<const uint4*>(xr + sp.head) + from, (to - from) * 16,
+                  &s.full[stage]);
+    };
+    for (int i = 0; i < kStages; ++i) load(first + i * step, i);
+    int stage = 0;
+    for (int64_t row = first; row < rows; row += step) {
+      named_sync(kReady + stage, 64);
+      if (lane == 0) {
+        const RowSplit sp = split_row(x + row * ld, cols);
+        int from, to;
+        slice(sp, from, to);
+        if (to > from)
+          bulk_store(reinterpret_cast<uint4*>(dx + row * ld_dx + sp.head) + from, s.stage[stage],
+                     (to - from) * 16);
+        bulk_commit();
+        bulk_wait_read();
+      }
+      __syncwarp();
+      load(row + kStages * step, stage);
+      stage = stage + 1 == kStages ? 0 : stage + 1;
+    }
+    if (lane == 0) bulk_wait();
+  } else {
+    // where this warp's pairs go: lane r's copy to CTA r
+    const uint32_t to_pair = remote_smem(&s.pair[0][rank * W + warp], lane < C ? lane : 0);
+    const uint32_t to_bar = remote_smem(&s.bar[0], lane < C ? lane : 0);
+    const uint64_t c2 = f2_make(a.c, a.c);
+    const bool edge = rank == 0 && warp == 0;  // has the rows' single elements
+    const auto single_at = [&](const T* xr) {
+      return edge ? single_of(split_row(xr, cols), lane, VW) : -1;
+    };
+    const T* xr = x + first * ld;
+    T* dr = dx + first * ld_dx;
+    int single = first < rows ? single_at(xr) : -1;
+    float xs = single >= 0 ? Elem<T>::to_f(xr[single]) : -INFINITY;
+    int par = 0, stage = 0;
+    uint32_t phase = 0, stage_phase = 0;
+    for (int64_t row = first; row < rows; row += step, xr += step * ld, dr += step * ld_dx) {
+      const RowSplit sp = split_row(xr, cols);
+      int from, to;
+      slice(sp, from, to);
       const int left = to - from - tid;  // the thread's packs end here
-      const bool edge = rank == 0 && warp == 0;  // has the row's single elements
-      const int single = edge ? single_of(sp, lane, VW) : -1;
-      float xs = single >= 0 ? Elem<T>::to_f(xr[single]) : -INFINITY;
+      const bool whole = __all_sync(0xffffffffu, left > (P - 1) * NT);
       if (tid == 0) bar_expect(&s.bar[par], C * W * 8);
-      float e[P][VW];
+      uint4* held = &s.stage[stage][0][tid];
+      // values, then exponentials, in pairs
+      uint64_t e[P][VW / 2];
       float m = fmaxf(kLowest, xs);
+      bar_wait(&s.full[stage], stage_phase, &s.lost);
 #pragma unroll
-      for (int k = 0; k < Q; ++k) {
-        cp_async_wait_pending<kQuads - 1>();
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint4 u = s.ring[slot][i][tid];
-          unpack<T>(u, e[4 * k + i]);
-          if ((4 * k + i) * NT >= left) {
-#pragma unroll
-            for (int j = 0; j < VW; ++j) e[4 * k + i][j] = -INFINITY;
-          }
-#pragma unroll
-          for (int j = 0; j < VW; j += 2) m = fmax3(m, e[4 * k + i][j], e[4 * k + i][j + 1]);
+      for (int i = 0; i < P; ++i) {
+        uint4 u = held[i * NT];
+        if (!whole && i * NT >= left) {
+          const uint32_t none = lowest_word<T>();
+          u = make_uint4(none, none, none, none);
         }
-        issue_next(slot);
-        slot = slot + 1 == kQuads ? 0 : slot + 1;
+        m = fmaxf(m, pack_max<T>(u));
+        to_pairs<T>(u, e[i]);
       }
       m = warp_max(m);
-      float sum = ex2((xs - m) * a.c);
-      xs = sum;
+      xs = ex2((xs - m) * a.c);
+      const uint64_t minus = f2_make(-m, -m);
+      uint64_t sum2 = f2_make(xs, 0.f);
 #pragma unroll
       for (int i = 0; i < P; ++i)
 #pragma unroll
-        for (int j = 0; j < VW; ++j) {
-          e[i][j] = ex2((e[i][j] - m) * a.c);
-          sum += e[i][j];
+        for (int j = 0; j < VW / 2; ++j) {
+          const uint64_t d = f2_mul(f2_add(e[i][j], minus), c2);
+          e[i][j] = f2_make(ex2(f2_lo(d)), ex2(f2_hi(d)));
+          sum2 = f2_add(sum2, e[i][j]);
         }
-      sum = warp_sum(sum);
+      const float sum = warp_sum(f2_lo(sum2) + f2_hi(sum2));
       if (lane < C) send_f2(to_pair + par * (uint32_t)sizeof(s.pair[0]), m, sum, to_bar + par * 8);
+      // the next row's single element travels while this row is exchanged
+      const float es = xs;
+      const int at_single = single;
+      single = row + step < rows ? single_at(xr + step * ld) : -1;
+      xs = single >= 0 ? Elem<T>::to_f((xr + step * ld)[single]) : -INFINITY;
       named_sync(kListed + par, NT + 32);
       const float by = s.by[par];
       const bool live = s.total[par] != 0.f;
@@ -620,23 +734,26 @@ distill_grad_kernel(const T* __restrict__ x, int64_t ld, Taught a, const float* 
       S = final_sum(warp_sum(S));
       if (s.lost) S = NAN;
       if (tid == 0) s.stat[par] = make_float2(M, S);
-      const float f = live ? ex2((m - M) * a.c) * (by / S) : 0.f;
-      T* dr = dx + row * ld_dx;
-      uint4* out = reinterpret_cast<uint4*>(dr + sp.head) + from + tid;
-      if (single >= 0) dr[single] = Elem<T>::from_f(live ? xs * f : 0.f);
+      if (live) {
+        const float f = ex2((m - M) * a.c) * (by / S);
+        const uint64_t f2 = f2_make(f, f);
+        if (at_single >= 0) dr[at_single] = Elem<T>::from_f(es * f);
 #pragma unroll
-      for (int i = 0; i < P; ++i) {
-        if (i * NT < left) {
+        for (int i = 0; i < P; ++i) held[i * NT] = from_pairs<T>(e[i], f2);
+      } else {
+        if (at_single >= 0) dr[at_single] = Elem<T>::from_f(0.f);
 #pragma unroll
-          for (int j = 0; j < VW; ++j) e[i][j] = live ? e[i][j] * f : 0.f;
-          st_stream(out + i * NT, pack<T>(e[i]));
-        }
+        for (int i = 0; i < P; ++i) held[i * NT] = make_uint4(0, 0, 0, 0);
       }
-      named_arrive(kStored + par, NT + 32);
+      bulk_fence();
+      named_arrive(kHeld + par, NT + 32);
       phase ^= par;
       par ^= 1;
+      if (++stage == kStages) {
+        stage = 0;
+        stage_phase ^= 1;
+      }
     }
-    cp_async_wait_all();
   }
   __syncwarp();
   cluster_sync_all();  // no CTA leaves while pairs may still be sent to it
@@ -714,7 +831,7 @@ int grad_clusters(int cluster, cudaLaunchConfig_t cfg) {
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kDevices) return 0;
   int n = known[dev][cluster].load(std::memory_order_relaxed);
   if (n == 0) {
-    if (cudaOccupancyMaxActiveClusters(&n, distill_grad_kernel<T, NT, NT == 512 ? 2 : NT == 256 ? 3 : 5>,
+    if (cudaOccupancyMaxActiveClusters(&n, distill_grad_kernel<T, NT, NT == 256 ? 2 : NT == 128 ? 4 : 7>,
                                        &cfg) != cudaSuccess)
       n = 0;
     (void)cudaGetLastError();
@@ -728,8 +845,8 @@ template <typename T, int NT>
 int run_grad(const void* x, int64_t ld, const Taught& a, const float* weight, int64_t weight_stride,
              int64_t rows, int64_t cols, float* loss, float* stats, void* dx, int64_t ld_dx,
              cudaStream_t stream) {
-  const auto kern = distill_grad_kernel<T, NT, NT == 512 ? 2 : NT == 256 ? 3 : 5>;
-  const int64_t cluster = ceil_div(cols, (int64_t)NT * kHold);
+  const auto kern = distill_grad_kernel<T, NT, NT == 256 ? 2 : NT == 128 ? 4 : 7>;
+  const int64_t cluster = ceil_div(cols, (int64_t)NT * kPacks * Elem<T>::kVec);
   if (cluster > kMaxCluster || a.k > kGradList) return -1;
   const size_t smem = sizeof(GradShared<NT>);
   // (per launch: the attributes are held per device)
@@ -741,7 +858,7 @@ int run_grad(const void* x, int64_t ld, const Taught& a, const float* weight, in
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)cluster);
-  cfg.blockDim = dim3(NT + 32);
+  cfg.blockDim = dim3(NT + kHelpers);
   cfg.dynamicSmemBytes = smem;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -752,7 +869,7 @@ int run_grad(const void* x, int64_t ld, const Taught& a, const float* weight, in
   cfg.numAttrs = 1;
   const int clusters = grad_clusters<T, NT>((int)cluster, cfg);
   if (clusters == 0) return -1;
-  return launch_cluster(kern, std::min<int64_t>(rows, clusters) * cluster, (int)cluster, NT + 32, smem,
+  return launch_cluster(kern, std::min<int64_t>(rows, clusters) * cluster, (int)cluster, NT + kHelpers, smem,
                         stream, reinterpret_cast<const T*>(x), ld, a, weight, weight_stride, rows,
                         (int)cols, loss, reinterpret_cast<float2*>(stats), reinterpret_cast<T*>(dx),
                         ld_dx);
@@ -834,9 +951,10 @@ FL_B200_API int fl_b200_distill_topk_grad(const void* logits, int64_t ld, const 
                                                      loss, stats, dlogits, ld_dlogits,
                                                      (cudaStream_t)stream);
       };
+      constexpr int kHold = kPacks * Elem<T>::kVec;  // elements a thread
+      if (cols <= 64 * kHold) return go(std::integral_constant<int, 64>{});
       if (cols <= 128 * kHold) return go(std::integral_constant<int, 128>{});
-      if (cols <= 256 * kHold) return go(std::integral_constant<int, 256>{});
-      return go(std::integral_constant<int, 512>{});
+      return go(std::integral_constant<int, 256>{});
     });
     if (st != -1) return st;
   }

@@ -136,6 +136,31 @@ __device__ __forceinline__ void bar_wait(uint64_t* bar, uint32_t parity, volatil
     }
   }
 }
+// Asynchronous bulk copies of 16-byte multiples between 16-byte boundaries:
+// global to this CTA's shared memory, counted on its barrier, and back, in
+// this thread's bulk groups.
+__device__ __forceinline__ void bulk_load(void* smem, const void* gmem, uint32_t bytes, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+          (uint32_t)__cvta_generic_to_shared(smem)),
+      "l"(gmem), "r"(bytes), "r"((uint32_t)__cvta_generic_to_shared(bar))
+      : "memory");
+}
+__device__ __forceinline__ void bulk_store(void* gmem, const void* smem, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(gmem),
+               "r"((uint32_t)__cvta_generic_to_shared(smem)), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+// Returns once the committed stores have read shared memory / are done.
+__device__ __forceinline__ void bulk_wait_read() {
+  asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+}
+__device__ __forceinline__ void bulk_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+// Orders this thread's shared memory accesses before later bulk copies (of
+// threads that a barrier puts after it).
+__device__ __forceinline__ void bulk_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
 // Named barriers: all `threads` threads meet (sync), or are counted without
 // waiting (arrive).
 __device__ __forceinline__ void named_sync(int id, int threads) {
