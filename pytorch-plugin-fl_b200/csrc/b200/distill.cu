@@ -333,14 +333,15 @@ distill_bwd_kernel(const float* __restrict__ dloss, int64_t dloss_stride, const 
 // each by one bulk copy, so that neither memory direction holds up the warps
 // (stores from registers did: a third of a row's time was theirs).
 //
-// Two further warps: one reads the teacher's lists a row ahead, puts the
-// gradients of the tokens they name in place, and in CTA 0 writes the loss;
-// the other issues the copies.
+// Two further warps, a row each in turn, read the teacher's lists ahead, put
+// the gradients of the tokens they name in place, issue the copies and in CTA 0
+// write the loss (one warp took longer over 64 entries than the holders over a
+// row).
 constexpr int kGradList = 256;       // teacher entries a row that this kernel takes
 constexpr int kPacks = 8;            // 16-byte packs a thread holds
 constexpr int kStages = 3;
 constexpr int kMaxCluster = 16;
-constexpr int kMarkBits = 16384;     // marks of the tokens named so far, by id modulo this
+constexpr int kMarkBits = 8192;      // marks of the tokens named so far, by id modulo this
 
 struct GradList {
   int id[kGradList];      // -1: absent
@@ -354,7 +355,7 @@ struct GradShared {
   uint4 stage[kStages][kPacks][NT];
   float2 pair[2][kMaxCluster * (NT / 32)];
   GradList list[2];
-  uint32_t marks[kMarkBits / 32];
+  uint32_t marks[2][kMarkBits / 32];
   float2 stat[2];   // (M, S) of the row, for the list's warp
   float by[2];      // w tau
   float total[2];   // of the list's 2^t2; 0: nothing taught
@@ -364,31 +365,70 @@ struct GradShared {
 };
 
 constexpr int kHelpers = 64;  // threads besides the NT that hold the row
-// Named barriers, two of each for alternate rows, one of the last a stage: a
-// barrier's next use follows, through the others, every wait on this one.
+// Named barriers, two of each for alternate rows: a barrier's next use follows,
+// through the other kind, every wait on this one.
 constexpr int kListed = 1;  // the list is known: the holders wait for its warp
 constexpr int kHeld = 3;    // the gradient is in place: the list's warp waits for the holders
-constexpr int kReady = 5;   // and the list's tokens: the copies' warp waits for the list's
 
-// A row's list on its way, kGradList / 32 entries a lane.
+// Warp-wide maximum; NaN only if every lane has one.
+__device__ __forceinline__ float warp_max(float v) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+// The same, NaN if any lane has one.
+__device__ __forceinline__ float warp_max_nan(float v) {
+  float r;
+  asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+// A row's list on its way, kGradList / 32 entries a lane, as loaded: a value
+// that is not touched until the next row's turn does not hold the warp up.
 struct ListAhead {
   static constexpr int kEach = kGradList / 32;
-  int id[kEach];    // -1: absent
-  float t[kEach];
+  long long id[kEach];
+  uint32_t t[kEach];
   float w;
 
   __device__ __forceinline__ void load(const Taught& a, const float* weight, int64_t weight_stride,
-                                       int64_t row, int cols) {
+                                       int64_t row) {
     const int lane = threadIdx.x & 31;
-    w = weight != nullptr ? weight[row * weight_stride] : 1.f;
+    w = 1.f;
+    if (weight != nullptr) w = weight[row * weight_stride];
+    const int64_t at = row * a.ld_ids + lane, at_t = row * a.ld_t + lane;
+    if (a.ids_dtype == FL_B200_I64) {
+      const long long* p = reinterpret_cast<const long long*>(a.ids) + at;
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      const int j = lane + 32 * i;
-      if (32 * i >= a.k) break;
-      const int64_t v = j < a.k ? load_index(a.ids, a.ids_dtype, row * a.ld_ids + j) : -1;
-      id[i] = v >= 0 && v < cols ? (int)v : -1;
-      t[i] = j < a.k ? load_float(a.t, a.t_dtype, row * a.ld_t + j) : 0.f;
+      for (int i = 0; i < kEach; ++i)
+        if (lane + 32 * i < a.k) id[i] = p[32 * i];
+    } else {
+      const uint32_t* p = reinterpret_cast<const uint32_t*>(a.ids) + at;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i)
+        if (lane + 32 * i < a.k) id[i] = p[32 * i];  // (zero-extended: negative ones end up past V)
     }
+    if (a.t_dtype == FL_B200_F32) {
+      const uint32_t* p = reinterpret_cast<const uint32_t*>(a.t) + at_t;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i)
+        if (lane + 32 * i < a.k) t[i] = p[32 * i];
+    } else {
+      const unsigned short* p = reinterpret_cast<const unsigned short*>(a.t) + at_t;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i)
+        if (lane + 32 * i < a.k) t[i] = p[32 * i];
+    }
+  }
+  __device__ __forceinline__ int token(int i, int k, int cols) const {  // -1: absent
+    const bool in = (int)(threadIdx.x & 31) + 32 * i < k && (unsigned long long)id[i] < (unsigned)cols;
+    return in ? (int)id[i] : -1;
+  }
+  __device__ __forceinline__ float logit(int i, int dtype) const {
+    if (dtype == FL_B200_F32) return __uint_as_float(t[i]);
+    if (dtype == FL_B200_BF16) return __uint_as_float(t[i] << 16);
+    return __half2float(__ushort_as_half((unsigned short)t[i]));
   }
 };
 
@@ -396,27 +436,35 @@ struct ListAhead {
 // Logits are read for the entries in [lo, hi).
 template <typename T, int NT>
 __device__ __forceinline__ void set_list(GradShared<NT>& s, int par, const Taught& a, const ListAhead& in,
-                                         const T* x, int lo, int hi) {
+                                         const T* x, int cols, int lo, int hi) {
+  constexpr int kEach = ListAhead::kEach;
   GradList& l = s.list[par];
   const int lane = threadIdx.x & 31;
-  float z[ListAhead::kEach], e[ListAhead::kEach];
+  int id[kEach];
+  T z[kEach];
+  float e[kEach];
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    if (32 * i >= a.k) break;
+    id[i] = in.token(i, a.k, cols);
+    if (id[i] >= lo && id[i] < hi) z[i] = x[id[i]];  // (used when the masses are stored)
+  }
   float top = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < ListAhead::kEach; ++i) {
+  for (int i = 0; i < kEach; ++i) {
     if (32 * i >= a.k) break;
-    z[i] = in.id[i] >= lo && in.id[i] < hi ? Elem<T>::to_f(x[in.id[i]]) : 0.f;
-    e[i] = in.id[i] >= 0 ? in.t[i] : -INFINITY;
+    e[i] = id[i] >= 0 ? in.logit(i, a.t_dtype) : -INFINITY;
     top = MaxOp::combine(top, e[i]);
   }
-  top = group_reduce_warp<MaxOp, 32>(top);
+  top = warp_max_nan(top);
   float total = 0.f;
   if (top != -INFINITY) {
 #pragma unroll
-    for (int i = 0; i < ListAhead::kEach; ++i) {
+    for (int i = 0; i < kEach; ++i) {
       if (32 * i >= a.k) break;
       const float t2 = (e[i] - top) * a.c;
       if (lane + 32 * i < a.k) l.t2[lane + 32 * i] = t2;
-      e[i] = in.id[i] >= 0 ? exp2f(t2) : 0.f;
+      e[i] = id[i] >= 0 ? exp2f(t2) : 0.f;
       total += e[i];
     }
   }
@@ -429,31 +477,32 @@ __device__ __forceinline__ void set_list(GradShared<NT>& s, int par, const Taugh
   named_arrive(kListed + par, NT + 32);  // the row may be written
   // masses: an id whose mark was set already may be a repeated one
   const float inverse = 1.f / total;
+  uint32_t before[kEach];
 #pragma unroll
-  for (int i = 0; i < ListAhead::kEach; ++i) {
+  for (int i = 0; i < kEach; ++i) {
     if (32 * i >= a.k) break;
-    const int j = lane + 32 * i, id = in.id[i];
-    bool again = false;
+    const int j = lane + 32 * i;
+    const uint32_t h = (uint32_t)id[i] % kMarkBits;
+    before[i] = id[i] >= 0 ? atomicOr(&s.marks[par][h / 32], 1u << (h % 32)) : 0;
     if (j < a.k) {
-      l.id[j] = id;
-      l.z[j] = z[i];
-      l.mass[j] = id >= 0 ? e[i] * inverse : -1.f;
+      l.id[j] = id[i];
+      l.mass[j] = id[i] >= 0 ? e[i] * inverse : -1.f;
     }
-    if (id >= 0) {
-      const uint32_t h = (uint32_t)id % kMarkBits;
-      again = (atomicOr(&s.marks[h / 32], 1u << (h % 32)) >> (h % 32)) & 1;
-    }
-    __syncwarp();
+  }
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    if (32 * i >= a.k) break;
+    const bool again = id[i] >= 0 && (before[i] >> ((uint32_t)id[i] % 32)) & 1;
     uint32_t votes = __ballot_sync(0xffffffffu, again);
     while (votes != 0) {
-      // the warp goes over the list so far for one such id: its first entry
+      // the warp goes over the list for one such id: its first entry
       // takes the sum of all
       const int same = l.id[32 * i + __ffs(votes) - 1];
       votes &= votes - 1;
-      const int end = min(a.k, 32 * i + 32);
-      int first = end;
+      int first = a.k;
       float mass = 0.f;
-      for (int n = lane; n < end; n += 32) {
+      for (int n = lane; n < a.k; n += 32) {
         if (l.id[n] != same) continue;
         first = min(first, n);
         if (l.mass[n] != -1.f) mass += l.mass[n];
@@ -461,24 +510,19 @@ __device__ __forceinline__ void set_list(GradShared<NT>& s, int par, const Taugh
       __syncwarp();
       first = __reduce_min_sync(0xffffffffu, first);
       mass = warp_sum(mass);
-      for (int n = lane; n < end; n += 32)
+      for (int n = lane; n < a.k; n += 32)
         if (l.id[n] == same) l.mass[n] = n == first ? mass : -1.f;
       __syncwarp();
     }
   }
 #pragma unroll
-  for (int i = 0; i < ListAhead::kEach; ++i) {
+  for (int i = 0; i < kEach; ++i) {
     if (32 * i >= a.k) break;
-    if (in.id[i] >= 0) s.marks[(uint32_t)in.id[i] % kMarkBits / 32] = 0;
+    if (id[i] >= 0) s.marks[par][(uint32_t)id[i] % kMarkBits / 32] = 0;
+    if (lane + 32 * i < a.k)
+      l.z[lane + 32 * i] = id[i] >= lo && id[i] < hi ? Elem<T>::to_f(z[i]) : 0.f;
   }
   __syncwarp();
-}
-
-// Warp-wide maximum; NaN only if every lane has one.
-__device__ __forceinline__ float warp_max(float v) {
-  float r;
-  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
-  return r;
 }
 
 // Maximum of a pack's elements (NaN ignored unless all are).
@@ -547,7 +591,7 @@ distill_grad_kernel(const T* __restrict__ x, int64_t ld, Taught a, const float* 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int C = (int)cluster_size(), rank = (int)cluster_rank();
   const int64_t first = cluster_id(), step = cluster_count();
-  for (int i = tid; i < kMarkBits / 32; i += NT + kHelpers) s.marks[i] = 0;
+  for (int i = tid; i < 2 * (kMarkBits / 32); i += NT + kHelpers) s.marks[0][i] = 0;
   if (tid == 0) {
     bar_init(&s.bar[0], 1);
     bar_init(&s.bar[1], 1);
@@ -565,44 +609,56 @@ distill_grad_kernel(const T* __restrict__ x, int64_t ld, Taught a, const float* 
     from = min(sp.nvec, rank * per);
     to = min(sp.nvec, from + per);
   };
-  if (warp == W) {
-    // the teacher's lists
+  if (warp >= W) {
+    // every other row's list, and its copies
+    const int par = warp - W;
     ListAhead next;
-    const auto set = [&](int64_t row, int par) {
+    const auto set = [&](int64_t row) {
       const T* xr = x + row * ld;
       const RowSplit sp = split_row(xr, cols);
       int from, to;
       slice(sp, from, to);
-      set_list<T, NT>(s, par, a, next, xr, rank == 0 ? 0 : sp.head + from * VW,
+      set_list<T, NT>(s, par, a, next, xr, cols, rank == 0 ? 0 : sp.head + from * VW,
                       rank == 0 ? cols : sp.head + to * VW);
+      if (row + 2 * step < rows) next.load(a, weight, weight_stride, row + 2 * step);
     };
-    if (first < rows) {
-      next.load(a, weight, weight_stride, first, cols);
-      set(first, 0);
-      if (first + step < rows) next.load(a, weight, weight_stride, first + step, cols);
+    const auto load = [&](int64_t row, int stage) {
+      if (row >= rows || lane != 0) return;
+      const T* xr = x + row * ld;
+      const RowSplit sp = split_row(xr, cols);
+      int from, to;
+      slice(sp, from, to);
+      bar_expect(&s.full[stage], (to - from) * 16);
+      if (to > from)
+        bulk_load(s.stage[stage], reinterpret_cast<const uint4*>(xr + sp.head) + from, (to - from) * 16,
+                  &s.full[stage]);
+    };
+    for (int i = par; i < kStages; i += 2) load(first + i * step, i);
+    if (first + par * step < rows) {
+      next.load(a, weight, weight_stride, first + par * step);
+      set(first + par * step);
     }
-    int par = 0, stage = 0;
-    for (int64_t row = first; row < rows; row += step, par ^= 1) {
-      if (row + step < rows) set(row + step, par ^ 1);
-      if (row + 2 * step < rows) next.load(a, weight, weight_stride, row + 2 * step, cols);
+    int stage = par;
+    for (int64_t row = first + par * step; row < rows; row += 2 * step) {
       named_sync(kHeld + par, NT + 32);
       const GradList& l = s.list[par];
       const float total = s.total[par], by = s.by[par];
       const float2 st = s.stat[par];
       const bool live = total != 0.f;
+      const RowSplit sp = split_row(x + row * ld, cols);
+      int from, to;
+      slice(sp, from, to);
+      T* dr = dx + row * ld_dx;
       if (live) {
-        const RowSplit sp = split_row(x + row * ld, cols);
-        int from, to;
-        slice(sp, from, to);
         const int lo = sp.head + from * VW, hi = sp.head + to * VW;
+        const float inverse = 1.f / st.y;
         T* held = reinterpret_cast<T*>(s.stage[stage]);
-        T* dr = dx + row * ld_dx;
         for (int j = lane; j < a.k; j += 32) {
           const int id = l.id[j];
           if (id < 0 || l.mass[j] == -1.f) continue;
           const bool single = id < sp.head || id >= sp.head + sp.nvec * VW;  // CTA 0's
           if (single ? rank != 0 : (id < lo || id >= hi)) continue;
-          const T g = Elem<T>::from_f(by * (ex2((l.z[j] - st.x) * a.c) / st.y - l.mass[j]));
+          const T g = Elem<T>::from_f(by * (ex2((l.z[j] - st.x) * a.c) * inverse - l.mass[j]));
           if (single) {
             dr[id] = g;
           } else {
@@ -612,7 +668,11 @@ distill_grad_kernel(const T* __restrict__ x, int64_t ld, Taught a, const float* 
         bulk_fence();
         __syncwarp();
       }
-      named_arrive(kReady + stage, 64);
+      if (lane == 0) {
+        if (to > from)
+          bulk_store(reinterpret_cast<uint4*>(dr + sp.head) + from, s.stage[stage], (to - from) * 16);
+        bulk_commit();
+      }
       if (rank == 0) {
         float d = 0.f;
         if (live) {
@@ -629,39 +689,11 @@ distill_grad_kernel(const T* __restrict__ x, int64_t ld, Taught a, const float* 
           stats[row] = live ? st : make_float2(0.f, 0.f);
         }
       }
-      __syncwarp();  // the list has been read
-      stage = stage + 1 == kStages ? 0 : stage + 1;
-    }
-  } else if (warp == W + 1) {
-    // the copies
-    const auto load = [&](int64_t row, int stage) {
-      if (row >= rows || lane != 0) return;
-      const T* xr = x + row * ld;
-      const RowSplit sp = split_row(xr, cols);
-      int from, to;
-      slice(sp, from, to);
-      bar_expect(&s.full[stage], (to - from) * 16);
-      if (to > from)
-        bulk_load(s.stage[stage], reinterpret_cast<const uint4*>(xr + sp.head) + from, (to - from) * 16,
-                  &s.full[stage]);
-    };
-    for (int i = 0; i < kStages; ++i) load(first + i * step, i);
-    int stage = 0;
-    for (int64_t row = first; row < rows; row += step) {
-      named_sync(kReady + stage, 64);
-      if (lane == 0) {
-        const RowSplit sp = split_row(x + row * ld, cols);
-        int from, to;
-        slice(sp, from, to);
-        if (to > from)
-          bulk_store(reinterpret_cast<uint4*>(dx + row * ld_dx + sp.head) + from, s.stage[stage],
-                     (to - from) * 16);
-        bulk_commit();
-        bulk_wait_read();
-      }
-      __syncwarp();
+      if (lane == 0) bulk_wait_read();
+      __syncwarp();  // the list has been read, and the stage
       load(row + kStages * step, stage);
-      stage = stage + 1 == kStages ? 0 : stage + 1;
+      if (row + 2 * step < rows) set(row + 2 * step);
+      stage = (stage + 2) % kStages;
     }
     if (lane == 0) bulk_wait();
   } else {
@@ -831,7 +863,7 @@ int grad_clusters(int cluster, cudaLaunchConfig_t cfg) {
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kDevices) return 0;
   int n = known[dev][cluster].load(std::memory_order_relaxed);
   if (n == 0) {
-    if (cudaOccupancyMaxActiveClusters(&n, distill_grad_kernel<T, NT, NT == 256 ? 2 : NT == 128 ? 4 : 7>,
+    if (cudaOccupancyMaxActiveClusters(&n, distill_grad_kernel<T, NT, NT == 256 ? 2 : NT == 128 ? 3 : 5>,
                                        &cfg) != cudaSuccess)
       n = 0;
     (void)cudaGetLastError();
@@ -845,7 +877,7 @@ template <typename T, int NT>
 int run_grad(const void* x, int64_t ld, const Taught& a, const float* weight, int64_t weight_stride,
              int64_t rows, int64_t cols, float* loss, float* stats, void* dx, int64_t ld_dx,
              cudaStream_t stream) {
-  const auto kern = distill_grad_kernel<T, NT, NT == 256 ? 2 : NT == 128 ? 4 : 7>;
+  const auto kern = distill_grad_kernel<T, NT, NT == 256 ? 2 : NT == 128 ? 3 : 5>;
   const int64_t cluster = ceil_div(cols, (int64_t)NT * kPacks * Elem<T>::kVec);
   if (cluster > kMaxCluster || a.k > kGradList) return -1;
   const size_t smem = sizeof(GradShared<NT>);
