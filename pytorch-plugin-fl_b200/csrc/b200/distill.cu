@@ -327,26 +327,26 @@ distill_bwd_kernel(const float* __restrict__ dloss, int64_t dloss_stride, const 
 // on chip, 128 bytes of logits a thread, as exponentials 2^((z - m_w) c)
 // against the warp's own maximum.  Every warp sends its (m_w, sum) to every
 // CTA of the cluster (st.async on a transaction barrier: no fence, no second
-// hop through a CTA total); each warp then folds all pairs to (M, S) and
-// writes w tau e 2^((m_w - M) c) / S over the logits in shared memory.  Three
+// hop through a CTA total), where one warp folds all pairs to (M, S); the
+// others then write w tau e 2^((m_w - M) c) / S over the logits in shared
+// memory.  Three
 // stages of a row's slice take turns: one arriving, one in hand, one leaving,
 // each by one bulk copy, so that neither memory direction holds up the warps
 // (stores from registers did: a third of a row's time was theirs).
 //
-// Two further warps, a row each in turn, read the teacher's lists ahead, put
-// the gradients of the tokens they name in place, issue the copies and in CTA 0
-// write the loss (one warp took longer over 64 entries than the holders over a
-// row).
+// That warp is one of two more, a row each in turn, which read the teacher's
+// lists ahead, put the gradients of the tokens they name in place, issue the
+// copies and in CTA 0 write the loss (a single one took longer over 64 entries
+// than the holders over a row).
 constexpr int kGradList = 256;       // teacher entries a row that this kernel takes
 constexpr int kPacks = 8;            // 16-byte packs a thread holds
 constexpr int kStages = 3;
 constexpr int kMaxCluster = 16;
 constexpr int kMarkBits = 8192;      // marks of the tokens named so far, by id modulo this
 
+// A list's tokens and masses, for the search after repeated ones.
 struct GradList {
   int id[kGradList];      // -1: absent
-  float t2[kGradList];    // (t - max t) c
-  float z[kGradList];     // the logit at id (CTA 0: every entry; else those of its slice)
   float mass[kGradList];  // sum of p over the entries with this id; -1 but at the first of them
 };
 
@@ -356,9 +356,8 @@ struct GradShared {
   float2 pair[2][kMaxCluster * (NT / 32)];
   GradList list[2];
   uint32_t marks[2][kMarkBits / 32];
-  float2 stat[2];   // (M, S) of the row, for the list's warp
-  float by[2];      // w tau
-  float total[2];   // of the list's 2^t2; 0: nothing taught
+  float2 scale[2];  // the row's M, and w tau / S
+  int live[2];      // whether anything is taught
   uint64_t bar[2];          // the row's pairs have come
   uint64_t full[kStages];   // the stage's logits have come
   int lost;
@@ -367,7 +366,7 @@ struct GradShared {
 constexpr int kHelpers = 64;  // threads besides the NT that hold the row
 // Named barriers, two of each for alternate rows: a barrier's next use follows,
 // through the other kind, every wait on this one.
-constexpr int kListed = 1;  // the list is known: the holders wait for its warp
+constexpr int kScaled = 1;  // the row's scale is known: the holders wait for the list's warp
 constexpr int kHeld = 3;    // the gradient is in place: the list's warp waits for the holders
 
 // Warp-wide maximum; NaN only if every lane has one.
@@ -432,98 +431,116 @@ struct ListAhead {
   }
 };
 
-// Sets up list `par` from the entries of row x that have arrived; one warp.
-// Logits are read for the entries in [lo, hi).
-template <typename T, int NT>
-__device__ __forceinline__ void set_list(GradShared<NT>& s, int par, const Taught& a, const ListAhead& in,
-                                         const T* x, int cols, int lo, int hi) {
-  constexpr int kEach = ListAhead::kEach;
-  GradList& l = s.list[par];
-  const int lane = threadIdx.x & 31;
-  int id[kEach];
-  T z[kEach];
-  float e[kEach];
-#pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    if (32 * i >= a.k) break;
-    id[i] = in.token(i, a.k, cols);
-    if (id[i] >= lo && id[i] < hi) z[i] = x[id[i]];  // (used when the masses are stored)
-  }
-  float top = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    if (32 * i >= a.k) break;
-    e[i] = id[i] >= 0 ? in.logit(i, a.t_dtype) : -INFINITY;
-    top = MaxOp::combine(top, e[i]);
-  }
-  top = warp_max_nan(top);
-  float total = 0.f;
-  if (top != -INFINITY) {
+// 1 / x within an ulp (x a sum of exponentials: normal, or NaN).
+__device__ __forceinline__ float reciprocal(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// A row's list in hand, spread over a warp as ListAhead is.  (Registers and
+// unrolled loops: what this warp does between a row's sums and its scale holds
+// up all the others, and a loop over shared memory took ten times as long.)
+template <typename T>
+struct ListHeld {
+  static constexpr int kEach = ListAhead::kEach;
+  int id[kEach];      // -1: absent
+  T z[kEach];         // the logit, of entries in [lo, hi)
+  float t2[kEach];    // (t - max t) c
+  float e[kEach];     // 2^t2, 0 where absent
+  float mass[kEach];  // as GradList's
+  float total;        // of e; 0 when nothing is taught
+  float by;           // w tau
+
+  __device__ __forceinline__ void set(const Taught& a, const ListAhead& in, const T* x, int cols, int lo,
+                                      int hi, GradList& l, uint32_t* marks) {
+    const int lane = threadIdx.x & 31;
+    by = in.w * a.tau;
+    float top = -INFINITY;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
       if (32 * i >= a.k) break;
-      const float t2 = (e[i] - top) * a.c;
-      if (lane + 32 * i < a.k) l.t2[lane + 32 * i] = t2;
-      e[i] = id[i] >= 0 ? exp2f(t2) : 0.f;
+      id[i] = in.token(i, a.k, cols);
+      if (id[i] >= lo && id[i] < hi) z[i] = x[id[i]];  // (not touched before the row is summed)
+    }
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      if (32 * i >= a.k) break;
+      t2[i] = id[i] >= 0 ? in.logit(i, a.t_dtype) : -INFINITY;
+      top = MaxOp::combine(top, t2[i]);
+    }
+    top = warp_max_nan(top);
+    total = 0.f;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      if (32 * i >= a.k) break;
+      t2[i] = (t2[i] - top) * a.c;
+      e[i] = id[i] >= 0 && top != -INFINITY ? ex2(t2[i]) : 0.f;
       total += e[i];
     }
-  }
-  total = warp_sum(total);
-  if (lane == 0) {
-    s.total[par] = total;
-    s.by[par] = in.w * a.tau;
-  }
-  __syncwarp();
-  named_arrive(kListed + par, NT + 32);  // the row may be written
-  // masses: an id whose mark was set already may be a repeated one
-  const float inverse = 1.f / total;
-  uint32_t before[kEach];
+    total = warp_sum(total);
+    const float inverse = reciprocal(total);
+    // an id whose mark was set already may be a repeated one
+    uint32_t again = 0;
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    if (32 * i >= a.k) break;
-    const int j = lane + 32 * i;
-    const uint32_t h = (uint32_t)id[i] % kMarkBits;
-    before[i] = id[i] >= 0 ? atomicOr(&s.marks[par][h / 32], 1u << (h % 32)) : 0;
-    if (j < a.k) {
-      l.id[j] = id[i];
-      l.mass[j] = id[i] >= 0 ? e[i] * inverse : -1.f;
+    for (int i = 0; i < kEach; ++i) {
+      if (32 * i >= a.k) break;
+      mass[i] = id[i] >= 0 ? e[i] * inverse : -1.f;
+      if (id[i] >= 0) {
+        const uint32_t h = (uint32_t)id[i] % kMarkBits;
+        again |= ((atomicOr(&marks[h / 32], 1u << (h % 32)) >> (h % 32)) & 1) << i;
+      }
     }
-  }
-  __syncwarp();
+    __syncwarp();
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    if (32 * i >= a.k) break;
-    const bool again = id[i] >= 0 && (before[i] >> ((uint32_t)id[i] % 32)) & 1;
-    uint32_t votes = __ballot_sync(0xffffffffu, again);
-    while (votes != 0) {
-      // the warp goes over the list for one such id: its first entry
-      // takes the sum of all
-      const int same = l.id[32 * i + __ffs(votes) - 1];
-      votes &= votes - 1;
-      int first = a.k;
-      float mass = 0.f;
-      for (int n = lane; n < a.k; n += 32) {
-        if (l.id[n] != same) continue;
-        first = min(first, n);
-        if (l.mass[n] != -1.f) mass += l.mass[n];
+    for (int i = 0; i < kEach; ++i) {
+      if (32 * i >= a.k) break;
+      if (id[i] >= 0) marks[(uint32_t)id[i] % kMarkBits / 32] = 0;
+    }
+    if (__any_sync(0xffffffffu, again != 0)) {
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        const int j = lane + 32 * i;
+        if (j < a.k) {
+          l.id[j] = id[i];
+          l.mass[j] = mass[i];
+        }
       }
       __syncwarp();
-      first = __reduce_min_sync(0xffffffffu, first);
-      mass = warp_sum(mass);
-      for (int n = lane; n < a.k; n += 32)
-        if (l.id[n] == same) l.mass[n] = n == first ? mass : -1.f;
-      __syncwarp();
+      merge(a.k, again, l);
+#pragma unroll
+      for (int i = 0; i < kEach; ++i)
+        if (lane + 32 * i < a.k) mass[i] = l.mass[lane + 32 * i];
+    }
+    __syncwarp();
+  }
+
+  // For each id under suspicion the warp goes over the list: its first entry
+  // takes the sum of all.
+  __device__ __noinline__ static void merge(int k, uint32_t again, GradList& l) {
+    const int lane = threadIdx.x & 31;
+    for (int i = 0; 32 * i < k; ++i) {
+      uint32_t votes = __ballot_sync(0xffffffffu, (again >> i) & 1);
+      while (votes != 0) {
+        const int same = l.id[32 * i + __ffs(votes) - 1];
+        votes &= votes - 1;
+        int first = k;
+        float sum = 0.f;
+        for (int n = lane; n < k; n += 32) {
+          if (l.id[n] != same) continue;
+          first = min(first, n);
+          if (l.mass[n] != -1.f) sum += l.mass[n];
+        }
+        __syncwarp();
+        first = __reduce_min_sync(0xffffffffu, first);
+        sum = warp_sum(sum);
+        for (int n = lane; n < k; n += 32)
+          if (l.id[n] == same) l.mass[n] = n == first ? sum : -1.f;
+        __syncwarp();
+      }
     }
   }
-#pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    if (32 * i >= a.k) break;
-    if (id[i] >= 0) s.marks[par][(uint32_t)id[i] % kMarkBits / 32] = 0;
-    if (lane + 32 * i < a.k)
-      l.z[lane + 32 * i] = id[i] >= lo && id[i] < hi ? Elem<T>::to_f(z[i]) : 0.f;
-  }
-  __syncwarp();
-}
+};
 
 // Maximum of a pack's elements (NaN ignored unless all are).
 template <typename T>
@@ -613,13 +630,15 @@ distill_grad_kernel(const T* __restrict__ x, int64_t ld, Taught a, const float* 
     // every other row's list, and its copies
     const int par = warp - W;
     ListAhead next;
+    ListHeld<T> list;
     const auto set = [&](int64_t row) {
       const T* xr = x + row * ld;
       const RowSplit sp = split_row(xr, cols);
       int from, to;
       slice(sp, from, to);
-      set_list<T, NT>(s, par, a, next, xr, cols, rank == 0 ? 0 : sp.head + from * VW,
-                      rank == 0 ? cols : sp.head + to * VW);
+      if (lane == 0) bar_expect(&s.bar[par], C * W * 8);
+      list.set(a, next, xr, cols, rank == 0 ? 0 : sp.head + from * VW,
+               rank == 0 ? cols : sp.head + to * VW, s.list[par], s.marks[par]);
       if (row + 2 * step < rows) next.load(a, weight, weight_stride, row + 2 * step);
     };
     const auto load = [&](int64_t row, int stage) {
@@ -639,26 +658,47 @@ distill_grad_kernel(const T* __restrict__ x, int64_t ld, Taught a, const float* 
       set(first + par * step);
     }
     int stage = par;
-    for (int64_t row = first + par * step; row < rows; row += 2 * step) {
-      named_sync(kHeld + par, NT + 32);
-      const GradList& l = s.list[par];
-      const float total = s.total[par], by = s.by[par];
-      const float2 st = s.stat[par];
-      const bool live = total != 0.f;
+    uint32_t phase = 0;
+    for (int64_t row = first + par * step; row < rows; row += 2 * step, phase ^= 1) {
+      bar_wait(&s.bar[par], phase, &s.lost);
+      constexpr int kPairs = kMaxCluster * W / 32;  // a lane's, at most
+      float2 q[kPairs];
+      float M = kLowest, S = 0.f;
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) {
+        q[i] = lane + 32 * i < C * W ? s.pair[par][lane + 32 * i] : make_float2(kLowest, 0.f);
+        M = fmaxf(M, q[i].x);
+      }
+      M = warp_max(M);
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) S += q[i].y * ex2((q[i].x - M) * a.c);
+      S = final_sum(warp_sum(S));
+      if (s.lost) S = NAN;
+      const float inverse = reciprocal(S);
+      const bool live = list.total != 0.f;
+      if (lane == 0) {
+        s.scale[par] = make_float2(M, list.by * inverse);
+        s.live[par] = live;
+      }
+      __syncwarp();
+      named_arrive(kScaled + par, NT + 32);
       const RowSplit sp = split_row(x + row * ld, cols);
       int from, to;
       slice(sp, from, to);
       T* dr = dx + row * ld_dx;
+      named_sync(kHeld + par, NT + 32);
       if (live) {
         const int lo = sp.head + from * VW, hi = sp.head + to * VW;
-        const float inverse = 1.f / st.y;
         T* held = reinterpret_cast<T*>(s.stage[stage]);
-        for (int j = lane; j < a.k; j += 32) {
-          const int id = l.id[j];
-          if (id < 0 || l.mass[j] == -1.f) continue;
+#pragma unroll
+        for (int i = 0; i < ListAhead::kEach; ++i) {
+          if (32 * i >= a.k) break;
+          const int id = list.id[i];
+          if (id < 0 || list.mass[i] == -1.f) continue;
           const bool single = id < sp.head || id >= sp.head + sp.nvec * VW;  // CTA 0's
           if (single ? rank != 0 : (id < lo || id >= hi)) continue;
-          const T g = Elem<T>::from_f(by * (ex2((l.z[j] - st.x) * a.c) * inverse - l.mass[j]));
+          const float q = ex2((Elem<T>::to_f(list.z[i]) - M) * a.c) * inverse;
+          const T g = Elem<T>::from_f(list.by * (q - list.mass[i]));
           if (single) {
             dr[id] = g;
           } else {
@@ -675,18 +715,17 @@ distill_grad_kernel(const T* __restrict__ x, int64_t ld, Taught a, const float* 
       }
       if (rank == 0) {
         float d = 0.f;
-        if (live) {
-          for (int j = lane; j < a.k; j += 32) {
-            if (l.id[j] < 0) continue;
-            const float e = exp2f(l.t2[j]);
-            if (e != 0.f) d += e * (l.t2[j] - (l.z[j] - st.x) * a.c);
-          }
+#pragma unroll
+        for (int i = 0; i < ListAhead::kEach; ++i) {
+          if (32 * i >= a.k) break;
+          if (live && list.id[i] >= 0 && list.e[i] != 0.f)
+            d += list.e[i] * (list.t2[i] - (Elem<T>::to_f(list.z[i]) - M) * a.c);
         }
         d = warp_sum(d);
         if (lane == 0) {
-          const float kl = live ? kLn2 * (d / total) + (logf(st.y) - logf(total)) : 0.f;
+          const float kl = live ? kLn2 * (d / list.total) + (logf(S) - logf(list.total)) : 0.f;
           loss[row] = a.tau * a.tau * kl;
-          stats[row] = live ? st : make_float2(0.f, 0.f);
+          stats[row] = live ? make_float2(M, S) : make_float2(0.f, 0.f);
         }
       }
       if (lane == 0) bulk_wait_read();
@@ -710,14 +749,13 @@ distill_grad_kernel(const T* __restrict__ x, int64_t ld, Taught a, const float* 
     int single = first < rows ? single_at(xr) : -1;
     float xs = single >= 0 ? Elem<T>::to_f(xr[single]) : -INFINITY;
     int par = 0, stage = 0;
-    uint32_t phase = 0, stage_phase = 0;
+    uint32_t stage_phase = 0;
     for (int64_t row = first; row < rows; row += step, xr += step * ld, dr += step * ld_dx) {
       const RowSplit sp = split_row(xr, cols);
       int from, to;
       slice(sp, from, to);
       const int left = to - from - tid;  // the thread's packs end here
       const bool whole = __all_sync(0xffffffffu, left > (P - 1) * NT);
-      if (tid == 0) bar_expect(&s.bar[par], C * W * 8);
       uint4* held = &s.stage[stage][0][tid];
       // values, then exponentials, in pairs
       uint64_t e[P][VW / 2];
@@ -752,22 +790,10 @@ distill_grad_kernel(const T* __restrict__ x, int64_t ld, Taught a, const float* 
       const int at_single = single;
       single = row + step < rows ? single_at(xr + step * ld) : -1;
       xs = single >= 0 ? Elem<T>::to_f((xr + step * ld)[single]) : -INFINITY;
-      named_sync(kListed + par, NT + 32);
-      const float by = s.by[par];
-      const bool live = s.total[par] != 0.f;
-      bar_wait(&s.bar[par], phase, &s.lost);
-      float M = kLowest, S = 0.f;
-      for (int i = lane; i < C * W; i += 32) M = fmaxf(M, s.pair[par][i].x);
-      M = warp_max(M);
-      for (int i = lane; i < C * W; i += 32) {
-        const float2 q = s.pair[par][i];
-        S += q.y * ex2((q.x - M) * a.c);
-      }
-      S = final_sum(warp_sum(S));
-      if (s.lost) S = NAN;
-      if (tid == 0) s.stat[par] = make_float2(M, S);
-      if (live) {
-        const float f = ex2((m - M) * a.c) * (by / S);
+      named_sync(kScaled + par, NT + 32);
+      if (s.live[par]) {
+        const float2 sc = s.scale[par];
+        const float f = ex2((m - sc.x) * a.c) * sc.y;
         const uint64_t f2 = f2_make(f, f);
         if (at_single >= 0) dr[at_single] = Elem<T>::from_f(es * f);
 #pragma unroll
@@ -779,7 +805,6 @@ distill_grad_kernel(const T* __restrict__ x, int64_t ld, Taught a, const float* 
       }
       bulk_fence();
       named_arrive(kHeld + par, NT + 32);
-      phase ^= par;
       par ^= 1;
       if (++stage == kStages) {
         stage = 0;
