@@ -338,7 +338,7 @@ distill_bwd_kernel(const float* __restrict__ dloss, int64_t dloss_stride, const 
 // lists ahead, put the gradients of the tokens they name in place, issue the
 // copies and in CTA 0 write the loss (a single one took longer over 64 entries
 // than the holders over a row).
-constexpr int kGradList = 256;       // teacher entries a row that this kernel takes
+constexpr int kGradList = 128;       // teacher entries a row that this kernel takes
 constexpr int kPacks = 8;            // 16-byte packs a thread holds
 constexpr int kStages = 3;
 constexpr int kMaxCluster = 16;
@@ -383,10 +383,34 @@ __device__ __forceinline__ float warp_max_nan(float v) {
   return r;
 }
 
-// A row's list on its way, kGradList / 32 entries a lane, as loaded: a value
+// An element's bits in a register of their own (a 16-bit register that a load
+// fills is copied at once, which waits for the load).
+template <typename T>
+__device__ __forceinline__ uint32_t load_bits(const T* p) {
+  if constexpr (sizeof(T) == 4) {
+    return __float_as_uint(*p);
+  } else {
+    return *reinterpret_cast<const unsigned short*>(p);
+  }
+}
+template <typename T>
+__device__ __forceinline__ float bits_value(uint32_t b) {
+  if constexpr (std::is_same<T, float>::value) {
+    return __uint_as_float(b);
+  } else if constexpr (std::is_same<T, __half>::value) {
+    return __half2float(__ushort_as_half((unsigned short)b));
+  } else {
+    return __uint_as_float(b << 16);
+  }
+}
+
+// A row's list on its way, E entries a lane, as loaded: a value
 // that is not touched until the next row's turn does not hold the warp up.
+// (For the same reason the loads are not conditional: lanes past the list
+// load its last entry.)
+template <int E>
 struct ListAhead {
-  static constexpr int kEach = kGradList / 32;
+  static constexpr int kEach = E;
   long long id[kEach];
   uint32_t t[kEach];
   float w;
@@ -396,28 +420,27 @@ struct ListAhead {
     const int lane = threadIdx.x & 31;
     w = 1.f;
     if (weight != nullptr) w = weight[row * weight_stride];
-    const int64_t at = row * a.ld_ids + lane, at_t = row * a.ld_t + lane;
+    const int64_t at = row * a.ld_ids, at_t = row * a.ld_t;
+    const auto each = [&](auto take) {
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        if (32 * i >= a.k) break;
+        take(i, min(lane + 32 * i, a.k - 1));
+      }
+    };
     if (a.ids_dtype == FL_B200_I64) {
       const long long* p = reinterpret_cast<const long long*>(a.ids) + at;
-#pragma unroll
-      for (int i = 0; i < kEach; ++i)
-        if (lane + 32 * i < a.k) id[i] = p[32 * i];
+      each([&](int i, int j) { id[i] = p[j]; });
     } else {
       const uint32_t* p = reinterpret_cast<const uint32_t*>(a.ids) + at;
-#pragma unroll
-      for (int i = 0; i < kEach; ++i)
-        if (lane + 32 * i < a.k) id[i] = p[32 * i];  // (zero-extended: negative ones end up past V)
+      each([&](int i, int j) { id[i] = p[j]; });  // (zero-extended: negative ones end up past V)
     }
     if (a.t_dtype == FL_B200_F32) {
-      const uint32_t* p = reinterpret_cast<const uint32_t*>(a.t) + at_t;
-#pragma unroll
-      for (int i = 0; i < kEach; ++i)
-        if (lane + 32 * i < a.k) t[i] = p[32 * i];
+      const float* p = reinterpret_cast<const float*>(a.t) + at_t;
+      each([&](int i, int j) { t[i] = load_bits(p + j); });
     } else {
-      const unsigned short* p = reinterpret_cast<const unsigned short*>(a.t) + at_t;
-#pragma unroll
-      for (int i = 0; i < kEach; ++i)
-        if (lane + 32 * i < a.k) t[i] = p[32 * i];
+      const __half* p = reinterpret_cast<const __half*>(a.t) + at_t;
+      each([&](int i, int j) { t[i] = load_bits(p + j); });
     }
   }
   __device__ __forceinline__ int token(int i, int k, int cols) const {  // -1: absent
@@ -425,9 +448,8 @@ struct ListAhead {
     return in ? (int)id[i] : -1;
   }
   __device__ __forceinline__ float logit(int i, int dtype) const {
-    if (dtype == FL_B200_F32) return __uint_as_float(t[i]);
-    if (dtype == FL_B200_BF16) return __uint_as_float(t[i] << 16);
-    return __half2float(__ushort_as_half((unsigned short)t[i]));
+    if (dtype == FL_B200_F32) return bits_value<float>(t[i]);
+    return dtype == FL_B200_BF16 ? bits_value<__nv_bfloat16>(t[i]) : bits_value<__half>(t[i]);
   }
 };
 
@@ -441,18 +463,18 @@ __device__ __forceinline__ float reciprocal(float x) {
 // A row's list in hand, spread over a warp as ListAhead is.  (Registers and
 // unrolled loops: what this warp does between a row's sums and its scale holds
 // up all the others, and a loop over shared memory took ten times as long.)
-template <typename T>
+template <typename T, int E>
 struct ListHeld {
-  static constexpr int kEach = ListAhead::kEach;
+  static constexpr int kEach = E;
   int id[kEach];      // -1: absent
-  T z[kEach];         // the logit, of entries in [lo, hi)
+  uint32_t z[kEach];  // the logit's bits, of entries in [lo, hi)
   float t2[kEach];    // (t - max t) c
   float e[kEach];     // 2^t2, 0 where absent
   float mass[kEach];  // as GradList's
   float total;        // of e; 0 when nothing is taught
   float by;           // w tau
 
-  __device__ __forceinline__ void set(const Taught& a, const ListAhead& in, const T* x, int cols, int lo,
+  __device__ __forceinline__ void set(const Taught& a, const ListAhead<E>& in, const T* x, int cols, int lo,
                                       int hi, GradList& l, uint32_t* marks) {
     const int lane = threadIdx.x & 31;
     by = in.w * a.tau;
@@ -461,7 +483,7 @@ struct ListHeld {
     for (int i = 0; i < kEach; ++i) {
       if (32 * i >= a.k) break;
       id[i] = in.token(i, a.k, cols);
-      if (id[i] >= lo && id[i] < hi) z[i] = x[id[i]];  // (not touched before the row is summed)
+      z[i] = load_bits(x + (id[i] >= lo && id[i] < hi ? id[i] : 0));  // (used once the row is summed)
     }
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
@@ -595,8 +617,9 @@ __device__ __forceinline__ uint4 from_pairs(const uint64_t (&e)[Elem<T>::kVec / 
   }
 }
 
-template <typename T, int NT, int MINB>
-__global__ void __launch_bounds__(NT + kHelpers, MINB)
+// E entries of a list a lane.
+template <typename T, int NT, int E>
+__global__ void __launch_bounds__(NT + kHelpers, NT == 256 ? 2 : NT == 128 ? 3 : 5)
 distill_grad_kernel(const T* __restrict__ x, int64_t ld, Taught a, const float* __restrict__ weight,
                     int64_t weight_stride, int64_t rows, int cols, float* __restrict__ loss,
                     float2* __restrict__ stats, T* __restrict__ dx, int64_t ld_dx) {
@@ -629,8 +652,8 @@ distill_grad_kernel(const T* __restrict__ x, int64_t ld, Taught a, const float* 
   if (warp >= W) {
     // every other row's list, and its copies
     const int par = warp - W;
-    ListAhead next;
-    ListHeld<T> list;
+    ListAhead<E> next;
+    ListHeld<T, E> list;
     const auto set = [&](int64_t row) {
       const T* xr = x + row * ld;
       const RowSplit sp = split_row(xr, cols);
@@ -691,19 +714,15 @@ distill_grad_kernel(const T* __restrict__ x, int64_t ld, Taught a, const float* 
         const int lo = sp.head + from * VW, hi = sp.head + to * VW;
         T* held = reinterpret_cast<T*>(s.stage[stage]);
 #pragma unroll
-        for (int i = 0; i < ListAhead::kEach; ++i) {
+        for (int i = 0; i < E; ++i) {
           if (32 * i >= a.k) break;
           const int id = list.id[i];
-          if (id < 0 || list.mass[i] == -1.f) continue;
-          const bool single = id < sp.head || id >= sp.head + sp.nvec * VW;  // CTA 0's
-          if (single ? rank != 0 : (id < lo || id >= hi)) continue;
-          const float q = ex2((Elem<T>::to_f(list.z[i]) - M) * a.c) * inverse;
+          const float q = ex2((bits_value<T>(list.z[i]) - M) * a.c) * inverse;
           const T g = Elem<T>::from_f(list.by * (q - list.mass[i]));
-          if (single) {
-            dr[id] = g;
-          } else {
-            held[id - lo] = g;
-          }
+          const bool mine = id >= 0 && list.mass[i] != -1.f;
+          if (mine && id >= lo && id < hi) held[id - lo] = g;
+          // the row's single elements are CTA 0's
+          if (mine && rank == 0 && (id < sp.head || id >= sp.head + sp.nvec * VW)) dr[id] = g;
         }
         bulk_fence();
         __syncwarp();
@@ -716,10 +735,10 @@ distill_grad_kernel(const T* __restrict__ x, int64_t ld, Taught a, const float* 
       if (rank == 0) {
         float d = 0.f;
 #pragma unroll
-        for (int i = 0; i < ListAhead::kEach; ++i) {
+        for (int i = 0; i < E; ++i) {
           if (32 * i >= a.k) break;
           if (live && list.id[i] >= 0 && list.e[i] != 0.f)
-            d += list.e[i] * (list.t2[i] - (Elem<T>::to_f(list.z[i]) - M) * a.c);
+            d += list.e[i] * (list.t2[i] - (bits_value<T>(list.z[i]) - M) * a.c);
         }
         d = warp_sum(d);
         if (lane == 0) {
@@ -880,7 +899,7 @@ int run_bwd(const float* dloss, int64_t dloss_stride, const void* x, int64_t ld,
 
 // Clusters of `cluster` CTAs of a kernel that are resident at once, asked for
 // once a device; 0 when the kernel cannot run so.
-template <typename T, int NT>
+template <typename T, int NT, int E>
 int grad_clusters(int cluster, cudaLaunchConfig_t cfg) {
   constexpr int kDevices = 64;
   static std::atomic<int> known[kDevices][kMaxCluster + 1];
@@ -888,9 +907,7 @@ int grad_clusters(int cluster, cudaLaunchConfig_t cfg) {
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kDevices) return 0;
   int n = known[dev][cluster].load(std::memory_order_relaxed);
   if (n == 0) {
-    if (cudaOccupancyMaxActiveClusters(&n, distill_grad_kernel<T, NT, NT == 256 ? 2 : NT == 128 ? 3 : 5>,
-                                       &cfg) != cudaSuccess)
-      n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, distill_grad_kernel<T, NT, E>, &cfg) != cudaSuccess) n = 0;
     (void)cudaGetLastError();
     known[dev][cluster].store(n > 0 ? n : -1, std::memory_order_relaxed);
   }
@@ -898,13 +915,13 @@ int grad_clusters(int cluster, cudaLaunchConfig_t cfg) {
 }
 
 // The one-pass kernel; returns -1 where it does not apply.
-template <typename T, int NT>
+template <typename T, int NT, int E>
 int run_grad(const void* x, int64_t ld, const Taught& a, const float* weight, int64_t weight_stride,
              int64_t rows, int64_t cols, float* loss, float* stats, void* dx, int64_t ld_dx,
              cudaStream_t stream) {
-  const auto kern = distill_grad_kernel<T, NT, NT == 256 ? 2 : NT == 128 ? 3 : 5>;
+  const auto kern = distill_grad_kernel<T, NT, E>;
   const int64_t cluster = ceil_div(cols, (int64_t)NT * kPacks * Elem<T>::kVec);
-  if (cluster > kMaxCluster || a.k > kGradList) return -1;
+  if (cluster > kMaxCluster) return -1;
   const size_t smem = sizeof(GradShared<NT>);
   // (per launch: the attributes are held per device)
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
@@ -924,7 +941,7 @@ int run_grad(const void* x, int64_t ld, const Taught& a, const float* weight, in
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const int clusters = grad_clusters<T, NT>((int)cluster, cfg);
+  const int clusters = grad_clusters<T, NT, E>((int)cluster, cfg);
   if (clusters == 0) return -1;
   return launch_cluster(kern, std::min<int64_t>(rows, clusters) * cluster, (int)cluster, NT + kHelpers, smem,
                         stream, reinterpret_cast<const T*>(x), ld, a, weight, weight_stride, rows,
@@ -1004,9 +1021,15 @@ FL_B200_API int fl_b200_distill_topk_grad(const void* logits, int64_t ld, const 
     st = dispatch_float(dtype, [&](auto t) {
       using T = decltype(t);
       const auto go = [&](auto threads) {
-        return run_grad<T, decltype(threads)::value>(logits, ld, a, row_weight, weight_stride, rows, cols,
-                                                     loss, stats, dlogits, ld_dlogits,
-                                                     (cudaStream_t)stream);
+        constexpr int NT = decltype(threads)::value;
+        const auto each = [&](auto entries) {
+          return run_grad<T, NT, decltype(entries)::value>(logits, ld, a, row_weight, weight_stride, rows,
+                                                           cols, loss, stats, dlogits, ld_dlogits,
+                                                           (cudaStream_t)stream);
+        };
+        if (k <= 64) return each(std::integral_constant<int, 2>{});
+        if (k <= 128) return each(std::integral_constant<int, 4>{});
+        return -1;
       };
       constexpr int kHold = kPacks * Elem<T>::kVec;  // elements a thread
       if (cols <= 64 * kHold) return go(std::integral_constant<int, 64>{});
