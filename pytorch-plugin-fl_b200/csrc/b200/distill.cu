@@ -26,9 +26,7 @@ namespace flb200 {
 namespace {
 
 constexpr int kMaxList = 1024;      // teacher entries a row
-constexpr int kStream = 512;        // threads that walk the row
-constexpr int kBlock = kStream + 32;  // and one warp for the teacher's list
-constexpr int kUnroll = 4;
+constexpr int kUnroll = 4;          // packs a thread loads before it uses one
 
 struct Taught {
   const void* t;
@@ -54,16 +52,33 @@ struct List {
 template <typename T>
 __device__ __forceinline__ void load_list(List& s, const Taught& a, const T* x, int64_t row, int cols,
                                           bool want_z) {
+  constexpr int U = 4;  // entries a lane whose loads are in flight together
   const int lane = threadIdx.x & 31;
   float top = -INFINITY;
-  for (int j = lane; j < a.k; j += 32) {
-    const int64_t id = load_index(a.ids, a.ids_dtype, row * a.ld_ids + j);
-    const bool in = id >= 0 && id < cols;
-    const float t = in ? load_float(a.t, a.t_dtype, row * a.ld_t + j) : -INFINITY;
-    s.id[j] = in ? (int)id : -1;
-    s.t2[j] = t;
-    if (want_z) s.z[j] = in ? Elem<T>::to_f(x[id]) : 0.f;
-    top = MaxOp::combine(top, t);
+  for (int j0 = lane; j0 < a.k; j0 += 32 * U) {
+    int64_t id[U];
+    float t[U];
+    T z[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int j = min(j0 + 32 * i, a.k - 1);
+      id[i] = load_index(a.ids, a.ids_dtype, row * a.ld_ids + j);
+      t[i] = load_float(a.t, a.t_dtype, row * a.ld_t + j);
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      if (id[i] < 0 || id[i] >= cols) id[i] = -1;
+      z[i] = x[want_z && id[i] >= 0 ? id[i] : 0];
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int j = j0 + 32 * i;
+      if (j >= a.k) break;
+      s.id[j] = (int)id[i];
+      s.t2[j] = id[i] >= 0 ? t[i] : -INFINITY;
+      s.z[j] = Elem<T>::to_f(z[i]);
+      top = MaxOp::combine(top, s.t2[j]);
+    }
   }
   top = group_reduce_warp<MaxOp, 32>(top);
   float total = 0.f;
@@ -130,244 +145,14 @@ __device__ __forceinline__ void fold(MaxSum& v, const float (&f)[N], float c) {
 // without a list.
 __device__ __forceinline__ float final_sum(float s) { return s == 0.f ? NAN : s; }
 
-// Loss and statistics.  One CTA a row, or a cluster of CTAs with a slice of
-// packs each when there are few rows.
-template <typename T>
-__global__ void __launch_bounds__(kBlock, 2)
-distill_fwd_kernel(const T* __restrict__ x, int64_t ld, Taught a, int cols,
-                   float* __restrict__ loss, float2* __restrict__ stats) {
-  constexpr int VW = Elem<T>::kVec;
-  __shared__ List list;
-  __shared__ float2 part[kStream / 32];
-  __shared__ float2 mine;
-  pdl_prologue();
-  const uint32_t rank = cluster_rank(), C = cluster_size();
-  const int64_t row = cluster_id();
-  const T* xr = x + row * ld;
-  const int tid = threadIdx.x;
-  if (tid >= kStream) {
-    if (rank == 0) load_list(list, a, xr, row, cols, true);
-  } else {
-    const RowSplit sp = split_row(xr, cols);
-    const uint4* body = reinterpret_cast<const uint4*>(xr + sp.head);
-    const int per = (sp.nvec + (int)C - 1) / (int)C;
-    const int end = min(sp.nvec, (int)(rank + 1) * per);
-    MaxSum v = {kLowest, 0.f};
-    if (rank == 0) {
-      const int e = single_of(sp, tid, VW);
-      if (e >= 0) {
-        const float f[1] = {Elem<T>::to_f(xr[e])};
-        fold<1>(v, f, a.c);
-      }
-    }
-    int p = (int)rank * per + tid;
-    for (; p + (kUnroll - 1) * kStream < end; p += kUnroll * kStream) {
-      uint4 u[kUnroll];
-#pragma unroll
-      for (int i = 0; i < kUnroll; ++i) u[i] = ld_stream(body + p + i * kStream);
-#pragma unroll
-      for (int i = 0; i < kUnroll; ++i) {
-        float f[VW];
-        unpack<T>(u[i], f);
-        fold<VW>(v, f, a.c);
-      }
-    }
-    for (; p < end; p += kStream) {
-      float f[VW];
-      unpack<T>(ld_stream(body + p), f);
-      fold<VW>(v, f, a.c);
-    }
-    v = warp_merge(v, a.c);
-    if ((tid & 31) == 0) part[tid >> 5] = make_float2(v.m, v.s);
-  }
-  __syncthreads();
-  if (tid >= kStream) {
-    const int lane = tid & 31;
-    const float2 q = lane < kStream / 32 ? part[lane] : make_float2(kLowest, 0.f);
-    MaxSum v = warp_merge({q.x, q.y}, a.c);
-    if (lane == 0) mine = make_float2(v.m, v.s);
-  }
-  if (C > 1) cluster_sync_all();
-  if (tid >= kStream && rank == 0) {
-    const int lane = tid & 31;
-    __syncwarp();
-    float2 q = make_float2(kLowest, 0.f);
-    if (lane < (int)C) q = C > 1 ? ld_remote_f2(remote_smem(&mine, lane)) : mine;
-    const MaxSum v = warp_merge({q.x, q.y}, a.c);
-    const bool live = list.total != 0.f;
-    const float sum = final_sum(v.s);
-    const float kl = live ? list_kl(list, a, v.m, sum) : 0.f;
-    if (lane == 0) {
-      loss[row] = a.tau * a.tau * kl;
-      stats[row] = live ? make_float2(v.m, sum) : make_float2(0.f, 0.f);
-    }
-  }
-  if (C > 1) cluster_sync_all();  // no CTA leaves while rank 0 may read its pair
-}
-
-// sum of p over the entries of the list that name entry j's token, and
-// whether j is the first of them (which writes the token's gradient).
-__device__ __forceinline__ bool token_mass(const List& s, int k, int j, float& mass) {
-  const int id = s.id[j];
-  float m = 0.f;
-  for (int i = 0; i < k; ++i) {
-    if (s.id[i] != id) continue;
-    if (i < j) return false;
-    m += exp2f(s.t2[i]);
-  }
-  mass = m / s.total;
-  return true;
-}
-
-// Gradients of both operands from the forward's statistics: q w tau streamed
-// over a chunk of the row, then the tokens of the teacher's list that lie in
-// it written again, whole, from fp32.
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(kBlock, 2)
-distill_bwd_kernel(const float* __restrict__ dloss, int64_t dloss_stride, const T* __restrict__ x,
-                   int64_t ld, const float2* __restrict__ stats, Taught a, int cols, int chunk,
-                   int chunks, T* __restrict__ dx, int64_t ld_dx, void* __restrict__ dt) {
-  constexpr int VW = Elem<T>::kVec;
-  __shared__ List list;
-  pdl_prologue();
-  const int64_t row = blockIdx.x / (unsigned)chunks;
-  const int part = (int)(blockIdx.x % (unsigned)chunks);
-  const T* xr = x + row * ld;
-  const int tid = threadIdx.x;
-  const float2 st = stats[row];
-  const bool live = st.y != 0.f;
-  const float gt = (dloss != nullptr ? dloss[row * dloss_stride] : 1.f) * a.tau;
-  const float f = gt / st.y;
-  const int from = part * chunk, to = min(cols, from + chunk);  // elements
-  if (tid >= kStream) {
-    if (live) {
-      const bool want = dt != nullptr && part == 0;
-      load_list(list, a, xr, row, cols, want);
-      if (want) {
-        const float kl = list_kl(list, a, st.x, st.y);
-        const float lse = logf(st.y), lt = logf(list.total);
-        for (int j = tid & 31; j < a.k; j += 32) {
-          float g = 0.f;
-          if (list.id[j] >= 0) {
-            const float e = exp2f(list.t2[j]);
-            if (e != 0.f) {
-              const float gap = kLn2 * (list.t2[j] - (list.z[j] - st.x) * a.c) + (lse - lt);
-              g = gt * (e / list.total) * (gap - kl);
-            }
-          }
-          store_float(dt, a.t_dtype, row * a.k + j, g);
-        }
-      }
-    } else if (dt != nullptr && part == 0) {
-      for (int j = tid & 31; j < a.k; j += 32) store_float(dt, a.t_dtype, row * a.k + j, 0.f);
-    }
-  } else if (dx != nullptr) {
-    T* dr = dx + row * ld_dx;
-    const auto grad = [&](float z) { return live ? ex2((z - st.x) * a.c) * f : 0.f; };
-    if constexpr (VEC) {
-      const RowSplit sp = split_row(xr, cols);
-      const uint4* body = reinterpret_cast<const uint4*>(xr + sp.head);
-      uint4* out = reinterpret_cast<uint4*>(dr + sp.head);
-      // pack p belongs to the chunk that holds element p * VW
-      const int p1 = part == chunks - 1 ? sp.nvec : min(sp.nvec, to / VW);
-      if (part == 0) {
-        const int e = single_of(sp, tid, VW);
-        if (e >= 0) dr[e] = Elem<T>::from_f(live ? grad(Elem<T>::to_f(xr[e])) : 0.f);
-      }
-      for (int p = from / VW + tid; p < p1; p += kUnroll * kStream) {
-        uint4 u[kUnroll];
-#pragma unroll
-        for (int i = 0; i < kUnroll; ++i)
-          if (live && p + i * kStream < p1) u[i] = ld_stream(body + p + i * kStream);
-#pragma unroll
-        for (int i = 0; i < kUnroll; ++i) {
-          if (p + i * kStream >= p1) break;
-          float v[VW];
-          if (live) unpack<T>(u[i], v);
-#pragma unroll
-          for (int j = 0; j < VW; ++j) v[j] = grad(v[j]);
-          st_stream(out + p + i * kStream, pack<T>(v));
-        }
-      }
-    } else {
-      for (int e = from + tid; e < to; e += kStream)
-        dr[e] = Elem<T>::from_f(live ? grad(Elem<T>::to_f(xr[e])) : 0.f);
-    }
-  }
-  if (!live || dx == nullptr) return;  // (the whole CTA)
-  __syncthreads();
-  // chunk 0 writes the row's single elements, the others only whole packs;
-  // here every chunk takes the tokens whose element it wrote
-  int first = from, last = to;
-  int single_lo = 0, single_hi = 0;  // [0, single_lo) and [single_hi, cols) belong to chunk 0
-  if constexpr (VEC) {
-    const RowSplit sp = split_row(xr, cols);
-    const int p1 = part == chunks - 1 ? sp.nvec : min(sp.nvec, to / VW);
-    first = sp.head + from / VW * VW;
-    last = sp.head + p1 * VW;
-    single_lo = sp.head;
-    single_hi = sp.head + sp.nvec * VW;
-  }
-  T* dr = dx + row * ld_dx;
-  for (int j = tid; j < a.k; j += kBlock) {
-    const int id = list.id[j];
-    if (id < 0) continue;
-    bool here = id >= first && id < last;
-    if constexpr (VEC) here = (id < single_lo || id >= single_hi) ? part == 0 : here;
-    float mass;
-    if (!here || !token_mass(list, a.k, j, mass)) continue;
-    const float q = ex2((Elem<T>::to_f(xr[id]) - st.x) * a.c) / st.y;
-    dr[id] = Elem<T>::from_f(gt * (q - mass));
-  }
-}
-
-// ---------------------------------------------- loss and gradient at once ---
-//
-// One read of the logits and one write of the gradient: a cluster holds a row
-// on chip, 128 bytes of logits a thread, as exponentials 2^((z - m_w) c)
-// against the warp's own maximum.  Every warp sends its (m_w, sum) to every
-// CTA of the cluster (st.async on a transaction barrier: no fence, no second
-// hop through a CTA total), where one warp folds all pairs to (M, S); the
-// others then write w tau e 2^((m_w - M) c) / S over the logits in shared
-// memory.  Three
-// stages of a row's slice take turns: one arriving, one in hand, one leaving,
-// each by one bulk copy, so that neither memory direction holds up the warps
-// (stores from registers did: a third of a row's time was theirs).
-//
-// That warp is one of two more, a row each in turn, which read the teacher's
-// lists ahead, put the gradients of the tokens they name in place, issue the
-// copies and in CTA 0 write the loss (a single one took longer over 64 entries
-// than the holders over a row).
-constexpr int kGradList = 128;       // teacher entries a row that this kernel takes
-constexpr int kPacks = 8;            // 16-byte packs a thread holds
-constexpr int kStages = 3;
-constexpr int kMaxCluster = 16;
-constexpr int kMarkBits = 8192;      // marks of the tokens named so far, by id modulo this
+constexpr int kGradList = 128;  // the longest list that a warp holds in registers
+constexpr int kMarkBits = 8192;  // marks of the tokens named so far, by id modulo this
 
 // A list's tokens and masses, for the search after repeated ones.
 struct GradList {
   int id[kGradList];      // -1: absent
   float mass[kGradList];  // sum of p over the entries with this id; -1 but at the first of them
 };
-
-template <int NT>
-struct GradShared {
-  uint4 stage[kStages][kPacks][NT];
-  float2 pair[2][kMaxCluster * (NT / 32)];
-  GradList list[2];
-  uint32_t marks[2][kMarkBits / 32];
-  float2 scale[2];  // the row's M, and w tau / S
-  int live[2];      // whether anything is taught
-  uint64_t bar[2];          // the row's pairs have come
-  uint64_t full[kStages];   // the stage's logits have come
-  int lost;
-};
-
-constexpr int kHelpers = 64;  // threads besides the NT that hold the row
-// Named barriers, two of each for alternate rows: a barrier's next use follows,
-// through the other kind, every wait on this one.
-constexpr int kScaled = 1;  // the row's scale is known: the holders wait for the list's warp
-constexpr int kHeld = 3;    // the gradient is in place: the list's warp waits for the holders
 
 // Warp-wide maximum; NaN only if every lane has one.
 __device__ __forceinline__ float warp_max(float v) {
@@ -617,6 +402,313 @@ __device__ __forceinline__ uint4 from_pairs(const uint64_t (&e)[Elem<T>::kVec / 
   }
 }
 
+// A row's list as the two-kernel path uses it: held by the last warp of the
+// CTA, E entries a lane, or in shared memory (E = 0: any length up to
+// kMaxList).
+template <typename T, int E>
+struct ListOf {
+  struct Shared {
+    GradList list;
+    uint32_t marks[kMarkBits / 32];
+  };
+  ListHeld<T, E> held;
+  float total;
+
+  __device__ __forceinline__ void load(Shared& s, const Taught& a, const float*, int64_t, const T* x,
+                                       int64_t row, int cols, int lo, int hi) {
+    ListAhead<E> in;
+    in.load(a, nullptr, 0, row);
+    for (int i = threadIdx.x & 31; i < kMarkBits / 32; i += 32) s.marks[i] = 0;
+    __syncwarp();
+    held.set(a, in, x, cols, lo, hi, s.list, s.marks);
+    total = held.total;
+  }
+  // sum of p_j ((t_j - max t) - (z_j - m)) / tau, by the warp
+  __device__ __forceinline__ float kl(Shared&, const Taught& a, float m, float sum) const {
+    float d = 0.f;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      if (32 * i >= a.k) break;
+      if (held.id[i] >= 0 && held.e[i] != 0.f)
+        d += held.e[i] * (held.t2[i] - (bits_value<T>(held.z[i]) - m) * a.c);
+    }
+    d = warp_sum(d);
+    return kLn2 * (d / total) + (logf(sum) - logf(total));
+  }
+  __device__ __forceinline__ void teacher(Shared& s, const Taught& a, float m, float sum, float gt,
+                                          void* dt, int64_t row) const {
+    const float all = kl(s, a, m, sum), logs = logf(sum) - logf(total);
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const int j = (int)(threadIdx.x & 31) + 32 * i;
+      if (j >= a.k) break;
+      float g = 0.f;
+      if (held.id[i] >= 0 && held.e[i] != 0.f) {
+        const float gap = kLn2 * (held.t2[i] - (bits_value<T>(held.z[i]) - m) * a.c) + logs;
+        g = gt * (held.e[i] / total) * (gap - all);
+      }
+      store_float(dt, a.t_dtype, row * a.k + j, g);
+    }
+  }
+  // Calls put(id, z, mass) once for every token of the list, by the warp.
+  template <typename F>
+  __device__ __forceinline__ void tokens(Shared&, const Taught& a, const T*, int warp_from, F put) const {
+    if ((int)threadIdx.x < warp_from) return;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      if (32 * i >= a.k) break;
+      if (held.id[i] >= 0 && held.mass[i] != -1.f)
+        put(held.id[i], bits_value<T>(held.z[i]), held.mass[i]);
+    }
+  }
+};
+
+template <typename T>
+struct ListOf<T, 0> {
+  using Shared = List;
+  float total;
+
+  __device__ __forceinline__ void load(Shared& s, const Taught& a, const float*, int64_t, const T* x,
+                                       int64_t row, int cols, int, int) {
+    load_list(s, a, x, row, cols, true);
+    total = s.total;
+  }
+  __device__ __forceinline__ float kl(Shared& s, const Taught& a, float m, float sum) const {
+    return list_kl(s, a, m, sum);
+  }
+  __device__ __forceinline__ void teacher(Shared& s, const Taught& a, float m, float sum, float gt,
+                                          void* dt, int64_t row) const {
+    const float all = list_kl(s, a, m, sum), logs = logf(sum) - logf(total);
+    for (int j = threadIdx.x & 31; j < a.k; j += 32) {
+      float g = 0.f;
+      const float e = s.id[j] >= 0 ? exp2f(s.t2[j]) : 0.f;
+      if (e != 0.f) {
+        const float gap = kLn2 * (s.t2[j] - (s.z[j] - m) * a.c) + logs;
+        g = gt * (e / total) * (gap - all);
+      }
+      store_float(dt, a.t_dtype, row * a.k + j, g);
+    }
+  }
+  // By the whole CTA: for each entry the list is searched, the first entry of
+  // an id calls for all.
+  template <typename F>
+  __device__ __forceinline__ void tokens(Shared& s, const Taught& a, const T*, int, F put) const {
+    for (int j = threadIdx.x; j < a.k; j += blockDim.x) {
+      const int id = s.id[j];
+      if (id < 0) continue;
+      float mass = 0.f;
+      bool first = true;
+      for (int i = 0; i < a.k && first; ++i) {
+        if (s.id[i] != id) continue;
+        first = i >= j;
+        mass += exp2f(s.t2[i]);
+      }
+      if (first) put(id, s.z[j], mass / s.total);
+    }
+  }
+};
+
+// Loss and statistics.  One CTA a row, or a cluster of CTAs with a slice of
+// packs each when there are few rows.
+template <typename T, int NS, int E>
+__global__ void __launch_bounds__(NS + 32, 1024 / NS)
+distill_fwd_kernel(const T* __restrict__ x, int64_t ld, Taught a, int cols,
+                   float* __restrict__ loss, float2* __restrict__ stats) {
+  constexpr int VW = Elem<T>::kVec;
+  __shared__ typename ListOf<T, E>::Shared shared;
+  ListOf<T, E> list;
+  __shared__ float2 part[NS / 32];
+  __shared__ float2 mine;
+  pdl_prologue();
+  const uint32_t rank = cluster_rank(), C = cluster_size();
+  const int64_t row = cluster_id();
+  const T* xr = x + row * ld;
+  const int tid = threadIdx.x;
+  if (tid >= NS) {
+    if (rank == 0) list.load(shared, a, nullptr, 0, xr, row, cols, 0, cols);
+  } else {
+    const RowSplit sp = split_row(xr, cols);
+    const uint4* body = reinterpret_cast<const uint4*>(xr + sp.head);
+    const int per = (sp.nvec + (int)C - 1) / (int)C;
+    const int end = min(sp.nvec, (int)(rank + 1) * per);
+    MaxSum v = {kLowest, 0.f};
+    if (rank == 0) {
+      const int e = single_of(sp, tid, VW);
+      if (e >= 0) {
+        const float f[1] = {Elem<T>::to_f(xr[e])};
+        fold<1>(v, f, a.c);
+      }
+    }
+    int p = (int)rank * per + tid;
+    for (; p + (kUnroll - 1) * NS < end; p += kUnroll * NS) {
+      uint4 u[kUnroll];
+#pragma unroll
+      for (int i = 0; i < kUnroll; ++i) u[i] = ld_stream(body + p + i * NS);
+#pragma unroll
+      for (int i = 0; i < kUnroll; ++i) {
+        float f[VW];
+        unpack<T>(u[i], f);
+        fold<VW>(v, f, a.c);
+      }
+    }
+    for (; p < end; p += NS) {
+      float f[VW];
+      unpack<T>(ld_stream(body + p), f);
+      fold<VW>(v, f, a.c);
+    }
+    v = warp_merge(v, a.c);
+    if ((tid & 31) == 0) part[tid >> 5] = make_float2(v.m, v.s);
+  }
+  __syncthreads();
+  if (tid >= NS) {
+    const int lane = tid & 31;
+    const float2 q = lane < NS / 32 ? part[lane] : make_float2(kLowest, 0.f);
+    MaxSum v = warp_merge({q.x, q.y}, a.c);
+    if (lane == 0) mine = make_float2(v.m, v.s);
+  }
+  if (C > 1) cluster_sync_all();
+  if (tid >= NS && rank == 0) {
+    const int lane = tid & 31;
+    __syncwarp();
+    float2 q = make_float2(kLowest, 0.f);
+    if (lane < (int)C) q = C > 1 ? ld_remote_f2(remote_smem(&mine, lane)) : mine;
+    const MaxSum v = warp_merge({q.x, q.y}, a.c);
+    const bool live = list.total != 0.f;
+    const float sum = final_sum(v.s);
+    const float kl = live ? list.kl(shared, a, v.m, sum) : 0.f;
+    if (lane == 0) {
+      loss[row] = a.tau * a.tau * kl;
+      stats[row] = live ? make_float2(v.m, sum) : make_float2(0.f, 0.f);
+    }
+  }
+  if (C > 1) cluster_sync_all();  // no CTA leaves while rank 0 may read its pair
+}
+
+// Gradients of both operands from the forward's statistics: q w tau streamed
+// over a chunk of the row, then the tokens of the teacher's list that lie in
+// it written again, whole, from fp32.
+template <typename T, bool VEC, int NS, int E>
+__global__ void __launch_bounds__(NS + 32, 1024 / NS)
+distill_bwd_kernel(const float* __restrict__ dloss, int64_t dloss_stride, const T* __restrict__ x,
+                   int64_t ld, const float2* __restrict__ stats, Taught a, int cols, int chunk,
+                   int chunks, T* __restrict__ dx, int64_t ld_dx, void* __restrict__ dt) {
+  constexpr int VW = Elem<T>::kVec;
+  __shared__ typename ListOf<T, E>::Shared shared;
+  ListOf<T, E> list;
+  pdl_prologue();
+  const int64_t row = blockIdx.x / (unsigned)chunks;
+  const int part = (int)(blockIdx.x % (unsigned)chunks);
+  const T* xr = x + row * ld;
+  T* dr = dx + row * ld_dx;
+  const int tid = threadIdx.x;
+  const float2 st = stats[row];
+  const bool live = st.y != 0.f;
+  const float gt = (dloss != nullptr ? dloss[row * dloss_stride] : 1.f) * a.tau;
+  const float f = gt / st.y;
+  // elements [from, to); whole packs where VEC: pack p belongs to the chunk
+  // that holds element p * VW, and the row's single elements to chunk 0
+  const int from = part * chunk, to = min(cols, from + chunk);
+  const RowSplit sp = split_row(xr, cols);
+  const int p0 = min(sp.nvec, from / VW), p1 = part == chunks - 1 ? sp.nvec : min(sp.nvec, to / VW);
+  const int lo = VEC ? sp.head + p0 * VW : from, hi = VEC ? sp.head + p1 * VW : to;
+  const bool want_dt = dt != nullptr && part == 0;
+  if (tid >= NS) {
+    if (live)
+      list.load(shared, a, nullptr, 0, xr, row, cols, part == 0 ? 0 : lo, part == 0 ? cols : hi);
+    if (want_dt) {
+      if (live) {
+        list.teacher(shared, a, st.x, st.y, gt, dt, row);
+      } else {
+        for (int j = tid - NS; j < a.k; j += 32) store_float(dt, a.t_dtype, row * a.k + j, 0.f);
+      }
+    }
+  } else if (dx != nullptr) {
+    const auto grad = [&](float z) { return live ? ex2((z - st.x) * a.c) * f : 0.f; };
+    if constexpr (VEC) {
+      const uint4* body = reinterpret_cast<const uint4*>(xr + sp.head);
+      uint4* out = reinterpret_cast<uint4*>(dr + sp.head);
+      if (part == 0) {
+        const int e = single_of(sp, tid, VW);
+        if (e >= 0) dr[e] = Elem<T>::from_f(live ? grad(Elem<T>::to_f(xr[e])) : 0.f);
+      }
+      if (live) {
+        const uint64_t minus = f2_make(-st.x, -st.x), c2 = f2_make(a.c, a.c), f2 = f2_make(f, f);
+        for (int p = p0 + tid; p < p1; p += kUnroll * NS) {
+          uint4 u[kUnroll];
+#pragma unroll
+          for (int i = 0; i < kUnroll; ++i)
+            if (p + i * NS < p1) u[i] = ld_stream(body + p + i * NS);
+#pragma unroll
+          for (int i = 0; i < kUnroll; ++i) {
+            if (p + i * NS >= p1) break;
+            uint64_t e[VW / 2];
+            to_pairs<T>(u[i], e);
+#pragma unroll
+            for (int j = 0; j < VW / 2; ++j) {
+              const uint64_t d = f2_mul(f2_add(e[j], minus), c2);
+              e[j] = f2_make(ex2(f2_lo(d)), ex2(f2_hi(d)));
+            }
+            st_stream(out + p + i * NS, from_pairs<T>(e, f2));
+          }
+        }
+      } else {
+        for (int p = p0 + tid; p < p1; p += NS) st_stream(out + p, make_uint4(0, 0, 0, 0));
+      }
+    } else {
+      for (int e = from + tid; e < to; e += NS)
+        dr[e] = Elem<T>::from_f(live ? grad(Elem<T>::to_f(xr[e])) : 0.f);
+    }
+  }
+  if (!live || dx == nullptr) return;  // (the whole CTA)
+  __syncthreads();                     // the chunk is stored
+  const auto put = [&](int id, float z, float mass) {
+    const bool single = VEC && (id < sp.head || id >= sp.head + sp.nvec * VW);
+    if (single ? part == 0 : (id >= lo && id < hi))
+      dr[id] = Elem<T>::from_f(gt * (ex2((z - st.x) * a.c) * reciprocal(st.y) - mass));
+  };
+  list.tokens(shared, a, xr, NS, put);
+}
+
+// ---------------------------------------------- loss and gradient at once ---
+//
+// One read of the logits and one write of the gradient: a cluster holds a row
+// on chip, 128 bytes of logits a thread, as exponentials 2^((z - m_w) c)
+// against the warp's own maximum.  Every warp sends its (m_w, sum) to every
+// CTA of the cluster (st.async on a transaction barrier: no fence, no second
+// hop through a CTA total), where one warp folds all pairs to (M, S); the
+// others then write w tau e 2^((m_w - M) c) / S over the logits in shared
+// memory.  Three
+// stages of a row's slice take turns: one arriving, one in hand, one leaving,
+// each by one bulk copy, so that neither memory direction holds up the warps
+// (stores from registers did: a third of a row's time was theirs).
+//
+// That warp is one of two more, a row each in turn, which read the teacher's
+// lists ahead, put the gradients of the tokens they name in place, issue the
+// copies and in CTA 0 write the loss (a single one took longer over 64 entries
+// than the holders over a row).
+constexpr int kPacks = 8;            // 16-byte packs a thread holds
+constexpr int kStages = 3;
+constexpr int kMaxCluster = 16;
+
+template <int NT>
+struct GradShared {
+  uint4 stage[kStages][kPacks][NT];
+  float2 pair[2][kMaxCluster * (NT / 32)];
+  GradList list[2];
+  uint32_t marks[2][kMarkBits / 32];
+  float2 scale[2];  // the row's M, and w tau / S
+  int live[2];      // whether anything is taught
+  uint64_t bar[2];          // the row's pairs have come
+  uint64_t full[kStages];   // the stage's logits have come
+  int lost;
+};
+
+constexpr int kHelpers = 64;  // threads besides the NT that hold the row
+// Named barriers, two of each for alternate rows: a barrier's next use follows,
+// through the other kind, every wait on this one.
+constexpr int kScaled = 1;  // the row's scale is known: the holders wait for the list's warp
+constexpr int kHeld = 3;    // the gradient is in place: the list's warp waits for the holders
+
 // E entries of a list a lane.
 template <typename T, int NT, int E>
 __global__ void __launch_bounds__(NT + kHelpers, NT == 256 ? 2 : NT == 128 ? 3 : 5)
@@ -861,40 +953,62 @@ bool same_phase(const void* x, int64_t ld, const void* y, int64_t ld_y, int64_t 
          (ld - ld_y) * size % 16 == 0;
 }
 
+// Calls go(NS, E): the threads that stream a row (and one warp more for its
+// list) and the list's entries a lane.  Rows of up to 16 KB go to CTAs of 128
+// threads, of which more are resident to hide the lists' latency (at 4096
+// bf16 columns: 3 times as fast as 512).
+template <typename T, typename F>
+int with_geometry(int64_t cols, int64_t k, F&& go) {
+  using Small = std::integral_constant<int, 128>;
+  using Large = std::integral_constant<int, 512>;
+  using Held = std::integral_constant<int, 2>;
+  using Any = std::integral_constant<int, 0>;
+  if (cols * (int64_t)sizeof(T) <= 16384) return k <= 64 && k > 0 ? go(Small{}, Held{}) : go(Small{}, Any{});
+  return k <= 64 && k > 0 ? go(Large{}, Held{}) : go(Large{}, Any{});
+}
+
 template <typename T>
 int run_fwd(const void* x, int64_t ld, const Taught& a, int64_t rows, int64_t cols, float* loss,
             float* stats, cudaStream_t stream) {
   DeviceInfo dev;
   const int st = current_device_info(&dev);
   if (st != FL_B200_OK) return st;
-  int cluster = 1;
-  while (cluster < 8 && rows * cluster < 2 * dev.sm_count &&
-         cols / (cluster * 2) >= kStream * Elem<T>::kVec)
-    cluster *= 2;
-  return launch_cluster(distill_fwd_kernel<T>, rows * cluster, cluster, kBlock, 0, stream,
-                        reinterpret_cast<const T*>(x), ld, a, (int)cols, loss,
-                        reinterpret_cast<float2*>(stats));
+  return with_geometry<T>(cols, a.k, [&](auto ns, auto e) {
+    constexpr int NS = decltype(ns)::value;
+    int cluster = 1;
+    while (cluster < 8 && rows * cluster < 2 * dev.sm_count && cols / (cluster * 2) >= NS * Elem<T>::kVec)
+      cluster *= 2;
+    return launch_cluster(distill_fwd_kernel<T, NS, decltype(e)::value>, rows * cluster, cluster, NS + 32,
+                          0, stream, reinterpret_cast<const T*>(x), ld, a, (int)cols, loss,
+                          reinterpret_cast<float2*>(stats));
+  });
 }
 
 template <typename T>
 int run_bwd(const float* dloss, int64_t dloss_stride, const void* x, int64_t ld, const float* stats,
             const Taught& a, int64_t rows, int64_t cols, void* dx, int64_t ld_dx, void* dt,
             cudaStream_t stream) {
+  DeviceInfo dev;
+  const int st = current_device_info(&dev);
+  if (st != FL_B200_OK) return st;
   const bool vec = dx == nullptr || same_phase(x, ld, dx, ld_dx, sizeof(T));
-  int chunks = 1;
-  int64_t chunk = cols;
-  if (dx != nullptr) {
-    chunk = (int64_t)kStream * kUnroll * Elem<T>::kVec;
-    chunks = (int)ceil_div(cols, chunk);
-  }
-  if (rows * chunks > 0x7fffffffLL) return FL_B200_ERR_TOO_LARGE;
-  const auto go = [&](auto kern) {
-    launch_k(kern, dim3((unsigned)(rows * chunks)), dim3(kBlock), 0, stream, dloss, dloss_stride,
-             reinterpret_cast<const T*>(x), ld, reinterpret_cast<const float2*>(stats), a, (int)cols,
-             (int)chunk, chunks, reinterpret_cast<T*>(dx), ld_dx, dt);
-    return launch_status();
-  };
-  return vec ? go(distill_bwd_kernel<T, true>) : go(distill_bwd_kernel<T, false>);
+  return with_geometry<T>(cols, a.k, [&](auto ns, auto e) {
+    constexpr int NS = decltype(ns)::value, E = decltype(e)::value;
+    // chunks of 4 rounds of loads, which hide the list's latency (2048 x 128256
+    // bf16: 201 us, 249 us with one round); shorter where rows are few
+    const int64_t round = (int64_t)NS * kUnroll * Elem<T>::kVec;
+    int64_t chunk = dx == nullptr ? cols : 4 * round;
+    while (chunk > round && rows * ceil_div(cols, chunk) < 4 * dev.sm_count) chunk /= 2;
+    const int64_t chunks = ceil_div(cols, chunk);
+    if (rows * chunks > 0x7fffffffLL) return (int)FL_B200_ERR_TOO_LARGE;
+    const auto go = [&](auto kern) {
+      launch_k(kern, dim3((unsigned)(rows * chunks)), dim3(NS + 32), 0, stream, dloss, dloss_stride,
+               reinterpret_cast<const T*>(x), ld, reinterpret_cast<const float2*>(stats), a, (int)cols,
+               (int)chunk, (int)chunks, reinterpret_cast<T*>(dx), ld_dx, dt);
+      return launch_status();
+    };
+    return vec ? go(distill_bwd_kernel<T, true, NS, E>) : go(distill_bwd_kernel<T, false, NS, E>);
+  });
 }
 
 // Clusters of `cluster` CTAs of a kernel that are resident at once, asked for
