@@ -124,20 +124,10 @@ __device__ __forceinline__ MaxSum warp_merge(MaxSum v, float c) {
   return v;
 }
 
-// Folds N values into v.
-template <int N>
-__device__ __forceinline__ void fold(MaxSum& v, const float (&f)[N], float c) {
-  float top = f[0];
-#pragma unroll
-  for (int i = 1; i < N; ++i) top = fmaxf(top, f[i]);
-  if (top > v.m) {
-    v.s *= ex2((v.m - top) * c);
-    v.m = top;
-  }
-  float s = 0.f;
-#pragma unroll
-  for (int i = 0; i < N; ++i) s += ex2((f[i] - v.m) * c);
-  v.s += s;
+// Folds one value into v.
+__device__ __forceinline__ void fold(MaxSum& v, float f, float c) {
+  const float m = fmaxf(v.m, f);
+  v = {m, v.s * ex2((v.m - m) * c) + ex2((f - m) * c)};
 }
 
 // A row's statistics are final once S is not 0: a row of -inf alone, whose
@@ -372,7 +362,7 @@ __device__ __forceinline__ float pack_max(const uint4& u) {
 }
 // A word of -infinities.
 template <typename T>
-__device__ __forceinline__ uint32_t lowest_word() {
+__device__ __forceinline__ constexpr uint32_t lowest_word() {
   return std::is_same<T, float>::value ? 0xff800000u
          : std::is_same<T, __half>::value ? 0xfc00fc00u
                                           : 0xff80ff80u;
@@ -400,6 +390,32 @@ __device__ __forceinline__ uint4 from_pairs(const uint64_t (&e)[Elem<T>::kVec / 
     return make_uint4(pair_to_bits<T>(f2_mul(e[0], f)), pair_to_bits<T>(f2_mul(e[1], f)),
                       pair_to_bits<T>(f2_mul(e[2], f)), pair_to_bits<T>(f2_mul(e[3], f)));
   }
+}
+
+// Folds N packs into v, the exponentials in fp32 pairs.
+template <typename T, int N>
+__device__ __forceinline__ void fold_packs(MaxSum& v, const uint4 (&u)[N], float c) {
+  constexpr int VW = Elem<T>::kVec;
+  float top = pack_max<T>(u[0]);
+#pragma unroll
+  for (int i = 1; i < N; ++i) top = fmaxf(top, pack_max<T>(u[i]));
+  if (top > v.m) {
+    v.s *= ex2((v.m - top) * c);
+    v.m = top;
+  }
+  const uint64_t minus = f2_make(-v.m, -v.m), c2 = f2_make(c, c);
+  uint64_t sum = 0;  // (two zeros)
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    uint64_t e[VW / 2];
+    to_pairs<T>(u[i], e);
+#pragma unroll
+    for (int j = 0; j < VW / 2; ++j) {
+      const uint64_t d = f2_mul(f2_add(e[j], minus), c2);
+      sum = f2_add(sum, f2_make(ex2(f2_lo(d)), ex2(f2_hi(d))));
+    }
+  }
+  v.s += f2_lo(sum) + f2_hi(sum);
 }
 
 // A row's list as the two-kernel path uses it: held by the last warp of the
@@ -534,27 +550,22 @@ distill_fwd_kernel(const T* __restrict__ x, int64_t ld, Taught a, int cols,
     MaxSum v = {kLowest, 0.f};
     if (rank == 0) {
       const int e = single_of(sp, tid, VW);
-      if (e >= 0) {
-        const float f[1] = {Elem<T>::to_f(xr[e])};
-        fold<1>(v, f, a.c);
-      }
+      if (e >= 0) fold(v, Elem<T>::to_f(xr[e]), a.c);
     }
     int p = (int)rank * per + tid;
-    for (; p + (kUnroll - 1) * NS < end; p += kUnroll * NS) {
+    for (; p + 7 * NS < end; p += 8 * NS) {
+      uint4 u[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) u[i] = ld_stream(body + p + i * NS);
+      fold_packs<T, 8>(v, u, a.c);
+    }
+    constexpr uint32_t none = lowest_word<T>();
+    for (; p < end; p += kUnroll * NS) {
       uint4 u[kUnroll];
 #pragma unroll
-      for (int i = 0; i < kUnroll; ++i) u[i] = ld_stream(body + p + i * NS);
-#pragma unroll
-      for (int i = 0; i < kUnroll; ++i) {
-        float f[VW];
-        unpack<T>(u[i], f);
-        fold<VW>(v, f, a.c);
-      }
-    }
-    for (; p < end; p += NS) {
-      float f[VW];
-      unpack<T>(ld_stream(body + p), f);
-      fold<VW>(v, f, a.c);
+      for (int i = 0; i < kUnroll; ++i)
+        u[i] = p + i * NS < end ? ld_stream(body + p + i * NS) : make_uint4(none, none, none, none);
+      fold_packs<T, kUnroll>(v, u, a.c);
     }
     v = warp_merge(v, a.c);
     if ((tid & 31) == 0) part[tid >> 5] = make_float2(v.m, v.s);
@@ -954,16 +965,17 @@ bool same_phase(const void* x, int64_t ld, const void* y, int64_t ld_y, int64_t 
 }
 
 // Calls go(NS, E): the threads that stream a row (and one warp more for its
-// list) and the list's entries a lane.  Rows of up to 16 KB go to CTAs of 128
-// threads, of which more are resident to hide the lists' latency (at 4096
-// bf16 columns: 3 times as fast as 512).
+// list) and the list's entries a lane.  Rows of up to 64 KB go to CTAs of 128
+// threads, of which more are resident to hide the lists' latency (forward,
+// 8192 x 16384 bf16: 52 us, 62 us with 256, 93 us with 512); from there on 256
+// do as well.
 template <typename T, typename F>
 int with_geometry(int64_t cols, int64_t k, F&& go) {
   using Small = std::integral_constant<int, 128>;
-  using Large = std::integral_constant<int, 512>;
+  using Large = std::integral_constant<int, 256>;
   using Held = std::integral_constant<int, 2>;
   using Any = std::integral_constant<int, 0>;
-  if (cols * (int64_t)sizeof(T) <= 16384) return k <= 64 && k > 0 ? go(Small{}, Held{}) : go(Small{}, Any{});
+  if (cols * (int64_t)sizeof(T) <= 65536) return k <= 64 && k > 0 ? go(Small{}, Held{}) : go(Small{}, Any{});
   return k <= 64 && k > 0 ? go(Large{}, Held{}) : go(Large{}, Any{});
 }
 
