@@ -3,6 +3,7 @@
 // 81-82, 138-181, 209-213, 248-268).  Registered for the flagos device and for plain
 // CUDA tensors (the memory is the same kind); each op allocates its outputs
 // on the input's device and launches on that device's current stream.
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
 #include <cmath>
@@ -427,6 +428,11 @@ const float* RowWeights(const std::optional<at::Tensor>& w, const Distill& d, at
   if (!w.has_value() || !w->defined()) return nullptr;
   SameDevice(d.x, *w, op);
   TORCH_CHECK(w->scalar_type() == at::kFloat, op, ": ", name, " must be float32, got ", w->scalar_type());
+  if (w->sizes() == d.lead && w->is_contiguous()) {
+    keep = *w;
+    stride = d.rx.rows > 1 ? 1 : 0;
+    return keep.data_ptr<float>();
+  }
   keep = w->expand(d.lead).reshape({d.rx.rows});
   stride = d.rx.rows > 1 ? keep.stride(0) : 0;
   return keep.data_ptr<float>();
@@ -543,6 +549,82 @@ std::tuple<at::Tensor, at::Tensor> VerifyDraft(const at::Tensor& draft_ids, cons
   return {tokens, accepted};
 }
 
+// ------------------------------------------------------------- autograd --
+// Of topk and distill_topk, registered natively: a decode step's or a small
+// batch's call is bound by the host, and a formula registered from Python
+// costs it 5 us, needed or not.
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+template <typename Fn>
+const c10::TypedOperatorHandle<Fn>& Below(const char* name) {
+  static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Fn>();
+  return op;
+}
+using TopkFn = std::tuple<at::Tensor, at::Tensor>(const at::Tensor&, int64_t);
+using DistillFn = std::tuple<at::Tensor, at::Tensor>(const at::Tensor&, const at::Tensor&,
+                                                     const at::Tensor&, double);
+
+// dx = dvalues at the indices, 0 elsewhere.
+struct TopkGrad : torch::autograd::Function<TopkGrad> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& x, int64_t k) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    auto [values, indices] = Below<TopkFn>("flagos::topk").call(x, k);
+    ctx->set_materialize_grads(false);
+    ctx->mark_non_differentiable({indices});
+    ctx->save_for_backward({indices});
+    ctx->saved_data["cols"] = x.size(-1);
+    return {values, indices};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    if (!grads[0].defined()) return {at::Tensor(), at::Tensor()};
+    return {TopkBackward(grads[0], ctx->get_saved_variables()[0], ctx->saved_data["cols"].toInt()),
+            at::Tensor()};
+  }
+};
+std::tuple<at::Tensor, at::Tensor> TopkAutograd(const at::Tensor& x, int64_t k) {
+  if (at::GradMode::is_enabled() && x.requires_grad()) {
+    auto out = TopkGrad::apply(x, k);
+    return {out[0], out[1]};
+  }
+  at::AutoDispatchBelowADInplaceOrView guard;
+  return Below<TopkFn>("flagos::topk").call(x, k);
+}
+
+// Both operands' gradients from the forward's row statistics, which have none.
+struct DistillGrad : torch::autograd::Function<DistillGrad> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& logits, const at::Tensor& teacher,
+                               const at::Tensor& ids, double temperature) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    auto [loss, stats] = Below<DistillFn>("flagos::distill_topk").call(logits, teacher, ids, temperature);
+    ctx->set_materialize_grads(false);
+    ctx->mark_non_differentiable({stats});
+    ctx->save_for_backward({logits, teacher, ids, stats});
+    ctx->saved_data["temperature"] = temperature;
+    return {loss, stats};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const bool logits = ctx->needs_input_grad(0), teacher = ctx->needs_input_grad(1);
+    variable_list none(4);
+    if (!grads[0].defined() || (!logits && !teacher)) return none;
+    const auto saved = ctx->get_saved_variables();
+    auto [dx, dt] = DistillTopkBackward(grads[0], saved[0], saved[3], saved[1], saved[2],
+                                        ctx->saved_data["temperature"].toDouble(), logits, teacher);
+    if (logits) none[0] = dx;
+    if (teacher) none[1] = dt;
+    return none;
+  }
+};
+std::tuple<at::Tensor, at::Tensor> DistillTopkAutograd(const at::Tensor& logits, const at::Tensor& teacher,
+                                                       const at::Tensor& ids, double temperature) {
+  if (at::GradMode::is_enabled() && (logits.requires_grad() || teacher.requires_grad())) {
+    auto out = DistillGrad::apply(logits, teacher, ids, temperature);
+    return {out[0], out[1]};
+  }
+  at::AutoDispatchBelowADInplaceOrView guard;
+  return Below<DistillFn>("flagos::distill_topk").call(logits, teacher, ids, temperature);
+}
+
 }  // namespace
 
 TORCH_LIBRARY(flagos, m) {
@@ -596,5 +678,15 @@ TORCH_LIBRARY(flagos, m) {
 
 TORCH_LIBRARY_IMPL(flagos, PrivateUse1, m) { FLB_FUSED_IMPLS(m) }
 TORCH_LIBRARY_IMPL(flagos, CUDA, m) { FLB_FUSED_IMPLS(m) }
+TORCH_LIBRARY_IMPL(flagos, Autograd, m) {
+  m.impl("topk", TopkAutograd);
+  m.impl("distill_topk", DistillTopkAutograd);
+  // Not differentiable: their results have no history.  (Without a word here
+  // PyTorch boxes every call to say so on a backward.)
+  m.impl("topk_backward", torch::CppFunction::makeFallthrough());
+  m.impl("distill_topk_backward", torch::CppFunction::makeFallthrough());
+  m.impl("distill_topk_grad", torch::CppFunction::makeFallthrough());
+  m.impl("verify_draft", torch::CppFunction::makeFallthrough());
+}
 
 }  // namespace flb200::aten

@@ -18,8 +18,6 @@
 // (m, S = sum 2^((z - m) c)) a row, S = 0 for a row without a list; the
 // backward multiplies by 1 / S what it exponentiates against the same m, so
 // the two agree to the rounding of the exponential itself.
-#include <atomic>
-
 #include "vocab_rows.cuh"
 
 namespace flb200 {
@@ -1049,13 +1047,8 @@ int run_grad(const void* x, int64_t ld, const Taught& a, const float* weight, in
   const int64_t cluster = ceil_div(cols, (int64_t)NT * kPacks * Elem<T>::kVec);
   if (cluster > kMaxCluster) return -1;
   const size_t smem = sizeof(GradShared<NT>);
-  // (per launch: the attributes are held per device)
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
-      (cluster > 8 &&
-       cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)) {
-    (void)cudaGetLastError();
-    return -1;
-  }
+  static std::atomic<int> allowed[64];
+  if (!allow_smem(kern, smem, cluster > 8, allowed)) return -1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)cluster);
   cfg.blockDim = dim3(NT + kHelpers);

@@ -527,11 +527,9 @@ FL_B200_API int fl_b200_topk_lastdim(const void* x, int64_t ld, int64_t rows, in
       while (cluster < 8 && rows * cluster < dev.sm_count && cluster * 2 * k <= kCap && k <= kShared &&
              cols / (cluster * 2) >= 2 * B * Elem<T>::kVec)
         cluster *= 2;
-      // (per launch: the attribute is held per device)
       const auto kern = topk_kernel<T, B>;
-      if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               (int)sizeof(Shared<B>)) != cudaSuccess)
-        return launch_status();
+      static std::atomic<int> allowed[64];
+      if (!allow_smem(kern, sizeof(Shared<B>), false, allowed)) return (int)FL_B200_ERR_LAUNCH;
       const int64_t ctas = std::min<int64_t>(rows, 1024 / B * dev.sm_count);
       return launch_cluster(kern, cluster > 1 ? rows * cluster : ctas, cluster, B, sizeof(Shared<B>),
                             (cudaStream_t)stream, reinterpret_cast<const T*>(x), ld, rows, (int)cols,

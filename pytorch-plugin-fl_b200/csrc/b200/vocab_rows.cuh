@@ -3,6 +3,8 @@
 // clusters that share one row, and small typed loads.
 #pragma once
 
+#include <atomic>
+
 #include "common.cuh"
 
 namespace flb200 {
@@ -192,6 +194,24 @@ __device__ __forceinline__ int64_t load_index(const void* p, int dtype, int64_t 
 }
 
 __device__ __forceinline__ float warp_sum(float v) { return group_reduce_warp<SumOp, 32>(v); }
+
+// Lets `kern` use `smem` bytes of dynamic shared memory, and clusters of more
+// than 8 CTAs where `wide`; asked for once a kernel and device (`done`, a
+// static of the caller's).
+template <typename K>
+inline bool allow_smem(K kern, size_t smem, bool wide, std::atomic<int> (&done)[64]) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
+  const int want = wide ? 2 : 1;
+  if (done[dev].load(std::memory_order_acquire) >= want) return true;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
+      (wide && cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)) {
+    set_last_cuda_error(cudaGetLastError());
+    return false;
+  }
+  done[dev].store(want, std::memory_order_release);
+  return true;
+}
 
 // Launches `kern` with `ctas` CTAs in clusters of `cluster`.
 template <typename... KArgs, typename... Args>

@@ -22,10 +22,7 @@ rounding the forward used.
 * masked_softmax(x, mask, scale): dx = softmax_backward(dy, y, x.dtype, scale);
   a mask that needs a gradient gets the unscaled product summed over the
   dims it broadcasts (HF's mask needs none)
-* topk(x, k) -> (values, indices): dx = dvalues at the indices, 0 elsewhere
-* distill_topk(logits, teacher, ids) -> (loss, stats): both operands' gradients
-  by distill_topk_backward from the forward's row statistics; the statistics
-  themselves have none
+(topk and distill_topk carry theirs natively, in csrc/aten/fused_ops.cc.)
 """
 
 from __future__ import annotations
@@ -174,37 +171,6 @@ def _masked_softmax_backward(ctx, dy):
     return dx, dmask, None, None, None
 
 
-# ---------------------------------------------------- rows of the vocabulary
-def _topk_setup(ctx, inputs, output):
-    ctx.set_materialize_grads(False)  # (no zeros made up for the indices)
-    ctx.save_for_backward(output[1])
-    ctx.cols = inputs[0].shape[-1]
-
-
-def _topk_backward(ctx, dvalues, _):
-    (indices,) = ctx.saved_tensors
-    if dvalues is None or not ctx.needs_input_grad[0]:
-        return None, None
-    return _F.topk_backward(dvalues, indices, ctx.cols), None
-
-
-def _distill_setup(ctx, inputs, output):
-    logits, teacher, ids, temperature = inputs
-    ctx.set_materialize_grads(False)
-    ctx.mark_non_differentiable(output[1])
-    ctx.save_for_backward(logits, teacher, ids, output[1])
-    ctx.temperature = temperature
-
-
-def _distill_backward(ctx, dloss, _):
-    logits, teacher, ids, stats = ctx.saved_tensors
-    need = ctx.needs_input_grad[:2]
-    if dloss is None or not any(need):
-        return None, None, None, None
-    dx, dt = _F.distill_topk_backward(dloss, logits, stats, teacher, ids, ctx.temperature, *need)
-    return dx if need[0] else None, dt if need[1] else None, None, None
-
-
 def register() -> None:
     """Attach the formulas to the flagos:: ops (once per process)."""
     reg = torch.library.register_autograd
@@ -216,5 +182,3 @@ def register() -> None:
     reg("flagos::swiglu_residual", _swiglu_res_backward, setup_context=_swiglu_res_setup)
     reg("flagos::causal_softmax", _softmax_backward, setup_context=_softmax_setup)
     reg("flagos::masked_softmax", _masked_softmax_backward, setup_context=_masked_softmax_setup)
-    reg("flagos::topk", _topk_backward, setup_context=_topk_setup)
-    reg("flagos::distill_topk", _distill_backward, setup_context=_distill_setup)
