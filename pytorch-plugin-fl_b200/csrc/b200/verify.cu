@@ -311,10 +311,12 @@ FL_B200_API int fl_b200_verify_draft(const int64_t* draft_ids, int64_t ld_ids, c
     VerifyArgs<T> a = {draft_ids, ld_ids, reinterpret_cast<const T*>(p), p_stride_b, p_stride_i,
                        reinterpret_cast<const T*>(q), q_stride_b, q_stride_i, uniform, ld_u, lens,
                        (int)drafts, (int)vocab, tokens, accepted};
-    // up to 8 CTAs a sequence, a pack a thread at least, until every SM has eight
+    // up to 8 CTAs a sequence, with three packs a thread at least, while all
+    // of them are resident at once (a sequence alone: 5.3 us with 8, 8.5 us
+    // with one; 500 sequences over 32000 float32: 24 us with one, 49 us with 8)
     int cluster = 1;
-    while (cluster < 8 && batch * cluster < 8 * dev.sm_count &&
-           vocab / (cluster * 2) >= kBlock * Elem<T>::kVec)
+    while (cluster < 8 && batch * cluster * 2 <= 4 * dev.sm_count &&
+           vocab / (cluster * 2) >= 3 * kBlock * Elem<T>::kVec)
       cluster *= 2;
     if (batch * cluster > 0x7fffffffLL) return (int)FL_B200_ERR_TOO_LARGE;
     return launch_cluster(verify_kernel<T>, batch * cluster, cluster, kBlock, 0, (cudaStream_t)stream, a);
