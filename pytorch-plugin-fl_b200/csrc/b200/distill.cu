@@ -134,13 +134,7 @@ __device__ __forceinline__ void fold(MaxSum& v, float f, float c) {
 __device__ __forceinline__ float final_sum(float s) { return s == 0.f ? NAN : s; }
 
 constexpr int kGradList = 128;  // the longest list that a warp holds in registers
-constexpr int kMarkBits = 8192;  // marks of the tokens named so far, by id modulo this
-
-// A list's tokens and masses, for the search after repeated ones.
-struct GradList {
-  int id[kGradList];      // -1: absent
-  float mass[kGradList];  // sum of p over the entries with this id; -1 but at the first of them
-};
+constexpr int kMarkBits = 16384;  // marks of the tokens named so far, by id modulo this
 
 // Warp-wide maximum; NaN only if every lane has one.
 __device__ __forceinline__ float warp_max(float v) {
@@ -243,13 +237,13 @@ struct ListHeld {
   uint32_t z[kEach];  // the logit's bits, of entries in [lo, hi)
   float t2[kEach];    // (t - max t) c
   float e[kEach];     // 2^t2, 0 where absent
-  float mass[kEach];  // as GradList's
+  float mass[kEach];  // sum of p over the entries with this id; -1 but at the first of them
   float total;        // of e; 0 when nothing is taught
   float by;           // w tau
 
+  // Everything but the masses.
   __device__ __forceinline__ void set(const Taught& a, const ListAhead<E>& in, const T* x, int cols, int lo,
-                                      int hi, GradList& l, uint32_t* marks) {
-    const int lane = threadIdx.x & 31;
+                                      int hi) {
     by = in.w * a.tau;
     float top = -INFINITY;
 #pragma unroll
@@ -274,6 +268,10 @@ struct ListHeld {
       total += e[i];
     }
     total = warp_sum(total);
+  }
+
+  __device__ __forceinline__ void set_masses(const Taught& a, uint32_t* marks) {
+    const int lane = threadIdx.x & 31;
     const float inverse = reciprocal(total);
     // an id whose mark was set already may be a repeated one
     uint32_t again = 0;
@@ -292,48 +290,33 @@ struct ListHeld {
       if (32 * i >= a.k) break;
       if (id[i] >= 0) marks[(uint32_t)id[i] % kMarkBits / 32] = 0;
     }
-    if (__any_sync(0xffffffffu, again != 0)) {
+    // each id under suspicion against the whole list: its first entry takes
+    // the sum of all
 #pragma unroll
-      for (int i = 0; i < kEach; ++i) {
-        const int j = lane + 32 * i;
-        if (j < a.k) {
-          l.id[j] = id[i];
-          l.mass[j] = mass[i];
-        }
-      }
-      __syncwarp();
-      merge(a.k, again, l);
-#pragma unroll
-      for (int i = 0; i < kEach; ++i)
-        if (lane + 32 * i < a.k) mass[i] = l.mass[lane + 32 * i];
-    }
-    __syncwarp();
-  }
-
-  // For each id under suspicion the warp goes over the list: its first entry
-  // takes the sum of all.
-  __device__ __noinline__ static void merge(int k, uint32_t again, GradList& l) {
-    const int lane = threadIdx.x & 31;
-    for (int i = 0; 32 * i < k; ++i) {
+    for (int i = 0; i < kEach; ++i) {
+      if (32 * i >= a.k) break;
       uint32_t votes = __ballot_sync(0xffffffffu, (again >> i) & 1);
       while (votes != 0) {
-        const int same = l.id[32 * i + __ffs(votes) - 1];
+        const int same = __shfl_sync(0xffffffffu, id[i], __ffs(votes) - 1);
         votes &= votes - 1;
-        int first = k;
+        int first = kGradList, count = 0;
         float sum = 0.f;
-        for (int n = lane; n < k; n += 32) {
-          if (l.id[n] != same) continue;
-          first = min(first, n);
-          if (l.mass[n] != -1.f) sum += l.mass[n];
+#pragma unroll
+        for (int n = kEach - 1; n >= 0; --n) {
+          if (32 * n >= a.k || id[n] != same) continue;
+          first = lane + 32 * n;
+          ++count;
+          if (mass[n] != -1.f) sum += mass[n];
         }
-        __syncwarp();
+        if (__reduce_add_sync(0xffffffffu, count) == 1) continue;  // another id with its mark
         first = __reduce_min_sync(0xffffffffu, first);
         sum = warp_sum(sum);
-        for (int n = lane; n < k; n += 32)
-          if (l.id[n] == same) l.mass[n] = n == first ? sum : -1.f;
-        __syncwarp();
+#pragma unroll
+        for (int n = 0; n < kEach; ++n)
+          if (32 * n < a.k && id[n] == same) mass[n] = lane + 32 * n == first ? sum : -1.f;
       }
     }
+    __syncwarp();
   }
 };
 
@@ -422,7 +405,6 @@ __device__ __forceinline__ void fold_packs(MaxSum& v, const uint4 (&u)[N], float
 template <typename T, int E>
 struct ListOf {
   struct Shared {
-    GradList list;
     uint32_t marks[kMarkBits / 32];
   };
   ListHeld<T, E> held;
@@ -434,7 +416,8 @@ struct ListOf {
     in.load(a, nullptr, 0, row);
     for (int i = threadIdx.x & 31; i < kMarkBits / 32; i += 32) s.marks[i] = 0;
     __syncwarp();
-    held.set(a, in, x, cols, lo, hi, s.list, s.marks);
+    held.set(a, in, x, cols, lo, hi);
+    held.set_masses(a, s.marks);
     total = held.total;
   }
   // sum of p_j ((t_j - max t) - (z_j - m)) / tau, by the warp
@@ -703,7 +686,6 @@ template <int NT>
 struct GradShared {
   uint4 stage[kStages][kPacks][NT];
   float2 pair[2][kMaxCluster * (NT / 32)];
-  GradList list[2];
   uint32_t marks[2][kMarkBits / 32];
   float2 scale[2];  // the row's M, and w tau / S
   int live[2];      // whether anything is taught
@@ -762,7 +744,7 @@ distill_grad_kernel(const T* __restrict__ x, int64_t ld, Taught a, const float* 
       slice(sp, from, to);
       if (lane == 0) bar_expect(&s.bar[par], C * W * 8);
       list.set(a, next, xr, cols, rank == 0 ? 0 : sp.head + from * VW,
-               rank == 0 ? cols : sp.head + to * VW, s.list[par], s.marks[par]);
+               rank == 0 ? cols : sp.head + to * VW);
       if (row + 2 * step < rows) next.load(a, weight, weight_stride, row + 2 * step);
     };
     const auto load = [&](int64_t row, int stage) {
@@ -806,6 +788,7 @@ distill_grad_kernel(const T* __restrict__ x, int64_t ld, Taught a, const float* 
       }
       __syncwarp();
       named_arrive(kScaled + par, NT + 32);
+      list.set_masses(a, s.marks[par]);  // (while the holders write the row)
       const RowSplit sp = split_row(x + row * ld, cols);
       int from, to;
       slice(sp, from, to);
@@ -848,10 +831,11 @@ distill_grad_kernel(const T* __restrict__ x, int64_t ld, Taught a, const float* 
           stats[row] = live ? make_float2(M, S) : make_float2(0.f, 0.f);
         }
       }
-      if (lane == 0) bulk_wait_read();
-      __syncwarp();  // the list has been read, and the stage
-      load(row + kStages * step, stage);
+      // (the store reads its stage meanwhile)
       if (row + 2 * step < rows) set(row + 2 * step);
+      if (lane == 0) bulk_wait_read();
+      __syncwarp();
+      load(row + kStages * step, stage);
       stage = (stage + 2) % kStages;
     }
     if (lane == 0) bulk_wait();
