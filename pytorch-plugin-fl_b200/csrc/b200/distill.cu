@@ -462,7 +462,13 @@ struct ListOf {
 
 template <typename T>
 struct ListOf<T, 0> {
-  using Shared = List;
+  static constexpr int kMarks = 65536;
+  struct Shared : List {
+    float mass[kMaxList];  // sum of p over the entries with this id; -1 but at the first of them
+    uint32_t marks[kMarks / 32];
+    short suspect[kMaxList];
+    int suspects;
+  };
   float total;
 
   __device__ __forceinline__ void load(Shared& s, const Taught& a, const float*, int64_t, const T* x,
@@ -486,22 +492,44 @@ struct ListOf<T, 0> {
       store_float(dt, a.t_dtype, row * a.k + j, g);
     }
   }
-  // By the whole CTA: for each entry the list is searched, the first entry of
-  // an id calls for all.
+  // By the whole CTA (several barriers).  An entry whose id's mark was set
+  // already may be a repeated one: a warp looks through the list for it.
   template <typename F>
   __device__ __forceinline__ void tokens(Shared& s, const Taught& a, const T*, int, F put) const {
+    const int lane = threadIdx.x & 31;
+    const float inverse = reciprocal(s.total);
+    for (int i = threadIdx.x; i < kMarks / 32; i += blockDim.x) s.marks[i] = 0;
+    if (threadIdx.x == 0) s.suspects = 0;
+    __syncthreads();
     for (int j = threadIdx.x; j < a.k; j += blockDim.x) {
       const int id = s.id[j];
-      if (id < 0) continue;
-      float mass = 0.f;
-      bool first = true;
-      for (int i = 0; i < a.k && first; ++i) {
-        if (s.id[i] != id) continue;
-        first = i >= j;
-        mass += exp2f(s.t2[i]);
-      }
-      if (first) put(id, s.z[j], mass / s.total);
+      s.mass[j] = id >= 0 ? exp2f(s.t2[j]) * inverse : -1.f;
+      const uint32_t h = (uint32_t)id % kMarks;
+      if (id >= 0 && (atomicOr(&s.marks[h / 32], 1u << (h % 32)) >> (h % 32)) & 1)
+        s.suspect[atomicAdd(&s.suspects, 1)] = (short)j;
     }
+    __syncthreads();
+    for (int n = threadIdx.x >> 5; n < s.suspects; n += blockDim.x >> 5) {
+      const int same = s.id[s.suspect[n]];
+      int first = kMaxList, count = 0;
+      float sum = 0.f;
+      for (int j = lane; j < a.k; j += 32) {
+        if (s.id[j] != same) continue;
+        first = min(first, j);
+        ++count;
+        sum += exp2f(s.t2[j]) * inverse;
+      }
+      __syncwarp();
+      if (__reduce_add_sync(0xffffffffu, count) == 1) continue;
+      first = __reduce_min_sync(0xffffffffu, first);
+      sum = warp_sum(sum);
+      // (two warps at one id write the same values)
+      for (int j = lane; j < a.k; j += 32)
+        if (s.id[j] == same) s.mass[j] = j == first ? sum : -1.f;
+    }
+    __syncthreads();
+    for (int j = threadIdx.x; j < a.k; j += blockDim.x)
+      if (s.id[j] >= 0 && s.mass[j] != -1.f) put(s.id[j], s.z[j], s.mass[j]);
   }
 };
 
@@ -989,9 +1017,10 @@ int run_bwd(const float* dloss, int64_t dloss_stride, const void* x, int64_t ld,
   return with_geometry<T>(cols, a.k, [&](auto ns, auto e) {
     constexpr int NS = decltype(ns)::value, E = decltype(e)::value;
     // chunks of 4 rounds of loads, which hide the list's latency (2048 x 128256
-    // bf16: 201 us, 249 us with one round); shorter where rows are few
+    // bf16: 201 us, 249 us with one round), of 16 for a long list; shorter where
+    // rows are few
     const int64_t round = (int64_t)NS * kUnroll * Elem<T>::kVec;
-    int64_t chunk = dx == nullptr ? cols : 4 * round;
+    int64_t chunk = dx == nullptr ? cols : (E == 0 ? 16 : 4) * round;
     while (chunk > round && rows * ceil_div(cols, chunk) < 4 * dev.sm_count) chunk /= 2;
     const int64_t chunks = ceil_div(cols, chunk);
     if (rows * chunks > 0x7fffffffLL) return (int)FL_B200_ERR_TOO_LARGE;

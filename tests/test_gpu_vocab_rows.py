@@ -291,6 +291,26 @@ def test_distill_special_rows(dtype, V):
     assert K.distill_topk(z, t, ids, 1.0)[0][1] == float("inf")
 
 
+@pytest.mark.parametrize("k", [2, 33, 64, 65, 128, 129, 300, 1024])
+def test_distill_repeated_tokens(k):
+    """Lists drawn from few tokens, one of a single token, one whose ids share
+    their low bits; of every length that a kernel holds in another way."""
+    R, V = 6, 70001
+    z, t, ids, w = make(R, V, k, torch.float32, k, holes=False)
+    g = gen(k + 1)
+    ids = torch.randint(0, 7, (R, k), generator=g) * 9973
+    ids[1] = 12345
+    ids[2] = torch.arange(k) % 4 * 16384 + 5            # equal modulo 16384
+    ids[3] = torch.arange(k) % 2 * 65536 + 3            # and modulo 65536
+    ids[4] = torch.randint(0, V, (k,), generator=g)
+    ids[5, ::2] = -1
+    check_distill(z, t, ids.to(DEV), w, 1.5, f"k={k}")
+    a = K.distill_topk_grad(z, t, ids.to(DEV), 1.5, w)
+    for _ in range(3):                                  # whatever the marks' order
+        b = K.distill_topk_grad(z, t, ids.to(DEV), 1.5, w)
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
 def test_distill_without_lists_or_rows():
     z = torch.randn(3, 50, device=DEV)
     t, ids = torch.zeros(3, 0, device=DEV), torch.zeros(3, 0, dtype=torch.int64, device=DEV)
