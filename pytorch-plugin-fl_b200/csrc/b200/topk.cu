@@ -460,8 +460,11 @@ topk_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int cols, int k, 
     if (rank == 0) {
       const auto put = [&](int place, uint64_t key) {
         const uint32_t at = ~(uint32_t)key;
+        const uint32_t v = (uint32_t)(key >> 32);
         indices[row * k + place] = at;
-        values[row * k + place] = xr[at];
+        // the key tells the value's bits but for a zero's sign and a NaN's payload
+        values[row * k + place] =
+            v == 0x80000000u || v == 0xffffffffu ? xr[at] : Elem<T>::from_f(key_value(v));
       };
       if (n <= B / 2) {
         place_all(put);
