@@ -252,18 +252,22 @@ __device__ __forceinline__ uint32_t kth_maximum(const Shared<B>& s, int k) {
   }
   lo = __reduce_min_sync(0xffffffffu, lo);
   hi = __reduce_max_sync(0xffffffffu, hi);
-  const int top = 32 - __clz(lo ^ hi);  // below it the keys' bits differ
+  // two bits a step, below those that lo and hi share: the counts of the three
+  // larger keys in ten bits each (at most B of them)
+  static_assert(B < 1024, "the counts' fields");
+  const int top = (32 - __clz(lo ^ hi) + 1) & ~1;
   uint32_t at = top < 32 ? lo >> top << top : 0;
-  for (int bit = top; bit-- > 0;) {
-    const uint32_t tried = at | (1u << bit);
+  for (int bit = top - 2; bit >= 0; bit -= 2) {
+    const uint32_t one = 1u << bit;
     int n = 0;
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) n += v[i] >= tried;
+    for (int i = 0; i < kEach; ++i)
+      n += (v[i] >= at + one) + ((v[i] >= at + 2 * one) << 10) + ((v[i] >= at + 3 * one) << 20);
     n = __reduce_add_sync(0xffffffffu, n);
-    if (n >= k) {
-      at = tried;
-      if (n <= k + k / 8) break;
-    }
+    const int n3 = n >> 20, n2 = (n >> 10) & 1023, n1 = n & 1023;
+    const int reached = n3 >= k ? n3 : n2 >= k ? n2 : n1 >= k ? n1 : 0;
+    at += n3 >= k ? 3 * one : n2 >= k ? 2 * one : n1 >= k ? one : 0;
+    if (reached != 0 && reached <= k + k / 8) break;
   }
   return at;  // (0 among the keys: lo = 0, and `at` stays 0 unless k reach more)
 }
@@ -306,6 +310,9 @@ __device__ __forceinline__ int collect(Shared<B>& s, const T* xr, int lo, int hi
   const RowSplit sp = split_row(xr + lo, hi - lo);
   const Packs src = {reinterpret_cast<const uint4*>(xr + lo + sp.head), sp.nvec};
   if (tid == 0) s.filled = s.listed = 0;
+  // the slice's single elements, used after the stream
+  const int single = single_of(sp, tid, VW);
+  const float alone = single >= 0 ? Elem<T>::to_f(xr[lo + single]) : 0.f;
   uint32_t group[kPacks];
 #pragma unroll
   for (int i = 0; i < kPacks; ++i) group[i] = word_lowest<T>();
@@ -352,11 +359,7 @@ __device__ __forceinline__ int collect(Shared<B>& s, const T* xr, int lo, int hi
       return m;
     });
   }
-  if (tid < sp.head) append(s, element_key(Elem<T>::to_f(xr[lo + tid]), (uint32_t)(lo + tid)));
-  if (tid < sp.tail) {
-    const int e = hi - sp.tail + tid;
-    append(s, element_key(Elem<T>::to_f(xr[e]), (uint32_t)e));
-  }
+  if (single >= 0) append(s, element_key(alone, (uint32_t)(lo + single)));
 #pragma unroll
   for (int i = 0; i < kPacks; ++i)
     if (group[i] >= max(least, 1u)) s.list[take_slot(&s.listed)] = (uint16_t)(i * B + tid);
@@ -364,16 +367,39 @@ __device__ __forceinline__ int collect(Shared<B>& s, const T* xr, int lo, int hi
   const int depth = (sp.nvec + kChunk - 1) / kChunk;  // packs of a group
   const int items = s.listed * depth;
   const float bar = key_value(least);  // (NaN while everything passes, or only NaN does)
-  for (int j = tid; j < items; j += B) {
-    const int p = s.list[j / depth] + j % depth * kChunk;
-    if (p >= sp.nvec) continue;
-    const uint4 u = ld_cached(src.body + p);
-    if (word_top<T>(pack_max<T>(u)) < bar) continue;
+  const auto look = [&](const uint4& u, int p) {
+    if (word_top<T>(pack_max<T>(u)) < bar) return;
     float f[VW];
     unpack<T>(u, f);
 #pragma unroll
     for (int i = 0; i < VW; ++i)
       if (value_key(f[i]) >= least) append(s, element_key(f[i], (uint32_t)(lo + sp.head + p * VW + i)));
+  };
+  if (depth == 1 && next.nvec == 0) {
+    // the stage still holds them
+    for (int j = tid; j < items; j += B) {
+      const int p = s.list[j];
+      look(s.stage[p / B][p % B], p);
+    }
+  } else {
+    // two packs a thread in flight; n / depth by a multiplication where that is
+    // exact (n < 4096 depth, off by less than n depth / 2^32 of a step)
+    const uint32_t over = depth < 1024 ? (uint32_t)((0x100000000ull + depth - 1) / depth) : 0;
+    for (int j = tid; j < items; j += 2 * B) {
+      int p[2];
+      uint4 u[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t n = min(j + i * B, items - 1);
+        const uint32_t entry = depth == 1 ? n : depth < 1024 ? __umulhi(n, over) : n / depth;
+        p[i] = s.list[entry] + (int)(n - entry * depth) * kChunk;
+        if (j + i * B >= items || p[i] >= sp.nvec) p[i] = -1;
+        u[i] = ld_cached(src.body + max(p[i], 0));
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (p[i] >= 0) look(u[i], p[i]);
+    }
   }
   __syncthreads();
   return s.filled;
@@ -425,16 +451,21 @@ topk_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int cols, int k, 
     };
     // few keys: each one's place is the number of keys above it
     const auto place_all = [&](auto put) {
-      int per_key = 32;
-      while (per_key * n > B) per_key >>= 1;
-      const int i = tid / per_key;
+      int shift = 5;  // 2^shift threads a key
+      while ((n << shift) > B) --shift;
+      const int i = tid >> shift, step = 1 << shift;
       const uint64_t key = i < n ? s.cand[i] : 0;
       int place = 0;
-      if (i < n)
-        for (int j = tid % per_key; j < n; j += per_key) place += s.cand[j] > key;
+      if (i < n) {
+        int j = tid & (step - 1);
+        for (; j + 3 * step < n; j += 4 * step)
+          place += (s.cand[j] > key) + (s.cand[j + step] > key) + (s.cand[j + 2 * step] > key) +
+                   (s.cand[j + 3 * step] > key);
+        for (; j < n; j += step) place += s.cand[j] > key;
+      }
       __syncwarp();
-      for (int o = per_key >> 1; o > 0; o >>= 1) place += __shfl_xor_sync(0xffffffffu, place, o);
-      if (i < n && tid % per_key == 0 && place < k) put(place, key);
+      for (int o = step >> 1; o > 0; o >>= 1) place += __shfl_xor_sync(0xffffffffu, place, o);
+      if (i < n && (tid & (step - 1)) == 0 && place < k) put(place, key);
     };
     if (n > most) shrink(most);
     if (C > 1) {
