@@ -6,8 +6,6 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
-#include <cmath>
-
 #include "tensor_utils.h"
 
 namespace flb200::aten {
@@ -408,7 +406,7 @@ Distill DistillArgs(const at::Tensor& logits, const at::Tensor& teacher, const a
   TORCH_CHECK(teacher.size(-1) <= FL_B200_DISTILL_MAX, op, ": at most ", std::to_string(FL_B200_DISTILL_MAX),
               " teacher logits a row, got ", std::to_string(teacher.size(-1)));
   TORCH_CHECK(logits.size(-1) > 0 || logits.numel() == 0, op, ": an empty vocabulary");
-  TORCH_CHECK(temperature > 0 && std::isfinite((float)temperature) && (float)temperature > 0, op,
+  TORCH_CHECK((float)temperature > 1e-37f && (float)temperature <= 3e38f, op,
               ": temperature must be positive and finite, got ", std::to_string(temperature));
   d.rx = Rows(logits, d.x);
   d.rt = Rows(teacher, d.t);

@@ -956,8 +956,9 @@ bool list_dtypes_ok(int t_dtype, int ids_dtype) {
 
 int check_shapes(int64_t rows, int64_t cols, int64_t k, float temperature) {
   FLB_CHECK_ARG(rows >= 0 && cols >= 0 && k >= 0);
-  FLB_CHECK_ARG(temperature > 0.f && temperature <= 3.0e38f);
-  if (k > kMaxList || cols > 0x7fffff00LL || rows > 0x7fffffffLL) return FL_B200_ERR_TOO_LARGE;
+  // (and log2(e) / temperature finite)
+  FLB_CHECK_ARG(temperature > 1e-37f && temperature <= 3.0e38f);
+  if (k > kMaxList || cols > kMaxCols || rows > 0x7fffffffLL) return FL_B200_ERR_TOO_LARGE;
   FLB_CHECK_ARG(rows == 0 || cols > 0);
   return FL_B200_OK;
 }
@@ -1122,6 +1123,7 @@ FL_B200_API int fl_b200_distill_topk_bwd(const float* dloss, int64_t dloss_strid
   FLB_CHECK_ARG(dloss_stride >= 0 && logits && stats && (k == 0 || (teacher && ids)));
   FLB_CHECK_ARG((rows == 1 || ld >= cols) && ld_t >= 0 && ld_ids >= 0);
   FLB_CHECK_ARG(dlogits == nullptr || rows == 1 || ld_dlogits >= cols);
+  FLB_CHECK_ARG(dlogits != logits);  // (tokens are read again after their row is stored)
   if (reinterpret_cast<uintptr_t>(stats) % 8) return FL_B200_ERR_MISALIGNED;
   const Taught a = taught(teacher, ld_t, t_dtype, ids, ld_ids, ids_dtype, k, temperature);
   return dispatch_float(dtype, [&](auto t) {
@@ -1138,7 +1140,7 @@ FL_B200_API int fl_b200_distill_topk_grad(const void* logits, int64_t ld, const 
                                           void* dlogits, int64_t ld_dlogits, int dtype,
                                           fl_b200_stream_t stream) {
   using namespace flb200;
-  FLB_CHECK_ARG(rows <= 0 || (dlogits && (rows == 1 || ld_dlogits >= cols)));
+  FLB_CHECK_ARG(rows <= 0 || (dlogits && dlogits != logits && (rows == 1 || ld_dlogits >= cols)));
   FLB_CHECK_ARG(weight_stride >= 0);
   int st = check_shapes(rows, cols, k, temperature);
   if (st != FL_B200_OK) return st;

@@ -545,7 +545,7 @@ FL_B200_API int fl_b200_topk_lastdim(const void* x, int64_t ld, int64_t rows, in
   using namespace flb200;
   FLB_CHECK_ARG(rows >= 0 && k >= 0 && k <= cols);
   if (!is_float_dtype(dtype)) return FL_B200_ERR_UNSUPPORTED_DTYPE;
-  if (k > kMaxTop || rows > 0x7fffffffLL || cols > 0x7fffff00LL) return FL_B200_ERR_TOO_LARGE;
+  if (k > kMaxTop || rows > 0x7fffffffLL || cols > kMaxCols) return FL_B200_ERR_TOO_LARGE;
   if (rows == 0 || k == 0) return FL_B200_OK;
   FLB_CHECK_ARG(x && values && indices && (rows == 1 || ld >= cols));
   DeviceInfo dev;
@@ -582,7 +582,7 @@ FL_B200_API int fl_b200_topk_bwd(const void* dvalues, const int64_t* indices, vo
   using namespace flb200;
   FLB_CHECK_ARG(rows >= 0 && k >= 0 && k <= cols);
   if (!is_float_dtype(dtype)) return FL_B200_ERR_UNSUPPORTED_DTYPE;
-  if (k > kMaxTop || rows > 0x7fffffffLL || cols > 0x7fffff00LL) return FL_B200_ERR_TOO_LARGE;
+  if (k > kMaxTop || rows > 0x7fffffffLL || cols > kMaxCols) return FL_B200_ERR_TOO_LARGE;
   if (rows == 0 || cols == 0) return FL_B200_OK;
   FLB_CHECK_ARG(dx && (k == 0 || (dvalues && indices)));
   return dispatch_float(dtype, [&](auto t) {

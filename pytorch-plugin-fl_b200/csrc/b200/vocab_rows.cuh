@@ -12,6 +12,8 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
+// Rows and indices in them are ints; the kernels add up to 2^17 to one.
+constexpr int64_t kMaxCols = 0x7ff00000;
 constexpr float kLowest = -3.402823466e+38f;  // running maxima start here, not at -inf:
                                               // x - m stays defined for x = -inf
 

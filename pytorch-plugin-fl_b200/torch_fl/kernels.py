@@ -553,10 +553,25 @@ def sum_i32_i64(x: torch.Tensor, full: bool) -> torch.Tensor:
 
 
 # ------------------------------------------------------ rows of the vocabulary
+def _one_device(*tensors) -> None:
+    """The kernels get plain pointers: every operand on the first one's GPU."""
+    kept = [t for t in tensors if t is not None]
+    if any(_device_index(t) != _device_index(kept[0]) for t in kept):
+        raise ValueError("operands must be on one device")
+
+
+def _rows_apart(x: torch.Tensor) -> tuple[torch.Tensor, int, int, int]:
+    """_rows_or_contig, of a copy where rows overlap (an expanded tensor)."""
+    x, rows, cols, ld = _rows_or_contig(x)
+    if rows > 1 and ld < cols:
+        x, rows, cols, ld = _rows_or_contig(x.contiguous())
+    return x, rows, cols, ld
+
+
 def topk_lastdim(x: torch.Tensor, k: int) -> tuple[torch.Tensor, torch.Tensor]:
     """(values, int64 indices) of the k largest over the last dim, descending;
     ties by ascending index, NaN above everything."""
-    x, rows, cols, ld = _rows_or_contig(x)
+    x, rows, cols, ld = _rows_apart(x)
     shape = list(x.shape[:-1]) + [k]
     values = torch.empty(shape, dtype=x.dtype, device=x.device)
     indices = torch.empty(shape, dtype=torch.int64, device=x.device)
@@ -570,6 +585,7 @@ def topk_backward(dvalues: torch.Tensor, indices: torch.Tensor, cols: int) -> to
     """dx [..., cols] of topk_lastdim's values."""
     if dvalues.shape != indices.shape or indices.dtype != torch.int64:
         raise ValueError("dvalues and int64 indices must match")
+    _one_device(dvalues, indices)
     dvalues, indices = dvalues.contiguous(), indices.contiguous()
     k = dvalues.shape[-1]
     rows = dvalues.shape[:-1].numel()
@@ -586,7 +602,8 @@ def _taught(logits, teacher_logits, teacher_ids):
         raise TypeError("teacher_ids must be int32 or int64")
     if teacher_logits.shape != teacher_ids.shape or teacher_ids.shape[:-1] != logits.shape[:-1]:
         raise ValueError("logits [..., vocab] with teacher_logits and teacher_ids [..., k] expected")
-    x, rows, cols, ld = _rows_or_contig(logits)
+    _one_device(logits, teacher_logits, teacher_ids)
+    x, rows, cols, ld = _rows_apart(logits)
     t, _, k, ld_t = _rows_or_contig(teacher_logits)
     i, _, _, ld_i = _rows_or_contig(teacher_ids)
     head = (x.data_ptr(), ld)
@@ -626,6 +643,7 @@ def distill_topk_backward(dloss: torch.Tensor | None, logits: torch.Tensor, stat
     (x, *keep), head, lists, rows, cols, k = _taught(logits, teacher_logits, teacher_ids)
     if stats.dtype != torch.float32 or tuple(stats.shape) != (rows, 2) or not stats.is_contiguous():
         raise ValueError("stats must be the forward's [rows, 2] float32 tensor")
+    _one_device(x, stats, dloss)
     w, wp, ws = _row_weight(dloss, logits.shape[:-1])
     dx = torch.empty(logits.shape, dtype=x.dtype, device=x.device) if need_logits else None
     dt = torch.empty(teacher_logits.shape, dtype=teacher_logits.dtype,
@@ -643,12 +661,15 @@ def distill_topk_grad(logits: torch.Tensor, teacher_logits: torch.Tensor, teache
                       out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """(loss, dlogits) of sum(row_weight * loss) in one call."""
     (x, *keep), head, lists, rows, cols, k = _taught(logits, teacher_logits, teacher_ids)
+    _one_device(x, row_weight, out)
     w, wp, ws = _row_weight(row_weight, logits.shape[:-1])
     loss = torch.empty(logits.shape[:-1], dtype=torch.float32, device=x.device)
     stats = torch.empty((rows, 2), dtype=torch.float32, device=x.device)
     dx = torch.empty(logits.shape, dtype=x.dtype, device=x.device) if out is None else out
     if dx.shape != logits.shape or dx.dtype != x.dtype:
         raise ValueError("out must have the logits' shape and dtype")
+    if out is not None and out.data_ptr() == x.data_ptr() and out.numel():
+        raise ValueError("the gradient is not computed in place")
     _, _, ldo = _rows_view(dx)
     with _on_device(x):
         _abi.call("fl_b200_distill_topk_grad", *head, *lists, wp, ws, rows, cols, k,
@@ -673,6 +694,7 @@ def verify_draft(draft_ids: torch.Tensor, target_probs: torch.Tensor,
         raise ValueError("draft_probs must be [batch, drafts, vocab] of target_probs' dtype")
     if draft_lens is not None and (tuple(draft_lens.shape) != (B,) or draft_lens.dtype != torch.int64):
         raise ValueError("draft_lens must be int64 [batch]")
+    _one_device(target_probs, draft_ids, draft_probs, uniform, draft_lens)
 
     def unit(t):
         return t if t is None or t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()

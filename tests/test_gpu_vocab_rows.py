@@ -114,6 +114,8 @@ def test_topk_strides_and_shapes():
     check_topk(x.transpose(0, 2), 3)
     check_topk(x[0, 0], 5)
     check_topk(x[:1].expand(4, 5, 3001), 5)
+    check_topk(x[0, :1].expand(4, 3001), 5)
+    check_topk(x[0, :1].expand(4, 3001), 5, fn=torch_fl.ops.topk)
     v, i = K.topk_lastdim(x[:0], 4)
     assert v.shape == (0, 5, 4)
     v, i = K.topk_lastdim(x, 0)
@@ -344,6 +346,33 @@ def test_distill_autograd_on_flagos():
     assert not stats.requires_grad              # the row statistics have no gradient
 
 
+def test_distill_shapes_of_every_rank():
+    z, t, ids, w = make(12, 333, 5, torch.float32, 33)
+    want = K.distill_topk_grad(z, t, ids, 2.0, w)
+    one = torch_fl.ops.distill_topk_grad(z[7], t[7], ids[7], 2.0, w[7])
+    # (a row off the boundary that its gradient's row begins on takes two
+    # kernels: the formula's bounds hold, bit equality with one kernel does not)
+    ref = ops.distill_topk_golden(np64(z), np64(t), np64(ids).astype(np.int64), 2.0, np64(w))
+    tol = bounds(z, t, ids, 2.0, w)
+    assert one[0].shape == () and one[1].shape == (333,)
+    within(one[0].view(1), ref[0][7:8], tol[0][7:8] + half_step(torch.float32, ref[0][7:8]), "one row's loss")
+    within(one[1], ref[1][7], tol[1][7] + half_step(torch.float32, ref[1][7]), "one row's gradient")
+    four = torch_fl.ops.distill_topk_grad(z.view(2, 3, 2, 333), t.view(2, 3, 2, 5), ids.view(2, 3, 2, 5), 2.0,
+                                          w.view(2, 3, 2))
+    assert torch.equal(four[0].view(12), want[0]) and torch.equal(four[1].view(12, 333), want[1])
+    # weights that broadcast, logits whose rows are one row, operands transposed
+    a = torch_fl.ops.distill_topk_grad(z.view(3, 4, 333), t.view(3, 4, 5), ids.view(3, 4, 5), 2.0, w[:3, None])
+    b = K.distill_topk_grad(z, t, ids, 2.0, w[:3].repeat_interleave(4))
+    assert torch.equal(a[1].view(12, 333), b[1])
+    same = z[:1].expand(12, 333)
+    a, b = (torch_fl.ops.distill_topk_grad(v, t, ids, 2.0, w) for v in (same, same.contiguous()))
+    c = K.distill_topk_grad(same, t, ids, 2.0, w)
+    assert torch.equal(a[1], b[1]) and torch.equal(a[0], b[0]) and torch.equal(a[1], c[1])
+    a = torch_fl.ops.distill_topk_grad(z.t().contiguous().t(), t.t().contiguous().t(),
+                                       ids.t().contiguous().t(), 2.0, w)
+    assert torch.equal(a[0], want[0]) and torch.equal(a[1], want[1])
+
+
 def test_distill_results_repeat():
     z, t, ids, w = make(40, 32000, 64, torch.bfloat16, 41)
     a = K.distill_topk_grad(z, t, ids, 2.0, w)
@@ -509,6 +538,48 @@ def test_streams_and_graph_replay():
     torch.cuda.synchronize()
     fresh = all_ops()
     assert all(torch.equal(a, b) for a, b in zip(held, fresh))
+
+
+def test_two_streams_at_once():
+    """The ops share no state: runs that overlap on two streams give what each
+    gives alone."""
+    sets = []
+    for n in range(2):
+        z, t, ids, w = make(300, 30011, 40, torch.bfloat16, 81 + n)
+        sets.append((z, t, ids, w, drafts(60, 4, 30011, torch.bfloat16, 91 + n)))
+
+    def all_ops(z, t, ids, w, v):
+        return [*torch_fl.ops.topk(z, 30), *torch_fl.ops.distill_topk_grad(z, t, ids, 2.0, w),
+                torch_fl.ops.distill_topk(z, t, ids, 2.0), *torch_fl.ops.verify_draft(*v)]
+
+    want = [all_ops(*s) for s in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for n, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[n].append(all_ops(*sets[n]))
+    torch.cuda.synchronize()
+    for n in range(2):
+        for run in got[n]:
+            assert all(torch.equal(a, b) for a, b in zip(run, want[n]))
+
+
+def test_many_rows_for_few_clusters():
+    """More rows than clusters are resident: the ring of stages turns many times."""
+    for R, V, k, dt in ((3000, 513, 9, torch.bfloat16), (1500, 9000, 70, torch.float16),
+                        (700, 20001, 100, torch.float32), (400, 40000, 30, torch.bfloat16)):
+        z, t, ids, w = make(R, V, k, dt, R)
+        check_distill(z, t, ids, w, 1.7, f"{R}x{V}x{k}")
+
+
+def test_vocabularies_past_eight_ctas():
+    """Clusters of more than 8 CTAs (131072 elements of 16 bits, 65536 of fp32)
+    and rows that no cluster holds."""
+    for R, V, dt in ((5, 151936, torch.bfloat16), (4, 262144, torch.float16), (4, 70000, torch.float32),
+                     (3, 131072, torch.float32), (3, 262145, torch.bfloat16), (3, 131073, torch.float32)):
+        check_distill(*make(R, V, 20, dt, R + V % 97), tau=1.3, what=f"{R}x{V}")
 
 
 def test_draft_model_from_teacher_to_verification():

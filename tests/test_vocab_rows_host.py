@@ -86,13 +86,13 @@ def _fwd(x=16, ld=8, t=16, t_dtype=1, ids=16, ids_dtype=4, rows=2, cols=8, k=4, 
                              rows, cols, k, tau, loss, stats, dtype, None)
 
 
-def _bwd(stride=1, ld_dx=8, tau=1.0, dtype=1, stats=16, t_dtype=1, k=4):
-    return lambda: _abi.call("fl_b200_distill_topk_bwd", 16, stride, 16, 8, stats, 16, 4, t_dtype, 16,
+def _bwd(stride=1, x=32, ld_dx=8, tau=1.0, dtype=1, stats=16, t_dtype=1, k=4):
+    return lambda: _abi.call("fl_b200_distill_topk_bwd", 16, stride, x, 8, stats, 16, 4, t_dtype, 16,
                              4, 4, 16, ld_dx, None, 2, 8, k, tau, dtype, None)
 
 
 def _grad(dx=16, k=4, tau=1.0, ld_dx=8):
-    return lambda: _abi.call("fl_b200_distill_topk_grad", 16, 8, 16, 4, 1, 16, 4, 4, None, 0, 2, 8, k,
+    return lambda: _abi.call("fl_b200_distill_topk_grad", 32, 8, 16, 4, 1, 16, 4, 4, None, 0, 2, 8, k,
                              tau, 16, 16, dx, ld_dx, 1, None)
 
 
@@ -116,11 +116,11 @@ def _verify(ids=16, p=16, u=16, batch=2, drafts=3, vocab=8, tokens=16, acc=16, d
     (_fwd(tau=float("inf")), INVALID), (_fwd(rows=-1), INVALID), (_fwd(cols=0, ld=0), INVALID),
     (_fwd(ld=7), INVALID), (_fwd(k=-1), INVALID), (_fwd(k=1025), TOO_LARGE),
     (_fwd(dtype=4), DTYPE), (_fwd(t_dtype=3), DTYPE), (_fwd(ids_dtype=0), DTYPE),
-    (_bwd(stride=-1), INVALID), (_bwd(ld_dx=7), INVALID), (_bwd(tau=0.0), INVALID),
+    (_bwd(stride=-1), INVALID), (_bwd(x=16), INVALID), (_bwd(ld_dx=7), INVALID), (_bwd(tau=0.0), INVALID),
     (_bwd(dtype=3), DTYPE), (_bwd(stats=None), INVALID), (_bwd(stats=12), MISALIGNED),
     (_bwd(t_dtype=4), DTYPE), (_bwd(k=1025), TOO_LARGE),
     (_grad(dx=None), INVALID), (_grad(k=1025), TOO_LARGE), (_grad(tau=-2.0), INVALID),
-    (_grad(ld_dx=7), INVALID),
+    (_grad(ld_dx=7), INVALID), (_grad(dx=32), INVALID), (_fwd(tau=1e-38), INVALID),
     (_verify(ids=None), INVALID), (_verify(p=None), INVALID), (_verify(u=None), INVALID),
     (_verify(tokens=None), INVALID), (_verify(acc=None), INVALID), (_verify(vocab=0), INVALID),
     (_verify(batch=-1), INVALID), (_verify(drafts=-1), INVALID), (_verify(dtype=4), DTYPE),
@@ -130,6 +130,25 @@ def test_bad_arguments_are_refused_on_the_host(call, status):
     with pytest.raises(_abi.FlB200Error) as e:
         call()
     assert e.value.status == status
+
+
+def test_tensor_entry_points_refuse_before_they_launch():
+    """K.*: shapes, types and CPU tensors are refused on the host."""
+    import torch
+
+    from torch_fl import kernels as K
+
+    x, t, ids = torch.zeros(4, 100), torch.zeros(4, 3), torch.zeros(4, 3, dtype=torch.int64)
+    p, u = torch.zeros(4, 4, 100), torch.zeros(4, 4)
+    for bad in (lambda: K.topk_lastdim(x, 2), lambda: K.topk_backward(t, ids, 100),
+                lambda: K.topk_backward(t, ids.int(), 100), lambda: K.distill_topk(x, t, ids),
+                lambda: K.distill_topk(x, t, ids.float()), lambda: K.distill_topk(x, t[:3], ids[:3]),
+                lambda: K.distill_topk_grad(x, t, ids, 1.0, out=x), lambda: K.verify_draft(ids, p, None, u),
+                lambda: K.verify_draft(ids.int(), p, None, u), lambda: K.verify_draft(ids, p[:, :3], None, u),
+                lambda: K.verify_draft(ids, p, p, u), lambda: K.verify_draft(ids, p, None, u[:, :2]),
+                lambda: K.verify_draft(ids, p, None, u, ids[0])):
+        with pytest.raises((RuntimeError, ValueError, TypeError)):
+            bad()
 
 
 def test_empty_work_is_a_no_op():
