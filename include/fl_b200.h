@@ -440,7 +440,7 @@ FL_B200_API int fl_b200_distill_topk_fwd(const void* logits, int64_t ld, const v
 /* Gradients for dloss[r * dloss_stride] (F32; NULL: 1 for every row):       *
  *   dlogits_v = dloss * temperature * (q_v - sum over id_j = v of p_j),      *
  *   dteacher_j = dloss * temperature * p_j (log p_j - log q[id_j] - KL).    *
- * dlogits (logits' dtype, stride ld_dlogits; not in place) and dteacher     *
+ * dlogits (logits' dtype, stride ld_dlogits; never logits) and dteacher     *
  * (the teacher's dtype, dense [rows, k]) may each be NULL.  Rows are stored *
  * 16 bytes at a time when the logits' and the gradient's rows begin at the   *
  * same offset from a 16-byte boundary, one element at a time otherwise.     */
@@ -452,7 +452,12 @@ FL_B200_API int fl_b200_distill_topk_bwd(const float* dloss, int64_t dloss_strid
                                          int64_t rows, int64_t cols, int64_t k, float temperature,
                                          int dtype, fl_b200_stream_t stream);
 /* Loss and dlogits at once, for row weights that are known beforehand       *
- * (row_weight takes dloss's place).  stats as in the forward.               */
+ * (row_weight takes dloss's place).  stats as in the forward.  The logits   *
+ * are read once and dlogits written once when the rows' offsets agree as    *
+ * above, a row has at most 262144 elements of 16 bits or 131072 of 32, and  *
+ * k <= 128; otherwise the forward and the backward run one after the other. *
+ * On the first way, a cluster whose parts fail to meet within seconds       *
+ * gives NaN instead of waiting on.                                          */
 FL_B200_API int fl_b200_distill_topk_grad(const void* logits, int64_t ld, const void* teacher,
                                           int64_t ld_t, int t_dtype, const void* ids,
                                           int64_t ld_ids, int ids_dtype, const float* row_weight,

@@ -140,7 +140,10 @@ struct Row {
 // A cluster of CTAs a sequence.  Every CTA judges the drafts for itself; the
 // row is cut into one segment a warp, in index order, and each warp sums its
 // own; the CTAs' totals meet through distributed shared memory, and the CTA
-// that has the mark walks the one segment that holds it again.
+// that has the mark walks the one segment that holds it again.  Bound by the
+// latency of these steps in turn, then by HBM: 256 sequences of 5 drafts over
+// 128256 fp32 in 47 us (197 MB read: 4.2 TB/s), one over 32000 in 5.2 us.  The
+// pipe that converts to 64-bit integers is busy 17% of the time.
 template <typename T>
 __global__ void __launch_bounds__(kBlock, 4) verify_kernel(VerifyArgs<T> a) {
   constexpr int VW = Elem<T>::kVec;
