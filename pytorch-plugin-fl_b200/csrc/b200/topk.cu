@@ -13,6 +13,7 @@ constexpr int kMaxTop = FL_B200_TOPK_MAX;
 constexpr int kPacks = 8;     // 16-byte packs a thread has in flight
 constexpr int kCap = 2048;    // candidates kept
 constexpr int kShared = 512;  // the longest list that clusters exchange
+constexpr int kRank = 256;    // up to as many keys are placed by counting the larger ones
 
 // Monotone 32-bit image of a value: unsigned order is float order, NaN on
 // top; never 0.
@@ -78,7 +79,7 @@ struct Shared {
     uint64_t top[kShared];  // this slice's largest, for CTA 0
     uint16_t list[kChunk];  // groups of packs that hold candidates
   };
-  int sums[2][kWarps];
+  int2 sums[2][kWarps];
   uint32_t run[B];  // the threads' maxima
   int hist[256];
   uint32_t least;
@@ -98,37 +99,37 @@ __device__ __forceinline__ int take_slot(int* counter) {
   return slot;
 }
 
-// Sum of v over the CTA, in every thread.  `parity` alternates between the
+// Sums over the CTA, in every thread, of three counts (at most 2^15 in all)
+// given as (first, second << 16) and third.  `parity` alternates between the
 // two halves of the scratch, so that one barrier a call is enough.
 template <int B>
-__device__ __forceinline__ int block_sum(Shared<B>& s, int v, int& parity) {
+__device__ __forceinline__ void block_sum3(Shared<B>& s, int& n12, int& n3, int& parity) {
   constexpr int kWarps = B / 32;
   const int lane = threadIdx.x & 31;
-  v = __reduce_add_sync(0xffffffffu, v);
-  if (lane == 0) s.sums[parity][threadIdx.x >> 5] = v;
+  n12 = __reduce_add_sync(0xffffffffu, n12);
+  n3 = __reduce_add_sync(0xffffffffu, n3);
+  if (lane == 0) s.sums[parity][threadIdx.x >> 5] = make_int2(n12, n3);
   __syncthreads();
-  v = __reduce_add_sync(0xffffffffu, lane < kWarps ? s.sums[parity][lane] : 0);
+  const int2 v = lane < kWarps ? s.sums[parity][lane] : make_int2(0, 0);
+  n12 = __reduce_add_sync(0xffffffffu, v.x);
+  n3 = __reduce_add_sync(0xffffffffu, v.y);
   parity ^= 1;
-  return v;
 }
 
 // A key K that at least k of the counted keys reach, and at most `enough`
-// where that is possible: found bit by bit below the bits that `lo` and `hi`
-// share, all counted keys lying between these two.  count(K) is the thread's
-// own number of keys >= K.
+// where that is possible: found from the top, two bits a step.  count(K) is
+// the thread's own number of keys >= K.
 template <typename K, int B, typename F>
-__device__ __forceinline__ K bisect(Shared<B>& s, K lo, K hi, int k, int enough, int& parity, F count) {
-  K at = lo;
-  int bit = (int)sizeof(K) * 8 - 1;
-  while (bit >= 0 && (((lo ^ hi) >> bit) & 1) == 0) --bit;
-  at = bit < 0 ? lo : (lo >> bit >> 1) << bit << 1;
-  for (; bit >= 0; --bit) {
-    const K tried = at | ((K)1 << bit);
-    const int n = block_sum(s, count(tried), parity);
-    if (n >= k) {
-      at = tried;
-      if (n <= enough) break;
-    }
+__device__ __forceinline__ K bisect(Shared<B>& s, int k, int enough, int& parity, F count) {
+  K at = 0;
+  for (int bit = (int)sizeof(K) * 8 - 2; bit >= 0; bit -= 2) {
+    const K one = (K)1 << bit;
+    int n12 = count(at + one) + (count(at + 2 * one) << 16), n3 = count(at + 3 * one);
+    block_sum3(s, n12, n3, parity);
+    const int n1 = n12 & 0xffff, n2 = n12 >> 16;
+    const int reached = n3 >= k ? n3 : n2 >= k ? n2 : n1 >= k ? n1 : 0;
+    at += n3 >= k ? 3 * one : n2 >= k ? 2 * one : n1 >= k ? one : 0;
+    if (reached != 0 && reached <= enough) break;
   }
   return at;
 }
@@ -223,12 +224,12 @@ __device__ __noinline__ void select_any(Shared<B>& s, const T* xr, int lo, int h
     const float f = i < hi ? Elem<T>::to_f(xr[i]) : 0.f;
     const bool is = i < hi && value_key(f) >> (32 - kBits) == value;
     const uint32_t vote = __ballot_sync(0xffffffffu, is);
-    if (lane == 0) s.sums[parity][tid >> 5] = __popc(vote);
+    if (lane == 0) s.sums[parity][tid >> 5].x = __popc(vote);
     __syncthreads();
     int before = taken, total = 0;
     for (int w = 0; w < B / 32; ++w) {
-      if (w < tid >> 5) before += s.sums[parity][w];
-      total += s.sums[parity][w];
+      if (w < tid >> 5) before += s.sums[parity][w].x;
+      total += s.sums[parity][w].x;
     }
     parity ^= 1;
     if (is && before + __popc(vote & ((1u << lane) - 1)) < need) append(s, element_key(f, (uint32_t)i));
@@ -299,7 +300,7 @@ __device__ __forceinline__ void issue(Shared<B>& s, const Packs& src, int base, 
 // and in a row without order little over k elements reach it.  Only the packs
 // of the groups that do, about k of kChunk, are read again (from L2) for their
 // elements.  Elements equal to the threshold are kept, so ties are settled by
-// index at the end.  For k <= B / 2 the k-th largest of the threads' maxima
+// index at the end.  For k <= 5 B / 8 the k-th largest of the threads' maxima
 // serves, which one warp finds: a little lower, and without a barrier a step.
 template <typename T, int B>
 __device__ __forceinline__ int collect(Shared<B>& s, const T* xr, int lo, int hi, int k,
@@ -341,7 +342,7 @@ __device__ __forceinline__ int collect(Shared<B>& s, const T* xr, int lo, int hi
     most = max(most, group[i]);
   }
   uint32_t least;
-  if (k <= B / 2) {
+  if (k <= 5 * B / 8) {
     s.run[tid] = most;
     __syncthreads();
     if (warp == 0) {
@@ -352,7 +353,7 @@ __device__ __forceinline__ int collect(Shared<B>& s, const T* xr, int lo, int hi
     least = s.least;
   } else {
     __syncthreads();
-    least = bisect<uint32_t>(s, 0u, ~0u, k, k + k / 8, parity, [&](uint32_t c) {
+    least = bisect<uint32_t>(s, k, k + k / 8, parity, [&](uint32_t c) {
       int m = 0;
 #pragma unroll
       for (int i = 0; i < kPacks; ++i) m += group[i] >= c;
@@ -432,7 +433,7 @@ topk_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int cols, int k, 
     const RowSplit sp = split_row(at, hi - lo);
     return Packs{reinterpret_cast<const uint4*>(at + sp.head), sp.nvec};
   };
-  const int most = max(k + k / 4, 128);  // keys to order at the end
+  const int most = max(k + k / 4, kRank);  // keys to order at the end
   const int64_t step = cluster_count();
   issue(s, packs_of(cluster_id()), 0, 0);
   issue(s, packs_of(cluster_id()), 0, 1);
@@ -445,7 +446,7 @@ topk_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int cols, int k, 
     }
     // to a few more than k at most, without their order
     const auto shrink = [&](int most) {
-      const uint64_t f = bisect<uint64_t>(s, 0ull, ~0ull, min(k, n), most, parity, [&](uint64_t c) {
+      const uint64_t f = bisect<uint64_t>(s, min(k, n), most, parity, [&](uint64_t c) {
         int m = 0;
         for (int j = tid; j < n; j += B) m += s.cand[j] >= c;
         return m;
@@ -474,7 +475,7 @@ topk_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int cols, int k, 
     if (n > most) shrink(most);
     if (C > 1) {
       // this slice's k largest, 0 past the last
-      if (n <= B / 2) {
+      if (n <= kRank) {
         for (int i = tid; i < k; i += B) s.top[i] = 0;
         __syncthreads();
         place_all([&](int place, uint64_t key) { s.top[place] = key; });
@@ -501,7 +502,7 @@ topk_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int cols, int k, 
         values[row * k + place] =
             v == 0x80000000u || v == 0xffffffffu ? xr[at] : Elem<T>::from_f(key_value(v));
       };
-      if (n <= B / 2) {
+      if (n <= kRank) {
         place_all(put);
       } else {
         int size = 1;
