@@ -87,17 +87,18 @@ struct Shared {
   uint4 stage[kPacks][B];  // packs on their way, each thread its own
 };
 
-// One more of `*counter`: the old value.  (Inline: these are rare, and what
+// `n` more of `*counter`: the old value.  (Inline: these are rare, and what
 // the compiler does to share one atomic among a warp's lanes costs more than
 // it saves.)
-__device__ __forceinline__ int take_slot(int* counter) {
+__device__ __forceinline__ int take_slots(int* counter, int n) {
   int slot;
-  asm volatile("atom.shared.add.s32 %0, [%1], 1;"
+  asm volatile("atom.shared.add.s32 %0, [%1], %2;"
                : "=r"(slot)
-               : "r"((uint32_t)__cvta_generic_to_shared(counter))
+               : "r"((uint32_t)__cvta_generic_to_shared(counter)), "r"(n)
                : "memory");
   return slot;
 }
+__device__ __forceinline__ int take_slot(int* counter) { return take_slots(counter, 1); }
 
 // Sums over the CTA, in every thread, of three counts (at most 2^15 in all)
 // given as (first, second << 16) and third.  `parity` alternates between the
@@ -117,14 +118,18 @@ __device__ __forceinline__ void block_sum3(Shared<B>& s, int& n12, int& n3, int&
 }
 
 // A key K that at least k of the counted keys reach, and at most `enough`
-// where that is possible: found from the top, two bits a step.  count(K) is
-// the thread's own number of keys >= K.
+// where that is possible: found from the top, two bits a step.  visit(see)
+// calls see for each of the thread's own keys.
 template <typename K, int B, typename F>
-__device__ __forceinline__ K bisect(Shared<B>& s, int k, int enough, int& parity, F count) {
+__device__ __forceinline__ K bisect(Shared<B>& s, int k, int enough, int& parity, F visit) {
   K at = 0;
   for (int bit = (int)sizeof(K) * 8 - 2; bit >= 0; bit -= 2) {
     const K one = (K)1 << bit;
-    int n12 = count(at + one) + (count(at + 2 * one) << 16), n3 = count(at + 3 * one);
+    int n12 = 0, n3 = 0;
+    visit([&](K key) {
+      n12 += (key >= at + one) + ((key >= at + 2 * one) << 16);
+      n3 += key >= at + 3 * one;
+    });
     block_sum3(s, n12, n3, parity);
     const int n1 = n12 & 0xffff, n2 = n12 >> 16;
     const int reached = n3 >= k ? n3 : n2 >= k ? n2 : n1 >= k ? n1 : 0;
@@ -353,11 +358,9 @@ __device__ __forceinline__ int collect(Shared<B>& s, const T* xr, int lo, int hi
     least = s.least;
   } else {
     __syncthreads();
-    least = bisect<uint32_t>(s, k, k + k / 8, parity, [&](uint32_t c) {
-      int m = 0;
+    least = bisect<uint32_t>(s, k, k + k / 8, parity, [&](auto see) {
 #pragma unroll
-      for (int i = 0; i < kPacks; ++i) m += group[i] >= c;
-      return m;
+      for (int i = 0; i < kPacks; ++i) see(group[i]);
     });
   }
   if (single >= 0) append(s, element_key(alone, (uint32_t)(lo + single)));
@@ -446,10 +449,8 @@ topk_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int cols, int k, 
     }
     // to a few more than k at most, without their order
     const auto shrink = [&](int most) {
-      const uint64_t f = bisect<uint64_t>(s, min(k, n), most, parity, [&](uint64_t c) {
-        int m = 0;
-        for (int j = tid; j < n; j += B) m += s.cand[j] >= c;
-        return m;
+      const uint64_t f = bisect<uint64_t>(s, min(k, n), most, parity, [&](auto see) {
+        for (int j = tid; j < n; j += B) see(s.cand[j]);
       });
       keep_above(s, n, f);
       n = s.filled;
@@ -519,6 +520,244 @@ topk_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int cols, int k, 
 
 constexpr int kBlock = 512;
 
+// The same with a warp a row, for many short rows: the CTA's barriers, one
+// after the other, took most of a short row's time (20000 x 1024 bf16, top 8,
+// 411 us against 45; 3916 x 5266, top 7, 90 against 21).  The warp's 256 slots
+// are the groups; threshold, second look and order run on shuffles and a list
+// in shared memory.
+constexpr int kRowWarps = 4;
+constexpr int kRowCap = 512;     // candidates listed
+constexpr int kRowSorted = 256;  // candidates put in order
+constexpr int kRowTop = 128;     // the largest k: half the slots, which some 180 elements reach
+
+struct RowShared {
+  uint64_t cand[kRowWarps][kRowCap];
+  uint8_t list[kRowWarps][256];  // slots that hold candidates
+  int filled[kRowWarps];
+};
+
+// Descending bitonic sort of n <= 32 N keys by a warp, N neighbours a lane:
+// shuffles only where partners are in two lanes.
+template <int N>
+__device__ __forceinline__ void warp_sort(uint64_t* keys, int n, int lane) {
+  uint64_t v[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = lane * N + i < n ? keys[lane * N + i] : 0;
+  const auto swap = [](uint64_t& a, uint64_t& b, bool larger_first) {
+    const uint64_t hi = a > b ? a : b, lo = a > b ? b : a;
+    a = larger_first ? hi : lo;
+    b = larger_first ? lo : hi;
+  };
+#pragma unroll
+  for (int size = 2; size <= N; size <<= 1) {
+#pragma unroll
+    for (int stride = size >> 1; stride > 0; stride >>= 1) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if ((i & stride) == 0) swap(v[i], v[i + stride], ((lane * N + i) & size) == 0);
+    }
+  }
+#pragma unroll 1
+  for (int lanes = 2; lanes <= 32; lanes <<= 1) {
+    const bool down = (lane & lanes) == 0;
+#pragma unroll 1
+    for (int other = lanes >> 1; other > 0; other >>= 1) {
+      const bool larger = ((lane & other) == 0) == down;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const uint64_t o = __shfl_xor_sync(0xffffffffu, v[i], other);
+        v[i] = (o > v[i]) == larger ? o : v[i];
+      }
+    }
+#pragma unroll
+    for (int stride = N >> 1; stride > 0; stride >>= 1) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if ((i & stride) == 0) swap(v[i], v[i + stride], down);
+    }
+  }
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < N; ++i) keys[lane * N + i] = v[i];
+  __syncwarp();
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kRowWarps * 32, 32 / kRowWarps)
+topk_rows_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int cols, int k,
+                 T* __restrict__ values, int64_t* __restrict__ indices) {
+  constexpr int VW = Elem<T>::kVec;
+  constexpr int S = 8, kChunk = 32 * S;
+  // the lowest bits that tell two values' keys apart
+  constexpr int kLast = std::is_same<T, float>::value ? 0 : std::is_same<T, __half>::value ? 12 : 16;
+  __shared__ RowShared s;
+  pdl_prologue();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  uint64_t* cand = s.cand[warp];
+  uint8_t* list = s.list[warp];
+  int* filled = &s.filled[warp];
+  const auto keep = [&](uint64_t key) {
+    const int slot = take_slot(filled);
+    if (slot < kRowCap) cand[slot] = key;
+  };
+  const int64_t step = (int64_t)gridDim.x * kRowWarps;
+  for (int64_t row = (int64_t)blockIdx.x * kRowWarps + warp; row < rows; row += step) {
+    const T* xr = x + row * ld;
+    const RowSplit sp = split_row(xr, cols);
+    const uint4* body = reinterpret_cast<const uint4*>(xr + sp.head);
+    const int single = single_of(sp, lane, VW);
+    const float alone = single >= 0 ? Elem<T>::to_f(xr[single]) : 0.f;
+    if (lane == 0) *filled = 0;
+    uint32_t v[S];
+#pragma unroll
+    for (int i = 0; i < S; ++i) v[i] = word_lowest<T>();
+    for (int base = lane; base < sp.nvec; base += kChunk) {
+      uint4 u[S];
+#pragma unroll
+      for (int i = 0; i < S; ++i)
+        if (base + 32 * i < sp.nvec) u[i] = ld_cached(body + base + 32 * i);
+#pragma unroll
+      for (int i = 0; i < S; ++i)
+        if (base + 32 * i < sp.nvec) v[i] = word_max<T>(v[i], pack_max<T>(u[i]));
+    }
+    uint32_t lo = 0xffffffffu, hi = 0;
+#pragma unroll
+    for (int i = 0; i < S; ++i) {
+      v[i] = lane + 32 * i < sp.nvec ? value_key(word_top<T>(v[i])) : 0;
+      lo = min(lo, v[i] - 1);  // (slots without a pack aside)
+      hi = max(hi, v[i]);
+    }
+    // the k-th largest of the slots' maxima, as in kth_maximum
+    lo = __reduce_min_sync(0xffffffffu, lo) + 1;
+    hi = __reduce_max_sync(0xffffffffu, hi);
+    const int top = (32 - __clz(lo ^ hi) + 1) & ~1;
+    uint32_t least = top < 32 ? lo >> top << top : 0;
+    for (int bit = top - 2; bit >= kLast; bit -= 2) {
+      const uint32_t one = 1u << bit;
+      int n = 0;
+#pragma unroll
+      for (int i = 0; i < S; ++i)
+        n += (v[i] >= least + one) + ((v[i] >= least + 2 * one) << 10) + ((v[i] >= least + 3 * one) << 20);
+      n = __reduce_add_sync(0xffffffffu, n);
+      const int n3 = n >> 20, n2 = (n >> 10) & 1023, n1 = n & 1023;
+      const int reached = n3 >= k ? n3 : n2 >= k ? n2 : n1 >= k ? n1 : 0;
+      least += n3 >= k ? 3 * one : n2 >= k ? 2 * one : n1 >= k ? one : 0;
+      if (reached != 0 && reached <= k + k / 8) break;
+    }
+    // the slots that reach it, and their packs' elements
+    uint32_t listed = 0;
+#pragma unroll
+    for (int i = 0; i < S; ++i) {
+      const bool in = v[i] >= max(least, 1u);
+      const uint32_t vote = __ballot_sync(0xffffffffu, in);
+      if (in) list[listed + __popc(vote & ((1u << lane) - 1))] = (uint8_t)(lane + 32 * i);
+      listed += __popc(vote);
+    }
+    __syncwarp();
+    if (single >= 0) keep(element_key(alone, (uint32_t)single));
+    const uint32_t depth = (sp.nvec + kChunk - 1) / kChunk, items = listed * depth;
+    for (uint32_t base = lane; base < items; base += 64) {
+      uint4 u[2];
+      int p[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t item = base + 32 * i, chunk = item / listed;
+        p[i] = item < items ? list[item - chunk * listed] + (int)(chunk * kChunk) : sp.nvec;
+        if (p[i] < sp.nvec) u[i] = ld_cached(body + p[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (p[i] >= sp.nvec) continue;
+        float f[VW];
+        unpack<T>(u[i], f);
+        uint32_t reach = 0;
+#pragma unroll
+        for (int j = 0; j < VW; ++j) reach |= (uint32_t)(value_key(f[j]) >= least) << j;
+        if (reach == 0) continue;
+        const int first = take_slots(filled, __popc(reach));
+#pragma unroll
+        for (int j = 0; j < VW; ++j) {
+          const int slot = first + __popc(reach & ((1u << j) - 1));
+          if ((reach >> j & 1) && slot < kRowCap)
+            cand[slot] = element_key(f[j], (uint32_t)(sp.head + p[i] * VW + j));
+        }
+      }
+    }
+    __syncwarp();
+    int n = *filled;
+    if (n > kRowSorted) {
+      // long ties and rows in order: a key that k to kRowSorted keys reach, two
+      // bits a walk over the list, or over the row where that did not fit
+      const bool listed_all = n <= kRowCap;
+      const auto each = [&](auto see) {
+        if (listed_all) {
+          for (int i = lane; i < n; i += 32) see(cand[i]);
+          return;
+        }
+        if (single >= 0) see(element_key(alone, (uint32_t)single));
+        for (int p = lane; p < sp.nvec; p += 32) {
+          float f[VW];
+          unpack<T>(ld_cached(body + p), f);
+#pragma unroll
+          for (int j = 0; j < VW; ++j) see(element_key(f[j], (uint32_t)(sp.head + p * VW + j)));
+        }
+      };
+      uint64_t at = 0;
+      for (int bit = 62; bit >= 0; bit -= 2) {
+        const uint64_t one = (uint64_t)1 << bit;
+        int n1 = 0, n2 = 0, n3 = 0;
+        each([&](uint64_t key) {
+          n1 += key >= at + one;
+          n2 += key >= at + 2 * one;
+          n3 += key >= at + 3 * one;
+        });
+        n1 = __reduce_add_sync(0xffffffffu, n1);
+        n2 = __reduce_add_sync(0xffffffffu, n2);
+        n3 = __reduce_add_sync(0xffffffffu, n3);
+        const int reached = n3 >= k ? n3 : n2 >= k ? n2 : n1 >= k ? n1 : 0;
+        at += n3 >= k ? 3 * one : n2 >= k ? 2 * one : n1 >= k ? one : 0;
+        if (reached != 0 && reached <= kRowSorted) break;
+      }
+      if (listed_all) {
+        int kept = 0;
+        for (int i = 0; i < n; i += 32) {
+          const uint64_t key = i + lane < n ? cand[i + lane] : 0;
+          const uint32_t vote = __ballot_sync(0xffffffffu, key >= at && key != 0);
+          __syncwarp();
+          if (vote >> lane & 1) cand[kept + __popc(vote & ((1u << lane) - 1))] = key;
+          kept += __popc(vote);
+          __syncwarp();
+        }
+        n = kept;
+      } else {
+        if (lane == 0) *filled = 0;
+        __syncwarp();
+        each([&](uint64_t key) {
+          if (key >= at) keep(key);
+        });
+        __syncwarp();
+        n = *filled;
+      }
+    }
+    if (n <= 32) {
+      warp_sort<1>(cand, n, lane);
+    } else if (n <= 64) {
+      warp_sort<2>(cand, n, lane);
+    } else if (n <= 128) {
+      warp_sort<4>(cand, n, lane);
+    } else {
+      warp_sort<8>(cand, n, lane);
+    }
+    for (int i = lane; i < k; i += 32) {
+      const uint64_t key = cand[i];
+      const uint32_t at = ~(uint32_t)key, w = (uint32_t)(key >> 32);
+      indices[row * k + i] = at;
+      values[row * k + i] = w == 0x80000000u || w == 0xffffffffu ? xr[at] : Elem<T>::from_f(key_value(w));
+    }
+    __syncwarp();  // the next row's candidates take these ones' place
+  }
+}
+
 // Gradient: zeros, and dvalues at the indices (distinct in a row).
 template <typename T>
 __global__ void __launch_bounds__(kBlock)
@@ -558,6 +797,15 @@ FL_B200_API int fl_b200_topk_lastdim(const void* x, int64_t ld, int64_t rows, in
   if (st != FL_B200_OK) return st;
   return dispatch_float(dtype, [&](auto t) {
     using T = decltype(t);
+    // many rows of at most 32 KB with at least 2 k packs: a warp a row
+    if (rows >= 8 * dev.sm_count && cols * (int64_t)sizeof(T) <= 32768 && k <= kRowTop &&
+        cols / Elem<T>::kVec >= 2 * k) {
+      const int64_t ctas = std::min<int64_t>(ceil_div(rows, kRowWarps), 32 / kRowWarps * dev.sm_count);
+      launch_k(topk_rows_kernel<T>, dim3((unsigned)ctas), dim3(kRowWarps * 32), 0, (cudaStream_t)stream,
+               reinterpret_cast<const T*>(x), ld, rows, (int)cols, (int)k, reinterpret_cast<T*>(values),
+               indices);
+      return launch_status();
+    }
     const auto go = [&](auto block) {
       constexpr int B = decltype(block)::value;
       // few rows: up to 8 CTAs a row, with two packs a thread at least, whose

@@ -57,9 +57,10 @@ def check_topk(x, k, what="", fn=K.topk_lastdim):
     x2 = x.reshape(-1, x.shape[-1])
     _, gi = ops.topk_golden(np64(x2), k)
     np.testing.assert_array_equal(i.cpu().numpy().reshape(-1, k), gi, err_msg=what)
-    want = torch.gather(x2.cpu(), -1, torch.from_numpy(gi)).reshape(v.shape)
     bits = torch.int32 if x.dtype == torch.float32 else torch.int16
-    assert torch.equal(v.cpu().view(bits), want.view(bits)), what  # the elements' own bits
+    # gathered as integers: a gather of bfloat16 on the CPU may give a NaN other bits
+    want = torch.gather(x2.cpu().view(bits), -1, torch.from_numpy(gi)).reshape(v.shape)
+    assert torch.equal(v.cpu().view(bits), want), what  # the elements' own bits
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -73,8 +74,24 @@ def test_topk(dtype, rows, cols, k):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-def test_topk_special_rows(dtype):
-    V = 20011
+@pytest.mark.parametrize("rows,cols,k", [(1300, 1001, 1), (1250, 4096, 130), (2500, 2053, 17), (1200, 513, 30),
+                                         (1184, 8100, 256), (1500, 3003, 100)])
+def test_topk_many_short_rows(dtype, rows, cols, k):
+    x = (2.5 * torch.randn(rows, cols, generator=gen(rows + k))).to(dtype)
+    x[3] = 1.0                                       # nothing but ties
+    x[4] = torch.arange(cols)
+    x[5] = -torch.arange(cols).float()
+    x[6, 7:] = -float("inf")
+    x[7, ::3] = float("nan")
+    x[8] = torch.where(torch.arange(cols) % 2 == 0, -0.0, 0.0)
+    x[9] = torch.finfo(dtype).min
+    check_topk(x.to(DEV), k)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("copies", [1, 120])
+def test_topk_special_rows(dtype, copies):
+    V = 20011 if copies == 1 else 5003
     g = gen(3)
     base = torch.randn(V, generator=g)
     rows = [torch.zeros(V), torch.full((V,), -float("inf")), torch.arange(V, 0, -1).float(),
@@ -88,8 +105,9 @@ def test_topk_special_rows(dtype):
     few[[V - 1, 3]] = torch.tensor([1.0, 2.0])
     last = torch.full((V,), -1.0)
     last[-300:] = 1.0
-    x = torch.stack(rows + [nan, inf, few, last, torch.full((V,), float("nan"))]).to(dtype).to(DEV)
-    for k in (1, 40, 300, 1024):
+    x = torch.stack(rows + [nan, inf, few, last, torch.full((V,), float("nan"))]).to(dtype)
+    x = x.repeat(copies, 1).to(DEV)
+    for k in (1, 40, 300, 1024) if copies == 1 else (1, 40, 255):
         check_topk(x, k, f"k={k}")
 
 
