@@ -797,8 +797,13 @@ FL_B200_API int fl_b200_topk_lastdim(const void* x, int64_t ld, int64_t rows, in
   if (st != FL_B200_OK) return st;
   return dispatch_float(dtype, [&](auto t) {
     using T = decltype(t);
-    // many rows of at most 32 KB with at least 2 k packs: a warp a row
-    if (rows >= 8 * dev.sm_count && cols * (int64_t)sizeof(T) <= 32768 && k <= kRowTop &&
+    // More rows of at most 32 KB than CTAs of 256 threads fit: a warp a row, if
+    // k is at most half the row's packs (1000 x 8000 bf16, top 64: 17.9 us, 28.5
+    // with a CTA a row).  Above 16 KB a warp's chain of steps is long: with a
+    // large k it takes more rows to hide (600 x 16000, top 64: 27.0 us, 19.0
+    // with a CTA a row; 1300 rows, top 128: 51.3 and 54.3).
+    const int64_t bytes = cols * (int64_t)sizeof(T);
+    if (rows > (bytes <= 16384 || k <= 32 ? 4 : 8) * dev.sm_count && bytes <= 32768 && k <= kRowTop &&
         cols / Elem<T>::kVec >= 2 * k) {
       const int64_t ctas = std::min<int64_t>(ceil_div(rows, kRowWarps), 32 / kRowWarps * dev.sm_count);
       launch_k(topk_rows_kernel<T>, dim3((unsigned)ctas), dim3(kRowWarps * 32), 0, (cudaStream_t)stream,

@@ -75,7 +75,7 @@ def test_topk(dtype, rows, cols, k):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rows,cols,k", [(1300, 1001, 1), (1250, 4096, 130), (2500, 2053, 17), (1200, 513, 30),
-                                         (1184, 8100, 256), (1500, 3003, 100)])
+                                         (1184, 8100, 256), (1500, 3003, 100), (593, 8001, 33), (900, 15999, 20)])
 def test_topk_many_short_rows(dtype, rows, cols, k):
     x = (2.5 * torch.randn(rows, cols, generator=gen(rows + k))).to(dtype)
     x[3] = 1.0                                       # nothing but ties
