@@ -120,13 +120,13 @@ __device__ __forceinline__ void block_sum3(Shared<B>& s, int& n12, int& n3, int&
 // A key K that at least k of the counted keys reach, and at most `enough`
 // where that is possible: found from the top, two bits a step.  visit(see)
 // calls see for each of the thread's own keys.
-template <typename K, int B, typename F>
-__device__ __forceinline__ K bisect(Shared<B>& s, int k, int enough, int& parity, F visit) {
-  K at = 0;
-  for (int bit = (int)sizeof(K) * 8 - 2; bit >= 0; bit -= 2) {
-    const K one = (K)1 << bit;
+template <int B, typename F>
+__device__ __forceinline__ uint32_t bisect(Shared<B>& s, int k, int enough, int& parity, F visit) {
+  uint32_t at = 0;
+  for (int bit = 30; bit >= 0; bit -= 2) {
+    const uint32_t one = 1u << bit;
     int n12 = 0, n3 = 0;
-    visit([&](K key) {
+    visit([&](uint32_t key) {
       n12 += (key >= at + one) + ((key >= at + 2 * one) << 16);
       n3 += key >= at + 3 * one;
     });
@@ -145,41 +145,100 @@ __device__ __forceinline__ void append(Shared<B>& s, uint64_t key) {
   if (slot < kCap) s.cand[slot] = key;
 }
 
-// Keeps the candidates at or above a 64-bit key.
-template <int B>
-__device__ __forceinline__ void keep_above(Shared<B>& s, int n, uint64_t floor) {
-  uint64_t mine[kCap / B];
-#pragma unroll
-  for (int i = 0; i < kCap / B; ++i) {
-    const int j = threadIdx.x + i * B;
-    mine[i] = j < n ? s.cand[j] : 0;
-  }
-  __syncthreads();
-  if (threadIdx.x == 0) s.filled = 0;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < kCap / B; ++i)
-    if (mine[i] >= floor && mine[i] != 0) append(s, mine[i]);
-  __syncthreads();
+// Descending bitonic sort, N neighbours a thread, t its place.  Partners in
+// two lanes meet by shuffles, those in two warps through shared memory.
+__device__ __forceinline__ void order(uint64_t& a, uint64_t& b, bool larger_first) {
+  const uint64_t hi = a > b ? a : b, lo = a > b ? b : a;
+  a = larger_first ? hi : lo;
+  b = larger_first ? lo : hi;
 }
-
-// Descending bitonic sort of the first n candidates, n a power of two.
-template <int B>
-__device__ __forceinline__ void sort_desc(Shared<B>& s, int n) {
-  for (int size = 2; size <= n; size <<= 1) {
-    for (int stride = size >> 1; stride > 0; stride >>= 1) {
-      __syncthreads();
-      for (int i = threadIdx.x; i < n / 2; i += B) {
-        const int lo = 2 * i - (i & (stride - 1));
-        const uint64_t a = s.cand[lo], b = s.cand[lo + stride];
-        if ((a < b) == ((lo & size) == 0)) {
-          s.cand[lo] = b;
-          s.cand[lo + stride] = a;
-        }
-      }
+// The steps of one merge of `lanes` lanes' keys.
+template <int N>
+__device__ __forceinline__ void merge_lanes(uint64_t (&v)[N], int lane, int lanes, bool down) {
+#pragma unroll 1
+  for (int other = lanes >> 1; other > 0; other >>= 1) {
+    const bool larger = ((lane & other) == 0) == down;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const uint64_t o = __shfl_xor_sync(0xffffffffu, v[i], other);
+      v[i] = (o > v[i]) == larger ? o : v[i];
     }
   }
+#pragma unroll
+  for (int stride = N >> 1; stride > 0; stride >>= 1) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if ((i & stride) == 0) order(v[i], v[i + stride], down);
+  }
+}
+// A warp's 32 N keys, the largest first where bit 5 of t is 0, else last.
+template <int N>
+__device__ __forceinline__ void sort_lanes(uint64_t (&v)[N], int t) {
+#pragma unroll
+  for (int size = 2; size <= N; size <<= 1) {
+#pragma unroll
+    for (int stride = size >> 1; stride > 0; stride >>= 1) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if ((i & stride) == 0) order(v[i], v[i + stride], ((t * N + i) & size) == 0);
+    }
+  }
+#pragma unroll 1
+  for (int lanes = 2; lanes <= 32; lanes <<= 1) merge_lanes(v, t, lanes, (t & lanes) == 0);
+}
+// n <= 32 N keys, by a warp.
+template <int N>
+__device__ __forceinline__ void warp_sort(uint64_t* keys, int n, int lane) {
+  uint64_t v[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = lane * N + i < n ? keys[lane * N + i] : 0;
+  sort_lanes(v, lane);
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < N; ++i) keys[lane * N + i] = v[i];
+  __syncwarp();
+}
+// n <= B N candidates, by the CTA.
+template <int N, int B>
+__device__ __forceinline__ void block_sort(Shared<B>& s, int n) {
+  const int t = threadIdx.x;
+  uint64_t v[N];
+  uint64_t* mine = s.cand + t * N;
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = t * N + i < n ? mine[i] : 0;
+  sort_lanes(v, t);
+  for (int threads = 64; threads <= B; threads <<= 1) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) mine[i] = v[i];
+    for (int stride = threads * N / 2; stride >= 32 * N; stride >>= 1) {
+      __syncthreads();
+      for (int i = t; i < B * N / 2; i += B) {
+        const int lo = 2 * i - (i & (stride - 1));
+        order(s.cand[lo], s.cand[lo + stride], (lo & threads * N) == 0);
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = mine[i];
+    merge_lanes(v, t, 32, (t & threads) == 0);
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) mine[i] = v[i];
   __syncthreads();
+}
+// The CTA's n candidates, in order.
+template <int B>
+__device__ __noinline__ void sort_desc(Shared<B>& s, int n) {
+  static_assert(kCap <= 8 * B, "keys a thread");
+  if (n <= B) {
+    block_sort<1>(s, n);
+  } else if (n <= 2 * B) {
+    block_sort<2>(s, n);
+  } else if (kCap <= 4 * B || n <= 4 * B) {
+    block_sort<4>(s, n);
+  } else {
+    block_sort<kCap / B>(s, n);
+  }
 }
 
 // The k largest keys of elements [lo, hi) in four passes (five in f16, six in
@@ -358,7 +417,7 @@ __device__ __forceinline__ int collect(Shared<B>& s, const T* xr, int lo, int hi
     least = s.least;
   } else {
     __syncthreads();
-    least = bisect<uint32_t>(s, k, k + k / 8, parity, [&](auto see) {
+    least = bisect(s, k, k + k / 8, parity, [&](auto see) {
 #pragma unroll
       for (int i = 0; i < kPacks; ++i) see(group[i]);
     });
@@ -436,7 +495,6 @@ topk_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int cols, int k, 
     const RowSplit sp = split_row(at, hi - lo);
     return Packs{reinterpret_cast<const uint4*>(at + sp.head), sp.nvec};
   };
-  const int most = max(k + k / 4, kRank);  // keys to order at the end
   const int64_t step = cluster_count();
   issue(s, packs_of(cluster_id()), 0, 0);
   issue(s, packs_of(cluster_id()), 0, 1);
@@ -447,14 +505,6 @@ topk_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int cols, int k, 
       select_any(s, xr, lo, hi, want);
       n = want;
     }
-    // to a few more than k at most, without their order
-    const auto shrink = [&](int most) {
-      const uint64_t f = bisect<uint64_t>(s, min(k, n), most, parity, [&](auto see) {
-        for (int j = tid; j < n; j += B) see(s.cand[j]);
-      });
-      keep_above(s, n, f);
-      n = s.filled;
-    };
     // few keys: each one's place is the number of keys above it
     const auto place_all = [&](auto put) {
       int shift = 5;  // 2^shift threads a key
@@ -473,7 +523,6 @@ topk_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int cols, int k, 
       for (int o = step >> 1; o > 0; o >>= 1) place += __shfl_xor_sync(0xffffffffu, place, o);
       if (i < n && (tid & (step - 1)) == 0 && place < k) put(place, key);
     };
-    if (n > most) shrink(most);
     if (C > 1) {
       // this slice's k largest, 0 past the last
       if (n <= kRank) {
@@ -481,7 +530,7 @@ topk_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int cols, int k, 
         __syncthreads();
         place_all([&](int place, uint64_t key) { s.top[place] = key; });
       } else {
-        if (n > k) shrink(k);
+        sort_desc(s, n);
         for (int i = tid; i < k; i += B) s.top[i] = i < n ? s.cand[i] : 0;
       }
       cluster_sync_all();
@@ -492,7 +541,6 @@ topk_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int cols, int k, 
         __syncthreads();
       }
       cluster_sync_all();  // the others' lists are read
-      if (rank == 0 && n > most) shrink(most);
     }
     if (rank == 0) {
       const auto put = [&](int place, uint64_t key) {
@@ -506,10 +554,7 @@ topk_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int cols, int k, 
       if (n <= kRank) {
         place_all(put);
       } else {
-        int size = 1;
-        while (size < n) size <<= 1;
-        for (int i = n + tid; i < size; i += B) s.cand[i] = 0;
-        sort_desc(s, size);
+        sort_desc(s, n);
         for (int i = tid; i < k; i += B) put(i, s.cand[i]);
       }
     }
@@ -535,52 +580,6 @@ struct RowShared {
   uint8_t list[kRowWarps][256];  // slots that hold candidates
   int filled[kRowWarps];
 };
-
-// Descending bitonic sort of n <= 32 N keys by a warp, N neighbours a lane:
-// shuffles only where partners are in two lanes.
-template <int N>
-__device__ __forceinline__ void warp_sort(uint64_t* keys, int n, int lane) {
-  uint64_t v[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = lane * N + i < n ? keys[lane * N + i] : 0;
-  const auto swap = [](uint64_t& a, uint64_t& b, bool larger_first) {
-    const uint64_t hi = a > b ? a : b, lo = a > b ? b : a;
-    a = larger_first ? hi : lo;
-    b = larger_first ? lo : hi;
-  };
-#pragma unroll
-  for (int size = 2; size <= N; size <<= 1) {
-#pragma unroll
-    for (int stride = size >> 1; stride > 0; stride >>= 1) {
-#pragma unroll
-      for (int i = 0; i < N; ++i)
-        if ((i & stride) == 0) swap(v[i], v[i + stride], ((lane * N + i) & size) == 0);
-    }
-  }
-#pragma unroll 1
-  for (int lanes = 2; lanes <= 32; lanes <<= 1) {
-    const bool down = (lane & lanes) == 0;
-#pragma unroll 1
-    for (int other = lanes >> 1; other > 0; other >>= 1) {
-      const bool larger = ((lane & other) == 0) == down;
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const uint64_t o = __shfl_xor_sync(0xffffffffu, v[i], other);
-        v[i] = (o > v[i]) == larger ? o : v[i];
-      }
-    }
-#pragma unroll
-    for (int stride = N >> 1; stride > 0; stride >>= 1) {
-#pragma unroll
-      for (int i = 0; i < N; ++i)
-        if ((i & stride) == 0) swap(v[i], v[i + stride], down);
-    }
-  }
-  __syncwarp();
-#pragma unroll
-  for (int i = 0; i < N; ++i) keys[lane * N + i] = v[i];
-  __syncwarp();
-}
 
 template <typename T>
 __global__ void __launch_bounds__(kRowWarps * 32, 32 / kRowWarps)
