@@ -13,7 +13,7 @@ constexpr int kMaxTop = FL_B200_TOPK_MAX;
 constexpr int kPacks = 8;     // 16-byte packs a thread has in flight
 constexpr int kCap = 2048;    // candidates kept
 constexpr int kShared = 512;  // the longest list that clusters exchange
-constexpr int kRank = 256;    // up to as many keys are placed by counting the larger ones
+constexpr int kRank = 128;    // up to as many keys are placed by counting the larger ones, more are sorted
 
 // Monotone 32-bit image of a value: unsigned order is float order, NaN on
 // top; never 0.
@@ -146,7 +146,11 @@ __device__ __forceinline__ void append(Shared<B>& s, uint64_t key) {
 }
 
 // Descending bitonic sort, N neighbours a thread, t its place.  Partners in
-// two lanes meet by shuffles, those in two warps through shared memory.
+// two lanes meet by shuffles, those in two warps through shared memory (six
+// barriers for eight warps; with one a step, after a search for the cut, 64 x
+// 32000 float32, top 1000, took 44 us, now 30).  Above 128 keys it beats
+// counting (1 x 5289 float32, top 120: 9.0 us, 11.8), below it does not (4096 x
+// 128256 bf16, top 64: 214 us, counted 178).
 __device__ __forceinline__ void order(uint64_t& a, uint64_t& b, bool larger_first) {
   const uint64_t hi = a > b ? a : b, lo = a > b ? b : a;
   a = larger_first ? hi : lo;
@@ -473,7 +477,7 @@ __device__ __forceinline__ int collect(Shared<B>& s, const T* xr, int lo, int hi
 // them all and orders the k largest of the row.  Bound by HBM for many rows:
 // 4096 x 128256 bf16, top 64, in 178 us (5.9 TB/s, 91% of the measured copy
 // rate).  Few rows are bound by the steps after the stream (threshold, second
-// look, order: 3 to 5 us): 333 x 40003 fp32, top 50, 18.4 us; 4 x 32000 bf16,
+// look, order: 3 to 5 us): 333 x 40003 fp32, top 50, 17.5 us; 4 x 32000 bf16,
 // top 8, 6.0 us.
 template <typename T, int B>
 __global__ void __launch_bounds__(B, 1024 / B)
@@ -567,9 +571,11 @@ constexpr int kBlock = 512;
 
 // The same with a warp a row, for many short rows: the CTA's barriers, one
 // after the other, took most of a short row's time (20000 x 1024 bf16, top 8,
-// 411 us against 45; 3916 x 5266, top 7, 90 against 21).  The warp's 256 slots
-// are the groups; threshold, second look and order run on shuffles and a list
-// in shared memory.
+// 411 us against 46; 8192 x 4096, top 64, 192 against 54).  The warp's 256
+// slots are the groups; threshold, second look and order run on shuffles and a
+// list in shared memory.  Bound by the instructions of these steps: two fifths
+// of the copy rate at 1500 x 12000 bf16, top 20 (16.6 us), a fifth at 8192 x
+// 4096, top 64.
 constexpr int kRowWarps = 4;
 constexpr int kRowCap = 512;     // candidates listed
 constexpr int kRowSorted = 256;  // candidates put in order
