@@ -573,7 +573,7 @@ constexpr int kBlock = 512;
 // after the other, took most of a short row's time (20000 x 1024 bf16, top 8,
 // 411 us against 46; 8192 x 4096, top 64, 192 against 54).  The warp's 256
 // slots are the groups; threshold, second look and order run on shuffles and a
-// list in shared memory.  Bound by the instructions of these steps: two fifths
+// list in shared memory.  Bound by the instructions of these steps: a third
 // of the copy rate at 1500 x 12000 bf16, top 20 (16.6 us), a fifth at 8192 x
 // 4096, top 64.
 constexpr int kRowWarps = 4;
