@@ -411,9 +411,14 @@ struct ListOf {
   float total;
 
   __device__ __forceinline__ void load(Shared& s, const Taught& a, const float*, int64_t, const T* x,
-                                       int64_t row, int cols, int lo, int hi) {
+                                       int64_t row, int cols, int lo, int hi, bool masses) {
     ListAhead<E> in;
     in.load(a, nullptr, 0, row);
+    if (!masses) {
+      held.set(a, in, x, cols, lo, hi);
+      total = held.total;
+      return;
+    }
     for (int i = threadIdx.x & 31; i < kMarkBits / 32; i += 32) s.marks[i] = 0;
     __syncwarp();
     held.set(a, in, x, cols, lo, hi);
@@ -472,7 +477,7 @@ struct ListOf<T, 0> {
   float total;
 
   __device__ __forceinline__ void load(Shared& s, const Taught& a, const float*, int64_t, const T* x,
-                                       int64_t row, int cols, int, int) {
+                                       int64_t row, int cols, int, int, bool) {
     load_list(s, a, x, row, cols, true);
     total = s.total;
   }
@@ -554,7 +559,7 @@ distill_fwd_kernel(const T* __restrict__ x, int64_t ld, Taught a, int cols,
   const T* xr = x + row * ld;
   const int tid = threadIdx.x;
   if (tid >= NS) {
-    if (rank == 0) list.load(shared, a, nullptr, 0, xr, row, cols, 0, cols);
+    if (rank == 0) list.load(shared, a, nullptr, 0, xr, row, cols, 0, cols, false);
   } else {
     const RowSplit sp = split_row(xr, cols);
     const uint4* body = reinterpret_cast<const uint4*>(xr + sp.head);
@@ -640,7 +645,7 @@ distill_bwd_kernel(const float* __restrict__ dloss, int64_t dloss_stride, const 
   const bool want_dt = dt != nullptr && part == 0;
   if (tid >= NS) {
     if (live)
-      list.load(shared, a, nullptr, 0, xr, row, cols, part == 0 ? 0 : lo, part == 0 ? cols : hi);
+      list.load(shared, a, nullptr, 0, xr, row, cols, part == 0 ? 0 : lo, part == 0 ? cols : hi, true);
     if (want_dt) {
       if (live) {
         list.teacher(shared, a, st.x, st.y, gt, dt, row);
@@ -693,6 +698,120 @@ distill_bwd_kernel(const float* __restrict__ dloss, int64_t dloss_stride, const 
       dr[id] = Elem<T>::from_f(gt * (ex2((z - st.x) * a.c) * reciprocal(st.y) - mass));
   };
   list.tokens(shared, a, xr, NS, put);
+}
+
+// Many short rows, a warp each: loss and statistics (LOSS), gradients (GRAD)
+// from given statistics, or both, the row's second read from L2.  In the
+// kernels above a row's chain (the list, its logits, the sums' meeting) holds a
+// whole CTA; here it holds a warp, of which 32 an SM are under way.
+constexpr int kRowWarps = 4;
+
+template <typename T, bool LOSS, bool GRAD>
+__global__ void __launch_bounds__(kRowWarps * 32, GRAD ? 6 : 8)
+distill_rows_kernel(const T* __restrict__ x, int64_t ld, Taught a, const float* __restrict__ weight,
+                    int64_t weight_stride, int64_t rows, int cols, float* __restrict__ loss,
+                    float2* __restrict__ stats, T* __restrict__ dx, int64_t ld_dx, void* __restrict__ dt) {
+  constexpr int VW = Elem<T>::kVec, U = kUnroll;
+  __shared__ typename ListOf<T, 2>::Shared shared[GRAD ? kRowWarps : 1];
+  ListOf<T, 2> list;
+  pdl_prologue();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t row = (int64_t)blockIdx.x * kRowWarps + warp;
+  if (row >= rows) return;
+  const T* xr = x + row * ld;
+  const RowSplit sp = split_row(xr, cols);
+  const uint4* body = reinterpret_cast<const uint4*>(xr + sp.head);
+  const int e = single_of(sp, lane, VW);
+  ListAhead<2> in;
+  in.load(a, weight, weight_stride, row);
+  float2 st = LOSS ? make_float2(0.f, 0.f) : stats[row];
+  const float alone = e >= 0 ? Elem<T>::to_f(xr[e]) : kLowest;
+  uint4 u[U];
+  constexpr uint32_t none = lowest_word<T>();
+  const auto load = [&](uint4 (&u)[U], int p) {
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      u[i] = p + 32 * i < sp.nvec ? (GRAD ? ld_cached(body + p + 32 * i) : ld_stream(body + p + 32 * i))
+                                  : make_uint4(none, none, none, none);
+  };
+  load(u, lane);
+  uint32_t* marks = shared[GRAD ? warp : 0].marks;
+  if constexpr (GRAD) {
+    for (int i = lane; i < kMarkBits / 32; i += 32) marks[i] = 0;
+    __syncwarp();
+  }
+  list.held.set(a, in, xr, cols, 0, cols);
+  list.total = list.held.total;
+  bool live = st.y != 0.f;
+  if constexpr (LOSS) {
+    MaxSum v = {kLowest, 0.f};
+    if (e >= 0) fold(v, alone, a.c);
+    for (int p = 32 * U; p < sp.nvec; p += 32 * U) {
+      uint4 next[U];
+      load(next, p + lane);
+      fold_packs<T, U>(v, u, a.c);
+#pragma unroll
+      for (int i = 0; i < U; ++i) u[i] = next[i];
+    }
+    fold_packs<T, U>(v, u, a.c);
+    v = warp_merge(v, a.c);
+    live = list.total != 0.f;
+    const float sum = final_sum(v.s);
+    const float kl = live ? list.kl(shared[0], a, v.m, sum) : 0.f;
+    st = live ? make_float2(v.m, sum) : make_float2(0.f, 0.f);
+    if (lane == 0) {
+      loss[row] = a.tau * a.tau * kl;
+      stats[row] = st;
+    }
+    if (GRAD) load(u, lane);
+  }
+  if constexpr (GRAD) {
+    T* dr = dx + row * ld_dx;
+    uint4* out = reinterpret_cast<uint4*>(dr + sp.head);
+    const float gt = list.held.by, f = gt / st.y;
+    if (dt != nullptr) {
+      if (live) {
+        list.teacher(shared[0], a, st.x, st.y, gt, dt, row);
+      } else {
+        for (int j = lane; j < a.k; j += 32) store_float(dt, a.t_dtype, row * a.k + j, 0.f);
+      }
+    }
+    if (!live) {
+      if (e >= 0) dr[e] = Elem<T>::from_f(0.f);
+      for (int p = lane; p < sp.nvec; p += 32) st_stream(out + p, make_uint4(0, 0, 0, 0));
+      return;
+    }
+    list.held.set_masses(a, marks);
+    if (e >= 0) dr[e] = Elem<T>::from_f(ex2((alone - st.x) * a.c) * f);
+    const uint64_t minus = f2_make(-st.x, -st.x), c2 = f2_make(a.c, a.c), f2 = f2_make(f, f);
+    const auto write = [&](int p) {
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        if (p + 32 * i >= sp.nvec) break;
+        uint64_t g[VW / 2];
+        to_pairs<T>(u[i], g);
+#pragma unroll
+        for (int j = 0; j < VW / 2; ++j) {
+          const uint64_t d = f2_mul(f2_add(g[j], minus), c2);
+          g[j] = f2_make(ex2(f2_lo(d)), ex2(f2_hi(d)));
+        }
+        st_stream(out + p + 32 * i, from_pairs<T>(g, f2));
+      }
+    };
+    int p = lane;
+    for (; p - lane + 32 * U < sp.nvec; p += 32 * U) {
+      uint4 next[U];
+      load(next, p + 32 * U);
+      write(p);
+#pragma unroll
+      for (int i = 0; i < U; ++i) u[i] = next[i];
+    }
+    write(p);
+    __syncwarp();  // the row is stored
+    list.tokens(shared[0], a, xr, 0, [&](int id, float z, float mass) {
+      dr[id] = Elem<T>::from_f(gt * (ex2((z - st.x) * a.c) * reciprocal(st.y) - mass));
+    });
+  }
 }
 
 // ---------------------------------------------- loss and gradient at once ---
@@ -1001,12 +1120,38 @@ int with_geometry(int64_t cols, int64_t k, F&& go) {
   return k <= 64 && k > 0 ? go(Large{}, Held{}) : go(Large{}, Any{});
 }
 
+// Whether a warp a row is the form to take, by the bytes of a row.  The loss
+// alone gains up to 16 KB (16000 rows of 1024 bf16, 32 entries: 11.2 us, 40.0
+// with a CTA a row; of 8000: 43, 71; 700 of 8000: 5.5, 6.7), the two at once up
+// to 4 KB, where the row is still in L1 when it is read again (16000 x 1024: 19
+// us, 45; 16000 x 4096: 53, 52).  The gradient alone has one read to hide its list
+// behind: up to 2 KB, or to 8 KB where rows are many (16000 x 4096: 45 us, 55;
+// 700 x 4096: 6.2, 4.0).
+enum class Rows { kLoss, kGrad, kBoth };
+bool short_rows(Rows what, const DeviceInfo& dev, int64_t rows, int64_t bytes, int64_t k) {
+  int64_t most = rows > 16 * dev.sm_count ? 8192 : 2048;
+  if (what == Rows::kLoss) most = 16384;
+  if (what == Rows::kBoth) most = 4096;
+  return k > 0 && k <= 64 && rows > 4 * dev.sm_count && bytes <= most;
+}
+template <typename T, bool LOSS, bool GRAD>
+int run_rows(const void* x, int64_t ld, const Taught& a, const float* weight, int64_t weight_stride,
+             int64_t rows, int64_t cols, float* loss, float* stats, void* dx, int64_t ld_dx, void* dt,
+             cudaStream_t stream) {
+  launch_k(distill_rows_kernel<T, LOSS, GRAD>, dim3((unsigned)ceil_div(rows, kRowWarps)), dim3(kRowWarps * 32),
+           0, stream, reinterpret_cast<const T*>(x), ld, a, weight, weight_stride, rows, (int)cols, loss,
+           reinterpret_cast<float2*>(stats), reinterpret_cast<T*>(dx), ld_dx, dt);
+  return launch_status();
+}
+
 template <typename T>
 int run_fwd(const void* x, int64_t ld, const Taught& a, int64_t rows, int64_t cols, float* loss,
             float* stats, cudaStream_t stream) {
   DeviceInfo dev;
   const int st = current_device_info(&dev);
   if (st != FL_B200_OK) return st;
+  if (short_rows(Rows::kLoss, dev, rows, cols * sizeof(T), a.k))
+    return run_rows<T, true, false>(x, ld, a, nullptr, 0, rows, cols, loss, stats, nullptr, 0, nullptr, stream);
   return with_geometry<T>(cols, a.k, [&](auto ns, auto e) {
     constexpr int NS = decltype(ns)::value;
     int cluster = 1;
@@ -1026,6 +1171,9 @@ int run_bwd(const float* dloss, int64_t dloss_stride, const void* x, int64_t ld,
   const int st = current_device_info(&dev);
   if (st != FL_B200_OK) return st;
   const bool vec = dx == nullptr || same_phase(x, ld, dx, ld_dx, sizeof(T));
+  if (dx != nullptr && vec && short_rows(Rows::kGrad, dev, rows, cols * sizeof(T), a.k))
+    return run_rows<T, false, true>(x, ld, a, dloss, dloss_stride, rows, cols, nullptr, const_cast<float*>(stats),
+                                    dx, ld_dx, dt, stream);
   return with_geometry<T>(cols, a.k, [&](auto ns, auto e) {
     constexpr int NS = decltype(ns)::value, E = decltype(e)::value;
     // chunks of 4 rounds of loads, which hide the list's latency (2048 x 128256
@@ -1163,8 +1311,14 @@ FL_B200_API int fl_b200_distill_topk_grad(const void* logits, int64_t ld, const 
   if (reinterpret_cast<uintptr_t>(stats) % 8) return FL_B200_ERR_MISALIGNED;
   if (same_phase(logits, ld, dlogits, ld_dlogits, dtype_size(dtype))) {
     const Taught a = taught(teacher, ld_t, t_dtype, ids, ld_ids, ids_dtype, k, temperature);
+    DeviceInfo dev;
+    st = current_device_info(&dev);
+    if (st != FL_B200_OK) return st;
     st = dispatch_float(dtype, [&](auto t) {
       using T = decltype(t);
+      if (short_rows(Rows::kBoth, dev, rows, cols * sizeof(T), k))
+        return run_rows<T, true, true>(logits, ld, a, row_weight, weight_stride, rows, cols, loss, stats,
+                                       dlogits, ld_dlogits, nullptr, (cudaStream_t)stream);
       const auto go = [&](auto threads) {
         constexpr int NT = decltype(threads)::value;
         const auto each = [&](auto entries) {

@@ -311,6 +311,54 @@ def test_distill_special_rows(dtype, V):
     assert K.distill_topk(z, t, ids, 1.0)[0][1] == float("inf")
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("R,V,k", [(593, 1000, 20), (2400, 2001, 64), (2500, 4090, 33), (600, 8000, 7),
+                                   (1200, 511, 60), (5000, 37, 3), (2401, 1023, 1), (2402, 1024, 32)])
+def test_distill_many_short_rows(dtype, R, V, k):
+    """Enough rows that each is a warp's; as elsewhere the rows between hold the edges."""
+    z, t, ids, w = make(R, V, k, dtype, R + V)
+    low = torch.finfo(dtype).min
+    z[10, 9:] = -float("inf")
+    ids[10] = torch.arange(k, device=DEV) % 7
+    z[11, V // 2:] = low
+    ids[11] = 3                             # one token throughout
+    z[12] = low
+    t[13] = -float("inf")
+    z[13, 5] = float("nan")
+    ids[14] = -1
+    z[14] = float("nan")
+    t[15, 1:] = -float("inf")
+    t[16] = low
+    z[17] = 0
+    w[18] = 0
+    check_distill(z, t, ids, w, 2.0)
+    loss, stats = K.distill_topk(z, t, ids, 2.0)
+    dz, dt = K.distill_topk_backward(w, z, stats, t, ids, 2.0, need_teacher=True)
+    alone, none = K.distill_topk_backward(w, z, stats, t, ids, 2.0)
+    assert none is None and torch.equal(alone, dz)
+    for r in (13, 14):
+        assert loss[r] == 0 and not dz[r].any() and not dt[r].any()
+    # rows of a wider matrix, beside which nothing is written
+    big = torch.zeros(R, V + 9, dtype=dtype, device=DEV)
+    big[:, 3:V + 3] = z
+    out = torch.full_like(big, 7.0)
+    l2, _ = K.distill_topk_grad(big[:, 3:V + 3], t, ids, 2.0, w, out=out[:, 3:V + 3])
+    l1, d1 = K.distill_topk_grad(z, t, ids, 2.0, w)
+    tol = bounds(z, t, ids, 2.0, w)
+    ref = ops.distill_topk_golden(np64(z), np64(t), np64(ids).astype(np.int64), 2.0, np64(w))
+    within(l2, ref[0], tol[0] + half_step(torch.float32, ref[0]), "loss, in a wider matrix")
+    within(out[:, 3:V + 3], ref[1], tol[1] + half_step(dtype, ref[1]), "gradient, in a wider matrix")
+    assert (out[:, :3] == 7).all() and (out[:, V + 3:] == 7).all()
+    # a row without a softmax is NaN, its neighbours are as they were
+    z[20, 1] = float("nan")
+    z[21] = -float("inf")
+    ids[20:22, 0] = 1
+    l3, d3 = K.distill_topk_grad(z, t, ids, 2.0, w)
+    assert torch.isnan(l3[20:22]).all() and torch.isnan(d3[20:22]).all()
+    rest = torch.tensor([r for r in range(R) if r not in (20, 21)], device=DEV)
+    assert torch.equal(l3[rest], l1[rest]) and torch.equal(d3[rest], d1[rest])
+
+
 @pytest.mark.parametrize("k", [2, 33, 64, 65, 128, 129, 300, 1024])
 def test_distill_repeated_tokens(k):
     """Lists drawn from few tokens, one of a single token, one whose ids share
