@@ -108,16 +108,18 @@ struct Row {
       if (lane == 0 && x >= from * VW && x < to * VW) s -= fixed(Elem<T>::to_f(p[without]));
     } else if (packed) {
       const uint4* qv = reinterpret_cast<const uint4*>(q + sp.head);
-      for (int i = from + lane; i < to; i += 32 * U) {
-        uint4 a[U], b[U];
-#pragma unroll
-        for (int k = 0; k < U; ++k) {
-          const bool in = i + 32 * k < to;
-          a[k] = in ? ld_cached(pv + i + 32 * k) : make_uint4(0, 0, 0, 0);
-          b[k] = in ? ld_cached(qv + i + 32 * k) : make_uint4(0, 0, 0, 0);
-        }
-#pragma unroll
-        for (int k = 0; k < U; ++k) add2(a[k], b[k]);
+      // one pack of each ahead: four at once, then summed, were no faster
+      const auto get = [&](const uint4* v, int i) {
+        return i < to ? ld_cached(v + i) : make_uint4(0, 0, 0, 0);
+      };
+      int i = from + lane;
+      uint4 a = get(pv, i), b = get(qv, i);
+      for (; i - lane < to; i += 64) {
+        const uint4 c = get(pv, i + 32), d = get(qv, i + 32);
+        add2(a, b);
+        a = get(pv, i + 64);
+        b = get(qv, i + 64);
+        add2(c, d);
       }
     } else {
       const int end = sp.head + to * VW;
