@@ -1123,15 +1123,15 @@ int with_geometry(int64_t cols, int64_t k, F&& go) {
 // Whether a warp a row is the form to take, by the bytes of a row.  The loss
 // alone gains up to 16 KB (16000 rows of 1024 bf16, 32 entries: 11.2 us, 40.0
 // with a CTA a row; of 8000: 43, 71; 700 of 8000: 5.5, 6.7), the two at once up
-// to 4 KB, where the row is still in L1 when it is read again (16000 x 1024: 19
-// us, 45; 16000 x 4096: 53, 52).  The gradient alone has one read to hide its list
+// to 6 KB, where the row is still in L1 when it is read again (16000 x 1024: 19
+// us, 45; 16000 x 2048: 32, 46; 16000 x 4096: 53, 52).  The gradient alone has one read to hide its list
 // behind: up to 2 KB, or to 8 KB where rows are many (16000 x 4096: 45 us, 55;
 // 700 x 4096: 6.2, 4.0).
 enum class Rows { kLoss, kGrad, kBoth };
 bool short_rows(Rows what, const DeviceInfo& dev, int64_t rows, int64_t bytes, int64_t k) {
   int64_t most = rows > 16 * dev.sm_count ? 8192 : 2048;
   if (what == Rows::kLoss) most = 16384;
-  if (what == Rows::kBoth) most = 4096;
+  if (what == Rows::kBoth) most = 6144;
   return k > 0 && k <= 64 && rows > 4 * dev.sm_count && bytes <= most;
 }
 template <typename T, bool LOSS, bool GRAD>

@@ -313,7 +313,8 @@ def test_distill_special_rows(dtype, V):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("R,V,k", [(593, 1000, 20), (2400, 2001, 64), (2500, 4090, 33), (600, 8000, 7),
-                                   (1200, 511, 60), (5000, 37, 3), (2401, 1023, 1), (2402, 1024, 32)])
+                                   (1200, 511, 60), (5000, 37, 3), (2401, 1023, 1), (2402, 1024, 32),
+                                   (1300, 2600, 40)])
 def test_distill_many_short_rows(dtype, R, V, k):
     """Enough rows that each is a warp's; as elsewhere the rows between hold the edges."""
     z, t, ids, w = make(R, V, k, dtype, R + V)
