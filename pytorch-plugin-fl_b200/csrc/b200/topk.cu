@@ -660,6 +660,7 @@ topk_rows_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int cols, in
     }
     __syncwarp();
     if (single >= 0) keep(element_key(alone, (uint32_t)single));
+    const float bar = key_value(least);  // (NaN while everything passes, or only NaN does)
     const uint32_t depth = (sp.nvec + kChunk - 1) / kChunk, items = listed * depth;
     for (uint32_t base = lane; base < items; base += 64) {
       uint4 u[2];
@@ -677,7 +678,7 @@ topk_rows_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int cols, in
         unpack<T>(u[i], f);
         uint32_t reach = 0;
 #pragma unroll
-        for (int j = 0; j < VW; ++j) reach |= (uint32_t)(value_key(f[j]) >= least) << j;
+        for (int j = 0; j < VW; ++j) reach |= (uint32_t)!(f[j] < bar) << j;
         if (reach == 0) continue;
         const int first = take_slots(filled, __popc(reach));
 #pragma unroll
