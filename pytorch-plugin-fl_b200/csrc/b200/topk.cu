@@ -151,20 +151,21 @@ __device__ __forceinline__ void append(Shared<B>& s, uint64_t key) {
 // 32000 float32, top 1000, took 44 us, now 30).  Above 128 keys it beats
 // counting (1 x 5289 float32, top 120: 9.0 us, 11.8), below it does not (4096 x
 // 128256 bf16, top 64: 214 us, counted 178).
-__device__ __forceinline__ void order(uint64_t& a, uint64_t& b, bool larger_first) {
-  const uint64_t hi = a > b ? a : b, lo = a > b ? b : a;
+template <typename K>
+__device__ __forceinline__ void order(K& a, K& b, bool larger_first) {
+  const K hi = a > b ? a : b, lo = a > b ? b : a;
   a = larger_first ? hi : lo;
   b = larger_first ? lo : hi;
 }
 // The steps of one merge of `lanes` lanes' keys.
-template <int N>
-__device__ __forceinline__ void merge_lanes(uint64_t (&v)[N], int lane, int lanes, bool down) {
+template <int N, typename K>
+__device__ __forceinline__ void merge_lanes(K (&v)[N], int lane, int lanes, bool down) {
 #pragma unroll 1
   for (int other = lanes >> 1; other > 0; other >>= 1) {
     const bool larger = ((lane & other) == 0) == down;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const uint64_t o = __shfl_xor_sync(0xffffffffu, v[i], other);
+      const K o = __shfl_xor_sync(0xffffffffu, v[i], other);
       v[i] = (o > v[i]) == larger ? o : v[i];
     }
   }
@@ -176,8 +177,8 @@ __device__ __forceinline__ void merge_lanes(uint64_t (&v)[N], int lane, int lane
   }
 }
 // A warp's 32 N keys, the largest first where bit 5 of t is 0, else last.
-template <int N>
-__device__ __forceinline__ void sort_lanes(uint64_t (&v)[N], int t) {
+template <int N, typename K>
+__device__ __forceinline__ void sort_lanes(K (&v)[N], int t) {
 #pragma unroll
   for (int size = 2; size <= N; size <<= 1) {
 #pragma unroll
@@ -571,7 +572,7 @@ constexpr int kBlock = 512;
 
 // The same with a warp a row, for many short rows: the CTA's barriers, one
 // after the other, took most of a short row's time (20000 x 1024 bf16, top 8,
-// 411 us against 46; 8192 x 4096, top 64, 192 against 54).  The warp's 256
+// 411 us against 37; 8192 x 4096, top 64, 192 against 54).  The warp's 256
 // slots are the groups; threshold, second look and order run on shuffles and a
 // list in shared memory.  Bound by the instructions of these steps: a third
 // of the copy rate at 1500 x 12000 bf16, top 20 (16.6 us), a fifth at 8192 x
@@ -587,14 +588,52 @@ struct RowShared {
   int filled[kRowWarps];
 };
 
+// The k-th largest of the lanes' maxima, k <= 32.
+template <int S>
+__device__ __forceinline__ uint32_t kth_lane(const uint32_t (&v)[S], int k, int lane) {
+  uint32_t m[1] = {v[0]};
+#pragma unroll
+  for (int i = 1; i < S; ++i) m[0] = max(m[0], v[i]);
+  sort_lanes(m, lane);
+  return __shfl_sync(0xffffffffu, m[0], k - 1);
+}
+
+// The k-th largest of the slots' (or one that a few more reach), as in kth_maximum.
+template <typename T, int S>
+__device__ __forceinline__ uint32_t search_slots(const uint32_t (&v)[S], int k) {
+  // the lowest bits that tell two values' keys apart
+  constexpr int kLast = std::is_same<T, float>::value ? 0 : std::is_same<T, __half>::value ? 12 : 16;
+  uint32_t lo = 0xffffffffu, hi = 0;
+#pragma unroll
+  for (int i = 0; i < S; ++i) {
+    lo = min(lo, v[i] - 1);  // (slots without a pack aside)
+    hi = max(hi, v[i]);
+  }
+  lo = __reduce_min_sync(0xffffffffu, lo) + 1;
+  hi = __reduce_max_sync(0xffffffffu, hi);
+  const int top = (32 - __clz(lo ^ hi) + 1) & ~1;
+  uint32_t least = top < 32 ? lo >> top << top : 0;
+  for (int bit = top - 2; bit >= kLast; bit -= 2) {
+    const uint32_t one = 1u << bit;
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < S; ++i)
+      n += (v[i] >= least + one) + ((v[i] >= least + 2 * one) << 10) + ((v[i] >= least + 3 * one) << 20);
+    n = __reduce_add_sync(0xffffffffu, n);
+    const int n3 = n >> 20, n2 = (n >> 10) & 1023, n1 = n & 1023;
+    const int reached = n3 >= k ? n3 : n2 >= k ? n2 : n1 >= k ? n1 : 0;
+    least += n3 >= k ? 3 * one : n2 >= k ? 2 * one : n1 >= k ? one : 0;
+    if (reached != 0 && reached <= k + k / 8) break;
+  }
+  return least;
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kRowWarps * 32, 32 / kRowWarps)
 topk_rows_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int cols, int k,
                  T* __restrict__ values, int64_t* __restrict__ indices) {
   constexpr int VW = Elem<T>::kVec;
   constexpr int S = 8, kChunk = 32 * S;
-  // the lowest bits that tell two values' keys apart
-  constexpr int kLast = std::is_same<T, float>::value ? 0 : std::is_same<T, __half>::value ? 12 : 16;
   __shared__ RowShared s;
   pdl_prologue();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -625,30 +664,13 @@ topk_rows_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int cols, in
       for (int i = 0; i < S; ++i)
         if (base + 32 * i < sp.nvec) v[i] = word_max<T>(v[i], pack_max<T>(u[i]));
     }
-    uint32_t lo = 0xffffffffu, hi = 0;
 #pragma unroll
-    for (int i = 0; i < S; ++i) {
-      v[i] = lane + 32 * i < sp.nvec ? value_key(word_top<T>(v[i])) : 0;
-      lo = min(lo, v[i] - 1);  // (slots without a pack aside)
-      hi = max(hi, v[i]);
-    }
-    // the k-th largest of the slots' maxima, as in kth_maximum
-    lo = __reduce_min_sync(0xffffffffu, lo) + 1;
-    hi = __reduce_max_sync(0xffffffffu, hi);
-    const int top = (32 - __clz(lo ^ hi) + 1) & ~1;
-    uint32_t least = top < 32 ? lo >> top << top : 0;
-    for (int bit = top - 2; bit >= kLast; bit -= 2) {
-      const uint32_t one = 1u << bit;
-      int n = 0;
-#pragma unroll
-      for (int i = 0; i < S; ++i)
-        n += (v[i] >= least + one) + ((v[i] >= least + 2 * one) << 10) + ((v[i] >= least + 3 * one) << 20);
-      n = __reduce_add_sync(0xffffffffu, n);
-      const int n3 = n >> 20, n2 = (n >> 10) & 1023, n1 = n & 1023;
-      const int reached = n3 >= k ? n3 : n2 >= k ? n2 : n1 >= k ? n1 : 0;
-      least += n3 >= k ? 3 * one : n2 >= k ? 2 * one : n1 >= k ? one : 0;
-      if (reached != 0 && reached <= k + k / 8) break;
-    }
+    for (int i = 0; i < S; ++i) v[i] = lane + 32 * i < sp.nvec ? value_key(word_top<T>(v[i])) : 0;
+    // up to k = 16 the lanes' maxima, which 1.4 k elements reach, in a sixth of
+    // the search's steps (20000 x 1024 bf16, top 8: 37 us, 45); past that the
+    // search, for its fewer candidates (1500 x 12000, top 20: 16.5 us, 17.7 with
+    // two maxima a lane)
+    const uint32_t least = k <= 16 ? kth_lane(v, k, lane) : search_slots<T>(v, k);
     // the slots that reach it, and their packs' elements
     uint32_t listed = 0;
 #pragma unroll
