@@ -78,6 +78,16 @@ FL_B200_API int fl_b200_last_cuda_error(void);
  * device (griddepcontrol.wait) before its first memory access, so results    *
  * are the same either way.  Process-wide; returns the previous setting.      */
 FL_B200_API int fl_b200_set_pdl(int enable);
+/* How long a kernel's wait for a copy or for another block may last, in      *
+ * nanoseconds (0 to 2e9, the default).  Only fl_b200_distill_topk_grad's     *
+ * clusters wait so, for microseconds.  A cluster that gives up a wait        *
+ * returns NaN for the loss, the stats and the gradient of every row it had,  *
+ * and is counted.  Process-wide, read at the launch; returns the previous    *
+ * setting.                                                                   */
+FL_B200_API int64_t fl_b200_set_wait_limit(int64_t nanoseconds);
+/* How many clusters have given up a wait on the current device since the    *
+ * library was loaded; waits for the device's work.                           */
+FL_B200_API int fl_b200_lost_waits(uint64_t* count);
 
 /* ------------------------------------------------------------------------ *
  * RMSNorm forward over the last dim:                                        *
@@ -456,8 +466,7 @@ FL_B200_API int fl_b200_distill_topk_bwd(const float* dloss, int64_t dloss_strid
  * are read once and dlogits written once when the rows' offsets agree as    *
  * above, a row has at most 262144 elements of 16 bits or 131072 of 32, and  *
  * k <= 128; otherwise the forward and the backward run one after the other. *
- * On the first way, a cluster whose parts fail to meet within seconds       *
- * gives NaN instead of waiting on.                                          */
+ * On the first way a cluster's waits have a limit (fl_b200_set_wait_limit). */
 FL_B200_API int fl_b200_distill_topk_grad(const void* logits, int64_t ld, const void* teacher,
                                           int64_t ld_t, int t_dtype, const void* ids,
                                           int64_t ld_ids, int ids_dtype, const float* row_weight,

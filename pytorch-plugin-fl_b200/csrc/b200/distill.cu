@@ -840,17 +840,63 @@ constexpr int kPacks = 8;            // 16-byte packs a thread holds
 constexpr int kStages = 3;
 constexpr int kMaxCluster = 16;
 
+// No wait lasts longer than a limit.  A thread that gives up tells every CTA of
+// the cluster; from then on its CTAs only step through their rows: nothing more
+// is expected of a barrier, sent or copied.  What had been under way is counted
+// at the end and waited for, so that nothing arrives in the shared memory of a
+// CTA that has left, and every row of the cluster is reported as NaN.
 template <int NT>
 struct GradShared {
   uint4 stage[kStages][kPacks][NT];
   float2 pair[2][kMaxCluster * (NT / 32)];
   uint32_t marks[2][kMarkBits / 32];
   float2 scale[2];  // the row's M, and w tau / S
-  int live[2];      // whether anything is taught
+  int state[2];     // kLive: something is taught; kDead: a wait has been given up
   uint64_t bar[2];          // the row's pairs have come
   uint64_t full[kStages];   // the stage's logits have come
-  int lost;
+  int lost;                 // a CTA of the cluster has given up a wait
+  int expected[2], loaded[kStages];  // phases begun, of bar and full
+  int sent[NT / 32];                 // rows whose pairs this warp has sent
 };
+constexpr int kLive = 1, kDead = 2;
+
+// Clusters that gave up a wait, on this device.
+__device__ unsigned long long lost_clusters;
+constexpr uint32_t kDrainLimit = 2000000000u;  // nanoseconds
+
+// Waits for what is still on its way to this CTA's shared memory, once no CTA
+// of the cluster sends or copies any more.  By one warp.  (All pairs that were
+// sent arrive: sent and expected bytes tell what each barrier is short of, or
+// has had beyond its last phase.)
+template <int NT>
+__device__ __noinline__ void drain(GradShared<NT>& s, int C) {
+  constexpr int W = NT / 32;
+  const int lane = threadIdx.x & 31;
+  const int zero = 0;
+  int pairs[2] = {0, 0};
+  if (lane < C) {
+    for (int w = 0; w < W; ++w) {
+      const int n = ld_remote_s32(remote_smem(&s.sent[w], lane));
+      pairs[0] += (n + 1) / 2;  // rows alternate between the barriers
+      pairs[1] += n / 2;
+    }
+  }
+  for (int par = 0; par < 2; ++par) {
+    const int n = __reduce_add_sync(0xffffffffu, pairs[par]);
+    if (lane != 0) continue;
+    const int begun = s.expected[par], over = n - begun * C * W;
+    if (over < 0) bar_give(&s.bar[par], -over * 8);
+    const bool settled = begun == 0 || bar_wait(&s.bar[par], (begun - 1) & 1, &zero, kDrainLimit);
+    if (over > 0 && settled) {
+      bar_expect(&s.bar[par], over * 8);
+      (void)bar_wait(&s.bar[par], begun & 1, &zero, kDrainLimit);
+    }
+  }
+  if (lane == 0) {
+    for (int i = 0; i < kStages; ++i)
+      if (s.loaded[i] > 0) (void)bar_wait(&s.full[i], (s.loaded[i] - 1) & 1, &zero, kDrainLimit);
+  }
+}
 
 constexpr int kHelpers = 64;  // threads besides the NT that hold the row
 // Named barriers, two of each for alternate rows: a barrier's next use follows,
@@ -858,12 +904,40 @@ constexpr int kHelpers = 64;  // threads besides the NT that hold the row
 constexpr int kScaled = 1;  // the row's scale is known: the holders wait for the list's warp
 constexpr int kHeld = 3;    // the gradient is in place: the list's warp waits for the holders
 
+// Reports every row of this cluster as NaN.
+template <typename T, int NT>
+__device__ __noinline__ void report_lost(const T* x, int64_t ld, int64_t rows, int cols, float* loss,
+                                         float2* stats, T* dx, int64_t ld_dx) {
+  constexpr int VW = Elem<T>::kVec;
+  const int tid = threadIdx.x;
+  const int C = (int)cluster_size(), rank = (int)cluster_rank();
+  const float none = NAN;
+  const uint32_t word = std::is_same<T, float>::value    ? __float_as_uint(none)
+                        : std::is_same<T, __half>::value ? 0x7e007e00u
+                                                         : 0x7fc07fc0u;
+  for (int64_t row = cluster_id(); row < rows; row += cluster_count()) {
+    const RowSplit sp = split_row(x + row * ld, cols);
+    T* dr = dx + row * ld_dx;
+    uint4* out = reinterpret_cast<uint4*>(dr + sp.head);
+    for (int p = rank * (NT + kHelpers) + tid; p < sp.nvec; p += C * (NT + kHelpers))
+      out[p] = make_uint4(word, word, word, word);
+    if (rank != 0) continue;
+    const int e = single_of(sp, tid, VW);
+    if (e >= 0) dr[e] = Elem<T>::from_f(none);
+    if (tid == 0) {
+      loss[row] = none;
+      stats[row] = make_float2(none, none);
+    }
+  }
+  if (rank == 0 && tid == 0) atomicAdd(&lost_clusters, 1ull);
+}
+
 // E entries of a list a lane.
 template <typename T, int NT, int E>
 __global__ void __launch_bounds__(NT + kHelpers, NT == 256 ? 2 : NT == 128 ? 3 : 5)
 distill_grad_kernel(const T* __restrict__ x, int64_t ld, Taught a, const float* __restrict__ weight,
                     int64_t weight_stride, int64_t rows, int cols, float* __restrict__ loss,
-                    float2* __restrict__ stats, T* __restrict__ dx, int64_t ld_dx) {
+                    float2* __restrict__ stats, T* __restrict__ dx, int64_t ld_dx, uint32_t limit) {
   constexpr int VW = Elem<T>::kVec;
   constexpr int P = kPacks;
   constexpr int W = NT / 32;
@@ -878,6 +952,8 @@ distill_grad_kernel(const T* __restrict__ x, int64_t ld, Taught a, const float* 
     bar_init(&s.bar[1], 1);
     for (int i = 0; i < kStages; ++i) bar_init(&s.full[i], 1);
     s.lost = 0;
+    s.expected[0] = s.expected[1] = 0;
+    for (int i = 0; i < kStages; ++i) s.loaded[i] = 0;
     bar_init_fence();
   }
   pdl_prologue();
@@ -890,9 +966,13 @@ distill_grad_kernel(const T* __restrict__ x, int64_t ld, Taught a, const float* 
     from = min(sp.nvec, rank * per);
     to = min(sp.nvec, from + per);
   };
+  const auto give_up = [&] {
+    for (int r = 0; r < (int)cluster_size(); ++r) st_remote_s32(remote_smem(&s.lost, r), 1);
+  };
   if (warp >= W) {
     // every other row's list, and its copies
     const int par = warp - W;
+    bool ok = true;  // no wait has been given up, as far as this warp knows
     ListAhead<E> next;
     ListHeld<T, E> list;
     const auto set = [&](int64_t row) {
@@ -900,18 +980,22 @@ distill_grad_kernel(const T* __restrict__ x, int64_t ld, Taught a, const float* 
       const RowSplit sp = split_row(xr, cols);
       int from, to;
       slice(sp, from, to);
-      if (lane == 0) bar_expect(&s.bar[par], C * W * 8);
+      if (lane == 0 && ok) {
+        bar_expect(&s.bar[par], C * W * 8);
+        ++s.expected[par];
+      }
       list.set(a, next, xr, cols, rank == 0 ? 0 : sp.head + from * VW,
                rank == 0 ? cols : sp.head + to * VW);
       if (row + 2 * step < rows) next.load(a, weight, weight_stride, row + 2 * step);
     };
     const auto load = [&](int64_t row, int stage) {
-      if (row >= rows || lane != 0) return;
+      if (row >= rows || lane != 0 || !ok) return;
       const T* xr = x + row * ld;
       const RowSplit sp = split_row(xr, cols);
       int from, to;
       slice(sp, from, to);
       bar_expect(&s.full[stage], (to - from) * 16);
+      ++s.loaded[stage];
       if (to > from)
         bulk_load(s.stage[stage], reinterpret_cast<const uint4*>(xr + sp.head) + from, (to - from) * 16,
                   &s.full[stage]);
@@ -924,7 +1008,11 @@ distill_grad_kernel(const T* __restrict__ x, int64_t ld, Taught a, const float* 
     int stage = par;
     uint32_t phase = 0;
     for (int64_t row = first + par * step; row < rows; row += 2 * step, phase ^= 1) {
-      bar_wait(&s.bar[par], phase, &s.lost);
+      if (ok && !bar_wait(&s.bar[par], phase, &s.lost, limit)) {
+        give_up();
+        ok = false;
+      }
+      const int lost = *(volatile int*)&s.lost;
       constexpr int kPairs = kMaxCluster * W / 32;  // a lane's, at most
       float2 q[kPairs];
       float M = kLowest, S = 0.f;
@@ -937,12 +1025,11 @@ distill_grad_kernel(const T* __restrict__ x, int64_t ld, Taught a, const float* 
 #pragma unroll
       for (int i = 0; i < kPairs; ++i) S += q[i].y * ex2((q[i].x - M) * a.c);
       S = final_sum(warp_sum(S));
-      if (s.lost) S = NAN;
       const float inverse = reciprocal(S);
       const bool live = list.total != 0.f;
       if (lane == 0) {
         s.scale[par] = make_float2(M, list.by * inverse);
-        s.live[par] = live;
+        s.state[par] = (live ? kLive : 0) | (ok && lost == 0 ? 0 : kDead);
       }
       __syncwarp();
       named_arrive(kScaled + par, NT + 32);
@@ -952,6 +1039,7 @@ distill_grad_kernel(const T* __restrict__ x, int64_t ld, Taught a, const float* 
       slice(sp, from, to);
       T* dr = dx + row * ld_dx;
       named_sync(kHeld + par, NT + 32);
+      ok = __all_sync(0xffffffffu, ok && *(volatile int*)&s.lost == 0);  // (so every holder had the row)
       if (live) {
         const int lo = sp.head + from * VW, hi = sp.head + to * VW;
         T* held = reinterpret_cast<T*>(s.stage[stage]);
@@ -970,7 +1058,7 @@ distill_grad_kernel(const T* __restrict__ x, int64_t ld, Taught a, const float* 
         __syncwarp();
       }
       if (lane == 0) {
-        if (to > from)
+        if (to > from && ok)
           bulk_store(reinterpret_cast<uint4*>(dr + sp.head) + from, s.stage[stage], (to - from) * 16);
         bulk_commit();
       }
@@ -1006,14 +1094,15 @@ distill_grad_kernel(const T* __restrict__ x, int64_t ld, Taught a, const float* 
     const auto single_at = [&](const T* xr) {
       return edge ? single_of(split_row(xr, cols), lane, VW) : -1;
     };
-    const T* xr = x + first * ld;
-    T* dr = dx + first * ld_dx;
-    int single = first < rows ? single_at(xr) : -1;
-    float xs = single >= 0 ? Elem<T>::to_f(xr[single]) : -INFINITY;
+    int single = single_at(x + first * ld);
+    float xs = single >= 0 ? Elem<T>::to_f((x + first * ld)[single]) : -INFINITY;
     int par = 0, stage = 0;
     uint32_t stage_phase = 0;
-    for (int64_t row = first; row < rows; row += step, xr += step * ld, dr += step * ld_dx) {
-      const RowSplit sp = split_row(xr, cols);
+    bool ok = true;
+    if (lane == 0) s.sent[warp] = 0;
+    // (32 bits hold a row and one step more)
+    for (uint32_t row = (uint32_t)first; row < (uint32_t)rows; row += (uint32_t)step) {
+      const RowSplit sp = split_row(x + row * ld, cols);
       int from, to;
       slice(sp, from, to);
       const int left = to - from - tid;  // the thread's packs end here
@@ -1022,7 +1111,7 @@ distill_grad_kernel(const T* __restrict__ x, int64_t ld, Taught a, const float* 
       // values, then exponentials, in pairs
       uint64_t e[P][VW / 2];
       float m = fmaxf(kLowest, xs);
-      bar_wait(&s.full[stage], stage_phase, &s.lost);
+      if (ok && !bar_wait(&s.full[stage], stage_phase, &s.lost, limit)) give_up();
 #pragma unroll
       for (int i = 0; i < P; ++i) {
         uint4 u = held[i * NT];
@@ -1046,22 +1135,28 @@ distill_grad_kernel(const T* __restrict__ x, int64_t ld, Taught a, const float* 
           sum2 = f2_add(sum2, e[i][j]);
         }
       const float sum = warp_sum(f2_lo(sum2) + f2_hi(sum2));
-      if (lane < C) send_f2(to_pair + par * (uint32_t)sizeof(s.pair[0]), m, sum, to_bar + par * 8);
+      if (ok) {
+        if (lane < C) send_f2(to_pair + par * (uint32_t)sizeof(s.pair[0]), m, sum, to_bar + par * 8);
+        if (lane == 0) ++s.sent[warp];
+      }
       // the next row's single element travels while this row is exchanged
       const float es = xs;
       const int at_single = single;
-      single = row + step < rows ? single_at(xr + step * ld) : -1;
-      xs = single >= 0 ? Elem<T>::to_f((xr + step * ld)[single]) : -INFINITY;
+      const T* following = x + (row + (uint32_t)step) * ld;
+      single = row + (uint32_t)step < (uint32_t)rows ? single_at(following) : -1;
+      xs = single >= 0 ? Elem<T>::to_f(following[single]) : -INFINITY;
       named_sync(kScaled + par, NT + 32);
-      if (s.live[par]) {
+      const int state = s.state[par];
+      ok = ok && (state & kDead) == 0;
+      if (state & kLive) {
         const float2 sc = s.scale[par];
         const float f = ex2((m - sc.x) * a.c) * sc.y;
         const uint64_t f2 = f2_make(f, f);
-        if (at_single >= 0) dr[at_single] = Elem<T>::from_f(es * f);
+        if (at_single >= 0) dx[row * ld_dx + at_single] = Elem<T>::from_f(es * f);
 #pragma unroll
         for (int i = 0; i < P; ++i) held[i * NT] = from_pairs<T>(e[i], f2);
       } else {
-        if (at_single >= 0) dr[at_single] = Elem<T>::from_f(0.f);
+        if (at_single >= 0) dx[row * ld_dx + at_single] = Elem<T>::from_f(0.f);
 #pragma unroll
         for (int i = 0; i < P; ++i) held[i * NT] = make_uint4(0, 0, 0, 0);
       }
@@ -1076,9 +1171,16 @@ distill_grad_kernel(const T* __restrict__ x, int64_t ld, Taught a, const float* 
   }
   __syncwarp();
   cluster_sync_all();  // no CTA leaves while pairs may still be sent to it
+  if (*(volatile int*)&s.lost == 0) return;  // (the same in every CTA of the cluster)
+  if (threadIdx.x < 32) drain(s, (int)cluster_size());
+  __syncwarp();
+  cluster_sync_all();  // the counts are read, and nothing of the cluster's is under way
+  report_lost<T, NT>(x, ld, rows, cols, loss, stats, dx, ld_dx);
 }
 
 // ------------------------------------------------------------------ host ---
+
+std::atomic<uint32_t> g_wait_limit{2000000000u};  // nanoseconds; fl_b200_set_wait_limit
 
 bool list_dtypes_ok(int t_dtype, int ids_dtype) {
   return is_float_dtype(t_dtype) && (ids_dtype == FL_B200_I32 || ids_dtype == FL_B200_I64);
@@ -1238,13 +1340,33 @@ int run_grad(const void* x, int64_t ld, const Taught& a, const float* weight, in
   return launch_cluster(kern, std::min<int64_t>(rows, clusters) * cluster, (int)cluster, NT + kHelpers, smem,
                         stream, reinterpret_cast<const T*>(x), ld, a, weight, weight_stride, rows,
                         (int)cols, loss, reinterpret_cast<float2*>(stats), reinterpret_cast<T*>(dx),
-                        ld_dx);
+                        ld_dx, g_wait_limit.load(std::memory_order_relaxed));
 }
 
 }  // namespace
 }  // namespace flb200
 
 extern "C" {
+
+FL_B200_API int64_t fl_b200_set_wait_limit(int64_t nanoseconds) {
+  const int64_t ns = std::min<int64_t>(std::max<int64_t>(nanoseconds, 0), 2000000000);
+  return flb200::g_wait_limit.exchange((uint32_t)ns, std::memory_order_relaxed);
+}
+
+FL_B200_API int fl_b200_lost_waits(uint64_t* count) {
+  using namespace flb200;
+  FLB_CHECK_ARG(count != nullptr);
+  unsigned long long n = 0;
+  cudaError_t e = cudaDeviceSynchronize();
+  if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&n, lost_clusters, sizeof n);
+  if (e != cudaSuccess) {
+    (void)cudaGetLastError();
+    set_last_cuda_error(e);
+    return FL_B200_ERR_NO_DEVICE;
+  }
+  *count = n;
+  return FL_B200_OK;
+}
 
 FL_B200_API int fl_b200_distill_topk_fwd(const void* logits, int64_t ld, const void* teacher,
                                          int64_t ld_t, int t_dtype, const void* ids, int64_t ld_ids,

@@ -87,6 +87,14 @@ __device__ __forceinline__ float2 ld_remote_f2(uint32_t addr) {
                : "memory");
   return v;
 }
+__device__ __forceinline__ int ld_remote_s32(uint32_t addr) {
+  int v;
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void st_remote_s32(uint32_t addr, int v) {
+  asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
 __device__ __forceinline__ long long ld_remote_s64(uint32_t addr) {
   long long v;
   asm volatile("ld.shared::cluster.s64 %0, [%1];" : "=l"(v) : "r"(addr) : "memory");
@@ -119,26 +127,52 @@ __device__ __forceinline__ void send_f2(uint32_t slot, float a, float b, uint32_
                "f"(a), "f"(b), "r"(bar)
                : "memory");
 }
-// Waits for the phase of this parity, a bounded number of tries (seconds;
-// a wait takes microseconds).  When they run out, *lost is set, after which
-// no wait of the CTA tries again; the caller reports what it computed then
-// as NaN.
-__device__ __forceinline__ void bar_wait(uint64_t* bar, uint32_t parity, volatile int* lost) {
-  const uint32_t addr = (uint32_t)__cvta_generic_to_shared(bar);
-  for (int tries = 0;; ++tries) {
-    uint32_t done;
-    asm volatile(
-        "{ .reg .pred p; mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2; "
-        "selp.u32 %0, 1, 0, p; }"
-        : "=r"(done)
-        : "r"(addr), "r"(parity)
-        : "memory");
-    if (done) return;
-    if (tries > (1 << 20) || *lost) {
-      *lost = 1;
-      return;
-    }
-  }
+// Counts `bytes` on this CTA's barrier as if they had come.
+__device__ __forceinline__ void bar_give(uint64_t* bar, int bytes) {
+  asm volatile("mbarrier.complete_tx.relaxed.cluster.shared::cta.b64 [%0], %1;" ::"r"(
+                   (uint32_t)__cvta_generic_to_shared(bar)),
+               "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ uint64_t nanoseconds() {
+  uint64_t t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+  return t;
+}
+// Whether the phase of this parity is over: at once, and after a while that
+// the hardware sets if it is not.
+__device__ __forceinline__ bool bar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{ .reg .pred p; mbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2; "
+      "selp.u32 %0, 1, 0, p; }"
+      : "=r"(done)
+      : "r"((uint32_t)__cvta_generic_to_shared(bar)), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+__device__ __forceinline__ bool bar_try(uint64_t* bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{ .reg .pred p; mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2; "
+      "selp.u32 %0, 1, 0, p; }"
+      : "=r"(done)
+      : "r"((uint32_t)__cvta_generic_to_shared(bar)), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+// Waits for the phase of this parity, `limit` nanoseconds at most (0: not at
+// all) and no longer once *lost is set; a wait takes microseconds.  Whether the
+// phase is over.
+__device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, const volatile int* lost,
+                                         uint32_t limit) {
+  if (bar_test(bar, parity)) return true;
+  if (limit == 0) return false;
+  if (bar_try(bar, parity)) return true;  // (before the clock is read, which takes longer)
+  const uint64_t start = nanoseconds();
+  while (!*lost && nanoseconds() - start < limit)
+    if (bar_try(bar, parity)) return true;
+  return false;
 }
 // Asynchronous bulk copies of 16-byte multiples between 16-byte boundaries:
 // global to this CTA's shared memory, counted on its barrier, and back, in

@@ -83,6 +83,8 @@ PROTOTYPES: dict[str, tuple] = {
     "fl_b200_softmax_bwd": (_i32, [_p, _i64, _p, _i64, _p, _i64, _i64, _i64, _i32, _i32, _p]),
     "fl_b200_softmax_bwd_scaled": (
         _i32, [_p, _i64, _p, _i64, _p, _i64, _i64, _i64, _f32, _i32, _i32, _p]),
+    "fl_b200_set_wait_limit": (_i64, [_i64]),
+    "fl_b200_lost_waits": (_i32, [C.POINTER(C.c_uint64)]),
     "fl_b200_topk_lastdim": (_i32, [_p, _i64, _i64, _i64, _i64, _p, _p, _i32, _p]),
     "fl_b200_topk_bwd": (_i32, [_p, _p, _p, _i64, _i64, _i64, _i32, _p]),
     "fl_b200_distill_topk_fwd": (
@@ -153,6 +155,20 @@ def set_pdl(enable: bool) -> bool:
     default) or without; returns the previous setting.  Results are the
     same either way."""
     return bool(load().fl_b200_set_pdl(1 if enable else 0))
+
+
+def set_wait_limit(nanoseconds: int) -> int:
+    """How long a kernel's waits for a copy or another block may last (2e9 by
+    default); returns the previous limit.  Clusters that give one up return
+    NaN for their rows and are counted by `lost_waits`."""
+    return load().fl_b200_set_wait_limit(int(nanoseconds))
+
+
+def lost_waits() -> int:
+    """Clusters that gave up a wait on the current device so far."""
+    n = C.c_uint64()
+    call("fl_b200_lost_waits", C.byref(n))
+    return n.value
 
 
 def i64_array(vals) -> C.Array:

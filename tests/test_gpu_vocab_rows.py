@@ -27,6 +27,7 @@ import torch
 import torch_fl
 from oracle import ops
 from tests import parity
+from torch_fl import _abi
 from torch_fl import kernels as K
 
 pytestmark = pytest.mark.gpu
@@ -647,6 +648,36 @@ def test_vocabularies_past_eight_ctas():
     for R, V, dt in ((5, 151936, torch.bfloat16), (4, 262144, torch.float16), (4, 70000, torch.float32),
                      (3, 131072, torch.float32), (3, 262145, torch.bfloat16), (3, 131073, torch.float32)):
         check_distill(*make(R, V, 20, dt, R + V % 97), tau=1.3, what=f"{R}x{V}")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("R,V,k", [(600, 8008, 20), (300, 40003, 64), (40, 128256, 100), (9, 100, 3)])
+def test_a_wait_that_runs_out_is_nan_for_the_whole_row(dtype, R, V, k):
+    """With a limit of 0 a wait that finds nothing gives up: every row is then
+    either whole or NaN throughout (loss, gradient), the clusters that gave up
+    are counted, and the next call is as before."""
+    z, t, ids, w = make(R, V, k, dtype, 97 + R)
+    want = K.distill_topk_grad(z, t, ids, 2.0, w)
+    before = _abi.lost_waits()
+    limit = _abi.set_wait_limit(0)
+    try:
+        runs = [K.distill_topk_grad(z, t, ids, 2.0, w) for _ in range(3)]
+        lost = _abi.lost_waits() - before
+    finally:
+        assert _abi.set_wait_limit(limit) == 0
+    assert limit == 2_000_000_000
+    nan = 0
+    for loss, dz in runs:
+        gone = torch.isnan(loss)
+        nan += int(gone.sum())
+        assert torch.isnan(dz[gone]).all()
+        assert torch.equal(loss[~gone], want[0][~gone]) and torch.equal(dz[~gone], want[1][~gone])
+    assert nan >= lost                                  # (a cluster has a row at least)
+    # (a few hundred bytes may have come before they are first looked for: then no wait runs out)
+    assert lost > 0 or z.numel() * z.element_size() < 1 << 16
+    again = K.distill_topk_grad(z, t, ids, 2.0, w)
+    assert torch.equal(again[0], want[0]) and torch.equal(again[1], want[1])
+    assert _abi.lost_waits() == before + lost
 
 
 def test_draft_model_from_teacher_to_verification():

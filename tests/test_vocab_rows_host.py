@@ -163,6 +163,13 @@ def test_empty_work_is_a_no_op():
               None, None, 0, 1, None)
 
 
+def test_the_wait_limit_is_clamped_and_comes_back():
+    first = _abi.set_wait_limit(-5)
+    assert first == 2_000_000_000
+    assert _abi.set_wait_limit(1 << 40) == 0
+    assert _abi.set_wait_limit(first) == 2_000_000_000
+
+
 def test_a_message_with_numbers_is_an_error_not_a_crash():
     """Native checks whose message holds integers raise (in a child process:
     they once ended it)."""
