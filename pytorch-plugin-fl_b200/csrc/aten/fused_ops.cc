@@ -560,10 +560,33 @@ const c10::TypedOperatorHandle<Fn>& Below(const char* name) {
   return op;
 }
 using TopkFn = std::tuple<at::Tensor, at::Tensor>(const at::Tensor&, int64_t);
+using TopkBackwardFn = at::Tensor(const at::Tensor&, const at::Tensor&, int64_t);
 using DistillFn = std::tuple<at::Tensor, at::Tensor>(const at::Tensor&, const at::Tensor&,
                                                      const at::Tensor&, double);
 
-// dx = dvalues at the indices, 0 elsewhere.
+// dx = dvalues at the indices, 0 elsewhere: linear in dvalues, whose own
+// gradient is dx's, gathered (0 where an index lies outside the row).
+struct TopkGradGrad : torch::autograd::Function<TopkGradGrad> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& dvalues, const at::Tensor& indices,
+                            int64_t cols) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    ctx->save_for_backward({indices});
+    ctx->saved_data["cols"] = cols;
+    return Below<TopkBackwardFn>("flagos::topk_backward").call(dvalues, indices, cols);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const int64_t cols = ctx->saved_data["cols"].toInt();
+    const at::Tensor indices = ctx->get_saved_variables()[0];
+    const at::Tensor taken = grads[0].gather(-1, indices.clamp(0, std::max<int64_t>(cols - 1, 0)));
+    return {at::where(indices.ge(0).logical_and(indices.lt(cols)), taken, at::zeros_like(taken)),
+            at::Tensor(), at::Tensor()};
+  }
+};
+at::Tensor TopkBackwardAutograd(const at::Tensor& dvalues, const at::Tensor& indices, int64_t cols) {
+  if (at::GradMode::is_enabled() && dvalues.requires_grad()) return TopkGradGrad::apply(dvalues, indices, cols);
+  at::AutoDispatchBelowADInplaceOrView guard;
+  return Below<TopkBackwardFn>("flagos::topk_backward").call(dvalues, indices, cols);
+}
 struct TopkGrad : torch::autograd::Function<TopkGrad> {
   static variable_list forward(AutogradContext* ctx, const at::Tensor& x, int64_t k) {
     at::AutoDispatchBelowADInplaceOrView guard;
@@ -576,8 +599,8 @@ struct TopkGrad : torch::autograd::Function<TopkGrad> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     if (!grads[0].defined()) return {at::Tensor(), at::Tensor()};
-    return {TopkBackward(grads[0], ctx->get_saved_variables()[0], ctx->saved_data["cols"].toInt()),
-            at::Tensor()};
+    const auto call = at::GradMode::is_enabled() ? TopkBackwardAutograd : TopkBackward;
+    return {call(grads[0], ctx->get_saved_variables()[0], ctx->saved_data["cols"].toInt()), at::Tensor()};
   }
 };
 std::tuple<at::Tensor, at::Tensor> TopkAutograd(const at::Tensor& x, int64_t k) {
@@ -678,10 +701,10 @@ TORCH_LIBRARY_IMPL(flagos, PrivateUse1, m) { FLB_FUSED_IMPLS(m) }
 TORCH_LIBRARY_IMPL(flagos, CUDA, m) { FLB_FUSED_IMPLS(m) }
 TORCH_LIBRARY_IMPL(flagos, Autograd, m) {
   m.impl("topk", TopkAutograd);
+  m.impl("topk_backward", TopkBackwardAutograd);
   m.impl("distill_topk", DistillTopkAutograd);
   // Not differentiable: their results have no history.  (Without a word here
   // PyTorch boxes every call to say so on a backward.)
-  m.impl("topk_backward", torch::CppFunction::makeFallthrough());
   m.impl("distill_topk_backward", torch::CppFunction::makeFallthrough());
   m.impl("distill_topk_grad", torch::CppFunction::makeFallthrough());
   m.impl("verify_draft", torch::CppFunction::makeFallthrough());

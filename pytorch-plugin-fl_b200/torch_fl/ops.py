@@ -82,7 +82,7 @@ def topk(x, k: int):
     """(values, indices) of the k <= 1024 largest elements over the last dim,
     descending; equal values (-0 and +0 among them) by ascending index, NaN
     above everything, so there is one right answer.  Gradient: dvalues at the
-    indices."""
+    indices, which can be differentiated again."""
     return torch.ops.flagos.topk(x, int(k))
 
 

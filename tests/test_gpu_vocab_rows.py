@@ -160,6 +160,32 @@ def test_topk_gradient():
         assert torch.equal(got, torch.zeros(5, 1001, dtype=dt, device=DEV).scatter_(1, idx, d))
 
 
+def test_topk_second_derivative():
+    """A penalty on the gradient through topk: f = sum v^3 has the gradient 3 v^2
+    at the indices, and sum of its squares 36 v^3.  Products of one sign
+    throughout, each through at most 16 roundings."""
+    x = torch.randn(4, 3, 257, generator=gen(8))
+    xf = x.to("flagos").requires_grad_()
+    v, i = torch_fl.ops.topk(xf, 5)
+    g, = torch.autograd.grad((v * v * v).sum(), xf, create_graph=True)
+    assert g.requires_grad
+    (xf.sum() + (g * g).sum()).backward()
+    vd = np64(torch.gather(x, -1, i.cpu()))
+    ref = np.ones(x.shape)
+    np.put_along_axis(ref, i.cpu().numpy(), 1 + 36 * vd ** 3, -1)
+    size = np.ones(x.shape)
+    np.put_along_axis(size, i.cpu().numpy(), 1 + 36 * np.abs(vd) ** 3, -1)
+    within(xf.grad, ref, 16 * U * size, "second derivative")
+    # by its own op, where an index may lie outside the row; and a third time
+    d = torch.randn(2, 3, generator=gen(9)).to("flagos").requires_grad_()
+    idx = torch.tensor([[5, -1, 0], [9, 3, 4]]).to("flagos")
+    dx = torch.ops.flagos.topk_backward(d, idx, 9)
+    c = torch.randn(2, 9, generator=gen(10))
+    (dx * c.to("flagos")).sum().backward()
+    want = torch.where((idx.cpu() >= 0) & (idx.cpu() < 9), torch.gather(c, -1, idx.cpu().clamp(0, 8)), 0.0)
+    assert torch.equal(d.grad.cpu(), want)
+
+
 # --------------------------------------------------------------- distillation
 def make(R, V, k, dtype, seed, t_dtype=None, ids_dtype=torch.int64, holes=True):
     g = gen(seed)
