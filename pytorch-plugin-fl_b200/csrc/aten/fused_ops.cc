@@ -563,6 +563,9 @@ using TopkFn = std::tuple<at::Tensor, at::Tensor>(const at::Tensor&, int64_t);
 using TopkBackwardFn = at::Tensor(const at::Tensor&, const at::Tensor&, int64_t);
 using DistillFn = std::tuple<at::Tensor, at::Tensor>(const at::Tensor&, const at::Tensor&,
                                                      const at::Tensor&, double);
+using DistillBackwardFn = std::tuple<at::Tensor, at::Tensor>(const at::Tensor&, const at::Tensor&,
+                                                             const at::Tensor&, const at::Tensor&,
+                                                             const at::Tensor&, double, bool, bool);
 
 // dx = dvalues at the indices, 0 elsewhere: linear in dvalues, whose own
 // gradient is dx's, gathered (0 where an index lies outside the row).
@@ -612,6 +615,34 @@ std::tuple<at::Tensor, at::Tensor> TopkAutograd(const at::Tensor& x, int64_t k) 
   return Below<TopkFn>("flagos::topk").call(x, k);
 }
 
+// The gradients where a graph of them is wanted: there is no second
+// derivative, which is said when it is asked for.
+struct DistillGradGrad : torch::autograd::Function<DistillGradGrad> {
+  static variable_list forward(AutogradContext*, const at::Tensor& dloss, const at::Tensor& logits,
+                               const at::Tensor& stats, const at::Tensor& teacher, const at::Tensor& ids,
+                               double temperature, bool need_logits, bool need_teacher) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    auto [dx, dt] = Below<DistillBackwardFn>("flagos::distill_topk_backward")
+                        .call(dloss, logits, stats, teacher, ids, temperature, need_logits, need_teacher);
+    return {dx, dt};
+  }
+  static variable_list backward(AutogradContext*, variable_list) {
+    TORCH_CHECK(false, "flagos::distill_topk: there is no second derivative");
+  }
+};
+std::tuple<at::Tensor, at::Tensor> DistillTopkBackwardAutograd(
+    const at::Tensor& dloss, const at::Tensor& logits, const at::Tensor& stats, const at::Tensor& teacher,
+    const at::Tensor& ids, double temperature, bool need_logits, bool need_teacher) {
+  if (at::GradMode::is_enabled() &&
+      (dloss.requires_grad() || logits.requires_grad() || teacher.requires_grad())) {
+    auto out = DistillGradGrad::apply(dloss, logits, stats, teacher, ids, temperature, need_logits, need_teacher);
+    return {out[0], out[1]};
+  }
+  at::AutoDispatchBelowADInplaceOrView guard;
+  return Below<DistillBackwardFn>("flagos::distill_topk_backward")
+      .call(dloss, logits, stats, teacher, ids, temperature, need_logits, need_teacher);
+}
+
 // Both operands' gradients from the forward's row statistics, which have none.
 struct DistillGrad : torch::autograd::Function<DistillGrad> {
   static variable_list forward(AutogradContext* ctx, const at::Tensor& logits, const at::Tensor& teacher,
@@ -629,8 +660,9 @@ struct DistillGrad : torch::autograd::Function<DistillGrad> {
     variable_list none(4);
     if (!grads[0].defined() || (!logits && !teacher)) return none;
     const auto saved = ctx->get_saved_variables();
-    auto [dx, dt] = DistillTopkBackward(grads[0], saved[0], saved[3], saved[1], saved[2],
-                                        ctx->saved_data["temperature"].toDouble(), logits, teacher);
+    const auto call = at::GradMode::is_enabled() ? DistillTopkBackwardAutograd : DistillTopkBackward;
+    auto [dx, dt] = call(grads[0], saved[0], saved[3], saved[1], saved[2],
+                         ctx->saved_data["temperature"].toDouble(), logits, teacher);
     if (logits) none[0] = dx;
     if (teacher) none[1] = dt;
     return none;
@@ -703,9 +735,9 @@ TORCH_LIBRARY_IMPL(flagos, Autograd, m) {
   m.impl("topk", TopkAutograd);
   m.impl("topk_backward", TopkBackwardAutograd);
   m.impl("distill_topk", DistillTopkAutograd);
+  m.impl("distill_topk_backward", DistillTopkBackwardAutograd);
   // Not differentiable: their results have no history.  (Without a word here
   // PyTorch boxes every call to say so on a backward.)
-  m.impl("distill_topk_backward", torch::CppFunction::makeFallthrough());
   m.impl("distill_topk_grad", torch::CppFunction::makeFallthrough());
   m.impl("verify_draft", torch::CppFunction::makeFallthrough());
 }

@@ -440,6 +440,30 @@ def test_distill_autograd_on_flagos():
     assert not stats.requires_grad              # the row statistics have no gradient
 
 
+def test_distill_second_derivative_is_refused():
+    """The gradient itself is there under create_graph; to differentiate it
+    again is an error, not a term that is missing."""
+    z, t, ids, _ = make(5, 700, 6, torch.float32, 32)
+    zf, tf = z.cpu().to("flagos").requires_grad_(), t.cpu().to("flagos").requires_grad_()
+    idf = ids.cpu().to("flagos")
+    plain = torch.autograd.grad(torch_fl.ops.distill_topk(zf, tf, idf, 2.0).sum(), (zf, tf))
+    loss = torch_fl.ops.distill_topk(zf, tf, idf, 2.0)
+    gz, gt = torch.autograd.grad(loss.sum(), (zf, tf), create_graph=True)
+    assert torch.equal(gz, plain[0]) and torch.equal(gt, plain[1])
+    for term in ((gz * gz).sum() + zf.sum(), (gt * gt).sum()):
+        with pytest.raises(RuntimeError, match="second derivative"):
+            term.backward(retain_graph=True)
+    # one operand alone, and by the backward's own op
+    loss = torch_fl.ops.distill_topk(zf, tf.detach(), idf, 2.0)
+    gz, = torch.autograd.grad(loss.sum(), zf, create_graph=True)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        (gz * gz).sum().backward()
+    loss, stats = torch.ops.flagos.distill_topk(zf.detach(), tf.detach(), idf, 2.0)
+    dx, _ = torch.ops.flagos.distill_topk_backward(torch.ones_like(loss), zf, stats, tf.detach(), idf, 2.0)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        dx.sum().backward()
+
+
 def test_distill_shapes_of_every_rank():
     z, t, ids, w = make(12, 333, 5, torch.float32, 33)
     want = K.distill_topk_grad(z, t, ids, 2.0, w)
