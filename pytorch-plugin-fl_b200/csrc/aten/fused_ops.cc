@@ -559,6 +559,10 @@ const c10::TypedOperatorHandle<Fn>& Below(const char* name) {
   static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Fn>();
   return op;
 }
+// There is no forward-mode formula: a tangent would be dropped unseen.
+void NoTangent(const at::Tensor& t, const char* op) {
+  TORCH_CHECK(!t._fw_grad(/*level=*/0).defined(), op, ": forward-mode derivatives are not there");
+}
 using TopkFn = std::tuple<at::Tensor, at::Tensor>(const at::Tensor&, int64_t);
 using TopkBackwardFn = at::Tensor(const at::Tensor&, const at::Tensor&, int64_t);
 using DistillFn = std::tuple<at::Tensor, at::Tensor>(const at::Tensor&, const at::Tensor&,
@@ -607,6 +611,7 @@ struct TopkGrad : torch::autograd::Function<TopkGrad> {
   }
 };
 std::tuple<at::Tensor, at::Tensor> TopkAutograd(const at::Tensor& x, int64_t k) {
+  NoTangent(x, "flagos::topk");
   if (at::GradMode::is_enabled() && x.requires_grad()) {
     auto out = TopkGrad::apply(x, k);
     return {out[0], out[1]};
@@ -670,6 +675,8 @@ struct DistillGrad : torch::autograd::Function<DistillGrad> {
 };
 std::tuple<at::Tensor, at::Tensor> DistillTopkAutograd(const at::Tensor& logits, const at::Tensor& teacher,
                                                        const at::Tensor& ids, double temperature) {
+  NoTangent(logits, "flagos::distill_topk");
+  NoTangent(teacher, "flagos::distill_topk");
   if (at::GradMode::is_enabled() && (logits.requires_grad() || teacher.requires_grad())) {
     auto out = DistillGrad::apply(logits, teacher, ids, temperature);
     return {out[0], out[1]};

@@ -97,7 +97,8 @@ def distill_topk(logits, teacher_logits, teacher_ids, temperature: float = 1.0):
     The teacher's softmax is over its list; entries whose id lies outside
     [0, vocab) (-1, say) are absent, and a row without any has loss 0 and zero
     gradients whatever its logits hold.  Repeated ids add.  Differentiable once
-    in logits and in teacher_logits (a second derivative raises); the gradient is computed from the saved
+    in logits and in teacher_logits (a second derivative raises, and so do
+    forward mode and torch.func's transforms of gradients); the gradient is computed from the saved
     logits, so they are read three times in all: `distill_topk_grad` reads
     them once."""
     return torch.ops.flagos.distill_topk(logits, teacher_logits, teacher_ids, float(temperature))[0]

@@ -464,6 +464,22 @@ def test_distill_second_derivative_is_refused():
         dx.sum().backward()
 
 
+def test_forward_mode_is_refused():
+    """There is no forward-mode formula; a tangent is not dropped unseen."""
+    import torch.autograd.forward_ad as fwd
+
+    z, t, ids, _ = make(5, 700, 6, torch.float32, 32)
+    zf, tf, idf = (v.cpu().to("flagos") for v in (z, t, ids))
+    with fwd.dual_level():
+        zd, td = fwd.make_dual(zf, torch.ones_like(zf)), fwd.make_dual(tf, torch.ones_like(tf))
+        for call in (lambda: torch_fl.ops.topk(zd, 3), lambda: torch_fl.ops.distill_topk(zd, tf, idf),
+                     lambda: torch_fl.ops.distill_topk(zf, td, idf)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        torch_fl.ops.topk(zf, 3)
+        torch_fl.ops.distill_topk(zf, tf, idf)
+
+
 def test_distill_shapes_of_every_rank():
     z, t, ids, w = make(12, 333, 5, torch.float32, 33)
     want = K.distill_topk_grad(z, t, ids, 2.0, w)
