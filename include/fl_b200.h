@@ -450,8 +450,9 @@ FL_B200_API int fl_b200_distill_topk_fwd(const void* logits, int64_t ld, const v
 /* Gradients for dloss[r * dloss_stride] (F32; NULL: 1 for every row):       *
  *   dlogits_v = dloss * temperature * (q_v - sum over id_j = v of p_j),      *
  *   dteacher_j = dloss * temperature * p_j (log p_j - log q[id_j] - KL).    *
- * dlogits (logits' dtype, stride ld_dlogits; never logits) and dteacher     *
- * (the teacher's dtype, dense [rows, k]) may each be NULL.  Rows are stored *
+ * dlogits (logits' dtype, stride ld_dlogits) and dteacher (the teacher's    *
+ * dtype, dense [rows, k]) may each be NULL; their rows share no memory with *
+ * an operand's, which is refused (here and below).  Rows are stored         *
  * 16 bytes at a time when the logits' and the gradient's rows begin at the   *
  * same offset from a 16-byte boundary, one element at a time otherwise.     */
 FL_B200_API int fl_b200_distill_topk_bwd(const float* dloss, int64_t dloss_stride,

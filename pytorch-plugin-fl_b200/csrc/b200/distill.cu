@@ -1207,6 +1207,32 @@ bool same_phase(const void* x, int64_t ld, const void* y, int64_t ld_y, int64_t 
          (ld - ld_y) * size % 16 == 0;
 }
 
+// The rows of a matrix in memory, and whether a row of one meets a row of
+// another.  (Rows may lie between each other's.)
+struct Region {
+  const void* p;
+  int64_t ld, cols, rows;  // elements
+  int64_t size;
+};
+bool meet(const Region& a, const Region& b) {
+  if (a.p == nullptr || b.p == nullptr || a.cols == 0 || b.cols == 0) return false;
+  const uintptr_t la = a.ld * a.size, lb = b.ld * b.size, na = a.cols * a.size, nb = b.cols * b.size;
+  uintptr_t x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
+  if (x + (a.rows - 1) * la + na <= y || y + (b.rows - 1) * lb + nb <= x) return false;
+  for (int64_t i = 0, j = 0; i < a.rows && j < b.rows;) {
+    if (x + na <= y) {
+      x += la;
+      ++i;
+    } else if (y + nb <= x) {
+      y += lb;
+      ++j;
+    } else {
+      return true;
+    }
+  }
+  return false;
+}
+
 // Calls go(NS, E): the threads that stream a row (and one warp more for its
 // list) and the list's entries a lane.  Rows of up to 64 KB go to CTAs of 128
 // threads, of which more are resident to hide the lists' latency (forward,
@@ -1404,8 +1430,18 @@ FL_B200_API int fl_b200_distill_topk_bwd(const float* dloss, int64_t dloss_strid
   FLB_CHECK_ARG(dloss_stride >= 0 && logits && stats && (k == 0 || (teacher && ids)));
   FLB_CHECK_ARG((rows == 1 || ld >= cols) && ld_t >= 0 && ld_ids >= 0);
   FLB_CHECK_ARG(dlogits == nullptr || rows == 1 || ld_dlogits >= cols);
-  FLB_CHECK_ARG(dlogits != logits);  // (tokens are read again after their row is stored)
   if (reinterpret_cast<uintptr_t>(stats) % 8) return FL_B200_ERR_MISALIGNED;
+  // an operand may be read after any row of a gradient is stored
+  const Region out[] = {{dlogits, ld_dlogits, cols, rows, dtype_size(dtype)},
+                        {dteacher, k, k, rows, dtype_size(t_dtype)}};
+  const Region in[] = {{logits, ld, cols, rows, dtype_size(dtype)},
+                       {teacher, ld_t, k, rows, dtype_size(t_dtype)},
+                       {ids, ld_ids, k, rows, dtype_size(ids_dtype)},
+                       {dloss, dloss_stride, 1, rows, 4},
+                       {stats, 2, 2, rows, 4}};
+  for (const Region& o : out)
+    for (const Region& i : in) FLB_CHECK_ARG(!meet(o, i));
+  FLB_CHECK_ARG(!meet(out[0], out[1]));
   const Taught a = taught(teacher, ld_t, t_dtype, ids, ld_ids, ids_dtype, k, temperature);
   return dispatch_float(dtype, [&](auto t) {
     return run_bwd<decltype(t)>(dloss, dloss_stride, logits, ld, stats, a, rows, cols, dlogits,
@@ -1421,7 +1457,7 @@ FL_B200_API int fl_b200_distill_topk_grad(const void* logits, int64_t ld, const 
                                           void* dlogits, int64_t ld_dlogits, int dtype,
                                           fl_b200_stream_t stream) {
   using namespace flb200;
-  FLB_CHECK_ARG(rows <= 0 || (dlogits && dlogits != logits && (rows == 1 || ld_dlogits >= cols)));
+  FLB_CHECK_ARG(rows <= 0 || (dlogits && (rows == 1 || ld_dlogits >= cols)));
   FLB_CHECK_ARG(weight_stride >= 0);
   int st = check_shapes(rows, cols, k, temperature);
   if (st != FL_B200_OK) return st;
@@ -1431,6 +1467,17 @@ FL_B200_API int fl_b200_distill_topk_grad(const void* logits, int64_t ld, const 
   FLB_CHECK_ARG(logits && loss && stats && (k == 0 || (teacher && ids)));
   FLB_CHECK_ARG((rows == 1 || ld >= cols) && ld_t >= 0 && ld_ids >= 0);
   if (reinterpret_cast<uintptr_t>(stats) % 8) return FL_B200_ERR_MISALIGNED;
+  // rows are read and stored in no order
+  const Region out[] = {{dlogits, ld_dlogits, cols, rows, dtype_size(dtype)},
+                        {loss, 1, 1, rows, 4},
+                        {stats, 2, 2, rows, 4}};
+  const Region in[] = {{logits, ld, cols, rows, dtype_size(dtype)},
+                       {teacher, ld_t, k, rows, dtype_size(t_dtype)},
+                       {ids, ld_ids, k, rows, dtype_size(ids_dtype)},
+                       {row_weight, weight_stride, 1, rows, 4}};
+  for (const Region& o : out)
+    for (const Region& i : in) FLB_CHECK_ARG(!meet(o, i));
+  FLB_CHECK_ARG(!meet(out[0], out[1]) && !meet(out[0], out[2]));
   if (same_phase(logits, ld, dlogits, ld_dlogits, dtype_size(dtype))) {
     const Taught a = taught(teacher, ld_t, t_dtype, ids, ld_ids, ids_dtype, k, temperature);
     DeviceInfo dev;

@@ -659,7 +659,8 @@ def distill_topk_backward(dloss: torch.Tensor | None, logits: torch.Tensor, stat
 def distill_topk_grad(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ids: torch.Tensor,
                       temperature: float = 1.0, row_weight: torch.Tensor | None = None,
                       out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
-    """(loss, dlogits) of sum(row_weight * loss) in one call."""
+    """(loss, dlogits) of sum(row_weight * loss) in one call.  out may hold the
+    gradient; its rows share no memory with an operand's."""
     (x, *keep), head, lists, rows, cols, k = _taught(logits, teacher_logits, teacher_ids)
     _one_device(x, row_weight, out)
     w, wp, ws = _row_weight(row_weight, logits.shape[:-1])
@@ -668,8 +669,6 @@ def distill_topk_grad(logits: torch.Tensor, teacher_logits: torch.Tensor, teache
     dx = torch.empty(logits.shape, dtype=x.dtype, device=x.device) if out is None else out
     if dx.shape != logits.shape or dx.dtype != x.dtype:
         raise ValueError("out must have the logits' shape and dtype")
-    if out is not None and out.data_ptr() == x.data_ptr() and out.numel():
-        raise ValueError("the gradient is not computed in place")
     _, _, ldo = _rows_view(dx)
     with _on_device(x):
         _abi.call("fl_b200_distill_topk_grad", *head, *lists, wp, ws, rows, cols, k,

@@ -302,6 +302,24 @@ def test_distill_mixed_types_and_strides():
     assert torch.equal(out[:, 1:2049], dz2) and not out[:, 0].any() and not out[:, 2049:].any()
 
 
+def test_distill_gradient_between_the_logits_rows():
+    """Logits and gradient as the two halves of one matrix's rows share no
+    memory and are computed; an `out` that meets the logits is refused."""
+    z, t, ids, w = make(6, 2048, 10, torch.bfloat16, 13)
+    want = K.distill_topk_grad(z, t, ids, 2.0, w)
+    both = torch.zeros(6, 4096, dtype=torch.bfloat16, device=DEV)
+    both[:, :2048] = z
+    loss, dz = K.distill_topk_grad(both[:, :2048], t, ids, 2.0, w, out=both[:, 2048:])
+    assert torch.equal(loss, want[0]) and torch.equal(dz, want[1]) and torch.equal(both[:, :2048], z)
+    wide = torch.zeros(7, 2048, dtype=torch.bfloat16, device=DEV)
+    for out in (z, both[:, 1024:3072], both[:, 2047:4095]):
+        logits = z if out is z else both[:, :2048]
+        with pytest.raises(_abi.FlB200Error, match="invalid argument"):
+            K.distill_topk_grad(logits, t, ids, 2.0, w, out=out)
+    with pytest.raises(_abi.FlB200Error, match="invalid argument"):
+        K.distill_topk_grad(wide[:6], t, ids, 2.0, w, out=wide[1:])
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("V", [999, 4096, 128256])
 def test_distill_special_rows(dtype, V):

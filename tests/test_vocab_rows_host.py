@@ -132,6 +132,34 @@ def test_bad_arguments_are_refused_on_the_host(call, status):
     assert e.value.status == status
 
 
+def _apart(grad=True, **at):
+    """A call over 4 rows of 8 bf16 logits, 2 teacher entries a row, each operand
+    in a 4 KB page of its own but where `at` puts it."""
+    names = ("logits", "teacher", "ids", "weight", "loss", "stats", "dlogits", "dteacher")
+    p = {n: 0x100000 + 0x1000 * i for i, n in enumerate(names)} | at
+    if grad:
+        return lambda: _abi.call("fl_b200_distill_topk_grad", p["logits"], 8, p["teacher"], 2, 1, p["ids"], 2, 4,
+                                 p["weight"], 1, 4, 8, 2, 1.0, p["loss"], p["stats"], p["dlogits"], 8, 1, None)
+    return lambda: _abi.call("fl_b200_distill_topk_bwd", p["weight"], 1, p["logits"], 8, p["stats"], p["teacher"], 2,
+                             1, p["ids"], 2, 4, p["dlogits"], 8, p["dteacher"], 4, 8, 2, 1.0, 1, None)
+
+
+@pytest.mark.parametrize("call", [
+    _apart(dlogits=0x100000), _apart(dlogits=0x100010), _apart(dlogits=0x100000 - 48), _apart(dlogits=0x10003e),
+    _apart(dlogits=0x101000 - 60), _apart(dlogits=0x102030), _apart(dlogits=0x103008), _apart(dlogits=0x104000),
+    _apart(dlogits=0x105010), _apart(loss=0x10000c), _apart(stats=0x102008), _apart(loss=0x103000),
+    _apart(False, dlogits=0x100010), _apart(False, dlogits=0x100000 - 16), _apart(False, dlogits=0x101004),
+    _apart(False, dteacher=0x101000), _apart(False, dteacher=0x10003e), _apart(False, dteacher=0x105004),
+    _apart(False, dteacher=0x106020), _apart(False, dteacher=0x103000), _apart(False, dlogits=0x102000),
+])
+def test_results_that_overlap_an_operand_are_refused(call):
+    """Rows are read and stored in no order: a result that shares memory with an
+    operand, at whatever offset, is a race."""
+    with pytest.raises(_abi.FlB200Error) as e:
+        call()
+    assert e.value.status == INVALID
+
+
 def test_tensor_entry_points_refuse_before_they_launch():
     """K.*: shapes, types and CPU tensors are refused on the host."""
     import torch
