@@ -645,7 +645,7 @@ distill_bwd_kernel(const float* __restrict__ dloss, int64_t dloss_stride, const 
   const bool want_dt = dt != nullptr && part == 0;
   if (tid >= NS) {
     if (live)
-      list.load(shared, a, nullptr, 0, xr, row, cols, part == 0 ? 0 : lo, part == 0 ? cols : hi, true);
+      list.load(shared, a, nullptr, 0, xr, row, cols, part == 0 ? 0 : lo, part == 0 ? cols : hi, dx != nullptr);
     if (want_dt) {
       if (live) {
         list.teacher(shared, a, st.x, st.y, gt, dt, row);
@@ -1306,10 +1306,10 @@ int run_bwd(const float* dloss, int64_t dloss_stride, const void* x, int64_t ld,
     constexpr int NS = decltype(ns)::value, E = decltype(e)::value;
     // chunks of 4 rounds of loads, which hide the list's latency (2048 x 128256
     // bf16: 201 us, 249 us with one round), of 16 for a long list; shorter where
-    // rows are few
+    //     // where rows are few; the teacher's gradient alone is one CTA's work
     const int64_t round = (int64_t)NS * kUnroll * Elem<T>::kVec;
     int64_t chunk = dx == nullptr ? cols : (E == 0 ? 16 : 4) * round;
-    while (chunk > round && rows * ceil_div(cols, chunk) < 4 * dev.sm_count) chunk /= 2;
+    while (dx != nullptr && chunk > round && rows * ceil_div(cols, chunk) < 4 * dev.sm_count) chunk /= 2;
     const int64_t chunks = ceil_div(cols, chunk);
     if (rows * chunks > 0x7fffffffLL) return (int)FL_B200_ERR_TOO_LARGE;
     const auto go = [&](auto kern) {

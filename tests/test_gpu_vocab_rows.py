@@ -458,6 +458,57 @@ def test_distill_autograd_on_flagos():
     assert not stats.requires_grad              # the row statistics have no gradient
 
 
+def blocks_of(call):
+    """Blocks of each kernel that the call launches, from a captured graph."""
+    import ctypes
+
+    class Params(ctypes.Structure):     # CUDA_KERNEL_NODE_PARAMS
+        _fields_ = [("func", ctypes.c_void_p), ("grid", ctypes.c_uint * 3), ("block", ctypes.c_uint * 3),
+                    ("smem", ctypes.c_uint), ("params", ctypes.c_void_p), ("extra", ctypes.c_void_p),
+                    ("kern", ctypes.c_void_p), ("ctx", ctypes.c_void_p)]
+
+    cuda = ctypes.CDLL("libcuda.so.1")
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(graph):
+        call()
+    raw, n = ctypes.c_void_p(graph.raw_cuda_graph()), ctypes.c_size_t()
+    assert cuda.cuGraphGetNodes(raw, None, ctypes.byref(n)) == 0
+    nodes = (ctypes.c_void_p * n.value)()
+    assert cuda.cuGraphGetNodes(raw, nodes, ctypes.byref(n)) == 0
+    blocks = []
+    for node in nodes:
+        kind = ctypes.c_int()
+        assert cuda.cuGraphNodeGetType(ctypes.c_void_p(node), ctypes.byref(kind)) == 0
+        if kind.value == 0:             # a kernel
+            p = Params()
+            assert cuda.cuGraphKernelNodeGetParams_v2(ctypes.c_void_p(node), ctypes.byref(p)) == 0
+            blocks.append(p.grid[0] * p.grid[1] * p.grid[2])
+    return blocks
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("R,V,k", [(1, 1000, 5), (4, 40003, 20), (9, 5001, 200), (300, 2000, 64), (700, 1000, 30)])
+def test_distill_teacher_gradient_alone(dtype, R, V, k):
+    """Without the student's gradient the teacher's is the same, and a block a
+    row does all there is to do."""
+    z, t, ids, w = make(R, V, k, dtype, 3 * R + k)
+    _, stats = K.distill_topk(z, t, ids, 2.0)
+    _, both = K.distill_topk_backward(w, z, stats, t, ids, 2.0, need_teacher=True)
+
+    def alone():
+        return K.distill_topk_backward(w, z, stats, t, ids, 2.0, need_logits=False, need_teacher=True)
+
+    none, dt = alone()
+    assert none is None
+    ref = ops.distill_topk_golden(np64(z), np64(t), np64(ids).astype(np.int64), 2.0, np64(w))
+    tol = bounds(z, t, ids, 2.0, w)
+    for got in (dt, both):
+        within(got, ref[2], tol[2] + half_step(dtype, ref[2]), "dteacher")
+    assert blocks_of(alone) == [R]
+
+
 def test_distill_second_derivative_is_refused():
     """The gradient itself is there under create_graph; to differentiate it
     again is an error, not a term that is missing."""
