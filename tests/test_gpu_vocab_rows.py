@@ -435,6 +435,74 @@ def test_distill_without_lists_or_rows():
     assert e[0].shape == (0,) and e[1].shape == (0, 50)
 
 
+def check_distill_ops(z, t, ids, w, tau, what=""):
+    """The public ops on flagos tensors: the loss, both gradients through
+    autograd for given row weights, and loss and gradient at once."""
+    zf, tf, idf, wf = (v if v.device.type == "flagos" else v.cpu().to("flagos") for v in (z, t, ids, w))
+    zf.requires_grad_(), tf.requires_grad_()
+    ref = ops.distill_topk_golden(np64(z), np64(t), np64(ids).astype(np.int64), tau, np64(w))
+    tol = bounds(z, t, ids, tau, w)
+    loss = torch_fl.ops.distill_topk(zf, tf, idf, tau)
+    within(loss, ref[0], tol[0] + half_step(torch.float32, ref[0]), what + " loss")
+    loss.backward(wf)
+    assert zf.grad.dtype == z.dtype and tf.grad.dtype == t.dtype
+    within(zf.grad, ref[1], tol[1] + half_step(z.dtype, ref[1]), what + " dlogits")
+    within(tf.grad, ref[2], tol[2] + half_step(t.dtype, ref[2]), what + " dteacher")
+    l2, dz = torch_fl.ops.distill_topk_grad(zf.detach(), tf.detach(), idf, tau, wf)
+    within(l2, ref[0], tol[0] + half_step(torch.float32, ref[0]), what + " grad's loss")
+    within(dz, ref[1], tol[1] + half_step(z.dtype, ref[1]), what + " grad's dlogits")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("R,V,k", [(3, 7, 3), (5, 513, 17), (9, 40003, 33), (4, 65536, 200), (2, 131077, 1000),
+                                   (700, 2001, 40), (3, 151936, 64)])
+def test_public_distill(dtype, R, V, k):
+    check_distill_ops(*make(R, V, k, dtype, R + 5 * V), tau=2.0, what=f"{R}x{V}x{k}")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("k", [6, 90, 300])
+def test_public_distill_special_rows(dtype, k):
+    """Masked vocabularies, sure and empty teachers, repeated and foreign tokens,
+    other list types and strides, through the public ops."""
+    V = 5003
+    z, t, ids, w = make(10, V, k, dtype, 23, t_dtype=torch.float32, ids_dtype=torch.int32)
+    low = torch.finfo(dtype).min
+    z[0, V // 3:], ids[0] = -float("inf"), torch.arange(k, device=DEV) + 2
+    z[1, V // 3:], ids[1] = low, torch.arange(k, device=DEV) + 2
+    z[2] = low
+    t[3], z[3, 5] = -float("inf"), float("nan")
+    ids[4], z[4] = -1, float("nan")
+    t[5, 1:] = -float("inf")
+    ids[6] = 17                             # one token throughout
+    ids[7] = torch.arange(k, device=DEV) % 3 * 1601 - 1
+    w[8] = 0
+    check_distill_ops(z, t, ids, w, 1.5, f"k={k}")
+    wide = torch.zeros(10, V + 40, dtype=dtype)
+    wide[:, 5:V + 5] = z.cpu()
+    lists = torch.full((10, 2 * k + 3), 9.0)
+    lists[:, 3:k + 3] = t.cpu()
+    wide, lists, one = wide.to("flagos"), lists.to("flagos"), w[:1].cpu().to("flagos")
+    check_distill_ops(wide[:, 5:V + 5], lists[:, 3:k + 3], ids, one.expand(10), 1.5, "strided")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_public_topk_and_verify(dtype):
+    """Special rows of every launch form, and both kinds of drafts, on flagos tensors."""
+    for copies, V, ks in ((1, 20011, (1, 40, 300, 1024)), (150, 3001, (1, 40, 128))):
+        x = torch.randn(5, V, generator=gen(12))
+        x[0], x[1, 9:] = 2.0, -float("inf")
+        x[2, ::3], x[3] = float("nan"), torch.arange(V) / 8
+        x = x.to(dtype).repeat(copies, 1).to("flagos")
+        for k in ks:
+            check_topk(x, k, f"k={k}", fn=torch_fl.ops.topk)
+    for with_q in (True, False):
+        ids, p, q, u, lens = (None if v is None else v.cpu().to("flagos")
+                              for v in drafts(7, 5, 9001, dtype, 14, with_q))
+        check_verify(ids, p, q, u, lens, fn=torch_fl.ops.verify_draft)
+        check_verify(ids, p, q, u, None, fn=torch_fl.ops.verify_draft)
+
+
 def test_distill_autograd_on_flagos():
     """The op's autograd against the fp64 formula, through a mean over rows
     (a broadcast gradient), for both operands and with leading dims."""
