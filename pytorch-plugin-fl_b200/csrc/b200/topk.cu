@@ -598,11 +598,17 @@ __device__ __forceinline__ uint32_t kth_lane(const uint32_t (&v)[S], int k, int 
   return __shfl_sync(0xffffffffu, m[0], k - 1);
 }
 
+// The lowest bits that tell two values' keys apart are from this one up: 16 of
+// a bf16 value's, 19 of an f16 value's (two more so that they come in pairs).
+template <typename T>
+__device__ __forceinline__ constexpr int key_bits_from() {
+  return std::is_same<T, float>::value ? 0 : std::is_same<T, __half>::value ? 12 : 16;
+}
+
 // The k-th largest of the slots' (or one that a few more reach), as in kth_maximum.
 template <typename T, int S>
 __device__ __forceinline__ uint32_t search_slots(const uint32_t (&v)[S], int k) {
-  // the lowest bits that tell two values' keys apart
-  constexpr int kLast = std::is_same<T, float>::value ? 0 : std::is_same<T, __half>::value ? 12 : 16;
+  constexpr int kLast = key_bits_from<T>();
   uint32_t lo = 0xffffffffu, hi = 0;
 #pragma unroll
   for (int i = 0; i < S; ++i) {
@@ -628,6 +634,148 @@ __device__ __forceinline__ uint32_t search_slots(const uint32_t (&v)[S], int k) 
   return least;
 }
 
+// For a row whose candidates did not fit (ties at the threshold `least`, as in
+// a masked row, or a row that rises): the elements above a value and the first
+// ones equal to it in index order, at least the k largest and at most
+// kRowSorted, into cand; their number.  By a warp, in two walks over the row
+// where fewer than k elements exceed the least of those that reach `least`, as
+// for a mask's; else in one more for two bits of the values' keys.
+template <typename T>
+__device__ __forceinline__ int row_select(const T* xr, int cols, int k, uint32_t least, uint64_t* cand,
+                                       int* filled) {
+  constexpr int VW = Elem<T>::kVec, kFrom = key_bits_from<T>();
+  const int lane = threadIdx.x & 31;
+  const RowSplit sp = split_row(xr, cols);
+  const uint4* body = reinterpret_cast<const uint4*>(xr + sp.head);
+  const int single = single_of(sp, lane, VW);
+  const uint32_t alone = single >= 0 ? value_key(Elem<T>::to_f(xr[single])) >> kFrom : 0;
+  const auto each = [&](auto see) {  // (keys, in no order)
+    if (single >= 0) see(alone);
+    for (int p = lane; p < sp.nvec; p += 64) {
+      uint4 u[2];
+      float f[VW];
+      u[0] = ld_cached(body + p);
+      if (p + 32 < sp.nvec) u[1] = ld_cached(body + p + 32);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (p + 32 * i >= sp.nvec) break;
+        unpack<T>(u[i], f);
+#pragma unroll
+        for (int j = 0; j < VW; ++j) see(value_key(f[j]) >> kFrom);
+      }
+    }
+  };
+  // the least key that reaches `least`, how many are it, how many exceed it
+  least >>= kFrom;
+  uint32_t lowest = 0xffffffffu;
+  int equal = 0, reach = 0;
+  each([&](uint32_t key) {
+    if (key < least) return;
+    ++reach;
+    if (key < lowest) equal = 0;
+    lowest = min(lowest, key);
+    equal += key == lowest;
+  });
+  uint32_t cut = __reduce_min_sync(0xffffffffu, lowest);
+  equal = __reduce_add_sync(0xffffffffu, lowest == cut ? equal : 0);
+  int above = __reduce_add_sync(0xffffffffu, reach) - equal;
+  uint32_t under = cut;  // the keys above this one are all taken
+  if (above >= k) {
+    cut = 0;
+    above = 0;
+    bool exact = true;
+    for (int bit = 30 - kFrom; bit >= 0; bit -= 2) {
+      const uint32_t one = 1u << bit;
+      int n1 = 0, n2 = 0, n3 = 0;
+      each([&](uint32_t key) {
+        n1 += key >= cut + one;
+        n2 += key >= cut + 2 * one;
+        n3 += key >= cut + 3 * one;
+      });
+      n1 = __reduce_add_sync(0xffffffffu, n1);
+      n2 = __reduce_add_sync(0xffffffffu, n2);
+      n3 = __reduce_add_sync(0xffffffffu, n3);
+      // (the fewest that are too few: those above the key in the end)
+      above = n1 < k ? n1 : n2 < k ? n2 : n3 < k ? n3 : above;
+      const int reached = n3 >= k ? n3 : n2 >= k ? n2 : n1 >= k ? n1 : 0;
+      cut += n3 >= k ? 3 * one : n2 >= k ? 2 * one : n1 >= k ? one : 0;
+      if (reached != 0 && reached <= kRowSorted) {
+        above = reached;
+        exact = false;
+        break;
+      }
+    }
+    under = exact ? cut : cut - 1;
+  }
+  const int need = max(0, k - above);
+  if (lane == 0) *filled = 0;
+  __syncwarp();
+  int taken = 0;  // of the ones equal to cut; they follow those above it
+  const auto first_ones = [&](uint32_t mine, int at) {  // this lane's, elements at + j, in lane order
+    const int count = __popc(mine);
+    int before = count;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, before, o);
+      if (lane >= o) before += x;
+    }
+    const int all = __shfl_sync(0xffffffffu, before, 31);
+    before += taken - count;
+    for (; mine != 0 && before < need; mine &= mine - 1, ++before) {
+      const int e = at + __ffs(mine) - 1;
+      cand[above + before] = element_key(Elem<T>::to_f(xr[e]), (uint32_t)e);
+    }
+    taken += all;
+  };
+  if (single >= 0 && alone > under) cand[take_slot(filled)] = element_key(Elem<T>::to_f(xr[single]), (uint32_t)single);
+  first_ones(lane < 8 && single >= 0 && alone == cut, single);
+  for (int base = 0; base < sp.nvec; base += 32) {
+    __syncwarp();
+    if (taken >= need && *(volatile int*)filled == above) break;
+    __syncwarp();
+    const int p = base + lane;
+    uint32_t mine = 0;
+    if (p < sp.nvec) {
+      float f[VW];
+      unpack<T>(ld_cached(body + p), f);
+#pragma unroll
+      for (int j = 0; j < VW; ++j) {
+        const uint32_t key = value_key(f[j]) >> kFrom;
+        mine |= (uint32_t)(key == cut) << j;
+        if (key > under) cand[take_slot(filled)] = element_key(f[j], (uint32_t)(sp.head + p * VW + j));
+      }
+    }
+    if (taken < need) first_ones(mine, sp.head + p * VW);
+  }
+  if (taken < need) first_ones(lane >= 8 && single >= 0 && alone == cut, single);
+  __syncwarp();
+  return above + need;
+}
+
+// The warp's rows that row_select is for: their first index is -1 - least.
+// (Apart from the others' loop, whose registers it would take.)
+template <typename T>
+__device__ __noinline__ void finish_late(const T* x, int64_t ld, int64_t rows, int cols, int k, T* values,
+                                         int64_t* indices, uint64_t* cand, int* filled) {
+  const int lane = threadIdx.x & 31;
+  const int64_t first = (int64_t)blockIdx.x * kRowWarps + (threadIdx.x >> 5);
+  for (int64_t row = first; row < rows; row += (int64_t)gridDim.x * kRowWarps) {
+    int64_t* ids = indices + row * k;
+    const int64_t mark = *(volatile int64_t*)ids;
+    __syncwarp();
+    if (mark >= 0) continue;
+    const T* xr = x + row * ld;
+    const int n = row_select<T>(xr, cols, k, (uint32_t)(-1 - mark), cand, filled);
+    warp_sort<kRowSorted / 32>(cand, n, lane);
+    for (int i = lane; i < k; i += 32) {
+      const uint32_t at = ~(uint32_t)cand[i];
+      ids[i] = at;
+      values[row * k + i] = xr[at];
+    }
+    __syncwarp();
+  }
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kRowWarps * 32, 32 / kRowWarps)
 topk_rows_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int cols, int k,
@@ -645,6 +793,7 @@ topk_rows_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int cols, in
     if (slot < kRowCap) cand[slot] = key;
   };
   const int64_t step = (int64_t)gridDim.x * kRowWarps;
+  bool late = false;
   for (int64_t row = (int64_t)blockIdx.x * kRowWarps + warp; row < rows; row += step) {
     const T* xr = x + row * ld;
     const RowSplit sp = split_row(xr, cols);
@@ -684,7 +833,7 @@ topk_rows_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int cols, in
     if (single >= 0) keep(element_key(alone, (uint32_t)single));
     const float bar = key_value(least);  // (NaN while everything passes, or only NaN does)
     const uint32_t depth = (sp.nvec + kChunk - 1) / kChunk, items = listed * depth;
-    for (uint32_t base = lane; base < items; base += 64) {
+    for (uint32_t base = lane; base < items && *(volatile int*)filled <= kRowCap; base += 64) {
       uint4 u[2];
       int p[2];
 #pragma unroll
@@ -713,32 +862,23 @@ topk_rows_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int cols, in
     }
     __syncwarp();
     int n = *filled;
+    if (n > kRowCap) {
+      if (lane == 0) indices[row * k] = -1 - (int64_t)least;
+      late = true;
+      __syncwarp();
+      continue;
+    }
     if (n > kRowSorted) {
-      // long ties and rows in order: a key that k to kRowSorted keys reach, two
-      // bits a walk over the list, or over the row where that did not fit
-      const bool listed_all = n <= kRowCap;
-      const auto each = [&](auto see) {
-        if (listed_all) {
-          for (int i = lane; i < n; i += 32) see(cand[i]);
-          return;
-        }
-        if (single >= 0) see(element_key(alone, (uint32_t)single));
-        for (int p = lane; p < sp.nvec; p += 32) {
-          float f[VW];
-          unpack<T>(ld_cached(body + p), f);
-#pragma unroll
-          for (int j = 0; j < VW; ++j) see(element_key(f[j], (uint32_t)(sp.head + p * VW + j)));
-        }
-      };
+      // a key that k to kRowSorted of the listed ones reach, two bits a walk
       uint64_t at = 0;
       for (int bit = 62; bit >= 0; bit -= 2) {
         const uint64_t one = (uint64_t)1 << bit;
         int n1 = 0, n2 = 0, n3 = 0;
-        each([&](uint64_t key) {
-          n1 += key >= at + one;
-          n2 += key >= at + 2 * one;
-          n3 += key >= at + 3 * one;
-        });
+        for (int i = lane; i < n; i += 32) {
+          n1 += cand[i] >= at + one;
+          n2 += cand[i] >= at + 2 * one;
+          n3 += cand[i] >= at + 3 * one;
+        }
         n1 = __reduce_add_sync(0xffffffffu, n1);
         n2 = __reduce_add_sync(0xffffffffu, n2);
         n3 = __reduce_add_sync(0xffffffffu, n3);
@@ -746,26 +886,16 @@ topk_rows_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int cols, in
         at += n3 >= k ? 3 * one : n2 >= k ? 2 * one : n1 >= k ? one : 0;
         if (reached != 0 && reached <= kRowSorted) break;
       }
-      if (listed_all) {
-        int kept = 0;
-        for (int i = 0; i < n; i += 32) {
-          const uint64_t key = i + lane < n ? cand[i + lane] : 0;
-          const uint32_t vote = __ballot_sync(0xffffffffu, key >= at && key != 0);
-          __syncwarp();
-          if (vote >> lane & 1) cand[kept + __popc(vote & ((1u << lane) - 1))] = key;
-          kept += __popc(vote);
-          __syncwarp();
-        }
-        n = kept;
-      } else {
-        if (lane == 0) *filled = 0;
+      int kept = 0;
+      for (int i = 0; i < n; i += 32) {
+        const uint64_t key = i + lane < n ? cand[i + lane] : 0;
+        const uint32_t vote = __ballot_sync(0xffffffffu, key >= at && key != 0);
         __syncwarp();
-        each([&](uint64_t key) {
-          if (key >= at) keep(key);
-        });
+        if (vote >> lane & 1) cand[kept + __popc(vote & ((1u << lane) - 1))] = key;
+        kept += __popc(vote);
         __syncwarp();
-        n = *filled;
       }
+      n = kept;
     }
     if (n <= 32) {
       warp_sort<1>(cand, n, lane);
@@ -784,6 +914,7 @@ topk_rows_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int cols, in
     }
     __syncwarp();  // the next row's candidates take these ones' place
   }
+  if (late) finish_late(x, ld, rows, cols, k, values, indices, cand, filled);
 }
 
 // Gradient: zeros, and dvalues at the indices (distinct in a row).

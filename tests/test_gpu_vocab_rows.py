@@ -112,6 +112,69 @@ def test_topk_special_rows(dtype, copies):
         check_topk(x, k, f"k={k}")
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("R,V,k", [(700, 4001, 64), (1300, 1024, 8), (640, 8150, 100), (2000, 2051, 17),
+                                   (600, 15990, 20), (5, 20011, 50), (300, 40003, 64), (64, 128256, 200),
+                                   (700, 9001, 400), (2, 300000, 1000), (4, 32000, 8)])
+def test_topk_masked_rows(dtype, R, V, k):
+    """Fewer live tokens than k, as many, a few more; ties below, between and
+    above them, in the single elements at either end too; rows that rise."""
+    g = gen(R + V)
+    x = torch.randn(R, V + 7, generator=g)[:, 3:V + 3]
+    mask = torch.full((R, V), -float("inf"))
+    mask[1::4] = torch.finfo(dtype).min
+    mask[2::4] = -0.5                                   # ties with live tokens on both sides
+    live = torch.zeros(R, V, dtype=torch.bool)
+    for r in range(R):
+        n = (0, 1, k - 1, k, k + 1, k // 2, 3 * k)[r % 7]
+        live[r, torch.randperm(V, generator=g)[:min(n, V)]] = True
+    x = torch.where(live, x, mask)
+    x[R // 2, V // 2] = float("nan")
+    x[R // 3, -1] = float("inf")
+    x[R - 1] = torch.arange(V) // 3                     # a rise, in threes
+    if R > 8:
+        x[4] = torch.where(torch.arange(V) % 2 == 0, 0.0, -0.0)
+        x[5, V - 5:] = -float("inf")                    # the tail among the ties
+        x[6, :V // 2] = 1.5                             # more ties than k, nothing above
+        x[7] = -torch.arange(V).float()
+    wide = torch.zeros(R, V + 7, dtype=dtype, device=DEV)
+    wide[:, 3:V + 3] = x.to(dtype).to(DEV)
+    check_topk(wide[:, 3:V + 3], k)
+    check_topk(wide[:, 3:V + 3].contiguous(), k)
+
+
+def replay_us(call, n=5):
+    """Device time of a call, from replays of a graph of n of them."""
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for _ in range(n):
+            call()
+    best = float("inf")
+    for _ in range(5):
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        graph.replay()
+        a.record()
+        graph.replay()
+        b.record()
+        torch.cuda.synchronize()
+        best = min(best, a.elapsed_time(b) * 1e3 / n)
+    return best
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("R,V,k", [(8192, 4096, 64), (1500, 7000, 20)])
+def test_topk_masked_rows_take_no_multiple_of_ten(dtype, R, V, k):
+    """Masked rows are walked a fixed number of times more, not once for each
+    bit of a key: within 6 times the time of rows without ties (2 to 4 on an
+    idle GPU; up to 37 when each bit took a walk)."""
+    x = torch.randn(R, V, device=DEV).to(dtype)
+    masked = x.masked_fill(torch.rand(R, V, device=DEV) * V > k // 3, -float("inf"))
+    plain, tied = (replay_us(lambda: K.topk_lastdim(v, k)) for v in (x, masked))
+    assert tied < 6 * plain, (plain, tied)
+
+
 def test_topk_rows_that_rise_late():
     """Rows in ascending blocks: whatever a scan has kept is beaten later."""
     V = 65536
