@@ -82,7 +82,7 @@ struct Shared {
   int2 sums[2][kWarps];
   uint32_t run[B];  // the threads' maxima
   int hist[256];
-  uint32_t least;
+  uint32_t least;  // collect's threshold
   int filled, listed, pick, above;
   uint4 stage[kPacks][B];  // packs on their way, each thread its own
 };
@@ -246,64 +246,138 @@ __device__ __noinline__ void sort_desc(Shared<B>& s, int n) {
   }
 }
 
-// The k largest keys of elements [lo, hi) in four passes (five in f16, six in
-// float32) that any values take: a histogram of the values' keys 8 bits at a time
-// down to the k-th largest value, the elements above it, and the first ones
-// equal to it in index order.  For slices whose candidates overflow: long
-// ties (a masked row, say) and rows that rise steeply.
+// The k largest keys of elements [lo, hi), at least k of which reach s.least,
+// whatever they are: for slices whose candidates overflow.  Where fewer than k
+// exceed the least of those (long ties, as in a masked row), one pass finds it
+// and one more the elements above it, and the first ones equal to it follow in
+// index order; else (rows that rise steeply) a histogram of the values' keys 8
+// bits at a time finds the k-th largest value first, in two to four passes.
 template <typename T, int B>
 __device__ __noinline__ void select_any(Shared<B>& s, const T* xr, int lo, int hi, int k) {
   // the upper bits that tell two values' keys apart: 16 of a bf16 value's, 19
   // of an f16 value's (5 + 10 bits and the sign, with fp32's 8 bits of exponent)
   constexpr int kBits = std::is_same<T, float>::value ? 32 : std::is_same<T, __half>::value ? 24 : 16;
-  const int tid = threadIdx.x, lane = tid & 31;
-  const int rounds = (hi - lo + B - 1) / B;
-  uint32_t value = 0;
-  int need = k;
-  for (int shift = kBits - 8; shift >= 0; shift -= 8) {
-    for (int i = tid; i < 256; i += B) s.hist[i] = 0;
-    __syncthreads();
-    for (int r = 0; r < rounds; ++r) {
-      const int i = lo + r * B + tid;
-      const uint32_t key = i < hi ? value_key(Elem<T>::to_f(xr[i])) >> (32 - kBits) : 0;
-      const bool in = i < hi && (uint64_t)key >> (shift + 8) == (uint64_t)value >> (shift + 8);
-      const uint32_t digit = in ? (key >> shift) & 255 : 256;
-      const uint32_t same = __match_any_sync(0xffffffffu, digit);
-      if (in && __ffs(same) - 1 == lane) atomicAdd(&s.hist[digit], __popc(same));
+  constexpr int VW = Elem<T>::kVec, kWarps = B / 32, U = 2;  // (with 4 the callers' registers spill)
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const RowSplit sp = split_row(xr + lo, hi - lo);
+  const uint4* body = reinterpret_cast<const uint4*>(xr + lo + sp.head);
+  const int single = single_of(sp, tid, VW);
+  const uint32_t alone = single >= 0 ? value_key(Elem<T>::to_f(xr[lo + single])) >> (32 - kBits) : 0;
+  const auto each = [&](auto see) {  // (keys and elements, in no order)
+    if (single >= 0) see(alone, single);
+    for (int p = tid; p < sp.nvec; p += U * B) {
+      uint4 u[U];
+#pragma unroll
+      for (int i = 0; i < U; ++i)
+        if (p + i * B < sp.nvec) u[i] = ld_cached(body + p + i * B);
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        if (p + i * B >= sp.nvec) break;
+        float f[VW];
+        unpack<T>(u[i], f);
+#pragma unroll
+        for (int j = 0; j < VW; ++j)
+          see(value_key(f[j]) >> (32 - kBits), sp.head + (p + i * B) * VW + j);
+      }
     }
-    __syncthreads();
-    if (tid == 0) {
-      int sum = 0, d = 255;
-      while (d > 0 && sum + s.hist[d] < need) sum += s.hist[d--];
-      s.pick = d;
-      s.above = sum;
-      s.filled = 0;
+  };
+  uint32_t value = 0xffffffffu;
+  int above = 0, need = k;
+  {
+    const uint32_t least = s.least >> (32 - kBits);
+    int equal = 0, reach = 0;
+    each([&](uint32_t key, int) {
+      if (key < least) return;
+      ++reach;
+      if (key < value) equal = 0;
+      value = min(value, key);
+      equal += key == value;
+    });
+    const uint32_t mine = value;
+    value = __reduce_min_sync(0xffffffffu, value);
+    equal = __reduce_add_sync(0xffffffffu, mine == value ? equal : 0);
+    reach = __reduce_add_sync(0xffffffffu, reach);
+    if (lane == 0) {
+      s.sums[0][warp] = make_int2((int)value, equal);
+      s.sums[1][warp].x = reach;
     }
+    if (tid == 0) s.filled = 0;
     __syncthreads();
-    value |= (uint32_t)s.pick << shift;
-    need -= s.above;
+    for (int w = 0; w < kWarps; ++w) value = min(value, (uint32_t)s.sums[0][w].x);
+    for (int w = 0; w < kWarps; ++w)
+      above += s.sums[1][w].x - ((uint32_t)s.sums[0][w].x == value ? s.sums[0][w].y : 0);
+    __syncthreads();
   }
-  for (int i = lo + tid; i < hi; i += B) {
-    const float f = Elem<T>::to_f(xr[i]);
-    if (value_key(f) >> (32 - kBits) > value) append(s, element_key(f, (uint32_t)i));
+  if (above < k) {
+    need = k - above;
+  } else {
+    const int rounds = (hi - lo + B - 1) / B;
+    value = 0;
+    for (int shift = kBits - 8; shift >= 0; shift -= 8) {
+      for (int i = tid; i < 256; i += B) s.hist[i] = 0;
+      __syncthreads();
+      for (int r = 0; r < rounds; ++r) {
+        const int i = lo + r * B + tid;
+        const uint32_t key = i < hi ? value_key(Elem<T>::to_f(xr[i])) >> (32 - kBits) : 0;
+        const bool in = i < hi && (uint64_t)key >> (shift + 8) == (uint64_t)value >> (shift + 8);
+        const uint32_t digit = in ? (key >> shift) & 255 : 256;
+        const uint32_t same = __match_any_sync(0xffffffffu, digit);
+        if (in && __ffs(same) - 1 == lane) atomicAdd(&s.hist[digit], __popc(same));
+      }
+      __syncthreads();
+      if (tid == 0) {
+        int sum = 0, d = 255;
+        while (d > 0 && sum + s.hist[d] < need) sum += s.hist[d--];
+        s.pick = d;
+        s.above = sum;
+      }
+      __syncthreads();
+      value |= (uint32_t)s.pick << shift;
+      need -= s.above;
+    }
   }
+  if (need < k) {
+    each([&](uint32_t key, int at) {
+      if (key > value) append(s, element_key(Elem<T>::to_f(xr[lo + at]), (uint32_t)(lo + at)));
+    });
+  }
+  // the first ones equal to it, in the order of threads: elements at + j
   int parity = 0, taken = 0;
-  for (int r = 0; r < rounds && taken < need; ++r) {
-    const int i = lo + r * B + tid;
-    const float f = i < hi ? Elem<T>::to_f(xr[i]) : 0.f;
-    const bool is = i < hi && value_key(f) >> (32 - kBits) == value;
-    const uint32_t vote = __ballot_sync(0xffffffffu, is);
-    if (lane == 0) s.sums[parity][tid >> 5].x = __popc(vote);
+  const auto first_ones = [&](uint32_t mine, int at) {
+    const int count = __popc(mine);
+    int before = count;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, before, o);
+      if (lane >= o) before += x;
+    }
+    if (lane == 31) s.sums[parity][warp].x = before;
     __syncthreads();
-    int before = taken, total = 0;
-    for (int w = 0; w < B / 32; ++w) {
-      if (w < tid >> 5) before += s.sums[parity][w].x;
-      total += s.sums[parity][w].x;
+    before += taken - count;
+    int all = 0;
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) before += s.sums[parity][w].x;
+      all += s.sums[parity][w].x;
     }
     parity ^= 1;
-    if (is && before + __popc(vote & ((1u << lane) - 1)) < need) append(s, element_key(f, (uint32_t)i));
-    taken += total;
+    for (; mine != 0 && before < need; mine &= mine - 1, ++before) {
+      const int e = lo + at + __ffs(mine) - 1;
+      append(s, element_key(Elem<T>::to_f(xr[e]), (uint32_t)e));
+    }
+    taken += all;
+  };
+  first_ones(tid < 8 && single >= 0 && alone == value, single);
+  for (int base = 0; base < sp.nvec && taken < need; base += B) {
+    uint32_t mine = 0;
+    if (base + tid < sp.nvec) {
+      float f[VW];
+      unpack<T>(ld_cached(body + base + tid), f);
+#pragma unroll
+      for (int j = 0; j < VW; ++j) mine |= (uint32_t)(value_key(f[j]) >> (32 - kBits) == value) << j;
+    }
+    first_ones(mine, sp.head + (base + tid) * VW);
   }
+  if (taken < need) first_ones(tid >= 8 && single >= 0 && alone == value, single);
   __syncthreads();
 }
 
@@ -426,6 +500,7 @@ __device__ __forceinline__ int collect(Shared<B>& s, const T* xr, int lo, int hi
 #pragma unroll
       for (int i = 0; i < kPacks; ++i) see(group[i]);
     });
+    if (tid == 0) s.least = least;
   }
   if (single >= 0) append(s, element_key(alone, (uint32_t)(lo + single)));
 #pragma unroll
@@ -443,9 +518,11 @@ __device__ __forceinline__ int collect(Shared<B>& s, const T* xr, int lo, int hi
     for (int i = 0; i < VW; ++i)
       if (value_key(f[i]) >= least) append(s, element_key(f[i], (uint32_t)(lo + sp.head + p * VW + i)));
   };
+  // (a tie of all the row is not counted to the end, one atomic an element)
+  const auto more_fit = [&] { return *(volatile int*)&s.filled <= kCap; };
   if (depth == 1 && next.nvec == 0) {
     // the stage still holds them
-    for (int j = tid; j < items; j += B) {
+    for (int j = tid; j < items && more_fit(); j += B) {
       const int p = s.list[j];
       look(s.stage[p / B][p % B], p);
     }
@@ -453,7 +530,7 @@ __device__ __forceinline__ int collect(Shared<B>& s, const T* xr, int lo, int hi
     // two packs a thread in flight; n / depth by a multiplication where that is
     // exact (n < 4096 depth, off by less than n depth / 2^32 of a step)
     const uint32_t over = depth < 1024 ? (uint32_t)((0x100000000ull + depth - 1) / depth) : 0;
-    for (int j = tid; j < items; j += 2 * B) {
+    for (int j = tid; j < items && more_fit(); j += 2 * B) {
       int p[2];
       uint4 u[2];
 #pragma unroll
