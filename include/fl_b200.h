@@ -426,7 +426,8 @@ FL_B200_API int fl_b200_topk_lastdim(const void* x, int64_t ld, int64_t rows, in
                                      int64_t k, void* values, int64_t* indices, int dtype,
                                      fl_b200_stream_t stream);
 /* Its gradient: dx (dense [rows, cols]) = 0 but dvalues at the indices       *
- * (both dense [rows, k]; an index outside the row is left out).             */
+ * (both dense [rows, k]; a row's indices differ, as topk's do, and one       *
+ * outside the row is left out).                                             */
 FL_B200_API int fl_b200_topk_bwd(const void* dvalues, const int64_t* indices, void* dx, int64_t rows,
                                  int64_t cols, int64_t k, int dtype, fl_b200_stream_t stream);
 
@@ -466,7 +467,10 @@ FL_B200_API int fl_b200_distill_topk_bwd(const float* dloss, int64_t dloss_strid
  * (row_weight takes dloss's place).  stats as in the forward.  The logits   *
  * are read once and dlogits written once when the rows' offsets agree as    *
  * above, a row has at most 262144 elements of 16 bits or 131072 of 32, and  *
- * k <= 128; otherwise the forward and the backward run one after the other. *
+ * k <= 128 (many rows of up to 6 KB with k <= 64 are read a second time,     *
+ * from cache); otherwise the forward and the backward run one after the      *
+ * other, with sums in another order: the two ways agree to the rounding of  *
+ * fp32 sums, not bit for bit.                                               *
  * On the first way a cluster's waits have a limit (fl_b200_set_wait_limit). */
 FL_B200_API int fl_b200_distill_topk_grad(const void* logits, int64_t ld, const void* teacher,
                                           int64_t ld_t, int t_dtype, const void* ids,

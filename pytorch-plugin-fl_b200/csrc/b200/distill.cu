@@ -541,9 +541,10 @@ struct ListOf<T, 0> {
 // Loss and statistics: one read of the logits, with the running maximum and
 // sum of a softmax in each thread.  One CTA a row, or a cluster of CTAs with a
 // slice of packs each when there are few rows; a further warp reads the list
-// meanwhile.  Bound by HBM: 8192 x 128256 bf16 in 301 us (7.0 TB/s, above the
-// 6.5 TB/s that a copy reaches, as nothing is written); 32 x 32000 fp32 takes
-// 3.5 us, its launch and three trips to memory.
+// meanwhile.  Bound by HBM: 8192 x 128256 bf16 in 302 us replayed from a graph
+// (7.0 TB/s, above the 6.5 TB/s that a copy reaches, as nothing is written) and
+// 330 to 360 us called again and again (5.8 to 6.4 TB/s); 32 x 32000 fp32 takes
+// 3.5 to 4.3 us, its launch and three trips to memory.
 template <typename T, int NS, int E>
 __global__ void __launch_bounds__(NS + 32, 1024 / NS)
 distill_fwd_kernel(const T* __restrict__ x, int64_t ld, Taught a, int cols,
@@ -616,8 +617,8 @@ distill_fwd_kernel(const T* __restrict__ x, int64_t ld, Taught a, int cols,
 // Gradients of both operands from the forward's statistics: q w tau streamed
 // over a chunk of the row, then the tokens of the teacher's list that lie in
 // it written again, whole, from fp32 (so that each element is rounded once).
-// Bound by HBM: 2048 x 128256 bf16 in 165 us (6.4 TB/s, 97% of the measured
-// copy rate), 203 us with 256 teacher logits.
+// Bound by HBM: 2048 x 128256 bf16 in 165 to 169 us (6.2 to 6.4 TB/s, 95 to
+// 97% of the measured copy rate), 203 to 211 us with 256 teacher logits.
 template <typename T, bool VEC, int NS, int E>
 __global__ void __launch_bounds__(NS + 32, 1024 / NS)
 distill_bwd_kernel(const float* __restrict__ dloss, int64_t dloss_stride, const T* __restrict__ x,
@@ -833,8 +834,9 @@ distill_rows_kernel(const T* __restrict__ x, int64_t ld, Taught a, const float* 
 // than the holders over a row).
 //
 // Measured (of the 6.5 TB/s that a copy reaches): 2048 x 128256 bf16 with 64
-// teacher logits 181 us (89%), 1024 x 128256 fp32 169 us (95%), 32768 x 8192
-// bf16 170 us (97%).  What is left for 16-bit types at long rows is the chain
+// teacher logits 182 us (89%), 1024 x 128256 fp32 178 us (91%), 32768 x 8192
+// bf16 172 us (96%).  (1 to 2% of the first two are the checks of given-up
+// waits.)  What is left for 16-bit types at long rows is the chain
 // of a row: wait, exponentials, exchange, scale, with two CTAs an SM to overlap.
 constexpr int kPacks = 8;            // 16-byte packs a thread holds
 constexpr int kStages = 3;

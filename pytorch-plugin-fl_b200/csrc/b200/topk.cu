@@ -146,7 +146,7 @@ __device__ __forceinline__ void append(Shared<B>& s, uint64_t key) {
 }
 
 // Descending bitonic sort, N neighbours a thread, t its place.  Partners in
-// two lanes meet by shuffles, those in two warps through shared memory (six
+// two lanes meet by shuffles, those in two warps through shared memory (ten
 // barriers for eight warps; with one a step, after a search for the cut, 64 x
 // 32000 float32, top 1000, took 44 us, now 30).  Above 128 keys it beats
 // counting (1 x 5289 float32, top 120: 9.0 us, 11.8), below it does not (4096 x
@@ -252,6 +252,8 @@ __device__ __noinline__ void sort_desc(Shared<B>& s, int n) {
 // and one more the elements above it, and the first ones equal to it follow in
 // index order; else (rows that rise steeply) a histogram of the values' keys 8
 // bits at a time finds the k-th largest value first, in two to four passes.
+// 4096 x 128256 bf16, top 64, masked but for 20: 916 us (4.8 ms with the
+// histograms for these too); 64 rows 30 us (145).
 template <typename T, int B>
 __device__ __noinline__ void select_any(Shared<B>& s, const T* xr, int lo, int hi, int k) {
   // the upper bits that tell two values' keys apart: 16 of a bf16 value's, 19
@@ -649,10 +651,10 @@ constexpr int kBlock = 512;
 
 // The same with a warp a row, for many short rows: the CTA's barriers, one
 // after the other, took most of a short row's time (20000 x 1024 bf16, top 8,
-// 411 us against 37; 8192 x 4096, top 64, 192 against 54).  The warp's 256
+// 411 us against 39; 8192 x 4096, top 64, 192 against 55).  The warp's 256
 // slots are the groups; threshold, second look and order run on shuffles and a
 // list in shared memory.  Bound by the instructions of these steps: a third
-// of the copy rate at 1500 x 12000 bf16, top 20 (16.6 us), a fifth at 8192 x
+// of the copy rate at 1500 x 12000 bf16, top 20 (17 us), a fifth at 8192 x
 // 4096, top 64.
 constexpr int kRowWarps = 4;
 constexpr int kRowCap = 512;     // candidates listed
@@ -716,7 +718,8 @@ __device__ __forceinline__ uint32_t search_slots(const uint32_t (&v)[S], int k) 
 // ones equal to it in index order, at least the k largest and at most
 // kRowSorted, into cand; their number.  By a warp, in two walks over the row
 // where fewer than k elements exceed the least of those that reach `least`, as
-// for a mask's; else in one more for two bits of the values' keys.
+// for a mask's; else in one more for two bits of the values' keys.  8192 x 4096
+// bf16, top 64, masked but for 20: 128 us (1068 by two bits of a 64-bit key).
 template <typename T>
 __device__ __forceinline__ int row_select(const T* xr, int cols, int k, uint32_t least, uint64_t* cand,
                                        int* filled) {

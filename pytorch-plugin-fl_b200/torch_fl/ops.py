@@ -99,8 +99,8 @@ def distill_topk(logits, teacher_logits, teacher_ids, temperature: float = 1.0):
     gradients whatever its logits hold.  Repeated ids add.  Differentiable once
     in logits and in teacher_logits (a second derivative raises, and so do
     forward mode and torch.func's transforms of gradients); the gradient is computed from the saved
-    logits, so they are read three times in all: `distill_topk_grad` reads
-    them once."""
+    logits, which the forward and the backward read once each;
+    `distill_topk_grad` reads them once for both."""
     return torch.ops.flagos.distill_topk(logits, teacher_logits, teacher_ids, float(temperature))[0]
 
 
