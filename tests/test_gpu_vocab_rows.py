@@ -375,7 +375,7 @@ def test_distill_gradient_between_the_logits_rows():
     loss, dz = K.distill_topk_grad(both[:, :2048], t, ids, 2.0, w, out=both[:, 2048:])
     assert torch.equal(loss, want[0]) and torch.equal(dz, want[1]) and torch.equal(both[:, :2048], z)
     wide = torch.zeros(7, 2048, dtype=torch.bfloat16, device=DEV)
-    for out in (z, both[:, 1024:3072], both[:, 2047:4095]):
+    for out in (z, both[:, 1000:3048], both[:, 2047:4095]):
         logits = z if out is z else both[:, :2048]
         with pytest.raises(_abi.FlB200Error, match="invalid argument"):
             K.distill_topk_grad(logits, t, ids, 2.0, w, out=out)
