@@ -503,6 +503,100 @@ FL_B200_API int fl_b200_verify_draft(const int64_t* draft_ids, int64_t ld_ids, c
                                      int64_t drafts, int64_t vocab, int64_t* tokens,
                                      int64_t* accepted, int dtype, fl_b200_stream_t stream);
 
+/* ------------------------------------------------------------------------ *
+ * A training step around the matrix products, in the forms newer decoders   *
+ * give it.  The reference has none of these (its HF path would run them op   *
+ * by op).                                                                   *
+ *                                                                           *
+ * Rotary positions without a table.  angle = position * inv_freq[i] for      *
+ * i < rot / 2, and                                                          *
+ *   (a, b) -> scale * (a cos - b sin, b cos + a sin)                        *
+ * with (a, b) = (x[i], x[i + rot / 2]) or, interleaved, (x[2i], x[2i + 1]);  *
+ * elements from rot on are copied.  inverse != 0 turns by -angle: with the   *
+ * same scale that is the gradient.  q and k are addressed as in              *
+ * fl_b200_rope_qk (k may be NULL, and either may have no heads), positions   *
+ * (I32/I64) as positions[b * spb + s * sps].  inv_freq is F32 [rot / 2], rot  *
+ * even, at most head_dim and FL_B200_ROTARY_MAX.  The angle is exact to      *
+ * fp64, its cosine fp32, the result rounded once.  Any alignment.  In place   *
+ * (an output with its input's address and strides) allowed, and then only   *
+ * the turned part is touched; otherwise outputs share no memory with their   *
+ * inputs.                                                                   */
+#define FL_B200_ROTARY_MAX 2048
+FL_B200_API int fl_b200_rotary(
+    const void* q, void* q_out, int64_t Hq, int64_t sqb, int64_t sqh, int64_t sqs, int64_t soqb, int64_t soqh,
+    int64_t soqs, const void* k, void* k_out, int64_t Hk, int64_t skb, int64_t skh, int64_t sks, int64_t sokb,
+    int64_t sokh, int64_t soks, const void* positions, int64_t spb, int64_t sps, int pos_dtype,
+    const float* inv_freq, int64_t rot, float scale, int interleaved, int inverse, int64_t B, int64_t S,
+    int64_t D, int dtype, fl_b200_stream_t stream);
+
+/* The norm after a block, its gate and scale, the residual add and the norm  *
+ * before the next block:                                                    *
+ *   h = residual + scale * gate * (offset + post) * x / rms(x),             *
+ *   y = (offset + pre) * h / rms(h),   rms(v) = sqrt(mean(v^2) + eps).       *
+ * x (stride ld_x), residual (ld_r), post, pre [cols] and gate share `dtype`; *
+ * y and h are dense and share no memory with an operand.  gate: dense rows,  *
+ * one for every rows_per_gate rows (rows or more: one for all); NULL: 1.     *
+ * y is the norm of h before its rounding.  Any alignment.                   */
+FL_B200_API int fl_b200_sandwich_norm(const void* x, int64_t ld_x, const void* residual, int64_t ld_r,
+                                      const void* post, const void* pre, const void* gate,
+                                      int64_t rows_per_gate, void* y, void* h, int64_t rows, int64_t cols,
+                                      float eps, float scale, float weight_offset, int dtype,
+                                      fl_b200_stream_t stream);
+/* Its gradients from dy, dh (NULL: none), x and the h that was stored: dx,    *
+ * dresidual (dense rows), dpost, dpre [cols] and dgate (the gate's shape;     *
+ * NULL without one).  Column sums have one order, so results repeat bit for   *
+ * bit on one GPU.  The workspace (16-byte aligned) holds the rows' statistics *
+ * and the sums' parts; its size depends on the current device's SM count.    */
+FL_B200_API size_t fl_b200_sandwich_norm_bwd_workspace_size(int64_t rows, int64_t cols);
+FL_B200_API int fl_b200_sandwich_norm_bwd(const void* dy, int64_t ld_dy, const void* dh, int64_t ld_dh,
+                                          const void* x, int64_t ld_x, const void* h, int64_t ld_h,
+                                          const void* post, const void* pre, const void* gate,
+                                          int64_t rows_per_gate, void* dx, void* dresidual, void* dpost,
+                                          void* dpre, void* dgate, int64_t rows, int64_t cols, float eps,
+                                          float scale, float weight_offset, int dtype, void* workspace,
+                                          size_t workspace_bytes, fl_b200_stream_t stream);
+
+/* Softmax of attention scores over each query's span of keys.  Row           *
+ * (b * heads + h) * q_len + q of x (stride ld_x) sees keys lo <= j < hi, the  *
+ * int32 pair at spans[b * span_sb + q * span_sq] (clamped to [0, cols]):     *
+ *   z = scale * x;  cap > 0: z = cap * tanh(z / cap);                        *
+ *   slopes != NULL: z -= slopes[h] * |p - j|,                               *
+ *   out = exp(z) / sum over the span of exp(z), 0 outside it,               *
+ * p = positions[b * pos_sb + q * pos_sq] (int32; NULL: q + cols - q_len).     *
+ * A row that sees nothing is 0.  Keys outside a span are never used, whatever *
+ * they hold; inside it softmax's rules hold (NaN, +inf or nothing but -inf    *
+ * give NaN).  out: in_dtype or F32, no memory shared with x.  Any alignment.  */
+FL_B200_API int fl_b200_span_softmax(const void* x, int64_t ld_x, const int32_t* spans, int64_t span_sb,
+                                     int64_t span_sq, const int32_t* positions, int64_t pos_sb, int64_t pos_sq,
+                                     const float* slopes, void* out, int64_t ld_out, int64_t rows, int64_t cols,
+                                     int64_t heads, int64_t q_len, float scale, float cap, int in_dtype,
+                                     int out_dtype, fl_b200_stream_t stream);
+/* Its gradient: dx = scale * (1 - tanh(scale * x / cap)^2) * y * (dy - sum of  *
+ * y dy over the span), 0 outside it.  dy and y share y_dtype; x_dtype is x's   *
+ * and dx's, and y_dtype x_dtype or F32.  x is read where cap > 0 only.         */
+FL_B200_API int fl_b200_span_softmax_bwd(const void* dy, int64_t ld_dy, const void* y, int64_t ld_y,
+                                         const void* x, int64_t ld_x, const int32_t* spans, int64_t span_sb,
+                                         int64_t span_sq, void* dx, int64_t ld_dx, int64_t rows, int64_t cols,
+                                         int64_t heads, int64_t q_len, float scale, float cap, int y_dtype,
+                                         int x_dtype, fl_b200_stream_t stream);
+
+/* The norm of `count` dense tensors (host arrays of addresses, element counts  *
+ * and dtypes, F32/BF16/F16 and mixed as they come) taken as one vector:       *
+ * sqrt(sum x^2), or max |x| with max_kind != 0; norm is one F32 on the device, *
+ * 0 for no tensors.  Squares that fp32 cannot hold are added in fp64.         */
+FL_B200_API size_t fl_b200_grad_norm_workspace_size(int64_t count);
+FL_B200_API int fl_b200_grad_norm(const void* const* tensors, const int64_t* numels, const int* dtypes,
+                                  int64_t count, int max_kind, float* norm, void* workspace,
+                                  size_t workspace_bytes, fl_b200_stream_t stream);
+/* The same, and outs[i] = tensors[i] * min(1, max_norm / (norm + 1e-6)), in    *
+ * fp32 with one rounding; a norm that is not finite makes a factor of NaN or   *
+ * 0 as the formula does.  Each output is its tensor itself or shares no memory *
+ * with it; fastest where both have the same offset from a 16-byte boundary.    *
+ * max_norm >= 0.                                                             */
+FL_B200_API int fl_b200_clip_grads(const void* const* tensors, void* const* outs, const int64_t* numels,
+                                   const int* dtypes, int64_t count, float max_norm, int max_kind, float* norm,
+                                   void* workspace, size_t workspace_bytes, fl_b200_stream_t stream);
+
 #ifdef __cplusplus
 } /* extern "C" */
 #endif

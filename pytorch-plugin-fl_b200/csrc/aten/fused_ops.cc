@@ -6,7 +6,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
-#include "tensor_utils.h"
+#include "fused_common.h"
 
 namespace flb200::aten {
 namespace {
@@ -15,27 +15,6 @@ int Rounding(c10::string_view r) {
   if (r == "fused") return FL_B200_ROUND_FUSED;
   if (r == "chain") return FL_B200_ROUND_CHAIN;
   TORCH_CHECK(false, "flagos: rounding must be 'fused' or 'chain', got '", std::string(r), "'");
-}
-
-int FloatCode(const at::Tensor& t, const char* op) {
-  const int c = B200Dtype(t.scalar_type());
-  TORCH_CHECK(c == FL_B200_F32 || c == FL_B200_BF16 || c == FL_B200_F16, op,
-              ": float32, bfloat16 or float16 expected, got ", t.scalar_type());
-  return c;
-}
-
-void SameDevice(const at::Tensor& a, const at::Tensor& b, const char* op) {
-  TORCH_CHECK(a.device() == b.device(), op, ": tensors on ", a.device(), " and ", b.device());
-}
-
-RowsView Rows(const at::Tensor& x, at::Tensor& keep) {
-  auto r = AsRows(x);
-  if (r) {
-    keep = x;
-    return *r;
-  }
-  keep = x.contiguous();
-  return *AsRows(keep);
 }
 
 // ---------------------------------------------------------------- RMSNorm --
@@ -554,15 +533,6 @@ std::tuple<at::Tensor, at::Tensor> VerifyDraft(const at::Tensor& draft_ids, cons
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
-template <typename Fn>
-const c10::TypedOperatorHandle<Fn>& Below(const char* name) {
-  static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Fn>();
-  return op;
-}
-// There is no forward-mode formula: a tangent would be dropped unseen.
-void NoTangent(const at::Tensor& t, const char* op) {
-  TORCH_CHECK(!t._fw_grad(/*level=*/0).defined(), op, ": forward-mode derivatives are not there");
-}
 using TopkFn = std::tuple<at::Tensor, at::Tensor>(const at::Tensor&, int64_t);
 using TopkBackwardFn = at::Tensor(const at::Tensor&, const at::Tensor&, int64_t);
 using DistillFn = std::tuple<at::Tensor, at::Tensor>(const at::Tensor&, const at::Tensor&,

@@ -1,0 +1,301 @@
+// Rotary positions from positions and frequencies: no table of cosines in
+// memory, halves or neighbours paired, the whole head or its first part.
+//
+//   angle = position * freq[i],  i < rot / 2
+//   (a, b) -> scale * (a cos - b sin, b cos + a sin)
+//
+// with (a, b) = (x[i], x[i + rot/2]) or (x[2i], x[2i+1]); the elements from
+// rot on stay as they are.  The inverse turns by -angle and is the adjoint:
+// with the same scale it is the gradient.
+//
+// The angle is taken in fp64 as a fraction of a turn, reduced to half a turn
+// there (exact), and only then rounded to fp32 for sincospif: a position of
+// 1e6 costs no digit of its cosine (fp32 angles lose 2^-4 of a radian
+// there).  The cosines stay fp32 and are scaled once; the rotation is fp32 with one rounding to the
+// heads' type.
+//
+// Bound by memory: every head is read and written once.  A warp takes a token
+// (or a part of its heads, for few tokens), its lanes compute the token's
+// cosines into shared memory (rot / 64 sincospif a lane, while the first
+// packs are on their way) and walk the (head, pack) items; all heads share
+// them.  The table's 16-byte chunks of neighbouring packs are neighbours, so
+// reading it has no bank conflicts.
+#include <numeric>
+
+#include "common.cuh"
+
+namespace flb200 {
+namespace {
+
+struct RotaryArgs {
+  const char* in[2];  // q, k
+  char* out[2];
+  int64_t sb[2], sh[2], ss[2], ob[2], oh[2], os[2];  // bytes
+  const void* pos;
+  int64_t pb, ps;  // elements
+  const float* freq;
+  float scale, sign;
+  int pos64, q_heads, heads, rot, splits;
+  uint32_t tokens, seq;
+  int items, copies;        // packs a head that turn (pairs of them where halves are paired) / stay
+  uint32_t items_m, copies_m;  // ceil(2^31 / items), ...
+  int copy_from, copy_to;   // item range of the packs that are copied
+  int split_b;              // bytes from a pack to its partner
+};
+
+// n / d from m = ceil(2^31 / d), exact while n * d < 2^31.
+__device__ __forceinline__ int quotient(int n, uint32_t m) { return (int)(((uint64_t)(uint32_t)n * m) >> 31); }
+
+template <int BYTES>
+struct RawOf;
+template <>
+struct RawOf<16> { using type = uint4; };
+template <>
+struct RawOf<8> { using type = uint2; };
+template <>
+struct RawOf<4> { using type = unsigned int; };
+template <>
+struct RawOf<2> { using type = unsigned short; };
+
+template <typename T, int VEC>
+struct Pack {
+  using Raw = typename RawOf<VEC * (int)sizeof(T)>::type;
+  union {
+    Raw raw;
+    T e[VEC];
+  };
+  __device__ __forceinline__ Pack() {}
+};
+
+// One chunk of the table: CH of an item's cosines and sines.
+template <int CH>
+struct alignas(CH * 4) Chunk {
+  float v[CH];
+};
+
+// VEC elements a pack.  An item is a pack and its partner half a turn part
+// away, or (NEIGH) one pack of neighbours; single elements are loaded as
+// pairs in both cases.
+template <typename T, int VEC, bool NEIGH>
+__global__ void __launch_bounds__(128)
+rotary_kernel(const __grid_constant__ RotaryArgs a) {
+  pdl_prologue();
+  constexpr bool PAIR = !NEIGH || VEC == 1;  // an item is two loads
+  constexpr int NE = PAIR ? VEC : VEC / 2;   // angles an item
+  constexpr int CH = 2 * NE < 4 ? 2 * NE : 4;
+  constexpr int NCH = 2 * NE / CH;
+  constexpr int U = PAIR ? 4 : 8;  // items in flight
+  constexpr int kSize = (int)sizeof(T);
+  extern __shared__ float4 smem4[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  float* table = reinterpret_cast<float*>(smem4) + warp * ((a.rot + 3) & ~3);
+  const uint32_t unit = blockIdx.x * 4u + warp;
+  const uint32_t token = unit / (uint32_t)a.splits;
+  if (token >= a.tokens) return;
+  const int part = (int)(unit - token * (uint32_t)a.splits);
+  const uint32_t b = token / a.seq, s = token - b * a.seq;
+  const char* q_in = a.in[0] + b * a.sb[0] + s * a.ss[0];
+  const char* k_in = a.in[1] + b * a.sb[1] + s * a.ss[1] - a.q_heads * a.sh[1];
+  char* q_out = a.out[0] + b * a.ob[0] + s * a.os[0];
+  char* k_out = a.out[1] + b * a.ob[1] + s * a.os[1] - a.q_heads * a.oh[1];
+  auto head_in = [&](int h) { return h < a.q_heads ? q_in + h * a.sh[0] : k_in + h * a.sh[1]; };
+  auto head_out = [&](int h) { return h < a.q_heads ? q_out + h * a.oh[0] : k_out + h * a.oh[1]; };
+  const int P = a.items;
+  const int total = a.heads * P;
+  const int step = a.splits * 32;
+  auto offset = [&](int j) { return (NEIGH && VEC == 1 ? 2 * j : j) * VEC * kSize; };
+  using Raw = typename Pack<T, VEC>::Raw;
+  Pack<T, VEC> lo[U], hi[PAIR ? U : 1];
+  auto load = [&](int it0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int it = it0 + u * step;
+      if (it < total) {
+        const int h = quotient(it, a.items_m);
+        const char* p = head_in(h) + offset(it - h * P);
+        lo[u].raw = __ldcs(reinterpret_cast<const Raw*>(p));
+        if constexpr (PAIR) hi[u].raw = __ldcs(reinterpret_cast<const Raw*>(p + a.split_b));
+      }
+    }
+  };
+  int it0 = part * 32 + lane;
+  load(it0);
+  {
+    const double pos = a.pos64 ? (double)static_cast<const int64_t*>(a.pos)[b * a.pb + s * a.ps]
+                               : (double)static_cast<const int32_t*>(a.pos)[b * a.pb + s * a.ps];
+    for (int f = lane; f < a.rot / 2; f += 32) {
+      // in turns; 0.15915494309189535 is 1 / (2 pi)
+      double t = pos * (double)__ldg(a.freq + f) * 0.15915494309189535;
+      t -= rint(t);
+      float sn, cs;
+      sincospif((float)(2.0 * t), &sn, &cs);
+      const int j = f / NE, e = f % NE;
+      table[((e / CH) * P + j) * CH + e % CH] = cs * a.scale;
+      table[(((NE + e) / CH) * P + j) * CH + (NE + e) % CH] = sn * (a.scale * a.sign);
+    }
+    __syncwarp();
+  }
+  while (it0 < total) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int it = it0 + u * step;
+      if (it >= total) break;
+      const int h = quotient(it, a.items_m);
+      const int j = it - h * P;
+      char* p = head_out(h) + offset(j);
+      float cs[2 * NE];
+#pragma unroll
+      for (int c = 0; c < NCH; ++c) {
+        const Chunk<CH> v = reinterpret_cast<const Chunk<CH>*>(table)[c * P + j];
+#pragma unroll
+        for (int e = 0; e < CH; ++e) cs[c * CH + e] = v.v[e];
+      }
+      if constexpr (PAIR) {
+        Pack<T, VEC> x, y;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          const float f = Elem<T>::to_f(lo[u].e[e]), g = Elem<T>::to_f(hi[u].e[e]);
+          x.e[e] = Elem<T>::from_f(fmaf(f, cs[e], -(g * cs[NE + e])));
+          y.e[e] = Elem<T>::from_f(fmaf(g, cs[e], f * cs[NE + e]));
+        }
+        __stcs(reinterpret_cast<Raw*>(p), x.raw);
+        __stcs(reinterpret_cast<Raw*>(p + a.split_b), y.raw);
+      } else {
+        Pack<T, VEC> x;
+#pragma unroll
+        for (int e = 0; e < NE; ++e) {
+          const float f = Elem<T>::to_f(lo[u].e[2 * e]), g = Elem<T>::to_f(lo[u].e[2 * e + 1]);
+          x.e[2 * e] = Elem<T>::from_f(fmaf(f, cs[e], -(g * cs[NE + e])));
+          x.e[2 * e + 1] = Elem<T>::from_f(fmaf(g, cs[e], f * cs[NE + e]));
+        }
+        __stcs(reinterpret_cast<Raw*>(p), x.raw);
+      }
+    }
+    it0 += U * step;
+    load(it0);
+  }
+  // the rest of each head, where it is not in place already
+  for (int c0 = a.copy_from + part * 32 + lane; c0 < a.copy_to; c0 += 8 * step) {
+    Raw v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int c = c0 + u * step;
+      if (c >= a.copy_to) break;
+      const int h = quotient(c, a.copies_m);
+      v[u] = __ldcs(reinterpret_cast<const Raw*>(head_in(h) + a.rot * kSize) + (c - h * a.copies));
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int c = c0 + u * step;
+      if (c >= a.copy_to) break;
+      const int h = quotient(c, a.copies_m);
+      __stcs(reinterpret_cast<Raw*>(head_out(h) + a.rot * kSize) + (c - h * a.copies), v[u]);
+    }
+  }
+}
+
+template <typename T, int VEC, bool NEIGH>
+int launch(RotaryArgs a, int64_t head_dim, cudaStream_t stream) {
+  DeviceInfo dev;
+  int st = current_device_info(&dev);
+  if (st != FL_B200_OK) return st;
+  constexpr bool PAIR = !NEIGH || VEC == 1;
+  a.items = PAIR ? a.rot / 2 / VEC : a.rot / VEC;
+  a.copies = (int)((head_dim - a.rot) / VEC);
+  a.split_b = (NEIGH ? 1 : a.rot / 2) * (int)sizeof(T);
+  const int64_t most = std::max(a.items, a.copies);
+  if (a.heads * most * most >= (1ll << 31)) return FL_B200_ERR_TOO_LARGE;
+  a.items_m = (uint32_t)ceil_div(1ll << 31, a.items);
+  a.copies_m = a.copies ? (uint32_t)ceil_div(1ll << 31, a.copies) : 0;
+  // heads whose rest lies in place already are not copied onto themselves
+  a.copy_from = a.in[0] == a.out[0] ? a.q_heads * a.copies : 0;
+  a.copy_to = (a.heads > a.q_heads && a.in[1] != a.out[1] ? a.heads : a.q_heads) * a.copies;
+  // A warp a token leaves most of the GPU idle below 16 warps an SM; then a
+  // token's items are dealt to as many warps as have 32 of them.
+  const int64_t work = (int64_t)a.heads * a.items;
+  const int64_t want = ceil_div(16ll * dev.sm_count, a.tokens);
+  a.splits = (int)std::max<int64_t>(1, std::min<int64_t>(want, ceil_div(work, 32)));
+  const int64_t units = (int64_t)a.tokens * a.splits;
+  const size_t smem = 4 * ((a.rot + 3) & ~3) * sizeof(float);
+  launch_k((rotary_kernel<T, VEC, NEIGH>), (unsigned)ceil_div(units, 4), 128, smem, stream, a);
+  return launch_status();
+}
+
+template <typename T, bool NEIGH>
+int by_width(const RotaryArgs& a, int64_t head_dim, int64_t unit, cudaStream_t stream) {
+  const int64_t vec = unit / (int64_t)sizeof(T);
+  if constexpr (sizeof(T) == 2)
+    if (vec == 8) return launch<T, 8, NEIGH>(a, head_dim, stream);
+  if (vec == 4) return launch<T, 4, NEIGH>(a, head_dim, stream);
+  if (vec == 2) return launch<T, 2, NEIGH>(a, head_dim, stream);
+  return launch<T, 1, NEIGH>(a, head_dim, stream);
+}
+
+// First and last byte of a [B, S, H, D] operand.
+struct Extent {
+  uintptr_t lo, hi;
+};
+Extent extent(const void* p, int64_t H, int64_t B, int64_t S, int64_t sb, int64_t sh, int64_t ss, int64_t D,
+              int64_t size) {
+  const uintptr_t lo = reinterpret_cast<uintptr_t>(p);
+  return {lo, lo + (uintptr_t)(((B - 1) * sb + (H - 1) * sh + (S - 1) * ss + D) * size)};
+}
+
+}  // namespace
+}  // namespace flb200
+
+extern "C" FL_B200_API int fl_b200_rotary(
+    const void* q, void* q_out, int64_t Hq, int64_t sqb, int64_t sqh, int64_t sqs, int64_t soqb, int64_t soqh,
+    int64_t soqs, const void* k, void* k_out, int64_t Hk, int64_t skb, int64_t skh, int64_t sks, int64_t sokb,
+    int64_t sokh, int64_t soks, const void* positions, int64_t spb, int64_t sps, int pos_dtype,
+    const float* inv_freq, int64_t rot, float scale, int interleaved, int inverse, int64_t B, int64_t S,
+    int64_t D, int dtype, fl_b200_stream_t stream) {
+  using namespace flb200;
+  FLB_CHECK_ARG(B >= 0 && S >= 0 && D >= 0 && Hq >= 0 && Hk >= 0);
+  FLB_CHECK_ARG(rot >= 2 && rot % 2 == 0 && rot <= D);
+  if (!is_float_dtype(dtype) || (pos_dtype != FL_B200_I32 && pos_dtype != FL_B200_I64))
+    return FL_B200_ERR_UNSUPPORTED_DTYPE;
+  if (k == nullptr) Hk = 0;
+  if (B == 0 || S == 0 || D == 0 || Hq + Hk == 0) return FL_B200_OK;
+  FLB_CHECK_ARG((Hq == 0 || (q && q_out)) && (Hk == 0 || k_out) && positions && inv_freq);
+  FLB_CHECK_ARG(sqb >= 0 && sqh >= 0 && sqs >= 0 && skb >= 0 && skh >= 0 && sks >= 0 && spb >= 0 && sps >= 0 &&
+                soqb >= 0 && soqh >= 0 && soqs >= 0 && sokb >= 0 && sokh >= 0 && soks >= 0);
+  if (rot > FL_B200_ROTARY_MAX || Hq + Hk > (1 << 20) || D > (1 << 20) || B > 0x7fffffff / S)
+    return FL_B200_ERR_TOO_LARGE;
+  const int64_t size = dtype_size(dtype);
+  RotaryArgs a = {};
+  int64_t unit = 16;  // every address is a multiple of it
+  auto tensor = [&](int t, const void* in, void* out, int64_t H, const int64_t (&si)[3], const int64_t (&so)[3]) {
+    if (H == 0) return true;
+    const bool same = in == out;
+    const int64_t n[3] = {B, H, S};
+    for (int d = 0; d < 3; ++d) {
+      if (n[d] == 1) continue;
+      if ((same && si[d] != so[d]) || so[d] == 0) return false;
+      unit = std::gcd(unit, std::gcd(si[d] * size, so[d] * size));
+    }
+    if (!same) {
+      const Extent x = extent(in, H, B, S, si[0], si[1], si[2], D, size);
+      const Extent y = extent(out, H, B, S, so[0], so[1], so[2], D, size);
+      if (x.lo < y.hi && y.lo < x.hi) return false;
+    }
+    unit = std::gcd(unit, (int64_t)((reinterpret_cast<uintptr_t>(in) | reinterpret_cast<uintptr_t>(out)) & 15));
+    a.in[t] = static_cast<const char*>(in);
+    a.out[t] = static_cast<char*>(out);
+    a.sb[t] = si[0] * size, a.sh[t] = si[1] * size, a.ss[t] = si[2] * size;
+    a.ob[t] = so[0] * size, a.oh[t] = so[1] * size, a.os[t] = so[2] * size;
+    return true;
+  };
+  FLB_CHECK_ARG(tensor(0, q, q_out, Hq, {sqb, sqh, sqs}, {soqb, soqh, soqs}));
+  FLB_CHECK_ARG(tensor(1, k, k_out, Hk, {skb, skh, sks}, {sokb, sokh, soks}));
+  unit = std::gcd(unit, std::gcd((D - rot) * size, (interleaved ? rot : rot / 2) * size));
+  a.pos = positions, a.pb = spb, a.ps = sps, a.pos64 = pos_dtype == FL_B200_I64;
+  a.freq = inv_freq, a.scale = scale, a.sign = inverse ? -1.f : 1.f;
+  a.q_heads = (int)Hq, a.heads = (int)(Hq + Hk), a.rot = (int)rot;
+  a.tokens = (uint32_t)(B * S), a.seq = (uint32_t)S;
+  auto* s = static_cast<cudaStream_t>(stream);
+  return dispatch_float(dtype, [&](auto tag) -> int {
+    using T = decltype(tag);
+    return interleaved ? by_width<T, true>(a, D, unit, s) : by_width<T, false>(a, D, unit, s);
+  });
+}

@@ -1,0 +1,464 @@
+// The norm after a block, its gate and scale, the residual add and the norm
+// before the next block in one pass, and the gradients.
+//
+//   n = x / sqrt(mean(x^2) + eps)
+//   h = residual + scale * gate * n * (o + post)        (gate 1 where none is given)
+//   y = h / sqrt(mean(h^2) + eps) * (o + pre)
+//
+// o is the weights' offset (0, or 1 for weights stored as differences from
+// 1); the gate holds one row for every `rows_per_gate` rows: one for all (a
+// gate a channel), one a sequence, or one a token.  Everything is fp32 and h
+// and y are rounded once: y is the norm of h before its rounding.
+//
+// Gradients, with m = h / sqrt(mean(h^2) + eps) from the h that was stored:
+//   g         = dh + (dy w - m mean(dy w m)) / sqrt(mean(h^2) + eps),  w = o + pre
+//   dresidual = g
+//   dpre      = sum over rows of dy m
+//   A         = sum over a gate row's rows of g n
+//   dgate     = scale (o + post) A,   dpost = scale * sum over gate rows of gate A
+//   dx        = (t - n mean(t n)) / sqrt(mean(x^2) + eps),  t = scale gate (o + post) g
+//
+// Bound by memory: x and the residual are read and h and y written once
+// forward; x, h, dy and dh are read and dx and dresidual written backward.
+//
+// Column sums.  The rows are dealt to C chunks in order.  A chunk holds
+// whole gate rows, which it finishes itself, and at most two it shares with
+// its neighbours (its first and its last), whose A it leaves in the
+// workspace; a last kernel adds dpre's and dpost's partial sums and those
+// shared A in the order of the chunks.  So every sum has one order, whatever
+// the gate's shape, and no atomics.
+#include "row_ladder.cuh"
+
+namespace flb200 {
+namespace {
+
+struct Sandwich {
+  const void *x, *res, *post, *pre, *gate;
+  int64_t ldx, ldr;
+  void *y, *h;
+  uint32_t rows, per_gate;
+  int cols;
+  float eps, scale, off;
+  // backward
+  const void *dy, *dh, *hs;
+  int64_t ldy, ldh, lds;
+  void *dx, *dres, *dpost, *dpre, *dgate;
+  float* ws;        // [chunks][4][cols]: dpre, dpost, A of the first and of the last gate row
+  float4* stats;    // [rows]: 1/rms(x), 1/rms(h), mean(dy w m)
+  uint32_t chunks, per_chunk;
+};
+
+template <typename T>
+__device__ __forceinline__ const T* gate_row(const Sandwich& a, uint32_t row) {
+  return a.gate == nullptr ? nullptr : static_cast<const T*>(a.gate) + (int64_t)(row / a.per_gate) * a.cols;
+}
+
+// Row in registers: TPR threads, VPT packs of x each; h stays fp32.
+template <typename T, int TPR, int VPT, int BLOCK>
+__global__ void __launch_bounds__(BLOCK, ladder_min_blocks<BLOCK>())
+sandwich_vec_kernel(const __grid_constant__ Sandwich a) {
+  pdl_prologue();
+  constexpr int VW = Elem<T>::kVec;
+  __shared__ float smem[BLOCK / 32];
+  const int lane = threadIdx.x % TPR;
+  const uint64_t row64 = (uint64_t)blockIdx.x * (BLOCK / TPR) + threadIdx.x / TPR;
+  const bool ok = row64 < a.rows;
+  const uint32_t row = ok ? (uint32_t)row64 : a.rows - 1;
+  const int nvec = a.cols / VW;
+  const T* xr = static_cast<const T*>(a.x) + row * a.ldx;
+  const T* rr = static_cast<const T*>(a.res) + row * a.ldr;
+  const T* gr = gate_row<T>(a, row);
+  uint4 x[VPT], r[VPT];
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int vi = lane + i * TPR;
+    const bool in = ok && vi < nvec;
+    x[i] = in ? ld_stream(xr + (int64_t)vi * VW) : make_uint4(0, 0, 0, 0);
+    r[i] = in ? ld_stream(rr + (int64_t)vi * VW) : make_uint4(0, 0, 0, 0);
+  }
+  float ss = 0.f;
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    float f[VW];
+    unpack<T>(x[i], f);
+#pragma unroll
+    for (int e = 0; e < VW; ++e) ss = fmaf(f[e], f[e], ss);
+  }
+  ss = row_reduce<SumOp, TPR, BLOCK>(ss, smem);
+  const float rx = a.scale / sqrtf(ss / (float)a.cols + a.eps);
+  float h[VPT][VW];
+  ss = 0.f;
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int vi = lane + i * TPR;
+    if (!ok || vi >= nvec) continue;
+    float f[VW], w[VW];
+    unpack<T>(opaque(x[i]), f);
+    unpack<T>(ld_cached(static_cast<const T*>(a.post) + (int64_t)vi * VW), w);
+#pragma unroll
+    for (int e = 0; e < VW; ++e) f[e] = f[e] * rx * (w[e] + a.off);
+    if (gr != nullptr) {
+      unpack<T>(ld_cached(gr + (int64_t)vi * VW), w);
+#pragma unroll
+      for (int e = 0; e < VW; ++e) f[e] *= w[e];
+    }
+    unpack<T>(r[i], w);
+#pragma unroll
+    for (int e = 0; e < VW; ++e) {
+      h[i][e] = f[e] + w[e];
+      ss = fmaf(h[i][e], h[i][e], ss);
+    }
+    st_stream(static_cast<T*>(a.h) + (int64_t)row * a.cols + (int64_t)vi * VW, pack<T>(h[i]));
+  }
+  ss = row_reduce<SumOp, TPR, BLOCK>(ss, smem);
+  const float rh = 1.0f / sqrtf(ss / (float)a.cols + a.eps);
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int vi = lane + i * TPR;
+    if (!ok || vi >= nvec) continue;
+    float w[VW];
+    unpack<T>(ld_cached(static_cast<const T*>(a.pre) + (int64_t)vi * VW), w);
+#pragma unroll
+    for (int e = 0; e < VW; ++e) w[e] = h[i][e] * rh * (w[e] + a.off);
+    st_stream(static_cast<T*>(a.y) + (int64_t)row * a.cols + (int64_t)vi * VW, pack<T>(w));
+  }
+}
+
+// Rows of any length and alignment: a CTA a row by single elements, x and the
+// residual read again from cache.
+template <typename T>
+__global__ void __launch_bounds__(512)
+sandwich_loop_kernel(const __grid_constant__ Sandwich a) {
+  pdl_prologue();
+  constexpr int BLOCK = 512;
+  __shared__ float smem[BLOCK / 32];
+  const T *post = static_cast<const T*>(a.post), *pre = static_cast<const T*>(a.pre);
+  for (uint32_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const T* xr = static_cast<const T*>(a.x) + row * a.ldx;
+    const T* rr = static_cast<const T*>(a.res) + row * a.ldr;
+    const T* gr = gate_row<T>(a, row);
+    T* hr = static_cast<T*>(a.h) + (int64_t)row * a.cols;
+    T* yr = static_cast<T*>(a.y) + (int64_t)row * a.cols;
+    float ss = 0.f;
+    for (int c = threadIdx.x; c < a.cols; c += BLOCK) {
+      const float f = Elem<T>::to_f(xr[c]);
+      ss = fmaf(f, f, ss);
+    }
+    ss = block_reduce<SumOp, BLOCK>(ss, smem);
+    const float rx = a.scale / sqrtf(ss / (float)a.cols + a.eps);
+    auto sum_of = [&](int c) {
+      float f = Elem<T>::to_f(xr[c]) * rx * (Elem<T>::to_f(post[c]) + a.off);
+      if (gr != nullptr) f *= Elem<T>::to_f(gr[c]);
+      return f + Elem<T>::to_f(rr[c]);
+    };
+    ss = 0.f;
+    for (int c = threadIdx.x; c < a.cols; c += BLOCK) {
+      const float f = sum_of(c);
+      ss = fmaf(f, f, ss);
+      hr[c] = Elem<T>::from_f(f);
+    }
+    ss = block_reduce<SumOp, BLOCK>(ss, smem);
+    const float rh = 1.0f / sqrtf(ss / (float)a.cols + a.eps);
+    for (int c = threadIdx.x; c < a.cols; c += BLOCK)
+      yr[c] = Elem<T>::from_f(sum_of(c) * rh * (Elem<T>::to_f(pre[c]) + a.off));
+  }
+}
+
+// ------------------------------------------------------------- backward ---
+// Rows of any length and alignment: the row gradients and the row's
+// statistics, then the column sums in a second pass over the operands.
+template <typename T>
+__global__ void __launch_bounds__(512)
+sandwich_bwd_rows_kernel(const __grid_constant__ Sandwich a) {
+  pdl_prologue();
+  constexpr int BLOCK = 512;
+  __shared__ float smem[BLOCK / 32];
+  const T *post = static_cast<const T*>(a.post), *pre = static_cast<const T*>(a.pre);
+  for (uint32_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const T* xr = static_cast<const T*>(a.x) + row * a.ldx;
+    const T* hr = static_cast<const T*>(a.hs) + row * a.lds;
+    const T* dyr = static_cast<const T*>(a.dy) + row * a.ldy;
+    const T* dhr = a.dh == nullptr ? nullptr : static_cast<const T*>(a.dh) + row * a.ldh;
+    const T* gr = gate_row<T>(a, row);
+    float sx = 0.f, sh = 0.f, sd = 0.f;
+    for (int c = threadIdx.x; c < a.cols; c += BLOCK) {
+      const float x = Elem<T>::to_f(xr[c]), h = Elem<T>::to_f(hr[c]);
+      const float d = Elem<T>::to_f(dyr[c]) * (Elem<T>::to_f(pre[c]) + a.off);
+      sx = fmaf(x, x, sx);
+      sh = fmaf(h, h, sh);
+      sd = fmaf(d, h, sd);
+    }
+    sx = block_reduce<SumOp, BLOCK>(sx, smem);
+    sh = block_reduce<SumOp, BLOCK>(sh, smem);
+    sd = block_reduce<SumOp, BLOCK>(sd, smem);
+    const float n = (float)a.cols;
+    const float rx = 1.0f / sqrtf(sx / n + a.eps), rh = 1.0f / sqrtf(sh / n + a.eps);
+    const float mean = sd * rh / n;
+    auto grad = [&](int c) {
+      const float d = Elem<T>::to_f(dyr[c]) * (Elem<T>::to_f(pre[c]) + a.off);
+      const float g = rh * (d - Elem<T>::to_f(hr[c]) * rh * mean);
+      return dhr == nullptr ? g : g + Elem<T>::to_f(dhr[c]);
+    };
+    auto weight = [&](int c) {
+      const float w = a.scale * (Elem<T>::to_f(post[c]) + a.off);
+      return gr == nullptr ? w : w * Elem<T>::to_f(gr[c]);
+    };
+    float st = 0.f;
+    for (int c = threadIdx.x; c < a.cols; c += BLOCK) {
+      const float g = grad(c);
+      st = fmaf(g * weight(c), Elem<T>::to_f(xr[c]), st);
+      static_cast<T*>(a.dres)[(int64_t)row * a.cols + c] = Elem<T>::from_f(g);
+    }
+    st = block_reduce<SumOp, BLOCK>(st, smem);
+    const float mean_t = st * rx / n;
+    for (int c = threadIdx.x; c < a.cols; c += BLOCK)
+      static_cast<T*>(a.dx)[(int64_t)row * a.cols + c] =
+          Elem<T>::from_f(rx * (grad(c) * weight(c) - Elem<T>::to_f(xr[c]) * rx * mean_t));
+    if (threadIdx.x == 0) a.stats[row] = make_float4(rx, rh, mean, 0.f);
+  }
+}
+
+// A thread a column of a chunk of rows (blockIdx.y).
+template <typename T>
+__global__ void __launch_bounds__(128)
+sandwich_bwd_cols_kernel(const __grid_constant__ Sandwich a) {
+  pdl_prologue();
+  const int c = blockIdx.x * 128 + threadIdx.x;
+  if (c >= a.cols) return;
+  const uint32_t chunk = blockIdx.y;
+  const uint32_t r0 = chunk * a.per_chunk, r1 = min(a.rows, r0 + a.per_chunk);
+  const float pre = Elem<T>::to_f(static_cast<const T*>(a.pre)[c]) + a.off;
+  const float post = a.scale * (Elem<T>::to_f(static_cast<const T*>(a.post)[c]) + a.off);
+  float dpre = 0.f, dpost = 0.f, shared[2] = {0.f, 0.f};
+  uint32_t row = r0;
+  while (row < r1) {  // one gate row a turn
+    const uint32_t seg = row / a.per_gate;
+    const uint64_t seg_end = (uint64_t)(seg + 1) * a.per_gate;
+    const uint32_t end = seg_end < r1 ? (uint32_t)seg_end : r1;
+    const bool whole = (uint64_t)seg * a.per_gate >= r0 && (seg_end <= r1 || (r1 == a.rows));
+    const bool is_first = seg == r0 / a.per_gate;
+    float sum = 0.f;
+#pragma unroll 4
+    for (; row < end; ++row) {
+      const float4 s = a.stats[row];
+      const float dy = Elem<T>::to_f(static_cast<const T*>(a.dy)[row * a.ldy + c]);
+      const float m = Elem<T>::to_f(static_cast<const T*>(a.hs)[row * a.lds + c]) * s.y;
+      const float x = Elem<T>::to_f(static_cast<const T*>(a.x)[row * a.ldx + c]);
+      float g = s.y * (dy * pre - m * s.z);
+      if (a.dh != nullptr) g += Elem<T>::to_f(static_cast<const T*>(a.dh)[row * a.ldh + c]);
+      dpre = fmaf(dy, m, dpre);
+      sum = fmaf(g, x * s.x, sum);
+    }
+    if (a.gate != nullptr) {
+      const int64_t at = (int64_t)seg * a.cols + c;
+      dpost = fmaf(a.scale * Elem<T>::to_f(static_cast<const T*>(a.gate)[at]), sum, dpost);
+      if (whole) static_cast<T*>(a.dgate)[at] = Elem<T>::from_f(post * sum);
+      else shared[is_first ? 0 : 1] = sum;
+    } else {
+      dpost = fmaf(a.scale, sum, dpost);
+    }
+  }
+  float* w = a.ws + (int64_t)chunk * 4 * a.cols + c;
+  w[0] = dpre;
+  w[a.cols] = dpost;
+  w[2ll * a.cols] = shared[0];
+  w[3ll * a.cols] = shared[1];
+}
+
+// Adds the chunks' partial sums: blockIdx.y == 0 dpre and dpost, y > 0 the
+// gate row that begins in chunk y - 1 and reaches into chunk y, if there is
+// one.  32 columns a CTA, 16 threads a column.
+template <typename T>
+__global__ void __launch_bounds__(512)
+sandwich_bwd_sum_kernel(const __grid_constant__ Sandwich a) {
+  pdl_prologue();
+  __shared__ float part[2][16][33];
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int c = blockIdx.x * 32 + tx;
+  const int64_t stride = 4ll * a.cols;
+  uint32_t from = 0, to = a.chunks, seg = 0;
+  if (blockIdx.y > 0) {
+    const uint32_t edge = blockIdx.y * a.per_chunk;  // the first row of chunk y
+    seg = edge / a.per_gate;
+    const uint64_t begin = (uint64_t)seg * a.per_gate;
+    if (a.gate == nullptr || begin == edge || begin < edge - a.per_chunk) return;  // (the whole CTA)
+    const uint64_t end = min((uint64_t)a.rows, begin + a.per_gate);
+    from = blockIdx.y - 1;
+    to = (uint32_t)((end - 1) / a.per_chunk) + 1;
+  }
+  float s0 = 0.f, s1 = 0.f;
+  if (c < a.cols) {
+    for (uint32_t k = from + ty; k < to; k += 16) {
+      const float* w = a.ws + k * stride + c;
+      if (blockIdx.y == 0) {
+        s0 += w[0];
+        s1 += w[a.cols];
+      } else {
+        // the chunk's first gate row, or its last
+        s0 += w[(seg == k * a.per_chunk / a.per_gate ? 2ll : 3ll) * a.cols];
+      }
+    }
+  }
+  part[0][ty][tx] = s0;
+  part[1][ty][tx] = s1;
+  __syncthreads();
+  if (ty != 0 || c >= a.cols) return;
+#pragma unroll
+  for (int k = 1; k < 16; ++k) {
+    s0 += part[0][k][tx];
+    s1 += part[1][k][tx];
+  }
+  if (blockIdx.y == 0) {
+    static_cast<T*>(a.dpre)[c] = Elem<T>::from_f(s0);
+    static_cast<T*>(a.dpost)[c] = Elem<T>::from_f(s1);
+  } else {
+    const float post = a.scale * (Elem<T>::to_f(static_cast<const T*>(a.post)[c]) + a.off);
+    static_cast<T*>(a.dgate)[(int64_t)seg * a.cols + c] = Elem<T>::from_f(post * s0);
+  }
+}
+
+// Chunks of the column sums: about two CTAs' worth of rows an SM, each at
+// least 8 rows.
+void plan_chunks(int64_t rows, int64_t cols, int sms, uint32_t* chunks, uint32_t* per_chunk) {
+  const int64_t tiles = ceil_div(cols, 128);
+  const int64_t want = std::max<int64_t>(1, ceil_div(8ll * sms, tiles));
+  const int64_t per = std::max<int64_t>(8, ceil_div(rows, want));
+  *per_chunk = (uint32_t)per;
+  *chunks = (uint32_t)ceil_div(rows, per);
+}
+
+template <typename T>
+int launch_fwd(const Sandwich& a, const DeviceInfo& dev, cudaStream_t stream) {
+  constexpr int VW = Elem<T>::kVec;
+  if (a.cols % VW == 0 && a.ldx % VW == 0 && a.ldr % VW == 0 && aligned16(a.x) && aligned16(a.res) &&
+      aligned16(a.post) && aligned16(a.pre) && aligned16(a.gate) && aligned16(a.y) && aligned16(a.h)) {
+    const int r = row_ladder<2>(a.cols / VW, [&](auto tpr, auto vpt) -> int {
+      constexpr int TPR = decltype(tpr)::value, VPT = decltype(vpt)::value;
+      constexpr int BLOCK = ladder_block<TPR>();
+      launch_k((sandwich_vec_kernel<T, TPR, VPT, BLOCK>), (unsigned)ceil_div(a.rows, BLOCK / TPR), BLOCK, 0, stream,
+               a);
+      return launch_status();
+    });
+    if (r >= 0) return r;
+  }
+  launch_k(sandwich_loop_kernel<T>, (unsigned)std::min<int64_t>(a.rows, 4ll * dev.sm_count), 512, 0, stream, a);
+  return launch_status();
+}
+
+template <typename T>
+int launch_bwd(Sandwich a, const DeviceInfo& dev, cudaStream_t stream) {
+  launch_k(sandwich_bwd_rows_kernel<T>, (unsigned)std::min<int64_t>(a.rows, 4ll * dev.sm_count), 512, 0, stream, a);
+  launch_k(sandwich_bwd_cols_kernel<T>, dim3((unsigned)ceil_div(a.cols, 128), a.chunks), 128, 0, stream, a);
+  launch_k(sandwich_bwd_sum_kernel<T>, dim3((unsigned)ceil_div(a.cols, 32), a.gate ? a.chunks : 1), 512, 0, stream,
+           a);
+  return launch_status();
+}
+
+// The bytes of a row operand (stride in elements of `size` bytes).
+struct Range {
+  uintptr_t lo, hi;
+  Range(const void* p, int64_t ld, int64_t rows, int64_t cols, int64_t size)
+      : lo(reinterpret_cast<uintptr_t>(p)), hi(p ? lo + (uintptr_t)(((rows - 1) * ld + cols) * size) : lo) {}
+  bool meets(const Range& o) const { return lo < o.hi && o.lo < hi; }
+};
+
+int check(Sandwich& a, int64_t rows, int64_t cols, int64_t per_gate, const void* gate, float eps, float scale,
+          float off) {
+  FLB_CHECK_ARG(gate == nullptr || per_gate >= 1);
+  FLB_CHECK_ARG(eps >= 0.f && scale == scale && off == off);
+  if (rows > 0x7fffffff || cols > 0x7fffff00) return FL_B200_ERR_TOO_LARGE;
+  a.rows = (uint32_t)rows, a.cols = (int)cols, a.gate = gate;
+  a.per_gate = (uint32_t)(gate == nullptr ? rows : std::min(per_gate, rows));
+  a.eps = eps, a.scale = scale, a.off = off;
+  return FL_B200_OK;
+}
+
+}  // namespace
+}  // namespace flb200
+
+extern "C" {
+
+FL_B200_API int fl_b200_sandwich_norm(const void* x, int64_t ld_x, const void* residual, int64_t ld_r,
+                                      const void* post, const void* pre, const void* gate,
+                                      int64_t rows_per_gate, void* y, void* h, int64_t rows, int64_t cols,
+                                      float eps, float scale, float weight_offset, int dtype,
+                                      fl_b200_stream_t stream) {
+  using namespace flb200;
+  FLB_CHECK_ARG(rows >= 0 && cols >= 0);
+  if (!is_float_dtype(dtype)) return FL_B200_ERR_UNSUPPORTED_DTYPE;
+  if (rows == 0 || cols == 0) return FL_B200_OK;
+  FLB_CHECK_ARG(x && residual && post && pre && y && h && ld_x >= cols && ld_r >= cols);
+  Sandwich a = {};
+  int st = check(a, rows, cols, rows_per_gate, gate, eps, scale, weight_offset);
+  if (st != FL_B200_OK) return st;
+  const int64_t size = dtype_size(dtype);
+  const Range ry(y, cols, rows, cols, size), rh(h, cols, rows, cols, size);
+  const Range in[] = {{x, ld_x, rows, cols, size}, {residual, ld_r, rows, cols, size},
+                      {gate, cols, gate ? ceil_div(rows, a.per_gate) : 1, cols, size}};
+  FLB_CHECK_ARG(!ry.meets(rh));
+  for (const Range& r : in) FLB_CHECK_ARG(!ry.meets(r) && !rh.meets(r));
+  a.x = x, a.ldx = ld_x, a.res = residual, a.ldr = ld_r, a.post = post, a.pre = pre, a.y = y, a.h = h;
+  DeviceInfo dev;
+  st = current_device_info(&dev);
+  if (st != FL_B200_OK) return st;
+  return dispatch_float(dtype, [&](auto tag) -> int {
+    return launch_fwd<decltype(tag)>(a, dev, static_cast<cudaStream_t>(stream));
+  });
+}
+
+FL_B200_API size_t fl_b200_sandwich_norm_bwd_workspace_size(int64_t rows, int64_t cols) {
+  using namespace flb200;
+  DeviceInfo dev;
+  if (rows <= 0 || cols <= 0 || current_device_info(&dev) != FL_B200_OK) return 0;
+  uint32_t chunks, per;
+  plan_chunks(rows, cols, dev.sm_count, &chunks, &per);
+  return (size_t)rows * sizeof(float4) + (size_t)chunks * 4 * cols * sizeof(float);
+}
+
+FL_B200_API int fl_b200_sandwich_norm_bwd(const void* dy, int64_t ld_dy, const void* dh, int64_t ld_dh,
+                                          const void* x, int64_t ld_x, const void* h, int64_t ld_h,
+                                          const void* post, const void* pre, const void* gate,
+                                          int64_t rows_per_gate, void* dx, void* dresidual, void* dpost,
+                                          void* dpre, void* dgate, int64_t rows, int64_t cols, float eps,
+                                          float scale, float weight_offset, int dtype, void* workspace,
+                                          size_t workspace_bytes, fl_b200_stream_t stream) {
+  using namespace flb200;
+  FLB_CHECK_ARG(rows >= 0 && cols >= 0);
+  if (!is_float_dtype(dtype)) return FL_B200_ERR_UNSUPPORTED_DTYPE;
+  if (cols == 0) return FL_B200_OK;
+  FLB_CHECK_ARG(dpost && dpre);
+  const int64_t size = dtype_size(dtype);
+  if (rows == 0) {  // sums over no rows
+    auto* s = static_cast<cudaStream_t>(stream);
+    if (cudaMemsetAsync(dpost, 0, cols * size, s) != cudaSuccess ||
+        cudaMemsetAsync(dpre, 0, cols * size, s) != cudaSuccess)
+      return launch_status();
+    return FL_B200_OK;
+  }
+  FLB_CHECK_ARG(dy && x && h && post && pre && dx && dresidual && (!gate || dgate));
+  FLB_CHECK_ARG(ld_dy >= cols && ld_x >= cols && ld_h >= cols && (!dh || ld_dh >= cols));
+  Sandwich a = {};
+  int st = check(a, rows, cols, rows_per_gate, gate, eps, scale, weight_offset);
+  if (st != FL_B200_OK) return st;
+  const Range rx(dx, cols, rows, cols, size), rr(dresidual, cols, rows, cols, size);
+  const Range in[] = {{dy, ld_dy, rows, cols, size}, {dh, ld_dh, rows, cols, size}, {x, ld_x, rows, cols, size},
+                      {h, ld_h, rows, cols, size}, {gate, cols, gate ? ceil_div(rows, a.per_gate) : 1, cols, size}};
+  FLB_CHECK_ARG(!rx.meets(rr));
+  for (const Range& r : in) FLB_CHECK_ARG(!rx.meets(r) && !rr.meets(r));
+  DeviceInfo dev;
+  st = current_device_info(&dev);
+  if (st != FL_B200_OK) return st;
+  if (workspace == nullptr || workspace_bytes < fl_b200_sandwich_norm_bwd_workspace_size(rows, cols))
+    return FL_B200_ERR_WORKSPACE;
+  if (!aligned16(workspace)) return FL_B200_ERR_MISALIGNED;
+  plan_chunks(rows, cols, dev.sm_count, &a.chunks, &a.per_chunk);
+  a.stats = static_cast<float4*>(workspace);
+  a.ws = reinterpret_cast<float*>(a.stats + rows);
+  a.dy = dy, a.ldy = ld_dy, a.dh = dh, a.ldh = ld_dh, a.x = x, a.ldx = ld_x, a.hs = h, a.lds = ld_h;
+  a.post = post, a.pre = pre, a.dx = dx, a.dres = dresidual, a.dpost = dpost, a.dpre = dpre, a.dgate = dgate;
+  return dispatch_float(dtype, [&](auto tag) -> int {
+    return launch_bwd<decltype(tag)>(a, dev, static_cast<cudaStream_t>(stream));
+  });
+}
+
+}  // extern "C"

@@ -98,6 +98,27 @@ PROTOTYPES: dict[str, tuple] = {
     "fl_b200_verify_draft": (
         _i32, [_p, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _p, _i64, _i64, _i64, _p, _p,
                _i32, _p]),
+    "fl_b200_rotary": (
+        _i32,
+        [_p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+         _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+         _p, _i64, _i64, _i32, _p, _i64, _f32, _i32, _i32, _i64, _i64, _i64, _i32, _p]),
+    "fl_b200_sandwich_norm": (
+        _i32, [_p, _i64, _p, _i64, _p, _p, _p, _i64, _p, _p, _i64, _i64, _f32, _f32, _f32, _i32, _p]),
+    "fl_b200_sandwich_norm_bwd_workspace_size": (_sz, [_i64, _i64]),
+    "fl_b200_sandwich_norm_bwd": (
+        _i32, [_p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _p, _p, _i64, _p, _p, _p, _p, _p,
+               _i64, _i64, _f32, _f32, _f32, _i32, _p, _sz, _p]),
+    "fl_b200_span_softmax": (
+        _i32, [_p, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _i64, _i64, _i64, _i64, _i64,
+               _f32, _f32, _i32, _i32, _p]),
+    "fl_b200_span_softmax_bwd": (
+        _i32, [_p, _i64, _p, _i64, _p, _i64, _p, _i64, _i64, _p, _i64, _i64, _i64, _i64, _i64,
+               _f32, _f32, _i32, _i32, _p]),
+    "fl_b200_grad_norm_workspace_size": (_sz, [_i64]),
+    "fl_b200_grad_norm": (_i32, [C.POINTER(_p), _pi64, C.POINTER(_i32), _i64, _i32, _p, _p, _sz, _p]),
+    "fl_b200_clip_grads": (
+        _i32, [C.POINTER(_p), C.POINTER(_p), _pi64, C.POINTER(_i32), _i64, _f32, _i32, _p, _p, _sz, _p]),
 }
 
 

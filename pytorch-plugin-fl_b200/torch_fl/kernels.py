@@ -13,6 +13,8 @@ The fused-op semantics follow the HF formulas the reference runs op by op:
 
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from . import _abi
@@ -550,6 +552,212 @@ def sum_i32_i64(x: torch.Tensor, full: bool) -> torch.Tensor:
         _abi.call("fl_b200_sum_i32_i64", x.data_ptr(), ld, rows, cols, out.data_ptr(),
                   int(full), wsp, wsn, _stream(x))
     return out
+
+
+# ---------------------------------- a training step around the matrix products
+def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv_freq: torch.Tensor,
+           scale: float = 1.0, interleaved: bool = False, inverse: bool = False, layout: str = "bhsd",
+           inplace: bool = False):
+    """q and k turned by positions * inv_freq (no table); inplace touches the
+    turned part of each head only."""
+    B, Hq, S, D, sq = _bhsd(q, layout)
+    ops = [t for t in (q, k, positions, inv_freq) if t is not None]
+    _one_device(*ops)
+    qo = q if inplace else torch.empty_like(q)
+    soq = _bhsd(qo, layout)[4]
+    Hk, sk, sok, ko = 0, (0, 0, 0), (0, 0, 0), None
+    if k is not None:
+        Bk, Hk, Sk, Dk, sk = _bhsd(k, layout)
+        if (Bk, Sk, Dk) != (B, S, D) or k.dtype != q.dtype:
+            raise ValueError("q and k disagree")
+        ko = k if inplace else torch.empty_like(k)
+        sok = _bhsd(ko, layout)[4]
+    if positions.dtype not in (torch.int32, torch.int64) or positions.dim() not in (1, 2) \
+            or positions.shape[-1] != S or (positions.dim() == 2 and positions.shape[0] not in (1, B)):
+        raise ValueError("positions must be int32 or int64 [seq] or [batch, seq]")
+    if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
+        raise ValueError("inv_freq must be a contiguous float32 [n] tensor")
+    spb = positions.stride(0) if positions.dim() == 2 and positions.shape[0] > 1 else 0
+    with _on_device(q):
+        _abi.call("fl_b200_rotary", q.data_ptr(), qo.data_ptr(), Hq, *sq, *soq,
+                  None if k is None else k.data_ptr(), None if k is None else ko.data_ptr(), Hk, *sk, *sok,
+                  positions.data_ptr(), spb, positions.stride(-1), _DT[positions.dtype],
+                  inv_freq.data_ptr(), 2 * inv_freq.numel(), float(scale), int(interleaved), int(inverse),
+                  B, S, D, dtype_code(q), _stream(q))
+    return qo, ko
+
+
+def _gate_rows(x: torch.Tensor, gate: torch.Tensor | None) -> int:
+    """How many of x's rows share a row of the gate."""
+    if gate is None or gate.dim() == 1:
+        return max(1, x.shape[:-1].numel())
+    d, per = x.dim() - 2, 1
+    while d >= 0 and gate.shape[d] == 1:
+        per *= x.shape[d]
+        d -= 1
+    if gate.dim() != x.dim() or gate.shape[:d + 1] != x.shape[:d + 1] or gate.shape[-1] != x.shape[-1]:
+        raise ValueError("gate must be [hidden], or x's shape with the last dims before hidden 1")
+    return max(1, per)
+
+
+def _sandwich_weights(x, post, pre, gate):
+    for w in (post, pre):
+        if w.dtype != x.dtype or w.shape != x.shape[-1:] or not w.is_contiguous():
+            raise ValueError("weights must be contiguous [hidden] tensors of x's dtype")
+    if gate is not None and (gate.dtype != x.dtype or gate.shape[-1:] != x.shape[-1:]):
+        raise ValueError("gate must have x's dtype and hidden size")
+
+
+def sandwich_norm(x: torch.Tensor, residual: torch.Tensor, post: torch.Tensor, pre: torch.Tensor, eps: float,
+                  gate: torch.Tensor | None = None, scale: float = 1.0,
+                  weight_offset: float = 0.0) -> tuple[torch.Tensor, torch.Tensor]:
+    """(y, h): h = residual + scale * gate * rms_norm(x) * (offset + post),
+    y = rms_norm(h) * (offset + pre)."""
+    if x.shape != residual.shape or x.dtype != residual.dtype:
+        raise ValueError("x and the residual must match")
+    _sandwich_weights(x, post, pre, gate)
+    _one_device(x, residual, post, pre, gate)
+    per = _gate_rows(x, gate)
+    gate = None if gate is None else gate.contiguous()
+    shape = x.shape
+    x, rows, cols, ldx = _rows_apart(x)
+    residual, _, _, ldr = _rows_apart(residual)
+    y, h = (torch.empty(shape, dtype=x.dtype, device=x.device) for _ in range(2))
+    with _on_device(x):
+        _abi.call("fl_b200_sandwich_norm", x.data_ptr(), ldx, residual.data_ptr(), ldr, post.data_ptr(),
+                  pre.data_ptr(), None if gate is None else gate.data_ptr(), per, y.data_ptr(), h.data_ptr(),
+                  rows, cols, float(eps), float(scale), float(weight_offset), dtype_code(x), _stream(x))
+    return y, h
+
+
+def sandwich_norm_backward(dy, dh, x, h, post, pre, eps: float, gate=None, scale: float = 1.0,
+                           weight_offset: float = 0.0):
+    """(dx, dresidual, dpost, dpre, dgate) of sandwich_norm; dh None: no
+    gradient of h; dgate None without a gate."""
+    for t in (dy, dh, h):
+        if t is not None and (t.shape != x.shape or t.dtype != x.dtype):
+            raise ValueError("dy, dh, x and h must match")
+    _sandwich_weights(x, post, pre, gate)
+    _one_device(x, dy, dh, h, post, pre, gate)
+    per = _gate_rows(x, gate)
+    gate = None if gate is None else gate.contiguous()
+    shape = x.shape
+    x, rows, cols, ldx = _rows_apart(x)
+    h, _, _, ldh = _rows_apart(h)
+    dy, _, _, ldy = _rows_apart(dy)
+    ldd = 0
+    if dh is not None:
+        dh, _, _, ldd = _rows_apart(dh)
+    dx, dres = (torch.empty(shape, dtype=x.dtype, device=x.device) for _ in range(2))
+    dpost, dpre = (torch.empty(cols, dtype=x.dtype, device=x.device) for _ in range(2))
+    dgate = None if gate is None else torch.empty_like(gate)
+    with _on_device(x):
+        nws = _abi.lib().fl_b200_sandwich_norm_bwd_workspace_size(rows, cols)
+        ws = torch.empty(max(nws, 16), dtype=torch.uint8, device=x.device)
+        _abi.call("fl_b200_sandwich_norm_bwd", dy.data_ptr(), ldy, None if dh is None else dh.data_ptr(), ldd,
+                  x.data_ptr(), ldx, h.data_ptr(), ldh, post.data_ptr(), pre.data_ptr(),
+                  None if gate is None else gate.data_ptr(), per, dx.data_ptr(), dres.data_ptr(),
+                  dpost.data_ptr(), dpre.data_ptr(), None if gate is None else dgate.data_ptr(), rows, cols,
+                  float(eps), float(scale), float(weight_offset), dtype_code(x), ws.data_ptr(), nws, _stream(x))
+    return dx, dres, dpost, dpre, dgate
+
+
+def _per_query(t: torch.Tensor, B: int, Q: int, tail: int) -> tuple[torch.Tensor, int, int]:
+    u = t if tail else t.unsqueeze(-1)
+    u = u.unsqueeze(0) if u.dim() == 2 else u
+    if t.dtype != torch.int32 or u.dim() != 3 or u.shape[0] not in (1, B) or u.shape[1] != Q \
+            or u.shape[2] != max(tail, 1):
+        raise ValueError("int32 values for each query expected")
+    if tail and u.stride(2) != 1:
+        u = u.contiguous()
+    return u, 0 if u.shape[0] == 1 else u.stride(0), u.stride(1)
+
+
+def span_softmax(x: torch.Tensor, spans: torch.Tensor, scale: float = 1.0, cap: float | None = None,
+                 slopes: torch.Tensor | None = None, positions: torch.Tensor | None = None,
+                 out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """softmax of scale * x (capped, biased by distance) over each query's span
+    of keys; zeros elsewhere."""
+    B, H, Q, Kn = _as_bhqk(x).shape
+    _one_device(x, spans, slopes, positions)
+    spans, sb, sq = _per_query(spans, B, Q, 2)
+    pb = pq = 0
+    if positions is not None:
+        positions, pb, pq = _per_query(positions, B, Q, 0)
+    if slopes is not None and (slopes.dtype != torch.float32 or slopes.shape != (H,) or not slopes.is_contiguous()):
+        raise ValueError("slopes must be a contiguous float32 [heads] tensor")
+    if cap is not None and not cap > 0:
+        raise ValueError("cap must be positive")
+    out = torch.empty(x.shape, dtype=out_dtype or x.dtype, device=x.device)
+    x, rows, cols, ld = _rows_apart(x)
+    with _on_device(x):
+        _abi.call("fl_b200_span_softmax", x.data_ptr(), ld, spans.data_ptr(), sb, sq,
+                  None if positions is None else positions.data_ptr(), pb, pq,
+                  None if slopes is None else slopes.data_ptr(), out.data_ptr(), cols, rows, cols, H, Q,
+                  float(scale), float(cap or 0.0), dtype_code(x), dtype_code(out), _stream(x))
+    return out
+
+
+def span_softmax_backward(dy: torch.Tensor, y: torch.Tensor, x: torch.Tensor, spans: torch.Tensor,
+                          scale: float = 1.0, cap: float | None = None) -> torch.Tensor:
+    if dy.shape != y.shape or dy.dtype != y.dtype or y.shape != x.shape:
+        raise ValueError("dy, y and x must match")
+    B, H, Q, Kn = _as_bhqk(y).shape
+    _one_device(x, y, dy, spans)
+    spans, sb, sq = _per_query(spans, B, Q, 2)
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    x, _, _, ldx = _rows_apart(x)
+    dy, _, _, ldd = _rows_apart(dy)
+    y, rows, cols, ldy = _rows_apart(y)
+    with _on_device(y):
+        _abi.call("fl_b200_span_softmax_bwd", dy.data_ptr(), ldd, y.data_ptr(), ldy, x.data_ptr(), ldx,
+                  spans.data_ptr(), sb, sq, dx.data_ptr(), cols, rows, cols, H, Q, float(scale),
+                  float(cap or 0.0), dtype_code(y), dtype_code(dx), _stream(y))
+    return dx
+
+
+def _grad_list(tensors):
+    n = len(tensors)
+    if n == 0:
+        raise ValueError("no tensors")
+    _one_device(*tensors)
+    if any(not t.is_contiguous() for t in tensors):
+        raise ValueError("contiguous tensors expected")
+    ptrs = (ctypes.c_void_p * n)(*[t.data_ptr() for t in tensors])
+    numels = _abi.i64_array([t.numel() for t in tensors])
+    dtypes = (ctypes.c_int * n)(*[dtype_code(t) for t in tensors])
+    return n, ptrs, numels, dtypes
+
+
+def grad_norm(tensors, max_kind: bool = False) -> torch.Tensor:
+    """The norm of the tensors taken as one vector: sqrt(sum x^2), or max |x|."""
+    n, ptrs, numels, dtypes = _grad_list(tensors)
+    t = tensors[0]
+    norm = torch.empty((), dtype=torch.float32, device=t.device)
+    with _on_device(t):
+        nws = _abi.lib().fl_b200_grad_norm_workspace_size(n)
+        ws = torch.empty(nws, dtype=torch.uint8, device=t.device)
+        _abi.call("fl_b200_grad_norm", ptrs, numels, dtypes, n, int(max_kind), norm.data_ptr(), ws.data_ptr(),
+                  nws, _stream(t))
+    return norm
+
+
+def clip_grads(tensors, max_norm: float, max_kind: bool = False, out=None):
+    """(clipped, norm): the tensors times min(1, max_norm / (norm + 1e-6))."""
+    n, ptrs, numels, dtypes = _grad_list(tensors)
+    out = [torch.empty_like(t) for t in tensors] if out is None else list(out)
+    if len(out) != n or any(o.shape != t.shape or o.dtype != t.dtype for o, t in zip(out, tensors)):
+        raise ValueError("each output must have its tensor's shape and dtype")
+    _one_device(tensors[0], *out)
+    outs = _grad_list(out)[1]
+    t = tensors[0]
+    norm = torch.empty((), dtype=torch.float32, device=t.device)
+    with _on_device(t):
+        nws = _abi.lib().fl_b200_grad_norm_workspace_size(n)
+        ws = torch.empty(nws, dtype=torch.uint8, device=t.device)
+        _abi.call("fl_b200_clip_grads", ptrs, outs, numels, dtypes, n, float(max_norm), int(max_kind),
+                  norm.data_ptr(), ws.data_ptr(), nws, _stream(t))
+    return out, norm
 
 
 # ------------------------------------------------------ rows of the vocabulary
