@@ -21,12 +21,12 @@
 // Bound by memory: x and the residual are read and h and y written once
 // forward; x, h, dy and dh are read and dx and dresidual written backward.
 //
-// Column sums.  The rows are dealt to C chunks in order.  A chunk holds
-// whole gate rows, which it finishes itself, and at most two it shares with
-// its neighbours (its first and its last), whose A it leaves in the
-// workspace; a last kernel adds dpre's and dpost's partial sums and those
-// shared A in the order of the chunks.  So every sum has one order, whatever
-// the gate's shape, and no atomics.
+// Column sums.  The rows are dealt to chunks in order.  A chunk holds whole
+// gate rows, which it finishes itself, and at most two it shares with its
+// neighbours (its first and its last), whose A it leaves in the workspace; a
+// last kernel adds dpre's and dpost's partial sums and those shared A in the
+// order of the chunks.  So every sum has one order, whatever the gate's
+// shape, and no atomics.
 #include "row_ladder.cuh"
 
 namespace flb200 {
@@ -43,9 +43,10 @@ struct Sandwich {
   const void *dy, *dh, *hs;
   int64_t ldy, ldh, lds;
   void *dx, *dres, *dpost, *dpre, *dgate;
-  float* ws;        // [chunks][4][cols]: dpre, dpost, A of the first and of the last gate row
-  float4* stats;    // [rows]: 1/rms(x), 1/rms(h), mean(dy w m)
-  uint32_t chunks, per_chunk;
+  float* parts;    // [n_parts][2][cols]: dpre, dpost
+  float* shared;   // [chunks][2][cols]: A of the first and of the last gate row
+  float4* stats;   // [rows]: 1/rms(x), 1/rms(h), mean(dy w m)
+  uint32_t chunks, per_chunk, n_parts;
 };
 
 template <typename T>
@@ -258,11 +259,11 @@ sandwich_bwd_cols_kernel(const __grid_constant__ Sandwich a) {
       dpost = fmaf(a.scale, sum, dpost);
     }
   }
-  float* w = a.ws + (int64_t)chunk * 4 * a.cols + c;
-  w[0] = dpre;
-  w[a.cols] = dpost;
-  w[2ll * a.cols] = shared[0];
-  w[3ll * a.cols] = shared[1];
+  const int64_t at = (int64_t)chunk * 2 * a.cols + c;
+  a.parts[at] = dpre;
+  a.parts[at + a.cols] = dpost;
+  a.shared[at] = shared[0];
+  a.shared[at + a.cols] = shared[1];
 }
 
 // Adds the chunks' partial sums: blockIdx.y == 0 dpre and dpost, y > 0 the
@@ -275,8 +276,8 @@ sandwich_bwd_sum_kernel(const __grid_constant__ Sandwich a) {
   __shared__ float part[2][16][33];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + tx;
-  const int64_t stride = 4ll * a.cols;
-  uint32_t from = 0, to = a.chunks, seg = 0;
+  const int64_t stride = 2ll * a.cols;
+  uint32_t from = 0, to = a.n_parts, seg = 0;
   if (blockIdx.y > 0) {
     const uint32_t edge = blockIdx.y * a.per_chunk;  // the first row of chunk y
     seg = edge / a.per_gate;
@@ -288,15 +289,17 @@ sandwich_bwd_sum_kernel(const __grid_constant__ Sandwich a) {
   }
   float s0 = 0.f, s1 = 0.f;
   if (c < a.cols) {
-    for (uint32_t k = from + ty; k < to; k += 16) {
-      const float* w = a.ws + k * stride + c;
-      if (blockIdx.y == 0) {
-        s0 += w[0];
-        s1 += w[a.cols];
-      } else {
-        // the chunk's first gate row, or its last
-        s0 += w[(seg == k * a.per_chunk / a.per_gate ? 2ll : 3ll) * a.cols];
+    if (blockIdx.y == 0) {
+#pragma unroll 4
+      for (uint32_t k = ty; k < to; k += 16) {
+        s0 += a.parts[k * stride + c];
+        s1 += a.parts[k * stride + a.cols + c];
       }
+    } else {
+      // the chunk's first gate row, or its last
+#pragma unroll 4
+      for (uint32_t k = from + ty; k < to; k += 16)
+        s0 += a.shared[k * stride + (seg == k * a.per_chunk / a.per_gate ? 0 : a.cols) + c];
     }
   }
   part[0][ty][tx] = s0;
@@ -317,14 +320,268 @@ sandwich_bwd_sum_kernel(const __grid_constant__ Sandwich a) {
   }
 }
 
-// Chunks of the column sums: about two CTAs' worth of rows an SM, each at
-// least 8 rows.
-void plan_chunks(int64_t rows, int64_t cols, int sms, uint32_t* chunks, uint32_t* per_chunk) {
-  const int64_t tiles = ceil_div(cols, 128);
-  const int64_t want = std::max<int64_t>(1, ceil_div(8ll * sms, tiles));
-  const int64_t per = std::max<int64_t>(8, ceil_div(rows, want));
-  *per_chunk = (uint32_t)per;
-  *chunks = (uint32_t)ceil_div(rows, per);
+// Sum over the TPR threads of a team (TPR a multiple of 32; its warps at
+// named barrier 1 + team), into every thread, in warp order.  Two halves of
+// `buf` are used in turn, so that no warp overwrites what another still reads.
+template <int TPR, int BLOCK>
+__device__ __forceinline__ float4 team_sum(float4 v, float4* buf, int half) {
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) {
+    v.x += __shfl_xor_sync(0xffffffffu, v.x, off);
+    v.y += __shfl_xor_sync(0xffffffffu, v.y, off);
+    v.z += __shfl_xor_sync(0xffffffffu, v.z, off);
+  }
+  if constexpr (TPR > 32) {
+    constexpr int W = TPR / 32;
+    const int team = threadIdx.x / TPR;
+    float4* h = buf + half * (BLOCK / 32);
+    if ((threadIdx.x & 31) == 0) h[threadIdx.x >> 5] = v;
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(TPR) : "memory");
+    v = h[team * W];
+#pragma unroll
+    for (int i = 1; i < W; ++i) {
+      const float4 o = h[team * W + i];
+      v.x += o.x, v.y += o.y, v.z += o.z;
+    }
+  }
+  return v;
+}
+
+// Rows staged in shared memory: a team of TPR threads takes a chunk of rows,
+// each thread the same VPT packs of every row, whose column sums it holds in
+// registers.  The next row's x, h, dy and dh are copied in by cp.async while
+// this one is worked on (a thread reads only what it copied, so no barrier
+// orders them).  Two barriers a row, for the two sums that hang together.
+// dpost's sums, which only the end of a gate row adds to, lie in shared
+// memory.
+template <typename T, int TPR, int VPT, int BLOCK>
+__global__ void __launch_bounds__(BLOCK, BLOCK <= 256 ? 2 : 1)
+sandwich_bwd_kernel(const __grid_constant__ Sandwich a) {
+  pdl_prologue();
+  constexpr int VW = Elem<T>::kVec;
+  constexpr int TEAMS = BLOCK / TPR;
+  constexpr int STAGE = 4 * VPT * BLOCK;  // packs
+  extern __shared__ uint4 dyn[];
+  __shared__ float4 sums[2 * BLOCK / 32];
+  uint4* stage = dyn + threadIdx.x;                                   // [stage][array][i][thread]
+  float* dpost = reinterpret_cast<float*>(dyn + 2 * STAGE) + threadIdx.x;  // [i][e][thread]
+  const int lane = threadIdx.x % TPR;
+  const uint32_t chunk = blockIdx.x * TEAMS + threadIdx.x / TPR;
+  const int nvec = a.cols / VW;
+  const float inv_n = 1.f / (float)a.cols;
+  const uint32_t r0 = min(a.rows, chunk * a.per_chunk), r1 = min(a.rows, r0 + a.per_chunk);
+  float dpre[VPT][VW], sum[VPT][VW];
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+#pragma unroll
+    for (int e = 0; e < VW; ++e) {
+      dpre[i][e] = sum[i][e] = 0.f;
+      dpost[(i * VW + e) * BLOCK] = 0.f;
+    }
+  }
+  auto fetch = [&](uint32_t row, int st) {
+    const T* src[4] = {static_cast<const T*>(a.x) + row * a.ldx, static_cast<const T*>(a.hs) + row * a.lds,
+                       static_cast<const T*>(a.dy) + row * a.ldy,
+                       a.dh == nullptr ? nullptr : static_cast<const T*>(a.dh) + row * a.ldh};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (src[k] == nullptr) continue;
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        const int vi = lane + i * TPR;
+        if (vi < nvec) cp_async16(stage + st * STAGE + (k * VPT + i) * BLOCK, src[k] + (int64_t)vi * VW);
+      }
+    }
+    cp_async_commit();
+  };
+  if (r0 < r1) fetch(r0, 0);
+  uint32_t seg = r0 / a.per_gate;
+  uint64_t seg_end = (uint64_t)(seg + 1) * a.per_gate;
+  bool first_seg = true;
+  for (uint32_t row = r0; row < r1; ++row) {
+    const int st = (row - r0) & 1;
+    if (row + 1 < r1) {
+      fetch(row + 1, st ^ 1);
+      cp_async_wait_pending<1>();
+    } else {
+      cp_async_wait_all();
+    }
+    const uint4* in = stage + st * STAGE;
+    auto get = [&](int k, int i, float (&f)[VW]) { unpack<T>(in[(k * VPT + i) * BLOCK], f); };
+    const T* gr = a.gate == nullptr ? nullptr : static_cast<const T*>(a.gate) + (int64_t)seg * a.cols;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int vi = lane + i * TPR;
+      if (vi >= nvec) continue;
+      float x[VW], h[VW], dy[VW], w[VW];
+      get(0, i, x);
+      get(1, i, h);
+      get(2, i, dy);
+      unpack<T>(ld_cached(static_cast<const T*>(a.pre) + (int64_t)vi * VW), w);
+#pragma unroll
+      for (int e = 0; e < VW; ++e) {
+        v.x = fmaf(x[e], x[e], v.x);
+        v.y = fmaf(h[e], h[e], v.y);
+        v.z = fmaf(dy[e] * (w[e] + a.off), h[e], v.z);
+      }
+    }
+    v = team_sum<TPR, BLOCK>(v, sums, 0);
+    const float rx = 1.0f / sqrtf(v.x * inv_n + a.eps), rh = 1.0f / sqrtf(v.y * inv_n + a.eps);
+    const float mean = v.z * rh * inv_n;
+    float t[VPT][VW];
+    float4 u = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int vi = lane + i * TPR;
+      if (vi >= nvec) continue;
+      float h[VW], dy[VW], w[VW];
+      get(1, i, h);
+      get(2, i, dy);
+      unpack<T>(ld_cached(static_cast<const T*>(a.pre) + (int64_t)vi * VW), w);
+#pragma unroll
+      for (int e = 0; e < VW; ++e) {
+        const float m = h[e] * rh;
+        dpre[i][e] = fmaf(dy[e], m, dpre[i][e]);
+        t[i][e] = rh * (dy[e] * (w[e] + a.off) - m * mean);
+      }
+      if (a.dh != nullptr) {
+        get(3, i, h);
+#pragma unroll
+        for (int e = 0; e < VW; ++e) t[i][e] += h[e];
+      }
+      st_stream(static_cast<T*>(a.dres) + (int64_t)row * a.cols + (int64_t)vi * VW, pack<T>(t[i]));
+      unpack<T>(ld_cached(static_cast<const T*>(a.post) + (int64_t)vi * VW), w);
+#pragma unroll
+      for (int e = 0; e < VW; ++e) w[e] = a.scale * (w[e] + a.off);
+      if (gr != nullptr) {
+        unpack<T>(ld_cached(gr + (int64_t)vi * VW), dy);
+#pragma unroll
+        for (int e = 0; e < VW; ++e) w[e] *= dy[e];
+      }
+      get(0, i, h);
+#pragma unroll
+      for (int e = 0; e < VW; ++e) {
+        sum[i][e] = fmaf(t[i][e], h[e] * rx, sum[i][e]);
+        t[i][e] *= w[e];
+        u.x = fmaf(t[i][e], h[e], u.x);
+      }
+    }
+    u = team_sum<TPR, BLOCK>(u, sums, 1);
+    const float mean_t = u.x * rx * inv_n;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int vi = lane + i * TPR;
+      if (vi >= nvec) continue;
+      float x[VW];
+      get(0, i, x);
+#pragma unroll
+      for (int e = 0; e < VW; ++e) x[e] = rx * (t[i][e] - x[e] * rx * mean_t);
+      st_stream(static_cast<T*>(a.dx) + (int64_t)row * a.cols + (int64_t)vi * VW, pack<T>(x));
+    }
+    if (row + 1 == seg_end || row + 1 == r1) {  // the gate row ends, or the chunk
+      const bool whole = (uint64_t)seg * a.per_gate >= r0 && (row + 1 == seg_end || r1 == a.rows);
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        const int vi = lane + i * TPR;
+        if (vi >= nvec) continue;
+        const int64_t c = (int64_t)vi * VW;
+        if (gr != nullptr) {
+          float gf[VW], w[VW];
+          unpack<T>(ld_cached(gr + c), gf);
+          unpack<T>(ld_cached(static_cast<const T*>(a.post) + c), w);
+#pragma unroll
+          for (int e = 0; e < VW; ++e) {
+            dpost[(i * VW + e) * BLOCK] = fmaf(a.scale * gf[e], sum[i][e], dpost[(i * VW + e) * BLOCK]);
+            w[e] = a.scale * (w[e] + a.off) * sum[i][e];
+          }
+          if (whole) {
+            st_stream(static_cast<T*>(a.dgate) + (int64_t)seg * a.cols + c, pack<T>(w));
+          } else {
+            float* sh = a.shared + ((int64_t)chunk * 2 + (first_seg ? 0 : 1)) * a.cols + c;
+#pragma unroll
+            for (int e = 0; e < VW; ++e) sh[e] = sum[i][e];
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < VW; ++e) dpost[(i * VW + e) * BLOCK] = a.scale * sum[i][e];
+        }
+#pragma unroll
+        for (int e = 0; e < VW; ++e) sum[i][e] = 0.f;
+      }
+      first_seg = false;
+      ++seg;
+      seg_end += a.per_gate;
+    }
+  }
+  // the CTA's partial sums: its teams' in order
+  if constexpr (TEAMS > 1) {
+    // [array][i][e][thread], over the stages that nothing is on its way to any more
+    float* all = reinterpret_cast<float*>(dyn);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+#pragma unroll
+      for (int e = 0; e < VW; ++e) all[(i * VW + e) * BLOCK + threadIdx.x] = dpre[i][e];
+    __syncthreads();
+    for (int c = threadIdx.x; c < a.cols; c += BLOCK) {
+      const int vi = c / VW, at = ((vi / TPR) * VW + c % VW) * BLOCK + vi % TPR;
+      float p = 0.f, q = 0.f;
+      const float* post = reinterpret_cast<const float*>(dyn + 2 * STAGE);
+      for (int k = 0; k < TEAMS; ++k) {
+        p += all[at + k * TPR];
+        q += post[at + k * TPR];
+      }
+      a.parts[(int64_t)blockIdx.x * 2 * a.cols + c] = p;
+      a.parts[((int64_t)blockIdx.x * 2 + 1) * a.cols + c] = q;
+    }
+  } else {
+    float* part = a.parts + (int64_t)blockIdx.x * 2 * a.cols;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int vi = lane + i * TPR;
+      if (vi >= nvec) continue;
+#pragma unroll
+      for (int e = 0; e < VW; ++e) {
+        part[vi * VW + e] = dpre[i][e];
+        part[a.cols + vi * VW + e] = dpost[(i * VW + e) * BLOCK];
+      }
+    }
+  }
+}
+
+// How the column sums are dealt: `team` threads a row (0: rows by single
+// elements and a second pass), chunks of rows, CTAs.
+struct Plan {
+  int team;
+  uint32_t chunks, per_chunk, n_parts;
+};
+Plan deal(int64_t rows, int64_t teams, int per_cta, int team) {
+  Plan p;
+  p.team = team;
+  p.per_chunk = (uint32_t)ceil_div(rows, std::min(rows, teams));
+  p.chunks = (uint32_t)ceil_div(rows, p.per_chunk);
+  p.n_parts = (uint32_t)ceil_div(p.chunks, per_cta);
+  return p;
+}
+// Teams of 32 to 512 threads of 2 packs, as many as are resident at once (a
+// CTA of 256 threads twice an SM, one of 512 once).
+constexpr int kBwdVpt = 2;
+Plan plan_teams(int64_t rows, int64_t packs, int sms) {
+  int team = 32;
+  while (team < 512 && (int64_t)team * kBwdVpt < packs) team *= 2;
+  const int per_cta = team >= 256 ? 1 : 256 / team;
+  return deal(rows, (int64_t)sms * (team == 512 ? 1 : 2) * per_cta, per_cta, team);
+}
+// About 8 CTAs an SM of 128 columns and at least 8 rows.
+Plan plan_columns(int64_t rows, int64_t cols, int sms) {
+  return deal(rows, std::max<int64_t>(1, std::min(ceil_div(8ll * sms, ceil_div(cols, 128)), ceil_div(rows, 8))), 1, 0);
+}
+// Both plans' needs (which of them a call takes hangs on its alignment too).
+size_t bwd_workspace(int64_t rows, int64_t cols, int64_t packs, int sms) {
+  const Plan a = plan_teams(rows, packs, sms), b = plan_columns(rows, cols, sms);
+  return (size_t)rows * sizeof(float4) +
+         (size_t)2 * cols * sizeof(float) * std::max<size_t>((size_t)a.chunks + a.n_parts, (size_t)b.chunks + b.n_parts);
 }
 
 template <typename T>
@@ -345,10 +602,44 @@ int launch_fwd(const Sandwich& a, const DeviceInfo& dev, cudaStream_t stream) {
   return launch_status();
 }
 
+template <typename T, int TPR>
+int launch_teams(const Sandwich& a, cudaStream_t stream) {
+  constexpr int BLOCK = TPR >= 256 ? TPR : 256;
+  constexpr int VW = Elem<T>::kVec;
+  // two stages of four operands, and dpost's sums
+  constexpr int smem = (2 * 4 * kBwdVpt * 16 + kBwdVpt * VW * 4) * BLOCK;
+  auto kern = sandwich_bwd_kernel<T, TPR, kBwdVpt, BLOCK>;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return launch_status();
+  launch_k(kern, a.n_parts, BLOCK, smem, stream, a);
+  return launch_status();
+}
+
 template <typename T>
-int launch_bwd(Sandwich a, const DeviceInfo& dev, cudaStream_t stream) {
-  launch_k(sandwich_bwd_rows_kernel<T>, (unsigned)std::min<int64_t>(a.rows, 4ll * dev.sm_count), 512, 0, stream, a);
-  launch_k(sandwich_bwd_cols_kernel<T>, dim3((unsigned)ceil_div(a.cols, 128), a.chunks), 128, 0, stream, a);
+int launch_bwd(Sandwich a, const DeviceInfo& dev, float* ws, cudaStream_t stream) {
+  constexpr int VW = Elem<T>::kVec;
+  const int64_t packs = a.cols / VW;
+  const bool staged = packs <= 512 * kBwdVpt && a.cols % VW == 0 && a.ldx % VW == 0 && a.lds % VW == 0 &&
+                      a.ldy % VW == 0 && a.ldh % VW == 0 && aligned16(a.x) && aligned16(a.hs) && aligned16(a.dy) &&
+                      aligned16(a.dh) && aligned16(a.post) && aligned16(a.pre) && aligned16(a.gate) &&
+                      aligned16(a.dx) && aligned16(a.dres) && aligned16(a.dgate);
+  const Plan p = staged ? plan_teams(a.rows, packs, dev.sm_count) : plan_columns(a.rows, a.cols, dev.sm_count);
+  a.chunks = p.chunks, a.per_chunk = p.per_chunk, a.n_parts = p.n_parts;
+  a.parts = ws;
+  a.shared = ws + (int64_t)2 * p.n_parts * a.cols;
+  int st = FL_B200_OK;
+  switch (p.team) {
+    case 0:
+      launch_k(sandwich_bwd_rows_kernel<T>, (unsigned)std::min<int64_t>(a.rows, 4ll * dev.sm_count), 512, 0, stream, a);
+      launch_k(sandwich_bwd_cols_kernel<T>, dim3((unsigned)ceil_div(a.cols, 128), a.chunks), 128, 0, stream, a);
+      break;
+    case 32: st = launch_teams<T, 32>(a, stream); break;
+    case 64: st = launch_teams<T, 64>(a, stream); break;
+    case 128: st = launch_teams<T, 128>(a, stream); break;
+    case 256: st = launch_teams<T, 256>(a, stream); break;
+    default: st = launch_teams<T, 512>(a, stream); break;
+  }
+  if (st != FL_B200_OK) return st;
   launch_k(sandwich_bwd_sum_kernel<T>, dim3((unsigned)ceil_div(a.cols, 32), a.gate ? a.chunks : 1), 512, 0, stream,
            a);
   return launch_status();
@@ -410,9 +701,9 @@ FL_B200_API size_t fl_b200_sandwich_norm_bwd_workspace_size(int64_t rows, int64_
   using namespace flb200;
   DeviceInfo dev;
   if (rows <= 0 || cols <= 0 || current_device_info(&dev) != FL_B200_OK) return 0;
-  uint32_t chunks, per;
-  plan_chunks(rows, cols, dev.sm_count, &chunks, &per);
-  return (size_t)rows * sizeof(float4) + (size_t)chunks * 4 * cols * sizeof(float);
+  if (rows > 0x7fffffff || cols > 0x7fffff00) return 0;
+  // (a pack holds 4 or 8 elements: the larger need of the two)
+  return std::max(bwd_workspace(rows, cols, cols / 4, dev.sm_count), bwd_workspace(rows, cols, cols / 8, dev.sm_count));
 }
 
 FL_B200_API int fl_b200_sandwich_norm_bwd(const void* dy, int64_t ld_dy, const void* dh, int64_t ld_dh,
@@ -451,13 +742,12 @@ FL_B200_API int fl_b200_sandwich_norm_bwd(const void* dy, int64_t ld_dy, const v
   if (workspace == nullptr || workspace_bytes < fl_b200_sandwich_norm_bwd_workspace_size(rows, cols))
     return FL_B200_ERR_WORKSPACE;
   if (!aligned16(workspace)) return FL_B200_ERR_MISALIGNED;
-  plan_chunks(rows, cols, dev.sm_count, &a.chunks, &a.per_chunk);
   a.stats = static_cast<float4*>(workspace);
-  a.ws = reinterpret_cast<float*>(a.stats + rows);
+  float* ws = reinterpret_cast<float*>(a.stats + rows);
   a.dy = dy, a.ldy = ld_dy, a.dh = dh, a.ldh = ld_dh, a.x = x, a.ldx = ld_x, a.hs = h, a.lds = ld_h;
   a.post = post, a.pre = pre, a.dx = dx, a.dres = dresidual, a.dpost = dpost, a.dpre = dpre, a.dgate = dgate;
   return dispatch_float(dtype, [&](auto tag) -> int {
-    return launch_bwd<decltype(tag)>(a, dev, static_cast<cudaStream_t>(stream));
+    return launch_bwd<decltype(tag)>(a, dev, ws, static_cast<cudaStream_t>(stream));
   });
 }
 

@@ -11,8 +11,8 @@
 //   dx_j = scale (1 - tanh^2) y_j (dy_j - sum over the span of y dy).
 //
 // Bound by memory: the span is read once, the row written once.  A row is
-// held in registers (at most 4 packs a thread, one warp for 128 packs, up to
-// 1024 threads), its scores as fp32 between the passes.  Rows need not begin
+// held in registers (a warp up to 256 packs, then a CTA of 4 packs a thread),
+// its scores as fp32 between the passes.  Rows need not begin
 // on a 16-byte boundary: they are walked by the aligned packs that cover
 // them, elements outside masked and the row's first and last pack stored by
 // element.  (An aligned pack that holds one byte of the row lies in that
@@ -56,6 +56,7 @@ struct SpanArgs {
   int64_t ldo;
   uint32_t rows, q_len, heads;
   int cols;
+  uint32_t unit;  // rows a warp takes in order
   float scale, cap;
   // backward
   const void* dy;
@@ -64,26 +65,57 @@ struct SpanArgs {
   int64_t ldy;
 };
 
+struct Raw {
+  int lo, hi, pos;
+  float slope;
+};
 struct Row {
-  int lo, hi;      // clamped; lo == hi: nothing is seen
+  int lo, hi;  // clamped; lo == hi: nothing is seen
   float pos, slope;
+  __device__ __forceinline__ Row(const Raw& r, int cols)
+      : lo(max(r.lo, 0)), hi(min(r.hi, cols)), pos((float)r.pos), slope(r.slope) {
+    if (hi <= lo) lo = hi = 0;
+  }
+};
+// Row `row`'s head and query, the latter kept up to date while rows are
+// walked in order (a division a row is 5 % of a short row's instructions).
+struct Walk {
+  uint32_t row, q;
+  const int32_t *span, *pos;
+  float slope;
+  __device__ __forceinline__ void to(const SpanArgs& a, uint32_t at) {
+    row = at;
+    const uint32_t bh = row / a.q_len;
+    q = row - bh * a.q_len;
+    const uint32_t b = bh / a.heads, h = bh - b * a.heads;
+    span = a.spans + b * a.spb + q * a.spq;
+    pos = a.pos == nullptr ? nullptr : a.pos + b * a.pb + q * a.pq;
+    slope = a.slopes == nullptr ? 0.f : __ldg(a.slopes + h);
+  }
+  __device__ __forceinline__ void next(const SpanArgs& a) {
+    if (q + 1 == a.q_len) return to(a, row + 1);
+    ++row;
+    ++q;
+    span += a.spq;
+    if (pos != nullptr) pos += a.pq;
+  }
+  // What the row's metadata hold, not looked at yet: the loads are on their
+  // way while other work goes on.
+  __device__ __forceinline__ Raw read(const SpanArgs& a) const {
+    Raw r;
+    r.lo = __ldg(span);
+    r.hi = __ldg(span + 1);
+    r.pos = 0;
+    if (a.slopes != nullptr) r.pos = pos != nullptr ? __ldg(pos) : (int)(q + (uint32_t)a.cols - a.q_len);
+    r.slope = slope;
+    return r;
+  }
+  __device__ __forceinline__ Row get(const SpanArgs& a) const { return Row(read(a), a.cols); }
 };
 __device__ __forceinline__ Row row_of(const SpanArgs& a, uint32_t row) {
-  const uint32_t bh = row / a.q_len, q = row - bh * a.q_len;
-  const uint32_t b = bh / a.heads, h = bh - b * a.heads;
-  const int32_t* s = a.spans + b * a.spb + q * a.spq;
-  Row r;
-  r.lo = max(__ldg(s), 0);
-  r.hi = min(__ldg(s + 1), a.cols);
-  if (r.hi <= r.lo) r.lo = r.hi = 0;
-  r.pos = 0.f;
-  r.slope = 0.f;
-  if (a.slopes != nullptr) {
-    r.slope = __ldg(a.slopes + h);
-    r.pos = a.pos != nullptr ? (float)__ldg(a.pos + b * a.pb + q * a.pq)
-                             : (float)((int64_t)q + a.cols - (int64_t)a.q_len);
-  }
-  return r;
+  Walk w;
+  w.to(a, row);
+  return w.get(a);
 }
 
 struct Score {
@@ -103,47 +135,98 @@ struct Score {
     const float q = rcp(1.f + ex2(x * mul));  // (1 - tanh) / 2
     return 4.f * q * (1.f - q);
   }
-};
-
-// N consecutive elements of T at a 16-byte boundary (N * size a multiple of 16).
-template <typename T, int N>
-struct Elems {
-  static constexpr int VW = Elem<T>::kVec;
-  uint4 w[N / VW];
-  __device__ __forceinline__ void load(const T* p) {
-#pragma unroll
-    for (int i = 0; i < N / VW; ++i) w[i] = ld_stream(p + i * VW);
+  // (1 - tanh) / 2 of a pair of x.
+  __device__ __forceinline__ uint64_t half_of(uint64_t x) const {
+    const uint64_t t = f2_mul(x, f2_make(mul, mul));
+    const uint64_t d = f2_add(f2_make(ex2(f2_lo(t)), ex2(f2_hi(t))), f2_make(1.f, 1.f));
+    return f2_make(rcp(f2_lo(d)), rcp(f2_hi(d)));
   }
-  __device__ __forceinline__ void clear() {
+  // P pairs in place, the first element at `key`.  Choices are made for a
+  // pack, not for each element.
+  template <int P>
+  __device__ __forceinline__ void pack(uint64_t (&z)[P], int key, const Row& r) const {
+    if (cap != 0.f) {
+      const uint64_t m = f2_make(-2.f * cap, -2.f * cap), c = f2_make(cap, cap);
 #pragma unroll
-    for (int i = 0; i < N / VW; ++i) w[i] = make_uint4(0, 0, 0, 0);
-  }
-  __device__ __forceinline__ void to(float (&f)[N]) const {
+      for (int e = 0; e < P; ++e) z[e] = f2_fma(half_of(z[e]), m, c);
+    } else {
 #pragma unroll
-    for (int i = 0; i < N / VW; ++i) {
-      float g[VW];
-      unpack<T>(w[i], g);
+      for (int e = 0; e < P; ++e) z[e] = f2_mul(z[e], f2_make(mul, mul));
+    }
+    if (biased) {
+      const float d = r.pos - (float)key;
 #pragma unroll
-      for (int e = 0; e < VW; ++e) f[i * VW + e] = g[e];
+      for (int e = 0; e < P; ++e)
+        z[e] = f2_make(fmaf(-r.slope, fabsf(d - (float)(2 * e)), f2_lo(z[e])),
+                       fmaf(-r.slope, fabsf(d - (float)(2 * e + 1)), f2_hi(z[e])));
     }
   }
 };
-// Stores f at virtual elements [v, v + N) of a row that holds [first, last).
+
+// N consecutive elements of T at a 16-byte boundary (N * size a multiple of
+// 16), as fp32 pairs when they are worked on.
 template <typename T, int N>
-__device__ __forceinline__ void store(T* row, int v, int first, int last, const float (&f)[N]) {
+struct Elems {
+  static constexpr int VW = Elem<T>::kVec;
+  static constexpr int WORDS = N * (int)sizeof(T) / 4;
+  uint32_t w[WORDS];
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < N / VW; ++i) {
+      word(i, ld_stream(p + i * VW));
+    }
+  }
+  __device__ __forceinline__ void word(int i, const uint4& u) {
+    w[4 * i] = u.x, w[4 * i + 1] = u.y, w[4 * i + 2] = u.z, w[4 * i + 3] = u.w;
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) w[i] = 0;
+  }
+  // Zeros but for elements [from, to).
+  __device__ __forceinline__ void keep(int from, int to) {
+    constexpr int P = 4 / (int)sizeof(T);  // elements a word
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) {
+      uint32_t mask = 0;
+#pragma unroll
+      for (int e = 0; e < P; ++e)
+        if (i * P + e >= from && i * P + e < to) mask |= (P == 1 ? 0xffffffffu : 0xffffu << (16 * e));
+      w[i] &= mask;
+    }
+  }
+  __device__ __forceinline__ void to(uint64_t (&f)[N / 2]) const {
+#pragma unroll
+    for (int e = 0; e < N / 2; ++e) {
+      if constexpr (std::is_same<T, float>::value) {
+        f[e] = f2_make(__uint_as_float(w[2 * e]), __uint_as_float(w[2 * e + 1]));
+      } else {
+        f[e] = pair_from_bits<T>(w[e]);
+      }
+    }
+  }
+};
+// Stores pairs at virtual elements [v, v + N) of a row that holds [first, last).
+template <typename T, int N>
+__device__ __forceinline__ void store(T* row, int v, int first, int last, const uint64_t (&f)[N / 2]) {
   constexpr int VW = Elem<T>::kVec;
   if (v >= first && v + N <= last) {
 #pragma unroll
     for (int i = 0; i < N / VW; ++i) {
-      float g[VW];
-#pragma unroll
-      for (int e = 0; e < VW; ++e) g[e] = f[i * VW + e];
-      st_stream(row + v + i * VW, pack<T>(g));
+      uint4 u;
+      if constexpr (std::is_same<T, float>::value) {
+        u = make_uint4(__float_as_uint(f2_lo(f[2 * i])), __float_as_uint(f2_hi(f[2 * i])),
+                       __float_as_uint(f2_lo(f[2 * i + 1])), __float_as_uint(f2_hi(f[2 * i + 1])));
+      } else {
+        u = make_uint4(pair_to_bits<T>(f[4 * i]), pair_to_bits<T>(f[4 * i + 1]), pair_to_bits<T>(f[4 * i + 2]),
+                       pair_to_bits<T>(f[4 * i + 3]));
+      }
+      st_stream(row + v + i * VW, u);
     }
   } else {
 #pragma unroll
     for (int e = 0; e < N; ++e)
-      if (v + e >= first && v + e < last) row[v + e] = Elem<T>::from_f(f[e]);
+      if (v + e >= first && v + e < last) row[v + e] = Elem<T>::from_f(e % 2 ? f2_hi(f[e / 2]) : f2_lo(f[e / 2]));
   }
 }
 
@@ -154,87 +237,284 @@ __device__ __forceinline__ int shift_of(const T* p) {
   return (int)((reinterpret_cast<uintptr_t>(p) & 15u) / sizeof(T));
 }
 
-// TPR threads a row, VPT packs each.
-template <typename TI, typename TO, int TPR, int VPT, int BLOCK>
-__global__ void __launch_bounds__(BLOCK, BLOCK <= 256 ? 4 : 1)
+// Where a row's packs lie: its own (virtual) elements [first, last), its
+// span's [lo, hi), the span's packs p0 ... p0 + count - 1.
+template <int N>
+struct Place {
+  int first, last, lo, hi, p0, count;
+  __device__ __forceinline__ Place(const Row& r, int shift, int cols)
+      : first(shift), last(shift + cols), lo(shift + r.lo), hi(shift + r.hi), p0(lo / N),
+        count(r.hi > r.lo ? (hi + N - 1) / N - p0 : 0) {}
+  __device__ __forceinline__ bool inside(int at) const { return at >= lo && at + N <= hi; }
+  // Pairs of the pack at `at`: `other` outside the span.
+  __device__ __forceinline__ void mask(uint64_t (&z)[N / 2], int at, float other) const {
+#pragma unroll
+    for (int e = 0; e < N / 2; ++e)
+      z[e] = f2_make(at + 2 * e >= lo && at + 2 * e < hi ? f2_lo(z[e]) : other,
+                     at + 2 * e + 1 >= lo && at + 2 * e + 1 < hi ? f2_hi(z[e]) : other);
+  }
+};
+// Zeros in the packs where nothing is seen, by the TPR threads of a row.
+template <typename TO, int N, int TPR>
+__device__ __forceinline__ void clear_outside(TO* row, const Place<N>& p, int lane) {
+  const int begin = p.first > 0 ? 1 : 0, end = p.last / N;     // whole packs
+  const int p0 = p.count ? max(p.p0, begin) : end;             // of them [begin, p0) and [p1, end)
+  const int p1 = p.count ? p.p0 + p.count : end;
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  const int before = max(p0 - begin, 0), all = before + max(end - p1, 0);
+#pragma unroll 2
+  for (int j = lane; j < all; j += TPR) {
+    const int v = j < before ? begin + j : p1 + (j - before);
+#pragma unroll
+    for (int i = 0; i < N / Elem<TO>::kVec; ++i) st_stream(row + v * N + i * Elem<TO>::kVec, zero);
+  }
+  // the row's first and last pack where they are not whole
+  if (p.first > 0 && (p.count == 0 || p.p0 > 0) && lane >= p.first && lane < N && lane < p.last)
+    row[lane] = Elem<TO>::from_f(0.f);
+  if (p.last % N != 0 && end >= begin && (p.count == 0 || p1 <= end) && lane < p.last - end * N)
+    row[end * N + lane] = Elem<TO>::from_f(0.f);
+}
+// Scores of the pack at virtual element `at` from its elements, -inf outside
+// the span; returns the larger of m and their maximum.  (What lies outside is
+// scored too and then dropped.)
+template <int N>
+__device__ __forceinline__ float scores_of(uint64_t (&z)[N / 2], int at, const Place<N>& p, const Row& r,
+                                           const Score& score, float m) {
+  score.pack<N / 2>(z, at - p.first, r);
+  if (!p.inside(at)) p.mask(z, at, -INFINITY);
+#pragma unroll
+  for (int e = 0; e < N / 2; ++e) m = fmax3(m, f2_lo(z[e]), f2_hi(z[e]));
+  return m;
+}
+// Turns scores into exponentials of their differences from m; the sum.  One
+// FMA an element: the rounding of m log2 e is a factor all of them share.  A
+// maximum that could overflow there is subtracted first.
+template <int N, int VPT, int TPR>
+__device__ __forceinline__ float exps_of(uint64_t (&z)[VPT][N / 2], int count, float m) {
+  float shift = m * kLog2e;
+  if (!(fabsf(m) < 1e30f)) {
+    shift = 0.f;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+      if (i * TPR < count) {
+#pragma unroll
+        for (int e = 0; e < N / 2; ++e) z[i][e] = f2_make(f2_lo(z[i][e]) - m, f2_hi(z[i][e]) - m);
+      }
+  }
+  const uint64_t l = f2_make(kLog2e, kLog2e), c = f2_make(-shift, -shift);
+  uint64_t s[2] = {f2_make(0.f, 0.f), f2_make(0.f, 0.f)};
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    if (i * TPR < count) {
+#pragma unroll
+      for (int e = 0; e < N / 2; ++e) {
+        const uint64_t t = f2_fma(z[i][e], l, c);
+        z[i][e] = f2_make(ex2(f2_lo(t)), ex2(f2_hi(t)));
+        s[e & 1] = f2_add(s[e & 1], z[i][e]);
+      }
+    }
+  }
+  s[0] = f2_add(s[0], s[1]);
+  return f2_lo(s[0]) + f2_hi(s[0]);
+}
+// Exponentials times inv, stored.  Outside the span they are 0, but 0 times
+// an inv that is not finite is not.
+template <typename TO, int N>
+__device__ __forceinline__ void put(TO* out, uint64_t (&z)[N / 2], int at, const Place<N>& p, float inv) {
+#pragma unroll
+  for (int e = 0; e < N / 2; ++e) z[e] = f2_mul(z[e], f2_make(inv, inv));
+  if (!(inv < 3e38f) && !p.inside(at)) p.mask(z, at, 0.f);
+  store<TO, N>(out, at, p.first, p.last, z);
+}
+
+// A warp takes `unit` rows in order, then those `unit` times the grid's warps
+// further on (so that rows that see little and rows that see much are spread).
+struct Rows {
+  Walk w;
+  uint32_t left;  // rows of this unit after this one
+  bool more;
+  __device__ __forceinline__ explicit Rows(const SpanArgs& a) {
+    const uint32_t unit = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+    more = (uint64_t)unit * a.unit < a.rows;
+    left = a.unit - 1;
+    if (more) w.to(a, unit * a.unit);
+  }
+  __device__ __forceinline__ void next(const SpanArgs& a) {
+    if (w.row + 1 >= a.rows) {
+      more = false;
+    } else if (left > 0) {
+      --left;
+      w.next(a);
+    } else {
+      const uint64_t to = (uint64_t)w.row + 1 - a.unit + (uint64_t)gridDim.x * (blockDim.x >> 5) * a.unit;
+      more = to < a.rows;
+      left = a.unit - 1;
+      if (more) w.to(a, (uint32_t)to);
+    }
+  }
+};
+
+// A warp a row.  Scores lie in shared memory, fp32, between the passes (a
+// lane reads only what it wrote, so nothing waits for anything): loops whose
+// length is the span's, few registers and 24 warps an SM, where scores in
+// registers gave code for every length, which a short span skipped at half
+// the price of running it, and 16 warps (2048 keys, spans of 200: 670 us
+// against ... for 524288 rows).  The first packs of the next row are loaded
+// while this one's sums go through the warp, and its span before that.
+template <typename TI, typename TO>
+__global__ void __launch_bounds__(256, 3)
+span_softmax_warp_kernel(const __grid_constant__ SpanArgs a, int room) {
+  pdl_prologue();
+  constexpr int N = Elem<TI>::kVec;
+  constexpr int Q = N / 4;  // quads of scores a pack
+  extern __shared__ float4 dyn[];
+  const int lane = threadIdx.x & 31;
+  // quad k of pack v at [k][v]: neighbouring packs' quads are neighbours.
+  // Lanes past the span's last pack go along (their scores are -inf), so
+  // that no pass asks for each lane; room is a multiple of 32.
+  float4* mine = dyn + (threadIdx.x >> 5) * room * Q + lane;
+  Rows rows(a);
+  if (!rows.more) return;
+  const Score score(a);
+  uint32_t row = rows.w.row;
+  Row r = rows.w.get(a);
+  rows.next(a);
+  Raw ahead = rows.more ? rows.w.read(a) : Raw{0, 0, 0, 0.f};
+  Elems<TI, N> v[2];
+  v[0].clear();
+  v[1].clear();
+  // packs at and at + 32 of a row's span
+  auto load = [&](const TI* xr, int at, int count) {
+    if (at < count) v[0].load(xr + at * N);
+    if (at + 32 < count) v[1].load(xr + (at + 32) * N);
+  };
+  auto place = [&](uint32_t rw, const Row& rr) {
+    return Place<N>(rr, shift_of(static_cast<const TI*>(a.x) + rw * a.ldx), a.cols);
+  };
+  auto span_at = [&](uint32_t rw, const Place<N>& p) {
+    return static_cast<const TI*>(a.x) + rw * a.ldx + (p.p0 * N - p.first);
+  };
+  Place<N> p = place(row, r);
+  const TI* xr = span_at(row, p);
+  load(xr, lane, p.count);
+  while (true) {
+    TO* out = static_cast<TO*>(a.out) + row * a.ldo - p.first;
+    clear_outside<TO, N, 32>(out, p, lane);
+    float m = -INFINITY;
+    int at = (p.p0 + lane) * N;
+    float4* z4 = mine;
+    auto keep = [&](const Elems<TI, N>& in) {
+      uint64_t z[N / 2];
+      in.to(z);
+      m = scores_of<N>(z, at, p, r, score, m);
+#pragma unroll
+      for (int k = 0; k < Q; ++k)
+        z4[k * room] = make_float4(f2_lo(z[2 * k]), f2_hi(z[2 * k]), f2_lo(z[2 * k + 1]), f2_hi(z[2 * k + 1]));
+      z4 += 32;
+      at += 32 * N;
+    };
+    for (int done = 0; done < p.count; done += 64) {
+      const Elems<TI, N> v0 = v[0], v1 = v[1];
+      load(xr, done + 64 + lane, p.count);
+      keep(v0);
+      if (done + 32 < p.count) keep(v1);
+    }
+    const bool more = rows.more;
+    const uint32_t then = rows.w.row;
+    const Row next(ahead, a.cols);
+    Place<N> then_p = p;
+    if (more) {
+      then_p = place(then, next);
+      xr = span_at(then, then_p);
+      load(xr, lane, then_p.count);
+      rows.next(a);
+      if (rows.more) ahead = rows.w.read(a);
+    }
+    m = group_reduce_warp<FastMaxOp, 32>(m);
+    // one FMA an element: the rounding of m log2 e is a factor all of them
+    // share; a maximum that could overflow there is subtracted first
+    float c = -m * kLog2e;
+    if (!(fabsf(m) < 1e30f)) {
+      c = 0.f;
+      z4 = mine;
+      for (int done = 0; done < p.count; done += 32, z4 += 32)
+        for (int k = 0; k < Q; ++k) {
+          const float4 f = z4[k * room];
+          z4[k * room] = make_float4(f.x - m, f.y - m, f.z - m, f.w - m);
+        }
+    }
+    const uint64_t l2 = f2_make(kLog2e, kLog2e), c2 = f2_make(c, c);
+    uint64_t s2[2] = {f2_make(0.f, 0.f), f2_make(0.f, 0.f)};
+    z4 = mine;
+    for (int done = 0; done < p.count; done += 32, z4 += 32) {
+#pragma unroll
+      for (int k = 0; k < Q; ++k) {
+        float4 f = z4[k * room];
+        const uint64_t t0 = f2_fma(f2_make(f.x, f.y), l2, c2), t1 = f2_fma(f2_make(f.z, f.w), l2, c2);
+        f = make_float4(ex2(f2_lo(t0)), ex2(f2_hi(t0)), ex2(f2_lo(t1)), ex2(f2_hi(t1)));
+        s2[0] = f2_add(s2[0], f2_make(f.x, f.y));
+        s2[1] = f2_add(s2[1], f2_make(f.z, f.w));
+        z4[k * room] = f;
+      }
+    }
+    s2[0] = f2_add(s2[0], s2[1]);
+    const float inv = 1.f / group_reduce_warp<SumOp, 32>(f2_lo(s2[0]) + f2_hi(s2[0]));
+    z4 = mine;
+    at = (p.p0 + lane) * N;
+    for (int left = p.count - lane; left > 0; left -= 32, z4 += 32, at += 32 * N) {
+      uint64_t z[N / 2];
+#pragma unroll
+      for (int k = 0; k < Q; ++k) {
+        const float4 f = z4[k * room];
+        z[2 * k] = f2_make(f.x, f.y);
+        z[2 * k + 1] = f2_make(f.z, f.w);
+      }
+      put<TO, N>(out, z, at, p, inv);
+    }
+    if (!more) return;
+    row = then;
+    r = next;
+    p = then_p;
+  }
+}
+
+// TPR threads a row, VPT packs each, a CTA a row.
+template <typename TI, typename TO, int TPR, int VPT>
+__global__ void __launch_bounds__(TPR, TPR <= 256 ? 4 : 1)
 span_softmax_kernel(const __grid_constant__ SpanArgs a) {
   pdl_prologue();
   constexpr int N = Elem<TI>::kVec;
-  constexpr int RPB = BLOCK / TPR;
-  __shared__ float smem[BLOCK / 32];
-  const int lane = threadIdx.x % TPR;
-  const uint64_t row64 = (uint64_t)blockIdx.x * RPB + threadIdx.x / TPR;
-  const bool ok = row64 < a.rows;
-  const uint32_t row = ok ? (uint32_t)row64 : a.rows - 1;
+  __shared__ float smem[TPR / 32];
+  const int lane = threadIdx.x;
+  const uint32_t row = blockIdx.x;
   const Row r = row_of(a, row);
   const Score score(a);
   const TI* xr = static_cast<const TI*>(a.x) + row * a.ldx;
   const int shift = shift_of(xr);
-  xr -= shift;
   TO* out = static_cast<TO*>(a.out) + row * a.ldo - shift;
-  const int first = shift, last = shift + a.cols;  // of the row, virtual
-  const int lo = shift + r.lo, hi = shift + r.hi;  // of the span
-  const int p0 = lo / N, n = (hi + N - 1) / N - p0;   // the span's packs
-  const int count = r.hi > r.lo ? n : 0;
+  const Place<N> p(r, shift, a.cols);
+  xr += (int64_t)p.p0 * N - shift;
   Elems<TI, N> v[VPT];
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
-    const int vi = lane + i * TPR;
-    if (ok && vi < count) v[i].load(xr + (int64_t)(p0 + vi) * N);
+    if (lane + i * TPR < p.count) v[i].load(xr + (int64_t)(lane + i * TPR) * N);
     else v[i].clear();
   }
-  if (ok) {  // what is not seen is 0
-    float zero[N];
-#pragma unroll
-    for (int e = 0; e < N; ++e) zero[e] = 0.f;
-    const int packs = (last + N - 1) / N;
-    const int until = count ? p0 : packs;
-    for (int p = lane; p < until; p += TPR) store<TO, N>(out, p * N, first, last, zero);
-    if (count)
-      for (int p = p0 + n + lane; p < packs; p += TPR) store<TO, N>(out, p * N, first, last, zero);
-  }
-  float z[VPT][N];
+  clear_outside<TO, N, TPR>(out, p, lane);
+  uint64_t z[VPT][N / 2];
   float m = -INFINITY;
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
-    const int vi = lane + i * TPR;
-    if (i * TPR < count) {
-      const int at = (p0 + vi) * N;
-      float f[N];
-      v[i].to(f);
-#pragma unroll
-      for (int e = 0; e < N; ++e) {
-        const bool in = at + e >= lo && at + e < hi;
-        z[i][e] = in ? score(f[e], at + e - shift, r) : -INFINITY;
-        m = fmaxf(m, z[i][e]);
-      }
+    if (i * TPR < p.count) {
+      v[i].to(z[i]);
+      m = scores_of<N>(z[i], (p.p0 + lane + i * TPR) * N, p, r, score, m);
     }
   }
-  m = row_reduce<FastMaxOp, TPR, BLOCK>(m, smem);
-  float s = 0.f;
+  m = row_reduce<FastMaxOp, TPR, TPR>(m, smem);
+  const float inv = 1.f / row_reduce<SumOp, TPR, TPR>(exps_of<N, VPT, TPR>(z, p.count, m), smem);
 #pragma unroll
-  for (int i = 0; i < VPT; ++i) {
-    if (i * TPR < count) {
-#pragma unroll
-      for (int e = 0; e < N; ++e) {
-        z[i][e] = exp_of(z[i][e] - m);
-        s += z[i][e];
-      }
-    }
-  }
-  s = row_reduce<SumOp, TPR, BLOCK>(s, smem);
-  const float inv = 1.f / s;
-#pragma unroll
-  for (int i = 0; i < VPT; ++i) {
-    const int vi = lane + i * TPR;
-    if (ok && vi < count) {
-      const int at = (p0 + vi) * N;
-      float f[N];
-#pragma unroll
-      for (int e = 0; e < N; ++e) f[e] = at + e >= lo && at + e < hi ? z[i][e] * inv : 0.f;
-      store<TO, N>(out, at, first, last, f);
-    }
-  }
+  for (int i = 0; i < VPT; ++i)
+    if (lane + i * TPR < p.count) put<TO, N>(out, z[i], (p.p0 + lane + i * TPR) * N, p, inv);
 }
 
 // Rows of any length and alignment: a CTA a row, the span read twice.
@@ -273,87 +553,189 @@ span_softmax_loop_kernel(const __grid_constant__ SpanArgs a) {
   }
 }
 
+// One row of the gradient by TPR threads (the CTA, or a warp of it).
 // TI: x's and dx's type, TY: y's and dy's.
-template <typename TI, typename TY, int TPR, int VPT, int BLOCK>
-__global__ void __launch_bounds__(BLOCK, BLOCK <= 256 ? 2 : 1)
-span_softmax_bwd_kernel(const __grid_constant__ SpanArgs a) {
-  pdl_prologue();
+template <typename TI, typename TY, int TPR, int VPT>
+__device__ __forceinline__ void span_bwd_row(const SpanArgs& a, uint32_t row, const Row& r, const Score& score,
+                                             int lane, float* smem) {
   constexpr int N = Elem<TI>::kVec;
-  constexpr int RPB = BLOCK / TPR;
-  __shared__ float smem[BLOCK / 32];
-  const int lane = threadIdx.x % TPR;
-  const uint64_t row64 = (uint64_t)blockIdx.x * RPB + threadIdx.x / TPR;
-  const bool ok = row64 < a.rows;
-  const uint32_t row = ok ? (uint32_t)row64 : a.rows - 1;
-  const Row r = row_of(a, row);
-  const Score score(a);
   const bool capped = score.cap != 0.f;
   TI* out = static_cast<TI*>(a.out) + row * a.ldo;
   const int shift = shift_of(out);
   out -= shift;
-  const TY* yr = static_cast<const TY*>(a.y) + row * a.ldy - shift;
-  const TY* dr = static_cast<const TY*>(a.dy) + row * a.ldd - shift;
-  const TI* xr = static_cast<const TI*>(a.x) + (capped ? row * a.ldx - shift : 0);
-  const int first = shift, last = shift + a.cols;
-  const int lo = shift + r.lo, hi = shift + r.hi;
-  const int p0 = lo / N, n = (hi + N - 1) / N - p0;
-  const int count = r.hi > r.lo ? n : 0;
+  const Place<N> p(r, shift, a.cols);
+  const int64_t skip = (int64_t)p.p0 * N - shift;
+  const TY* yr = static_cast<const TY*>(a.y) + row * a.ldy + skip;
+  const TY* dr = static_cast<const TY*>(a.dy) + row * a.ldd + skip;
+  const TI* xr = static_cast<const TI*>(a.x) + (capped ? row * a.ldx + skip : 0);
   Elems<TY, N> y[VPT], d[VPT];
   Elems<TI, N> x[VPT];
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     const int vi = lane + i * TPR;
-    if (ok && vi < count) {
-      y[i].load(yr + (int64_t)(p0 + vi) * N);
-      d[i].load(dr + (int64_t)(p0 + vi) * N);
-      if (capped) x[i].load(xr + (int64_t)(p0 + vi) * N);
+    if (vi < p.count) {
+      y[i].load(yr + (int64_t)vi * N);
+      d[i].load(dr + (int64_t)vi * N);
+      if (capped) x[i].load(xr + (int64_t)vi * N);
     } else {
       y[i].clear();
       d[i].clear();
     }
   }
-  if (ok) {
-    float zero[N];
-#pragma unroll
-    for (int e = 0; e < N; ++e) zero[e] = 0.f;
-    const int packs = (last + N - 1) / N;
-    const int until = count ? p0 : packs;
-    for (int p = lane; p < until; p += TPR) store<TI, N>(out, p * N, first, last, zero);
-    if (count)
-      for (int p = p0 + n + lane; p < packs; p += TPR) store<TI, N>(out, p * N, first, last, zero);
-  }
-  float sum = 0.f;
+  clear_outside<TI, N, TPR>(out, p, lane);
+  uint64_t acc[2] = {f2_make(0.f, 0.f), f2_make(0.f, 0.f)};
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
-    if (i * TPR < count) {
-      const int at = (p0 + lane + i * TPR) * N;
-      float f[N], g[N];
+    if (i * TPR < p.count) {
+      const int at = (p.p0 + lane + i * TPR) * N;
+      if (!p.inside(at)) {  // what lies outside counts as 0 from here on
+        y[i].keep(p.lo - at, p.hi - at);
+        d[i].keep(p.lo - at, p.hi - at);
+        if (capped) x[i].keep(p.lo - at, p.hi - at);
+      }
+      uint64_t f[N / 2], g[N / 2];
       y[i].to(f);
       d[i].to(g);
 #pragma unroll
-      for (int e = 0; e < N; ++e)
-        if (at + e >= lo && at + e < hi) sum = fmaf(f[e], g[e], sum);
+      for (int e = 0; e < N / 2; ++e) acc[e & 1] = f2_fma(f[e], g[e], acc[e & 1]);
     }
   }
-  sum = row_reduce<SumOp, TPR, BLOCK>(sum, smem);
+  acc[0] = f2_add(acc[0], acc[1]);
+  const float sum = row_reduce<SumOp, TPR, TPR>(f2_lo(acc[0]) + f2_hi(acc[0]), smem);
+  // 1 - tanh^2 = 4 (q - q^2), q = (1 - tanh) / 2
+  const float by = capped ? 4.f * a.scale : a.scale;
+  const uint64_t minus = f2_make(-sum, -sum), times = f2_make(by, by), one = f2_make(-1.f, -1.f);
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     const int vi = lane + i * TPR;
-    if (ok && vi < count) {
-      const int at = (p0 + vi) * N;
-      float f[N], g[N], h[N];
+    if (vi < p.count) {
+      const int at = (p.p0 + vi) * N;
+      uint64_t f[N / 2], g[N / 2];
       y[i].to(f);
       d[i].to(g);
-      if (capped) x[i].to(h);
 #pragma unroll
-      for (int e = 0; e < N; ++e) {
-        float t = a.scale * f[e] * (g[e] - sum);
-        if (capped) t *= score.slope(h[e]);
-        f[e] = at + e >= lo && at + e < hi ? t : 0.f;
+      for (int e = 0; e < N / 2; ++e) f[e] = f2_mul(f2_mul(f[e], times), f2_add(g[e], minus));
+      if (capped) {
+        x[i].to(g);
+#pragma unroll
+        for (int e = 0; e < N / 2; ++e) {
+          const uint64_t q = score.half_of(g[e]);
+          f[e] = f2_mul(f[e], f2_fma(f2_mul(q, one), q, q));
+        }
       }
-      store<TI, N>(out, at, first, last, f);
+      if (!(fabsf(sum) < 3e38f) && !p.inside(at)) p.mask(f, at, 0.f);  // (0 times a sum that is not finite)
+      store<TI, N>(out, at, p.first, p.last, f);
     }
   }
+}
+
+// A warp a row: y, dy and x (where capped) copied into shared memory by
+// cp.async, as many bytes in flight as a row has and no registers for them;
+// a lane reads only what it copied.
+template <typename TI, typename TY>
+__global__ void __launch_bounds__(128, sizeof(TY) == sizeof(TI) ? 7 : 5)
+span_softmax_bwd_warp_kernel(const __grid_constant__ SpanArgs a, int room) {
+  pdl_prologue();
+  constexpr int N = Elem<TI>::kVec;
+  constexpr int W = (int)(sizeof(TY) / sizeof(TI));  // 16-byte words of y a pack
+  extern __shared__ uint4 words[];
+  const int lane = threadIdx.x & 31;
+  const Score score(a);
+  const bool capped = score.cap != 0.f;
+  // word k of pack v at [k][v]: y's, dy's, x's
+  uint4* mine = words + (threadIdx.x >> 5) * room * (2 * W + (capped ? 1 : 0)) + lane;
+  Rows rows(a);
+  if (!rows.more) return;
+  uint32_t row = rows.w.row;
+  Row r = rows.w.get(a);
+  const float by = capped ? 4.f * a.scale : a.scale;  // 1 - tanh^2 = 4 (q - q^2), q = (1 - tanh) / 2
+  const uint64_t times = f2_make(by, by), minus_one = f2_make(-1.f, -1.f);
+  while (true) {
+    TI* out = static_cast<TI*>(a.out) + row * a.ldo;
+    const int shift = shift_of(out);
+    out -= shift;
+    const Place<N> p(r, shift, a.cols);
+    const int skip = p.p0 * N - shift;
+    const TY* yr = static_cast<const TY*>(a.y) + row * a.ldy + skip;
+    const TY* dr = static_cast<const TY*>(a.dy) + row * a.ldd + skip;
+    const TI* xr = static_cast<const TI*>(a.x) + (capped ? row * a.ldx + skip : 0);
+    for (int vi = 0; vi < p.count - lane; vi += 32) {
+      const int64_t at = (int64_t)(lane + vi) * N;
+#pragma unroll
+      for (int k = 0; k < W; ++k) {
+        cp_async16(mine + k * room + vi, yr + at + k * Elem<TY>::kVec);
+        cp_async16(mine + (W + k) * room + vi, dr + at + k * Elem<TY>::kVec);
+      }
+      if (capped) cp_async16(mine + 2 * W * room + vi, xr + at);
+    }
+    cp_async_commit();
+    rows.next(a);
+    const bool more = rows.more;
+    const Raw ahead = more ? rows.w.read(a) : Raw{0, 0, 0, 0.f};
+    clear_outside<TI, N, 32>(out, p, lane);
+    cp_async_wait_all();
+    auto get = [&](int vi, Elems<TY, N>& y, Elems<TY, N>& d) {
+#pragma unroll
+      for (int k = 0; k < W; ++k) {
+        y.word(k, mine[k * room + vi]);
+        d.word(k, mine[(W + k) * room + vi]);
+      }
+      const int at = (p.p0 + lane + vi) * N;
+      if (!p.inside(at)) {  // what lies outside counts as 0
+        y.keep(p.lo - at, p.hi - at);
+        d.keep(p.lo - at, p.hi - at);
+      }
+    };
+    uint64_t acc[2] = {f2_make(0.f, 0.f), f2_make(0.f, 0.f)};
+    // (lanes past the span's last pack go along with nothing)
+    for (int vi = 0; vi < p.count; vi += 32) {
+      Elems<TY, N> y, d;
+      get(vi, y, d);
+      uint64_t f[N / 2], g[N / 2];
+      y.to(f);
+      d.to(g);
+#pragma unroll
+      for (int e = 0; e < N / 2; ++e) acc[e & 1] = f2_fma(f[e], g[e], acc[e & 1]);
+    }
+    acc[0] = f2_add(acc[0], acc[1]);
+    const float sum = group_reduce_warp<SumOp, 32>(f2_lo(acc[0]) + f2_hi(acc[0]));
+    const uint64_t minus = f2_make(-sum, -sum);
+    for (int vi = 0; vi < p.count - lane; vi += 32) {
+      const int at = (p.p0 + lane + vi) * N;
+      Elems<TY, N> y, d;
+      get(vi, y, d);
+      uint64_t f[N / 2], g[N / 2];
+      y.to(f);
+      d.to(g);
+#pragma unroll
+      for (int e = 0; e < N / 2; ++e) f[e] = f2_mul(f2_mul(f[e], times), f2_add(g[e], minus));
+      if (capped) {
+        Elems<TI, N> x;
+        x.word(0, mine[2 * W * room + vi]);
+        if (!p.inside(at)) x.keep(p.lo - at, p.hi - at);
+        x.to(g);
+#pragma unroll
+        for (int e = 0; e < N / 2; ++e) {
+          const uint64_t q = score.half_of(g[e]);
+          f[e] = f2_mul(f[e], f2_fma(f2_mul(q, minus_one), q, q));
+        }
+      }
+      if (!(fabsf(sum) < 3e38f) && !p.inside(at)) p.mask(f, at, 0.f);  // (0 times a sum that is not finite)
+      store<TI, N>(out, at, p.first, p.last, f);
+    }
+    if (!more) return;
+    row = rows.w.row;
+    r = Row(ahead, a.cols);
+  }
+}
+
+// A CTA a row.
+template <typename TI, typename TY, int TPR, int VPT>
+__global__ void __launch_bounds__(TPR, TPR <= 256 ? 2 : 1)
+span_softmax_bwd_kernel(const __grid_constant__ SpanArgs a) {
+  pdl_prologue();
+  __shared__ float smem[TPR / 32];
+  span_bwd_row<TI, TY, TPR, VPT>(a, blockIdx.x, row_of(a, blockIdx.x), Score(a), threadIdx.x, smem);
 }
 
 template <typename TI, typename TY>
@@ -385,21 +767,33 @@ span_softmax_bwd_loop_kernel(const __grid_constant__ SpanArgs a) {
   }
 }
 
-// Calls f(TPR, VPT) for rows covered by `packs` packs, at most 4 a thread;
-// -1: longer than that.
+// Calls f(TPR) for rows covered by `packs` packs: a warp up to `warp` packs,
+// then a CTA of 4 packs a thread; -1: longer than that.
 template <typename F>
-int span_ladder(int64_t packs, F&& f) {
+int span_ladder(int64_t packs, int64_t warp, F&& f) {
   using std::integral_constant;
-  using V4 = integral_constant<int, 4>;
-  if (packs <= 32) return f(integral_constant<int, 32>{}, integral_constant<int, 1>{});
-  if (packs <= 64) return f(integral_constant<int, 32>{}, integral_constant<int, 2>{});
-  if (packs <= 128) return f(integral_constant<int, 32>{}, V4{});
-  if (packs <= 256) return f(integral_constant<int, 64>{}, V4{});
-  if (packs <= 512) return f(integral_constant<int, 128>{}, V4{});
-  if (packs <= 1024) return f(integral_constant<int, 256>{}, V4{});
-  if (packs <= 2048) return f(integral_constant<int, 512>{}, V4{});
-  if (packs <= 4096) return f(integral_constant<int, 1024>{}, V4{});
+  if (packs <= warp) return f(integral_constant<int, 32>{});
+  if (packs <= 256) return f(integral_constant<int, 64>{});
+  if (packs <= 512) return f(integral_constant<int, 128>{});
+  if (packs <= 1024) return f(integral_constant<int, 256>{});
+  if (packs <= 2048) return f(integral_constant<int, 512>{});
+  if (packs <= 4096) return f(integral_constant<int, 1024>{});
   return -1;
+}
+// Launches CTAs of BLOCK threads, as many as are resident at once (`most` an
+// SM by their registers), with `each` bytes of shared memory a warp.  Warps
+// that have many rows take 8 in order.
+template <int BLOCK, typename K>
+int launch_warps(K kernel, int most, SpanArgs& a, int room, int each, const DeviceInfo& dev, cudaStream_t stream) {
+  constexpr int kWarps = BLOCK / 32;
+  const int smem = each * kWarps;
+  if (smem > 48 * 1024 &&
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+    return launch_status();
+  const int64_t ctas = (int64_t)std::max(1, std::min(most, 228 * 1024 / (smem + 1024))) * dev.sm_count;
+  a.unit = a.rows >= ctas * kWarps * 32 ? 8 : 1;
+  launch_k(kernel, (unsigned)std::min<int64_t>(ctas, ceil_div(a.rows, kWarps * a.unit)), BLOCK, smem, stream, a, room);
+  return launch_status();
 }
 
 // Whether rows at p and q (strides in elements) begin at the same element of
@@ -412,17 +806,27 @@ bool in_step(const void* p, int64_t lp, const void* q, int64_t lq, int64_t rows)
   return (ep - eq) % w == 0 && (rows <= 1 || (lp - lq) % w == 0);
 }
 
+// The most packs that cover a row: one more where rows begin inside one.
+template <typename T>
+int64_t packs_of(const void* p, int64_t ld, int64_t cols, int64_t rows) {
+  constexpr int64_t N = Elem<T>::kVec;
+  return ceil_div(cols, N) + (aligned16(p) && (rows <= 1 || ld % N == 0) ? 0 : 1);
+}
+
 template <typename TI, typename TO>
-int launch_fwd(const SpanArgs& a, const DeviceInfo& dev, cudaStream_t stream) {
-  constexpr int N = Elem<TI>::kVec;
+int launch_fwd(SpanArgs a, const DeviceInfo& dev, cudaStream_t stream) {
   if (in_step<TI, TO>(a.x, a.ldx, a.out, a.ldo, a.rows)) {
-    const int64_t packs = (a.cols + 2 * (N - 1)) / N;
-    const int st = span_ladder(packs, [&](auto tpr, auto vpt) -> int {
-      constexpr int TPR = decltype(tpr)::value, VPT = decltype(vpt)::value;
-      constexpr int BLOCK = TPR >= 256 ? TPR : 256;
-      launch_k((span_softmax_kernel<TI, TO, TPR, VPT, BLOCK>), (unsigned)ceil_div(a.rows, BLOCK / TPR), BLOCK, 0,
-               stream, a);
-      return launch_status();
+    const int64_t packs = packs_of<TI>(a.x, a.ldx, a.cols, a.rows);
+    // 65 KB of scores for 8 warps: three CTAs an SM up to 2048 keys
+    const int st = span_ladder(packs, 2056 / Elem<TI>::kVec, [&](auto tpr) -> int {
+      constexpr int TPR = decltype(tpr)::value;
+      if constexpr (TPR == 32) {
+        const int room = (int)(ceil_div(packs, 32) * 32);
+        return launch_warps<256>(span_softmax_warp_kernel<TI, TO>, 3, a, room, room * Elem<TI>::kVec * 4, dev, stream);
+      } else {
+        launch_k((span_softmax_kernel<TI, TO, TPR, 4>), a.rows, TPR, 0, stream, a);
+        return launch_status();
+      }
     });
     if (st >= 0) return st;
   }
@@ -432,17 +836,21 @@ int launch_fwd(const SpanArgs& a, const DeviceInfo& dev, cudaStream_t stream) {
 }
 
 template <typename TI, typename TY>
-int launch_bwd(const SpanArgs& a, const DeviceInfo& dev, cudaStream_t stream) {
-  constexpr int N = Elem<TI>::kVec;
+int launch_bwd(SpanArgs a, const DeviceInfo& dev, cudaStream_t stream) {
   if (in_step<TI, TY>(a.out, a.ldo, a.y, a.ldy, a.rows) && in_step<TI, TY>(a.out, a.ldo, a.dy, a.ldd, a.rows) &&
       (!(a.cap > 0.f) || in_step<TI, TI>(a.out, a.ldo, a.x, a.ldx, a.rows))) {
-    const int64_t packs = (a.cols + 2 * (N - 1)) / N;
-    const int st = span_ladder(packs, [&](auto tpr, auto vpt) -> int {
-      constexpr int TPR = decltype(tpr)::value, VPT = decltype(vpt)::value;
-      constexpr int BLOCK = TPR >= 256 ? TPR : 256;
-      launch_k((span_softmax_bwd_kernel<TI, TY, TPR, VPT, BLOCK>), (unsigned)ceil_div(a.rows, BLOCK / TPR), BLOCK,
-               0, stream, a);
-      return launch_status();
+    const int64_t packs = packs_of<TI>(a.out, a.ldo, a.cols, a.rows);
+    // up to 12 KB a warp (20 where y is wider than x): 16 warps an SM
+    const int st = span_ladder(packs, 257, [&](auto tpr) -> int {
+      constexpr int TPR = decltype(tpr)::value;
+      if constexpr (TPR == 32) {
+        const int room = (int)(ceil_div(packs, 32) * 32);
+        const int each = room * 16 * (2 * (int)(sizeof(TY) / sizeof(TI)) + (a.cap > 0.f ? 1 : 0));
+        return launch_warps<128>(span_softmax_bwd_warp_kernel<TI, TY>, sizeof(TY) == sizeof(TI) ? 7 : 5, a, room, each, dev, stream);
+      } else {
+        launch_k((span_softmax_bwd_kernel<TI, TY, TPR, 4>), a.rows, TPR, 0, stream, a);
+        return launch_status();
+      }
     });
     if (st >= 0) return st;
   }
