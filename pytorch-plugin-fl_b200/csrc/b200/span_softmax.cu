@@ -254,25 +254,66 @@ struct Place {
                      at + 2 * e + 1 >= lo && at + 2 * e + 1 < hi ? f2_hi(z[e]) : other);
   }
 };
-// Zeros in the packs where nothing is seen, by the TPR threads of a row.
+// Where nothing is seen: whole packs [begin, p0) and [p1, end), and the
+// row's first and last pack where they are not whole.
+template <typename TO, int N>
+struct Outside {
+  int begin, p0, p1, end;
+  __device__ __forceinline__ explicit Outside(const Place<N>& p) {
+    begin = p.first > 0 ? 1 : 0;
+    end = p.last / N;
+    p0 = p.count ? max(p.p0, begin) : end;
+    p1 = p.count ? p.p0 + p.count : end;
+  }
+  __device__ __forceinline__ void edges(TO* row, const Place<N>& p, int lane) const {
+    if (p.first > 0 && (p.count == 0 || p.p0 > 0) && lane >= p.first && lane < N && lane < p.last)
+      row[lane] = Elem<TO>::from_f(0.f);
+    if (p.last % N != 0 && end >= begin && (p.count == 0 || p1 <= end) && lane < p.last - end * N)
+      row[end * N + lane] = Elem<TO>::from_f(0.f);
+  }
+};
+// Zeros there by the TPR threads of a row.
 template <typename TO, int N, int TPR>
 __device__ __forceinline__ void clear_outside(TO* row, const Place<N>& p, int lane) {
-  const int begin = p.first > 0 ? 1 : 0, end = p.last / N;     // whole packs
-  const int p0 = p.count ? max(p.p0, begin) : end;             // of them [begin, p0) and [p1, end)
-  const int p1 = p.count ? p.p0 + p.count : end;
+  const Outside<TO, N> o(p);
   const uint4 zero = make_uint4(0, 0, 0, 0);
-  const int before = max(p0 - begin, 0), all = before + max(end - p1, 0);
+  const int before = max(o.p0 - o.begin, 0), all = before + max(o.end - o.p1, 0);
 #pragma unroll 2
   for (int j = lane; j < all; j += TPR) {
-    const int v = j < before ? begin + j : p1 + (j - before);
+    const int v = j < before ? o.begin + j : o.p1 + (j - before);
 #pragma unroll
     for (int i = 0; i < N / Elem<TO>::kVec; ++i) st_stream(row + v * N + i * Elem<TO>::kVec, zero);
   }
-  // the row's first and last pack where they are not whole
-  if (p.first > 0 && (p.count == 0 || p.p0 > 0) && lane >= p.first && lane < N && lane < p.last)
-    row[lane] = Elem<TO>::from_f(0.f);
-  if (p.last % N != 0 && end >= begin && (p.count == 0 || p1 <= end) && lane < p.last - end * N)
-    row[end * N + lane] = Elem<TO>::from_f(0.f);
+  o.edges(row, p, lane);
+}
+// Zeros there by the warp of a row as bulk copies of 1 KB of zeros in shared
+// memory: one instruction for what takes a loop of stores.
+constexpr int kZeroBytes = 1024;
+template <typename TO, int N>
+__device__ __forceinline__ void clear_outside_bulk(TO* row, const Place<N>& p, int lane, uint32_t zeros) {
+  const Outside<TO, N> o(p);
+  constexpr int kPack = N * (int)sizeof(TO);
+#pragma unroll
+  for (int side = 0; side < 2; ++side) {
+    char* to = reinterpret_cast<char*>(row) + (side == 0 ? o.begin : o.p1) * kPack;
+    const int bytes = (side == 0 ? o.p0 - o.begin : o.end - o.p1) * kPack;
+    for (int at = lane * kZeroBytes; at < bytes; at += 32 * kZeroBytes)
+      asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(to + at), "r"(zeros),
+                   "r"(min(kZeroBytes, bytes - at))
+                   : "memory");
+  }
+  o.edges(row, p, lane);
+}
+// The CTA's zeros; every thread of it calls this once.
+__device__ __forceinline__ uint32_t make_zeros(void* smem) {
+  for (int i = threadIdx.x; i < kZeroBytes / 16; i += blockDim.x) static_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // seen by the copies
+  __syncthreads();
+  return (uint32_t)__cvta_generic_to_shared(smem);
+}
+// Before a thread leaves: its copies have read the zeros.
+__device__ __forceinline__ void finish_zeros() {
+  asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group.read 0;" ::: "memory");
 }
 // Scores of the pack at virtual element `at` from its elements, -inf outside
 // the span; returns the larger of m and their maximum.  (What lies outside is
@@ -369,10 +410,12 @@ span_softmax_warp_kernel(const __grid_constant__ SpanArgs a, int room) {
   constexpr int Q = N / 4;  // quads of scores a pack
   extern __shared__ float4 dyn[];
   const int lane = threadIdx.x & 31;
-  // quad k of pack v at [k][v]: neighbouring packs' quads are neighbours.
-  // Lanes past the span's last pack go along (their scores are -inf), so
-  // that no pass asks for each lane; room is a multiple of 32.
-  float4* mine = dyn + (threadIdx.x >> 5) * room * Q + lane;
+  const uint32_t zeros = make_zeros(dyn);
+  // Quad k of pack v at [v / 32][k][v % 32]: neighbouring packs' quads are
+  // neighbours.  Lanes past the span's last pack go along (their scores are
+  // -inf), so that no pass asks for each lane; room is a multiple of 32.
+  constexpr int kBlock = 32 * Q;
+  float4* mine = dyn + kZeroBytes / 16 + (threadIdx.x >> 5) * room * Q + lane;
   Rows rows(a);
   if (!rows.more) return;
   const Score score(a);
@@ -399,7 +442,7 @@ span_softmax_warp_kernel(const __grid_constant__ SpanArgs a, int room) {
   load(xr, lane, p.count);
   while (true) {
     TO* out = static_cast<TO*>(a.out) + row * a.ldo - p.first;
-    clear_outside<TO, N, 32>(out, p, lane);
+    clear_outside_bulk<TO, N>(out, p, lane, zeros);
     float m = -INFINITY;
     int at = (p.p0 + lane) * N;
     float4* z4 = mine;
@@ -409,8 +452,8 @@ span_softmax_warp_kernel(const __grid_constant__ SpanArgs a, int room) {
       m = scores_of<N>(z, at, p, r, score, m);
 #pragma unroll
       for (int k = 0; k < Q; ++k)
-        z4[k * room] = make_float4(f2_lo(z[2 * k]), f2_hi(z[2 * k]), f2_lo(z[2 * k + 1]), f2_hi(z[2 * k + 1]));
-      z4 += 32;
+        z4[k * 32] = make_float4(f2_lo(z[2 * k]), f2_hi(z[2 * k]), f2_lo(z[2 * k + 1]), f2_hi(z[2 * k + 1]));
+      z4 += kBlock;
       at += 32 * N;
     };
     for (int done = 0; done < p.count; done += 64) {
@@ -437,45 +480,46 @@ span_softmax_warp_kernel(const __grid_constant__ SpanArgs a, int room) {
     if (!(fabsf(m) < 1e30f)) {
       c = 0.f;
       z4 = mine;
-      for (int done = 0; done < p.count; done += 32, z4 += 32)
+      for (int done = 0; done < p.count; done += 32, z4 += kBlock)
         for (int k = 0; k < Q; ++k) {
-          const float4 f = z4[k * room];
-          z4[k * room] = make_float4(f.x - m, f.y - m, f.z - m, f.w - m);
+          const float4 f = z4[k * 32];
+          z4[k * 32] = make_float4(f.x - m, f.y - m, f.z - m, f.w - m);
         }
     }
     const uint64_t l2 = f2_make(kLog2e, kLog2e), c2 = f2_make(c, c);
     uint64_t s2[2] = {f2_make(0.f, 0.f), f2_make(0.f, 0.f)};
     z4 = mine;
-    for (int done = 0; done < p.count; done += 32, z4 += 32) {
+    for (int done = 0; done < p.count; done += 32, z4 += kBlock) {
 #pragma unroll
       for (int k = 0; k < Q; ++k) {
-        float4 f = z4[k * room];
+        float4 f = z4[k * 32];
         const uint64_t t0 = f2_fma(f2_make(f.x, f.y), l2, c2), t1 = f2_fma(f2_make(f.z, f.w), l2, c2);
         f = make_float4(ex2(f2_lo(t0)), ex2(f2_hi(t0)), ex2(f2_lo(t1)), ex2(f2_hi(t1)));
         s2[0] = f2_add(s2[0], f2_make(f.x, f.y));
         s2[1] = f2_add(s2[1], f2_make(f.z, f.w));
-        z4[k * room] = f;
+        z4[k * 32] = f;
       }
     }
     s2[0] = f2_add(s2[0], s2[1]);
-    const float inv = 1.f / group_reduce_warp<SumOp, 32>(f2_lo(s2[0]) + f2_hi(s2[0]));
+    const float inv = rcp(group_reduce_warp<SumOp, 32>(f2_lo(s2[0]) + f2_hi(s2[0])));
     z4 = mine;
     at = (p.p0 + lane) * N;
-    for (int left = p.count - lane; left > 0; left -= 32, z4 += 32, at += 32 * N) {
+    for (int left = p.count - lane; left > 0; left -= 32, z4 += kBlock, at += 32 * N) {
       uint64_t z[N / 2];
 #pragma unroll
       for (int k = 0; k < Q; ++k) {
-        const float4 f = z4[k * room];
+        const float4 f = z4[k * 32];
         z[2 * k] = f2_make(f.x, f.y);
         z[2 * k + 1] = f2_make(f.z, f.w);
       }
       put<TO, N>(out, z, at, p, inv);
     }
-    if (!more) return;
+    if (!more) break;
     row = then;
     r = next;
     p = then_p;
   }
+  finish_zeros();
 }
 
 // TPR threads a row, VPT packs each, a CTA a row.
@@ -642,8 +686,10 @@ span_softmax_bwd_warp_kernel(const __grid_constant__ SpanArgs a, int room) {
   const int lane = threadIdx.x & 31;
   const Score score(a);
   const bool capped = score.cap != 0.f;
-  // word k of pack v at [k][v]: y's, dy's, x's
-  uint4* mine = words + (threadIdx.x >> 5) * room * (2 * W + (capped ? 1 : 0)) + lane;
+  const uint32_t zeros = make_zeros(words);
+  // word k of pack v at [v / 32][k][v % 32]: y's, dy's, x's
+  const int kinds = 2 * W + (capped ? 1 : 0);
+  uint4* mine = words + kZeroBytes / 16 + (threadIdx.x >> 5) * room * kinds + lane;
   Rows rows(a);
   if (!rows.more) return;
   uint32_t row = rows.w.row;
@@ -659,38 +705,40 @@ span_softmax_bwd_warp_kernel(const __grid_constant__ SpanArgs a, int room) {
     const TY* yr = static_cast<const TY*>(a.y) + row * a.ldy + skip;
     const TY* dr = static_cast<const TY*>(a.dy) + row * a.ldd + skip;
     const TI* xr = static_cast<const TI*>(a.x) + (capped ? row * a.ldx + skip : 0);
-    for (int vi = 0; vi < p.count - lane; vi += 32) {
-      const int64_t at = (int64_t)(lane + vi) * N;
+    uint4* w = mine;
+    int at = lane * N;
+    for (int left = p.count - lane; left > 0; left -= 32, w += 32 * kinds, at += 32 * N) {
 #pragma unroll
       for (int k = 0; k < W; ++k) {
-        cp_async16(mine + k * room + vi, yr + at + k * Elem<TY>::kVec);
-        cp_async16(mine + (W + k) * room + vi, dr + at + k * Elem<TY>::kVec);
+        cp_async16(w + k * 32, yr + at + k * Elem<TY>::kVec);
+        cp_async16(w + (W + k) * 32, dr + at + k * Elem<TY>::kVec);
       }
-      if (capped) cp_async16(mine + 2 * W * room + vi, xr + at);
+      if (capped) cp_async16(w + 2 * W * 32, xr + at);
     }
     cp_async_commit();
     rows.next(a);
     const bool more = rows.more;
     const Raw ahead = more ? rows.w.read(a) : Raw{0, 0, 0, 0.f};
-    clear_outside<TI, N, 32>(out, p, lane);
+    clear_outside_bulk<TI, N>(out, p, lane, zeros);
     cp_async_wait_all();
-    auto get = [&](int vi, Elems<TY, N>& y, Elems<TY, N>& d) {
+    Elems<TY, N> y, d;
+    auto get = [&]() {
 #pragma unroll
       for (int k = 0; k < W; ++k) {
-        y.word(k, mine[k * room + vi]);
-        d.word(k, mine[(W + k) * room + vi]);
+        y.word(k, w[k * 32]);
+        d.word(k, w[(W + k) * 32]);
       }
-      const int at = (p.p0 + lane + vi) * N;
       if (!p.inside(at)) {  // what lies outside counts as 0
         y.keep(p.lo - at, p.hi - at);
         d.keep(p.lo - at, p.hi - at);
       }
     };
     uint64_t acc[2] = {f2_make(0.f, 0.f), f2_make(0.f, 0.f)};
+    w = mine;
+    at = (p.p0 + lane) * N;
     // (lanes past the span's last pack go along with nothing)
-    for (int vi = 0; vi < p.count; vi += 32) {
-      Elems<TY, N> y, d;
-      get(vi, y, d);
+    for (int done = 0; done < p.count; done += 32, w += 32 * kinds, at += 32 * N) {
+      get();
       uint64_t f[N / 2], g[N / 2];
       y.to(f);
       d.to(g);
@@ -700,10 +748,11 @@ span_softmax_bwd_warp_kernel(const __grid_constant__ SpanArgs a, int room) {
     acc[0] = f2_add(acc[0], acc[1]);
     const float sum = group_reduce_warp<SumOp, 32>(f2_lo(acc[0]) + f2_hi(acc[0]));
     const uint64_t minus = f2_make(-sum, -sum);
-    for (int vi = 0; vi < p.count - lane; vi += 32) {
-      const int at = (p.p0 + lane + vi) * N;
-      Elems<TY, N> y, d;
-      get(vi, y, d);
+    const bool odd = !(fabsf(sum) < 3e38f);  // 0 times it is not 0
+    w = mine;
+    at = (p.p0 + lane) * N;
+    for (int left = p.count - lane; left > 0; left -= 32, w += 32 * kinds, at += 32 * N) {
+      get();
       uint64_t f[N / 2], g[N / 2];
       y.to(f);
       d.to(g);
@@ -711,7 +760,7 @@ span_softmax_bwd_warp_kernel(const __grid_constant__ SpanArgs a, int room) {
       for (int e = 0; e < N / 2; ++e) f[e] = f2_mul(f2_mul(f[e], times), f2_add(g[e], minus));
       if (capped) {
         Elems<TI, N> x;
-        x.word(0, mine[2 * W * room + vi]);
+        x.word(0, w[2 * W * 32]);
         if (!p.inside(at)) x.keep(p.lo - at, p.hi - at);
         x.to(g);
 #pragma unroll
@@ -720,13 +769,14 @@ span_softmax_bwd_warp_kernel(const __grid_constant__ SpanArgs a, int room) {
           f[e] = f2_mul(f[e], f2_fma(f2_mul(q, minus_one), q, q));
         }
       }
-      if (!(fabsf(sum) < 3e38f) && !p.inside(at)) p.mask(f, at, 0.f);  // (0 times a sum that is not finite)
+      if (odd && !p.inside(at)) p.mask(f, at, 0.f);
       store<TI, N>(out, at, p.first, p.last, f);
     }
-    if (!more) return;
+    if (!more) break;
     row = rows.w.row;
     r = Row(ahead, a.cols);
   }
+  finish_zeros();
 }
 
 // A CTA a row.
@@ -786,7 +836,7 @@ int span_ladder(int64_t packs, int64_t warp, F&& f) {
 template <int BLOCK, typename K>
 int launch_warps(K kernel, int most, SpanArgs& a, int room, int each, const DeviceInfo& dev, cudaStream_t stream) {
   constexpr int kWarps = BLOCK / 32;
-  const int smem = each * kWarps;
+  const int smem = each * kWarps + kZeroBytes;
   if (smem > 48 * 1024 &&
       cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return launch_status();
