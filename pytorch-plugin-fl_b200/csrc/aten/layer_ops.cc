@@ -8,6 +8,7 @@
 #include <cmath>
 
 #include "fused_common.h"
+#include "layer_ops.h"
 
 namespace flb200::aten {
 namespace {
@@ -262,90 +263,42 @@ at::Tensor SpanSoftmaxBackward(const at::Tensor& dy_in, const at::Tensor& y_in, 
 }
 
 // ------------------------------------------------------- gradient clipping --
-// The list's addresses, counts and types.  Tensors whose elements fill their
-// memory in some order are taken as they lie.
+// The list's addresses, counts and types.
 struct GradList {
   std::vector<const void*> in;
   std::vector<void*> out;
   std::vector<int64_t> numel;
   std::vector<int> dtype;
-  void add(const at::Tensor& t, const at::Tensor& device_of, const char* op) {
-    dtype.push_back(FloatCode(t, op));
-    SameDevice(device_of, t, op);
-    in.push_back(t.data_ptr());
+  explicit GradList(size_t n) {
+    in.reserve(n), out.reserve(n), numel.reserve(n), dtype.reserve(n);
+  }
+  void add(const at::Tensor& t) {
+    in.push_back(t.const_data_ptr());
     numel.push_back(t.numel());
+    dtype.push_back(B200Dtype(t.scalar_type()));
   }
 };
+// Tensors may come here without the dispatcher: nothing but memory of the
+// first one's GPU is taken.
+void CheckGrad(const at::Tensor& t, const at::Tensor& first, const char* op) {
+  TORCH_CHECK(t.defined() && (t.is_cuda() || t.is_privateuseone()) && t.layout() == at::kStrided && !t.is_neg(), op,
+              ": dense tensors on a GPU expected");
+  SameDevice(first, t, op);
+  (void)FloatCode(t, op);
+}
 int NormKind(double norm_type, const char* op) {
   TORCH_CHECK(norm_type == 2.0 || norm_type == INFINITY, op, ": norm_type must be 2 or inf, got ",
               std::to_string(norm_type));
   return norm_type == 2.0 ? 0 : 1;
 }
-// (the schemas' lists are not empty: an op of an empty list has no device)
 at::Tensor GradWorkspace(const at::Tensor& t, int64_t count) {
   return at::empty({(int64_t)std::max<size_t>(fl_b200_grad_norm_workspace_size(count), 16)},
                    t.options().dtype(at::kByte));
 }
 
-at::Tensor GradNorm(at::TensorList grads, double norm_type) {
-  const char* op = "flagos::grad_norm";
-  const int kind = NormKind(norm_type, op);
-  TORCH_CHECK(!grads.empty(), op, ": no tensors");
-  GradList l;
-  std::vector<at::Tensor> keep;
-  for (const at::Tensor& t : grads) {
-    keep.push_back(t.is_non_overlapping_and_dense() ? t : t.contiguous());
-    l.add(keep.back(), grads[0], op);
-  }
-  GpuGuard g(grads[0]);
-  at::Tensor norm = at::empty({}, grads[0].options().dtype(at::kFloat));
-  at::Tensor ws = GradWorkspace(grads[0], l.in.size());
-  CheckB200(fl_b200_grad_norm(l.in.data(), l.numel.data(), l.dtype.data(), l.in.size(), kind,
-                              norm.data_ptr<float>(), ws.data_ptr(), ws.numel(), StreamOf(grads[0])),
-            op);
-  return norm;
-}
-
-at::Tensor ClipGradsOut(at::TensorList grads, double max_norm, double norm_type, at::TensorList out) {
-  const char* op = "flagos::clip_grads";
-  const int kind = NormKind(norm_type, op);
-  TORCH_CHECK(!grads.empty(), op, ": no tensors");
-  TORCH_CHECK(max_norm >= 0, op, ": max_norm must be at least 0, got ", std::to_string(max_norm));
-  TORCH_CHECK(out.size() == grads.size(), op, ": one output for each tensor");
-  GradList l;
-  std::vector<at::Tensor> keep, strided;
-  std::vector<size_t> back;
-  for (size_t i = 0; i < grads.size(); ++i) {
-    const at::Tensor &t = grads[i], &o = out[i];
-    SameDevice(grads[0], o, op);
-    TORCH_CHECK(o.sizes() == t.sizes() && o.scalar_type() == t.scalar_type(), op,
-                ": each output must have its tensor's shape and dtype");
-    const bool dense = o.is_non_overlapping_and_dense();
-    if (dense && t.strides() == o.strides()) {
-      keep.push_back(t);
-      l.add(t, grads[0], op);
-      l.out.push_back(o.data_ptr());
-    } else {  // a dense copy, clipped in place and copied to where it belongs
-      at::Tensor c = t.clone(at::MemoryFormat::Contiguous);
-      keep.push_back(c);
-      l.add(c, grads[0], op);
-      l.out.push_back(c.data_ptr());
-      back.push_back(i);
-    }
-  }
-  GpuGuard g(grads[0]);
-  at::Tensor norm = at::empty({}, grads[0].options().dtype(at::kFloat));
-  at::Tensor ws = GradWorkspace(grads[0], l.in.size());
-  CheckB200(fl_b200_clip_grads(l.in.data(), l.out.data(), l.numel.data(), l.dtype.data(), l.in.size(),
-                               (float)max_norm, kind, norm.data_ptr<float>(), ws.data_ptr(), ws.numel(),
-                               StreamOf(grads[0])),
-            op);
-  for (const size_t i : back) out[i].copy_(keep[i]);
-  return norm;
-}
-
 std::tuple<std::vector<at::Tensor>, at::Tensor> ClipGrads(at::TensorList grads, double max_norm, double norm_type) {
   std::vector<at::Tensor> out;
+  out.reserve(grads.size());
   for (const at::Tensor& t : grads) out.push_back(at::empty_like(t));
   at::Tensor norm = ClipGradsOut(grads, max_norm, norm_type, out);
   return {out, norm};
@@ -570,6 +523,70 @@ at::Tensor SpanAutograd(const at::Tensor& x, const at::Tensor& spans, double sca
 }
 
 }  // namespace
+
+// Tensors whose elements fill their memory in some order are taken as they lie.
+at::Tensor GradNorm(at::TensorList grads, double norm_type) {
+  const char* op = "flagos::grad_norm";
+  const int kind = NormKind(norm_type, op);
+  TORCH_CHECK(!grads.empty(), op, ": no tensors");
+  GradList l(grads.size());
+  std::vector<at::Tensor> keep;
+  for (const at::Tensor& t : grads) {
+    CheckGrad(t, grads[0], op);
+    if (t.is_non_overlapping_and_dense()) {
+      l.add(t);
+    } else {
+      keep.push_back(t.contiguous());
+      l.add(keep.back());
+    }
+  }
+  GpuGuard g(grads[0]);
+  at::Tensor norm = at::empty({}, grads[0].options().dtype(at::kFloat));
+  at::Tensor ws = GradWorkspace(grads[0], l.in.size());
+  CheckB200(fl_b200_grad_norm(l.in.data(), l.numel.data(), l.dtype.data(), l.in.size(), kind,
+                              norm.data_ptr<float>(), ws.data_ptr(), ws.numel(), StreamOf(grads[0])),
+            op);
+  return norm;
+}
+
+at::Tensor ClipGradsOut(at::TensorList grads, double max_norm, double norm_type, at::TensorList out) {
+  const char* op = "flagos::clip_grads";
+  const int kind = NormKind(norm_type, op);
+  TORCH_CHECK(!grads.empty(), op, ": no tensors");
+  TORCH_CHECK(max_norm >= 0, op, ": max_norm must be at least 0, got ", std::to_string(max_norm));
+  TORCH_CHECK(out.size() == grads.size(), op, ": one output for each tensor");
+  GradList l(grads.size());
+  std::vector<std::pair<size_t, at::Tensor>> copies;
+  for (size_t i = 0; i < grads.size(); ++i) {
+    const at::Tensor &t = grads[i], &o = out[i];
+    CheckGrad(t, grads[0], op);
+    if (!t.is_same(o)) {
+      CheckGrad(o, grads[0], op);
+      TORCH_CHECK(o.sizes() == t.sizes() && o.scalar_type() == t.scalar_type(), op,
+                  ": each output must have its tensor's shape and dtype");
+    }
+    if (o.is_non_overlapping_and_dense() && (t.is_same(o) || t.strides() == o.strides())) {
+      l.add(t);
+      l.out.push_back(o.mutable_data_ptr());
+    } else {  // a dense copy, clipped in place and copied to where it belongs
+      copies.emplace_back(i, t.clone(at::MemoryFormat::Contiguous));
+      l.add(copies.back().second);
+      l.out.push_back(copies.back().second.mutable_data_ptr());
+    }
+  }
+  GpuGuard g(grads[0]);
+  at::Tensor norm = at::empty({}, grads[0].options().dtype(at::kFloat));
+  at::Tensor ws = GradWorkspace(grads[0], l.in.size());
+  CheckB200(fl_b200_clip_grads(l.in.data(), l.out.data(), l.numel.data(), l.dtype.data(), l.in.size(),
+                               (float)max_norm, kind, norm.data_ptr<float>(), ws.data_ptr(), ws.numel(),
+                               StreamOf(grads[0])),
+            op);
+  for (const at::Tensor& o : out)  // autograd is told that they were written
+    if (!o.is_inference()) o.unsafeGetTensorImpl()->bump_version();
+  at::NoGradGuard no_grad;
+  for (const auto& [i, c] : copies) out[i].copy_(c);
+  return norm;
+}
 
 TORCH_LIBRARY_FRAGMENT(flagos, m) {
   m.def("rotary(Tensor q, Tensor k, Tensor positions, Tensor inv_freq, float scale=1.0, "

@@ -7,8 +7,8 @@
 // table of tensors is a kernel parameter, so nothing is copied to the device
 // and a captured graph holds its own.  (Lists longer than one table take a
 // launch of each kind for every table.)  Work is dealt in chunks of 32 KB; a
-// resident CTA walks every gridDim-th chunk and looks the tensor up by going
-// forward in the table.  The first launch leaves one fp64 partial sum a CTA;
+// resident CTA walks every gridDim-th chunk and looks its tensor up in the
+// table.  The first launch leaves one fp64 partial sum a CTA;
 // every CTA of the second adds them all in one order (a few hundred loads
 // from L2), so there are no atomics, nothing to set to zero and the norm has
 // one order of addition for a given list and GPU.
@@ -43,6 +43,20 @@ struct Table {
   uint32_t first[MAXT + 1];
   uint8_t dtype[MAXT];
 };
+
+// The tensor of chunk c: a few steps where a walk from one end took as many as
+// there are tensors (2 us of the launch for 128).
+template <int MAXT>
+__device__ __forceinline__ int tensor_of(const Table<MAXT>& tab, uint32_t c, int last) {
+  if (tab.first[last] <= c && c < tab.first[last + 1]) return last;  // as the chunk before
+  int lo = 0, hi = tab.count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) / 2;
+    if (tab.first[mid] <= c) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
 
 // The packs of a tensor: elements from the first 16-byte boundary at or
 // before its first one.
@@ -120,7 +134,7 @@ norm_kernel(const __grid_constant__ Table<MAXT> tab, double* partial) {
   uint32_t top = 0;
   int t = 0;
   for (uint32_t c = blockIdx.x; c < tab.chunks; c += gridDim.x) {
-    while (c >= tab.first[t + 1]) ++t;
+    t = tensor_of(tab, c, t);
     const int64_t chunk = c - tab.first[t];
     switch (tab.dtype[t]) {
       case FL_B200_F32: add_chunk<float, MAX>(tab.in[t], tab.numel[t], chunk, sum, top); break;
@@ -214,10 +228,10 @@ scale_kernel(const __grid_constant__ Table<MAXT> tab, const double* partial, int
   // NaN stays NaN: a comparison with it is false
   const double ratio = (double)bound / (r + 1e-6);
   const float factor = ratio >= 1.0 ? 1.f : (float)ratio;
-  int t = tab.count - 1;
+  int t = 0;
   for (uint32_t i = blockIdx.x; i < tab.chunks; i += gridDim.x) {
     const uint32_t c = tab.chunks - 1 - i;
-    while (c < tab.first[t]) --t;
+    t = tensor_of(tab, c, t);
     if (factor == 1.f && tab.in[t] == tab.out[t]) continue;
     const int64_t chunk = c - tab.first[t];
     switch (tab.dtype[t]) {

@@ -90,6 +90,15 @@ __device__ __forceinline__ uint4 ld_stream(const void* p) {
       : "l"(p));
   return r;
 }
+// The same where it stands: the compiler may move ld_stream down to its first
+// use, past the work that was meant to hide its latency.
+__device__ __forceinline__ uint4 ld_stream_now(const void* p) {
+  uint4 r;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+               : "l"(p));
+  return r;
+}
 // Cached read-only load: small operands re-read by many rows (weights, tables).
 __device__ __forceinline__ uint4 ld_cached(const void* p) {
   return __ldg(reinterpret_cast<const uint4*>(p));

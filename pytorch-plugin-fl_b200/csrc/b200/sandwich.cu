@@ -54,13 +54,97 @@ __device__ __forceinline__ const T* gate_row(const Sandwich& a, uint32_t row) {
   return a.gate == nullptr ? nullptr : static_cast<const T*>(a.gate) + (int64_t)(row / a.per_gate) * a.cols;
 }
 
+// A 16-byte pack as fp32 pairs and back.
+template <typename T>
+struct Pairs {
+  static constexpr int P = Elem<T>::kVec / 2;
+  uint64_t v[P];
+  __device__ __forceinline__ Pairs() {}
+  __device__ __forceinline__ explicit Pairs(const uint4& u) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    if constexpr (std::is_same<T, float>::value) {
+      v[0] = f2_make(__uint_as_float(w[0]), __uint_as_float(w[1]));
+      v[1] = f2_make(__uint_as_float(w[2]), __uint_as_float(w[3]));
+    } else {
+#pragma unroll
+      for (int p = 0; p < P; ++p) v[p] = pair_from_bits<T>(w[p]);
+    }
+  }
+  __device__ __forceinline__ uint4 bits() const {
+    if constexpr (std::is_same<T, float>::value) {
+      return make_uint4(__float_as_uint(f2_lo(v[0])), __float_as_uint(f2_hi(v[0])), __float_as_uint(f2_lo(v[1])),
+                        __float_as_uint(f2_hi(v[1])));
+    } else {
+      return make_uint4(pair_to_bits<T>(v[0]), pair_to_bits<T>(v[1]), pair_to_bits<T>(v[2]), pair_to_bits<T>(v[3]));
+    }
+  }
+};
+__device__ __forceinline__ uint64_t both(float x) { return f2_make(x, x); }
+
+// Barrier of a team's warps.  Its number is a constant in the instruction: a
+// kernel whose barrier stands in a register holds all 16, of which an SM has
+// enough for four CTAs.
+template <int TPR, int BLOCK>
+__device__ __forceinline__ void team_barrier(int team) {
+  if constexpr (BLOCK == TPR) {
+    __syncthreads();
+  } else {
+    static_assert(BLOCK / TPR <= 4, "barriers 1 to 4");
+    if (team == 0) asm volatile("bar.sync 1, %0;" ::"n"(TPR) : "memory");
+    else if (team == 1) asm volatile("bar.sync 2, %0;" ::"n"(TPR) : "memory");
+    else if (team == 2) asm volatile("bar.sync 3, %0;" ::"n"(TPR) : "memory");
+    else asm volatile("bar.sync 4, %0;" ::"n"(TPR) : "memory");
+  }
+}
+
+// Sums of K values over the TPR threads of a row or team (TPR a power of two;
+// from 64 on its warps meet at named barrier 1 + team), into every thread, in
+// warp order.  One barrier: consecutive calls use different halves of `buf`,
+// so that no warp overwrites what another still reads.
+template <int TPR, int BLOCK, int K>
+__device__ __forceinline__ void team_sum(float (&v)[K], float4* buf, int half) {
+  static_assert(K <= 4, "a float4 of values");
+#pragma unroll
+  for (int off = (TPR < 32 ? TPR : 32) / 2; off > 0; off >>= 1) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], off);
+  }
+  if constexpr (TPR > 32) {
+    constexpr int W = TPR / 32;
+    const int team = threadIdx.x / TPR;
+    if constexpr (K == 1) {
+      float* h = reinterpret_cast<float*>(buf + half * (BLOCK / 32));
+      if ((threadIdx.x & 31) == 0) h[threadIdx.x >> 5] = v[0];
+      team_barrier<TPR, BLOCK>(team);
+      v[0] = h[team * W];
+#pragma unroll
+      for (int i = 1; i < W; ++i) v[0] += h[team * W + i];
+    } else {
+      float4* h = buf + half * (BLOCK / 32);
+      if ((threadIdx.x & 31) == 0)
+        h[threadIdx.x >> 5] = make_float4(v[0], v[1], K > 2 ? v[K > 2 ? 2 : 0] : 0.f, K > 3 ? v[K > 3 ? 3 : 0] : 0.f);
+      team_barrier<TPR, BLOCK>(team);
+      float4 t = h[team * W];
+#pragma unroll
+      for (int i = 1; i < W; ++i) {
+        const float4 o = h[team * W + i];
+        t.x += o.x, t.y += o.y, t.z += o.z, t.w += o.w;
+      }
+      v[0] = t.x, v[1] = t.y;
+      if constexpr (K > 2) v[2] = t.z;
+      if constexpr (K > 3) v[3] = t.w;
+    }
+  }
+}
+
 // Row in registers: TPR threads, VPT packs of x each; h stays fp32.
 template <typename T, int TPR, int VPT, int BLOCK>
 __global__ void __launch_bounds__(BLOCK, ladder_min_blocks<BLOCK>())
 sandwich_vec_kernel(const __grid_constant__ Sandwich a) {
   pdl_prologue();
-  constexpr int VW = Elem<T>::kVec;
-  __shared__ float smem[BLOCK / 32];
+  constexpr int VW = Elem<T>::kVec, P = VW / 2;
+  __shared__ float4 sums[2 * BLOCK / 32];
+  const float inv_n = 1.f / (float)a.cols;
   const int lane = threadIdx.x % TPR;
   const uint64_t row64 = (uint64_t)blockIdx.x * (BLOCK / TPR) + threadIdx.x / TPR;
   const bool ok = row64 < a.rows;
@@ -77,51 +161,50 @@ sandwich_vec_kernel(const __grid_constant__ Sandwich a) {
     x[i] = in ? ld_stream(xr + (int64_t)vi * VW) : make_uint4(0, 0, 0, 0);
     r[i] = in ? ld_stream(rr + (int64_t)vi * VW) : make_uint4(0, 0, 0, 0);
   }
-  float ss = 0.f;
+  uint64_t s2 = both(0.f);
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
-    float f[VW];
-    unpack<T>(x[i], f);
+    const Pairs<T> f(x[i]);
 #pragma unroll
-    for (int e = 0; e < VW; ++e) ss = fmaf(f[e], f[e], ss);
+    for (int p = 0; p < P; ++p) s2 = f2_fma(f.v[p], f.v[p], s2);
   }
-  ss = row_reduce<SumOp, TPR, BLOCK>(ss, smem);
-  const float rx = a.scale / sqrtf(ss / (float)a.cols + a.eps);
-  float h[VPT][VW];
-  ss = 0.f;
+  float ss[1] = {f2_lo(s2) + f2_hi(s2)};
+  ss[0] = row_reduce<SumOp, TPR, BLOCK>(ss[0], reinterpret_cast<float*>(sums));
+  const uint64_t rx = both(a.scale / sqrtf(ss[0] / (float)a.cols + a.eps)), off = both(a.off);
+  Pairs<T> h[VPT];
+  s2 = both(0.f);
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     const int vi = lane + i * TPR;
     if (!ok || vi >= nvec) continue;
-    float f[VW], w[VW];
-    unpack<T>(opaque(x[i]), f);
-    unpack<T>(ld_cached(static_cast<const T*>(a.post) + (int64_t)vi * VW), w);
+    Pairs<T> f(opaque(x[i]));
+    const Pairs<T> w(ld_cached(static_cast<const T*>(a.post) + (int64_t)vi * VW));
 #pragma unroll
-    for (int e = 0; e < VW; ++e) f[e] = f[e] * rx * (w[e] + a.off);
+    for (int p = 0; p < P; ++p) f.v[p] = f2_mul(f2_mul(f.v[p], rx), f2_add(w.v[p], off));
     if (gr != nullptr) {
-      unpack<T>(ld_cached(gr + (int64_t)vi * VW), w);
+      const Pairs<T> g(ld_cached(gr + (int64_t)vi * VW));
 #pragma unroll
-      for (int e = 0; e < VW; ++e) f[e] *= w[e];
+      for (int p = 0; p < P; ++p) f.v[p] = f2_mul(f.v[p], g.v[p]);
     }
-    unpack<T>(r[i], w);
+    const Pairs<T> q(r[i]);
 #pragma unroll
-    for (int e = 0; e < VW; ++e) {
-      h[i][e] = f[e] + w[e];
-      ss = fmaf(h[i][e], h[i][e], ss);
+    for (int p = 0; p < P; ++p) {
+      h[i].v[p] = f2_add(f.v[p], q.v[p]);
+      s2 = f2_fma(h[i].v[p], h[i].v[p], s2);
     }
-    st_stream(static_cast<T*>(a.h) + (int64_t)row * a.cols + (int64_t)vi * VW, pack<T>(h[i]));
+    st_stream(static_cast<T*>(a.h) + (int64_t)row * a.cols + (int64_t)vi * VW, h[i].bits());
   }
-  ss = row_reduce<SumOp, TPR, BLOCK>(ss, smem);
-  const float rh = 1.0f / sqrtf(ss / (float)a.cols + a.eps);
+  ss[0] = f2_lo(s2) + f2_hi(s2);
+  ss[0] = row_reduce<SumOp, TPR, BLOCK>(ss[0], reinterpret_cast<float*>(sums));
+  const uint64_t rh = both(1.0f / sqrtf(ss[0] / (float)a.cols + a.eps));
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     const int vi = lane + i * TPR;
     if (!ok || vi >= nvec) continue;
-    float w[VW];
-    unpack<T>(ld_cached(static_cast<const T*>(a.pre) + (int64_t)vi * VW), w);
+    Pairs<T> w(ld_cached(static_cast<const T*>(a.pre) + (int64_t)vi * VW));
 #pragma unroll
-    for (int e = 0; e < VW; ++e) w[e] = h[i][e] * rh * (w[e] + a.off);
-    st_stream(static_cast<T*>(a.y) + (int64_t)row * a.cols + (int64_t)vi * VW, pack<T>(w));
+    for (int p = 0; p < P; ++p) w.v[p] = f2_mul(f2_mul(h[i].v[p], rh), f2_add(w.v[p], off));
+    st_stream(static_cast<T*>(a.y) + (int64_t)row * a.cols + (int64_t)vi * VW, w.bits());
   }
 }
 
@@ -266,40 +349,41 @@ sandwich_bwd_cols_kernel(const __grid_constant__ Sandwich a) {
   a.shared[at + a.cols] = shared[1];
 }
 
-// Adds the chunks' partial sums: blockIdx.y == 0 dpre and dpost, y > 0 the
-// gate row that begins in chunk y - 1 and reaches into chunk y, if there is
-// one.  32 columns a CTA, 16 threads a column.
+// Adds the chunks' partial sums: blockIdx.y == 0 dpre and dpost, y > 0 a gate
+// row that chunks share, if there is one: gate row y - 1, or, of more gate
+// rows than chunks, the one that begins in chunk y - 1 and reaches into the
+// next.  32 columns a CTA, 16 threads a column.
 template <typename T>
 __global__ void __launch_bounds__(512)
-sandwich_bwd_sum_kernel(const __grid_constant__ Sandwich a) {
+sandwich_bwd_sum_kernel(const __grid_constant__ Sandwich a, int by_gate) {
   pdl_prologue();
   __shared__ float part[2][16][33];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + tx;
   const int64_t stride = 2ll * a.cols;
   uint32_t from = 0, to = a.n_parts, seg = 0;
+  uint64_t begin = 0;
   if (blockIdx.y > 0) {
-    const uint32_t edge = blockIdx.y * a.per_chunk;  // the first row of chunk y
-    seg = edge / a.per_gate;
-    const uint64_t begin = (uint64_t)seg * a.per_gate;
-    if (a.gate == nullptr || begin == edge || begin < edge - a.per_chunk) return;  // (the whole CTA)
-    const uint64_t end = min((uint64_t)a.rows, begin + a.per_gate);
-    from = blockIdx.y - 1;
-    to = (uint32_t)((end - 1) / a.per_chunk) + 1;
+    seg = by_gate ? blockIdx.y - 1 : blockIdx.y * a.per_chunk / a.per_gate;
+    begin = (uint64_t)seg * a.per_gate;
+    from = (uint32_t)(begin / a.per_chunk);
+    to = (uint32_t)((min((uint64_t)a.rows, begin + a.per_gate) - 1) / a.per_chunk) + 1;
+    if (to - from < 2 || (!by_gate && from != blockIdx.y - 1)) return;  // (the whole CTA)
   }
   float s0 = 0.f, s1 = 0.f;
   if (c < a.cols) {
     if (blockIdx.y == 0) {
-#pragma unroll 4
+#pragma unroll 8
       for (uint32_t k = ty; k < to; k += 16) {
         s0 += a.parts[k * stride + c];
         s1 += a.parts[k * stride + a.cols + c];
       }
     } else {
-      // the chunk's first gate row, or its last
-#pragma unroll 4
+      // the last gate row of the chunk it begins in (its first where both begin
+      // together), the first of the others
+#pragma unroll 8
       for (uint32_t k = from + ty; k < to; k += 16)
-        s0 += a.shared[k * stride + (seg == k * a.per_chunk / a.per_gate ? 0 : a.cols) + c];
+        s0 += a.shared[k * stride + (k == from && begin != (uint64_t)from * a.per_chunk ? a.cols : 0) + c];
     }
   }
   part[0][ty][tx] = s0;
@@ -320,63 +404,46 @@ sandwich_bwd_sum_kernel(const __grid_constant__ Sandwich a) {
   }
 }
 
-// Sum over the TPR threads of a team (TPR a multiple of 32; its warps at
-// named barrier 1 + team), into every thread, in warp order.  Two halves of
-// `buf` are used in turn, so that no warp overwrites what another still reads.
-template <int TPR, int BLOCK>
-__device__ __forceinline__ float4 team_sum(float4 v, float4* buf, int half) {
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) {
-    v.x += __shfl_xor_sync(0xffffffffu, v.x, off);
-    v.y += __shfl_xor_sync(0xffffffffu, v.y, off);
-    v.z += __shfl_xor_sync(0xffffffffu, v.z, off);
-  }
-  if constexpr (TPR > 32) {
-    constexpr int W = TPR / 32;
-    const int team = threadIdx.x / TPR;
-    float4* h = buf + half * (BLOCK / 32);
-    if ((threadIdx.x & 31) == 0) h[threadIdx.x >> 5] = v;
-    asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(TPR) : "memory");
-    v = h[team * W];
-#pragma unroll
-    for (int i = 1; i < W; ++i) {
-      const float4 o = h[team * W + i];
-      v.x += o.x, v.y += o.y, v.z += o.z;
-    }
-  }
-  return v;
-}
-
 // Rows staged in shared memory: a team of TPR threads takes a chunk of rows,
 // each thread the same VPT packs of every row, whose column sums it holds in
 // registers.  The next row's x, h, dy and dh are copied in by cp.async while
 // this one is worked on (a thread reads only what it copied, so no barrier
 // orders them).  Two barriers a row, for the two sums that hang together.
 // dpost's sums, which only the end of a gate row adds to, lie in shared
-// memory.
+// memory, and so do the weights as fp32 (converted from their own type for
+// every row they took a third of the instructions).
 template <typename T, int TPR, int VPT, int BLOCK>
 __global__ void __launch_bounds__(BLOCK, BLOCK <= 256 ? 2 : 1)
 sandwich_bwd_kernel(const __grid_constant__ Sandwich a) {
   pdl_prologue();
-  constexpr int VW = Elem<T>::kVec;
+  constexpr int VW = Elem<T>::kVec, P = VW / 2;
   constexpr int TEAMS = BLOCK / TPR;
   constexpr int STAGE = 4 * VPT * BLOCK;  // packs
   extern __shared__ uint4 dyn[];
   __shared__ float4 sums[2 * BLOCK / 32];
-  uint4* stage = dyn + threadIdx.x;                                   // [stage][array][i][thread]
-  float* dpost = reinterpret_cast<float*>(dyn + 2 * STAGE) + threadIdx.x;  // [i][e][thread]
+  uint4* stage = dyn + threadIdx.x;  // [stage][array][i][thread]
+  // dpost's sums, o + pre, and scale * gate * (o + post) of the gate row: pairs
+  // 2 k and 2 k + 1 of pack i at [i][k][thread]
+  constexpr int QUADS = VPT * (VW / 4) * BLOCK;
+  ulonglong2* dpost = reinterpret_cast<ulonglong2*>(dyn + 2 * STAGE) + threadIdx.x;
+  ulonglong2 *pre = dpost + QUADS, *post = pre + QUADS;
   const int lane = threadIdx.x % TPR;
   const uint32_t chunk = blockIdx.x * TEAMS + threadIdx.x / TPR;
   const int nvec = a.cols / VW;
   const float inv_n = 1.f / (float)a.cols;
   const uint32_t r0 = min(a.rows, chunk * a.per_chunk), r1 = min(a.rows, r0 + a.per_chunk);
-  float dpre[VPT][VW], sum[VPT][VW];
+  const uint64_t off = both(a.off), zero = both(0.f);
+  uint64_t dpre[VPT][P], sum[VPT][P];
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
+    const int vi = lane + i * TPR;
+    const Pairs<T> w(vi < nvec ? ld_cached(static_cast<const T*>(a.pre) + (int64_t)vi * VW) : make_uint4(0, 0, 0, 0));
 #pragma unroll
-    for (int e = 0; e < VW; ++e) {
-      dpre[i][e] = sum[i][e] = 0.f;
-      dpost[(i * VW + e) * BLOCK] = 0.f;
+    for (int p = 0; p < P; ++p) dpre[i][p] = sum[i][p] = zero;
+#pragma unroll
+    for (int k = 0; k < P / 2; ++k) {
+      dpost[(i * (P / 2) + k) * BLOCK] = make_ulonglong2(zero, zero);
+      pre[(i * (P / 2) + k) * BLOCK] = make_ulonglong2(f2_add(w.v[2 * k], off), f2_add(w.v[2 * k + 1], off));
     }
   }
   auto fetch = [&](uint32_t row, int st) {
@@ -397,7 +464,7 @@ sandwich_bwd_kernel(const __grid_constant__ Sandwich a) {
   if (r0 < r1) fetch(r0, 0);
   uint32_t seg = r0 / a.per_gate;
   uint64_t seg_end = (uint64_t)(seg + 1) * a.per_gate;
-  bool first_seg = true;
+  bool first_seg = true, fresh = true;
   for (uint32_t row = r0; row < r1; ++row) {
     const int st = (row - r0) & 1;
     if (row + 1 < r1) {
@@ -407,77 +474,96 @@ sandwich_bwd_kernel(const __grid_constant__ Sandwich a) {
       cp_async_wait_all();
     }
     const uint4* in = stage + st * STAGE;
-    auto get = [&](int k, int i, float (&f)[VW]) { unpack<T>(in[(k * VPT + i) * BLOCK], f); };
     const T* gr = a.gate == nullptr ? nullptr : static_cast<const T*>(a.gate) + (int64_t)seg * a.cols;
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (fresh) {  // a gate row begins
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        const int vi = lane + i * TPR;
+        if (vi >= nvec) continue;
+        Pairs<T> w(ld_cached(static_cast<const T*>(a.post) + (int64_t)vi * VW));
+#pragma unroll
+        for (int p = 0; p < P; ++p) w.v[p] = f2_mul(f2_add(w.v[p], off), both(a.scale));
+        if (gr != nullptr) {
+          const Pairs<T> g(ld_cached(gr + (int64_t)vi * VW));
+#pragma unroll
+          for (int p = 0; p < P; ++p) w.v[p] = f2_mul(w.v[p], g.v[p]);
+        }
+#pragma unroll
+        for (int k = 0; k < P / 2; ++k) post[(i * (P / 2) + k) * BLOCK] = make_ulonglong2(w.v[2 * k], w.v[2 * k + 1]);
+      }
+      fresh = false;
+    }
+    uint64_t vx = zero, vh = zero, vd = zero;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      const int vi = lane + i * TPR;
-      if (vi >= nvec) continue;
-      float x[VW], h[VW], dy[VW], w[VW];
-      get(0, i, x);
-      get(1, i, h);
-      get(2, i, dy);
-      unpack<T>(ld_cached(static_cast<const T*>(a.pre) + (int64_t)vi * VW), w);
+      if (lane + i * TPR >= nvec) continue;
+      const Pairs<T> x(in[i * BLOCK]), h(in[(VPT + i) * BLOCK]), dy(in[(2 * VPT + i) * BLOCK]);
 #pragma unroll
-      for (int e = 0; e < VW; ++e) {
-        v.x = fmaf(x[e], x[e], v.x);
-        v.y = fmaf(h[e], h[e], v.y);
-        v.z = fmaf(dy[e] * (w[e] + a.off), h[e], v.z);
+      for (int k = 0; k < P / 2; ++k) {
+        const ulonglong2 w = pre[(i * (P / 2) + k) * BLOCK];
+        vd = f2_fma(f2_mul(dy.v[2 * k], w.x), h.v[2 * k], vd);
+        vd = f2_fma(f2_mul(dy.v[2 * k + 1], w.y), h.v[2 * k + 1], vd);
+      }
+#pragma unroll
+      for (int p = 0; p < P; ++p) {
+        vx = f2_fma(x.v[p], x.v[p], vx);
+        vh = f2_fma(h.v[p], h.v[p], vh);
       }
     }
-    v = team_sum<TPR, BLOCK>(v, sums, 0);
-    const float rx = 1.0f / sqrtf(v.x * inv_n + a.eps), rh = 1.0f / sqrtf(v.y * inv_n + a.eps);
-    const float mean = v.z * rh * inv_n;
-    float t[VPT][VW];
-    float4 u = make_float4(0.f, 0.f, 0.f, 0.f);
+    float v[3] = {f2_lo(vx) + f2_hi(vx), f2_lo(vh) + f2_hi(vh), f2_lo(vd) + f2_hi(vd)};
+    team_sum<TPR, BLOCK>(v, sums, 0);
+    const float rx = rsqrtf(fmaf(v[0], inv_n, a.eps)), rh = rsqrtf(fmaf(v[1], inv_n, a.eps));
+    const uint64_t rx2 = both(rx), rh2 = both(rh), mean2 = both(-(v[2] * rh * inv_n));
+    uint64_t t[VPT][P], vt = zero;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int vi = lane + i * TPR;
       if (vi >= nvec) continue;
-      float h[VW], dy[VW], w[VW];
-      get(1, i, h);
-      get(2, i, dy);
-      unpack<T>(ld_cached(static_cast<const T*>(a.pre) + (int64_t)vi * VW), w);
-#pragma unroll
-      for (int e = 0; e < VW; ++e) {
-        const float m = h[e] * rh;
-        dpre[i][e] = fmaf(dy[e], m, dpre[i][e]);
-        t[i][e] = rh * (dy[e] * (w[e] + a.off) - m * mean);
-      }
+      const Pairs<T> h(in[(VPT + i) * BLOCK]), dy(in[(2 * VPT + i) * BLOCK]);
+      Pairs<T> g;
       if (a.dh != nullptr) {
-        get(3, i, h);
+        g = Pairs<T>(in[(3 * VPT + i) * BLOCK]);
+      } else {
 #pragma unroll
-        for (int e = 0; e < VW; ++e) t[i][e] += h[e];
+        for (int p = 0; p < P; ++p) g.v[p] = zero;
       }
-      st_stream(static_cast<T*>(a.dres) + (int64_t)row * a.cols + (int64_t)vi * VW, pack<T>(t[i]));
-      unpack<T>(ld_cached(static_cast<const T*>(a.post) + (int64_t)vi * VW), w);
 #pragma unroll
-      for (int e = 0; e < VW; ++e) w[e] = a.scale * (w[e] + a.off);
-      if (gr != nullptr) {
-        unpack<T>(ld_cached(gr + (int64_t)vi * VW), dy);
+      for (int k = 0; k < P / 2; ++k) {
+        const ulonglong2 w = pre[(i * (P / 2) + k) * BLOCK];
 #pragma unroll
-        for (int e = 0; e < VW; ++e) w[e] *= dy[e];
+        for (int q = 0; q < 2; ++q) {
+          const int p = 2 * k + q;
+          const uint64_t m = f2_mul(h.v[p], rh2);
+          dpre[i][p] = f2_fma(dy.v[p], m, dpre[i][p]);
+          g.v[p] = f2_fma(rh2, f2_fma(m, mean2, f2_mul(dy.v[p], q ? w.y : w.x)), g.v[p]);
+        }
       }
-      get(0, i, h);
+      st_stream(static_cast<T*>(a.dres) + (int64_t)row * a.cols + (int64_t)vi * VW, g.bits());
+      const Pairs<T> x(in[i * BLOCK]);
 #pragma unroll
-      for (int e = 0; e < VW; ++e) {
-        sum[i][e] = fmaf(t[i][e], h[e] * rx, sum[i][e]);
-        t[i][e] *= w[e];
-        u.x = fmaf(t[i][e], h[e], u.x);
+      for (int k = 0; k < P / 2; ++k) {
+        const ulonglong2 w = post[(i * (P / 2) + k) * BLOCK];
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const int p = 2 * k + q;
+          sum[i][p] = f2_fma(g.v[p], f2_mul(x.v[p], rx2), sum[i][p]);
+          t[i][p] = f2_mul(g.v[p], q ? w.y : w.x);
+          vt = f2_fma(t[i][p], x.v[p], vt);
+        }
       }
     }
-    u = team_sum<TPR, BLOCK>(u, sums, 1);
-    const float mean_t = u.x * rx * inv_n;
+    float u[1] = {f2_lo(vt) + f2_hi(vt)};
+    team_sum<TPR, BLOCK>(u, sums, 1);
+    // rx (t - n mean(t n)) with n = x rx
+    const uint64_t back = both(-(rx * rx * (u[0] * rx * inv_n)));
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int vi = lane + i * TPR;
       if (vi >= nvec) continue;
-      float x[VW];
-      get(0, i, x);
+      Pairs<T> x(in[i * BLOCK]);
 #pragma unroll
-      for (int e = 0; e < VW; ++e) x[e] = rx * (t[i][e] - x[e] * rx * mean_t);
-      st_stream(static_cast<T*>(a.dx) + (int64_t)row * a.cols + (int64_t)vi * VW, pack<T>(x));
+      for (int p = 0; p < P; ++p) x.v[p] = f2_fma(x.v[p], back, f2_mul(t[i][p], rx2));
+      st_stream(static_cast<T*>(a.dx) + (int64_t)row * a.cols + (int64_t)vi * VW, x.bits());
     }
     if (row + 1 == seg_end || row + 1 == r1) {  // the gate row ends, or the chunk
       const bool whole = (uint64_t)seg * a.per_gate >= r0 && (row + 1 == seg_end || r1 == a.rows);
@@ -486,65 +572,77 @@ sandwich_bwd_kernel(const __grid_constant__ Sandwich a) {
         const int vi = lane + i * TPR;
         if (vi >= nvec) continue;
         const int64_t c = (int64_t)vi * VW;
+        Pairs<T> g;
         if (gr != nullptr) {
-          float gf[VW], w[VW];
-          unpack<T>(ld_cached(gr + c), gf);
-          unpack<T>(ld_cached(static_cast<const T*>(a.post) + c), w);
-#pragma unroll
-          for (int e = 0; e < VW; ++e) {
-            dpost[(i * VW + e) * BLOCK] = fmaf(a.scale * gf[e], sum[i][e], dpost[(i * VW + e) * BLOCK]);
-            w[e] = a.scale * (w[e] + a.off) * sum[i][e];
-          }
+          g = Pairs<T>(ld_cached(gr + c));
           if (whole) {
-            st_stream(static_cast<T*>(a.dgate) + (int64_t)seg * a.cols + c, pack<T>(w));
+            Pairs<T> w(ld_cached(static_cast<const T*>(a.post) + c));
+#pragma unroll
+            for (int p = 0; p < P; ++p) w.v[p] = f2_mul(f2_mul(f2_add(w.v[p], off), both(a.scale)), sum[i][p]);
+            st_stream(static_cast<T*>(a.dgate) + (int64_t)seg * a.cols + c, w.bits());
           } else {
             float* sh = a.shared + ((int64_t)chunk * 2 + (first_seg ? 0 : 1)) * a.cols + c;
 #pragma unroll
-            for (int e = 0; e < VW; ++e) sh[e] = sum[i][e];
+            for (int p = 0; p < P; ++p) {
+              sh[2 * p] = f2_lo(sum[i][p]);
+              sh[2 * p + 1] = f2_hi(sum[i][p]);
+            }
           }
         } else {
 #pragma unroll
-          for (int e = 0; e < VW; ++e) dpost[(i * VW + e) * BLOCK] = a.scale * sum[i][e];
+          for (int p = 0; p < P; ++p) g.v[p] = both(1.f);
         }
 #pragma unroll
-        for (int e = 0; e < VW; ++e) sum[i][e] = 0.f;
+        for (int k = 0; k < P / 2; ++k) {
+          ulonglong2& d = dpost[(i * (P / 2) + k) * BLOCK];
+          d = make_ulonglong2(f2_fma(f2_mul(g.v[2 * k], both(a.scale)), sum[i][2 * k], d.x),
+                              f2_fma(f2_mul(g.v[2 * k + 1], both(a.scale)), sum[i][2 * k + 1], d.y));
+        }
+#pragma unroll
+        for (int p = 0; p < P; ++p) sum[i][p] = zero;
       }
       first_seg = false;
+      fresh = true;
       ++seg;
       seg_end += a.per_gate;
     }
   }
   // the CTA's partial sums: its teams' in order
+  float* part = a.parts + (int64_t)blockIdx.x * 2 * a.cols;
   if constexpr (TEAMS > 1) {
-    // [array][i][e][thread], over the stages that nothing is on its way to any more
-    float* all = reinterpret_cast<float*>(dyn);
+    // dpre laid out as dpost, over the stages that nothing is on its way to any more
+    ulonglong2* all = reinterpret_cast<ulonglong2*>(dyn);
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < VPT; ++i)
 #pragma unroll
-      for (int e = 0; e < VW; ++e) all[(i * VW + e) * BLOCK + threadIdx.x] = dpre[i][e];
+      for (int k = 0; k < P / 2; ++k)
+        all[(i * (P / 2) + k) * BLOCK + threadIdx.x] = make_ulonglong2(dpre[i][2 * k], dpre[i][2 * k + 1]);
     __syncthreads();
+    const float *dp = reinterpret_cast<const float*>(dyn), *dq = reinterpret_cast<const float*>(dyn + 2 * STAGE);
     for (int c = threadIdx.x; c < a.cols; c += BLOCK) {
-      const int vi = c / VW, at = ((vi / TPR) * VW + c % VW) * BLOCK + vi % TPR;
+      const int vi = c / VW;
+      const int at = (((vi / TPR) * (P / 2) + c % VW / 4) * BLOCK + vi % TPR) * 4 + c % 4;
       float p = 0.f, q = 0.f;
-      const float* post = reinterpret_cast<const float*>(dyn + 2 * STAGE);
       for (int k = 0; k < TEAMS; ++k) {
-        p += all[at + k * TPR];
-        q += post[at + k * TPR];
+        p += dp[at + k * TPR * 4];
+        q += dq[at + k * TPR * 4];
       }
-      a.parts[(int64_t)blockIdx.x * 2 * a.cols + c] = p;
-      a.parts[((int64_t)blockIdx.x * 2 + 1) * a.cols + c] = q;
+      part[c] = p;
+      part[a.cols + c] = q;
     }
   } else {
-    float* part = a.parts + (int64_t)blockIdx.x * 2 * a.cols;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int vi = lane + i * TPR;
       if (vi >= nvec) continue;
 #pragma unroll
-      for (int e = 0; e < VW; ++e) {
-        part[vi * VW + e] = dpre[i][e];
-        part[a.cols + vi * VW + e] = dpost[(i * VW + e) * BLOCK];
+      for (int k = 0; k < P / 2; ++k) {
+        const ulonglong2 d = dpost[(i * (P / 2) + k) * BLOCK];
+        const int c = vi * VW + 4 * k;
+        *reinterpret_cast<float4*>(part + c) = make_float4(f2_lo(dpre[i][2 * k]), f2_hi(dpre[i][2 * k]),
+                                                           f2_lo(dpre[i][2 * k + 1]), f2_hi(dpre[i][2 * k + 1]));
+        *reinterpret_cast<float4*>(part + a.cols + c) = make_float4(f2_lo(d.x), f2_hi(d.x), f2_lo(d.y), f2_hi(d.y));
       }
     }
   }
@@ -589,6 +687,7 @@ int launch_fwd(const Sandwich& a, const DeviceInfo& dev, cudaStream_t stream) {
   constexpr int VW = Elem<T>::kVec;
   if (a.cols % VW == 0 && a.ldx % VW == 0 && a.ldr % VW == 0 && aligned16(a.x) && aligned16(a.res) &&
       aligned16(a.post) && aligned16(a.pre) && aligned16(a.gate) && aligned16(a.y) && aligned16(a.h)) {
+    // 4096 columns of 16 bits: 256 threads of two packs (65536 rows 346 us; 128 of four 465 us)
     const int r = row_ladder<2>(a.cols / VW, [&](auto tpr, auto vpt) -> int {
       constexpr int TPR = decltype(tpr)::value, VPT = decltype(vpt)::value;
       constexpr int BLOCK = ladder_block<TPR>();
@@ -606,8 +705,8 @@ template <typename T, int TPR>
 int launch_teams(const Sandwich& a, cudaStream_t stream) {
   constexpr int BLOCK = TPR >= 256 ? TPR : 256;
   constexpr int VW = Elem<T>::kVec;
-  // two stages of four operands, and dpost's sums
-  constexpr int smem = (2 * 4 * kBwdVpt * 16 + kBwdVpt * VW * 4) * BLOCK;
+  // two stages of four operands; dpost's sums and the two weights in fp32
+  constexpr int smem = (2 * 4 * kBwdVpt * 16 + 3 * kBwdVpt * VW * 4) * BLOCK;
   auto kern = sandwich_bwd_kernel<T, TPR, kBwdVpt, BLOCK>;
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return launch_status();
@@ -640,8 +739,10 @@ int launch_bwd(Sandwich a, const DeviceInfo& dev, float* ws, cudaStream_t stream
     default: st = launch_teams<T, 512>(a, stream); break;
   }
   if (st != FL_B200_OK) return st;
-  launch_k(sandwich_bwd_sum_kernel<T>, dim3((unsigned)ceil_div(a.cols, 32), a.gate ? a.chunks : 1), 512, 0, stream,
-           a);
+  const int64_t gates = a.gate ? ceil_div(a.rows, a.per_gate) : 0;
+  const int by_gate = gates < a.chunks;
+  const int64_t sums = a.chunks == 1 ? 1 : 1 + std::min<int64_t>(gates, a.chunks - 1);
+  launch_k(sandwich_bwd_sum_kernel<T>, dim3((unsigned)ceil_div(a.cols, 32), (unsigned)sums), 512, 0, stream, a, by_gate);
   return launch_status();
 }
 

@@ -173,7 +173,7 @@ struct Elems {
   __device__ __forceinline__ void load(const T* p) {
 #pragma unroll
     for (int i = 0; i < N / VW; ++i) {
-      word(i, ld_stream(p + i * VW));
+      word(i, ld_stream_now(p + i * VW));
     }
   }
   __device__ __forceinline__ void word(int i, const uint4& u) {

@@ -10,6 +10,7 @@
 #include <torch/extension.h>
 
 #include "aten/dispatch.h"
+#include "aten/layer_ops.h"
 #include "aten/ops.h"
 #include "aten/tensor_utils.h"
 #include "runtime/runtime.h"
@@ -99,4 +100,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     return d;
   });
   m.def("_empty_cache", &R::empty_cache);
+  m.def("_grad_norm", [](const std::vector<at::Tensor>& grads, double norm_type) {
+    return flb200::aten::GradNorm(grads, norm_type);
+  });
+  m.def("_clip_grads_out", [](const std::vector<at::Tensor>& grads, double max_norm, double norm_type,
+                              const std::vector<at::Tensor>& out) {
+    return flb200::aten::ClipGradsOut(grads, max_norm, norm_type, out);
+  });
 }

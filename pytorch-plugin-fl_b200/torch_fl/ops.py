@@ -13,6 +13,8 @@ import os
 
 import torch
 
+from . import _C
+
 
 def default_rounding() -> str:
     r = os.environ.get("FLAGOS_B200_ROUNDING", "fused")
@@ -262,7 +264,7 @@ def grad_norm(grads, norm_type: float = 2.0):
     """The norm of all tensors of a list taken as one vector (2, or inf for the
     largest magnitude): float32, on the device, in two launches.  Types may be
     mixed; squares that fp32 cannot hold are added in fp64."""
-    return torch.ops.flagos.grad_norm(_grads(grads), float(norm_type))
+    return _C._grad_norm(_grads(grads), float(norm_type))
 
 
 def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None):
@@ -274,7 +276,7 @@ def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None):
     if out is None:
         return torch.ops.flagos.clip_grads(grads, float(max_norm), float(norm_type))
     out = list(out)
-    return out, torch.ops.flagos.clip_grads_out(grads, float(max_norm), float(norm_type), out)
+    return out, _C._clip_grads_out(grads, float(max_norm), float(norm_type), out)
 
 
 def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False):

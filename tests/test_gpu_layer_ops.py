@@ -930,3 +930,20 @@ def test_pdl_changes_nothing():
     finally:
         torch_fl._abi.set_pdl(before)
     assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+def test_clip_through_the_dispatcher_and_versions():
+    ts = [torch.randn(300, generator=gen(i)).to(DEV) for i in range(3)]
+    want, n = torch_fl.ops.clip_grads(ts, 0.5)
+    assert torch.equal(torch.ops.flagos.grad_norm(ts, 2.0), n)
+    got, n2 = torch.ops.flagos.clip_grads(ts, 0.5, 2.0)
+    assert torch.equal(n, n2) and all(torch.equal(a, b) for a, b in zip(got, want))
+    out = [torch.empty_like(t) for t in ts]
+    before = [t._version for t in out]
+    assert torch.equal(torch.ops.flagos.clip_grads_out(ts, 0.5, 2.0, out), n)
+    assert all(torch.equal(a, b) for a, b in zip(out, want))
+    assert all(t._version > b for t, b in zip(out, before))
+    with pytest.raises(RuntimeError):
+        torch_fl.ops.clip_grads([ts[0], torch.zeros(3)], 1.0, out=[ts[0], torch.zeros(3)])   # on the CPU
+    with pytest.raises(RuntimeError):
+        torch_fl.ops.grad_norm([torch.zeros(3)])
