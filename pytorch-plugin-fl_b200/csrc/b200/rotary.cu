@@ -39,7 +39,9 @@ struct RotaryArgs {
   uint32_t tokens, seq;
   int items, copies;        // packs a head that turn (pairs of them where halves are paired) / stay
   uint32_t items_m, copies_m;  // ceil(2^31 / items), ...
-  int copy_from, copy_to;   // item range of the packs that are copied
+  int copy_from, copy_to;   // item range of a token's packs that are copied
+  int group;                // tokens a warp
+  uint32_t token_m, copy_m;    // ceil(2^31 / a token's items), ... of its copies
   int split_b;              // bytes from a pack to its partner
 };
 
@@ -96,7 +98,8 @@ struct alignas(CH * 4) Chunk {
 // pairs in both cases.
 // 64 registers: 32 warps an SM (65536 tokens of 40 heads of 128 bf16: 212 us,
 // with 88 registers and 20 warps 239 us).
-template <typename T, int VEC, bool NEIGH>
+// MANY: a warp takes `group` tokens, whose heads have few packs.
+template <typename T, int VEC, bool NEIGH, bool MANY>
 __global__ void __launch_bounds__(128, 8)
 rotary_kernel(const __grid_constant__ RotaryArgs a) {
   pdl_prologue();
@@ -108,20 +111,41 @@ rotary_kernel(const __grid_constant__ RotaryArgs a) {
   constexpr int kSize = (int)sizeof(T);
   extern __shared__ float4 smem4[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  float* table = reinterpret_cast<float*>(smem4) + warp * ((a.rot + 3) & ~3);
+  const int group = MANY ? a.group : 1;
+  float* table = reinterpret_cast<float*>(smem4) + warp * ((group * a.rot + 3) & ~3);
   const uint32_t unit = blockIdx.x * 4u + warp;
-  const uint32_t token = unit / (uint32_t)a.splits;
-  if (token >= a.tokens) return;
-  const int part = (int)(unit - token * (uint32_t)a.splits);
-  const uint32_t b = token / a.seq, s = token - b * a.seq;
-  const char* q_in = a.in[0] + b * a.sb[0] + s * a.ss[0];
-  const char* k_in = a.in[1] + b * a.sb[1] + s * a.ss[1] - a.q_heads * a.sh[1];
-  char* q_out = a.out[0] + b * a.ob[0] + s * a.os[0];
-  char* k_out = a.out[1] + b * a.ob[1] + s * a.os[1] - a.q_heads * a.oh[1];
-  auto head_in = [&](int h) { return h < a.q_heads ? q_in + h * a.sh[0] : k_in + h * a.sh[1]; };
-  auto head_out = [&](int h) { return h < a.q_heads ? q_out + h * a.oh[0] : k_out + h * a.oh[1]; };
+  const uint32_t first = MANY ? unit * (uint32_t)group : unit / (uint32_t)a.splits;
+  if (first >= a.tokens) return;
+  const int part = MANY ? 0 : (int)(unit - first * (uint32_t)a.splits);
+  const int here = MANY ? (int)min((uint32_t)group, a.tokens - first) : 1;  // tokens
+  const uint32_t b0 = first / a.seq, s0 = first - b0 * a.seq;
+  // token `tok` of the warp's
+  auto where = [&](int tok, uint32_t* b, uint32_t* s) {
+    *b = b0, *s = s0 + tok;
+    if constexpr (MANY)
+      while (*s >= a.seq) *s -= a.seq, ++*b;
+  };
+  const char* q_in = a.in[0] + b0 * a.sb[0] + s0 * a.ss[0];
+  const char* k_in = a.in[1] + b0 * a.sb[1] + s0 * a.ss[1] - a.q_heads * a.sh[1];
+  char* q_out = a.out[0] + b0 * a.ob[0] + s0 * a.os[0];
+  char* k_out = a.out[1] + b0 * a.ob[1] + s0 * a.os[1] - a.q_heads * a.oh[1];
+  auto head_in = [&](int tok, int h) -> const char* {
+    if constexpr (!MANY) return h < a.q_heads ? q_in + h * a.sh[0] : k_in + h * a.sh[1];
+    uint32_t b, s;
+    where(tok, &b, &s);
+    const int t = h >= a.q_heads;
+    return (t ? a.in[1] : a.in[0]) + b * a.sb[t] + s * a.ss[t] + (h - (t ? a.q_heads : 0)) * a.sh[t];
+  };
+  auto head_out = [&](int tok, int h) -> char* {
+    if constexpr (!MANY) return h < a.q_heads ? q_out + h * a.oh[0] : k_out + h * a.oh[1];
+    uint32_t b, s;
+    where(tok, &b, &s);
+    const int t = h >= a.q_heads;
+    return (t ? a.out[1] : a.out[0]) + b * a.ob[t] + s * a.os[t] + (h - (t ? a.q_heads : 0)) * a.oh[t];
+  };
+  const int each = a.heads * a.items, copies = a.copy_to - a.copy_from;  // a token's
   const int P = a.items;
-  const int total = a.heads * P;
+  const int total = here * each;
   const int step = a.splits * 32;
   auto offset = [&](int j) { return (NEIGH && VEC == 1 ? 2 * j : j) * VEC * kSize; };
   using Raw = typename Pack<T, VEC>::Raw;
@@ -131,8 +155,9 @@ rotary_kernel(const __grid_constant__ RotaryArgs a) {
     for (int u = 0; u < U; ++u) {
       const int it = it0 + u * step;
       if (it < total) {
-        const int h = quotient(it, a.items_m);
-        const char* p = head_in(h) + offset(it - h * P);
+        const int tok = MANY ? quotient(it, a.token_m) : 0;
+        const int of = it - tok * each, h = quotient(of, a.items_m);
+        const char* p = head_in(tok, h) + offset(of - h * P);
         ld_now(lo[u].raw, p);
         if constexpr (PAIR) ld_now(hi[u].raw, p + a.split_b);
       }
@@ -140,33 +165,41 @@ rotary_kernel(const __grid_constant__ RotaryArgs a) {
   };
   int it0 = part * 32 + lane;
   load(it0);
-  {
-    const double pos = a.pos64 ? (double)static_cast<const int64_t*>(a.pos)[b * a.pb + s * a.ps]
-                               : (double)static_cast<const int32_t*>(a.pos)[b * a.pb + s * a.ps];
-    for (int f = lane; f < a.rot / 2; f += 32) {
-      // in turns; 0.15915494309189535 is 1 / (2 pi)
-      double t = pos * (double)__ldg(a.freq + f) * 0.15915494309189535;
-      t -= rint(t);
-      float sn, cs;
-      sincospif((float)(2.0 * t), &sn, &cs);
-      const int j = f / NE, e = f % NE;
-      table[((e / CH) * P + j) * CH + e % CH] = cs * a.scale;
-      table[(((NE + e) / CH) * P + j) * CH + (NE + e) % CH] = sn * (a.scale * a.sign);
+  auto position = [&](uint32_t b, uint32_t s) {
+    return a.pos64 ? (double)static_cast<const int64_t*>(a.pos)[b * a.pb + s * a.ps]
+                   : (double)static_cast<const int32_t*>(a.pos)[b * a.pb + s * a.ps];
+  };
+  double pos = MANY ? 0.0 : position(b0, s0);
+  for (int f = lane; f < here * (a.rot / 2); f += 32) {
+    const int tok = MANY ? f / (a.rot / 2) : 0, i = MANY ? f - tok * (a.rot / 2) : f;
+    if constexpr (MANY) {
+      uint32_t b, s;
+      where(tok, &b, &s);
+      pos = position(b, s);
     }
-    __syncwarp();
+    // in turns; 0.15915494309189535 is 1 / (2 pi)
+    double t = pos * (double)__ldg(a.freq + i) * 0.15915494309189535;
+    t -= rint(t);
+    float sn, cs;
+    sincospif((float)(2.0 * t), &sn, &cs);
+    float* to = table + tok * a.rot;
+    const int j = i / NE, e = i % NE;
+    to[((e / CH) * P + j) * CH + e % CH] = cs * a.scale;
+    to[(((NE + e) / CH) * P + j) * CH + (NE + e) % CH] = sn * (a.scale * a.sign);
   }
+  __syncwarp();
   while (it0 < total) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int it = it0 + u * step;
       if (it >= total) break;
-      const int h = quotient(it, a.items_m);
-      const int j = it - h * P;
-      char* p = head_out(h) + offset(j);
+      const int tok = MANY ? quotient(it, a.token_m) : 0;
+      const int of = it - tok * each, h = quotient(of, a.items_m), j = of - h * P;
+      char* p = head_out(tok, h) + offset(j);
       float cs[2 * NE];
 #pragma unroll
       for (int c = 0; c < NCH; ++c) {
-        const Chunk<CH> v = reinterpret_cast<const Chunk<CH>*>(table)[c * P + j];
+        const Chunk<CH> v = reinterpret_cast<const Chunk<CH>*>(table + tok * a.rot)[c * P + j];
 #pragma unroll
         for (int e = 0; e < CH; ++e) cs[c * CH + e] = v.v[e];
       }
@@ -195,21 +228,23 @@ rotary_kernel(const __grid_constant__ RotaryArgs a) {
     load(it0);
   }
   // the rest of each head, where it is not in place already
-  for (int c0 = a.copy_from + part * 32 + lane; c0 < a.copy_to; c0 += 8 * step) {
+  for (int c0 = part * 32 + lane; c0 < here * copies; c0 += 8 * step) {
     Raw v[8];
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
       const int c = c0 + u * step;
-      if (c >= a.copy_to) break;
-      const int h = quotient(c, a.copies_m);
-      v[u] = __ldcs(reinterpret_cast<const Raw*>(head_in(h) + a.rot * kSize) + (c - h * a.copies));
+      if (c >= here * copies) break;
+      const int tok = MANY ? quotient(c, a.copy_m) : 0;
+      const int of = c - tok * copies + a.copy_from, h = quotient(of, a.copies_m);
+      ld_now(v[u], head_in(tok, h) + a.rot * kSize + (of - h * a.copies) * (int)sizeof(Raw));
     }
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
       const int c = c0 + u * step;
-      if (c >= a.copy_to) break;
-      const int h = quotient(c, a.copies_m);
-      __stcs(reinterpret_cast<Raw*>(head_out(h) + a.rot * kSize) + (c - h * a.copies), v[u]);
+      if (c >= here * copies) break;
+      const int tok = MANY ? quotient(c, a.copy_m) : 0;
+      const int of = c - tok * copies + a.copy_from, h = quotient(of, a.copies_m);
+      __stcs(reinterpret_cast<Raw*>(head_out(tok, h) + a.rot * kSize) + (of - h * a.copies), v[u]);
     }
   }
 }
@@ -230,14 +265,28 @@ int launch(RotaryArgs a, int64_t head_dim, cudaStream_t stream) {
   // heads whose rest lies in place already are not copied onto themselves
   a.copy_from = a.in[0] == a.out[0] ? a.q_heads * a.copies : 0;
   a.copy_to = (a.heads > a.q_heads && a.in[1] != a.out[1] ? a.heads : a.q_heads) * a.copies;
+  if (a.copy_to < a.copy_from) a.copy_to = a.copy_from;
+  const int64_t each = (int64_t)a.heads * a.items;
+  // Tokens of few packs (one or two heads) share a warp, whose lanes and loads
+  // in flight they would not fill alone, while that leaves 32 warps an SM.
+  a.group = (int)std::max<int64_t>(1, std::min({(int64_t)8, (int64_t)(128 / each), (int64_t)(2048 / a.rot),
+                                                (int64_t)a.tokens / (32 * dev.sm_count)}));
+  if (a.group > 1) {
+    a.splits = 1;
+    a.token_m = (uint32_t)ceil_div(1ll << 31, each);
+    a.copy_m = a.copy_to > a.copy_from ? (uint32_t)ceil_div(1ll << 31, a.copy_to - a.copy_from) : 0;
+    const size_t smem = 4 * ((a.group * a.rot + 3) & ~3) * sizeof(float);
+    launch_k((rotary_kernel<T, VEC, NEIGH, true>), (unsigned)ceil_div(ceil_div(a.tokens, a.group), 4), 128, smem,
+             stream, a);
+    return launch_status();
+  }
   // A warp a token leaves most of the GPU idle below 16 warps an SM; then a
   // token's items are dealt to as many warps as have 32 of them.
-  const int64_t work = (int64_t)a.heads * a.items;
   const int64_t want = ceil_div(16ll * dev.sm_count, a.tokens);
-  a.splits = (int)std::max<int64_t>(1, std::min<int64_t>(want, ceil_div(work, 32)));
+  a.splits = (int)std::max<int64_t>(1, std::min<int64_t>(want, ceil_div(each, 32)));
   const int64_t units = (int64_t)a.tokens * a.splits;
   const size_t smem = 4 * ((a.rot + 3) & ~3) * sizeof(float);
-  launch_k((rotary_kernel<T, VEC, NEIGH>), (unsigned)ceil_div(units, 4), 128, smem, stream, a);
+  launch_k((rotary_kernel<T, VEC, NEIGH, false>), (unsigned)ceil_div(units, 4), 128, smem, stream, a);
   return launch_status();
 }
 

@@ -208,112 +208,186 @@ sandwich_vec_kernel(const __grid_constant__ Sandwich a) {
   }
 }
 
-// Rows of any length and alignment: a CTA a row by single elements, x and the
-// residual read again from cache.
-template <typename T>
-__global__ void __launch_bounds__(512)
+// VEC elements (a 16-byte pack, or one) as fp32 and back.
+template <typename T, int VEC>
+__device__ __forceinline__ void get(const T* p, float (&f)[VEC]) {
+  if constexpr (VEC == 1) f[0] = Elem<T>::to_f(*p);
+  else unpack<T>(ld_plain(p), f);
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void put(T* p, const float (&f)[VEC]) {
+  if constexpr (VEC == 1) *p = Elem<T>::from_f(f[0]);
+  else st_stream(p, pack<T>(f));
+}
+
+// Rows of any length (VEC a pack) and alignment (VEC 1): TPR threads a row, x
+// and the residual read again from cache.
+template <typename T, int VEC, int TPR>
+__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR)
 sandwich_loop_kernel(const __grid_constant__ Sandwich a) {
   pdl_prologue();
-  constexpr int BLOCK = 512;
-  __shared__ float smem[BLOCK / 32];
+  constexpr int BLOCK = TPR < 128 ? 128 : TPR, TEAMS = BLOCK / TPR;
+  __shared__ float4 sums[2 * BLOCK / 32];
   const T *post = static_cast<const T*>(a.post), *pre = static_cast<const T*>(a.pre);
-  for (uint32_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+  const int lane = threadIdx.x % TPR * VEC;
+  const float inv_n = 1.f / (float)a.cols;
+  for (uint32_t row = blockIdx.x * TEAMS + threadIdx.x / TPR; row < a.rows; row += gridDim.x * TEAMS) {
     const T* xr = static_cast<const T*>(a.x) + row * a.ldx;
     const T* rr = static_cast<const T*>(a.res) + row * a.ldr;
     const T* gr = gate_row<T>(a, row);
     T* hr = static_cast<T*>(a.h) + (int64_t)row * a.cols;
     T* yr = static_cast<T*>(a.y) + (int64_t)row * a.cols;
-    float ss = 0.f;
-    for (int c = threadIdx.x; c < a.cols; c += BLOCK) {
-      const float f = Elem<T>::to_f(xr[c]);
-      ss = fmaf(f, f, ss);
+    float ss[1] = {0.f};
+#pragma unroll 4
+    for (int c = lane; c < a.cols; c += TPR * VEC) {
+      float f[VEC];
+      get<T, VEC>(xr + c, f);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) ss[0] = fmaf(f[e], f[e], ss[0]);
     }
-    ss = block_reduce<SumOp, BLOCK>(ss, smem);
-    const float rx = a.scale / sqrtf(ss / (float)a.cols + a.eps);
-    auto sum_of = [&](int c) {
-      float f = Elem<T>::to_f(xr[c]) * rx * (Elem<T>::to_f(post[c]) + a.off);
-      if (gr != nullptr) f *= Elem<T>::to_f(gr[c]);
-      return f + Elem<T>::to_f(rr[c]);
+    team_sum<TPR, BLOCK>(ss, sums, 0);
+    const float rx = a.scale * rsqrtf(fmaf(ss[0], inv_n, a.eps));
+    auto sum_of = [&](int c, float (&f)[VEC]) {
+      float w[VEC];
+      get<T, VEC>(xr + c, f);
+      get<T, VEC>(post + c, w);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) f[e] = f[e] * rx * (w[e] + a.off);
+      if (gr != nullptr) {
+        get<T, VEC>(gr + c, w);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) f[e] *= w[e];
+      }
+      get<T, VEC>(rr + c, w);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) f[e] += w[e];
     };
-    ss = 0.f;
-    for (int c = threadIdx.x; c < a.cols; c += BLOCK) {
-      const float f = sum_of(c);
-      ss = fmaf(f, f, ss);
-      hr[c] = Elem<T>::from_f(f);
+    ss[0] = 0.f;
+#pragma unroll 2
+    for (int c = lane; c < a.cols; c += TPR * VEC) {
+      float f[VEC];
+      sum_of(c, f);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) ss[0] = fmaf(f[e], f[e], ss[0]);
+      put<T, VEC>(hr + c, f);
     }
-    ss = block_reduce<SumOp, BLOCK>(ss, smem);
-    const float rh = 1.0f / sqrtf(ss / (float)a.cols + a.eps);
-    for (int c = threadIdx.x; c < a.cols; c += BLOCK)
-      yr[c] = Elem<T>::from_f(sum_of(c) * rh * (Elem<T>::to_f(pre[c]) + a.off));
+    team_sum<TPR, BLOCK>(ss, sums, 1);
+    const float rh = rsqrtf(fmaf(ss[0], inv_n, a.eps));
+#pragma unroll 2
+    for (int c = lane; c < a.cols; c += TPR * VEC) {
+      float f[VEC], w[VEC];
+      sum_of(c, f);
+      get<T, VEC>(pre + c, w);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) f[e] = f[e] * rh * (w[e] + a.off);
+      put<T, VEC>(yr + c, f);
+    }
   }
 }
 
 // ------------------------------------------------------------- backward ---
 // Rows of any length and alignment: the row gradients and the row's
 // statistics, then the column sums in a second pass over the operands.
-template <typename T>
-__global__ void __launch_bounds__(512)
+template <typename T, int VEC, int TPR>
+__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR)
 sandwich_bwd_rows_kernel(const __grid_constant__ Sandwich a) {
   pdl_prologue();
-  constexpr int BLOCK = 512;
-  __shared__ float smem[BLOCK / 32];
+  constexpr int BLOCK = TPR < 128 ? 128 : TPR, TEAMS = BLOCK / TPR;
+  __shared__ float4 sums[2 * BLOCK / 32];
   const T *post = static_cast<const T*>(a.post), *pre = static_cast<const T*>(a.pre);
-  for (uint32_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+  const int lane = threadIdx.x % TPR * VEC;
+  const float inv_n = 1.f / (float)a.cols;
+  for (uint32_t row = blockIdx.x * TEAMS + threadIdx.x / TPR; row < a.rows; row += gridDim.x * TEAMS) {
     const T* xr = static_cast<const T*>(a.x) + row * a.ldx;
     const T* hr = static_cast<const T*>(a.hs) + row * a.lds;
     const T* dyr = static_cast<const T*>(a.dy) + row * a.ldy;
     const T* dhr = a.dh == nullptr ? nullptr : static_cast<const T*>(a.dh) + row * a.ldh;
     const T* gr = gate_row<T>(a, row);
-    float sx = 0.f, sh = 0.f, sd = 0.f;
-    for (int c = threadIdx.x; c < a.cols; c += BLOCK) {
-      const float x = Elem<T>::to_f(xr[c]), h = Elem<T>::to_f(hr[c]);
-      const float d = Elem<T>::to_f(dyr[c]) * (Elem<T>::to_f(pre[c]) + a.off);
-      sx = fmaf(x, x, sx);
-      sh = fmaf(h, h, sh);
-      sd = fmaf(d, h, sd);
+    float v[3] = {0.f, 0.f, 0.f};
+#pragma unroll 2
+    for (int c = lane; c < a.cols; c += TPR * VEC) {
+      float x[VEC], h[VEC], d[VEC], w[VEC];
+      get<T, VEC>(xr + c, x);
+      get<T, VEC>(hr + c, h);
+      get<T, VEC>(dyr + c, d);
+      get<T, VEC>(pre + c, w);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        v[0] = fmaf(x[e], x[e], v[0]);
+        v[1] = fmaf(h[e], h[e], v[1]);
+        v[2] = fmaf(d[e] * (w[e] + a.off), h[e], v[2]);
+      }
     }
-    sx = block_reduce<SumOp, BLOCK>(sx, smem);
-    sh = block_reduce<SumOp, BLOCK>(sh, smem);
-    sd = block_reduce<SumOp, BLOCK>(sd, smem);
-    const float n = (float)a.cols;
-    const float rx = 1.0f / sqrtf(sx / n + a.eps), rh = 1.0f / sqrtf(sh / n + a.eps);
-    const float mean = sd * rh / n;
-    auto grad = [&](int c) {
-      const float d = Elem<T>::to_f(dyr[c]) * (Elem<T>::to_f(pre[c]) + a.off);
-      const float g = rh * (d - Elem<T>::to_f(hr[c]) * rh * mean);
-      return dhr == nullptr ? g : g + Elem<T>::to_f(dhr[c]);
+    team_sum<TPR, BLOCK>(v, sums, 0);
+    const float rx = rsqrtf(fmaf(v[0], inv_n, a.eps)), rh = rsqrtf(fmaf(v[1], inv_n, a.eps));
+    const float mean = v[2] * rh * inv_n;
+    auto grad = [&](int c, float (&g)[VEC]) {
+      float h[VEC], w[VEC];
+      get<T, VEC>(dyr + c, g);
+      get<T, VEC>(hr + c, h);
+      get<T, VEC>(pre + c, w);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) g[e] = rh * (g[e] * (w[e] + a.off) - h[e] * rh * mean);
+      if (dhr != nullptr) {
+        get<T, VEC>(dhr + c, w);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) g[e] += w[e];
+      }
     };
-    auto weight = [&](int c) {
-      const float w = a.scale * (Elem<T>::to_f(post[c]) + a.off);
-      return gr == nullptr ? w : w * Elem<T>::to_f(gr[c]);
+    auto weigh = [&](int c, float (&g)[VEC]) {
+      float w[VEC];
+      get<T, VEC>(post + c, w);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) g[e] *= a.scale * (w[e] + a.off);
+      if (gr != nullptr) {
+        get<T, VEC>(gr + c, w);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) g[e] *= w[e];
+      }
     };
-    float st = 0.f;
-    for (int c = threadIdx.x; c < a.cols; c += BLOCK) {
-      const float g = grad(c);
-      st = fmaf(g * weight(c), Elem<T>::to_f(xr[c]), st);
-      static_cast<T*>(a.dres)[(int64_t)row * a.cols + c] = Elem<T>::from_f(g);
+    float u[1] = {0.f};
+#pragma unroll 2
+    for (int c = lane; c < a.cols; c += TPR * VEC) {
+      float g[VEC], x[VEC];
+      grad(c, g);
+      put<T, VEC>(static_cast<T*>(a.dres) + (int64_t)row * a.cols + c, g);
+      weigh(c, g);
+      get<T, VEC>(xr + c, x);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) u[0] = fmaf(g[e], x[e], u[0]);
     }
-    st = block_reduce<SumOp, BLOCK>(st, smem);
-    const float mean_t = st * rx / n;
-    for (int c = threadIdx.x; c < a.cols; c += BLOCK)
-      static_cast<T*>(a.dx)[(int64_t)row * a.cols + c] =
-          Elem<T>::from_f(rx * (grad(c) * weight(c) - Elem<T>::to_f(xr[c]) * rx * mean_t));
-    if (threadIdx.x == 0) a.stats[row] = make_float4(rx, rh, mean, 0.f);
+    team_sum<TPR, BLOCK>(u, sums, 1);
+    const float back = rx * rx * (u[0] * rx * inv_n);
+#pragma unroll 2
+    for (int c = lane; c < a.cols; c += TPR * VEC) {
+      float g[VEC], x[VEC];
+      grad(c, g);
+      weigh(c, g);
+      get<T, VEC>(xr + c, x);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) g[e] = rx * g[e] - x[e] * back;
+      put<T, VEC>(static_cast<T*>(a.dx) + (int64_t)row * a.cols + c, g);
+    }
+    if (lane == 0) a.stats[row] = make_float4(rx, rh, mean, 0.f);
   }
 }
 
-// A thread a column of a chunk of rows (blockIdx.y).
-template <typename T>
+// A thread VEC columns of a chunk of rows (blockIdx.y).
+template <typename T, int VEC>
 __global__ void __launch_bounds__(128)
 sandwich_bwd_cols_kernel(const __grid_constant__ Sandwich a) {
   pdl_prologue();
-  const int c = blockIdx.x * 128 + threadIdx.x;
+  const int c = (blockIdx.x * 128 + threadIdx.x) * VEC;
   if (c >= a.cols) return;
   const uint32_t chunk = blockIdx.y;
   const uint32_t r0 = chunk * a.per_chunk, r1 = min(a.rows, r0 + a.per_chunk);
-  const float pre = Elem<T>::to_f(static_cast<const T*>(a.pre)[c]) + a.off;
-  const float post = a.scale * (Elem<T>::to_f(static_cast<const T*>(a.post)[c]) + a.off);
-  float dpre = 0.f, dpost = 0.f, shared[2] = {0.f, 0.f};
+  float pre[VEC], dpre[VEC], dpost[VEC], sum[VEC];
+  get<T, VEC>(static_cast<const T*>(a.pre) + c, pre);
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) {
+    pre[e] += a.off;
+    dpre[e] = dpost[e] = sum[e] = 0.f;
+  }
   uint32_t row = r0;
   while (row < r1) {  // one gate row a turn
     const uint32_t seg = row / a.per_gate;
@@ -321,32 +395,56 @@ sandwich_bwd_cols_kernel(const __grid_constant__ Sandwich a) {
     const uint32_t end = seg_end < r1 ? (uint32_t)seg_end : r1;
     const bool whole = (uint64_t)seg * a.per_gate >= r0 && (seg_end <= r1 || (r1 == a.rows));
     const bool is_first = seg == r0 / a.per_gate;
-    float sum = 0.f;
-#pragma unroll 4
+#pragma unroll(VEC == 1 ? 4 : 2)
     for (; row < end; ++row) {
       const float4 s = a.stats[row];
-      const float dy = Elem<T>::to_f(static_cast<const T*>(a.dy)[row * a.ldy + c]);
-      const float m = Elem<T>::to_f(static_cast<const T*>(a.hs)[row * a.lds + c]) * s.y;
-      const float x = Elem<T>::to_f(static_cast<const T*>(a.x)[row * a.ldx + c]);
-      float g = s.y * (dy * pre - m * s.z);
-      if (a.dh != nullptr) g += Elem<T>::to_f(static_cast<const T*>(a.dh)[row * a.ldh + c]);
-      dpre = fmaf(dy, m, dpre);
-      sum = fmaf(g, x * s.x, sum);
+      float dy[VEC], m[VEC], x[VEC], g[VEC];
+      get<T, VEC>(static_cast<const T*>(a.dy) + row * a.ldy + c, dy);
+      get<T, VEC>(static_cast<const T*>(a.hs) + row * a.lds + c, m);
+      get<T, VEC>(static_cast<const T*>(a.x) + row * a.ldx + c, x);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        m[e] *= s.y;
+        g[e] = s.y * (dy[e] * pre[e] - m[e] * s.z);
+        dpre[e] = fmaf(dy[e], m[e], dpre[e]);
+      }
+      if (a.dh != nullptr) {
+        get<T, VEC>(static_cast<const T*>(a.dh) + row * a.ldh + c, m);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) g[e] += m[e];
+      }
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) sum[e] = fmaf(g[e], x[e] * s.x, sum[e]);
     }
     if (a.gate != nullptr) {
       const int64_t at = (int64_t)seg * a.cols + c;
-      dpost = fmaf(a.scale * Elem<T>::to_f(static_cast<const T*>(a.gate)[at]), sum, dpost);
-      if (whole) static_cast<T*>(a.dgate)[at] = Elem<T>::from_f(post * sum);
-      else shared[is_first ? 0 : 1] = sum;
+      float g[VEC], w[VEC];
+      get<T, VEC>(static_cast<const T*>(a.gate) + at, g);
+      get<T, VEC>(static_cast<const T*>(a.post) + c, w);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        dpost[e] = fmaf(a.scale * g[e], sum[e], dpost[e]);
+        w[e] = a.scale * (w[e] + a.off) * sum[e];
+      }
+      if (whole) {
+        put<T, VEC>(static_cast<T*>(a.dgate) + at, w);
+      } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) a.shared[((int64_t)chunk * 2 + (is_first ? 0 : 1)) * a.cols + c + e] = sum[e];
+      }
     } else {
-      dpost = fmaf(a.scale, sum, dpost);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) dpost[e] = a.scale * sum[e];
     }
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) sum[e] = 0.f;
   }
   const int64_t at = (int64_t)chunk * 2 * a.cols + c;
-  a.parts[at] = dpre;
-  a.parts[at + a.cols] = dpost;
-  a.shared[at] = shared[0];
-  a.shared[at + a.cols] = shared[1];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) {
+    a.parts[at + e] = dpre[e];
+    a.parts[at + a.cols + e] = dpost[e];
+  }
 }
 
 // Adds the chunks' partial sums: blockIdx.y == 0 dpre and dpost, y > 0 a gate
@@ -671,22 +769,39 @@ Plan plan_teams(int64_t rows, int64_t packs, int sms) {
   const int per_cta = team >= 256 ? 1 : 256 / team;
   return deal(rows, (int64_t)sms * (team == 512 ? 1 : 2) * per_cta, per_cta, team);
 }
-// About 8 CTAs an SM of 128 columns and at least 8 rows.
-Plan plan_columns(int64_t rows, int64_t cols, int sms) {
-  return deal(rows, std::max<int64_t>(1, std::min(ceil_div(8ll * sms, ceil_div(cols, 128)), ceil_div(rows, 8))), 1, 0);
+// About 8 CTAs an SM of 128 columns (or packs) and at least 8 rows.
+Plan plan_columns(int64_t rows, int64_t units, int sms) {
+  return deal(rows, std::max<int64_t>(1, std::min(ceil_div(8ll * sms, ceil_div(std::max<int64_t>(units, 1), 128)), ceil_div(rows, 8))), 1, 0);
 }
-// Both plans' needs (which of them a call takes hangs on its alignment too).
+// All plans' needs (which of them a call takes hangs on its alignment too).
 size_t bwd_workspace(int64_t rows, int64_t cols, int64_t packs, int sms) {
-  const Plan a = plan_teams(rows, packs, sms), b = plan_columns(rows, cols, sms);
-  return (size_t)rows * sizeof(float4) +
-         (size_t)2 * cols * sizeof(float) * std::max<size_t>((size_t)a.chunks + a.n_parts, (size_t)b.chunks + b.n_parts);
+  size_t most = 0;
+  for (const Plan& p : {plan_teams(rows, packs, sms), plan_columns(rows, cols, sms), plan_columns(rows, packs, sms)})
+    most = std::max(most, (size_t)p.chunks + p.n_parts);
+  return (size_t)rows * sizeof(float4) + (size_t)2 * cols * sizeof(float) * most;
+}
+
+// Calls f(VEC, TPR) for rows read by packs or by single elements: at least
+// four of them a thread, up to 512 threads.
+template <typename T, typename F>
+void by_length(int64_t cols, bool packs, F&& f) {
+  using std::integral_constant;
+  auto threads = [&](auto vec) {
+    const int64_t units = cols / decltype(vec)::value;
+    if (units <= 128) f(vec, integral_constant<int, 32>{});
+    else if (units <= 1024) f(vec, integral_constant<int, 128>{});
+    else f(vec, integral_constant<int, 512>{});
+  };
+  if (packs) threads(integral_constant<int, Elem<T>::kVec>{});
+  else threads(integral_constant<int, 1>{});
 }
 
 template <typename T>
 int launch_fwd(const Sandwich& a, const DeviceInfo& dev, cudaStream_t stream) {
   constexpr int VW = Elem<T>::kVec;
-  if (a.cols % VW == 0 && a.ldx % VW == 0 && a.ldr % VW == 0 && aligned16(a.x) && aligned16(a.res) &&
-      aligned16(a.post) && aligned16(a.pre) && aligned16(a.gate) && aligned16(a.y) && aligned16(a.h)) {
+  const bool packs = a.cols % VW == 0 && a.ldx % VW == 0 && a.ldr % VW == 0 && aligned16(a.x) && aligned16(a.res) &&
+                     aligned16(a.post) && aligned16(a.pre) && aligned16(a.gate) && aligned16(a.y) && aligned16(a.h);
+  if (packs) {
     // 4096 columns of 16 bits: 256 threads of two packs (65536 rows 346 us; 128 of four 465 us)
     const int r = row_ladder<2>(a.cols / VW, [&](auto tpr, auto vpt) -> int {
       constexpr int TPR = decltype(tpr)::value, VPT = decltype(vpt)::value;
@@ -697,7 +812,12 @@ int launch_fwd(const Sandwich& a, const DeviceInfo& dev, cudaStream_t stream) {
     });
     if (r >= 0) return r;
   }
-  launch_k(sandwich_loop_kernel<T>, (unsigned)std::min<int64_t>(a.rows, 4ll * dev.sm_count), 512, 0, stream, a);
+  by_length<T>(a.cols, packs, [&](auto vec, auto tpr) {
+    constexpr int TPR = decltype(tpr)::value, BLOCK = TPR < 128 ? 128 : TPR;
+    launch_k((sandwich_loop_kernel<T, decltype(vec)::value, TPR>),
+             (unsigned)std::min<int64_t>(ceil_div(a.rows, BLOCK / TPR), 2048ll / BLOCK * dev.sm_count), BLOCK, 0, stream,
+             a);
+  });
   return launch_status();
 }
 
@@ -718,19 +838,26 @@ template <typename T>
 int launch_bwd(Sandwich a, const DeviceInfo& dev, float* ws, cudaStream_t stream) {
   constexpr int VW = Elem<T>::kVec;
   const int64_t packs = a.cols / VW;
-  const bool staged = packs <= 512 * kBwdVpt && a.cols % VW == 0 && a.ldx % VW == 0 && a.lds % VW == 0 &&
+  const bool whole = a.cols % VW == 0 && a.ldx % VW == 0 && a.lds % VW == 0 &&
                       a.ldy % VW == 0 && a.ldh % VW == 0 && aligned16(a.x) && aligned16(a.hs) && aligned16(a.dy) &&
                       aligned16(a.dh) && aligned16(a.post) && aligned16(a.pre) && aligned16(a.gate) &&
                       aligned16(a.dx) && aligned16(a.dres) && aligned16(a.dgate);
-  const Plan p = staged ? plan_teams(a.rows, packs, dev.sm_count) : plan_columns(a.rows, a.cols, dev.sm_count);
+  const Plan p = whole && packs <= 512 * kBwdVpt ? plan_teams(a.rows, packs, dev.sm_count)
+                                                 : plan_columns(a.rows, whole ? packs : a.cols, dev.sm_count);
   a.chunks = p.chunks, a.per_chunk = p.per_chunk, a.n_parts = p.n_parts;
   a.parts = ws;
   a.shared = ws + (int64_t)2 * p.n_parts * a.cols;
   int st = FL_B200_OK;
   switch (p.team) {
     case 0:
-      launch_k(sandwich_bwd_rows_kernel<T>, (unsigned)std::min<int64_t>(a.rows, 4ll * dev.sm_count), 512, 0, stream, a);
-      launch_k(sandwich_bwd_cols_kernel<T>, dim3((unsigned)ceil_div(a.cols, 128), a.chunks), 128, 0, stream, a);
+      by_length<T>(a.cols, whole, [&](auto vec, auto tpr) {
+        constexpr int VEC = decltype(vec)::value, TPR = decltype(tpr)::value, BLOCK = TPR < 128 ? 128 : TPR;
+        launch_k((sandwich_bwd_rows_kernel<T, VEC, TPR>),
+                 (unsigned)std::min<int64_t>(ceil_div(a.rows, BLOCK / TPR), 2048ll / BLOCK * dev.sm_count), BLOCK, 0,
+                 stream, a);
+        launch_k((sandwich_bwd_cols_kernel<T, VEC>), dim3((unsigned)ceil_div(a.cols, 128 * VEC), a.chunks), 128, 0,
+                 stream, a);
+      });
       break;
     case 32: st = launch_teams<T, 32>(a, stream); break;
     case 64: st = launch_teams<T, 64>(a, stream); break;
@@ -741,7 +868,8 @@ int launch_bwd(Sandwich a, const DeviceInfo& dev, float* ws, cudaStream_t stream
   if (st != FL_B200_OK) return st;
   const int64_t gates = a.gate ? ceil_div(a.rows, a.per_gate) : 0;
   const int by_gate = gates < a.chunks;
-  const int64_t sums = a.chunks == 1 ? 1 : 1 + std::min<int64_t>(gates, a.chunks - 1);
+  // (chunks of whole gate rows share none)
+  const int64_t sums = a.per_chunk % a.per_gate == 0 ? 1 : 1 + std::min<int64_t>(gates, a.chunks - 1);
   launch_k(sandwich_bwd_sum_kernel<T>, dim3((unsigned)ceil_div(a.cols, 32), (unsigned)sums), 512, 0, stream, a, by_gate);
   return launch_status();
 }

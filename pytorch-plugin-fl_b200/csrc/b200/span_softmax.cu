@@ -561,7 +561,73 @@ span_softmax_kernel(const __grid_constant__ SpanArgs a) {
     if (lane + i * TPR < p.count) put<TO, N>(out, z[i], (p.p0 + lane + i * TPR) * N, p, inv);
 }
 
-// Rows of any length and alignment: a CTA a row, the span read twice.
+// Rows too long for registers: a CTA of 1024 threads a row, the span read
+// twice, the second time from L2.
+template <typename TI, typename TO>
+__global__ void __launch_bounds__(1024)
+span_softmax_long_kernel(const __grid_constant__ SpanArgs a) {
+  pdl_prologue();
+  constexpr int N = Elem<TI>::kVec, TPR = 1024, U = 2;
+  __shared__ float smem[TPR / 32];
+  const int lane = threadIdx.x;
+  const uint32_t row = blockIdx.x;
+  const Row r = row_of(a, row);
+  const Score score(a);
+  const TI* xr = static_cast<const TI*>(a.x) + row * a.ldx;
+  const int shift = shift_of(xr);
+  TO* out = static_cast<TO*>(a.out) + row * a.ldo - shift;
+  const Place<N> p(r, shift, a.cols);
+  xr += (int64_t)p.p0 * N - shift;
+  float m = -INFINITY, s = 0.f;
+  Elems<TI, N> v[U];
+  auto load = [&](int vi) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (vi + u * TPR < p.count) v[u].load(xr + (int64_t)(vi + u * TPR) * N);
+  };
+  load(lane);
+  clear_outside<TO, N, TPR>(out, p, lane);
+  for (int vi = lane; vi < p.count; vi += U * TPR) {
+    Elems<TI, N> w[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) w[u] = v[u];
+    load(vi + U * TPR);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (vi + u * TPR >= p.count) continue;
+      uint64_t z[1][N / 2];
+      w[u].to(z[0]);
+      const float top = scores_of<N>(z[0], (p.p0 + vi + u * TPR) * N, p, r, score, m);
+      if (top > m) {
+        s *= exp_of(m - top);
+        m = top;
+      }
+      // (-inf so far: nothing to add, unless a NaN came without raising the maximum)
+      const float more = exps_of<N, 1, TPR>(z, TPR, m == -INFINITY ? 0.f : m);
+      s += more;
+    }
+  }
+  const float top = row_reduce<FastMaxOp, TPR, TPR>(m, smem);
+  s = row_reduce<SumOp, TPR, TPR>(m == -INFINITY && s == 0.f ? 0.f : s * exp_of(m - top), smem);
+  // (nothing but -inf: 0 / 0 as in softmax)
+  const float inv = 1.f / s, base = top == -INFINITY ? 0.f : top;
+  for (int vi = lane; vi < p.count; vi += U * TPR) {
+    load(vi);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (vi + u * TPR >= p.count) continue;
+      uint64_t z[1][N / 2];
+      const int at = (p.p0 + vi + u * TPR) * N;
+      v[u].to(z[0]);
+      (void)scores_of<N>(z[0], at, p, r, score, -INFINITY);
+      (void)exps_of<N, 1, TPR>(z, TPR, base);
+      put<TO, N>(out, z[0], at, p, inv);
+    }
+  }
+}
+
+// Rows whose output lies otherwise than their input: a CTA a row by single
+// elements.
 template <typename TI, typename TO>
 __global__ void __launch_bounds__(512)
 span_softmax_loop_kernel(const __grid_constant__ SpanArgs a) {
@@ -788,6 +854,73 @@ span_softmax_bwd_kernel(const __grid_constant__ SpanArgs a) {
   span_bwd_row<TI, TY, TPR, VPT>(a, blockIdx.x, row_of(a, blockIdx.x), Score(a), threadIdx.x, smem);
 }
 
+// Rows too long for registers: a CTA of 1024 threads a row, y and dy read
+// twice.
+template <typename TI, typename TY>
+__global__ void __launch_bounds__(1024)
+span_softmax_bwd_long_kernel(const __grid_constant__ SpanArgs a) {
+  pdl_prologue();
+  constexpr int N = Elem<TI>::kVec, TPR = 1024;
+  __shared__ float smem[TPR / 32];
+  const int lane = threadIdx.x;
+  const uint32_t row = blockIdx.x;
+  const Row r = row_of(a, row);
+  const Score score(a);
+  const bool capped = score.cap != 0.f;
+  TI* out = static_cast<TI*>(a.out) + row * a.ldo;
+  const int shift = shift_of(out);
+  out -= shift;
+  const Place<N> p(r, shift, a.cols);
+  const int64_t skip = (int64_t)p.p0 * N - shift;
+  const TY* yr = static_cast<const TY*>(a.y) + row * a.ldy + skip;
+  const TY* dr = static_cast<const TY*>(a.dy) + row * a.ldd + skip;
+  const TI* xr = static_cast<const TI*>(a.x) + (capped ? row * a.ldx + skip : 0);
+  clear_outside<TI, N, TPR>(out, p, lane);
+  uint64_t f[N / 2], g[N / 2], acc[2] = {f2_make(0.f, 0.f), f2_make(0.f, 0.f)};
+  auto get = [&](int vi) {
+    Elems<TY, N> y, d;
+    y.load(yr + (int64_t)vi * N);
+    d.load(dr + (int64_t)vi * N);
+    const int at = (p.p0 + vi) * N;
+    if (!p.inside(at)) {
+      y.keep(p.lo - at, p.hi - at);
+      d.keep(p.lo - at, p.hi - at);
+    }
+    y.to(f);
+    d.to(g);
+  };
+#pragma unroll 2
+  for (int vi = lane; vi < p.count; vi += TPR) {
+    get(vi);
+#pragma unroll
+    for (int e = 0; e < N / 2; ++e) acc[e & 1] = f2_fma(f[e], g[e], acc[e & 1]);
+  }
+  acc[0] = f2_add(acc[0], acc[1]);
+  const float sum = row_reduce<SumOp, TPR, TPR>(f2_lo(acc[0]) + f2_hi(acc[0]), smem);
+  const float by = capped ? 4.f * a.scale : a.scale;
+  const uint64_t minus = f2_make(-sum, -sum), times = f2_make(by, by), minus_one = f2_make(-1.f, -1.f);
+#pragma unroll 2
+  for (int vi = lane; vi < p.count; vi += TPR) {
+    const int at = (p.p0 + vi) * N;
+    Elems<TI, N> x;
+    if (capped) x.load(xr + (int64_t)vi * N);
+    get(vi);
+#pragma unroll
+    for (int e = 0; e < N / 2; ++e) f[e] = f2_mul(f2_mul(f[e], times), f2_add(g[e], minus));
+    if (capped) {
+      if (!p.inside(at)) x.keep(p.lo - at, p.hi - at);
+      x.to(g);
+#pragma unroll
+      for (int e = 0; e < N / 2; ++e) {
+        const uint64_t q = score.half_of(g[e]);
+        f[e] = f2_mul(f[e], f2_fma(f2_mul(q, minus_one), q, q));
+      }
+    }
+    if (!(fabsf(sum) < 3e38f) && !p.inside(at)) p.mask(f, at, 0.f);
+    store<TI, N>(out, at, p.first, p.last, f);
+  }
+}
+
 template <typename TI, typename TY>
 __global__ void __launch_bounds__(512)
 span_softmax_bwd_loop_kernel(const __grid_constant__ SpanArgs a) {
@@ -879,6 +1012,8 @@ int launch_fwd(SpanArgs a, const DeviceInfo& dev, cudaStream_t stream) {
       }
     });
     if (st >= 0) return st;
+    launch_k((span_softmax_long_kernel<TI, TO>), a.rows, 1024, 0, stream, a);
+    return launch_status();
   }
   const unsigned grid = (unsigned)std::min<int64_t>(a.rows, 4ll * dev.sm_count);
   launch_k((span_softmax_loop_kernel<TI, TO>), grid, 512, 0, stream, a);
@@ -903,6 +1038,8 @@ int launch_bwd(SpanArgs a, const DeviceInfo& dev, cudaStream_t stream) {
       }
     });
     if (st >= 0) return st;
+    launch_k((span_softmax_bwd_long_kernel<TI, TY>), a.rows, 1024, 0, stream, a);
+    return launch_status();
   }
   const unsigned grid = (unsigned)std::min<int64_t>(a.rows, 4ll * dev.sm_count);
   launch_k((span_softmax_bwd_loop_kernel<TI, TY>), grid, 512, 0, stream, a);

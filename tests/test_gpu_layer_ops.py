@@ -947,3 +947,45 @@ def test_clip_through_the_dispatcher_and_versions():
         torch_fl.ops.clip_grads([ts[0], torch.zeros(3)], 1.0, out=[ts[0], torch.zeros(3)])   # on the CPU
     with pytest.raises(RuntimeError):
         torch_fl.ops.grad_norm([torch.zeros(3)])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("B,S,Hq,Hk,D,n", [(7, 3001, 1, 1, 80, 40), (30, 997, 2, 1, 64, 8), (1500, 13, 1, 0, 16, 4),
+                                           (9000, 2, 1, 1, 24, 5), (20000, 1, 1, 1, 8, 4)])
+def test_rotary_many_tokens_of_few_heads(dtype, B, S, Hq, Hk, D, n):
+    g = gen(B + S)
+    q, k = (torch.randn(B, S, h, D, generator=g).to(dtype).to(DEV) for h in (Hq, Hk))
+    freq = (1e4 ** (-torch.arange(n, dtype=torch.float64) / n)).float().to(DEV)
+    pos = torch.randint(0, 131072, (B, S), generator=g).to(DEV)
+    for interleaved in (False, True):
+        check_rotary(q, k, pos, freq, 1.25, interleaved)
+
+
+@pytest.mark.parametrize("gate", ["none", "channel", "sequence", "token"])
+@pytest.mark.parametrize("B,S,H", [(3, 700, 1001), (2, 9, 9280), (5, 60, 758), (1, 3, 33000), (300, 2, 129), (2, 150, 10248)])
+def test_sandwich_rows_by_packs_and_by_elements(gate, B, S, H):
+    test_sandwich(torch.float16, gate, (B, S, H))
+    test_sandwich(torch.float32, gate, (B, S, H))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cap,bias", [(None, False), (20.0, True)])
+def test_span_softmax_long_rows(dtype, cap, bias):
+    g = gen(41)
+    for n in (33000, 70001):
+        x = (4 * torch.randn(1, 2, 5, n, generator=g)).to(dtype).to(DEV)
+        slopes = torch.tensor([0.01, 0.001]).to(DEV) if bias else None
+        check_span(x, random_spans(1, 5, n, g), 0.5, cap, slopes)
+        x[0, 0, 1, n // 3:n // 2] = -math.inf                   # whole packs of nothing
+        if not cap:
+            y = torch_fl.ops.span_softmax(x, torch.tensor([[0, n]] * 5).int().to(DEV))
+            assert not torch.isnan(y).any() and not y[0, 0, 1, n // 3:n // 2].any()
+            assert abs(float(y[0, 0, 1].double().sum()) - 1) < 2.0 ** -8
+
+
+def test_span_softmax_output_in_another_step():
+    """Rows that begin elsewhere in a 16-byte pack than their results do."""
+    g = gen(42)
+    wide = (2 * torch.randn(2, 2, 6, 97, generator=g)).half().to(DEV)
+    for at in range(4):
+        check_span(wide[..., at:at + 90], random_spans(2, 6, 90, g), 0.5, 20.0)
