@@ -456,23 +456,47 @@ span_softmax_warp_kernel(const __grid_constant__ SpanArgs a, int room) {
       z4 += kBlock;
       at += 32 * N;
     };
+    const bool more = rows.more;
+    const uint32_t then = rows.w.row;
+    const Row next(ahead, a.cols);
+    Place<N> then_p = p;
+    auto turn = [&]() {  // to the next row
+      if (!more) return;
+      then_p = place(then, next);
+      xr = span_at(then, then_p);
+      load(xr, lane, then_p.count);
+      rows.next(a);
+      if (rows.more) ahead = rows.w.read(a);
+    };
+    if (p.count <= 64) {  // two packs a lane: they stay in registers
+      const bool two = p.count > 32;
+      uint64_t y[2][1][N / 2];
+      v[0].to(y[0][0]);
+      m = scores_of<N>(y[0][0], at, p, r, score, m);
+      if (two) {
+        v[1].to(y[1][0]);
+        m = scores_of<N>(y[1][0], at + 32 * N, p, r, score, m);
+      }
+      m = group_reduce_warp<FastMaxOp, 32>(m);
+      float s = exps_of<N, 1, 32>(y[0], 1, m);
+      if (two) s += exps_of<N, 1, 32>(y[1], 1, m);
+      const float inv = rcp(group_reduce_warp<SumOp, 32>(s));
+      if (lane < p.count) put<TO, N>(out, y[0][0], at, p, inv);
+      if (lane + 32 < p.count) put<TO, N>(out, y[1][0], at + 32 * N, p, inv);
+      turn();
+      if (!more) break;
+      row = then;
+      r = next;
+      p = then_p;
+      continue;
+    }
     for (int done = 0; done < p.count; done += 64) {
       const Elems<TI, N> v0 = v[0], v1 = v[1];
       load(xr, done + 64 + lane, p.count);
       keep(v0);
       if (done + 32 < p.count) keep(v1);
     }
-    const bool more = rows.more;
-    const uint32_t then = rows.w.row;
-    const Row next(ahead, a.cols);
-    Place<N> then_p = p;
-    if (more) {
-      then_p = place(then, next);
-      xr = span_at(then, then_p);
-      load(xr, lane, then_p.count);
-      rows.next(a);
-      if (rows.more) ahead = rows.w.read(a);
-    }
+    turn();
     m = group_reduce_warp<FastMaxOp, 32>(m);
     // one FMA an element: the rounding of m log2 e is a factor all of them
     // share; a maximum that could overflow there is subtracted first
