@@ -6,17 +6,20 @@
 //   z_j -= slope_h |p - j| where slopes are given, p the query's position;
 //   y_j = exp(z_j) / sum over the span of exp(z);  0 outside it.
 // Causal and sliding-window masks, packed documents, bidirectional prefixes
-// and padded batches are all spans, so there is no mask tensor, and keys
-// outside a span are never read.
+// and padded batches are all spans, so there is no mask tensor, and of what
+// lies outside a span only the rest of its first and last 16 bytes is read.
 //   dx_j = scale (1 - tanh^2) y_j (dy_j - sum over the span of y dy).
 //
-// Bound by memory: the span is read once, the row written once.  A row is
-// held in registers (a warp up to 256 packs, then a CTA of 4 packs a thread),
-// its scores as fp32 between the passes.  Rows need not begin
-// on a 16-byte boundary: they are walked by the aligned packs that cover
-// them, elements outside masked and the row's first and last pack stored by
-// element.  (An aligned pack that holds one byte of the row lies in that
-// byte's page, so reading all of it is safe.)
+// The span is read once and the row written once (a row too long for a CTA's
+// registers is read a second time, from L2): a warp a row up to 2048 keys of
+// 16 bits, then a CTA a row, scores as fp32 between the passes.  Long spans
+// are bound by memory (2048 of 2048 keys, bf16: 4.5 TB/s), short ones by the
+// instructions a row costs before its first key (340 of the 470 of a row of
+// 200 keys, 5.4 TB/s with the zeros around them), capped ones by theirs.
+// Rows need not begin on a 16-byte boundary: they are walked by the aligned
+// packs that cover them, elements outside masked and the row's first and last
+// pack stored by element.  (An aligned pack that holds one byte of the row
+// lies in that byte's page, so reading all of it is safe.)
 //
 // Exponentials are ex2.approx (2^-22 relative) of differences from the row's
 // maximum.  tanh u = 1 - 2 / (1 + 2^(2 u log2 e)) by ex2.approx and
@@ -71,9 +74,10 @@ struct Raw {
 };
 struct Row {
   int lo, hi;  // clamped; lo == hi: nothing is seen
-  float pos, slope;
+  int pos;     // whole, so that the distance to a key is exact wherever both lie
+  float slope;
   __device__ __forceinline__ Row(const Raw& r, int cols)
-      : lo(max(r.lo, 0)), hi(min(r.hi, cols)), pos((float)r.pos), slope(r.slope) {
+      : lo(max(r.lo, 0)), hi(min(r.hi, cols)), pos(min(max(r.pos, -(1 << 30)), 1 << 30)), slope(r.slope) {
     if (hi <= lo) lo = hi = 0;
   }
 };
@@ -126,7 +130,7 @@ struct Score {
   __device__ __forceinline__ float operator()(float x, int key, const Row& r) const {
     float z = x * mul;
     if (cap != 0.f) z = fmaf(-2.f * cap, rcp(1.f + ex2(z)), cap);
-    if (biased) z = fmaf(-r.slope, fabsf(r.pos - (float)key), z);
+    if (biased) z = fmaf(-r.slope, fabsf((float)(r.pos - key)), z);
     return z;
   }
   // d(score) / d(scale x): 1 - tanh^2 = 4 e / (1 + e)^2
@@ -154,7 +158,7 @@ struct Score {
       for (int e = 0; e < P; ++e) z[e] = f2_mul(z[e], f2_make(mul, mul));
     }
     if (biased) {
-      const float d = r.pos - (float)key;
+      const float d = (float)(r.pos - key);
 #pragma unroll
       for (int e = 0; e < P; ++e)
         z[e] = f2_make(fmaf(-r.slope, fabsf(d - (float)(2 * e)), f2_lo(z[e])),
@@ -328,12 +332,14 @@ __device__ __forceinline__ float scores_of(uint64_t (&z)[N / 2], int at, const P
   return m;
 }
 // Turns scores into exponentials of their differences from m; the sum.  One
-// FMA an element: the rounding of m log2 e is a factor all of them share.  A
-// maximum that could overflow there is subtracted first.
+// FMA an element: the rounding of m log2 e, up to 2^-24 |m| log2 e, is a
+// factor 2^that which all of them share.  Where it could overflow, the maximum
+// is subtracted first.
+constexpr float kWide = 1e6f;
 template <int N, int VPT, int TPR>
 __device__ __forceinline__ float exps_of(uint64_t (&z)[VPT][N / 2], int count, float m) {
   float shift = m * kLog2e;
-  if (!(fabsf(m) < 1e30f)) {
+  if (!(fabsf(m) < kWide)) {
     shift = 0.f;
 #pragma unroll
     for (int i = 0; i < VPT; ++i)
@@ -357,6 +363,21 @@ __device__ __forceinline__ float exps_of(uint64_t (&z)[VPT][N / 2], int count, f
   }
   s[0] = f2_add(s[0], s[1]);
   return f2_lo(s[0]) + f2_hi(s[0]);
+}
+// The same of one pack where a row's exponentials are not all taken from one
+// maximum (by threads with their own, and again in a second pass): the
+// factor would not be shared, so the difference is rounded first.
+template <int N>
+__device__ __forceinline__ float exps_from(uint64_t (&z)[N / 2], float m) {
+  const uint64_t l = f2_make(kLog2e, kLog2e), c = f2_make(-m, -m);
+  uint64_t s = f2_make(0.f, 0.f);
+#pragma unroll
+  for (int e = 0; e < N / 2; ++e) {
+    const uint64_t t = f2_mul(f2_add(z[e], c), l);
+    z[e] = f2_make(ex2(f2_lo(t)), ex2(f2_hi(t)));
+    s = f2_add(s, z[e]);
+  }
+  return f2_lo(s) + f2_hi(s);
 }
 // Exponentials times inv, stored.  Outside the span they are 0, but 0 times
 // an inv that is not finite is not.
@@ -395,13 +416,16 @@ struct Rows {
   }
 };
 
-// A warp a row.  Scores lie in shared memory, fp32, between the passes (a
-// lane reads only what it wrote, so nothing waits for anything): loops whose
-// length is the span's, few registers and 24 warps an SM, where scores in
-// registers gave code for every length, which a short span skipped at half
-// the price of running it, and 16 warps (2048 keys, spans of 200: 670 us
-// against ... for 524288 rows).  The first packs of the next row are loaded
-// while this one's sums go through the warp, and its span before that.
+// A warp a row.  Spans of up to 64 packs stay in registers; longer ones have
+// their scores in shared memory, fp32, between the passes (a lane reads only
+// what it wrote, so nothing waits for anything): loops whose length is the
+// span's, 80 registers and 24 warps an SM.  All of 2048 scores in registers
+// took 110 to 128 of them and 16 warps, code for every length that a short
+// span skipped at half the price of running it, and spills, which this much
+// shared memory leaves no L1 for: 524288 rows of 2048, packed documents,
+// 1431 us with 116 bytes of spills and 672 us without; this 470 us.  The first
+// packs of the next row are loaded while this one's sums go through the warp,
+// and its span before that.
 template <typename TI, typename TO>
 __global__ void __launch_bounds__(256, 3)
 span_softmax_warp_kernel(const __grid_constant__ SpanArgs a, int room) {
@@ -498,10 +522,8 @@ span_softmax_warp_kernel(const __grid_constant__ SpanArgs a, int room) {
     }
     turn();
     m = group_reduce_warp<FastMaxOp, 32>(m);
-    // one FMA an element: the rounding of m log2 e is a factor all of them
-    // share; a maximum that could overflow there is subtracted first
-    float c = -m * kLog2e;
-    if (!(fabsf(m) < 1e30f)) {
+    float c = -m * kLog2e;  // as in exps_of
+    if (!(fabsf(m) < kWide)) {
       c = 0.f;
       z4 = mine;
       for (int done = 0; done < p.count; done += 32, z4 += kBlock)
@@ -627,8 +649,7 @@ span_softmax_long_kernel(const __grid_constant__ SpanArgs a) {
         m = top;
       }
       // (-inf so far: nothing to add, unless a NaN came without raising the maximum)
-      const float more = exps_of<N, 1, TPR>(z, TPR, m == -INFINITY ? 0.f : m);
-      s += more;
+      s += exps_from<N>(z[0], m == -INFINITY ? 0.f : m);
     }
   }
   const float top = row_reduce<FastMaxOp, TPR, TPR>(m, smem);
@@ -644,7 +665,7 @@ span_softmax_long_kernel(const __grid_constant__ SpanArgs a) {
       const int at = (p.p0 + vi + u * TPR) * N;
       v[u].to(z[0]);
       (void)scores_of<N>(z[0], at, p, r, score, -INFINITY);
-      (void)exps_of<N, 1, TPR>(z, TPR, base);
+      (void)exps_from<N>(z[0], base);
       put<TO, N>(out, z[0], at, p, inv);
     }
   }

@@ -989,3 +989,31 @@ def test_span_softmax_output_in_another_step():
     wide = (2 * torch.randn(2, 2, 6, 97, generator=g)).half().to(DEV)
     for at in range(4):
         check_span(wide[..., at:at + 90], random_spans(2, 6, 90, g), 0.5, 20.0)
+
+
+@pytest.mark.parametrize("n", [40, 700, 5000, 40000])
+def test_span_softmax_rows_far_from_zero(n):
+    """Rows whose maximum is so far from 0 that log2 e times it has no digits
+    left behind the point, or no room; the differences in a row stay exact."""
+    g = gen(51)
+    big = [1e3, -1e4, 1e6, -1e7, 1e9, -1e15, 1e22, -1e30, 1e37, 3e38]
+    x = torch.stack([c + torch.randint(0, 9, (n,), generator=g) * max(1.0, abs(c) * 2.0 ** -23) for c in big])
+    y = torch_fl.ops.span_softmax(x[None, None].to(DEV), torch.tensor([[1, n - 1]] * len(big)).int().to(DEV))[0, 0]
+    want = torch.softmax(x[:, 1:n - 1].double(), -1)
+    got = y[:, 1:n - 1].cpu().double()
+    # scale 1: scores are exact; a difference's rounding and ex2, sums of positive terms
+    assert ((got - want).abs() <= want * (n / 512 + 100) * U + 2.0 ** -126).all()
+
+
+def test_span_softmax_distances_far_out():
+    """Positions and keys past 2^24, where floats are whole no longer."""
+    n = 64
+    pos = torch.tensor([(1 << 25) + 3, -(1 << 25) - 1, 5, (1 << 31) - 1, -(1 << 31)], dtype=torch.int32)
+    x = torch.zeros(1, 1, 5, n, device=DEV)
+    y = torch_fl.ops.span_softmax(x, torch.tensor([[0, n]] * 5).int().to(DEV), slopes=torch.ones(1, device=DEV),
+                                  positions=pos.to(DEV)).cpu().double()[0, 0]
+    assert not torch.isnan(y).any()
+    for r in (2,):
+        want = torch.softmax(-(pos[r].double() - torch.arange(n)).abs(), -1)
+        assert ((y[r] - want).abs() <= 100 * U * want + 2.0 ** -126).all()
+    assert torch.allclose(y.sum(-1), torch.ones(5, dtype=torch.float64), atol=1e-5)
