@@ -519,8 +519,8 @@ FL_B200_API int fl_b200_verify_draft(const int64_t* draft_ids, int64_t ld_ids, c
  * even, at most head_dim and FL_B200_ROTARY_MAX.  The angle is exact to      *
  * fp64, its cosine fp32, the result rounded once.  Any alignment.  In place   *
  * (an output with its input's address and strides) allowed, and then only   *
- * the turned part is touched; otherwise outputs share no memory with their   *
- * inputs.                                                                   */
+ * the turned part is touched; otherwise outputs share no memory with inputs,  *
+ * and never with each other.  Heads times the square of a head's packs stay below 2^31.         */
 #define FL_B200_ROTARY_MAX 2048
 FL_B200_API int fl_b200_rotary(
     const void* q, void* q_out, int64_t Hq, int64_t sqb, int64_t sqh, int64_t sqs, int64_t soqb, int64_t soqh,
@@ -562,7 +562,8 @@ FL_B200_API int fl_b200_sandwich_norm_bwd(const void* dy, int64_t ld_dy, const v
  *   z = scale * x;  cap > 0: z = cap * tanh(z / cap);                        *
  *   slopes != NULL: z -= slopes[h] * |p - j|,                               *
  *   out = exp(z) / sum over the span of exp(z), 0 outside it,               *
- * p = positions[b * pos_sb + q * pos_sq] (int32; NULL: q + cols - q_len).     *
+ * p = positions[b * pos_sb + q * pos_sq] (int32, clamped to +-2^30; NULL:      *
+ * q + cols - q_len).                                                         *
  * A row that sees nothing is 0.  Keys outside a span are never used, whatever *
  * they hold; inside it softmax's rules hold (NaN, +inf or nothing but -inf    *
  * give NaN).  out: in_dtype or F32, no memory shared with x.  Any alignment.  */
@@ -590,9 +591,10 @@ FL_B200_API int fl_b200_grad_norm(const void* const* tensors, const int64_t* num
                                   size_t workspace_bytes, fl_b200_stream_t stream);
 /* The same, and outs[i] = tensors[i] * min(1, max_norm / (norm + 1e-6)), in    *
  * fp32 with one rounding; a norm that is not finite makes a factor of NaN or   *
- * 0 as the formula does.  Each output is its tensor itself or shares no memory *
- * with it; fastest where both have the same offset from a 16-byte boundary.    *
- * max_norm >= 0.                                                             */
+ * 0 as the formula does.  Each output is its tensor itself, or shares no       *
+ * memory with any tensor; no two outputs share any (a list that names one      *
+ * tensor twice is refused).  Fastest where a tensor and its output have the    *
+ * same offset from a 16-byte boundary.  max_norm >= 0.                        */
 FL_B200_API int fl_b200_clip_grads(const void* const* tensors, void* const* outs, const int64_t* numels,
                                    const int* dtypes, int64_t count, float max_norm, int max_kind, float* norm,
                                    void* workspace, size_t workspace_bytes, fl_b200_stream_t stream);

@@ -271,7 +271,9 @@ def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None):
     """(clipped, norm): every tensor of the list times
     min(1, max_norm / (norm + 1e-6)), and the norm before, in two launches.
     `out`: tensors of the same shapes and types to write to (a bucket's views,
-    say, or the gradients themselves)."""
+    say, or the gradients themselves), of which no two share memory; a list
+    that names one tensor twice cannot be clipped in place.  Not
+    differentiable."""
     grads = _grads(grads)
     if out is None:
         return torch.ops.flagos.clip_grads(grads, float(max_norm), float(norm_type))

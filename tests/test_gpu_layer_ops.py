@@ -1017,3 +1017,24 @@ def test_span_softmax_distances_far_out():
         want = torch.softmax(-(pos[r].double() - torch.arange(n)).abs(), -1)
         assert ((y[r] - want).abs() <= 100 * U * want + 2.0 ** -126).all()
     assert torch.allclose(y.sum(-1), torch.ones(5, dtype=torch.float64), atol=1e-5)
+
+
+def test_clip_refuses_outputs_that_meet():
+    a, b = torch.ones(1000, device=DEV), torch.full((1000,), 2.0, device=DEV)
+    for grads, out in (([a, a], [a, a]), ([a, b], [b, a]), ([a[:500], a[400:]], [a[:500], a[400:]]),
+                       ([a, b], [a, a]), ([a[:10], b], [a[5:15], b])):
+        with pytest.raises(RuntimeError):
+            torch_fl.ops.clip_grads(grads, 0.1, out=out)
+    assert bool((a == 1).all()) and bool((b == 2).all())
+    # neighbours in one buffer do not meet; one tensor may be counted twice, and clipped to new outputs
+    torch_fl.ops.clip_grads([a[:500], a[500:]], 0.1, out=[a[:500], a[500:]])
+    check_clip([b, b], 0.1)
+
+
+def test_spans_of_documents_on_flagos():
+    ids = torch.tensor([[4, 4, 4, 9, 9, 0], [1, 1, 2, 2, 2, 2]])
+    kw = dict(lengths=torch.tensor([5, 6]), prefix=torch.tensor([2, 0]), window=3)
+    want = torch_fl.ops.attention_spans(6, 6, documents=ids, **kw)
+    got = torch_fl.ops.attention_spans(6, 6, documents=ids.to("flagos"),
+                                       **{k: v.to("flagos") if torch.is_tensor(v) else v for k, v in kw.items()})
+    assert got.device.type == "flagos" and torch.equal(got.cpu(), want)

@@ -154,3 +154,15 @@ def test_empty_calls_touch_nothing():
     sandwich(x=None, rows=0)
     span(x=None, rows=0)
     span(x=None, cols=0)
+
+
+@pytest.mark.parametrize("p,q,n", [((4096, 4096), (4096, 4096), (10, 10)), ((4096, 8192), (8192, 4096), (10, 10)),
+                                   ((4096, 4096 + 16), (1 << 14, 1 << 15), (10, 10)),
+                                   ((4096, 8192), (1 << 14, (1 << 14) + 36), (10, 10))])
+def test_outputs_that_meet_are_refused(p, q, n):
+    """The same tensor twice in place, two that swap places, outputs over each
+    other; two tensors that meet are refused by the workspace only."""
+    with pytest.raises(_abi.FlB200Error) as ei:
+        clip(p=p, q=q, n=n, dtypes=(F32, F32))
+    meets = p[0] == q[0] or p[0] == q[1] or q[1] - q[0] < 40
+    assert ei.value.status == (1 if meets else 6) or (not meets and ei.value.status in (5, 6))
