@@ -138,10 +138,10 @@ __device__ __forceinline__ void team_sum(float (&v)[K], float4* buf, int half) {
 }
 
 // Row in registers: TPR threads, VPT packs of x each; h stays fp32.  65536 x
-// 4096 bf16: 348 us, 6.2 TB/s.  Faster arithmetic is slower here: with rsqrtf
-// for the IEEE square root and division, and one barrier a sum for two, every
-// CTA's stores follow its loads sooner, and the same launch takes 383 to
-// 401 us, whatever the order of its stores.
+// 4096 bf16: 348 us at first, 382 us over seconds.  Faster arithmetic is
+// slower here: with rsqrtf for the IEEE square root and division, and one
+// barrier a sum for two, every CTA's stores follow its loads sooner, and the
+// same launch takes 383 to 401 us at first, whatever the order of its stores.
 template <typename T, int TPR, int VPT, int BLOCK>
 __global__ void __launch_bounds__(BLOCK, ladder_min_blocks<BLOCK>())
 sandwich_vec_kernel(const __grid_constant__ Sandwich a) {
@@ -209,6 +209,115 @@ sandwich_vec_kernel(const __grid_constant__ Sandwich a) {
 #pragma unroll
     for (int p = 0; p < P; ++p) w.v[p] = f2_mul(f2_mul(h[i].v[p], rh), f2_add(w.v[p], off));
     st_stream(static_cast<T*>(a.y) + (int64_t)row * a.cols + (int64_t)vi * VW, w.bits());
+  }
+}
+
+// The same rows staged in shared memory: resident CTAs walk rows in runs, each
+// thread the same VPT packs of every row; the next row's x and residual are
+// copied in by cp.async while this one is worked on, and the weights (and the
+// gate row while it lasts) stay in registers.  65536 x 4096 bf16: 338 us over
+// seconds (6.4 TB/s) with three CTAs an SM; two 414 us, four 367 us.
+template <int TPR, int VPT>
+constexpr int staged_ctas() {
+  return VPT > 2 ? 1 : TPR >= 512 ? 2 : 768 / TPR;
+}
+template <typename T, int TPR, int VPT>
+__global__ void __launch_bounds__(TPR, staged_ctas<TPR, VPT>())
+sandwich_staged_kernel(const __grid_constant__ Sandwich a) {
+  pdl_prologue();
+  constexpr int VW = Elem<T>::kVec, P = VW / 2;
+  constexpr int STAGE = 2 * VPT * TPR;
+  extern __shared__ uint4 dyn[];
+  __shared__ float4 sums[2 * TPR / 32];
+  uint4* stage = dyn + threadIdx.x;
+  const int lane = threadIdx.x;
+  const int nvec = a.cols / VW;
+  const float inv_n = 1.f / (float)a.cols;
+  const uint64_t off = both(a.off);
+  uint4 post[VPT], pre[VPT], gate[VPT];
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int vi = min(lane + i * TPR, nvec - 1);
+    post[i] = ld_cached(static_cast<const T*>(a.post) + (int64_t)vi * VW);
+    pre[i] = ld_cached(static_cast<const T*>(a.pre) + (int64_t)vi * VW);
+  }
+  auto fetch = [&](uint32_t row, int st) {
+    const T* xr = static_cast<const T*>(a.x) + row * a.ldx;
+    const T* rr = static_cast<const T*>(a.res) + row * a.ldr;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int vi = lane + i * TPR;
+      if (vi < nvec) {
+        cp_async16(stage + st * STAGE + i * TPR, xr + (int64_t)vi * VW);
+        cp_async16(stage + st * STAGE + (VPT + i) * TPR, rr + (int64_t)vi * VW);
+      }
+    }
+    cp_async_commit();
+  };
+  uint32_t row = blockIdx.x;
+  fetch(row, 0);
+  uint32_t seg = 0xffffffffu;
+  int st = 0;
+  for (; row < a.rows; row += gridDim.x, st ^= 1) {
+    if (row + gridDim.x < a.rows) {
+      fetch(row + gridDim.x, st ^ 1);
+      cp_async_wait_pending<1>();
+    } else {
+      cp_async_wait_all();
+    }
+    const uint4* in = stage + st * STAGE;
+    if (a.gate != nullptr && row / a.per_gate != seg) {
+      seg = row / a.per_gate;
+#pragma unroll
+      for (int i = 0; i < VPT; ++i)
+        gate[i] = ld_cached(static_cast<const T*>(a.gate) + (int64_t)seg * a.cols + (int64_t)min(lane + i * TPR, nvec - 1) * VW);
+    }
+    uint64_t s2 = both(0.f);
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      if (lane + i * TPR >= nvec) continue;
+      const Pairs<T> f(in[i * TPR]);
+#pragma unroll
+      for (int p = 0; p < P; ++p) s2 = f2_fma(f.v[p], f.v[p], s2);
+    }
+    float ss[1] = {f2_lo(s2) + f2_hi(s2)};
+    team_sum<TPR, TPR>(ss, sums, 0);
+    const uint64_t rx = both(a.scale * rsqrtf(fmaf(ss[0], inv_n, a.eps)));
+    Pairs<T> h[VPT];
+    s2 = both(0.f);
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int vi = lane + i * TPR;
+      if (vi >= nvec) continue;
+      Pairs<T> f(in[i * TPR]);
+      const Pairs<T> w(opaque(post[i]));
+#pragma unroll
+      for (int p = 0; p < P; ++p) f.v[p] = f2_mul(f2_mul(f.v[p], rx), f2_add(w.v[p], off));
+      if (a.gate != nullptr) {
+        const Pairs<T> g(opaque(gate[i]));
+#pragma unroll
+        for (int p = 0; p < P; ++p) f.v[p] = f2_mul(f.v[p], g.v[p]);
+      }
+      const Pairs<T> q(in[(VPT + i) * TPR]);
+#pragma unroll
+      for (int p = 0; p < P; ++p) {
+        h[i].v[p] = f2_add(f.v[p], q.v[p]);
+        s2 = f2_fma(h[i].v[p], h[i].v[p], s2);
+      }
+      st_stream(static_cast<T*>(a.h) + (int64_t)row * a.cols + (int64_t)vi * VW, h[i].bits());
+    }
+    ss[0] = f2_lo(s2) + f2_hi(s2);
+    team_sum<TPR, TPR>(ss, sums, 1);
+    const uint64_t rh = both(rsqrtf(fmaf(ss[0], inv_n, a.eps)));
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int vi = lane + i * TPR;
+      if (vi >= nvec) continue;
+      Pairs<T> w(opaque(pre[i]));
+#pragma unroll
+      for (int p = 0; p < P; ++p) w.v[p] = f2_mul(f2_mul(h[i].v[p], rh), f2_add(w.v[p], off));
+      st_stream(static_cast<T*>(a.y) + (int64_t)row * a.cols + (int64_t)vi * VW, w.bits());
+    }
   }
 }
 
@@ -800,6 +909,20 @@ void by_length(int64_t cols, bool packs, F&& f) {
   else threads(integral_constant<int, 1>{});
 }
 
+// The staged kernel where its resident CTAs have at least 8 rows each; -1: too
+// few rows.
+template <typename T, int TPR, int VPT>
+int launch_staged(const Sandwich& a, const DeviceInfo& dev, cudaStream_t stream) {
+  constexpr int kCtas = staged_ctas<TPR, VPT>();
+  if (a.rows < 8ll * kCtas * dev.sm_count) return -1;
+  auto kern = sandwich_staged_kernel<T, TPR, VPT>;
+  constexpr int smem = 2 * 2 * VPT * TPR * 16;
+  if (smem > 48 * 1024 && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+    return launch_status();
+  launch_k(kern, kCtas * dev.sm_count, TPR, smem, stream, a);
+  return launch_status();
+}
+
 template <typename T>
 int launch_fwd(const Sandwich& a, const DeviceInfo& dev, cudaStream_t stream) {
   constexpr int VW = Elem<T>::kVec;
@@ -807,6 +930,19 @@ int launch_fwd(const Sandwich& a, const DeviceInfo& dev, cudaStream_t stream) {
                      aligned16(a.post) && aligned16(a.pre) && aligned16(a.gate) && aligned16(a.y) && aligned16(a.h);
   if (packs) {
     // 4096 columns of 16 bits: 256 threads of two packs (65536 rows 346 us; 128 of four 465 us)
+    const int64_t n = a.cols / VW;
+    // Where staging pays, over seconds, 4.3 GB a launch, against one CTA a row
+    // group: 16 bits, 192 packs 358 us (427), 512 335 (377), 640 409 (496), 1024
+    // 355 (405), 1280 378 (629), 2048 342 (474); 32 bits, 1280 329 (585), 2048 358
+    // (446).  Where not: 16 bits, 256 packs 387 (361); 32 bits, 512 373 (315).
+    int st = -1;
+    if constexpr (sizeof(T) == 2) {
+      if (n > 128 && n < 256) st = launch_staged<T, 128, 2>(a, dev, stream);
+      else if (n > 256 && n <= 512) st = launch_staged<T, 256, 2>(a, dev, stream);
+      else if (n > 512 && n <= 1024) st = launch_staged<T, 512, 2>(a, dev, stream);
+    }
+    if (n > 1024 && n <= 2048) st = launch_staged<T, 512, 4>(a, dev, stream);
+    if (st >= 0) return st;
     const int r = row_ladder<2>(a.cols / VW, [&](auto tpr, auto vpt) -> int {
       constexpr int TPR = decltype(tpr)::value, VPT = decltype(vpt)::value;
       constexpr int BLOCK = ladder_block<TPR>();

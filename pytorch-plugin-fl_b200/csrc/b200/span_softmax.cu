@@ -997,14 +997,14 @@ span_softmax_bwd_loop_kernel(const __grid_constant__ SpanArgs a) {
   }
 }
 
-// Calls f(TPR) for rows covered by `packs` packs: a warp up to `warp` packs,
+// Calls f(TPR) for rows covered by `packs` packs: a warp up to WARP packs,
 // then a CTA of 4 packs a thread; -1: longer than that.
-template <typename F>
-int span_ladder(int64_t packs, int64_t warp, F&& f) {
+template <int WARP, typename F>
+int span_ladder(int64_t packs, F&& f) {
   using std::integral_constant;
-  if (packs <= warp) return f(integral_constant<int, 32>{});
-  if (packs <= 256) return f(integral_constant<int, 64>{});
-  if (packs <= 512) return f(integral_constant<int, 128>{});
+  if (packs <= WARP) return f(integral_constant<int, 32>{});
+  if constexpr (WARP < 512)
+    if (packs <= 512) return f(integral_constant<int, 128>{});
   if (packs <= 1024) return f(integral_constant<int, 256>{});
   if (packs <= 2048) return f(integral_constant<int, 512>{});
   if (packs <= 4096) return f(integral_constant<int, 1024>{});
@@ -1048,7 +1048,7 @@ int launch_fwd(SpanArgs a, const DeviceInfo& dev, cudaStream_t stream) {
   if (in_step<TI, TO>(a.x, a.ldx, a.out, a.ldo, a.rows)) {
     const int64_t packs = packs_of<TI>(a.x, a.ldx, a.cols, a.rows);
     // 65 KB of scores for 8 warps: three CTAs an SM up to 2048 keys
-    const int st = span_ladder(packs, 2056 / Elem<TI>::kVec, [&](auto tpr) -> int {
+    const int st = span_ladder<2056 / Elem<TI>::kVec>(packs, [&](auto tpr) -> int {
       constexpr int TPR = decltype(tpr)::value;
       if constexpr (TPR == 32) {
         const int room = (int)(ceil_div(packs, 32) * 32);
@@ -1073,7 +1073,7 @@ int launch_bwd(SpanArgs a, const DeviceInfo& dev, cudaStream_t stream) {
       (!(a.cap > 0.f) || in_step<TI, TI>(a.out, a.ldo, a.x, a.ldx, a.rows))) {
     const int64_t packs = packs_of<TI>(a.out, a.ldo, a.cols, a.rows);
     // up to 12 KB a warp (20 where y is wider than x): 16 warps an SM
-    const int st = span_ladder(packs, 257, [&](auto tpr) -> int {
+    const int st = span_ladder<257>(packs, [&](auto tpr) -> int {
       constexpr int TPR = decltype(tpr)::value;
       if constexpr (TPR == 32) {
         const int room = (int)(ceil_div(packs, 32) * 32);

@@ -22,7 +22,8 @@ rounding the forward used.
 * masked_softmax(x, mask, scale): dx = softmax_backward(dy, y, x.dtype, scale);
   a mask that needs a gradient gets the unscaled product summed over the
   dims it broadcasts (HF's mask needs none)
-(topk and distill_topk carry theirs natively, in csrc/aten/fused_ops.cc.)
+(topk and distill_topk carry theirs natively, in csrc/aten/fused_ops.cc, and
+rotary, sandwich_norm and span_softmax in csrc/aten/layer_ops.cc.)
 """
 
 from __future__ import annotations

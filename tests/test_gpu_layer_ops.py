@@ -1038,3 +1038,26 @@ def test_spans_of_documents_on_flagos():
     got = torch_fl.ops.attention_spans(6, 6, documents=ids.to("flagos"),
                                        **{k: v.to("flagos") if torch.is_tensor(v) else v for k, v in kw.items()})
     assert got.device.type == "flagos" and torch.equal(got.cpu(), want)
+
+
+@pytest.mark.parametrize("gate", ["none", "channel", "sequence", "token"])
+@pytest.mark.parametrize("dtype,H", [(torch.bfloat16, 1032), (torch.float16, 4088), (torch.bfloat16, 8192),
+                                     (torch.bfloat16, 16376), (torch.float32, 4104), (torch.float32, 8192)])
+def test_sandwich_many_rows(dtype, H, gate):
+    """Rows enough for resident CTAs that walk them."""
+    rows = 4800 if H < 4000 else 7200 if H < 5000 and dtype != torch.float32 else 3000
+    B, S = 6, rows // 6 + 1
+    x, res, post, pre, gt, *_ = sandwich_inputs((B, S, H), gate, dtype, H, 1.0)
+    y, h = torch_fl.ops.sandwich_norm(x, res, post, pre, 1e-6, gt, 0.5, 1.0)
+    pick = torch.tensor([0, 1, S - 1, S, 2 * S + 3, 3 * S, B * S // 2, B * S - 2, B * S - 1])
+    flat = lambda t: np64(t.reshape(B * S, H)[pick.to(DEV)])
+    wide = None if gt is None else flat(gt.expand(B, S, H))
+    wy, wh = sandwich_want(flat(x), flat(res), np64(post), np64(pre), wide, np.float32(1e-6), 0.5, 1.0)
+    close(h.view(B * S, H)[pick.to(DEV)], wh, dtype, "h")
+    close(y.view(B * S, H)[pick.to(DEV)], wy, dtype, "y")
+    # every row as the same rows alone, but for the order of its sums
+    y1, h1 = torch_fl.ops.sandwich_norm(x[1:2], res[1:2], post, pre, 1e-6, gt[1:2] if gt is not None and gt.dim() == 3 else gt,
+                                        0.5, 1.0)
+    step = torch.finfo(dtype).eps * 1.01
+    assert bool(((h[1:2].float() - h1.float()).abs() <= step * h1.float().abs() + 1e-5).all())
+    assert bool(((y[1:2].float() - y1.float()).abs() <= step * y1.float().abs() + 1e-5).all())
