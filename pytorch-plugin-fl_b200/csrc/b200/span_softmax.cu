@@ -247,8 +247,8 @@ template <int N>
 struct Place {
   int first, last, lo, hi, p0, count;
   __device__ __forceinline__ Place(const Row& r, int shift, int cols)
-      : first(shift), last(shift + cols), lo(shift + r.lo), hi(shift + r.hi), p0(lo / N),
-        count(r.hi > r.lo ? (hi + N - 1) / N - p0 : 0) {}
+      : first(shift), last(shift + cols), lo(shift + r.lo), hi(shift + r.hi), p0((int)((uint32_t)lo / N)),
+        count(r.hi > r.lo ? (int)((uint32_t)(hi + N - 1) / N) - p0 : 0) {}
   __device__ __forceinline__ bool inside(int at) const { return at >= lo && at + N <= hi; }
   // Pairs of the pack at `at`: `other` outside the span.
   __device__ __forceinline__ void mask(uint64_t (&z)[N / 2], int at, float other) const {
@@ -265,14 +265,14 @@ struct Outside {
   int begin, p0, p1, end;
   __device__ __forceinline__ explicit Outside(const Place<N>& p) {
     begin = p.first > 0 ? 1 : 0;
-    end = p.last / N;
+    end = (int)((uint32_t)p.last / N);
     p0 = p.count ? max(p.p0, begin) : end;
     p1 = p.count ? p.p0 + p.count : end;
   }
   __device__ __forceinline__ void edges(TO* row, const Place<N>& p, int lane) const {
     if (p.first > 0 && (p.count == 0 || p.p0 > 0) && lane >= p.first && lane < N && lane < p.last)
       row[lane] = Elem<TO>::from_f(0.f);
-    if (p.last % N != 0 && end >= begin && (p.count == 0 || p1 <= end) && lane < p.last - end * N)
+    if ((uint32_t)p.last % N != 0 && end >= begin && (p.count == 0 || p1 <= end) && lane < p.last - end * N)
       row[end * N + lane] = Elem<TO>::from_f(0.f);
   }
 };
@@ -301,7 +301,8 @@ __device__ __forceinline__ void clear_outside_bulk(TO* row, const Place<N>& p, i
   for (int side = 0; side < 2; ++side) {
     char* to = reinterpret_cast<char*>(row) + (side == 0 ? o.begin : o.p1) * kPack;
     const int bytes = (side == 0 ? o.p0 - o.begin : o.end - o.p1) * kPack;
-    for (int at = lane * kZeroBytes; at < bytes; at += 32 * kZeroBytes)
+    const int at = lane * kZeroBytes;  // (a warp's rows have less than 32 KB)
+    if (at < bytes)
       asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(to + at), "r"(zeros),
                    "r"(min(kZeroBytes, bytes - at))
                    : "memory");
