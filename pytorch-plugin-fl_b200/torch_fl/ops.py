@@ -81,6 +81,12 @@ def masked_softmax(x, mask=None, scale: float = 1.0, dtype: torch.dtype | None =
 
 
 # ---------------------------------- a training step around the matrix products
+# (the one overload each has: a call need not look for it)
+_rotary = torch.ops.flagos.rotary.default
+_sandwich_norm = torch.ops.flagos.sandwich_norm.default
+_span_softmax = torch.ops.flagos.span_softmax.default
+
+
 def rotary(q, k, positions, inv_freq, scale: float = 1.0, interleaved: bool = False,
            unsqueeze_dim: int = 1, inverse: bool = False):
     """(q, k) with each head turned by its token's position, without a table of
@@ -95,8 +101,8 @@ def rotary(q, k, positions, inv_freq, scale: float = 1.0, interleaved: bool = Fa
     (`rope_frequencies`).  Angles are exact to fp64 at any position, the result
     is rounded once.  inverse turns back: with the same scale it is the
     gradient.  Differentiable in q and k, any number of times."""
-    return torch.ops.flagos.rotary(q, k, positions, inv_freq, float(scale), bool(interleaved),
-                                   int(unsqueeze_dim), bool(inverse))
+    return _rotary(q, k, positions, inv_freq, float(scale), bool(interleaved), int(unsqueeze_dim),
+                   bool(inverse))
 
 
 def rope_frequencies(dim: int, theta: float = 1e4, method: str = "default", factor: float = 1.0,
@@ -168,8 +174,8 @@ def sandwich_norm(x, residual, post_weight, pre_weight, eps: float, gate=None, s
     from 1.  fp32 throughout, h and y rounded once (y from h before its
     rounding).  Differentiable once in every tensor; the gradient is computed
     from x and the stored h."""
-    return torch.ops.flagos.sandwich_norm(x, residual, post_weight, pre_weight, gate, float(eps),
-                                          float(scale), float(weight_offset))
+    return _sandwich_norm(x, residual, post_weight, pre_weight, gate, float(eps), float(scale),
+                          float(weight_offset))
 
 
 def span_softmax(x, spans, scale: float = 1.0, cap: float | None = None, slopes=None, positions=None,
@@ -186,8 +192,8 @@ def span_softmax(x, spans, scale: float = 1.0, cap: float | None = None, slopes=
     positions are int32 [Q] or [B, Q], None: q + K - Q.  A query that sees
     nothing gets zeros; keys outside a span are not used, whatever they hold.
     dtype None = x's, or float32.  Differentiable once, in x."""
-    return torch.ops.flagos.span_softmax(x, spans, float(scale), None if cap is None else float(cap),
-                                         slopes, positions, dtype)
+    return _span_softmax(x, spans, float(scale), None if cap is None else float(cap), slopes, positions,
+                         dtype)
 
 
 def attention_spans(q_len: int, k_len: int, causal: bool = True, window: int | None = None,

@@ -1061,3 +1061,22 @@ def test_sandwich_many_rows(dtype, H, gate):
     step = torch.finfo(dtype).eps * 1.01
     assert bool(((h[1:2].float() - h1.float()).abs() <= step * h1.float().abs() + 1e-5).all())
     assert bool(((y[1:2].float() - y1.float()).abs() <= step * y1.float().abs() + 1e-5).all())
+
+
+def test_dispatch_modes_see_the_ops():
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    seen = []
+
+    class Watch(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            seen.append(func.name())
+            return func(*args, **(kwargs or {}))
+
+    s = everything_inputs(7)
+    want = everything(s)
+    with Watch():
+        got = everything(s)
+    for name in ("rotary", "sandwich_norm", "sandwich_norm_backward", "span_softmax", "span_softmax_backward"):
+        assert any(f"flagos::{name}" == n.split(".")[0] for n in seen), (name, seen)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
