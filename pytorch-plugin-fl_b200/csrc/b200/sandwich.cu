@@ -27,6 +27,8 @@
 // last kernel adds dpre's and dpost's partial sums and those shared A in the
 // order of the chunks.  So every sum has one order, whatever the gate's
 // shape, and no atomics.
+#include <initializer_list>
+
 #include "row_ladder.cuh"
 
 namespace flb200 {
@@ -321,19 +323,30 @@ sandwich_staged_kernel(const __grid_constant__ Sandwich a) {
   }
 }
 
-// VEC elements (a 16-byte pack, or one) as fp32 and back.
+// VEC elements (a 16-byte pack, two, or one) as fp32 and back.
+template <typename T>
+struct alignas(2 * sizeof(T)) Two {
+  T v[2];
+};
 template <typename T, int VEC>
 __device__ __forceinline__ void get(const T* p, float (&f)[VEC]) {
-  if constexpr (VEC == 1) f[0] = Elem<T>::to_f(*p);
-  else unpack<T>(ld_plain(p), f);
+  if constexpr (VEC == 1) {
+    f[0] = Elem<T>::to_f(*p);
+  } else if constexpr (VEC == 2) {
+    const Two<T> u = *reinterpret_cast<const Two<T>*>(p);
+    f[0] = Elem<T>::to_f(u.v[0]), f[1] = Elem<T>::to_f(u.v[1]);
+  } else {
+    unpack<T>(ld_plain(p), f);
+  }
 }
 template <typename T, int VEC>
 __device__ __forceinline__ void put(T* p, const float (&f)[VEC]) {
   if constexpr (VEC == 1) *p = Elem<T>::from_f(f[0]);
+  else if constexpr (VEC == 2) *reinterpret_cast<Two<T>*>(p) = Two<T>{{Elem<T>::from_f(f[0]), Elem<T>::from_f(f[1])}};
   else st_stream(p, pack<T>(f));
 }
 
-// Rows of any length (VEC a pack) and alignment (VEC 1): TPR threads a row, x
+// Rows of any length (VEC a pack) and alignment (VEC 2, 1): TPR threads a row, x
 // and the residual read again from cache.
 template <typename T, int VEC, int TPR>
 __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR)
@@ -508,7 +521,7 @@ sandwich_bwd_cols_kernel(const __grid_constant__ Sandwich a) {
     const uint32_t end = seg_end < r1 ? (uint32_t)seg_end : r1;
     const bool whole = (uint64_t)seg * a.per_gate >= r0 && (seg_end <= r1 || (r1 == a.rows));
     const bool is_first = seg == r0 / a.per_gate;
-#pragma unroll(VEC == 1 ? 4 : 2)
+#pragma unroll(VEC <= 2 ? 4 : 2)
     for (; row < end; ++row) {
       const float4 s = a.stats[row];
       float dy[VEC], m[VEC], x[VEC], g[VEC];
@@ -882,22 +895,35 @@ Plan plan_teams(int64_t rows, int64_t packs, int sms) {
   const int per_cta = team >= 256 ? 1 : 256 / team;
   return deal(rows, (int64_t)sms * (team == 512 ? 1 : 2) * per_cta, per_cta, team);
 }
-// About 8 CTAs an SM of 128 columns (or packs) and at least 8 rows.
+// About 8 CTAs an SM of 128 columns (or pairs, or packs) and at least 8 rows.
 Plan plan_columns(int64_t rows, int64_t units, int sms) {
   return deal(rows, std::max<int64_t>(1, std::min(ceil_div(8ll * sms, ceil_div(std::max<int64_t>(units, 1), 128)), ceil_div(rows, 8))), 1, 0);
 }
 // All plans' needs (which of them a call takes hangs on its alignment too).
 size_t bwd_workspace(int64_t rows, int64_t cols, int64_t packs, int sms) {
   size_t most = 0;
-  for (const Plan& p : {plan_teams(rows, packs, sms), plan_columns(rows, cols, sms), plan_columns(rows, packs, sms)})
+  for (const Plan& p : {plan_teams(rows, packs, sms), plan_columns(rows, cols, sms), plan_columns(rows, cols / 2, sms),
+                        plan_columns(rows, packs, sms)})
     most = std::max(most, (size_t)p.chunks + p.n_parts);
   return (size_t)rows * sizeof(float4) + (size_t)2 * cols * sizeof(float) * most;
 }
 
-// Calls f(VEC, TPR) for rows read by packs or by single elements: at least
-// four of them a thread, up to 512 threads.
+// The most elements at once that every address and stride allows: a pack, two
+// or one.
+template <typename T>
+int width_of(int64_t cols, std::initializer_list<int64_t> strides, std::initializer_list<const void*> pointers) {
+  for (const int w : {Elem<T>::kVec, 2}) {
+    bool ok = cols % w == 0;
+    for (const int64_t s : strides) ok = ok && s % w == 0;
+    for (const void* p : pointers) ok = ok && reinterpret_cast<uintptr_t>(p) % (w * sizeof(T)) == 0;
+    if (ok) return w;
+  }
+  return 1;
+}
+// Calls f(VEC, TPR) for rows read `width` elements at once: at least four of
+// these a thread, up to 512 threads.
 template <typename T, typename F>
-void by_length(int64_t cols, bool packs, F&& f) {
+void by_length(int64_t cols, int width, F&& f) {
   using std::integral_constant;
   auto threads = [&](auto vec) {
     const int64_t units = cols / decltype(vec)::value;
@@ -905,7 +931,8 @@ void by_length(int64_t cols, bool packs, F&& f) {
     else if (units <= 1024) f(vec, integral_constant<int, 128>{});
     else f(vec, integral_constant<int, 512>{});
   };
-  if (packs) threads(integral_constant<int, Elem<T>::kVec>{});
+  if (width == Elem<T>::kVec) threads(integral_constant<int, Elem<T>::kVec>{});
+  else if (width == 2) threads(integral_constant<int, 2>{});
   else threads(integral_constant<int, 1>{});
 }
 
@@ -926,9 +953,8 @@ int launch_staged(const Sandwich& a, const DeviceInfo& dev, cudaStream_t stream)
 template <typename T>
 int launch_fwd(const Sandwich& a, const DeviceInfo& dev, cudaStream_t stream) {
   constexpr int VW = Elem<T>::kVec;
-  const bool packs = a.cols % VW == 0 && a.ldx % VW == 0 && a.ldr % VW == 0 && aligned16(a.x) && aligned16(a.res) &&
-                     aligned16(a.post) && aligned16(a.pre) && aligned16(a.gate) && aligned16(a.y) && aligned16(a.h);
-  if (packs) {
+  const int width = width_of<T>(a.cols, {a.ldx, a.ldr}, {a.x, a.res, a.post, a.pre, a.gate, a.y, a.h});
+  if (width == VW) {
     // 4096 columns of 16 bits: 256 threads of two packs (65536 rows 346 us; 128 of four 465 us)
     const int64_t n = a.cols / VW;
     // Where staging pays, over seconds, 4.3 GB a launch, against one CTA a row
@@ -952,7 +978,7 @@ int launch_fwd(const Sandwich& a, const DeviceInfo& dev, cudaStream_t stream) {
     });
     if (r >= 0) return r;
   }
-  by_length<T>(a.cols, packs, [&](auto vec, auto tpr) {
+  by_length<T>(a.cols, width, [&](auto vec, auto tpr) {
     constexpr int TPR = decltype(tpr)::value, BLOCK = TPR < 128 ? 128 : TPR;
     launch_k((sandwich_loop_kernel<T, decltype(vec)::value, TPR>),
              (unsigned)std::min<int64_t>(ceil_div(a.rows, BLOCK / TPR), 2048ll / BLOCK * dev.sm_count), BLOCK, 0, stream,
@@ -978,19 +1004,17 @@ template <typename T>
 int launch_bwd(Sandwich a, const DeviceInfo& dev, float* ws, cudaStream_t stream) {
   constexpr int VW = Elem<T>::kVec;
   const int64_t packs = a.cols / VW;
-  const bool whole = a.cols % VW == 0 && a.ldx % VW == 0 && a.lds % VW == 0 &&
-                      a.ldy % VW == 0 && a.ldh % VW == 0 && aligned16(a.x) && aligned16(a.hs) && aligned16(a.dy) &&
-                      aligned16(a.dh) && aligned16(a.post) && aligned16(a.pre) && aligned16(a.gate) &&
-                      aligned16(a.dx) && aligned16(a.dres) && aligned16(a.dgate);
-  const Plan p = whole && packs <= 512 * kBwdVpt ? plan_teams(a.rows, packs, dev.sm_count)
-                                                 : plan_columns(a.rows, whole ? packs : a.cols, dev.sm_count);
+  const int width = width_of<T>(a.cols, {a.ldx, a.lds, a.ldy, a.ldh},
+                                {a.x, a.hs, a.dy, a.dh, a.post, a.pre, a.gate, a.dx, a.dres, a.dgate});
+  const Plan p = width == VW && packs <= 512 * kBwdVpt ? plan_teams(a.rows, packs, dev.sm_count)
+                                                       : plan_columns(a.rows, a.cols / width, dev.sm_count);
   a.chunks = p.chunks, a.per_chunk = p.per_chunk, a.n_parts = p.n_parts;
   a.parts = ws;
   a.shared = ws + (int64_t)2 * p.n_parts * a.cols;
   int st = FL_B200_OK;
   switch (p.team) {
     case 0:
-      by_length<T>(a.cols, whole, [&](auto vec, auto tpr) {
+      by_length<T>(a.cols, width, [&](auto vec, auto tpr) {
         constexpr int VEC = decltype(vec)::value, TPR = decltype(tpr)::value, BLOCK = TPR < 128 ? 128 : TPR;
         launch_k((sandwich_bwd_rows_kernel<T, VEC, TPR>),
                  (unsigned)std::min<int64_t>(ceil_div(a.rows, BLOCK / TPR), 2048ll / BLOCK * dev.sm_count), BLOCK, 0,

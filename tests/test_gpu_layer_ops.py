@@ -1080,3 +1080,22 @@ def test_dispatch_modes_see_the_ops():
     for name in ("rotary", "sandwich_norm", "sandwich_norm_backward", "span_softmax", "span_softmax_backward"):
         assert any(f"flagos::{name}" == n.split(".")[0] for n in seen), (name, seen)
     assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("at", [1, 2, 4, 6])
+def test_sandwich_offsets(dtype, at):
+    """Rows that begin one, two or four elements into a pack, forward and backward."""
+    x, res, post, pre, gt, dy, dh = sandwich_inputs((3, 11, 130), "sequence", dtype, at, 1.0)
+    wide = [torch.zeros(3, 11, 150, dtype=dtype, device=DEV)[..., at:at + 130].copy_(t) for t in (x, res, dy, dh)]
+    y, h = torch_fl.ops.sandwich_norm(wide[0], wide[1], post, pre, 1e-6, gt, 0.5, 1.0)
+    wy, wh = sandwich_want(np64(x), np64(res), np64(post), np64(pre), np64(gt), np.float32(1e-6), 0.5, 1.0)
+    close(h, wh, dtype, "h"), close(y, wy, dtype, "y")
+    got = torch.ops.flagos.sandwich_norm_backward(wide[2], wide[3], wide[0], h, post, pre, gt, 1e-6, 0.5, 1.0)
+    flat = lambda t: np64(t).reshape(33, -1)
+    dx, g, dpost, dpre, terms, down = sandwich_back_want(
+        flat(dy), flat(dh), flat(x), flat(h), np64(post), np64(pre),
+        np.broadcast_to(np64(gt), x.shape).reshape(33, -1), np.float32(1e-6), 0.5, 1.0)
+    close(got[0].reshape(33, -1), dx, dtype, "dx"), close(got[1].reshape(33, -1), g, dtype, "dresidual")
+    close(got[2][None], dpost, dtype, "dpost"), close(got[3][None], dpre, dtype, "dpre")
+    close(got[4], Num(terms.v.reshape(x.shape), terms.e.reshape(x.shape)).sum(1, down), dtype, "dgate")
