@@ -22,9 +22,12 @@
 // lies in that byte's page, so reading all of it is safe.)
 //
 // Exponentials are ex2.approx (2^-22 relative) of differences from the row's
-// maximum.  tanh u = 1 - 2 / (1 + 2^(2 u log2 e)) by ex2.approx and
-// rcp.approx: off by some 2^-22 absolutely, as the capped score is by cap
-// times that (tanh.approx would be off by 2^-11).
+// maximum.  Capped scores for 16-bit results take tanh u = 1 - 2 / (1 + 2^(2 u
+// log2 e)) by ex2.approx and rcp.approx: off by some 2^-22 absolutely, as the
+// score is by cap times that (tanh.approx would be off by 2^-11).  Up to a cap
+// of 256 that is an eighth of half a step of fp16; larger caps and fp32
+// results, which resolve it, take tanhf, off by a few 2^-24 of the score (4 x 32
+// x 2048 x 2048 f32, documents, cap 50: 460 us, 458 with the other).
 #include "common.cuh"
 
 namespace flb200 {
@@ -122,14 +125,18 @@ __device__ __forceinline__ Row row_of(const SpanArgs& a, uint32_t row) {
   return w.get(a);
 }
 
+// EXACT: tanh by tanhf, for capped scores (see above).
+template <bool EXACT>
 struct Score {
   float mul, cap;  // cap 0: none
   bool biased;
   __device__ __forceinline__ Score(const SpanArgs& a)
-      : mul(a.cap > 0.f ? 2.f * kLog2e * (a.scale / a.cap) : a.scale), cap(a.cap), biased(a.slopes != nullptr) {}
+      : mul(a.cap > 0.f ? (EXACT ? 1.f : 2.f * kLog2e) * (a.scale / a.cap) : a.scale), cap(a.cap),
+        biased(a.slopes != nullptr) {}
   __device__ __forceinline__ float operator()(float x, int key, const Row& r) const {
     float z = x * mul;
-    if (cap != 0.f) z = fmaf(-2.f * cap, rcp(1.f + ex2(z)), cap);
+    if constexpr (EXACT) z = cap * tanhf(z);
+    else if (cap != 0.f) z = fmaf(-2.f * cap, rcp(1.f + ex2(z)), cap);
     if (biased) z = fmaf(-r.slope, fabsf((float)(r.pos - key)), z);
     return z;
   }
@@ -149,7 +156,10 @@ struct Score {
   // pack, not for each element.
   template <int P>
   __device__ __forceinline__ void pack(uint64_t (&z)[P], int key, const Row& r) const {
-    if (cap != 0.f) {
+    if constexpr (EXACT) {
+#pragma unroll
+      for (int e = 0; e < P; ++e) z[e] = f2_make(cap * tanhf(f2_lo(z[e]) * mul), cap * tanhf(f2_hi(z[e]) * mul));
+    } else if (cap != 0.f) {
       const uint64_t m = f2_make(-2.f * cap, -2.f * cap), c = f2_make(cap, cap);
 #pragma unroll
       for (int e = 0; e < P; ++e) z[e] = f2_fma(half_of(z[e]), m, c);
@@ -323,10 +333,10 @@ __device__ __forceinline__ void finish_zeros() {
 // Scores of the pack at virtual element `at` from its elements, -inf outside
 // the span; returns the larger of m and their maximum.  (What lies outside is
 // scored too and then dropped.)
-template <int N>
+template <int N, bool EXACT>
 __device__ __forceinline__ float scores_of(uint64_t (&z)[N / 2], int at, const Place<N>& p, const Row& r,
-                                           const Score& score, float m) {
-  score.pack<N / 2>(z, at - p.first, r);
+                                           const Score<EXACT>& score, float m) {
+  score.template pack<N / 2>(z, at - p.first, r);
   if (!p.inside(at)) p.mask(z, at, -INFINITY);
 #pragma unroll
   for (int e = 0; e < N / 2; ++e) m = fmax3(m, f2_lo(z[e]), f2_hi(z[e]));
@@ -429,7 +439,7 @@ struct Rows {
 // sums go through the warp, and every row's span is read one row ahead.
 // Neither an earlier load of the next row, nor more but shorter runs of rows
 // for an even end, nor fewer instructions with 20 warps changed that.
-template <typename TI, typename TO>
+template <typename TI, typename TO, bool EXACT>
 __global__ void __launch_bounds__(256, 3)
 span_softmax_warp_kernel(const __grid_constant__ SpanArgs a, int room) {
   pdl_prologue();
@@ -445,7 +455,7 @@ span_softmax_warp_kernel(const __grid_constant__ SpanArgs a, int room) {
   float4* mine = dyn + kZeroBytes / 16 + (threadIdx.x >> 5) * room * Q + lane;
   Rows rows(a);
   if (!rows.more) return;
-  const Score score(a);
+  const Score<EXACT> score(a);
   uint32_t row = rows.w.row;
   Row r = rows.w.get(a);
   rows.next(a);
@@ -572,7 +582,7 @@ span_softmax_warp_kernel(const __grid_constant__ SpanArgs a, int room) {
 }
 
 // TPR threads a row, VPT packs each, a CTA a row.
-template <typename TI, typename TO, int TPR, int VPT>
+template <typename TI, typename TO, bool EXACT, int TPR, int VPT>
 __global__ void __launch_bounds__(TPR, TPR <= 256 ? 4 : 1)
 span_softmax_kernel(const __grid_constant__ SpanArgs a) {
   pdl_prologue();
@@ -581,7 +591,7 @@ span_softmax_kernel(const __grid_constant__ SpanArgs a) {
   const int lane = threadIdx.x;
   const uint32_t row = blockIdx.x;
   const Row r = row_of(a, row);
-  const Score score(a);
+  const Score<EXACT> score(a);
   const TI* xr = static_cast<const TI*>(a.x) + row * a.ldx;
   const int shift = shift_of(xr);
   TO* out = static_cast<TO*>(a.out) + row * a.ldo - shift;
@@ -612,7 +622,7 @@ span_softmax_kernel(const __grid_constant__ SpanArgs a) {
 
 // Rows too long for registers: a CTA of 1024 threads a row, the span read
 // twice, the second time from L2.
-template <typename TI, typename TO>
+template <typename TI, typename TO, bool EXACT>
 __global__ void __launch_bounds__(1024)
 span_softmax_long_kernel(const __grid_constant__ SpanArgs a) {
   pdl_prologue();
@@ -621,7 +631,7 @@ span_softmax_long_kernel(const __grid_constant__ SpanArgs a) {
   const int lane = threadIdx.x;
   const uint32_t row = blockIdx.x;
   const Row r = row_of(a, row);
-  const Score score(a);
+  const Score<EXACT> score(a);
   const TI* xr = static_cast<const TI*>(a.x) + row * a.ldx;
   const int shift = shift_of(xr);
   TO* out = static_cast<TO*>(a.out) + row * a.ldo - shift;
@@ -676,13 +686,13 @@ span_softmax_long_kernel(const __grid_constant__ SpanArgs a) {
 
 // Rows whose output lies otherwise than their input: a CTA a row by single
 // elements.
-template <typename TI, typename TO>
+template <typename TI, typename TO, bool EXACT>
 __global__ void __launch_bounds__(512)
 span_softmax_loop_kernel(const __grid_constant__ SpanArgs a) {
   pdl_prologue();
   constexpr int BLOCK = 512;
   __shared__ float smem[BLOCK / 32];
-  const Score score(a);
+  const Score<EXACT> score(a);
   for (uint32_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const Row r = row_of(a, row);
     const TI* xr = static_cast<const TI*>(a.x) + row * a.ldx;
@@ -714,7 +724,7 @@ span_softmax_loop_kernel(const __grid_constant__ SpanArgs a) {
 // One row of the gradient by TPR threads (the CTA, or a warp of it).
 // TI: x's and dx's type, TY: y's and dy's.
 template <typename TI, typename TY, int TPR, int VPT>
-__device__ __forceinline__ void span_bwd_row(const SpanArgs& a, uint32_t row, const Row& r, const Score& score,
+__device__ __forceinline__ void span_bwd_row(const SpanArgs& a, uint32_t row, const Row& r, const Score<false>& score,
                                              int lane, float* smem) {
   constexpr int N = Elem<TI>::kVec;
   const bool capped = score.cap != 0.f;
@@ -798,7 +808,7 @@ span_softmax_bwd_warp_kernel(const __grid_constant__ SpanArgs a, int room) {
   constexpr int W = (int)(sizeof(TY) / sizeof(TI));  // 16-byte words of y a pack
   extern __shared__ uint4 words[];
   const int lane = threadIdx.x & 31;
-  const Score score(a);
+  const Score<false> score(a);
   const bool capped = score.cap != 0.f;
   const uint32_t zeros = make_zeros(words);
   // word k of pack v at [v / 32][k][v % 32]: y's, dy's, x's
@@ -899,7 +909,7 @@ __global__ void __launch_bounds__(TPR, TPR <= 256 ? 2 : 1)
 span_softmax_bwd_kernel(const __grid_constant__ SpanArgs a) {
   pdl_prologue();
   __shared__ float smem[TPR / 32];
-  span_bwd_row<TI, TY, TPR, VPT>(a, blockIdx.x, row_of(a, blockIdx.x), Score(a), threadIdx.x, smem);
+  span_bwd_row<TI, TY, TPR, VPT>(a, blockIdx.x, row_of(a, blockIdx.x), Score<false>(a), threadIdx.x, smem);
 }
 
 // Rows too long for registers: a CTA of 1024 threads a row, y and dy read
@@ -913,7 +923,7 @@ span_softmax_bwd_long_kernel(const __grid_constant__ SpanArgs a) {
   const int lane = threadIdx.x;
   const uint32_t row = blockIdx.x;
   const Row r = row_of(a, row);
-  const Score score(a);
+  const Score<false> score(a);
   const bool capped = score.cap != 0.f;
   TI* out = static_cast<TI*>(a.out) + row * a.ldo;
   const int shift = shift_of(out);
@@ -975,7 +985,7 @@ span_softmax_bwd_loop_kernel(const __grid_constant__ SpanArgs a) {
   pdl_prologue();
   constexpr int BLOCK = 512;
   __shared__ float smem[BLOCK / 32];
-  const Score score(a);
+  const Score<false> score(a);
   const bool capped = score.cap != 0.f;
   for (uint32_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const Row r = row_of(a, row);
@@ -1044,8 +1054,8 @@ int64_t packs_of(const void* p, int64_t ld, int64_t cols, int64_t rows) {
   return ceil_div(cols, N) + (aligned16(p) && (rows <= 1 || ld % N == 0) ? 0 : 1);
 }
 
-template <typename TI, typename TO>
-int launch_fwd(SpanArgs a, const DeviceInfo& dev, cudaStream_t stream) {
+template <typename TI, typename TO, bool EXACT>
+int launch_fwd_as(SpanArgs a, const DeviceInfo& dev, cudaStream_t stream) {
   if (in_step<TI, TO>(a.x, a.ldx, a.out, a.ldo, a.rows)) {
     const int64_t packs = packs_of<TI>(a.x, a.ldx, a.cols, a.rows);
     // 65 KB of scores for 8 warps: three CTAs an SM up to 2048 keys
@@ -1053,19 +1063,24 @@ int launch_fwd(SpanArgs a, const DeviceInfo& dev, cudaStream_t stream) {
       constexpr int TPR = decltype(tpr)::value;
       if constexpr (TPR == 32) {
         const int room = (int)(ceil_div(packs, 32) * 32);
-        return launch_warps<256>(span_softmax_warp_kernel<TI, TO>, 3, a, room, room * Elem<TI>::kVec * 4, dev, stream);
+        return launch_warps<256>(span_softmax_warp_kernel<TI, TO, EXACT>, 3, a, room, room * Elem<TI>::kVec * 4, dev, stream);
       } else {
-        launch_k((span_softmax_kernel<TI, TO, TPR, 4>), a.rows, TPR, 0, stream, a);
+        launch_k((span_softmax_kernel<TI, TO, EXACT, TPR, 4>), a.rows, TPR, 0, stream, a);
         return launch_status();
       }
     });
     if (st >= 0) return st;
-    launch_k((span_softmax_long_kernel<TI, TO>), a.rows, 1024, 0, stream, a);
+    launch_k((span_softmax_long_kernel<TI, TO, EXACT>), a.rows, 1024, 0, stream, a);
     return launch_status();
   }
   const unsigned grid = (unsigned)std::min<int64_t>(a.rows, 4ll * dev.sm_count);
-  launch_k((span_softmax_loop_kernel<TI, TO>), grid, 512, 0, stream, a);
+  launch_k((span_softmax_loop_kernel<TI, TO, EXACT>), grid, 512, 0, stream, a);
   return launch_status();
+}
+template <typename TI, typename TO>
+int launch_fwd(const SpanArgs& a, const DeviceInfo& dev, cudaStream_t stream) {
+  const bool exact = a.cap > (std::is_same<TO, float>::value ? 0.f : 256.f);
+  return exact ? launch_fwd_as<TI, TO, true>(a, dev, stream) : launch_fwd_as<TI, TO, false>(a, dev, stream);
 }
 
 template <typename TI, typename TY>

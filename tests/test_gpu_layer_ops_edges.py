@@ -1,0 +1,69 @@
+"""The operators of a training step around the matrix products, on the GPU, at
+the sizes, layouts and values where they can go wrong: kernels that walk many
+rows or chunks, capped scores that fp32 resolves, results in another type than
+the scores, overlapping operands, calls from several threads.
+
+Tolerances as in test_gpu_layer_ops: bounds in fp32 carried along, u = 2^-24 a
+rounding, and half a step of the stored type.
+"""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import torch_fl
+from torch_fl import kernels as K
+
+from .test_gpu_layer_ops import DEV, TYPES, U, Num, close, gen, np64, random_spans, span_back_want
+
+pytestmark = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------- span softmax
+def capped_want(x, spans, scale, cap):
+    """softmax of cap * tanh(scale x / cap) over each span, and what fp32 may
+    be off: scale / cap and its product with x are rounded (the tanh passes on
+    u (1 - tanh^2) of that), tanhf is good to 2 units in the last place, its
+    product with the cap is rounded."""
+    n = x.shape[-1]
+    key = np.arange(n)
+    lo, hi = (np.clip(spans[..., i], 0, n)[:, None, :, None] for i in (0, 1))
+    seen = np.broadcast_to((key >= lo) & (key < hi), x.shape)
+    u = np.where(seen, x, 0.0) * scale / cap
+    t = np.tanh(u)
+    z, e = cap * t, cap * (np.abs(u) * (1 - t * t) * 2 * U + 5 * U * np.abs(t))
+    top = np.where(seen, z, -np.inf).max(-1, keepdims=True)
+    top = np.where(np.isfinite(top), top, 0)
+    p = np.where(seen, np.exp(z - top), 0.0)
+    # the scores' own error and the maximum's; the rounding of the difference
+    # times log2 e, its conversion and ex2 (4 u)
+    off = e + np.where(seen, e, 0).max(-1, keepdims=True) + 4 * U * (np.abs(z) + np.abs(top))
+    ep = p * np.expm1(off) + 4 * U * p + seen * 2.0 ** -126
+    s = p.sum(-1, keepdims=True)
+    rel = (ep.sum(-1, keepdims=True) + (n / 512 + 60) * U * s) / np.where(s > 0, s, 1)
+    y = p / np.where(s > 0, s, 1)
+    return Num(y, np.where(seen, ep / np.where(s > 0, s, 1) + y * rel / (1 - rel) + 3 * U * y, 0)), seen
+
+
+@pytest.mark.parametrize("n", [70, 700, 5000, 40000])
+@pytest.mark.parametrize("dtype,out,cap", [
+    (torch.float32, None, 50.0), (torch.float32, None, 1e5), (torch.bfloat16, torch.float32, 50.0),
+    (torch.float16, None, 2000.0), (torch.bfloat16, None, 1e5)])
+def test_capped_scores_keep_their_digits(dtype, out, cap, n):
+    """Scores far below the cap, where tanh is nearly the identity: an absolute
+    error of the tanh would be the cap times as large in the score."""
+    g = gen(n)
+    x = (3 * torch.randn(2, 2, 6, n, generator=g)).to(dtype).to(DEV)
+    wide = torch.zeros(2, 2, 6, n + 9, dtype=dtype, device=DEV)
+    shifted = wide[..., 1:n + 1].copy_(x)                       # rows in another step than their results
+    spans = random_spans(2, 6, n, g)
+    for xs in (x, shifted):
+        y = torch_fl.ops.span_softmax(xs, spans, 0.5, cap, dtype=out)
+        want, seen = capped_want(np64(x), spans.cpu().numpy(), 0.5, float(np.float32(cap)))
+        close(y, want, y.dtype, "y")
+        assert not np64(y)[~seen].any()
+        dy = torch.randn(x.shape, generator=g).to(y.dtype).to(DEV)
+        dx = torch.ops.flagos.span_softmax_backward(dy, y, xs, spans, 0.5, cap)
+        close(dx, span_back_want(np64(dy), np64(y), np64(x), seen, 0.5, float(np.float32(cap))), dtype, "dx")
