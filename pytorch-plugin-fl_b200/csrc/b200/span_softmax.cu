@@ -18,8 +18,9 @@
 // 200 keys, 5.4 TB/s with the zeros around them), capped ones by theirs.
 // Rows need not begin on a 16-byte boundary: they are walked by the aligned
 // packs that cover them, elements outside masked and the row's first and last
-// pack stored by element.  (An aligned pack that holds one byte of the row
-// lies in that byte's page, so reading all of it is safe.)
+// pack stored by element.  (16 aligned bytes that hold one byte of the row lie
+// in that byte's page, so reading all of them is safe; of a pack of 32 bytes,
+// fp32 beside 16-bit scores, each half is read only if it does.)
 //
 // Exponentials are ex2.approx (2^-22 relative) of differences from the row's
 // maximum.  Capped scores for 16-bit results take tanh u = 1 - 2 / (1 + 2^(2 u
@@ -29,6 +30,7 @@
 // results, which resolve it, take tanhf, off by a few 2^-24 of the score (4 x 32
 // x 2048 x 2048 f32, documents, cap 50: 460 us, 458 with the other).
 #include "common.cuh"
+#include "span_place.cuh"
 
 namespace flb200 {
 namespace {
@@ -251,15 +253,11 @@ __device__ __forceinline__ int shift_of(const T* p) {
   return (int)((reinterpret_cast<uintptr_t>(p) & 15u) / sizeof(T));
 }
 
-// Where a row's packs lie: its own (virtual) elements [first, last), its
-// span's [lo, hi), the span's packs p0 ... p0 + count - 1.
 template <int N>
-struct Place {
-  int first, last, lo, hi, p0, count;
-  __device__ __forceinline__ Place(const Row& r, int shift, int cols)
-      : first(shift), last(shift + cols), lo(shift + r.lo), hi(shift + r.hi), p0((int)((uint32_t)lo / N)),
-        count(r.hi > r.lo ? (int)((uint32_t)(hi + N - 1) / N) - p0 : 0) {}
-  __device__ __forceinline__ bool inside(int at) const { return at >= lo && at + N <= hi; }
+struct Place : Packs<N> {
+  using Packs<N>::lo;
+  using Packs<N>::hi;
+  __device__ __forceinline__ Place(const Row& r, int shift, int cols) : Packs<N>(r.lo, r.hi, shift, cols) {}
   // Pairs of the pack at `at`: `other` outside the span.
   __device__ __forceinline__ void mask(uint64_t (&z)[N / 2], int at, float other) const {
 #pragma unroll
@@ -268,6 +266,14 @@ struct Place {
                      at + 2 * e + 1 >= lo && at + 2 * e + 1 < hi ? f2_hi(z[e]) : other);
   }
 };
+// Pack `at` of y or dy: its words that hold something of the span, else zeros.
+template <typename T, int N>
+__device__ __forceinline__ void load_words(Elems<T, N>& v, const T* from, int at, const Place<N>& p) {
+  constexpr int VW = Elem<T>::kVec;
+#pragma unroll
+  for (int k = 0; k < N / VW; ++k)
+    v.word(k, N == VW || p.meets(at + k * VW, VW) ? ld_stream_now(from + k * VW) : make_uint4(0, 0, 0, 0));
+}
 // Where nothing is seen: whole packs [begin, p0) and [p1, end), and the
 // row's first and last pack where they are not whole.
 template <typename TO, int N>
@@ -742,8 +748,8 @@ __device__ __forceinline__ void span_bwd_row(const SpanArgs& a, uint32_t row, co
   for (int i = 0; i < VPT; ++i) {
     const int vi = lane + i * TPR;
     if (vi < p.count) {
-      y[i].load(yr + (int64_t)vi * N);
-      d[i].load(dr + (int64_t)vi * N);
+      load_words(y[i], yr + (int64_t)vi * N, (p.p0 + vi) * N, p);
+      load_words(d[i], dr + (int64_t)vi * N, (p.p0 + vi) * N, p);
       if (capped) x[i].load(xr + (int64_t)vi * N);
     } else {
       y[i].clear();
@@ -834,8 +840,13 @@ span_softmax_bwd_warp_kernel(const __grid_constant__ SpanArgs a, int room) {
     for (int left = p.count - lane; left > 0; left -= 32, w += 32 * kinds, at += 32 * N) {
 #pragma unroll
       for (int k = 0; k < W; ++k) {
-        cp_async16(w + k * 32, yr + at + k * Elem<TY>::kVec);
-        cp_async16(w + (W + k) * 32, dr + at + k * Elem<TY>::kVec);
+        constexpr int VW = Elem<TY>::kVec;
+        if (W == 1 || p.meets(p.p0 * N + at + k * VW, VW)) {
+          cp_async16(w + k * 32, yr + at + k * VW);
+          cp_async16(w + (W + k) * 32, dr + at + k * VW);
+        } else {
+          w[k * 32] = w[(W + k) * 32] = make_uint4(0, 0, 0, 0);
+        }
       }
       if (capped) cp_async16(w + 2 * W * 32, xr + at);
     }
@@ -937,9 +948,9 @@ span_softmax_bwd_long_kernel(const __grid_constant__ SpanArgs a) {
   uint64_t f[N / 2], g[N / 2], acc[2] = {f2_make(0.f, 0.f), f2_make(0.f, 0.f)};
   auto get = [&](int vi) {
     Elems<TY, N> y, d;
-    y.load(yr + (int64_t)vi * N);
-    d.load(dr + (int64_t)vi * N);
     const int at = (p.p0 + vi) * N;
+    load_words(y, yr + (int64_t)vi * N, at, p);
+    load_words(d, dr + (int64_t)vi * N, at, p);
     if (!p.inside(at)) {
       y.keep(p.lo - at, p.hi - at);
       d.keep(p.lo - at, p.hi - at);

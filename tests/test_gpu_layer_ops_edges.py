@@ -67,3 +67,32 @@ def test_capped_scores_keep_their_digits(dtype, out, cap, n):
         dy = torch.randn(x.shape, generator=g).to(y.dtype).to(DEV)
         dx = torch.ops.flagos.span_softmax_backward(dy, y, xs, spans, 0.5, cap)
         close(dx, span_back_want(np64(dy), np64(y), np64(x), seen, 0.5, float(np.float32(cap))), dtype, "dx")
+
+
+@pytest.mark.parametrize("K_", [12, 60, 700, 1004, 5004, 40004])
+@pytest.mark.parametrize("cap", [None, 20.0])
+def test_gradient_of_fp32_weights_at_the_edges_of_their_memory(K_, cap):
+    """fp32 y and dy beside 16-bit x: a pack of x is two 16-byte words of them,
+    of which the first or the last may hold nothing of the row.  Views in a
+    buffer of NaN, results that begin inside a pack."""
+    g = gen(K_)
+    x = (2 * torch.randn(1, 1, 3, K_, generator=g)).bfloat16().to(DEV)
+    spans = torch.tensor([[0, K_], [K_ - 3, K_], [1, 2]]).int().to(DEV)
+    y = torch_fl.ops.span_softmax(x, spans, 0.5, cap, dtype=torch.float32)
+    dy = torch.randn(1, 1, 3, K_, generator=g).to(DEV)
+    want = torch.ops.flagos.span_softmax_backward(dy, y, x, spans, 0.5, cap)
+    for at in (0, 4, 8):
+        bufs = [torch.full((3 * K_ + 16,), math.nan, device=DEV) for _ in range(2)]
+        views = [b[at:at + 3 * K_].view(1, 1, 3, K_).copy_(t) for b, t in zip(bufs, (y, dy))]
+        got = torch.ops.flagos.span_softmax_backward(views[1], views[0], x, spans, 0.5, cap)
+        assert torch.equal(got, want)
+        # dx (and x) 4 elements into a pack, y and dy at the start of one
+        xs, dx = (torch.full((3 * K_ + 16,), math.nan, device=DEV).bfloat16() for _ in range(2))
+        xs[4:4 + 3 * K_] = x.flatten()
+        K._abi.call("fl_b200_span_softmax_bwd", views[1].data_ptr(), K_, views[0].data_ptr(), K_, xs[4:].data_ptr(), K_,
+                    spans.data_ptr(), 0, 2, dx[4:].data_ptr(), K_, 3, K_, 1, 3, 0.5, cap or 0.0, K._abi.F32,
+                    K._abi.BF16, K._stream(x))
+        # (another share of the sum for each thread: fp32 sums of some terms around 1)
+        a, b = dx[4:4 + 3 * K_].double(), want.flatten().double()
+        assert bool(((a - b).abs() <= 2.0 ** -7 * b.abs() + 60 * U * float(dy.abs().max())).all())
+        assert bool(torch.isnan(dx[:4]).all()) and bool(torch.isnan(dx[4 + 3 * K_:]).all())
