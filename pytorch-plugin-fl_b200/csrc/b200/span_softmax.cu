@@ -1032,15 +1032,19 @@ int span_ladder(int64_t packs, F&& f) {
   if (packs <= 4096) return f(integral_constant<int, 1024>{});
   return -1;
 }
+// Packs in whole turns of a warp.
+constexpr int room_of(int64_t packs) { return (int)((packs + 31) / 32 * 32); }
 // Launches CTAs of BLOCK threads, as many as are resident at once (`most` an
-// SM by their registers), with `each` bytes of shared memory a warp.  Warps
-// that have many rows take 8 in order.
-template <int BLOCK, typename K>
+// SM by their registers), with `room` packs of `each` bytes of shared memory a
+// warp.  Warps that have many rows take 8 in order.  What the kernel may take
+// (MOST bytes) is a constant: it belongs to the function, and another thread
+// may be between its own call's setting and launch.
+template <int BLOCK, int MOST, typename K>
 int launch_warps(K kernel, int most, SpanArgs& a, int room, int each, const DeviceInfo& dev, cudaStream_t stream) {
   constexpr int kWarps = BLOCK / 32;
-  const int smem = each * kWarps + kZeroBytes;
+  const int smem = room * each * kWarps + kZeroBytes;
   if (smem > 48 * 1024 &&
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST) != cudaSuccess)
     return launch_status();
   const int64_t ctas = (int64_t)std::max(1, std::min(most, 228 * 1024 / (smem + 1024))) * dev.sm_count;
   a.unit = a.rows >= ctas * kWarps * 32 ? 8 : 1;
@@ -1070,11 +1074,12 @@ int launch_fwd_as(SpanArgs a, const DeviceInfo& dev, cudaStream_t stream) {
   if (in_step<TI, TO>(a.x, a.ldx, a.out, a.ldo, a.rows)) {
     const int64_t packs = packs_of<TI>(a.x, a.ldx, a.cols, a.rows);
     // 65 KB of scores for 8 warps: three CTAs an SM up to 2048 keys
-    const int st = span_ladder<2056 / Elem<TI>::kVec>(packs, [&](auto tpr) -> int {
+    constexpr int kWarpPacks = 2056 / Elem<TI>::kVec, kEach = Elem<TI>::kVec * 4;
+    const int st = span_ladder<kWarpPacks>(packs, [&](auto tpr) -> int {
       constexpr int TPR = decltype(tpr)::value;
       if constexpr (TPR == 32) {
-        const int room = (int)(ceil_div(packs, 32) * 32);
-        return launch_warps<256>(span_softmax_warp_kernel<TI, TO, EXACT>, 3, a, room, room * Elem<TI>::kVec * 4, dev, stream);
+        return launch_warps<256, room_of(kWarpPacks) * kEach * 8 + kZeroBytes>(
+            span_softmax_warp_kernel<TI, TO, EXACT>, 3, a, room_of(packs), kEach, dev, stream);
       } else {
         launch_k((span_softmax_kernel<TI, TO, EXACT, TPR, 4>), a.rows, TPR, 0, stream, a);
         return launch_status();
@@ -1100,12 +1105,13 @@ int launch_bwd(SpanArgs a, const DeviceInfo& dev, cudaStream_t stream) {
       (!(a.cap > 0.f) || in_step<TI, TI>(a.out, a.ldo, a.x, a.ldx, a.rows))) {
     const int64_t packs = packs_of<TI>(a.out, a.ldo, a.cols, a.rows);
     // up to 12 KB a warp (20 where y is wider than x): 16 warps an SM
-    const int st = span_ladder<257>(packs, [&](auto tpr) -> int {
+    constexpr int kWarpPacks = 257, kWords = 2 * (int)(sizeof(TY) / sizeof(TI));
+    const int st = span_ladder<kWarpPacks>(packs, [&](auto tpr) -> int {
       constexpr int TPR = decltype(tpr)::value;
       if constexpr (TPR == 32) {
-        const int room = (int)(ceil_div(packs, 32) * 32);
-        const int each = room * 16 * (2 * (int)(sizeof(TY) / sizeof(TI)) + (a.cap > 0.f ? 1 : 0));
-        return launch_warps<128>(span_softmax_bwd_warp_kernel<TI, TY>, sizeof(TY) == sizeof(TI) ? 7 : 5, a, room, each, dev, stream);
+        return launch_warps<128, room_of(kWarpPacks) * (kWords + 1) * 16 * 4 + kZeroBytes>(
+            span_softmax_bwd_warp_kernel<TI, TY>, sizeof(TY) == sizeof(TI) ? 7 : 5, a, room_of(packs),
+            16 * (kWords + (a.cap > 0.f ? 1 : 0)), dev, stream);
       } else {
         launch_k((span_softmax_bwd_kernel<TI, TY, TPR, 4>), a.rows, TPR, 0, stream, a);
         return launch_status();

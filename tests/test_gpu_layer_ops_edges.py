@@ -96,3 +96,57 @@ def test_gradient_of_fp32_weights_at_the_edges_of_their_memory(K_, cap):
         a, b = dx[4:4 + 3 * K_].double(), want.flatten().double()
         assert bool(((a - b).abs() <= 2.0 ** -7 * b.abs() + 60 * U * float(dy.abs().max())).all())
         assert bool(torch.isnan(dx[:4]).all()) and bool(torch.isnan(dx[4 + 3 * K_:]).all())
+
+
+def test_calls_of_different_lengths_from_two_threads():
+    """Rows of 1531 and of 2048 keys want different amounts of shared memory of
+    one kernel: neither thread's calls may take it from the other's.  (The C
+    entries themselves, so that both threads are in them at once.)"""
+    import threading
+
+    lib, made = K._abi.lib(), {}
+    for n in (1531, 2048):
+        x = (2 * torch.randn(1, 1, 4, n, generator=gen(n))).bfloat16().to(DEV)
+        spans = torch.tensor([[0, n]] * 4).int().to(DEV)
+        y = K.span_softmax(x, spans, 0.5, 20.0, out_dtype=torch.float32)
+        dx = K.span_softmax_backward(y, y, x, spans, 0.5, 20.0)
+        y2, dx2 = torch.zeros_like(y), torch.zeros_like(dx)
+        stream = torch.cuda.Stream()
+        fwd = (x.data_ptr(), n, spans.data_ptr(), 0, 2, None, 0, 0, None, y2.data_ptr(), n, 4, n, 1, 4, 0.5, 20.0,
+               K._abi.BF16, K._abi.F32, stream.cuda_stream)
+        bwd = (y.data_ptr(), n, y.data_ptr(), n, x.data_ptr(), n, spans.data_ptr(), 0, 2, dx2.data_ptr(), n, 4, n, 1, 4,
+               0.5, 20.0, K._abi.F32, K._abi.BF16, stream.cuda_stream)
+        made[n] = (x, spans, y, dx, y2, dx2, stream, fwd, bwd)
+    torch.cuda.synchronize()
+    ready, status = threading.Barrier(2), {n: set() for n in made}
+
+    def work(n):
+        fwd, bwd = made[n][-2:]
+        ready.wait(60)
+        for _ in range(5000):
+            status[n].add(lib.fl_b200_span_softmax(*fwd))
+            status[n].add(lib.fl_b200_span_softmax_bwd(*bwd))
+
+    threads = [threading.Thread(target=work, args=(n,)) for n in made]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    torch.cuda.synchronize()
+    assert status == {n: {0} for n in made}
+    for x, spans, y, dx, y2, dx2, *_ in made.values():
+        assert torch.equal(y, y2) and torch.equal(dx, dx2)
+
+
+def test_rows_of_different_lengths_in_one_graph():
+    g = gen(62)
+    xs = [(2 * torch.randn(1, 1, 4, n, generator=g)).bfloat16().to(DEV) for n in (2048, 1531, 2056, 40)]
+    spans = [torch.tensor([[0, x.shape[-1]]] * 4).int().to(DEV) for x in xs]
+    run = lambda: [K.span_softmax(x, s, 0.5, 20.0) for x, s in zip(xs, spans)]
+    want = run()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run()
+    K.span_softmax(xs[3], spans[3])                         # the last length before the replay is the shortest
+    K.span_softmax(xs[1], spans[1])
+    [t.zero_() for t in got]
+    graph.replay()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
