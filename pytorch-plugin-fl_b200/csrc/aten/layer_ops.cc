@@ -22,6 +22,13 @@ HeadsView Heads(const at::Tensor& t, int64_t unsqueeze_dim) {
   return {t.size(0), t.size(h), t.size(s), t.size(3), t.stride(0), t.stride(h), t.stride(s)};
 }
 
+// A result laid out as t where that keeps its heads whole: of overlapping
+// views (windows of one row, say) the densest layout has another dim innermost.
+at::Tensor HeadsLike(const at::Tensor& t) {
+  at::Tensor o = at::empty_like(t);
+  return o.size(-1) <= 1 || o.stride(-1) == 1 ? o : at::empty(t.sizes(), t.options());
+}
+
 std::tuple<at::Tensor, at::Tensor> Rotary(const at::Tensor& q_in, const at::Tensor& k_in,
                                           const at::Tensor& positions, const at::Tensor& inv_freq, double scale,
                                           bool interleaved, int64_t unsqueeze_dim, bool inverse) {
@@ -52,7 +59,7 @@ std::tuple<at::Tensor, at::Tensor> Rotary(const at::Tensor& q_in, const at::Tens
   TORCH_CHECK(std::isfinite(scale), op, ": scale must be finite");
   const int64_t pb = positions.dim() == 2 && positions.size(0) > 1 ? positions.stride(0) : 0;
   at::Tensor freq = inv_freq.contiguous();
-  at::Tensor qo = at::empty_like(q), ko = at::empty_like(k);
+  at::Tensor qo = HeadsLike(q), ko = HeadsLike(k);
   const HeadsView oq = Heads(qo, unsqueeze_dim), ok = Heads(ko, unsqueeze_dim);
   if (q.numel() == 0 && k.numel() == 0) return {qo, ko};
   GpuGuard g(q);

@@ -555,6 +555,13 @@ def sum_i32_i64(x: torch.Tensor, full: bool) -> torch.Tensor:
 
 
 # ---------------------------------- a training step around the matrix products
+def _heads_like(t: torch.Tensor) -> torch.Tensor:
+    """A result laid out as t where that keeps its heads whole (of overlapping
+    views another dim would be innermost)."""
+    o = torch.empty_like(t)
+    return o if o.stride(-1) == 1 else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
 def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv_freq: torch.Tensor,
            scale: float = 1.0, interleaved: bool = False, inverse: bool = False, layout: str = "bhsd",
            inplace: bool = False):
@@ -563,14 +570,14 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv
     B, Hq, S, D, sq = _bhsd(q, layout)
     ops = [t for t in (q, k, positions, inv_freq) if t is not None]
     _one_device(*ops)
-    qo = q if inplace else torch.empty_like(q)
+    qo = q if inplace else _heads_like(q)
     soq = _bhsd(qo, layout)[4]
     Hk, sk, sok, ko = 0, (0, 0, 0), (0, 0, 0), None
     if k is not None:
         Bk, Hk, Sk, Dk, sk = _bhsd(k, layout)
         if (Bk, Sk, Dk) != (B, S, D) or k.dtype != q.dtype:
             raise ValueError("q and k disagree")
-        ko = k if inplace else torch.empty_like(k)
+        ko = k if inplace else _heads_like(k)
         sok = _bhsd(ko, layout)[4]
     if positions.dtype not in (torch.int32, torch.int64) or positions.dim() not in (1, 2) \
             or positions.shape[-1] != S or (positions.dim() == 2 and positions.shape[0] not in (1, B)):

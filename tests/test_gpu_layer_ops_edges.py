@@ -16,7 +16,8 @@ import torch
 import torch_fl
 from torch_fl import kernels as K
 
-from .test_gpu_layer_ops import DEV, TYPES, U, Num, close, gen, np64, random_spans, span_back_want
+from .test_gpu_layer_ops import (DEV, TYPES, U, Num, check_rotary, close, gen, np64, random_spans,
+                                 span_back_want)
 
 pytestmark = pytest.mark.gpu
 
@@ -149,4 +150,25 @@ def test_rows_of_different_lengths_in_one_graph():
     K.span_softmax(xs[1], spans[1])
     [t.zero_() for t in got]
     graph.replay()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# --------------------------------------------------------------------- rotary
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [1, 2])
+def test_rotary_of_overlapping_views(dtype, dim):
+    """Windows of one row: tokens one element apart, of which a result laid
+    out alike would have its heads' elements apart."""
+    g = gen(71)
+    row = torch.randn(64, generator=g).to(dtype).to(DEV)
+    q = row.unfold(0, 16, 1)[:8][None, :, None]                            # [1, 8, 1, 16], strides (8, 1, 16, 1)
+    k = row.unfold(0, 16, 3)[:8][None, :, None].expand(1, 8, 2, 16)
+    assert torch.empty_like(q).stride(-1) != 1
+    freq, pos = torch.rand(8, generator=g).to(DEV), torch.arange(8, device=DEV)
+    if dim == 1:
+        q, k = q.transpose(1, 2), k.transpose(1, 2)
+    check_rotary(q, k, pos, freq, layout="bshd" if dim == 2 else "bhsd")
+    layout = "bshd" if dim == 2 else "bhsd"
+    got = K.rotary(q, k, pos, freq, layout=layout)
+    want = K.rotary(q.contiguous(), k.contiguous(), pos, freq, layout=layout)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
