@@ -506,7 +506,8 @@ FL_B200_API int fl_b200_verify_draft(const int64_t* draft_ids, int64_t ld_ids, c
 /* ------------------------------------------------------------------------ *
  * A training step around the matrix products, in the forms newer decoders   *
  * give it.  The reference has none of these (its HF path would run them op   *
- * by op).                                                                   *
+ * by op).  Addresses are multiples of their elements' size (else             *
+ * FL_B200_ERR_MISALIGNED); "any alignment" is any such.                     *
  *                                                                           *
  * Rotary positions without a table.  angle = position * inv_freq[i] for      *
  * i < rot / 2, and                                                          *

@@ -351,6 +351,7 @@ int any(const List& l, int max_kind, float bound, float* norm, void* workspace, 
         cudaStream_t stream) {
   FLB_CHECK_ARG(l.count >= 0 && norm && (max_kind == 0 || max_kind == 1));
   FLB_CHECK_ARG(l.count == 0 || (l.in && l.numel && l.dtype));
+  if (!aligned_to(4, {norm})) return FL_B200_ERR_MISALIGNED;
   int64_t tensors = 0;
   for (int64_t i = 0; i < l.count; ++i) {
     if (!is_float_dtype(l.dtype[i])) return FL_B200_ERR_UNSUPPORTED_DTYPE;

@@ -11,6 +11,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <initializer_list>
 #include <type_traits>
 #include <utility>
 
@@ -133,6 +134,12 @@ __device__ __forceinline__ void st_stream32(void* p, const Pack32& v) {
                "r"(v.lo.x), "r"(v.lo.y), "r"(v.lo.z), "r"(v.lo.w), "r"(v.hi.x), "r"(v.hi.y),
                "r"(v.hi.z), "r"(v.hi.w)
                : "memory");
+}
+// Whether every address is a multiple of `size` (NULL is).
+inline bool aligned_to(int64_t size, std::initializer_list<const void*> pointers) {
+  for (const void* p : pointers)
+    if (reinterpret_cast<uintptr_t>(p) % (uintptr_t)size != 0) return false;
+  return true;
 }
 inline bool aligned32(const void* p) {
   return (reinterpret_cast<uintptr_t>(p) & 31u) == 0;

@@ -336,6 +336,9 @@ extern "C" FL_B200_API int fl_b200_rotary(
   if (rot > FL_B200_ROTARY_MAX || Hq + Hk > (1 << 20) || D > (1 << 20) || B > 0x7fffffff / S)
     return FL_B200_ERR_TOO_LARGE;
   const int64_t size = dtype_size(dtype);
+  if ((Hq && !aligned_to(size, {q, q_out})) || (Hk && !aligned_to(size, {k, k_out})) || !aligned_to(4, {inv_freq}) ||
+      !aligned_to(dtype_size(pos_dtype), {positions}))
+    return FL_B200_ERR_MISALIGNED;
   RotaryArgs a = {};
   int64_t unit = 16;  // every address is a multiple of it
   auto tensor = [&](int t, const void* in, void* out, int64_t H, const int64_t (&si)[3], const int64_t (&so)[3]) {

@@ -27,8 +27,6 @@
 // last kernel adds dpre's and dpost's partial sums and those shared A in the
 // order of the chunks.  So every sum has one order, whatever the gate's
 // shape, and no atomics.
-#include <initializer_list>
-
 #include "row_ladder.cuh"
 
 namespace flb200 {
@@ -1079,6 +1077,7 @@ FL_B200_API int fl_b200_sandwich_norm(const void* x, int64_t ld_x, const void* r
   int st = check(a, rows, cols, rows_per_gate, gate, eps, scale, weight_offset);
   if (st != FL_B200_OK) return st;
   const int64_t size = dtype_size(dtype);
+  if (!aligned_to(size, {x, residual, post, pre, gate, y, h})) return FL_B200_ERR_MISALIGNED;
   const Range ry(y, cols, rows, cols, size), rh(h, cols, rows, cols, size);
   const Range in[] = {{x, ld_x, rows, cols, size}, {residual, ld_r, rows, cols, size},
                       {gate, cols, gate ? ceil_div(rows, a.per_gate) : 1, cols, size}};
@@ -1115,6 +1114,7 @@ FL_B200_API int fl_b200_sandwich_norm_bwd(const void* dy, int64_t ld_dy, const v
   if (cols == 0) return FL_B200_OK;
   FLB_CHECK_ARG(dpost && dpre);
   const int64_t size = dtype_size(dtype);
+  if (!aligned_to(size, {dpost, dpre})) return FL_B200_ERR_MISALIGNED;
   if (rows == 0) {  // sums over no rows
     auto* s = static_cast<cudaStream_t>(stream);
     if (cudaMemsetAsync(dpost, 0, cols * size, s) != cudaSuccess ||
@@ -1127,6 +1127,7 @@ FL_B200_API int fl_b200_sandwich_norm_bwd(const void* dy, int64_t ld_dy, const v
   Sandwich a = {};
   int st = check(a, rows, cols, rows_per_gate, gate, eps, scale, weight_offset);
   if (st != FL_B200_OK) return st;
+  if (!aligned_to(size, {dy, dh, x, h, post, pre, gate, dx, dresidual, dgate})) return FL_B200_ERR_MISALIGNED;
   const Range rx(dx, cols, rows, cols, size), rr(dresidual, cols, rows, cols, size);
   const Range in[] = {{dy, ld_dy, rows, cols, size}, {dh, ld_dh, rows, cols, size}, {x, ld_x, rows, cols, size},
                       {h, ld_h, rows, cols, size}, {gate, cols, gate ? ceil_div(rows, a.per_gate) : 1, cols, size}};

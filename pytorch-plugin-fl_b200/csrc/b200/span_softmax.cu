@@ -1168,6 +1168,9 @@ FL_B200_API int fl_b200_span_softmax(const void* x, int64_t ld_x, const int32_t*
   a.spb = span_sb, a.spq = span_sq, a.pos = positions, a.pb = pos_sb, a.pq = pos_sq;
   int st = check(a, spans, rows, cols, heads, q_len, scale, cap);
   if (st != FL_B200_OK) return st;
+  if (!aligned_to(dtype_size(in_dtype), {x}) || !aligned_to(dtype_size(out_dtype), {out}) ||
+      !aligned_to(4, {spans, positions, slopes}))
+    return FL_B200_ERR_MISALIGNED;
   FLB_CHECK_ARG(!overlap(x, ld_x, dtype_size(in_dtype), out, ld_out, dtype_size(out_dtype), rows, cols));
   a.x = x, a.ldx = ld_x, a.out = out, a.ldo = ld_out, a.slopes = slopes;
   DeviceInfo dev;
@@ -1196,6 +1199,8 @@ FL_B200_API int fl_b200_span_softmax_bwd(const void* dy, int64_t ld_dy, const vo
   int st = check(a, spans, rows, cols, heads, q_len, scale, cap);
   if (st != FL_B200_OK) return st;
   const int sx = dtype_size(x_dtype), sy = dtype_size(y_dtype);
+  if (!aligned_to(sx, {dx}) || (cap > 0.f && !aligned_to(sx, {x})) || !aligned_to(sy, {dy, y}) || !aligned_to(4, {spans}))
+    return FL_B200_ERR_MISALIGNED;
   FLB_CHECK_ARG(!overlap(dx, ld_dx, sx, dy, ld_dy, sy, rows, cols) &&
                 !overlap(dx, ld_dx, sx, y, ld_y, sy, rows, cols));
   if (cap > 0.f) {

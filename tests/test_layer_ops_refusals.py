@@ -1,0 +1,82 @@
+"""What the C entries of the operators of a training step around the matrix
+products refuse before anything is launched.  CPU only: each call here returns
+its status on the host."""
+
+import ctypes
+
+import pytest
+
+from torch_fl import _abi
+
+BF16, F16, F32, I32, I64 = _abi.BF16, _abi.F16, _abi.F32, _abi.I32, _abi.I64
+INVALID, MISALIGNED, WORKSPACE = 1, 3, 6
+Q, K, QO, KO, POS, FREQ = 1 << 20, 2 << 20, 3 << 20, 4 << 20, 5 << 20, 6 << 20
+
+
+def status(name, *args):
+    return getattr(_abi.lib(), name)(*args)
+
+
+def rotary(q=Q, qo=QO, k=K, ko=KO, pos=POS, freq=FREQ, Hq=2, Hk=1, B=2, S=4, D=8, rot=8, dtype=BF16, pd=I32, layout="bshd",
+           sq=None, sk=None, sqo=None, sko=None):
+    """Strides are over (b, h, s)."""
+    dense = lambda H: (S * H * D, D, H * D) if layout == "bshd" else (H * S * D, S * D, D)
+    return status("fl_b200_rotary", q, qo, Hq, *(sq or dense(Hq)), *(sqo or sq or dense(Hq)), k, ko, Hk, *(sk or dense(Hk)),
+                  *(sko or sk or dense(Hk)), pos, 0, 1, pd, freq, rot, 1.0, 0, 0, B, S, D, dtype, None)
+
+
+P = [i << 20 for i in range(1, 20)]
+FWD = dict(x=P[0], r=P[1], post=P[2], pre=P[3], gate=P[4], y=P[5], h=P[6])
+BWD = dict(dy=P[0], dh=P[1], x=P[2], h=P[3], post=P[4], pre=P[5], gate=P[6], dx=P[7], dres=P[8], dpost=P[9], dpre=P[10],
+           dgate=P[11], ws=P[12])
+
+
+def sandwich(dtype=BF16, rows=8, cols=16, per=4, **at):
+    a = {**FWD, **at}
+    return status("fl_b200_sandwich_norm", a["x"], cols, a["r"], cols, a["post"], a["pre"], a["gate"], per, a["y"], a["h"],
+                  rows, cols, 1e-6, 1.0, 0.0, dtype, None)
+
+
+def sandwich_bwd(dtype=BF16, rows=8, cols=16, per=4, bytes_=0, **at):
+    a = {**BWD, **at}
+    return status("fl_b200_sandwich_norm_bwd", a["dy"], cols, a["dh"], cols, a["x"], cols, a["h"], cols, a["post"], a["pre"],
+                  a["gate"], per, a["dx"], a["dres"], a["dpost"], a["dpre"], a["dgate"], rows, cols, 1e-6, 1.0, 0.0, dtype,
+                  a["ws"], bytes_, None)
+
+
+def span(x=P[0], out=P[1], spans=P[2], pos=P[3], slopes=P[4], rows=8, cols=16, heads=2, q=2, scale=1.0, cap=0.0, dtype=BF16,
+         od=None):
+    return status("fl_b200_span_softmax", x, cols, spans, 4, 2, pos, 2, 1, slopes, out, cols, rows, cols, heads, q, scale, cap,
+                  dtype, dtype if od is None else od, None)
+
+
+def span_bwd(dy=P[0], y=P[1], x=P[2], spans=P[3], dx=P[4], rows=8, cols=16, heads=2, q=2, scale=1.0, cap=0.0, dtype=BF16,
+             yd=None):
+    return status("fl_b200_span_softmax_bwd", dy, cols, y, cols, x, cols, spans, 4, 2, dx, cols, rows, cols, heads, q, scale,
+                  cap, dtype if yd is None else yd, dtype, None)
+
+
+def grad_norm(p=4096, norm=64, dtype=F32):
+    return status("fl_b200_grad_norm", (ctypes.c_void_p * 1)(p), _abi.i64_array([10]), (ctypes.c_int * 1)(dtype), 1, 0, norm,
+                  None, 0, None)
+
+
+# ----------------------------------------------------------------- alignment
+@pytest.mark.parametrize("call", [
+    lambda: rotary(q=Q + 1), lambda: rotary(qo=QO + 1), lambda: rotary(k=K + 1), lambda: rotary(ko=KO + 1),
+    lambda: rotary(q=Q + 2, dtype=F32), lambda: rotary(q=Q + 3, qo=Q + 3), lambda: rotary(freq=FREQ + 2),
+    lambda: rotary(pos=POS + 2), lambda: rotary(pos=POS + 4, pd=I64),
+    *[lambda n=n: sandwich(**{n: FWD[n] + 1}) for n in FWD], *[lambda n=n: sandwich(F32, **{n: FWD[n] + 2}) for n in FWD],
+    *[lambda n=n: sandwich_bwd(**{n: BWD[n] + 1}) for n in BWD if n != "ws"],
+    *[lambda n=n: sandwich_bwd(F32, **{n: BWD[n] + 2}) for n in BWD if n != "ws"],
+    lambda: sandwich_bwd(rows=0, dpost=P[9] + 1), lambda: sandwich_bwd(F32, rows=0, dpre=P[9] + 2),
+    lambda: span(x=P[0] + 1), lambda: span(out=P[1] + 1), lambda: span(out=P[1] + 2, od=F32), lambda: span(spans=P[2] + 2),
+    lambda: span(pos=P[3] + 1), lambda: span(slopes=P[4] + 2),
+    lambda: span_bwd(dy=P[0] + 1), lambda: span_bwd(y=P[1] + 1), lambda: span_bwd(y=P[1] + 2, yd=F32),
+    lambda: span_bwd(dy=P[0] + 2, yd=F32), lambda: span_bwd(x=P[2] + 1, cap=1.0), lambda: span_bwd(spans=P[3] + 2),
+    lambda: span_bwd(dx=P[4] + 1),
+    lambda: grad_norm(norm=66), lambda: grad_norm(p=4098),
+])
+def test_addresses_inside_an_element_are_refused(call):
+    """Before the kernels read or write by elements there."""
+    assert call() == MISALIGNED
