@@ -519,9 +519,11 @@ FL_B200_API int fl_b200_verify_draft(const int64_t* draft_ids, int64_t ld_ids, c
  * (I32/I64) as positions[b * spb + s * sps].  inv_freq is F32 [rot / 2], rot  *
  * even, at most head_dim and FL_B200_ROTARY_MAX.  The angle is exact to      *
  * fp64, its cosine fp32, the result rounded once.  Any alignment.  In place   *
- * (an output with its input's address and strides) allowed, and then only   *
- * the turned part is touched; otherwise outputs share no memory with inputs,  *
- * and never with each other.  Heads times the square of a head's packs stay below 2^31.         */
+ * (an output with its input's address and strides) allowed, and then only    *
+ * the turned part is touched; otherwise an output shares no memory with q or  *
+ * k, and never with the other output or itself (refused; views of one tensor  *
+ * beside each other are fine).  Heads times the square of a head's packs stay *
+ * below 2^31.                                                                */
 #define FL_B200_ROTARY_MAX 2048
 FL_B200_API int fl_b200_rotary(
     const void* q, void* q_out, int64_t Hq, int64_t sqb, int64_t sqh, int64_t sqs, int64_t soqb, int64_t soqh,

@@ -24,6 +24,7 @@
 #include <numeric>
 
 #include "common.cuh"
+#include "heads_place.cuh"
 
 namespace flb200 {
 namespace {
@@ -304,16 +305,6 @@ int by_width(const RotaryArgs& a, int64_t head_dim, int64_t unit, cudaStream_t s
   return launch<T, 1, NEIGH>(a, head_dim, stream);
 }
 
-// First and last byte of a [B, S, H, D] operand.
-struct Extent {
-  uintptr_t lo, hi;
-};
-Extent extent(const void* p, int64_t H, int64_t B, int64_t S, int64_t sb, int64_t sh, int64_t ss, int64_t D,
-              int64_t size) {
-  const uintptr_t lo = reinterpret_cast<uintptr_t>(p);
-  return {lo, lo + (uintptr_t)(((B - 1) * sb + (H - 1) * sh + (S - 1) * ss + D) * size)};
-}
-
 }  // namespace
 }  // namespace flb200
 
@@ -341,20 +332,22 @@ extern "C" FL_B200_API int fl_b200_rotary(
     return FL_B200_ERR_MISALIGNED;
   RotaryArgs a = {};
   int64_t unit = 16;  // every address is a multiple of it
+  Heads ins[2], outs[2];
+  const auto meeting = [&](const void* p, const Heads& x, const void* r, const Heads& y) {
+    return meet((int64_t)(reinterpret_cast<uintptr_t>(r) - reinterpret_cast<uintptr_t>(p)), x, y, D * size);
+  };
   auto tensor = [&](int t, const void* in, void* out, int64_t H, const int64_t (&si)[3], const int64_t (&so)[3]) {
     if (H == 0) return true;
     const bool same = in == out;
     const int64_t n[3] = {B, H, S};
     for (int d = 0; d < 3; ++d) {
+      ins[t].n[d] = outs[t].n[d] = n[d];
+      ins[t].st[d] = si[d] * size, outs[t].st[d] = so[d] * size;
       if (n[d] == 1) continue;
-      if ((same && si[d] != so[d]) || so[d] == 0) return false;
+      if (same && si[d] != so[d]) return false;
       unit = std::gcd(unit, std::gcd(si[d] * size, so[d] * size));
     }
-    if (!same) {
-      const Extent x = extent(in, H, B, S, si[0], si[1], si[2], D, size);
-      const Extent y = extent(out, H, B, S, so[0], so[1], so[2], D, size);
-      if (x.lo < y.hi && y.lo < x.hi) return false;
-    }
+    if (meets_itself(outs[t], D * size) || (!same && meeting(in, ins[t], out, outs[t]))) return false;
     unit = std::gcd(unit, (int64_t)((reinterpret_cast<uintptr_t>(in) | reinterpret_cast<uintptr_t>(out)) & 15));
     a.in[t] = static_cast<const char*>(in);
     a.out[t] = static_cast<char*>(out);
@@ -364,7 +357,9 @@ extern "C" FL_B200_API int fl_b200_rotary(
   };
   FLB_CHECK_ARG(tensor(0, q, q_out, Hq, {sqb, sqh, sqs}, {soqb, soqh, soqs}));
   FLB_CHECK_ARG(tensor(1, k, k_out, Hk, {skb, skh, sks}, {sokb, sokh, soks}));
-  FLB_CHECK_ARG(Hq == 0 || Hk == 0 || q_out != k_out);  // (in place, q and k of one tensor)
+  if (Hq && Hk)
+    FLB_CHECK_ARG(!meeting(q_out, outs[0], k_out, outs[1]) && !meeting(q_out, outs[0], k, ins[1]) &&
+                  !meeting(k_out, outs[1], q, ins[0]));
   unit = std::gcd(unit, std::gcd((D - rot) * size, (interleaved ? rot : rot / 2) * size));
   a.pos = positions, a.pb = spb, a.ps = sps, a.pos64 = pos_dtype == FL_B200_I64;
   a.freq = inv_freq, a.scale = scale, a.sign = inverse ? -1.f : 1.f;

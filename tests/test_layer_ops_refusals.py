@@ -80,3 +80,23 @@ def grad_norm(p=4096, norm=64, dtype=F32):
 def test_addresses_inside_an_element_are_refused(call):
     """Before the kernels read or write by elements there."""
     assert call() == MISALIGNED
+
+
+# ------------------------------------------------------------------- overlaps
+FUSED = dict(sq=(4 * 40, 8, 40), sk=(4 * 40, 8, 40), B=2, S=4, D=8, Hq=2, Hk=1)  # [B, S, 5 heads of 8] bf16
+
+
+@pytest.mark.parametrize("call", [
+    lambda: rotary(qo=K),                                                # q's result over k
+    lambda: rotary(qo=K + 64),
+    lambda: rotary(ko=Q), lambda: rotary(ko=Q + 16 * 7),                 # k's over q, over its last head
+    lambda: rotary(qo=QO, ko=QO), lambda: rotary(qo=QO, ko=QO + 16),     # the results over each other
+    lambda: rotary(q=Q, qo=Q, k=Q, ko=Q), lambda: rotary(q=Q, qo=Q, k=Q + 16, ko=Q + 16),
+    lambda: rotary(q=Q, qo=Q, k=Q + 16, ko=Q + 16, **FUSED),             # k is q's second head
+    lambda: rotary(q=Q, qo=Q + 16, k=Q + 64, ko=Q + 64, **FUSED),        # q moved by one head
+    lambda: rotary(q=Q, qo=QO, k=Q + 32, ko=QO + 16, **FUSED),
+    lambda: rotary(sqo=(64, 4, 16)), lambda: rotary(q=Q, qo=Q, sq=(32, 1, 8)),  # heads of a result over each other
+    lambda: rotary(q=Q, qo=Q, sq=(1, 1, 1)),
+])
+def test_outputs_over_operands_or_each_other_are_refused(call):
+    assert call() == INVALID
