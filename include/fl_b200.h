@@ -548,7 +548,8 @@ FL_B200_API int fl_b200_sandwich_norm(const void* x, int64_t ld_x, const void* r
 /* Its gradients from dy, dh (NULL: none), x and the h that was stored: dx,    *
  * dresidual (dense rows), dpost, dpre [cols] and dgate (the gate's shape;     *
  * NULL without one).  Column sums have one order, so results repeat bit for   *
- * bit on one GPU.  The workspace (16-byte aligned) holds the rows' statistics *
+ * bit on one GPU.  No output shares memory with an operand or another one     *
+ * (refused).  The workspace (16-byte aligned) holds the rows' statistics      *
  * and the sums' parts; its size depends on the current device's SM count.    */
 FL_B200_API size_t fl_b200_sandwich_norm_bwd_workspace_size(int64_t rows, int64_t cols);
 FL_B200_API int fl_b200_sandwich_norm_bwd(const void* dy, int64_t ld_dy, const void* dh, int64_t ld_dh,

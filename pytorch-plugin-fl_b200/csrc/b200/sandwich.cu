@@ -1080,6 +1080,7 @@ FL_B200_API int fl_b200_sandwich_norm(const void* x, int64_t ld_x, const void* r
   if (!aligned_to(size, {x, residual, post, pre, gate, y, h})) return FL_B200_ERR_MISALIGNED;
   const Range ry(y, cols, rows, cols, size), rh(h, cols, rows, cols, size);
   const Range in[] = {{x, ld_x, rows, cols, size}, {residual, ld_r, rows, cols, size},
+                      {post, cols, 1, cols, size}, {pre, cols, 1, cols, size},
                       {gate, cols, gate ? ceil_div(rows, a.per_gate) : 1, cols, size}};
   FLB_CHECK_ARG(!ry.meets(rh));
   for (const Range& r : in) FLB_CHECK_ARG(!ry.meets(r) && !rh.meets(r));
@@ -1128,11 +1129,16 @@ FL_B200_API int fl_b200_sandwich_norm_bwd(const void* dy, int64_t ld_dy, const v
   int st = check(a, rows, cols, rows_per_gate, gate, eps, scale, weight_offset);
   if (st != FL_B200_OK) return st;
   if (!aligned_to(size, {dy, dh, x, h, post, pre, gate, dx, dresidual, dgate})) return FL_B200_ERR_MISALIGNED;
-  const Range rx(dx, cols, rows, cols, size), rr(dresidual, cols, rows, cols, size);
+  const int64_t gates = gate ? ceil_div(rows, a.per_gate) : 1;
+  const Range out[] = {{dx, cols, rows, cols, size}, {dresidual, cols, rows, cols, size}, {dpost, cols, 1, cols, size},
+                       {dpre, cols, 1, cols, size}, {gate ? dgate : nullptr, cols, gates, cols, size}};
   const Range in[] = {{dy, ld_dy, rows, cols, size}, {dh, ld_dh, rows, cols, size}, {x, ld_x, rows, cols, size},
-                      {h, ld_h, rows, cols, size}, {gate, cols, gate ? ceil_div(rows, a.per_gate) : 1, cols, size}};
-  FLB_CHECK_ARG(!rx.meets(rr));
-  for (const Range& r : in) FLB_CHECK_ARG(!rx.meets(r) && !rr.meets(r));
+                      {h, ld_h, rows, cols, size}, {post, cols, 1, cols, size}, {pre, cols, 1, cols, size},
+                      {gate, cols, gates, cols, size}};
+  for (const Range& o : out) {
+    for (const Range& r : in) FLB_CHECK_ARG(!o.meets(r));
+    for (const Range& r : out) FLB_CHECK_ARG(&r == &o || !o.meets(r));
+  }
   DeviceInfo dev;
   st = current_device_info(&dev);
   if (st != FL_B200_OK) return st;

@@ -97,6 +97,11 @@ FUSED = dict(sq=(4 * 40, 8, 40), sk=(4 * 40, 8, 40), B=2, S=4, D=8, Hq=2, Hk=1) 
     lambda: rotary(q=Q, qo=QO, k=Q + 32, ko=QO + 16, **FUSED),
     lambda: rotary(sqo=(64, 4, 16)), lambda: rotary(q=Q, qo=Q, sq=(32, 1, 8)),  # heads of a result over each other
     lambda: rotary(q=Q, qo=Q, sq=(1, 1, 1)),
+    *[lambda n=n, o=o: sandwich(**{o: FWD[n]}) for n in ("x", "r", "post", "pre", "gate") for o in ("y", "h")],
+    lambda: sandwich(y=P[6] + 16), lambda: sandwich(h=P[2] + 16),
+    *[lambda n=n, o=o: sandwich_bwd(**{o: BWD[n]}) for n in BWD for o in ("dx", "dres", "dpost", "dpre", "dgate")
+      if n != o and n != "ws"],
+    lambda: sandwich_bwd(dgate=P[7] + 32), lambda: sandwich_bwd(dpost=P[10] + 16),
 ])
 def test_outputs_over_operands_or_each_other_are_refused(call):
     assert call() == INVALID
