@@ -566,6 +566,7 @@ FL_B200_API int fl_b200_sandwich_norm_bwd(const void* dy, int64_t ld_dy, const v
  *   z = scale * x;  cap > 0: z = cap * tanh(z / cap);                        *
  *   slopes != NULL: z -= slopes[h] * |p - j|,                               *
  *   out = exp(z) / sum over the span of exp(z), 0 outside it,               *
+ * scale is finite, and so is scale / cap in fp32 (refused otherwise);         *
  * p = positions[b * pos_sb + q * pos_sq] (int32, clamped to +-2^30; NULL:      *
  * q + cols - q_len).                                                         *
  * A row that sees nothing is 0.  Keys outside a span are never used, whatever *

@@ -1140,6 +1140,8 @@ int check(SpanArgs& a, const int32_t* spans, int64_t rows, int64_t cols, int64_t
   FLB_CHECK_ARG(spans && heads > 0 && q_len > 0 && rows % (heads * q_len) == 0);
   FLB_CHECK_ARG(a.spb >= 0 && a.spq >= 0 && a.pb >= 0 && a.pq >= 0);
   FLB_CHECK_ARG(scale == scale && cap >= 0.f && cap <= 3e38f);
+  // a score of 0 has to stay one: no infinite factor
+  FLB_CHECK_ARG(fabsf(scale) <= 3e38f && (cap == 0.f || fabsf(2.f * kLog2e * (scale / cap)) <= 3e38f));
   if (rows > 0x7fffffff || cols > 0x7fffff00) return FL_B200_ERR_TOO_LARGE;
   a.spans = spans;
   a.rows = (uint32_t)rows, a.q_len = (uint32_t)q_len, a.heads = (uint32_t)heads;

@@ -680,11 +680,21 @@ def _per_query(t: torch.Tensor, B: int, Q: int, tail: int) -> tuple[torch.Tensor
     return u, 0 if u.shape[0] == 1 else u.stride(0), u.stride(1)
 
 
+def _cap(cap: float | None) -> float:
+    """The cap as the kernels take it: 0 stands for none, so no cap may round to it."""
+    if cap is None:
+        return 0.0
+    if not 0 < ctypes.c_float(cap).value <= 3e38:
+        raise ValueError(f"cap must be positive and finite in float32, got {cap}")
+    return float(cap)
+
+
 def span_softmax(x: torch.Tensor, spans: torch.Tensor, scale: float = 1.0, cap: float | None = None,
                  slopes: torch.Tensor | None = None, positions: torch.Tensor | None = None,
                  out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """softmax of scale * x (capped, biased by distance) over each query's span
     of keys; zeros elsewhere."""
+    cap = _cap(cap)
     B, H, Q, Kn = _as_bhqk(x).shape
     _one_device(x, spans, slopes, positions)
     spans, sb, sq = _per_query(spans, B, Q, 2)
@@ -693,15 +703,13 @@ def span_softmax(x: torch.Tensor, spans: torch.Tensor, scale: float = 1.0, cap: 
         positions, pb, pq = _per_query(positions, B, Q, 0)
     if slopes is not None and (slopes.dtype != torch.float32 or slopes.shape != (H,) or not slopes.is_contiguous()):
         raise ValueError("slopes must be a contiguous float32 [heads] tensor")
-    if cap is not None and not cap > 0:
-        raise ValueError("cap must be positive")
     out = torch.empty(x.shape, dtype=out_dtype or x.dtype, device=x.device)
     x, rows, cols, ld = _rows_apart(x)
     with _on_device(x):
         _abi.call("fl_b200_span_softmax", x.data_ptr(), ld, spans.data_ptr(), sb, sq,
                   None if positions is None else positions.data_ptr(), pb, pq,
                   None if slopes is None else slopes.data_ptr(), out.data_ptr(), cols, rows, cols, H, Q,
-                  float(scale), float(cap or 0.0), dtype_code(x), dtype_code(out), _stream(x))
+                  float(scale), cap, dtype_code(x), dtype_code(out), _stream(x))
     return out
 
 
@@ -709,6 +717,7 @@ def span_softmax_backward(dy: torch.Tensor, y: torch.Tensor, x: torch.Tensor, sp
                           scale: float = 1.0, cap: float | None = None) -> torch.Tensor:
     if dy.shape != y.shape or dy.dtype != y.dtype or y.shape != x.shape:
         raise ValueError("dy, y and x must match")
+    cap = _cap(cap)
     B, H, Q, Kn = _as_bhqk(y).shape
     _one_device(x, y, dy, spans)
     spans, sb, sq = _per_query(spans, B, Q, 2)
@@ -719,7 +728,7 @@ def span_softmax_backward(dy: torch.Tensor, y: torch.Tensor, x: torch.Tensor, sp
     with _on_device(y):
         _abi.call("fl_b200_span_softmax_bwd", dy.data_ptr(), ldd, y.data_ptr(), ldy, x.data_ptr(), ldx,
                   spans.data_ptr(), sb, sq, dx.data_ptr(), cols, rows, cols, H, Q, float(scale),
-                  float(cap or 0.0), dtype_code(y), dtype_code(dx), _stream(y))
+                  cap, dtype_code(y), dtype_code(dx), _stream(y))
     return dx
 
 

@@ -3,8 +3,10 @@ products refuse before anything is launched.  CPU only: each call here returns
 its status on the host."""
 
 import ctypes
+import math
 
 import pytest
+import torch
 
 from torch_fl import _abi
 
@@ -105,3 +107,25 @@ FUSED = dict(sq=(4 * 40, 8, 40), sk=(4 * 40, 8, 40), B=2, S=4, D=8, Hq=2, Hk=1) 
 ])
 def test_outputs_over_operands_or_each_other_are_refused(call):
     assert call() == INVALID
+
+
+# ------------------------------------------------------------- caps and scales
+@pytest.mark.parametrize("call", [
+    *[lambda kw=kw, f=f: f(**kw) for f in (span, span_bwd) for kw in (
+        dict(scale=math.inf), dict(scale=-math.inf), dict(cap=1e-40), dict(scale=1e30, cap=1e-20), dict(scale=-2e38, cap=1.0),
+        dict(cap=math.inf))],
+])
+def test_factors_that_are_infinite_are_refused(call):
+    """0 times them would be NaN."""
+    assert call() == INVALID
+
+
+@pytest.mark.parametrize("cap", [0.0, -1.0, 1e-60, 1e60, math.inf, math.nan])
+def test_caps_that_fp32_does_not_hold_are_refused(cap):
+    """One that rounds to 0 would be none."""
+    from torch_fl import kernels
+
+    x, spans = torch.zeros(1, 1, 2, 4), torch.zeros(2, 2, dtype=torch.int32)
+    for call in (lambda: kernels.span_softmax(x, spans, 1.0, cap), lambda: kernels.span_softmax_backward(x, x, x, spans, 1.0, cap)):
+        with pytest.raises(ValueError, match="cap"):
+            call()
