@@ -568,7 +568,7 @@ FL_B200_API int fl_b200_sandwich_norm_bwd(const void* dy, int64_t ld_dy, const v
  *   out = exp(z) / sum over the span of exp(z), 0 outside it,               *
  * scale is finite, and so is scale / cap in fp32 (refused otherwise);         *
  * p = positions[b * pos_sb + q * pos_sq] (int32, clamped to +-2^30; NULL:      *
- * q + cols - q_len).                                                         *
+ * q + cols - q_len).  With slopes cols is at most 2^30 - 4096 and q_len 2^30.  *
  * A row that sees nothing is 0.  Keys outside a span are never used, whatever *
  * they hold; inside it softmax's rules hold (NaN, +inf or nothing but -inf    *
  * give NaN).  out: in_dtype or F32, no memory shared with x.  Any alignment.  */

@@ -1170,6 +1170,8 @@ FL_B200_API int fl_b200_span_softmax(const void* x, int64_t ld_x, const int32_t*
   a.spb = span_sb, a.spq = span_sq, a.pos = positions, a.pb = pos_sb, a.pq = pos_sq;
   int st = check(a, spans, rows, cols, heads, q_len, scale, cap);
   if (st != FL_B200_OK) return st;
+  // the distance from a position of up to +-2^30 to a key is a 32-bit number
+  if (slopes != nullptr && (cols > (1 << 30) - 4096 || q_len > 1 << 30)) return FL_B200_ERR_TOO_LARGE;
   if (!aligned_to(dtype_size(in_dtype), {x}) || !aligned_to(dtype_size(out_dtype), {out}) ||
       !aligned_to(4, {spans, positions, slopes}))
     return FL_B200_ERR_MISALIGNED;

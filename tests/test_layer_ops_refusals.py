@@ -129,3 +129,13 @@ def test_caps_that_fp32_does_not_hold_are_refused(cap):
     for call in (lambda: kernels.span_softmax(x, spans, 1.0, cap), lambda: kernels.span_softmax_backward(x, x, x, spans, 1.0, cap)):
         with pytest.raises(ValueError, match="cap"):
             call()
+
+
+TOO_LARGE = 7
+
+
+def test_distances_past_32_bits_are_refused():
+    """A position of -2^30 is more than 2^31 from the last key of such a row."""
+    wide = dict(rows=1, heads=1, q=1, cols=(1 << 30) + 8)
+    assert span(**wide) == TOO_LARGE
+    assert span(rows=(1 << 30) + 1, heads=1, q=(1 << 30) + 1) == TOO_LARGE
