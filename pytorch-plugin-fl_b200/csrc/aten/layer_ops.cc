@@ -2,6 +2,7 @@
 // positions without a table, the norms around a block with its gate and
 // residual add, softmax over spans of keys, and the clipping of gradients.
 // Autograd is registered natively beside them.
+#include <ATen/MemoryOverlap.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
@@ -576,6 +577,8 @@ at::Tensor ClipGradsOut(at::TensorList grads, double max_norm, double norm_type,
       l.add(t);
       l.out.push_back(o.mutable_data_ptr());
     } else {  // a dense copy, clipped in place and copied to where it belongs
+      TORCH_CHECK(at::has_internal_overlap(o) != at::MemOverlap::Yes, op,
+                  ": an output whose elements share memory (an expanded tensor) cannot be written");
       copies.emplace_back(i, t.clone(at::MemoryFormat::Contiguous));
       l.add(copies.back().second);
       l.out.push_back(copies.back().second.mutable_data_ptr());

@@ -172,3 +172,12 @@ def test_rotary_of_overlapping_views(dtype, dim):
     got = K.rotary(q, k, pos, freq, layout=layout)
     want = K.rotary(q.contiguous(), k.contiguous(), pos, freq, layout=layout)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# ------------------------------------------------------------------- clipping
+def test_clip_refuses_expanded_outputs_before_it_writes_any():
+    a, b = torch.full((1000,), 2.0, device=DEV), torch.ones(3, 1, device=DEV).expand(3, 4)
+    c = torch.ones(8, 9, device=DEV)[:, :5]
+    with pytest.raises(RuntimeError, match="share memory"):
+        torch_fl.ops.clip_grads([a, c, b], 0.1, out=[a, c, b])
+    assert bool((a == 2).all()) and bool((b == 1).all()) and bool((c == 1).all())
