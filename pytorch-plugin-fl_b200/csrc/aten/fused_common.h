@@ -28,13 +28,14 @@ inline RowsView Rows(const at::Tensor& x, at::Tensor& keep) {
   return *AsRows(keep);
 }
 
-// An op's handle, looked up once.  It is kept by its signature, so two ops of
-// one signature need a type each.
-template <typename Fn>
-const c10::TypedOperatorHandle<Fn>& Below(const char* name) {
-  static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Fn>();
-  return op;
-}
+// The handle of the op `name` with signature Fn, looked up once at each place
+// that names it: the lambda, and so its static, is that place's own, and ops
+// of one signature do not share a handle.
+#define FLB_OP(Fn, name)                                                                                   \
+  ([]() -> const c10::TypedOperatorHandle<Fn>& {                                                           \
+    static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Fn>();           \
+    return op;                                                                                             \
+  }())
 // There is no forward-mode formula: a tangent would be dropped unseen.
 inline void NoTangent(const at::Tensor& t, const char* op) {
   TORCH_CHECK(!t._fw_grad(/*level=*/0).defined(), op, ": forward-mode derivatives are not there");

@@ -549,7 +549,7 @@ struct TopkGradGrad : torch::autograd::Function<TopkGradGrad> {
     at::AutoDispatchBelowADInplaceOrView guard;
     ctx->save_for_backward({indices});
     ctx->saved_data["cols"] = cols;
-    return Below<TopkBackwardFn>("flagos::topk_backward").call(dvalues, indices, cols);
+    return FLB_OP(TopkBackwardFn, "flagos::topk_backward").call(dvalues, indices, cols);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const int64_t cols = ctx->saved_data["cols"].toInt();
@@ -562,12 +562,12 @@ struct TopkGradGrad : torch::autograd::Function<TopkGradGrad> {
 at::Tensor TopkBackwardAutograd(const at::Tensor& dvalues, const at::Tensor& indices, int64_t cols) {
   if (at::GradMode::is_enabled() && dvalues.requires_grad()) return TopkGradGrad::apply(dvalues, indices, cols);
   at::AutoDispatchBelowADInplaceOrView guard;
-  return Below<TopkBackwardFn>("flagos::topk_backward").call(dvalues, indices, cols);
+  return FLB_OP(TopkBackwardFn, "flagos::topk_backward").call(dvalues, indices, cols);
 }
 struct TopkGrad : torch::autograd::Function<TopkGrad> {
   static variable_list forward(AutogradContext* ctx, const at::Tensor& x, int64_t k) {
     at::AutoDispatchBelowADInplaceOrView guard;
-    auto [values, indices] = Below<TopkFn>("flagos::topk").call(x, k);
+    auto [values, indices] = FLB_OP(TopkFn, "flagos::topk").call(x, k);
     ctx->set_materialize_grads(false);
     ctx->mark_non_differentiable({indices});
     ctx->save_for_backward({indices});
@@ -587,7 +587,7 @@ std::tuple<at::Tensor, at::Tensor> TopkAutograd(const at::Tensor& x, int64_t k) 
     return {out[0], out[1]};
   }
   at::AutoDispatchBelowADInplaceOrView guard;
-  return Below<TopkFn>("flagos::topk").call(x, k);
+  return FLB_OP(TopkFn, "flagos::topk").call(x, k);
 }
 
 // The gradients where a graph of them is wanted: there is no second
@@ -597,7 +597,7 @@ struct DistillGradGrad : torch::autograd::Function<DistillGradGrad> {
                                const at::Tensor& stats, const at::Tensor& teacher, const at::Tensor& ids,
                                double temperature, bool need_logits, bool need_teacher) {
     at::AutoDispatchBelowADInplaceOrView guard;
-    auto [dx, dt] = Below<DistillBackwardFn>("flagos::distill_topk_backward")
+    auto [dx, dt] = FLB_OP(DistillBackwardFn, "flagos::distill_topk_backward")
                         .call(dloss, logits, stats, teacher, ids, temperature, need_logits, need_teacher);
     return {dx, dt};
   }
@@ -614,7 +614,7 @@ std::tuple<at::Tensor, at::Tensor> DistillTopkBackwardAutograd(
     return {out[0], out[1]};
   }
   at::AutoDispatchBelowADInplaceOrView guard;
-  return Below<DistillBackwardFn>("flagos::distill_topk_backward")
+  return FLB_OP(DistillBackwardFn, "flagos::distill_topk_backward")
       .call(dloss, logits, stats, teacher, ids, temperature, need_logits, need_teacher);
 }
 
@@ -623,7 +623,7 @@ struct DistillGrad : torch::autograd::Function<DistillGrad> {
   static variable_list forward(AutogradContext* ctx, const at::Tensor& logits, const at::Tensor& teacher,
                                const at::Tensor& ids, double temperature) {
     at::AutoDispatchBelowADInplaceOrView guard;
-    auto [loss, stats] = Below<DistillFn>("flagos::distill_topk").call(logits, teacher, ids, temperature);
+    auto [loss, stats] = FLB_OP(DistillFn, "flagos::distill_topk").call(logits, teacher, ids, temperature);
     ctx->set_materialize_grads(false);
     ctx->mark_non_differentiable({stats});
     ctx->save_for_backward({logits, teacher, ids, stats});
@@ -652,7 +652,7 @@ std::tuple<at::Tensor, at::Tensor> DistillTopkAutograd(const at::Tensor& logits,
     return {out[0], out[1]};
   }
   at::AutoDispatchBelowADInplaceOrView guard;
-  return Below<DistillFn>("flagos::distill_topk").call(logits, teacher, ids, temperature);
+  return FLB_OP(DistillFn, "flagos::distill_topk").call(logits, teacher, ids, temperature);
 }
 
 }  // namespace

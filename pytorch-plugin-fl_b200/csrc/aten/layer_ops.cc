@@ -325,7 +325,7 @@ using torch::autograd::variable_list;
 
 using RotaryFn = std::tuple<at::Tensor, at::Tensor>(const at::Tensor&, const at::Tensor&, const at::Tensor&,
                                                     const at::Tensor&, double, bool, int64_t, bool);
-const c10::TypedOperatorHandle<RotaryFn>& RotaryOp() { return Below<RotaryFn>("flagos::rotary"); }
+const c10::TypedOperatorHandle<RotaryFn>& RotaryOp() { return FLB_OP(RotaryFn, "flagos::rotary"); }
 
 // Linear in q and k: the gradient is the same op the other way round, which
 // carries its own gradient.
@@ -392,7 +392,7 @@ struct SandwichGradGrad : torch::autograd::Function<SandwichGradGrad> {
                                const at::Tensor& pre, const std::optional<at::Tensor>& gate, double eps,
                                double scale, double offset) {
     at::AutoDispatchBelowADInplaceOrView guard;
-    auto [a, b, c, d, e] = Below<SandwichBackwardFn>("flagos::sandwich_norm_backward")
+    auto [a, b, c, d, e] = FLB_OP(SandwichBackwardFn, "flagos::sandwich_norm_backward")
                                .call(dy, dh, x, h, post, pre, gate, eps, scale, offset);
     return {a, b, c, d, e};
   }
@@ -410,7 +410,7 @@ Five SandwichBackwardAutograd(const at::Tensor& dy, const std::optional<at::Tens
     return {out[0], out[1], out[2], out[3], out[4]};
   }
   at::AutoDispatchBelowADInplaceOrView guard;
-  return Below<SandwichBackwardFn>("flagos::sandwich_norm_backward")
+  return FLB_OP(SandwichBackwardFn, "flagos::sandwich_norm_backward")
       .call(dy, dh, x, h, post, pre, gate, eps, scale, offset);
 }
 struct SandwichGrad : torch::autograd::Function<SandwichGrad> {
@@ -418,7 +418,7 @@ struct SandwichGrad : torch::autograd::Function<SandwichGrad> {
                                const at::Tensor& post, const at::Tensor& pre,
                                const std::optional<at::Tensor>& gate, double eps, double scale, double offset) {
     at::AutoDispatchBelowADInplaceOrView guard;
-    auto [y, h] = Below<SandwichFn>("flagos::sandwich_norm").call(x, residual, post, pre, gate, eps, scale, offset);
+    auto [y, h] = FLB_OP(SandwichFn, "flagos::sandwich_norm").call(x, residual, post, pre, gate, eps, scale, offset);
     ctx->set_materialize_grads(false);
     const bool gated = gate.has_value() && gate->defined();
     ctx->save_for_backward({x, h, post, pre, gated ? *gate : at::Tensor()});
@@ -463,7 +463,7 @@ std::tuple<at::Tensor, at::Tensor> SandwichAutograd(const at::Tensor& x, const a
     return {out[0], out[1]};
   }
   at::AutoDispatchBelowADInplaceOrView guard;
-  return Below<SandwichFn>("flagos::sandwich_norm").call(x, residual, post, pre, gate, eps, scale, offset);
+  return FLB_OP(SandwichFn, "flagos::sandwich_norm").call(x, residual, post, pre, gate, eps, scale, offset);
 }
 
 using SpanFn = at::Tensor(const at::Tensor&, const at::Tensor&, double, std::optional<double>,
@@ -476,7 +476,7 @@ struct SpanGradGrad : torch::autograd::Function<SpanGradGrad> {
   static at::Tensor forward(AutogradContext*, const at::Tensor& dy, const at::Tensor& y, const at::Tensor& x,
                             const at::Tensor& spans, double scale, std::optional<double> cap) {
     at::AutoDispatchBelowADInplaceOrView guard;
-    return Below<SpanBackwardFn>("flagos::span_softmax_backward").call(dy, y, x, spans, scale, cap);
+    return FLB_OP(SpanBackwardFn, "flagos::span_softmax_backward").call(dy, y, x, spans, scale, cap);
   }
   FLB_NO_SECOND("flagos::span_softmax")
 };
@@ -485,7 +485,7 @@ at::Tensor SpanBackwardAutograd(const at::Tensor& dy, const at::Tensor& y, const
   if (at::GradMode::is_enabled() && (dy.requires_grad() || y.requires_grad() || x.requires_grad()))
     return SpanGradGrad::apply(dy, y, x, spans, scale, cap);
   at::AutoDispatchBelowADInplaceOrView guard;
-  return Below<SpanBackwardFn>("flagos::span_softmax_backward").call(dy, y, x, spans, scale, cap);
+  return FLB_OP(SpanBackwardFn, "flagos::span_softmax_backward").call(dy, y, x, spans, scale, cap);
 }
 // Saves y, and x only where the cap's slope needs it (else an empty tensor of
 // x's type stands for it: the gradient takes its dtype).
@@ -494,7 +494,7 @@ struct SpanGrad : torch::autograd::Function<SpanGrad> {
                             std::optional<double> cap, const std::optional<at::Tensor>& slopes,
                             const std::optional<at::Tensor>& positions, std::optional<at::ScalarType> dtype) {
     at::AutoDispatchBelowADInplaceOrView guard;
-    at::Tensor y = Below<SpanFn>("flagos::span_softmax").call(x, spans, scale, cap, slopes, positions, dtype);
+    at::Tensor y = FLB_OP(SpanFn, "flagos::span_softmax").call(x, spans, scale, cap, slopes, positions, dtype);
     ctx->save_for_backward({y, spans, cap.has_value() ? x : at::Tensor()});
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["cap"] = cap;
@@ -527,7 +527,7 @@ at::Tensor SpanAutograd(const at::Tensor& x, const at::Tensor& spans, double sca
     if (x.requires_grad()) return SpanGrad::apply(x, spans, scale, cap, slopes, positions, dtype);
   }
   at::AutoDispatchBelowADInplaceOrView guard;
-  return Below<SpanFn>("flagos::span_softmax").call(x, spans, scale, cap, slopes, positions, dtype);
+  return FLB_OP(SpanFn, "flagos::span_softmax").call(x, spans, scale, cap, slopes, positions, dtype);
 }
 
 }  // namespace
