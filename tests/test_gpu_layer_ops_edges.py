@@ -16,8 +16,9 @@ import torch
 import torch_fl
 from torch_fl import kernels as K
 
-from .test_gpu_layer_ops import (DEV, TYPES, U, Num, check_rotary, close, gen, np64, random_spans,
-                                 span_back_want)
+from .test_gpu_layer_ops import (DEV, TYPES, U, Num, check_clip, check_rotary, close, gen, np64, random_spans,
+                                 sandwich_inputs, sandwich_want, span_back_want, span_want)
+from .test_gpu_layer_ops import test_sandwich as check_sandwich
 
 pytestmark = pytest.mark.gpu
 
@@ -181,3 +182,110 @@ def test_clip_refuses_expanded_outputs_before_it_writes_any():
     with pytest.raises(RuntimeError, match="share memory"):
         torch_fl.ops.clip_grads([a, c, b], 0.1, out=[a, c, b])
     assert bool((a == 2).all()) and bool((b == 1).all()) and bool((c == 1).all())
+
+
+# ------------------------------------------------- kernels that walk many rows
+def sms():
+    return torch.cuda.get_device_properties(0).multi_processor_count
+
+
+def mixed_spans(B, Q, n, g):
+    """Of every kind in turn: empty, one key, a short run, up to 64 packs, all."""
+    lo = torch.randint(0, n, (B, Q), generator=g, device=DEV)
+    length = torch.stack([torch.zeros_like(lo), torch.ones_like(lo), torch.randint(2, 40, (B, Q), generator=g, device=DEV),
+                          torch.randint(1, 500, (B, Q), generator=g, device=DEV), torch.full_like(lo, n)], -1)
+    kind = torch.randint(0, 5, (B, Q, 1), generator=g, device=DEV)
+    length = length.gather(-1, kind)[..., 0]
+    lo = torch.where(length == n, 0, lo)
+    return torch.stack([lo, (lo + length).clamp(max=n)], -1).int()
+
+
+@pytest.mark.parametrize("dtype,out", [(torch.bfloat16, None), (torch.float16, torch.float32), (torch.float32, None)])
+@pytest.mark.parametrize("cap,bias", [(None, False), (20.0, True)])
+@pytest.mark.parametrize("n,many", [(43, True), (251, True), (252, False), (700, False), (1301, False)])
+def test_span_softmax_walks_rows(dtype, out, cap, bias, n, many):
+    """Rows enough that every resident warp takes a second one (5000), and runs
+    of eight (from 32 rows a warp on): rows are what they are in launches where
+    no warp has two, bit for bit, and picked ones are right in 64 bits."""
+    H = 3
+    rows = 32 * 28 * sms() + 2000 if many else 40 * sms()         # (28: the gradient's warps an SM)
+    B, Q = (7, rows // 21 + 1) if many else (5, rows // 15 + 1)
+    g = torch.Generator(device=DEV).manual_seed(n)
+    wide = (3 * torch.randn(B, H, Q, n + 5, generator=g, device=DEV)).to(dtype)
+    slopes = torch.tensor([0.5, 0.01, 0.0], device=DEV) if bias else None
+    spans = mixed_spans(B, Q, n, g)
+    pos = torch.randint(0, n, (B, Q), generator=g, device=DEV).int()
+    for x in (wide[..., :n].contiguous(), wide[..., 4:n + 4]):
+        y = torch_fl.ops.span_softmax(x, spans, 0.5, cap, slopes, pos, out)
+        dy = torch.randn(x.shape, generator=g, device=DEV).to(y.dtype)
+        dx = torch.ops.flagos.span_softmax_backward(dy, y, x, spans, 0.5, cap)
+        step = 900                                                # 2700 rows: fewer than either kernel's warps
+        assert H * step < 20 * sms()
+        alike = 0
+        for b in range(0, B, 2 if many else 1):
+            for q0 in range(0, Q if x.is_contiguous() else 0, step):
+                part, at = (slice(b, b + 1), slice(q0, q0 + step)), (slice(b, b + 1), slice(None), slice(q0, q0 + step))
+                few = x[at].contiguous()
+                y1 = torch_fl.ops.span_softmax(few, spans[part], 0.5, cap, slopes, pos[part], out)
+                dx1 = torch.ops.flagos.span_softmax_backward(dy[at].contiguous(), y[at].contiguous(), few, spans[part], 0.5, cap)
+                for h in range(H):
+                    # a row that begins elsewhere in a 16-byte pack has its elements with other lanes, and so
+                    # its sums in another order: the same bits are owed where it begins alike
+                    moved = (b * H + h) * Q + q0 - h * few.shape[2]
+                    if moved * n * few.element_size() % 16 == 0:
+                        alike += 1
+                        assert torch.equal(y1[:, h], y[at][:, h]) and torch.equal(dx1[:, h], dx[at][:, h])
+        assert alike > 0 or not x.is_contiguous()
+        pick = torch.randint(0, B * Q, (160,), generator=g, device=DEV).cpu()
+        for h in range(H):
+            take = lambda t: t[pick // Q, h, pick % Q][:, None, None]
+            sp, ps = (t.reshape(B * Q, *t.shape[2:])[pick.to(DEV)][:, None] for t in (spans, pos))
+            want, seen = span_want(np64(take(x)), sp.cpu().numpy(), 0.5, cap, None if slopes is None else np64(slopes[h:h + 1]),
+                                   ps.cpu().numpy().astype(np.float64))
+            close(take(y), want, y.dtype, f"y of head {h}")
+            assert not np64(take(y))[~seen].any()
+            close(take(dx), span_back_want(np64(take(dy)), np64(take(y)), np64(take(x)), seen, 0.5, cap), dtype, f"dx of head {h}")
+            assert not np64(take(dx))[~seen].any()
+
+
+@pytest.mark.parametrize("gate", ["none", "channel", "sequence", "token"])
+@pytest.mark.parametrize("dtype,H", [(torch.bfloat16, 1032), (torch.float16, 1288), (torch.bfloat16, 2040)])
+def test_sandwich_staged_rows_of_129_to_255_packs(dtype, H, gate):
+    """Six resident CTAs an SM that walk at least eight rows each."""
+    B, S = 5, 8 * 6 * sms() // 5 + 20
+    x, res, post, pre, gt, *_ = sandwich_inputs((B, S, H), gate, dtype, H, 1.0)
+    y, h = torch_fl.ops.sandwich_norm(x, res, post, pre, 1e-6, gt, 0.5, 1.0)
+    pick = torch.cat([torch.tensor([0, 1, S - 1, S, B * S - 2, B * S - 1]),
+                      torch.randint(0, B * S, (400,), generator=gen(H))]).to(DEV)
+    flat = lambda t: np64(t.reshape(B * S, H)[pick])
+    wide = None if gt is None else flat(gt.expand(B, S, H))
+    wy, wh = sandwich_want(flat(x), flat(res), np64(post), np64(pre), wide, np.float32(1e-6), 0.5, 1.0)
+    close(h.view(B * S, H)[pick], wh, dtype, "h")
+    close(y.view(B * S, H)[pick], wy, dtype, "y")
+
+
+@pytest.mark.parametrize("dtype,gate", [(torch.bfloat16, "none"), (torch.bfloat16, "channel"), (torch.bfloat16, "sequence"),
+                                        (torch.float16, "token"), (torch.float32, "sequence")])
+@pytest.mark.parametrize("team,packs", [(32, 33), (64, 125), (128, 255), (256, 512), (512, 1000)])
+def test_sandwich_gradient_walks_chunks(dtype, gate, team, packs):
+    """Five rows and more a team's chunk, of gate rows that end inside it."""
+    H = packs * 16 // torch.finfo(dtype).bits * 8
+    teams = sms() * (1 if team == 512 else 2) * max(1, 256 // team)
+    S = 37
+    B = 5 * teams // S + 2
+    check_sandwich(dtype, gate, (B, S, H))
+
+
+@pytest.mark.parametrize("kind", [2.0, math.inf])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_clip_walks_chunks(dtype, kind):
+    """More chunks of 32 KB than there are resident CTAs."""
+    g = gen(81)
+    sizes = [3000001, 5, 40000, 7000003, 64, 1, 2500000]
+    ts = [(torch.randn(n, generator=g) * 0.01 * (1 + i % 3)).to(dtype).to(DEV) for i, n in enumerate(sizes)]
+    assert sum(t.numel() * t.element_size() for t in ts) > 4 * sms() * 32768
+    check_clip(ts, 0.003, kind)
+    bucket = torch.zeros(sum(sizes) + 1, dtype=dtype, device=DEV)
+    check_clip(ts, 0.003, kind, list(bucket[1:].split(sizes)))    # packed without gaps: by elements
+    assert float(bucket[0]) == 0
+    check_clip(ts, 0.003, kind, ts)

@@ -11,7 +11,7 @@ import torch
 from torch_fl import _abi
 
 BF16, F16, F32, I32, I64 = _abi.BF16, _abi.F16, _abi.F32, _abi.I32, _abi.I64
-INVALID, MISALIGNED, WORKSPACE = 1, 3, 6
+INVALID, MISALIGNED, WORKSPACE = 1, 3, 5
 Q, K, QO, KO, POS, FREQ = 1 << 20, 2 << 20, 3 << 20, 4 << 20, 5 << 20, 6 << 20
 
 
@@ -139,3 +139,32 @@ def test_distances_past_32_bits_are_refused():
     wide = dict(rows=1, heads=1, q=1, cols=(1 << 30) + 8)
     assert span(**wide) == TOO_LARGE
     assert span(rows=(1 << 30) + 1, heads=1, q=(1 << 30) + 1) == TOO_LARGE
+
+
+# ------------------------------------------------------------- what is not refused
+def test_clipping_outputs_told_from_each_other():
+    """One status each: lists whose outputs meet are refused as arguments, the
+    others come as far as the workspace that is not there."""
+    def clip(p, q, n=(10, 10)):
+        c = len(p)
+        return status("fl_b200_clip_grads", (ctypes.c_void_p * c)(*p), (ctypes.c_void_p * c)(*q), _abi.i64_array(n),
+                      (ctypes.c_int * c)(*[F32] * c), c, 1.0, 0, 64, None, 0, None)
+
+    # (without a GPU the call ends before it looks at the workspace)
+    fine = WORKSPACE if torch.cuda.is_available() else clip((), (), ())
+    assert fine not in (0, INVALID)
+    assert clip((4096, 4096), (4096, 4096)) == INVALID
+    assert clip((4096, 8192), (8192, 4096)) == INVALID
+    assert clip((4096, 8192), (1 << 14, (1 << 14) + 36)) == INVALID
+    assert clip((4096, 4096 + 36), (1 << 14, 4096)) == INVALID
+    assert clip((4096, 4096 + 16), (1 << 14, 1 << 15)) == fine           # tensors may meet
+    assert clip((4096, 8192), (1 << 14, (1 << 14) + 40)) == fine         # neighbours
+    assert clip((4096, 4096 + 40), (4096, 4096 + 40)) == fine            # in place
+    assert clip((4096, 4096), (1 << 14, 4096), (0, 10)) == fine          # an empty one meets nothing
+
+
+def test_spans_without_keys_are_empty():
+    from torch_fl import ops
+
+    s = ops.attention_spans(2, 0)
+    assert s.shape == (1, 2, 2) and bool((s[..., 0] >= s[..., 1]).all())
