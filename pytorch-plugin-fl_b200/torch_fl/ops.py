@@ -283,7 +283,7 @@ def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None):
     grads = _grads(grads)
     if out is None:
         return torch.ops.flagos.clip_grads(grads, float(max_norm), float(norm_type))
-    out = list(out)
+    out = _grads(out)
     return out, _C._clip_grads_out(grads, float(max_norm), float(norm_type), out)
 
 

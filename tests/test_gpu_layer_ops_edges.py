@@ -289,3 +289,11 @@ def test_clip_walks_chunks(dtype, kind):
     check_clip(ts, 0.003, kind, list(bucket[1:].split(sizes)))    # packed without gaps: by elements
     assert float(bucket[0]) == 0
     check_clip(ts, 0.003, kind, ts)
+
+
+def test_clip_of_one_tensor_and_its_output():
+    """A tensor stands for a list of one, as an output too."""
+    a = torch.full((3, 1000), 2.0, device=DEV)
+    for out in (torch.zeros_like(a), a):
+        got, n = torch_fl.ops.clip_grads(a, 1.0, out=out)
+        assert got[0] is out and abs(float(out.double().norm()) - 1) < 1e-5 and abs(float(n) - 12000 ** 0.5) < 1e-4
