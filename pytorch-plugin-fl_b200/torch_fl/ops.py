@@ -146,6 +146,9 @@ def rope_frequencies(dim: int, theta: float = 1e4, method: str = "default", fact
             if method == "llama3":
                 keep = ((turns - low_turns) / (high_turns - low_turns)).clamp(0, 1)
             else:
+                if theta <= 1:
+                    raise ValueError("yarn: theta must be above 1")
+
                 def index(t):  # the (real) i whose frequency turns t times
                     return dim * math.log(original_len / (t * 2 * math.pi)) / (2 * math.log(theta))
 

@@ -168,3 +168,12 @@ def test_spans_without_keys_are_empty():
 
     s = ops.attention_spans(2, 0)
     assert s.shape == (1, 2, 2) and bool((s[..., 0] >= s[..., 1]).all())
+
+
+# ----------------------------------------------------------- arguments in Python
+def test_yarn_needs_a_base_above_one():
+    from torch_fl import ops
+
+    for theta in (1.0, 0.5):
+        with pytest.raises(ValueError, match="theta"):
+            ops.rope_frequencies(64, theta, "yarn", 4.0, 2048)
