@@ -599,7 +599,7 @@ def _gate_rows(x: torch.Tensor, gate: torch.Tensor | None) -> int:
     if gate is None or gate.dim() == 1:
         return max(1, x.shape[:-1].numel())
     d, per = x.dim() - 2, 1
-    while d >= 0 and gate.shape[d] == 1:
+    while gate.dim() == x.dim() and d >= 0 and gate.shape[d] == 1:
         per *= x.shape[d]
         d -= 1
     if gate.dim() != x.dim() or gate.shape[:d + 1] != x.shape[:d + 1] or gate.shape[-1] != x.shape[-1]:

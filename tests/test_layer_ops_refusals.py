@@ -177,3 +177,11 @@ def test_yarn_needs_a_base_above_one():
     for theta in (1.0, 0.5):
         with pytest.raises(ValueError, match="theta"):
             ops.rope_frequencies(64, theta, "yarn", 4.0, 2048)
+
+
+def test_gates_of_fewer_dims_are_refused():
+    from torch_fl import kernels
+
+    with pytest.raises(ValueError, match="gate"):
+        kernels._gate_rows(torch.zeros(2, 3, 4, 8), torch.zeros(1, 8))
+    assert kernels._gate_rows(torch.zeros(2, 3, 4, 8), torch.zeros(2, 1, 1, 8)) == 12
