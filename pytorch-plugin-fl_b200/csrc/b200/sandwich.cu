@@ -140,15 +140,14 @@ __device__ __forceinline__ void team_sum(float (&v)[K], float4* buf, int half) {
 // Row in registers: TPR threads, VPT packs of x each; h stays fp32.  65536 x
 // 4096 bf16: 348 us at first, 382 us over seconds.  Faster arithmetic is
 // slower here: with rsqrtf for the IEEE square root and division, and one
-// barrier a sum for two, every CTA's stores follow its loads sooner, and the
-// same launch takes 383 to 401 us at first, whatever the order of its stores.
+// barrier a sum for two, the same launch takes 383 to 401 us at first, whatever
+// the order of its stores; why was not found.
 template <typename T, int TPR, int VPT, int BLOCK>
 __global__ void __launch_bounds__(BLOCK, ladder_min_blocks<BLOCK>())
 sandwich_vec_kernel(const __grid_constant__ Sandwich a) {
   pdl_prologue();
   constexpr int VW = Elem<T>::kVec, P = VW / 2;
   __shared__ float4 sums[2 * BLOCK / 32];
-  const float inv_n = 1.f / (float)a.cols;
   const int lane = threadIdx.x % TPR;
   const uint64_t row64 = (uint64_t)blockIdx.x * (BLOCK / TPR) + threadIdx.x / TPR;
   const bool ok = row64 < a.rows;
@@ -212,10 +211,12 @@ sandwich_vec_kernel(const __grid_constant__ Sandwich a) {
   }
 }
 
-// The same rows staged in shared memory: resident CTAs walk rows in runs, each
-// thread the same VPT packs of every row; the next row's x and residual are
-// copied in by cp.async while this one is worked on, and the weights (and the
-// gate row while it lasts) stay in registers.  65536 x 4096 bf16: 338 us over
+// The same rows staged in shared memory: resident CTAs take every gridDim-th
+// row, each thread the same VPT packs of every row; the next row's x and
+// residual are copied in by cp.async while this one is worked on, and the
+// weights stay in registers.  The gate row does while it lasts: a gate a channel
+// for good, one a sequence for its rows over the grid's; one a token is loaded
+// for every row when the row's turn comes.  65536 x 4096 bf16: 338 us over
 // seconds (6.4 TB/s) with three CTAs an SM; two 414 us, four 367 us.
 template <int TPR, int VPT>
 constexpr int staged_ctas() {
@@ -958,7 +959,8 @@ int launch_fwd(const Sandwich& a, const DeviceInfo& dev, cudaStream_t stream) {
     // Where staging pays, over seconds, 4.3 GB a launch, against one CTA a row
     // group: 16 bits, 192 packs 358 us (427), 512 335 (377), 640 409 (496), 1024
     // 355 (405), 1280 378 (629), 2048 342 (474); 32 bits, 1280 329 (585), 2048 358
-    // (446).  Where not: 16 bits, 256 packs 387 (361); 32 bits, 512 373 (315).
+    // (446).  Where not: 16 bits, 256 packs 387 (361); 32 bits, 512 373 (315).  The
+    // other 32-bit rows of up to 1024 packs were not measured and take the latter.
     int st = -1;
     if constexpr (sizeof(T) == 2) {
       if (n > 128 && n < 256) st = launch_staged<T, 128, 2>(a, dev, stream);
@@ -1032,10 +1034,7 @@ int launch_bwd(Sandwich a, const DeviceInfo& dev, float* ws, cudaStream_t stream
   const int by_gate = gates < a.chunks;
   // (chunks of whole gate rows share none)
   const int64_t sums = a.per_chunk % a.per_gate == 0 ? 1 : 1 + std::min<int64_t>(gates, a.chunks - 1);
-  // Launched when the rows are done, not beside them: CTAs of this kernel that
-  // wait on the SMs took 5 % of the rows' rate (forward and backward of 32768 x
-  // 4096 bf16: 466 us, 489 us with programmatic launch).
-  sandwich_bwd_sum_kernel<T><<<dim3((unsigned)ceil_div(a.cols, 32), (unsigned)sums), 512, 0, stream>>>(a, by_gate);
+  launch_k((sandwich_bwd_sum_kernel<T>), dim3((unsigned)ceil_div(a.cols, 32), (unsigned)sums), 512, 0, stream, a, by_gate);
   return launch_status();
 }
 

@@ -440,8 +440,8 @@ struct Rows {
 // took 110 to 128 of them and 16 warps, code for every length that a short
 // span skipped at half the price of running it, and spills, which this much
 // shared memory leaves no L1 for: 524288 rows of 2048, packed documents,
-// capped, 1431 us with 116 bytes of spills and 672 us without; this 480 us
-// (4.9 TB/s).  The first packs of the next row are loaded while a long span's
+// capped, 1431 us with 116 bytes of spills and 672 us without; this 455 to
+// 480 us (4.9 TB/s).  The first packs of the next row are loaded while a long span's
 // sums go through the warp, and every row's span is read one row ahead.
 // Neither an earlier load of the next row, nor more but shorter runs of rows
 // for an even end, nor fewer instructions with 20 warps changed that.

@@ -291,9 +291,10 @@ def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None):
 
 
 def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False):
-    """torch.nn.utils.clip_grad_norm_ on the device: clips the parameters'
-    gradients in place and returns their norm; the host does not wait, except
-    with error_if_nonfinite."""
+    """torch.nn.utils.clip_grad_norm_ on the device, for dense gradients of one
+    GPU and norms 2 and inf: clips the parameters' gradients in place and
+    returns their norm; the host does not wait, except with
+    error_if_nonfinite."""
     if isinstance(parameters, torch.Tensor):
         parameters = [parameters]
     grads = [p.grad for p in parameters if p.grad is not None]
