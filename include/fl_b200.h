@@ -539,7 +539,8 @@ FL_B200_API int fl_b200_rotary(
  * x (stride ld_x), residual (ld_r), post, pre [cols] and gate share `dtype`; *
  * y and h are dense and share no memory with an operand.  gate: dense rows,  *
  * one for every rows_per_gate rows (rows or more: one for all); NULL: 1.     *
- * y is the norm of h before its rounding.  Any alignment.                   */
+ * y is the norm of h before its rounding.  Any alignment; cols at most         *
+ * 0x7fff0000.                                                               */
 FL_B200_API int fl_b200_sandwich_norm(const void* x, int64_t ld_x, const void* residual, int64_t ld_r,
                                       const void* post, const void* pre, const void* gate,
                                       int64_t rows_per_gate, void* y, void* h, int64_t rows, int64_t cols,
@@ -571,7 +572,8 @@ FL_B200_API int fl_b200_sandwich_norm_bwd(const void* dy, int64_t ld_dy, const v
  * q + cols - q_len).  With slopes cols is at most 2^30 - 4096 and q_len 2^30.  *
  * A row that sees nothing is 0.  Keys outside a span are never used, whatever *
  * they hold; inside it softmax's rules hold (NaN, +inf or nothing but -inf    *
- * give NaN).  out: in_dtype or F32, no memory shared with x.  Any alignment.  */
+ * give NaN).  out: in_dtype or F32, no memory shared with x.  Any alignment;  *
+ * cols at most 0x7fff0000.                                                   */
 FL_B200_API int fl_b200_span_softmax(const void* x, int64_t ld_x, const int32_t* spans, int64_t span_sb,
                                      int64_t span_sq, const int32_t* positions, int64_t pos_sb, int64_t pos_sq,
                                      const float* slopes, void* out, int64_t ld_out, int64_t rows, int64_t cols,

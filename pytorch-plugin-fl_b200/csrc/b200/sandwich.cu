@@ -32,6 +32,10 @@
 namespace flb200 {
 namespace {
 
+// Column counters are ints, and a loop's last step passes the row's end by up
+// to 4 turns of 512 threads of 8 elements.
+constexpr int64_t kMaxCols = 0x7fff0000;
+
 struct Sandwich {
   const void *x, *res, *post, *pre, *gate;
   int64_t ldx, ldr;
@@ -1050,7 +1054,7 @@ int check(Sandwich& a, int64_t rows, int64_t cols, int64_t per_gate, const void*
           float off) {
   FLB_CHECK_ARG(gate == nullptr || per_gate >= 1);
   FLB_CHECK_ARG(eps >= 0.f && scale == scale && off == off);
-  if (rows > 0x7fffffff || cols > 0x7fffff00) return FL_B200_ERR_TOO_LARGE;
+  if (rows > 0x7fffffff || cols > kMaxCols) return FL_B200_ERR_TOO_LARGE;
   a.rows = (uint32_t)rows, a.cols = (int)cols, a.gate = gate;
   a.per_gate = (uint32_t)(gate == nullptr ? rows : std::min(per_gate, rows));
   a.eps = eps, a.scale = scale, a.off = off;
@@ -1096,7 +1100,7 @@ FL_B200_API size_t fl_b200_sandwich_norm_bwd_workspace_size(int64_t rows, int64_
   using namespace flb200;
   DeviceInfo dev;
   if (rows <= 0 || cols <= 0 || current_device_info(&dev) != FL_B200_OK) return 0;
-  if (rows > 0x7fffffff || cols > 0x7fffff00) return 0;
+  if (rows > 0x7fffffff || cols > kMaxCols) return 0;
   // (a pack holds 4 or 8 elements: the larger need of the two)
   return std::max(bwd_workspace(rows, cols, cols / 4, dev.sm_count), bwd_workspace(rows, cols, cols / 8, dev.sm_count));
 }

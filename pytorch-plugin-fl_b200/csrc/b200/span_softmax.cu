@@ -52,6 +52,9 @@ __device__ __forceinline__ float rcp(float x) {
 // maximum: times log2 e, a row of the type's lowest value would be -inf.
 __device__ __forceinline__ float exp_of(float d) { return ex2(d * kLog2e); }
 
+// Key counters are ints, and a loop's last step passes the row's end.
+constexpr int64_t kMaxCols = 0x7fff0000;
+
 struct SpanArgs {
   const void* x;
   int64_t ldx;
@@ -1142,7 +1145,7 @@ int check(SpanArgs& a, const int32_t* spans, int64_t rows, int64_t cols, int64_t
   FLB_CHECK_ARG(scale == scale && cap >= 0.f && cap <= 3e38f);
   // a score of 0 has to stay one: no infinite factor
   FLB_CHECK_ARG(fabsf(scale) <= 3e38f && (cap == 0.f || fabsf(2.f * kLog2e * (scale / cap)) <= 3e38f));
-  if (rows > 0x7fffffff || cols > 0x7fffff00) return FL_B200_ERR_TOO_LARGE;
+  if (rows > 0x7fffffff || cols > kMaxCols) return FL_B200_ERR_TOO_LARGE;
   a.spans = spans;
   a.rows = (uint32_t)rows, a.q_len = (uint32_t)q_len, a.heads = (uint32_t)heads;
   a.cols = (int)cols;

@@ -185,3 +185,11 @@ def test_gates_of_fewer_dims_are_refused():
     with pytest.raises(ValueError, match="gate"):
         kernels._gate_rows(torch.zeros(2, 3, 4, 8), torch.zeros(1, 8))
     assert kernels._gate_rows(torch.zeros(2, 3, 4, 8), torch.zeros(2, 1, 1, 8)) == 12
+
+
+@pytest.mark.parametrize("call", [sandwich, sandwich_bwd, lambda **kw: span(heads=1, q=1, slopes=None, **kw),
+                                  lambda **kw: span_bwd(heads=1, q=1, **kw)])
+def test_rows_whose_end_passes_31_bits_in_a_loop_are_refused(call):
+    """A counter of elements that steps past 2^31 - 1 wraps around."""
+    assert call(rows=1, cols=0x7fff0001) == TOO_LARGE
+    assert call(rows=1, cols=0x7fffff00) == TOO_LARGE
