@@ -1,5 +1,5 @@
-"""The examples of README.md and INTEGRATION.md that use the operators of a
-training step around the matrix products, run as they stand there."""
+"""The documents' examples that use the operators of a training step around the
+matrix products, run as they stand there."""
 
 import os
 import re
