@@ -297,3 +297,23 @@ def test_clip_of_one_tensor_and_its_output():
     for out in (torch.zeros_like(a), a):
         got, n = torch_fl.ops.clip_grads(a, 1.0, out=out)
         assert got[0] is out and abs(float(out.double().norm()) - 1) < 1e-5 and abs(float(n) - 12000 ** 0.5) < 1e-4
+
+
+def test_dispatch_modes_see_the_norm_and_the_clipping():
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    seen = []
+
+    class Watch(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            seen.append(func.name())
+            return func(*args, **(kwargs or {}))
+
+    ts = [torch.randn(n, generator=gen(n)).to(DEV) for n in (7, 5000)]
+    out = [torch.empty_like(t) for t in ts]
+    want, n = torch_fl.ops.clip_grads(ts, 0.5, out=[torch.empty_like(t) for t in ts])
+    with Watch():
+        got, n1 = torch_fl.ops.clip_grads(ts, 0.5, out=out)
+        n2 = torch_fl.ops.grad_norm(ts)
+    assert {"flagos::clip_grads_out", "flagos::grad_norm"} <= {s.split(".")[0] for s in seen}
+    assert float(n) == float(n1) == float(n2) and all(a is o and torch.equal(a, b) for a, o, b in zip(got, out, want))
